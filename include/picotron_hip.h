@@ -151,6 +151,24 @@ int pt_rope(const void* x0, void* y0, const int64_t* desc0, const void* x1, void
             const float* sin_table, int64_t table_rows, int layout, int inverse, int dtype,
             void* stream);
 
+/* Rotary embedding at given positions: pairs (by `layout`, as in pt_rope) of the first rotary_dim
+ * elements of each head turn by position * f_i and are multiplied by `scale`; the other elements
+ * are copied.  Tensors and descriptors as in pt_rope; y must not overlap x.
+ * The position of (batch b, sequence index s) is position_offset plus the integer of
+ * position_bytes (4 or 8) bytes at positions[b * position_batch_stride + s * position_seq_stride],
+ * or plus s where positions is NULL; any value, negative ones too.  Descriptors of one call share
+ * the batch and sequence sizes that the positions are for.
+ * turns[i] (device, rotary_dim/2 entries) is f_i / (2 pi) as a fraction of 2^64, so that
+ * the angle is position * turns[i] modulo 2^64, exact to |position| * 2^-65 turns.
+ * inverse = 1 rotates by minus the angles (the backward, with the same scale).
+ * No reference counterpart: the reference rotates whole heads at positions 0..seq-1
+ * (src/picotron/nn/rope.py:13-51). */
+int pt_rope_at(const void* x0, void* y0, const int64_t* desc0, const void* x1, void* y1,
+               const int64_t* desc1, int64_t head_dim, int64_t rotary_dim, const void* positions,
+               int position_bytes, int64_t position_batch_stride, int64_t position_seq_stride,
+               int64_t position_offset, const uint64_t* turns, float scale, int layout, int inverse,
+               int dtype, void* stream);
+
 /* ---------------------------------------------------------------- Cross-entropy
  * Mean cross-entropy over rows whose target != ignore_index, fused with its gradient.
  * Row (o, i), o < outer, i < inner, starts at logits + o*outer_stride + i*inner_stride

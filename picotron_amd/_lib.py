@@ -76,6 +76,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
          c_int64, c_int, c_int, c_int, c_void_p],
     ),
+    "pt_rope_at": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int,
+         c_int64, c_int64, c_int64, c_void_p, c_float, c_int, c_int, c_int, c_void_p],
+    ),
     "pt_cross_entropy_workspace_bytes": (c_size_t, [c_int64]),
     "pt_cross_entropy": (
         c_int,

@@ -10,16 +10,29 @@ back otherwise.
 The reference implements only the interleaved layout.  ``layout="rotate_half"`` (pairs
 ``(i, i + head_dim/2)``, the Llama/HF convention) is an addition; both layouts share the
 same angle table.
+
+So are rotations of a part of the head (``rotary_dim``), of frequencies scaled to longer contexts
+(``scaling``) and at given positions (``forward(query, key, positions)``): any of them takes the
+kernel that forms its angles from the positions (``triton_apply_rotary_at``) in place of the
+tables, or :func:`apply_rotary_at` where it cannot run.  :class:`RotaryFrequencies` holds
+the frequencies for both.
 """
 
 from __future__ import annotations
 
+import math
 import warnings
+from collections.abc import Mapping
 
 import torch
 from torch import Tensor, nn
 
-from picotron_amd.nn.triton_kernels.rope import triton_apply_rotary_embedding_pair
+from picotron_amd import ops
+from picotron_amd.nn.triton_kernels.rope import (
+    TritonRoPEUnavailable,
+    triton_apply_rotary_at,
+    triton_apply_rotary_embedding_pair,
+)
 
 LAYOUTS = ("interleaved", "rotate_half")
 
@@ -78,8 +91,137 @@ def apply_rotary_embedding_rotate_half(states: Tensor, cosine: Tensor, sine: Ten
     return torch.cat((first * cosine - second * sine, first * sine + second * cosine), dim=-1)
 
 
+# scaling type -> (required keys, optional keys with their defaults)
+_SCALINGS = {
+    "linear": (("factor",), {}),
+    "ntk": (("factor",), {}),
+    "yarn": (("factor", "original_max_positions"), {"beta_fast": 32.0, "beta_slow": 1.0, "attention_factor": None}),
+    "llama3": (("factor", "original_max_positions"), {"low_freq_factor": 1.0, "high_freq_factor": 4.0}),
+}
+
+
+def _checked_scaling(scaling: Mapping) -> dict:
+    kind = scaling.get("type")
+    if kind not in _SCALINGS:
+        raise ValueError(f"rotary scaling type must be one of {sorted(_SCALINGS)}; got {kind!r}.")
+    required, optional = _SCALINGS[kind]
+    missing = [key for key in required if key not in scaling]
+    unknown = sorted(set(scaling) - {"type", *required, *optional})
+    if missing or unknown:
+        raise ValueError(f"rotary scaling {kind!r}: missing {missing}, unknown {unknown}.")
+    values = {**optional, **scaling}
+    for key, value in values.items():
+        if key != "type" and value is not None and not (math.isfinite(value) and value > 0):
+            raise ValueError(f"rotary scaling {key} must be a positive number; got {value!r}.")
+    return values
+
+
+class RotaryFrequencies:
+    """Radians per position of each rotated pair (``frequencies``, fp64 on the CPU) and the factor on cosine and sine
+    (``attention_factor``): ``theta^(-2i/rotary_dim)``, scaled to contexts longer than those of training by ``scaling``:
+
+    - ``{"type": "linear", "factor": F}``: every frequency / F (positions interpolated);
+    - ``{"type": "ntk", "factor": F}``: theta * F^(rotary_dim / (rotary_dim - 2));
+    - ``{"type": "yarn", "factor": F, "original_max_positions": L}``: / F for pairs that turn less than ``beta_slow``
+      (1) times over L positions, kept for those above ``beta_fast`` (32), a linear ramp over the pairs between, and an
+      ``attention_factor`` of 0.1 ln F + 1 unless given;
+    - ``{"type": "llama3", "factor": F, "original_max_positions": L}``: / F below ``low_freq_factor`` (1) turns over L
+      positions, kept above ``high_freq_factor`` (4), interpolated linearly in the number of turns between.
+
+    It is a plan that a model keeps: :meth:`turns` is copied to a device once (before a graph capture
+    that uses it there)."""
+
+    def __init__(self, rotary_dim: int, theta: float = 10_000.0, *, scaling: Mapping | None = None) -> None:
+        if rotary_dim <= 0 or rotary_dim % 2 != 0:
+            raise ValueError("RoPE requires an even, positive rotary dimension.")
+        if not (math.isfinite(theta) and theta > 0):
+            raise ValueError("rope_theta must be positive.")
+        self.rotary_dim = rotary_dim
+        self.attention_factor = 1.0
+        i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        if scaling is None:
+            self.frequencies = theta ** (-2.0 * i / rotary_dim)
+        else:
+            self._scale(_checked_scaling(scaling), theta, i)
+        self._turns: dict[torch.device, Tensor] = {}
+
+    def _scale(self, s: dict, theta: float, i: Tensor) -> None:
+        dim, factor = self.rotary_dim, s["factor"]
+        if s["type"] == "ntk":
+            theta = theta * factor ** (dim / max(dim - 2, 1))
+        f = theta ** (-2.0 * i / dim)
+        if s["type"] == "linear":
+            f = f / factor
+        elif s["type"] == "yarn":
+            length = s["original_max_positions"]
+            if theta == 1.0:
+                raise ValueError("rotary scaling 'yarn' needs a theta other than 1.")
+
+            def pair_with(turns: float) -> float:  # the pair that turns so often over the original positions
+                return dim * math.log(length / (2 * math.pi * turns)) / (2 * math.log(theta))
+
+            low = max(math.floor(pair_with(s["beta_fast"])), 0)
+            high = min(math.ceil(pair_with(s["beta_slow"])), dim - 1)
+            ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+            f = f * (1 - ramp) + f / factor * ramp
+            given = s["attention_factor"]
+            self.attention_factor = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+        elif s["type"] == "llama3":
+            low, high = s["low_freq_factor"], s["high_freq_factor"]
+            if high <= low:
+                raise ValueError("rotary scaling 'llama3' needs high_freq_factor above low_freq_factor.")
+            turns = s["original_max_positions"] * f / (2 * math.pi)
+            keep = ((turns - low) / (high - low)).clamp(0, 1)
+            f = f / factor * (1 - keep) + f * keep
+        self.frequencies = f
+
+    def turns(self, device: torch.device) -> Tensor:
+        """int64 on ``device``: the bits of each frequency as a fraction of a turn per position, times 2^64."""
+
+        found = self._turns.get(device)
+        if found is None:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise TritonRoPEUnavailable(
+                    "HIP RoPE: the frequencies are first used on this device during graph capture; run the same call "
+                    "once before capturing it.")
+            bits = [round(math.fmod(f / (2 * math.pi), 1.0) * 2**64) % 2**64 for f in self.frequencies.tolist()]
+            found = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64).to(device)
+            self._turns[device] = found
+        return found
+
+
+def apply_rotary_at(
+    states: Tensor, positions: Tensor | int | None, frequencies: RotaryFrequencies, *, layout: str = "interleaved"
+) -> Tensor:
+    """The rotation of ``triton_apply_rotary_at`` in PyTorch: angles in fp64, the rotation in fp32 (fp64 for fp64
+    states), one rounding to the states' type."""
+
+    seq, dim = states.size(-2), frequencies.rotary_dim
+    if dim > states.size(-1):
+        raise ValueError("RoPE frequencies cover more than the attention head dimension.")
+    if not isinstance(positions, Tensor):
+        positions = torch.arange(seq, device=states.device) + int(positions or 0)
+    ops._position_strides(positions, states.size(0), seq)
+    positions = positions if positions.dim() == 2 else positions[None]
+    angles = positions[:, None, :, None].double() * frequencies.frequencies.to(states.device)
+    compute = torch.promote_types(states.dtype, torch.float32)
+    cosine, sine = ((f(angles) * frequencies.attention_factor).to(compute) for f in (torch.cos, torch.sin))
+    part = states[..., :dim].to(compute)
+    if layout == "interleaved":
+        first, second = part[..., 0::2], part[..., 1::2]
+    else:
+        first, second = part[..., : dim // 2], part[..., dim // 2 :]
+    rotated = (first * cosine - second * sine, first * sine + second * cosine)
+    part = torch.stack(rotated, dim=-1).flatten(-2) if layout == "interleaved" else torch.cat(rotated, dim=-1)
+    return torch.cat((part.to(states.dtype), states[..., dim:]), dim=-1)
+
+
 class RotaryEmbedding(nn.Module):
-    """Apply RoPE to attention query and key tensors."""
+    """Apply RoPE to attention query and key tensors.
+
+    ``rotary_dim`` (default: the whole head) rotates the first elements of each head; ``scaling`` is
+    :class:`RotaryFrequencies`'s.  With either, or with positions given to :meth:`forward`, the angles come from the
+    positions themselves; without them from fp32 tables, as in the reference."""
 
     def __init__(
         self,
@@ -88,6 +230,8 @@ class RotaryEmbedding(nn.Module):
         *,
         use_triton_rope: bool = False,
         layout: str = "interleaved",
+        rotary_dim: int | None = None,
+        scaling: Mapping | None = None,
     ) -> None:
         super().__init__()
         if head_dim % 2 != 0:
@@ -101,6 +245,10 @@ class RotaryEmbedding(nn.Module):
         self.layout = layout
         self.use_triton_rope = use_triton_rope
         self._triton_fallback_warned = False
+        if rotary_dim is not None and not 0 < rotary_dim <= head_dim:
+            raise ValueError("rotary_dim must be positive and at most head_dim.")
+        self.frequencies = RotaryFrequencies(head_dim if rotary_dim is None else rotary_dim, theta, scaling=scaling)
+        self._plain = scaling is None and self.frequencies.rotary_dim == head_dim
         # One fp32 table pair per device, as long as the longest sequence seen: position p's
         # angles do not depend on the table length, and the kernel reads rows 0..seq-1 of a
         # longer table, so variable sequence lengths share one pair instead of one each.
@@ -115,8 +263,29 @@ class RotaryEmbedding(nn.Module):
             self._fp32_tables[device] = tables
         return tables
 
-    def forward(self, query: Tensor, key: Tensor) -> tuple[Tensor, Tensor]:
-        """Rotate query and key using their shared sequence positions."""
+    def _at(self, query: Tensor, key: Tensor, positions: Tensor | int | None) -> tuple[Tensor, Tensor]:
+        if self.use_triton_rope:
+            try:
+                return triton_apply_rotary_at(query, key, positions, self.frequencies, layout=self.layout)
+            except Exception as error:
+                self._warn(error)
+        return (apply_rotary_at(query, positions, self.frequencies, layout=self.layout),
+                apply_rotary_at(key, positions, self.frequencies, layout=self.layout))
+
+    def _warn(self, error: Exception) -> None:
+        if not self._triton_fallback_warned:
+            warnings.warn(
+                f"Triton RoPE unavailable; using PyTorch fallback: {error}",
+                RuntimeWarning,
+                stacklevel=2,
+            )
+            self._triton_fallback_warned = True
+
+    def forward(
+        self, query: Tensor, key: Tensor, positions: Tensor | int | None = None
+    ) -> tuple[Tensor, Tensor]:
+        """Rotate query and key using their shared sequence positions: 0 to seq - 1, or ``positions`` (those of
+        ``triton_apply_rotary_at``)."""
 
         if (
             query.size(0) != key.size(0)
@@ -124,6 +293,8 @@ class RotaryEmbedding(nn.Module):
             or query.size(-1) != key.size(-1)
         ):
             raise ValueError("RoPE query and key must share batch, sequence, and head dimensions.")
+        if positions is not None or not self._plain:
+            return self._at(query, key, positions)
         if self.use_triton_rope:
             try:
                 cosine, sine = self._tables_fp32(query.size(-2), query.device)

@@ -33,6 +33,7 @@ from picotron_amd.nn.triton_kernels.rmsnorm import (
 )
 from picotron_amd.nn.triton_kernels.rope import (
     TritonRoPEUnavailable,
+    triton_apply_rotary_at,
     triton_apply_rotary_embedding,
     triton_apply_rotary_embedding_pair,
 )
@@ -61,6 +62,7 @@ __all__ = [
     # additions beyond the reference surface
     "FusedAdamWStepFailed",
     "triton_adamw_step",
+    "triton_apply_rotary_at",
     "triton_apply_rotary_embedding_pair",
     "triton_clip_grad_norm_and_step",
     "triton_grad_scaler_step",

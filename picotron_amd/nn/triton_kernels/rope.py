@@ -119,3 +119,86 @@ def triton_apply_rotary_embedding_pair(
         return ops.rope(query, cosine.float(), sine.float(), layout=layout, x1=key)
     out_q, out_k = _RoPEFunction.apply(layout, False, cosine.float(), sine.float(), query, key)
     return out_q, out_k
+
+
+class _RoPEAtFunction(torch.autograd.Function):
+    """Rotate one or two (B, H, S, D) views at their positions; the backward is the rotation the other way."""
+
+    @staticmethod
+    def forward(ctx, how: tuple, turns: Tensor, positions: Tensor | None, *states: Tensor):  # type: ignore[override]
+        ctx.how = how  # (offset, scale, layout, inverse)
+        ctx.has_positions = positions is not None
+        ctx.save_for_backward(turns, *((positions,) if positions is not None else ()))
+        out0, out1 = _rotate_at(how, turns, positions, states)
+        return (out0,) if out1 is None else (out0, out1)
+
+    @staticmethod
+    def backward(ctx, *grads: Tensor):  # type: ignore[override]
+        turns, positions = (*ctx.saved_tensors, None)[:2]
+        offset, scale, layout, inverse = ctx.how
+        how = (offset, scale, layout, not inverse)
+        present = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
+        results: list[Tensor | None] = [None] * len(grads)
+        if present:
+            g = [_last_dim_contiguous(grads[i]) for i in present]
+            if torch.is_grad_enabled() and not ops._compiling():
+                d = _RoPEAtFunction.apply(how, turns, positions, *g)  # create_graph=True
+            else:
+                d = _rotate_at(how, turns, positions, g)
+            for i, x in zip(present, d):
+                results[i] = x
+        return (None, None, None, *results)
+
+
+def _rotate_at(how: tuple, turns: Tensor, positions: Tensor | None, states) -> tuple[Tensor, Tensor | None]:
+    offset, scale, layout, inverse = how
+    return ops.rope_at(states[0], turns, positions=positions, offset=offset, scale=scale, layout=layout, inverse=inverse,
+                       x1=states[1] if len(states) > 1 else None)
+
+
+def triton_apply_rotary_at(
+    query: Tensor, key: Tensor | None, positions: Tensor | int | None, frequencies, *, layout: str = "interleaved"
+) -> tuple[Tensor, Tensor | None]:
+    """Rotate query and key (or a single tensor, with ``key`` None) at given positions in one kernel launch.
+
+    ``query`` and ``key`` are (batch, heads, seq, head_dim) views with a contiguous head_dim (head counts may differ).
+    ``positions`` is an int32 or int64 tensor of (seq,), (1, seq) or (batch, seq) -- any values: packed documents,
+    one decoded token per sequence, far into a context -- or an integer, the position of the first token, or None (0).
+    ``frequencies`` is a :class:`picotron_amd.nn.RotaryFrequencies`, whose rotary_dim may be less than head_dim: the rest of a
+    head is copied.  Outputs are new tensors; the backward turns the other way.  Angles carry no rounding of
+    position times frequency (the reference's tables do: rope.py:13-32), so they are as exact at position 10^6 as at 1.
+    """
+
+    states = [query] if key is None else [query, key]
+    offset = 0
+    if isinstance(positions, Tensor):
+        require_hip(TritonRoPEUnavailable, "RoPE", *states, positions)
+    else:
+        offset, positions = int(positions or 0), None
+        require_hip(TritonRoPEUnavailable, "RoPE", *states)
+    if layout not in ops.LAYOUTS:
+        raise TritonRoPEUnavailable(f"RoPE layout must be one of {sorted(ops.LAYOUTS)}.")
+    for s in states:
+        if (s.ndim != 4 or s.size(-1) != query.size(-1) or s.stride(-1) != 1 or s.size(-1) % 2 != 0
+                or s.dtype not in (torch.float32, torch.float16, torch.bfloat16) or s.dtype != query.dtype
+                or s.device != query.device):
+            raise TritonRoPEUnavailable(
+                "HIP RoPE requires 4-D (batch, heads, seq, head_dim) float states of one dtype and device with an even, "
+                "contiguous head_dim.")
+        if s.size(0) != query.size(0) or s.size(2) != query.size(2):
+            raise TritonRoPEUnavailable("RoPE query and key must share batch and sequence sizes.")
+    if frequencies.rotary_dim > query.size(-1):
+        raise TritonRoPEUnavailable("HIP RoPE requires frequencies of at most head_dim elements.")
+    if positions is not None:
+        if positions.device != query.device:
+            raise TritonRoPEUnavailable("RoPE positions must be on the states' device.")
+        try:
+            ops._position_strides(positions, query.size(0), query.size(2))
+        except ValueError as error:
+            raise TritonRoPEUnavailable(f"{error}.") from error
+    turns, scale = frequencies.turns(query.device), frequencies.attention_factor
+    how = (offset, scale, layout, False)
+    if no_graph(*states):
+        return _rotate_at(how, turns, positions, states)
+    out = _RoPEAtFunction.apply(how, turns, positions, *states)
+    return out[0], (out[1] if key is not None else None)

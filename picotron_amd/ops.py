@@ -94,6 +94,16 @@ def _check_cuda(*tensors: Tensor) -> torch.device:
     return device
 
 
+def _call_on(device: torch.device, fn: str, *args) -> None:
+    """:func:`_lib.raw_call` with ``device`` the current one, which a launch on its stream needs."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.raw_call(fn, *args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.raw_call(fn, *args, _stream(device))
+
+
 # ------------------------------------------------------------------ RMSNorm
 
 
@@ -382,6 +392,78 @@ def rope(
         None if x1 is None else descs[1],
         head_dim, cos.data_ptr(), sin.data_ptr(), cos.size(0), LAYOUTS[layout], int(inverse),
         dtype_code(x0.dtype), _stream(device),
+    )
+    return outs[0], (outs[1] if x1 is not None else None)
+
+
+def _position_strides(positions: Tensor | None, batch: int, seq: int) -> tuple[int, int]:
+    """(batch stride, sequence stride) of (seq,), (1, seq) or (batch, seq) positions."""
+
+    if positions is None:
+        return 0, 0
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("RoPE positions must be int32 or int64")
+    shape = tuple(positions.shape)
+    if shape == (seq,):
+        return 0, positions.stride(0)
+    if shape in ((batch, seq), (1, seq)):
+        return (positions.stride(0) if shape[0] > 1 else 0), positions.stride(1)
+    raise ValueError(f"RoPE positions must be (seq,), (1, seq) or (batch, seq), here with batch {batch} and seq {seq}; "
+                     f"got {shape}")
+
+
+def rope_at(
+    x0: Tensor,
+    turns: Tensor,
+    *,
+    positions: Tensor | None = None,
+    offset: int = 0,
+    scale: float = 1.0,
+    layout: str = "interleaved",
+    inverse: bool = False,
+    x1: Tensor | None = None,
+) -> tuple[Tensor, Tensor | None]:
+    """Rotate the first ``2 * turns.numel()`` elements of each head of (batch, heads, seq, head_dim) views x0
+    (and x1) by their positions' angles; the others are copied.
+
+    ``turns``: int64, the bits of each pair's fraction of a turn per position times 2^64
+    (:meth:`picotron_amd.nn.RotaryFrequencies.turns`).  ``positions``: int32 or int64 of (seq,), (1, seq) or
+    (batch, seq), 0 to seq - 1 when absent; ``offset`` is added to each.  Cosine and sine are multiplied by
+    ``scale``.  Outputs are new tensors with the inputs' logical shape and memory layout.
+    """
+
+    if _compiling():
+        if x1 is None:
+            return torch.ops.picotron_amd.rope_at(x0, turns, positions, offset, scale, layout, bool(inverse)), None
+        y0, y1 = torch.ops.picotron_amd.rope_at_pair(x0, x1, turns, positions, offset, scale, layout, bool(inverse))
+        return y0, y1
+    tensors = [x0] if x1 is None else [x0, x1]
+    device = _check_cuda(*tensors, turns, *([] if positions is None else [positions]))
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
+    for t in tensors:
+        if t.dim() != 4 or t.size(-1) != x0.size(-1) or t.stride(-1) != 1:
+            raise ValueError("RoPE states must be 4-D (batch, heads, seq, head_dim), head_dim contiguous")
+        if t.dtype != x0.dtype:
+            raise ValueError("query and key must share a dtype")
+        if t.size(0) != x0.size(0) or t.size(2) != x0.size(2):
+            raise ValueError("RoPE query and key must share batch and sequence sizes")
+    if turns.dtype != torch.int64 or turns.dim() != 1 or not turns.is_contiguous() or turns.numel() * 2 > x0.size(-1):
+        raise ValueError("RoPE turns must be contiguous int64, one for each rotated pair of a head")
+    if not -(1 << 63) <= offset < 1 << 63:
+        raise ValueError("the RoPE position offset must fit 64 bits")
+    pbs, pss = _position_strides(positions, x0.size(0), x0.size(2))
+    outs = [torch.empty_like(t) for t in tensors]
+    descs = [_rope_desc(t, o) for t, o in zip(tensors, outs)]
+    _call_on(
+        device,
+        "pt_rope_at",
+        x0.data_ptr(), outs[0].data_ptr(), descs[0],
+        None if x1 is None else x1.data_ptr(), None if x1 is None else outs[1].data_ptr(),
+        None if x1 is None else descs[1],
+        x0.size(-1), 2 * turns.numel(), _ptr(positions) if x0.numel() else None,
+        0 if positions is None else positions.element_size(), pbs, pss, int(offset), turns.data_ptr(), float(scale),
+        LAYOUTS[layout], int(inverse), dtype_code(x0.dtype),
     )
     return outs[0], (outs[1] if x1 is not None else None)
 
@@ -954,4 +1036,27 @@ def _op_rope_pair(
 
 @_op_rope_pair.register_fake
 def _(x0, x1, cos, sin, layout, inverse):
+    return torch.empty_like(x0), torch.empty_like(x1)
+
+
+@torch.library.custom_op("picotron_amd::rope_at", mutates_args=())
+def _op_rope_at(x: Tensor, turns: Tensor, positions: Tensor | None, offset: int, scale: float, layout: str,
+                inverse: bool) -> Tensor:
+    return rope_at(x, turns, positions=positions, offset=offset, scale=scale, layout=layout, inverse=inverse)[0]
+
+
+@_op_rope_at.register_fake
+def _(x, turns, positions, offset, scale, layout, inverse):
+    return torch.empty_like(x)
+
+
+@torch.library.custom_op("picotron_amd::rope_at_pair", mutates_args=())
+def _op_rope_at_pair(x0: Tensor, x1: Tensor, turns: Tensor, positions: Tensor | None, offset: int, scale: float,
+                     layout: str, inverse: bool) -> tuple[Tensor, Tensor]:
+    y0, y1 = rope_at(x0, turns, positions=positions, offset=offset, scale=scale, layout=layout, inverse=inverse, x1=x1)
+    return y0, y1
+
+
+@_op_rope_at_pair.register_fake
+def _(x0, x1, turns, positions, offset, scale, layout, inverse):
     return torch.empty_like(x0), torch.empty_like(x1)

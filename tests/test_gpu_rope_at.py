@@ -1,0 +1,257 @@
+"""The rotary embedding at positions on the GPU against angles in 64 bits: layouts, parts of a head that are no whole
+vectors, positions of every form and size, strided views, its gradients, other streams, graphs, and refusals."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from gpu_util import randn
+from picotron_amd import ops
+from picotron_amd.nn import RotaryEmbedding, RotaryFrequencies
+from picotron_amd.nn.triton_kernels import TritonRoPEUnavailable, triton_apply_rotary_at
+
+pytestmark = pytest.mark.gpu
+
+YARN = dict(type="yarn", factor=16.0, original_max_positions=8192)
+
+
+def reference(x, positions, f, layout, inverse=False):
+    """(rotated in 64 bits, the pair's |u| + |w| at each element).  The angle's turns are reduced before they are
+    rounded: position times each half of the frequency's bits, modulo 1."""
+
+    seq, dim = x.size(2), f.rotary_dim
+    if not isinstance(positions, torch.Tensor):
+        positions = torch.arange(seq, device=x.device) + positions
+    p = positions.to(torch.int64).reshape(-1, seq)[:, None, :, None]
+    turn = p * f.turns(x.device)  # modulo 2^64
+    angle = turn.double() * 2.0**-64 * (2 * torch.pi) * (-1 if inverse else 1)
+    c, s = angle.cos() * f.attention_factor, angle.sin() * f.attention_factor
+    part = x[..., :dim].double()
+    u, w = (part[..., 0::2], part[..., 1::2]) if layout == "interleaved" else (part[..., : dim // 2], part[..., dim // 2 :])
+    join = (lambda a, b: torch.stack((a, b), -1).flatten(-2)) if layout == "interleaved" else (lambda a, b: torch.cat((a, b), -1))
+    size = u.abs() + w.abs()
+    return (torch.cat((join(u * c - w * s, u * s + w * c), x[..., dim:].double()), -1),
+            torch.cat((join(size, size), torch.zeros_like(x[..., dim:], dtype=torch.float64)), -1))
+
+
+def check(y, x, positions, f, layout, inverse=False):
+    """Cosine and sine within 9e-8, their product with the factor one rounding more (1.5e-7 in all), two roundings
+    of a term (1.2e-7), the angle 2^-32 turns: 3e-7 of |u| + |w| by the factor; then one rounding to the type."""
+
+    y64, size = reference(x, positions, f, layout, inverse)
+    half = torch.finfo(x.dtype).eps / 2
+    tiny = torch.finfo(x.dtype).tiny * half  # half the step of a subnormal
+    off = (y.double() - y64).abs()
+    bound = 3e-7 * f.attention_factor * size * (1 + half) + half * y64.abs() + tiny
+    assert (off <= bound).all(), float((off / bound).nan_to_num(0).max())
+    assert torch.equal(y[..., f.rotary_dim:], x[..., f.rotary_dim:])
+
+
+def states(b, h, s, d, dtype, device, seed, memory="bshd"):
+    if memory == "bshd":
+        return randn((b, s, h, d), dtype, device, seed).transpose(1, 2)
+    if memory == "bhsd":
+        return randn((b, h, s, d), dtype, device, seed)
+    if memory == "slice":  # query or key of one fused projection: rows off 16-byte boundaries
+        return randn((b, s, h, d + 3), dtype, device, seed)[..., 1:d + 1].transpose(1, 2)
+    return randn((s, h, b, d), dtype, device, seed).permute(2, 1, 0, 3)  # sbhd
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+@pytest.mark.parametrize("dim,part", [(128, 128), (128, 32), (80, 20), (80, 40), (96, 96), (64, 2), (10, 10), (10, 6), (8, 8), (4, 2), (2, 2),
+                                      (24, 18), (34, 34), (256, 64)])
+def test_parts_of_heads(gpu, dtype, layout, dim, part):
+    f = RotaryFrequencies(part, 5e5, scaling=YARN)
+    q, k = states(2, 5, 7, dim, dtype, gpu, 1), states(2, 2, 7, dim, dtype, gpu, 2)
+    positions = torch.randint(0, 1 << 20, (2, 7), device=gpu)
+    a, b = triton_apply_rotary_at(q, k, positions, f, layout=layout)
+    check(a, q, positions, f, layout)
+    check(b, k, positions, f, layout)
+    assert a.stride() == q.stride()
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+@pytest.mark.parametrize("memory", ["bshd", "bhsd", "slice", "sbhd"])
+@pytest.mark.parametrize("form", ["offset", "seq", "one", "each", "int32", "strided", "broadcast"])
+def test_positions_and_memory(gpu, layout, memory, form):
+    b, s = 3, 9
+    f = RotaryFrequencies(48, 1e4)
+    x = states(b, 6, s, 64, torch.bfloat16, gpu, 3, memory)
+    at = torch.randint(0, 1 << 24, (b, s), device=gpu)
+    positions = {"offset": 123_457, "seq": at[0], "one": at[:1], "each": at, "int32": at.int(),
+                 "strided": at.repeat_interleave(2, 1)[:, ::2].t().contiguous().t(), "broadcast": at[:, :1].expand(b, s)}[form]
+    y, none = triton_apply_rotary_at(x, None, positions, f, layout=layout)
+    assert none is None
+    check(y, x, positions, f, layout)
+
+
+@pytest.mark.parametrize("positions", [[0, 1, 2**31 - 1, 2**31], [2**32 + 1, 2**40, 2**62, 2**63 - 1], [-1, -2**31, -2**63, -(2**40)]])
+def test_any_integer_is_a_position(gpu, positions):
+    f = RotaryFrequencies(32, 1e6)
+    x = states(1, 3, 4, 32, torch.float32, gpu, 4)
+    p = torch.tensor(positions, device=gpu)
+    check(triton_apply_rotary_at(x, None, p, f)[0], x, p, f, "interleaved")
+    # offsets are added modulo 2^64 too
+    y = ops.rope_at(x, f.turns(gpu), positions=p, offset=5)[0]
+    check(y, x, p + 5, f, "interleaved")
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_shapes(gpu, seed):
+    r = random.Random(seed)
+    dim = 2 * r.randint(1, 70)
+    f = RotaryFrequencies(2 * r.randint(1, dim // 2), 5e5)
+    b, s, h = r.randint(1, 4), r.choice([1, 2, 33, 300]), r.randint(1, 9)
+    dtype = r.choice([torch.float32, torch.float16, torch.bfloat16])
+    layout = r.choice(["interleaved", "rotate_half"])
+    memory = r.choice(["bshd", "bhsd", "slice", "sbhd"])
+    print(f"rope_at b={b} h={h} s={s} dim={dim} part={f.rotary_dim} {dtype} {layout} {memory}", flush=True)
+    q, k = states(b, h, s, dim, dtype, gpu, seed, memory), states(b, r.randint(1, 3), s, dim, dtype, gpu, seed + 1, memory)
+    p = torch.randint(0, 1 << 20, (b, s), device=gpu)
+    for out, x in zip(triton_apply_rotary_at(q, k, p, f, layout=layout), (q, k)):
+        check(out, x, p, f, layout)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+@pytest.mark.parametrize("batch,seq,heads,dim", [(2, 4100, 32, 128), (1, 16500, 7, 80), (3, 1500, 6, 64)])
+def test_large_calls(gpu, layout, batch, seq, heads, dim):
+    """Above the sizes at which the launch changes: heads per item, nontemporal streams."""
+
+    f = RotaryFrequencies(dim, 5e5)
+    q, k = (states(batch, h, seq, dim, torch.bfloat16, gpu, 5) for h in (heads, 3))
+    p = torch.randint(0, 1 << 20, (batch, seq), device=gpu)
+    for out, x in zip(triton_apply_rotary_at(q, k, p, f, layout=layout), (q, k)):
+        check(out, x, p, f, layout)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+def test_gradients(gpu, layout):
+    f = RotaryFrequencies(20, 1e4, scaling=YARN)
+    q, k = (states(2, h, 5, 32, torch.float32, gpu, h).requires_grad_() for h in (4, 2))
+    p = torch.randint(0, 1 << 16, (2, 5), device=gpu)
+    outs = triton_apply_rotary_at(q, k, p, f, layout=layout)
+    ups = [torch.randn_like(o).requires_grad_() for o in outs]
+    grads = torch.autograd.grad(outs, (q, k), ups, create_graph=True)
+    for g, up in zip(grads, ups):
+        check(g.detach(), up.detach(), p, f, layout, inverse=True)
+    # the map is linear: a difference of any size gives the derivative, here along one direction
+    v = torch.randn_like(q)
+    up = triton_apply_rotary_at((q + v).detach(), None, p, f, layout=layout)[0] - triton_apply_rotary_at(q.detach(), None, p, f, layout=layout)[0]
+    # 20 * 3e-7 of sums of |u| + |w| (below 16) for each of 2 * 4 * 5 * 32 products with |ups| below 5
+    assert abs(float((grads[0] * v).sum() - (ups[0] * up).sum())) < 1280 * 3e-7 * 16 * 5
+    # only one of two outputs used, and a gradient with another layout
+    (gk,) = torch.autograd.grad(triton_apply_rotary_at(q, k, p, f, layout=layout)[1], (k,), ups[1].detach().transpose(-1, -2).contiguous().transpose(-1, -2))
+    assert torch.equal(gk, grads[1])
+    # twice differentiable: the gradient of a gradient is the rotation of what arrives
+    (gg,) = torch.autograd.grad(grads[0], (ups[0],), v)
+    check(gg, v, p, f, layout)
+
+
+def test_module_trains_through_the_kernel(gpu):
+    rope = RotaryEmbedding(64, 1e4, use_triton_rope=True, layout="rotate_half", rotary_dim=32, scaling=YARN)
+    q, k = (states(2, h, 6, 64, torch.float32, gpu, h).requires_grad_() for h in (4, 2))
+    p = torch.arange(6, device=gpu).repeat(2, 1)
+    a, b = rope(q, k, p)
+    (a.sum() + b.square().sum()).backward()
+    assert not rope._triton_fallback_warned
+    check(a.detach(), q.detach(), p, rope.frequencies, "rotate_half")
+    check(q.grad, torch.ones_like(q), p, rope.frequencies, "rotate_half", inverse=True)
+
+
+def test_special_values_stay_where_they_are(gpu):
+    f = RotaryFrequencies(8, 1e4)
+    x = torch.ones(1, 1, 3, 24, device=gpu)
+    x[0, 0, 1, 1], x[0, 0, 1, 20], x[0, 0, 2, 9] = float("inf"), float("nan"), float("-inf")
+    for layout in ("interleaved", "rotate_half"):
+        y = triton_apply_rotary_at(x, None, 0, f, layout=layout)[0]
+        assert torch.equal(y[..., 8:].isnan(), x[..., 8:].isnan()) and torch.equal(y[..., 8:].isinf(), x[..., 8:].isinf())
+        bad = ~y[0, 0, 1, :8].isfinite()
+        assert bad.nonzero().flatten().tolist() == ([0, 1] if layout == "interleaved" else [1, 5])
+
+
+def test_empty_and_single(gpu):
+    f = RotaryFrequencies(8, 1e4)
+    for shape in ((0, 2, 3, 8), (2, 0, 3, 8), (2, 2, 0, 8)):
+        x = torch.empty(shape, device=gpu)
+        p = torch.zeros(shape[0], shape[2], dtype=torch.int64, device=gpu)
+        assert triton_apply_rotary_at(x, None, p, f)[0].shape == shape
+    q, k = states(2, 3, 4, 8, torch.float32, gpu, 1), torch.empty(2, 0, 4, 8, device=gpu)
+    a, b = triton_apply_rotary_at(q, k, 3, f)
+    check(a, q, 3, f, "interleaved")
+    assert b.shape == k.shape
+    a, b = triton_apply_rotary_at(k, q, 3, f)
+    check(b, q, 3, f, "interleaved")
+
+
+def test_another_stream_and_replays(gpu):
+    """A decode loop: positions advance in their tensor between the replays of one captured rotation."""
+
+    f = RotaryFrequencies(128, 5e5, scaling=YARN)
+    q, k = states(4, 8, 1, 128, torch.bfloat16, gpu, 1), states(4, 2, 1, 128, torch.bfloat16, gpu, 2)
+    p = torch.tensor([[5], [1000], [0], [77]], device=gpu)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        first = triton_apply_rotary_at(q, k, p, f, layout="rotate_half")
+    torch.cuda.current_stream().wait_stream(stream)
+    check(first[0], q, p, f, "rotate_half")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        a, b = triton_apply_rotary_at(q, k, p, f, layout="rotate_half")
+    for step in range(4):
+        q.copy_(states(4, 8, 1, 128, torch.bfloat16, gpu, 10 + step))
+        p += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = triton_apply_rotary_at(q, k, p, f, layout="rotate_half")
+        assert torch.equal(a, eager[0]) and torch.equal(b, eager[1]), step
+    fresh = RotaryFrequencies(128, 5e5)
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+        with pytest.raises(TritonRoPEUnavailable, match="capture"):
+            triton_apply_rotary_at(q, k, p, fresh)
+
+
+def test_compiles_into_one_graph(gpu):
+    rope = RotaryEmbedding(64, 1e4, use_triton_rope=True, rotary_dim=32)
+    q, k = (states(2, h, 6, 64, torch.float32, gpu, h).requires_grad_() for h in (4, 2))
+    p = torch.arange(6, device=gpu).repeat(2, 1)
+    eager = rope(q, k, p)
+    compiled = torch.compile(rope, backend="aot_eager", fullgraph=True)
+    out = compiled(q, k, p)
+    assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+    g = torch.randn_like(q)
+    assert torch.equal(torch.autograd.grad(out[0], q, g)[0], torch.autograd.grad(eager[0], q, g)[0])
+
+
+@pytest.mark.parametrize("case", ["layout", "odd", "dtype", "mixed", "rank", "stride", "key", "part", "shape", "float positions", "cpu positions"])
+def test_refusals(gpu, case):
+    q = torch.randn(2, 3, 4, 8, device=gpu)
+    k, p, f, layout = q, torch.zeros(2, 4, dtype=torch.int64, device=gpu), RotaryFrequencies(8), "interleaved"
+    if case == "layout":
+        layout = "other"
+    elif case == "odd":
+        q = k = torch.randn(2, 3, 4, 9, device=gpu)
+    elif case == "dtype":
+        q = k = q.double()
+    elif case == "mixed":
+        k = k.bfloat16()
+    elif case == "rank":
+        q = k = q[0]
+    elif case == "stride":
+        q = k = torch.randn(2, 3, 4, 16, device=gpu)[..., ::2]
+    elif case == "key":
+        k = k[:, :, :3]
+    elif case == "part":
+        f = RotaryFrequencies(10)
+    elif case == "shape":
+        p = p[:, :2]
+    elif case == "float positions":
+        p = p.float()
+    else:
+        p = p.cpu()
+    with pytest.raises(TritonRoPEUnavailable):
+        triton_apply_rotary_at(q, k, p, f, layout=layout)
