@@ -353,6 +353,41 @@ int pt_grad_stats(const int64_t* table, int64_t n_tensors, int64_t total_blocks,
 int pt_grad_scale(const int64_t* table, int64_t n_tensors, int64_t total_blocks,
                   const float* scale, void* stream);
 
+/* ---------------------------------------------------------------- AdamW, 8-bit moments
+ * pt_adamw_step with the two moments of a parameter kept in a byte an element, in blocks of
+ * pt_adamw8_scale_elems() (256) elements with a scale byte each.  Parameters and gradients have type
+ * `dtype`; arithmetic is fp32.  No reference counterpart (the reference keeps torch's fp32 moments,
+ * src/picotron/training/train_loop.py:308-325).
+ * `table` is a DEVICE array of n_tensors records of 8 int64:
+ *   {param address, grad address, exp_avg codes, exp_avg scales, exp_avg_sq codes, exp_avg_sq
+ *    scales, numel, first block index}
+ * "first block index": the running sum of ceil(numel / pt_adamw8_block_elems()) over the preceding
+ * records; total_blocks: the sum over all, at most 2^24.  Every record has numel >= 1.  Codes are
+ * ceil(numel / 256) * 256 bytes, 4-byte aligned, scales ceil(numel / 256) bytes; all zero at first.
+ *   scale byte E: the exponent field of the block's largest magnitude as fp32 (16 at least; 255 for
+ *     an infinity or NaN: the block then reads as NaN);
+ *   exp_avg code: the sign, and under it bits 26-20 of the fp32 number |m| * 2^(14 - E);
+ *   exp_avg_sq code: bits 27-20 of v * 2^(30 - E), 1 at least where v > 0.
+ * Both are rounded stochastically: 20 random bits are added to the fp32 number's before the lower
+ * bits are dropped.  With stochastic_params != 0 bf16 parameters are rounded so too (16 bits), else
+ * to nearest.  The bits are a hash of `seed`, the step and the element's place in the table: a call
+ * repeated on the same data gives the same bits.
+ * `step` is the step number after the increment.  With device_step non-NULL (an fp32 device scalar) the
+ * call advances that count by 1 and takes it instead, through 64 bytes of device `workspace` (16-byte
+ * aligned): nothing on the host then depends on the step, and the launches can be captured in a graph.
+ * grad_scale (device fp32, may be NULL) multiplies every gradient as it is read.
+ *   pt_adamw8_moments: the moments' values as `dtype`, element i of table block b at [b * 1024 + i], zeros
+ *     behind a tensor's last element (param and grad addresses are not read); 16-byte aligned outputs of
+ *     total_blocks * 1024 elements. */
+int64_t pt_adamw8_block_elems(void);
+int64_t pt_adamw8_scale_elems(void);
+int pt_adamw8_step(const int64_t* table, int64_t n_tensors, int64_t total_blocks, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, double step,
+                   float* device_step, void* workspace, const float* grad_scale, uint32_t seed,
+                   int stochastic_params, int dtype, void* stream);
+int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blocks, void* exp_avg,
+                      void* exp_avg_sq, int dtype, void* stream);
+
 /* ---------------------------------------------------------------- Utility
  * Device-to-device copy of `bytes` (multiple of 16, 16-byte aligned pointers) with the
  * same 128-bit load/store pattern as the streaming kernels.  No reference counterpart:

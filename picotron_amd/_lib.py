@@ -16,7 +16,7 @@ import os
 import sys
 import threading
 import warnings
-from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(os.environ.get("PICOTRON_HIP_LIB", Path(__file__).with_name("libpicotron_hip.so")))
@@ -138,6 +138,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_void_p, c_size_t, c_void_p],
     ),
     "pt_grad_scale": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "pt_adamw8_block_elems": (c_int64, []),
+    "pt_adamw8_scale_elems": (c_int64, []),
+    "pt_adamw8_step": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_double, c_double, c_double, c_double, c_double, c_double, c_void_p,
+         c_void_p, c_void_p, c_uint32, c_int, c_int, c_void_p],
+    ),
+    "pt_adamw8_moments": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
     "pt_copy": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

@@ -23,6 +23,9 @@ train loop runs right before the step (reference src/picotron/training/train_loo
 and ``_clip_gradients`` :338-350, i.e. ``torch.nn.utils.clip_grad_norm_``): one kernel reads
 the gradients for the norm and the clip coefficient stays on the device, where the step
 applies it as it reads each gradient, instead of a separate read-modify-write pass.
+
+Both take :class:`picotron_amd.optim.AdamW8bit` as well: fp32, fp16 or bf16 parameters with
+gradients of their type (the clipping fp32 ones only) and moments in 8 bits.
 """
 
 from __future__ import annotations
@@ -36,6 +39,7 @@ from torch import Tensor
 from torch.optim import Optimizer
 
 from picotron_amd import _lib, ops
+from picotron_amd.optim import AdamW8bit
 
 
 class TritonAdamWUnavailable(RuntimeError):
@@ -366,9 +370,87 @@ def _run(optimizer: Optimizer, groups, device: torch.device, grad_scale: Tensor 
     _launch(optimizer, groups, launches, grad_scale, write_grad)
 
 
-def triton_adamw_step(optimizer: Optimizer) -> None:
-    """One AdamW step of ``optimizer`` with the fused HIP kernel (or raise unavailable)."""
+def _plan_8bit(optimizer: AdamW8bit) -> tuple[list[tuple[dict, list[Tensor]]], torch.device | None]:
+    """:func:`_plan` for 8-bit moments: everything that can be refused, before any state changes."""
 
+    groups, device, blocks = [], None, 0
+    state_of = optimizer.state
+    for group in optimizer.param_groups:
+        for key in ("lr", "eps", "weight_decay"):
+            if isinstance(group[key], Tensor):
+                raise _reject(f"tensor-valued {key}")
+        if any(isinstance(b, Tensor) for b in group["betas"]):
+            raise _reject("tensor-valued betas")
+        params = [p for p in group["params"] if p.grad is not None]
+        for p in params:
+            g = p.grad
+            if not p.is_cuda or not g.is_cuda:
+                raise _reject("CPU tensors")
+            if p.dtype not in (torch.float32, torch.float16, torch.bfloat16) or g.dtype != p.dtype:
+                raise _reject(f"{p.dtype} parameters with {g.dtype} gradients")
+            if g.is_sparse or not p.is_contiguous() or not g.is_contiguous() or g.device != p.device:
+                raise _reject("parameters or gradients that are not dense and contiguous on one device")
+            if device is None:
+                device = p.device
+                _require_library(device)
+            elif p.device != device:
+                raise _reject("parameters on several devices")
+            state = state_of.get(p)
+            if state:
+                reason = ops.adamw8_reason(p, state)
+                if reason is not None:
+                    raise _reject(reason)
+                step = state.get("step")
+                if not isinstance(step, Tensor) or step.numel() != 1 or (
+                        group["capturable"] and (step.device != device or step.dtype != torch.float32)):
+                    raise _reject("optimizer states whose step is not one element (fp32 on the device for a capturable group)")
+            blocks += (p.numel() + ops.adamw8_sizes()[0] - 1) // ops.adamw8_sizes()[0]
+        groups.append((group, params))
+    if blocks * 256 > 0xFFFFFFFF:
+        raise _reject("more than 2^24 blocks of elements")
+    if device is not None and torch.cuda.is_current_stream_capturing():
+        if not all(group["capturable"] and all(state_of.get(p) for p in params if p.numel()) for group, params in groups if params):
+            raise TritonAdamWUnavailable(
+                "HIP AdamW: a step can be captured for capturable groups whose state exists; run it once before.")
+    return groups, device
+
+
+def _require_library(device: torch.device) -> None:
+    reason = _lib.unavailable_reason()
+    if reason is not None:
+        raise TritonAdamWUnavailable(f"HIP kernel library unavailable: {reason}")
+    if not ops.device_supported(device.index if device.index is not None else torch.cuda.current_device()):
+        raise _reject("devices other than gfx950")
+
+
+def _run_8bit(optimizer: AdamW8bit, groups, device: torch.device, grad_scale: Tensor | None = None) -> None:
+    launches = []
+    for group, params, states, step, seed in optimizer.buckets(groups):
+        host_table, blocks = ops.adamw8_table(params, [p.grad for p in params], states)
+        launches.append((_device_table(host_table, device), blocks, params[0].dtype, states, group, step, seed))
+    _committed(_launch_8bit, launches, grad_scale)
+
+
+def _launch_8bit(launches: list, grad_scale: Tensor | None) -> None:
+    for table, blocks, dtype, states, group, step, seed in launches:
+        if not isinstance(step, Tensor):
+            step = _next_step(step)
+            torch._foreach_add_([state["step"] for state in states], 1.0)
+        beta1, beta2 = group["betas"]
+        ops.adamw8_step(table, blocks, dtype, lr=group["lr"], beta1=beta1, beta2=beta2, eps=group["eps"],
+                        weight_decay=group["weight_decay"], step=step, seed=seed,
+                        stochastic=group["stochastic_rounding"], grad_scale=grad_scale)
+
+
+def triton_adamw_step(optimizer: Optimizer) -> None:
+    """One AdamW step of ``optimizer`` (a ``torch.optim.AdamW`` or an ``AdamW8bit``) with the fused HIP
+    kernel (or raise unavailable)."""
+
+    if isinstance(optimizer, AdamW8bit):
+        groups, device = _plan_8bit(optimizer)
+        if device is not None:
+            _run_8bit(optimizer, groups, device)
+        return
     scan = _scan(optimizer)
     if scan is not None:
         scan.run(None, False)
@@ -390,6 +472,8 @@ def triton_clip_grad_norm_and_step(
     write of every gradient less) while the update still uses the clipped ones.
     """
 
+    if isinstance(optimizer, AdamW8bit):
+        return _clip_and_step_8bit(optimizer, max_norm, write_back_grads)
     scan = _scan(optimizer)
     if scan is not None:
         total_norm, coef = ops.clip_grad_norm(scan.grad_table(), scan.blocks, float(max_norm))
@@ -402,6 +486,20 @@ def triton_clip_grad_norm_and_step(
     host_table, total_blocks = ops.adamw_table(grads, grads, grads, grads)
     total_norm, coef = ops.clip_grad_norm(_device_table(host_table, device), total_blocks, float(max_norm))
     _run(optimizer, groups, device, coef, write_back_grads)
+    return total_norm
+
+
+def _clip_and_step_8bit(optimizer: AdamW8bit, max_norm: float, write_back_grads: bool) -> Tensor:
+    groups, device = _plan_8bit(optimizer)
+    grads, _ = _grads_of(p for _, params in groups for p in params)  # fp32 ones, or refused
+    if device is None:
+        return torch.tensor(0.0)
+    table, blocks = _grad_table(grads, device)
+    total_norm, coef = ops.clip_grad_norm(table, blocks, float(max_norm))
+    if write_back_grads:
+        _committed(ops.grad_scale, table, blocks, coef)
+        coef = None
+    _run_8bit(optimizer, groups, device, coef)
     return total_norm
 
 

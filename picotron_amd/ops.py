@@ -873,6 +873,109 @@ def adamw_step_device_step(
     )
 
 
+_ADAMW8_STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
+
+
+@functools.lru_cache(maxsize=None)
+def adamw8_sizes() -> tuple[int, int]:
+    """(elements of a table block, elements that share a scale) of the AdamW step with 8-bit moments."""
+
+    return int(_lib.lib().pt_adamw8_block_elems()), int(_lib.lib().pt_adamw8_scale_elems())
+
+
+def adamw8_reason(p: Tensor, state: dict) -> str | None:
+    """Why the kernel's raw pointers may not be given parameter ``p`` and its 8-bit ``state``; None if they may."""
+
+    if not p.is_cuda or p.dtype not in _DTYPE_CODES or p.is_sparse or not p.is_contiguous():
+        return "parameters that are not dense contiguous fp32, fp16 or bf16 GPU tensors"
+    per = adamw8_sizes()[1]
+    blocks = (p.numel() + per - 1) // per
+    for key in _ADAMW8_STATE:
+        t = state.get(key)
+        shape = (blocks,) if key.endswith("scale") else (blocks, per)
+        if (not isinstance(t, Tensor) or t.dtype != torch.uint8 or t.device != p.device or tuple(t.shape) != shape
+                or not t.is_contiguous() or (len(shape) == 2 and t.data_ptr() % 4 != 0)):
+            return f"8-bit states whose {key} is not {shape} contiguous uint8 on the parameter's device"
+    return None
+
+
+def adamw8_ready(params: list[Tensor], states: list[dict]) -> bool:
+    """True if the HIP kernels can read these parameters' 8-bit states."""
+
+    return (params[0].is_cuda and _lib.is_available() and device_supported(params[0].device.index)
+            and all(adamw8_reason(p, state) is None for p, state in zip(params, states)))
+
+
+def adamw8_table(params: list[Tensor], grads: list[Tensor], states: list[dict]) -> tuple[Tensor, int]:
+    """Host int64 [n, 8] table for :func:`adamw8_step` and its block count (no empty parameters)."""
+
+    per = adamw8_sizes()[0]
+    rows = []
+    first = 0
+    for p, g, state in zip(params, grads, states):
+        n = p.numel()
+        rows += (p.data_ptr(), g.data_ptr(), state["exp_avg"].data_ptr(), state["exp_avg_scale"].data_ptr(),
+                 state["exp_avg_sq"].data_ptr(), state["exp_avg_sq_scale"].data_ptr(), n, first)
+        first += (n + per - 1) // per
+    return torch.from_numpy(np.array(rows, dtype=np.int64).reshape(-1, 8)), first
+
+
+def adamw8_step(
+    table_device: Tensor,
+    total_blocks: int,
+    dtype: torch.dtype,
+    *,
+    lr: float,
+    beta1: float,
+    beta2: float,
+    eps: float,
+    weight_decay: float,
+    step: float | Tensor,
+    seed: int,
+    stochastic: bool,
+    grad_scale: Tensor | None = None,
+) -> None:
+    """One AdamW step with 8-bit moments over the tensors (parameters of ``dtype``) in a device table built from
+    :func:`adamw8_table`.  ``step``: the step's number, or the fp32 device scalar that counts them, which the call
+    advances.  ``grad_scale`` (fp32 device scalar) multiplies every gradient as it is read."""
+
+    device = _check_cuda(table_device)
+    workspace = device_step = None
+    if isinstance(step, Tensor):
+        if step.dtype != torch.float32 or step.numel() != 1 or step.device != device:
+            raise ValueError("a device step must be one fp32 element on the table's device")
+        device_step, step = step, 0.0
+        workspace = torch.empty(64, dtype=torch.uint8, device=device)
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device):
+        raise ValueError("grad_scale must be one fp32 element on the table's device")
+    _call_on(
+        device, "pt_adamw8_step", table_device.data_ptr(), table_device.size(0), int(total_blocks), float(lr), float(beta1),
+        float(beta2), float(eps), float(weight_decay), float(step), _ptr(device_step), _ptr(workspace), _ptr(grad_scale),
+        int(seed) & 0xFFFFFFFF, int(stochastic), dtype_code(dtype),
+    )
+
+
+def adamw8_moments(
+    params: list[Tensor], states: list[dict], dtype: torch.dtype = torch.float32
+) -> tuple[Tensor, Tensor, list[tuple[Tensor, int]]]:
+    """The values of 8-bit moments, flat: (exp_avg, exp_avg_sq, each parameter's place), zeros between them."""
+
+    device = _check_cuda(*params)
+    for p, state in zip(params, states):
+        reason = adamw8_reason(p, state)
+        if reason is not None:
+            raise ValueError(f"AdamW moments: {reason}")
+    table, blocks = adamw8_table(params, params, states)
+    per = adamw8_sizes()[0]
+    m = torch.empty(blocks * per, dtype=dtype, device=device)
+    v = torch.empty_like(m)
+    places = [(p, first * per) for p, first in zip(params, table[:, 7].tolist())]
+    table = table.to(device)
+    _call_on(device, "pt_adamw8_moments", table.data_ptr(), len(params), blocks, m.data_ptr(), v.data_ptr(),
+             dtype_code(dtype))
+    return m, v, places
+
+
 def clip_grad_norm(table_device: Tensor, total_blocks: int, max_norm: float) -> tuple[Tensor, Tensor]:
     """(total_norm, clip_coef) fp32 device scalars over the gradients of a table built by
     :func:`adamw_table`: torch.nn.utils.clip_grad_norm_'s norm and clamped coefficient."""

@@ -1,0 +1,264 @@
+"""AdamW with 8-bit moments, on the CPU: the codes, the rounding's expected value, the update against AdamW in 64
+bits, checkpoints, and what is refused."""
+
+from __future__ import annotations
+
+import copy
+import ctypes
+import math
+
+import pytest
+import torch
+
+from picotron_amd import _lib, ops
+from picotron_amd.nn.triton_kernels import AdamWStepWithFallback, TritonAdamWUnavailable, triton_adamw_step, triton_clip_grad_norm_and_step
+from picotron_amd.optim import BLOCK, TOP_M, TOP_V, AdamW8bit, decode, encode, mixed_seed, random_bits
+
+NEAREST = 1 << 19
+
+
+def nearest(blocks):
+    return torch.full((blocks, BLOCK), NEAREST, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("top", [TOP_M, TOP_V])
+@pytest.mark.parametrize("scale", [16, 17, 100, 127, 200, 254])
+def test_every_code_keeps_its_value(top, scale):
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 256)
+    values = decode(codes, torch.tensor([scale], dtype=torch.uint8), top)
+    size = codes.double() % 128 if top == TOP_M else codes.double()
+    e, f = (size / 8).floor(), size % 8
+    exact = torch.where(e > 0, (1 + f / 8) * 2.0**e, f / 4) * 2.0 ** (scale - 127 - top)
+    exact = torch.where((codes > 127) & (top == TOP_M), -exact, exact)
+    # the second moment's 32nd exponent is only reached by rounding up: 2^(255 - 127) at a scale of 254 is infinite
+    finite = exact.abs() < 2.0**128
+    assert torch.equal(values.double()[finite], exact[finite]) and values[~finite].isinf().all()
+    in_range = size < 8 * (top + 1)  # of a block whose largest magnitude has this scale
+    back, scales = encode(torch.where(in_range, values, values.flatten()[8 * top]), nearest(1), top)
+    assert scales.item() == scale
+    zero = (top == TOP_M) & (codes == 128)
+    assert torch.equal(back[in_range & ~zero], codes[in_range & ~zero])
+
+
+def test_rounding_goes_to_a_neighbour_and_its_mean_is_the_value():
+    torch.manual_seed(0)
+    blocks = 64
+    for top, values in ((TOP_M, torch.randn(BLOCK) * torch.logspace(-8, 0, BLOCK)), (TOP_V, torch.rand(BLOCK) * torch.logspace(-12, 0, BLOCK))):
+        values[0] = 1.5  # one scale for every block
+        v = values.expand(blocks, BLOCK).contiguous()
+        total = torch.zeros(BLOCK, dtype=torch.float64)
+        for seed in range(32):
+            r = random_bits(seed * blocks // 4, blocks * BLOCK, mixed_seed(3, seed), v.device).view(blocks, BLOCK)
+            codes, scales = encode(v, (r >> 12) & 0xFFFFF, top)
+            got = decode(codes, scales, top).double()
+            lowest = 2.0 ** (127 - 126 - top - 3 + 127 - 127)  # subnormal step at a scale of 127
+            step = torch.maximum(2.0 ** (v.double().abs().log2().floor() - 3), torch.tensor(lowest, dtype=torch.float64))
+            assert ((got - v.double()).abs() <= step).all()
+            total += got.sum(0)
+        n = 32 * blocks
+        off = (total / n - values.double()).abs()
+        # the error of one rounding has a standard deviation of at most step / 2; five of the mean's.  Below the lowest code
+        # a positive second moment takes that code instead
+        kept = slice(None) if top == TOP_M else values > lowest
+        assert (off <= 5 * step[0] / 2 / math.sqrt(n))[kept].all()
+
+
+def test_random_bits_do_not_depend_on_where_they_start():
+    whole = random_bits(0, 4096, 12345, torch.device("cpu"))
+    assert torch.equal(whole[1024:2048], random_bits(1, 1024, 12345, torch.device("cpu")))
+    bits = torch.stack([(random_bits(0, 1 << 16, mixed_seed(7, 1), whole.device) >> i) & 1 for i in range(32)]).double()
+    # each bit's mean over 2^16 draws: five standard deviations of 1/512
+    assert ((bits.mean(1) - 0.5).abs() < 5 / 512).all()
+    # and neighbours agree half of the time
+    assert (((bits[:, 1:] == bits[:, :-1]).double().mean(1) - 0.5).abs() < 5 / 512).all()
+    # places pass 32 bits without an error
+    assert random_bits((1 << 24) - 1, 1024, 5, whole.device).shape == (1024,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_one_step_is_adamw_rounded(dtype):
+    torch.manual_seed(1)
+    hp = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    p = torch.nn.Parameter((torch.randn(3, 700) * 0.02).to(dtype))
+    p.grad = (torch.randn(3, 700) * 1e-2).to(dtype)
+    start = p.detach().clone()
+    optimizer = AdamW8bit([p], **hp)
+    optimizer.step()
+    g = p.grad.double()
+    m, v = 0.1 * g, 0.01 * g * g
+    update = hp["lr"] * (m / 0.1) / ((v / 0.01).sqrt() + 1e-8)
+    x = start.double() * (1 - 1e-3) - update
+    # fp32 roundings of the parts, whose sizes are |x| and |update| at most together, and one step of the parameter's type
+    # (rounded stochastically in bf16, to nearest else), a subnormal's at least
+    step = torch.finfo(dtype).eps * (1.0 if dtype == torch.bfloat16 else 0.5)
+    bound = step * (x.abs() + torch.finfo(dtype).tiny) + 2.0**-21 * (x.abs() + update.abs())
+    assert ((p.double() - x).abs() <= bound).all()
+    got_m, got_v, places = optimizer.moments()
+    assert places == [(p, 0)] and got_m.numel() == 3 * 1024
+    assert not got_m[2100:].any() and not got_v[2100:].any()
+    # neighbours of the value: a step of the fraction's last bit, at least the block's subnormal one
+    for got, want, top in ((got_m, m, TOP_M), (got_v, v, TOP_V)):
+        want = torch.cat((want.flatten(), torch.zeros(9 * 256 - 2100, dtype=torch.float64))).view(9, 256)
+        low = 2.0 ** (want.abs().amax(1, keepdim=True).log2().floor() + 1 - top - 3)
+        size = torch.maximum(2.0 ** (want.abs().clamp_min(1e-300).log2().floor() - 3), low)
+        assert ((got[:9 * 256].view(9, 256).double() - want).abs() <= size * 1.001).all()
+
+
+def test_moments_follow_a_slow_average():
+    """What rounding to nearest would not do: the second moment decays with beta2 = 0.999 once the gradient is gone."""
+
+    p = torch.nn.Parameter(torch.zeros(4096))
+    optimizer = AdamW8bit([p], lr=0.0, betas=(0.9, 0.999), weight_decay=0.0)
+    p.grad = torch.ones(4096)
+    optimizer.step()
+    first = optimizer.moments()[1].mean()
+    p.grad = torch.zeros(4096)
+    for _ in range(200):
+        optimizer.step()
+    # the mean of 4096 random walks, each of a standard deviation below 1/3 (a step of 1/8 is taken with a probability of 1/100,
+    # two hundred times): five of the mean's
+    assert abs(float(optimizer.moments()[1].mean() / first) - 0.999**200) < 5 / 3 / 64
+
+
+def test_positive_second_moments_stay_positive():
+    p = torch.nn.Parameter(torch.zeros(256))
+    g = torch.full((256,), 1e-9)
+    g[0] = 1e3
+    p.grad = g
+    optimizer = AdamW8bit([p])
+    optimizer.step()
+    assert (optimizer.moments()[1][:256] > 0).all()
+    p.grad = torch.zeros(256)
+    for _ in range(3):
+        optimizer.step()
+    assert p.isfinite().all() and (p.abs() <= 1e-2).all()
+
+
+def test_a_gradient_that_is_no_number_stays_in_its_block():
+    p = torch.nn.Parameter(torch.zeros(700))
+    p.grad = torch.ones(700)
+    p.grad[300] = float("nan")
+    optimizer = AdamW8bit([p])
+    optimizer.step()
+    m, v, _ = optimizer.moments()
+    for moment in (m, v):
+        assert moment[256:512].isnan().all() and moment[:256].isfinite().all() and moment[512:].isfinite().all()
+    assert p[300].isnan() and p.isnan().sum() == 1
+    p.grad = torch.ones(700)
+    optimizer.step()
+    assert p[256:512].isnan().all() and p[:256].isfinite().all()
+
+
+def _trained(dtype=torch.float32, **options):
+    torch.manual_seed(2)
+    params = [torch.nn.Parameter((torch.randn(s) * 0.02).to(dtype)) for s in ((5, 300), (7,), (0,), (1024,))]
+    optimizer = AdamW8bit(params, lr=1e-3, seed=11, **options)
+    for _ in range(3):
+        for p in params:
+            p.grad = torch.randn_like(p)
+        optimizer.step()
+    return params, optimizer
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_checkpoint_round_trip(dtype, capturable):
+    params, optimizer = _trained(dtype, capturable=capturable)
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = AdamW8bit(copies, lr=1.0)
+    other.load_state_dict(copy.deepcopy(optimizer.state_dict()))
+    assert other.param_groups[0]["seed"] == 11 and other.param_groups[0]["lr"] == 1e-3
+    for p, q in zip(params, copies):
+        q.grad = p.grad
+        for key, value in optimizer.state[p].items():
+            assert torch.equal(value, other.state[q][key]) and value.dtype == other.state[q][key].dtype, key
+    optimizer.step()
+    other.step()
+    for p, q in zip(params, copies):
+        assert torch.equal(p, q)
+    if capturable:
+        assert len({id(other.state[q]["step"]) for q in copies if q.numel()}) == 1
+
+
+def test_state_of_torch_adamw_is_taken():
+    torch.manual_seed(3)
+    p = torch.nn.Parameter(torch.randn(300))
+    q = torch.nn.Parameter(p.detach().clone())
+    theirs = torch.optim.AdamW([p], lr=1e-3)
+    p.grad = torch.randn(300)
+    theirs.step()
+    ours = AdamW8bit([q])
+    ours.load_state_dict(theirs.state_dict())
+    m, v, _ = ours.moments()
+    # the nearest code: half a step of 1/8 (the top of each binade's spacing relative to its bottom), or of a subnormal
+    state = theirs.state[p]
+    for got, want in ((m[:300], state["exp_avg"]), (v[:300], state["exp_avg_sq"])):
+        assert ((got - want).abs() <= want.abs() / 16 + want.abs().max() * 2.0**-16).all()
+    q.grad = p.grad
+    ours.step()
+    with pytest.raises(ValueError, match="amsgrad"):
+        AdamW8bit([q]).load_state_dict(torch.optim.AdamW([p], amsgrad=True).state_dict())
+
+
+@pytest.mark.parametrize("bad", [dict(lr=-1.0), dict(eps=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(weight_decay=-1.0),
+                                 dict(lr=torch.tensor(1.0))])
+def test_constructor_refuses(bad):
+    with pytest.raises(ValueError):
+        AdamW8bit([torch.nn.Parameter(torch.zeros(3))], **bad)
+
+
+def test_fused_step_refuses_the_cpu_and_the_stepper_falls_back():
+    params, optimizer = _trained()
+    before = [p.detach().clone() for p in params]
+    with pytest.raises(TritonAdamWUnavailable):
+        triton_adamw_step(optimizer)
+    with pytest.raises(TritonAdamWUnavailable):
+        triton_clip_grad_norm_and_step(optimizer, 1.0)
+    assert all(torch.equal(p, b) for p, b in zip(params, before))
+    with pytest.warns(RuntimeWarning, match="Triton AdamW unavailable"):
+        AdamWStepWithFallback(use_triton=True).step(optimizer)
+    assert not torch.equal(params[0], before[0]) and float(optimizer.state[params[0]]["step"]) == 4.0
+
+
+def test_sizes():
+    assert ops.adamw8_sizes() == (1024, BLOCK)
+
+
+_TABLE = (ctypes.c_int64 * 8)()
+_T = ctypes.addressof(_TABLE)
+
+
+@pytest.mark.parametrize("args,code", [
+    ((None, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T + 4, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T, -1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T, 2, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T, 1, 1 << 25, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 0, None), _lib.PT_EUNSUPPORTED),
+    ((_T, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 0.0, None, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, float("nan"), None, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 9, None), _lib.PT_EINVAL),
+    ((_T, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, 4096, None, None, 0, 0, 0, None), _lib.PT_EINVAL),
+    ((_T, 1, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, 4096, 4100, None, 0, 0, 0, None), _lib.PT_EINVAL),
+])
+def test_step_entry_point_refuses(args, code):
+    assert _lib.lib().pt_adamw8_step(*args) == code
+    assert _lib.lib().pt_last_error().decode().startswith("pt_adamw8_step")
+
+
+@pytest.mark.parametrize("args,code", [
+    ((None, 1, 1, 4096, 4096, 0, None), _lib.PT_EINVAL), ((_T, 1, 1, None, 4096, 0, None), _lib.PT_EINVAL),
+    ((_T, 1, 1, 4096, 4104, 0, None), _lib.PT_EINVAL), ((_T, 1, 1, 4096, 4096, 5, None), _lib.PT_EINVAL),
+    ((_T, 1, 1 << 25, 4096, 4096, 0, None), _lib.PT_EUNSUPPORTED),
+])
+def test_moments_entry_point_refuses(args, code):
+    assert _lib.lib().pt_adamw8_moments(*args) == code
+    assert _lib.lib().pt_last_error().decode().startswith("pt_adamw8_moments")
+
+
+def test_nothing_to_do():
+    assert _lib.lib().pt_adamw8_step(None, 0, 0, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None, None, None, 0, 0, 0, None) == _lib.PT_OK
+    assert _lib.lib().pt_adamw8_moments(None, 0, 0, None, None, 0, None) == _lib.PT_OK
+    empty = AdamW8bit([torch.nn.Parameter(torch.zeros(0))])
+    empty.param_groups[0]["params"][0].grad = torch.zeros(0)
+    empty.step()
+    assert empty.moments()[2] == []
