@@ -250,6 +250,50 @@ int pt_cross_entropy_shifted_scale_grad(void* dlogits, int64_t batch, int64_t se
                                         int64_t logits_batch_stride, int64_t logits_seq_stride,
                                         const void* workspace, int dtype, void* stream);
 
+/* ---------------------------------------------------------------- Preference loss
+ * Sequence log-probabilities of (batch, seq, vocab) logits, and the preference loss on pairs of
+ * them.  Row (b, t) starts at logits + b*batch_stride + t*seq_stride and holds `vocab` contiguous
+ * logits; its label is labels[b*l_batch_stride + (t+shift)*l_seq_stride] (int64; shift 1 for
+ * next-token logits against the sequence's own labels, 0 for labels already shifted).  Positions
+ * whose label is ignore_index, and with shift the last one, are left out.
+ *   y_b = sum over the kept positions of logit[label] - log-sum-exp   (divided by their number, when
+ *     there are any, with average != 0); a label outside [0, vocab) makes y_b NaN.
+ * pt_sequence_log_probs writes y (fp32, one a sequence).  pt_preference_loss takes 2 * pairs sequences,
+ * sequence i the chosen one of pair i and i + pairs the rejected one, and `reference` (fp32, 2 *
+ * pairs; NULL: zeros), and writes y, rewards_b = beta * (y_b - reference_b) and, with
+ * h_i = rewards_i - rewards_{i+pairs}, the mean over pairs of
+ *   kind 0: -(1 - e) * ln sigmoid(h) - e * ln sigmoid(-h)   (e = label_smoothing)
+ *   kind 1: max(0, 1 - h)
+ *   kind 2: (h / beta - 1 / (2 * beta))^2
+ * Both leave in `workspace` (pt_sequence_log_probs_workspace_bytes, 16-byte aligned, the caller's until
+ * the backward has run) what pt_sequence_log_probs_bwd reads: it writes every row of
+ *   dlogits = g_b * ([j == label] - softmax)   at kept positions, 0 elsewhere
+ * in fp32 arithmetic, rounded once, to grad (rows at g_batch_stride, g_seq_stride, in the 16-byte phase
+ * of the logits rows, another tensor than the logits).  g_b is grad_log_probs[b] (divided by the number
+ * of kept positions for an average), after pt_sequence_log_probs; or, after pt_preference_loss, d loss /
+ * d y_b times the fp32 device scalar *grad_loss: exactly one of the two pointers is given.
+ * Replaces the DPO trainer's log_softmax and gather over whole logits
+ * (src/picotron_dpo/dpo_trainer.py:297) and autograd's backward of them. */
+size_t pt_sequence_log_probs_workspace_bytes(int64_t batch, int64_t seq, int64_t vocab, int dtype);
+int pt_sequence_log_probs(const void* logits, int64_t batch, int64_t seq, int64_t batch_stride,
+                          int64_t seq_stride, int64_t vocab, const int64_t* labels,
+                          int64_t l_batch_stride, int64_t l_seq_stride, int shift,
+                          int64_t ignore_index, int average, float* log_probs, void* workspace,
+                          size_t workspace_bytes, int dtype, void* stream);
+int pt_preference_loss(const void* logits, int64_t pairs, int64_t seq, int64_t batch_stride,
+                       int64_t seq_stride, int64_t vocab, const int64_t* labels,
+                       int64_t l_batch_stride, int64_t l_seq_stride, int shift, int64_t ignore_index,
+                       int average, const float* reference, float beta, float label_smoothing, int kind,
+                       float* loss, float* rewards, float* log_probs, void* workspace,
+                       size_t workspace_bytes, int dtype, void* stream);
+int pt_sequence_log_probs_bwd(const void* logits, int64_t batch, int64_t seq, int64_t batch_stride,
+                              int64_t seq_stride, int64_t vocab, const int64_t* labels,
+                              int64_t l_batch_stride, int64_t l_seq_stride, int shift,
+                              int64_t ignore_index, const float* grad_log_probs,
+                              const float* grad_loss, void* grad, int64_t g_batch_stride,
+                              int64_t g_seq_stride, const void* workspace, size_t workspace_bytes,
+                              int dtype, void* stream);
+
 /* ---------------------------------------------------------------- AdamW
  * One decoupled-weight-decay Adam step over many fp32 tensors in one launch, with
  * torch.optim.AdamW's single-tensor arithmetic (amsgrad=False, maximize=False), per element:

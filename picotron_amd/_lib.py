@@ -105,6 +105,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
          c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p],
     ),
+    "pt_sequence_log_probs_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "pt_sequence_log_probs": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64,
+         c_int, c_void_p, c_void_p, c_size_t, c_int, c_void_p],
+    ),
+    "pt_preference_loss": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64,
+         c_int, c_void_p, c_float, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int,
+         c_void_p],
+    ),
+    "pt_sequence_log_probs_bwd": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64,
+         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_int, c_void_p],
+    ),
     "pt_adamw_block_elems": (c_int64, []),
     "pt_adamw_step": (
         c_int,

@@ -25,6 +25,15 @@ from picotron_amd.nn.triton_kernels.cross_entropy import (
     TritonCrossEntropyUnavailable,
     triton_cross_entropy,
 )
+from picotron_amd.nn.triton_kernels.preference import (
+    PreferenceLoss,
+    PreferenceLossWithFallback,
+    TritonPreferenceUnavailable,
+    preference_loss_with_pytorch,
+    sequence_log_probs_with_pytorch,
+    triton_preference_loss,
+    triton_sequence_log_probs,
+)
 from picotron_amd.nn.triton_kernels.rmsnorm import (
     TritonRMSNormUnavailable,
     rms_norm_with_pytorch_forward,
@@ -61,12 +70,19 @@ __all__ = [
     "rms_norm_with_pytorch_forward",
     # additions beyond the reference surface
     "FusedAdamWStepFailed",
+    "PreferenceLoss",
+    "PreferenceLossWithFallback",
+    "TritonPreferenceUnavailable",
+    "preference_loss_with_pytorch",
+    "sequence_log_probs_with_pytorch",
     "triton_adamw_step",
     "triton_apply_rotary_at",
     "triton_apply_rotary_embedding_pair",
     "triton_clip_grad_norm_and_step",
     "triton_grad_scaler_step",
+    "triton_preference_loss",
     "triton_residual_rms_norm",
+    "triton_sequence_log_probs",
     "triton_unscale_and_check_",
     "triton_unscale_clip_and_step",
     "triton_zero_clip_grad_norm_",

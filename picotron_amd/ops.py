@@ -714,6 +714,97 @@ def cross_entropy_shifted_scale_grad(
     )
 
 
+# ------------------------------------------------------------------ preference loss
+
+PREFERENCE_LOSSES = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+
+
+def _sequence_rows(logits: Tensor, labels: Tensor, shift: bool) -> tuple:
+    """(seq, batch stride, seq stride, vocab, labels, their strides, shift) of (batch, seq, vocab) logits and (batch, seq)
+    labels, as the entry points take them."""
+
+    if logits.dim() != 3 or logits.size(2) < 1:
+        raise ValueError("logits must be (batch, seq, vocab)")
+    if logits.stride(2) != 1 and logits.size(2) > 1:
+        raise ValueError("logits need a contiguous vocabulary dimension")
+    if labels.dtype != torch.int64 or tuple(labels.shape) != tuple(logits.shape[:2]):
+        raise ValueError(f"labels must be int64 of shape {tuple(logits.shape[:2])}")
+    return (logits.size(1), logits.stride(0), logits.stride(1), logits.size(2), labels.data_ptr(), labels.stride(0),
+            labels.stride(1), int(shift))
+
+
+def _sequence_workspace(logits: Tensor) -> tuple[Tensor, int]:
+    size = int(_lib.lib().pt_sequence_log_probs_workspace_bytes(*logits.shape, dtype_code(logits.dtype)))
+    return torch.empty(max(size, 16), dtype=torch.uint8, device=logits.device), size
+
+
+def sequence_log_probs(
+    logits: Tensor, labels: Tensor, *, shift: bool = True, ignore_index: int = -100, average: bool = False
+) -> tuple[Tensor, Tensor]:
+    """(log-probability of each sequence's kept labels, fp32; workspace for :func:`sequence_log_probs_bwd`)."""
+
+    device = _check_cuda(logits, labels)
+    rows = _sequence_rows(logits, labels, shift)
+    ws, size = _sequence_workspace(logits)
+    out = torch.empty(logits.size(0), dtype=torch.float32, device=device)
+    _call_on(device, "pt_sequence_log_probs", logits.data_ptr(), logits.size(0), *rows, int(ignore_index), int(average),
+             out.data_ptr(), ws.data_ptr(), size, dtype_code(logits.dtype))
+    return out, ws
+
+
+def preference_loss(
+    logits: Tensor, labels: Tensor, reference: Tensor | None, *, beta: float, label_smoothing: float = 0.0,
+    kind: str = "sigmoid", shift: bool = True, ignore_index: int = -100, average: bool = False,
+) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(loss, rewards, log-probabilities, workspace) over logits whose first half of sequences are the chosen ones of
+    the pairs and whose second half the rejected ones; ``reference``: fp32 log-probabilities, or None for zeros."""
+
+    device = _check_cuda(logits, labels, *([] if reference is None else [reference]))
+    rows = _sequence_rows(logits, labels, shift)
+    batch = logits.size(0)
+    if batch < 2 or batch % 2 != 0:
+        raise ValueError("a preference loss takes pairs: an even number of sequences, the chosen ones first")
+    if reference is not None and (reference.dtype != torch.float32 or tuple(reference.shape) != (batch,)
+                                  or not reference.is_contiguous()):
+        raise ValueError("reference log-probabilities must be contiguous fp32, one a sequence")
+    if kind not in PREFERENCE_LOSSES:
+        raise ValueError(f"loss must be one of {sorted(PREFERENCE_LOSSES)}")
+    ws, size = _sequence_workspace(logits)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    rewards = torch.empty(batch, dtype=torch.float32, device=device)
+    log_probs = torch.empty_like(rewards)
+    _call_on(device, "pt_preference_loss", logits.data_ptr(), batch // 2, *rows, int(ignore_index), int(average),
+             _ptr(reference), float(beta), float(label_smoothing), PREFERENCE_LOSSES[kind], loss.data_ptr(),
+             rewards.data_ptr(), log_probs.data_ptr(), ws.data_ptr(), size, dtype_code(logits.dtype))
+    return loss, rewards, log_probs, ws
+
+
+def sequence_log_probs_bwd(
+    logits: Tensor, labels: Tensor, workspace: Tensor, *, grad_log_probs: Tensor | None = None,
+    grad_loss: Tensor | None = None, shift: bool = True, ignore_index: int = -100,
+) -> Tensor:
+    """The logits' gradient, from the gradient of the log-probabilities or of the preference loss (a scalar) whose
+    forward left ``workspace``."""
+
+    up = grad_log_probs if grad_log_probs is not None else grad_loss
+    device = _check_cuda(logits, labels, workspace, up)
+    grad = ce_grad_buffer(logits, 2)
+    if grad is None:  # rows that overlap in memory (an expanded tensor)
+        logits = logits.contiguous()
+        grad = ce_grad_buffer(logits, 2)
+    rows = _sequence_rows(logits, labels, shift)
+    up = up.detach().to(torch.float32).contiguous()
+    if up.numel() != (1 if grad_log_probs is None else logits.size(0)):
+        raise ValueError("one gradient a sequence, or one of the loss")
+    size = int(_lib.lib().pt_sequence_log_probs_workspace_bytes(*logits.shape, dtype_code(logits.dtype)))
+    if workspace.numel() < size:
+        raise ValueError("the workspace is not that of these logits")
+    _call_on(device, "pt_sequence_log_probs_bwd", logits.data_ptr(), logits.size(0), *rows, int(ignore_index),
+             up.data_ptr() if grad_log_probs is not None else None, up.data_ptr() if grad_log_probs is None else None,
+             grad.data_ptr(), grad.stride(0), grad.stride(1), workspace.data_ptr(), size, dtype_code(logits.dtype))
+    return grad
+
+
 # ------------------------------------------------------------------ AdamW
 
 
