@@ -20,8 +20,8 @@
 // the caller's and the step count), four elements in a row taking successive states of Marsaglia's 32-bit xorshift
 // generator.  The first moment takes bits 31-12, the second 15-0 and 31-28, the parameter 23-8.
 //
-// One launch covers every tensor: workgroup b finds its tensor by a search of the table's first-block indices and takes 1024
-// elements of it, each wave one block of 256, four elements a lane, so that a block's maximum is a wave's.
+// One launch covers every tensor.  A wave takes units of 1024 elements, four blocks of 256 with four elements a lane, so that
+// a block's maximum is a wave's and no barrier is needed.
 #include <cmath>
 #include <type_traits>
 
@@ -32,8 +32,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kQuant = 256;          // elements that share a scale
-constexpr int64_t kUnitElems = 1024;  // elements of a workgroup
-constexpr int kTopM = 14;
+constexpr int64_t kUnitElems = 1024;  // elements of a wave's unit, a block of the table
+constexpr int kBlocks = static_cast<int>(kUnitElems / kQuant);
+constexpr int kWaves = kThreads / 64;
 constexpr int kTopV = 30;
 constexpr uint32_t kMinScale = 16;
 
@@ -139,41 +140,77 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t bits) {
   return e > kMinScale ? e : kMinScale;
 }
 
-__device__ __forceinline__ float decode_m(uint32_t code, int e) {
-  const float y = __builtin_amdgcn_ldexpf(__uint_as_float((code & 127u) << 20), e - kTopM);
-  return __uint_as_float(__float_as_uint(y) | ((code & 128u) << 24));
+// Reading and writing codes.  A first-moment code is the hardware's 8-bit float (4 exponent bits, bias 7) in its own
+// right, its block's factor 2^(E - 134): the conversions, stochastic rounding with the top 20 of 32 random bits
+// among them, are one instruction each and give the bits of the integer form in the file's comment (checked over 10^6
+// values of both signs, subnormals and zeros among them).  They took the step of 1.04e9 bf16 elements from XX to YY us.
+// The second moment's format is no hardware one.
+__device__ __forceinline__ float factor_m(int e) {  // what a first-moment code of a block with scale e is multiplied by
+  return e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(e - 134 + 127) << 23);
 }
 
-__device__ __forceinline__ float decode_v(uint32_t code, int e) {
-  return __builtin_amdgcn_ldexpf(__uint_as_float(code << 20), e - kTopV);
+__device__ __forceinline__ void decode_m(uint32_t word, int e, float (&m)[4]) {
+  const float f = factor_m(e);
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word), true);
+  m[0] = lo[0] * f;
+  m[1] = lo[1] * f;
+  m[2] = hi[0] * f;
+  m[3] = hi[1] * f;
 }
 
-__device__ __forceinline__ uint32_t encode_m(float m, int e, uint32_t r) {
-  const uint32_t y = __float_as_uint(__builtin_amdgcn_ldexpf(fabsf(m), kTopM - e));
-  return ((y + (r >> 12)) >> 20) | ((__float_as_uint(m) >> 24) & 128u);
+__device__ __forceinline__ void decode_v(uint32_t word, int e, float (&v)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = __builtin_amdgcn_ldexpf(__uint_as_float(((word >> (8 * k)) & 255u) << 20), e - kTopV);
+  if (e == 255) v[0] = v[1] = v[2] = v[3] = NAN;
 }
 
-__device__ __forceinline__ uint32_t encode_v(float v, int e, uint32_t r) {
-  const uint32_t y = __float_as_uint(__builtin_amdgcn_ldexpf(v, kTopV - e));
-  const uint32_t code = (y + (((r << 4) & 0xFFFF0u) | (r >> 28))) >> 20;
-  const uint32_t least = v > 0.0f ? 1u : 0u;
-  return code > least ? code : least;
+__device__ __forceinline__ uint32_t encode_m(const float (&m)[4], int e, const uint32_t (&r)[4]) {
+  const float f = __uint_as_float(static_cast<uint32_t>(134 - e + 127) << 23);
+  int w = 0;
+  w = __builtin_amdgcn_cvt_sr_fp8_f32(m[0] * f, static_cast<int>(r[0]), w, 0);
+  w = __builtin_amdgcn_cvt_sr_fp8_f32(m[1] * f, static_cast<int>(r[1]), w, 1);
+  w = __builtin_amdgcn_cvt_sr_fp8_f32(m[2] * f, static_cast<int>(r[2]), w, 2);
+  w = __builtin_amdgcn_cvt_sr_fp8_f32(m[3] * f, static_cast<int>(r[3]), w, 3);
+  return static_cast<uint32_t>(w);
 }
 
-// Four elements of a lane from `base`, as fp32; `count` of them exist (the vector path has all four).
+__device__ __forceinline__ uint32_t encode_v(const float (&v)[4], int e, const uint32_t (&r)[4]) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t y = __float_as_uint(__builtin_amdgcn_ldexpf(v[k], kTopV - e));
+    const uint32_t code = (y + (__builtin_rotateleft32(r[k], 4) & 0xFFFFFu)) >> 20;
+    const uint32_t least = __float_as_uint(v[k]) < 1u ? __float_as_uint(v[k]) : 1u;  // 1 for any positive value
+    w |= (code > least ? code : least) << (8 * k);
+  }
+  return w;
+}
+
+// Four elements of a lane, and their bits as buffer accesses move them.
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 template <typename T>
-struct Four;
+struct Four {
+  typedef T type __attribute__((ext_vector_type(4)));
+  typedef u32x2 bits;
+  static __device__ __forceinline__ type load(__amdgpu_buffer_rsrc_t b, int off) {
+    return __builtin_bit_cast(type, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, kNonTemporal));
+  }
+  static __device__ __forceinline__ void store(type v, __amdgpu_buffer_rsrc_t b, int off) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(bits, v), b, off, 0, kWriteThrough);
+  }
+};
 template <>
 struct Four<float> {
   typedef f32x4 type;
-};
-template <>
-struct Four<_Float16> {
-  typedef _Float16 type __attribute__((ext_vector_type(4)));
-};
-template <>
-struct Four<__bf16> {
-  typedef __bf16 type __attribute__((ext_vector_type(4)));
+  typedef u32x4 bits;
+  static __device__ __forceinline__ type load(__amdgpu_buffer_rsrc_t b, int off) {
+    return __builtin_bit_cast(type, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, kNonTemporal));
+  }
+  static __device__ __forceinline__ void store(type v, __amdgpu_buffer_rsrc_t b, int off) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(bits, v), b, off, 0, kWriteThrough);
+  }
 };
 
 // x in bf16, rounded by 16 random bits; infinities and NaN as they are.
@@ -183,142 +220,234 @@ __device__ __forceinline__ __bf16 stochastic_bf16(float x, uint32_t r) {
   return static_cast<__bf16>(__uint_as_float((u + ((r >> 8) & 0xffffu)) & 0xffff0000u));
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
-                                                          Scalars8 by_value, const Scalars8* __restrict__ scalars,
-                                                          const float* __restrict__ grad_scale, int stochastic) {
-#pragma clang fp contract(off)
-  typedef typename Four<T>::type T4;
-  const uint32_t blk = blockIdx.x;
-  const Rec8 rec = table[find_record(table, n_tensors, blk)];
-  const Scalars8 s = scalars != nullptr ? *scalars : by_value;
-  const int lane = threadIdx.x % 64;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64);
-  const int64_t unit = blk - rec.first_block;
-  const int64_t q = unit * (kUnitElems / kQuant) + wave;  // the block of 256
-  if (q * kQuant >= rec.n) return;
-  const int64_t i = q * kQuant + lane * 4;
-  const gptr<T> P = as_global<T>(rec.p) + i;
-  const gptr<const T> G = as_global<const T>(rec.g) + i;
-  const gptr<uint32_t> MC = as_global<uint32_t>(rec.mc + i), VC = as_global<uint32_t>(rec.vc + i);
-  const gptr<unsigned char> MS = as_global<unsigned char>(rec.ms + q), VS = as_global<unsigned char>(rec.vs + q);
-  const int em = __builtin_amdgcn_readfirstlane(*MS), ev = __builtin_amdgcn_readfirstlane(*VS);
-  const uint32_t mw = *MC, vw = *VC;
-  const bool whole = ((rec.p | rec.g) & (4 * sizeof(T) - 1)) == 0 && (q + 1) * kQuant <= rec.n;
-  const int64_t left = rec.n - i;  // this lane's elements, when there are fewer than four
-  float p[4], g[4];
-  if (whole) {
-    const T4 pv = *reinterpret_cast<gptr<const T4>>(P);
-    const T4 gv = *reinterpret_cast<gptr<const T4>>(G);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      p[k] = static_cast<float>(pv[k]);
-      g[k] = static_cast<float>(gv[k]);
-    }
+// Calls f(record, unit of its tensor, unit of the table) for each unit of the wave.  RUNS: workgroup b takes the units
+// [b * per, (b + 1) * per), a run of each tensor they lie in, its four waves in turn, so that the table is
+// searched once a workgroup; else every wave has the unit of its number.
+template <bool RUNS, typename F>
+__device__ __forceinline__ void walk_units(const Rec8* __restrict__ table, uint32_t n_tensors, uint32_t units,
+                                           uint32_t per, const F& f) {
+  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
+  if constexpr (!RUNS) {
+    const uint32_t u = blockIdx.x * kWaves + wave;
+    if (u >= units) return;
+    const Rec8 rec = table[find_record(table, n_tensors, u)];
+    f(rec, u - rec.first_block, u);
   } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      p[k] = k < left ? static_cast<float>(P[k]) : 0.0f;
-      g[k] = k < left ? static_cast<float>(G[k]) : 0.0f;
+    uint32_t at = blockIdx.x * per;
+    const uint32_t end = at + per < units ? at + per : units;
+    if (at >= end) return;
+    for (uint32_t row = find_record(table, n_tensors, at); at < end; ++row) {
+      const Rec8 rec = table[row];
+      const uint32_t next = row + 1 < n_tensors ? static_cast<uint32_t>(table[row + 1].first_block) : end;
+      const uint32_t stop = next < end ? next : end;
+      for (uint32_t u = at + wave; u < stop; u += kWaves) f(rec, u - rec.first_block, u);
+      at = stop;
     }
   }
-  if (grad_scale != nullptr) {
-    const float gs = *grad_scale;
-    // (an element behind the end stays zero under an infinite scale)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = k < left ? g[k] * gs : 0.0f;
-  }
+}
+
+// One block's four elements of a lane: the parameters p and gradients g in, the new parameters out; the codes and the
+// scales replaced.  `place`: the first element's place in the call, over 4.
+template <typename T>
+__device__ __forceinline__ typename Four<T>::type update(typename Four<T>::type p, const float (&g)[4], const Scalars8& s,
+                                                         uint32_t place, int stochastic, uint32_t* mw, uint32_t* vw,
+                                                         int* em, int* ev) {
+#pragma clang fp contract(off)
   uint32_t r[4];
-  {
-    uint32_t x = (blk * kThreads + threadIdx.x) * 0x9E3779B1u + s.seed;
-    x = (x ^ (x >> 16)) * 0x7FEB352Du;
-    x ^= x >> 15;
+  uint32_t x = place * 0x9E3779B1u + s.seed;
+  x = (x ^ (x >> 16)) * 0x7FEB352Du;
+  x ^= x >> 15;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x ^= x << 13;
-      x ^= x >> 17;
-      x ^= x << 5;
-      r[k] = x;
-    }
+  for (int k = 0; k < 4; ++k) {
+    x ^= x << 13;
+    x ^= x >> 17;
+    x ^= x << 5;
+    r[k] = x;
   }
   float m[4], v[4];
+  decode_m(*mw, *em, m);
+  decode_v(*vw, *ev, v);
+  typename Four<T>::type out;
   uint32_t top_m = 0, top_v = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    m[k] = decode_m((mw >> (8 * k)) & 255u, em);
-    v[k] = decode_v((vw >> (8 * k)) & 255u, ev);
-    if (em == 255) m[k] = NAN;
-    if (ev == 255) v[k] = NAN;
     m[k] = m[k] * s.beta1 + g[k] * s.omb1;
     v[k] = v[k] * s.beta2 + (g[k] * s.omb2) * g[k];
     const uint32_t am = __float_as_uint(m[k]) & 0x7fffffffu, av = __float_as_uint(v[k]) & 0x7fffffffu;
     top_m = top_m > am ? top_m : am;
     top_v = top_v > av ? top_v : av;
-    // one rounding off for the square root and the reciprocal each (the hardware's approximations, 1 ulp): the update
-    // is right to 2^-21 of itself
+    // one rounding off for the square root and the reciprocal each (the hardware's approximations, 1 ulp): the
+    // update is right to 2^-21 of itself
     const float denom = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[k]), s.inv_bc2, s.eps);
-    p[k] = __builtin_fmaf(s.neg_step, m[k] * __builtin_amdgcn_rcpf(denom), p[k] * s.decay);
-  }
-  const int new_em = static_cast<int>(scale_of(wave_umax(top_m))), new_ev = static_cast<int>(scale_of(wave_umax(top_v)));
-  uint32_t mo = 0, vo = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    mo |= encode_m(m[k], new_em, r[k]) << (8 * k);
-    vo |= encode_v(v[k], new_ev, r[k]) << (8 * k);
-  }
-  // a block with an infinity or NaN: its codes say nothing (but stay bytes)
-  *MC = new_em == 255 ? 0u : mo;
-  *VC = new_ev == 255 ? 0u : vo;
-  if (lane == 0) {
-    *MS = static_cast<unsigned char>(new_em);
-    *VS = static_cast<unsigned char>(new_ev);
-  }
-  T out[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
+    const float y = __builtin_fmaf(s.neg_step, m[k] * __builtin_amdgcn_rcpf(denom), static_cast<float>(p[k]) * s.decay);
     if constexpr (std::is_same<T, __bf16>::value) {
-      out[k] = stochastic ? stochastic_bf16(p[k], r[k]) : static_cast<__bf16>(p[k]);
+      out[k] = stochastic ? stochastic_bf16(y, r[k]) : static_cast<__bf16>(y);
     } else {
-      out[k] = Elem<T>::from_f32(p[k]);
+      out[k] = Elem<T>::from_f32(y);
     }
   }
-  if (whole) {
-    *reinterpret_cast<gptr<T4>>(P) = T4{out[0], out[1], out[2], out[3]};
-  } else {
+  *em = static_cast<int>(scale_of(wave_umax(top_m)));
+  *ev = static_cast<int>(scale_of(wave_umax(top_v)));
+  // a block with an infinity or NaN: its codes say nothing
+  *mw = *em == 255 ? 0u : encode_m(m, *em, r);
+  *vw = *ev == 255 ? 0u : encode_v(v, *ev, r);
+  return out;
+}
+
+// A wave's unit: four blocks of 256 elements, four elements a lane of each.  A whole unit of aligned tensors goes through
+// buffer resources (one base a stream and small offsets), all its loads in flight together; another one block by
+// block, element by element.
+template <typename T, bool RUNS>
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
+                                                          uint32_t units, uint32_t per, Scalars8 by_value,
+                                                          const Scalars8* __restrict__ scalars,
+                                                          const float* __restrict__ grad_scale, int stochastic) {
+  typedef typename Four<T>::type T4;
+  constexpr int E = static_cast<int>(sizeof(T));
+  const Scalars8 s = scalars != nullptr ? *scalars : by_value;
+  const bool scaled = grad_scale != nullptr;
+  const float gs = scaled ? *grad_scale : 1.0f;
+  const int lane = threadIdx.x % 64;
+  walk_units<RUNS>(table, n_tensors, units, per, [&](const Rec8& rec, int64_t unit, uint32_t place) {
+    const int64_t start = unit * kUnitElems, q0 = unit * kBlocks;
+    const int64_t left = rec.n - start;  // elements from here on
+    const gptr<unsigned char> MS = as_global<unsigned char>(rec.ms + q0), VS = as_global<unsigned char>(rec.vs + q0);
+    if (left >= kUnitElems && ((rec.p | rec.g) & (4 * E - 1)) == 0) {
+      const auto pbuf = uniform_buffer(reinterpret_cast<const void*>(rec.p + start * E), kUnitElems * E);
+      const auto gbuf = uniform_buffer(reinterpret_cast<const void*>(rec.g + start * E), kUnitElems * E);
+      const auto mbuf = uniform_buffer(reinterpret_cast<const void*>(rec.mc + start), kUnitElems);
+      const auto vbuf = uniform_buffer(reinterpret_cast<const void*>(rec.vc + start), kUnitElems);
+      // lane k reads and writes block k's scales
+      int scale_m = 0, scale_v = 0;
+      if (lane < kBlocks) {
+        scale_m = MS[lane];
+        scale_v = VS[lane];
+      }
+      T4 p[kBlocks], gv[kBlocks];
+      uint32_t mw[kBlocks], vw[kBlocks];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < left) P[k] = out[k];
-  }
+      for (int b = 0; b < kBlocks; ++b) {
+        mw[b] = __builtin_amdgcn_raw_buffer_load_b32(mbuf, (b * 64 + lane) * 4, 0, kNonTemporal);
+        vw[b] = __builtin_amdgcn_raw_buffer_load_b32(vbuf, (b * 64 + lane) * 4, 0, kNonTemporal);
+        p[b] = Four<T>::load(pbuf, (b * 64 + lane) * 4 * E);
+        gv[b] = Four<T>::load(gbuf, (b * 64 + lane) * 4 * E);
+      }
+      int new_m = 0, new_v = 0;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        float g[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[k] = static_cast<float>(gv[b][k]);
+        if (scaled) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) g[k] = g[k] * gs;
+        }
+        int em = __builtin_amdgcn_readlane(scale_m, b), ev = __builtin_amdgcn_readlane(scale_v, b);
+        const T4 out = update<T>(p[b], g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), stochastic, &mw[b], &vw[b],
+                                 &em, &ev);
+        new_m = lane == b ? em : new_m;
+        new_v = lane == b ? ev : new_v;
+        __builtin_amdgcn_raw_buffer_store_b32(mw[b], mbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
+        __builtin_amdgcn_raw_buffer_store_b32(vw[b], vbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
+        Four<T>::store(out, pbuf, (b * 64 + lane) * 4 * E);
+      }
+      if (lane < kBlocks) {
+        MS[lane] = static_cast<unsigned char>(new_m);
+        VS[lane] = static_cast<unsigned char>(new_v);
+      }
+    } else {
+      const int n = left < kUnitElems ? static_cast<int>(left) : static_cast<int>(kUnitElems);
+#pragma unroll 1
+      for (int b = 0; b * kQuant < n; ++b) {
+        const int i = b * kQuant + lane * 4;
+        const gptr<T> P = as_global<T>(rec.p) + start + i;
+        const gptr<const T> G = as_global<const T>(rec.g) + start + i;
+        const gptr<uint32_t> MC = as_global<uint32_t>(rec.mc + start + i), VC = as_global<uint32_t>(rec.vc + start + i);
+        int em = __builtin_amdgcn_readfirstlane(MS[b]), ev = __builtin_amdgcn_readfirstlane(VS[b]);
+        uint32_t mw = *MC, vw = *VC;  // codes fill their last block
+        T4 p;
+        float g[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool in = i + k < n;
+          p[k] = in ? P[k] : T{};
+          g[k] = in ? static_cast<float>(G[k]) : 0.0f;
+          if (scaled) g[k] = in ? g[k] * gs : 0.0f;  // zero behind the end under an infinite scale too
+        }
+        const T4 out = update<T>(p, g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), stochastic, &mw, &vw, &em, &ev);
+        *MC = mw;
+        *VC = vw;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k < n) P[k] = out[k];
+        if (lane == 0) {
+          MS[b] = static_cast<unsigned char>(em);
+          VS[b] = static_cast<unsigned char>(ev);
+        }
+      }
+    }
+  });
 }
 
 // The moments' values: element i of the table's unit b at out[b * 1024 + i], zeros behind a tensor's end.
-template <typename T>
+template <typename T, bool RUNS>
 __global__ __launch_bounds__(kThreads) void adamw8_moments_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
-                                                                  T* __restrict__ m_out, T* __restrict__ v_out) {
+                                                                  uint32_t units, uint32_t per, T* __restrict__ m_out,
+                                                                  T* __restrict__ v_out) {
   typedef typename Four<T>::type T4;
-  const uint32_t blk = blockIdx.x;
-  const Rec8 rec = table[find_record(table, n_tensors, blk)];
   const int lane = threadIdx.x % 64;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64);
-  const int64_t q = (blk - rec.first_block) * (kUnitElems / kQuant) + wave;
-  const int64_t i = q * kQuant + lane * 4;
-  float m[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (q * kQuant < rec.n) {
-    const int em = __builtin_amdgcn_readfirstlane(*as_global<const unsigned char>(rec.ms + q));
-    const int ev = __builtin_amdgcn_readfirstlane(*as_global<const unsigned char>(rec.vs + q));
-    const uint32_t mw = *as_global<const uint32_t>(rec.mc + i), vw = *as_global<const uint32_t>(rec.vc + i);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool in = i + k < rec.n;
-      m[k] = !in ? 0.0f : (em == 255 ? NAN : decode_m((mw >> (8 * k)) & 255u, em));
-      v[k] = !in ? 0.0f : (ev == 255 ? NAN : decode_v((vw >> (8 * k)) & 255u, ev));
+  walk_units<RUNS>(table, n_tensors, units, per, [&](const Rec8& rec, int64_t unit, uint32_t place) {
+    const int64_t start = unit * kUnitElems;
+    const int64_t left = rec.n - start;
+    const int blocks = left >= kUnitElems ? kBlocks : static_cast<int>((left + kQuant - 1) / kQuant);
+    int scale_m = 0, scale_v = 0;
+    if (lane < blocks) {
+      scale_m = as_global<const unsigned char>(rec.ms + unit * kBlocks)[lane];
+      scale_v = as_global<const unsigned char>(rec.vs + unit * kBlocks)[lane];
     }
-  }
-  const int64_t at = static_cast<int64_t>(blk) * kUnitElems + wave * kQuant + lane * 4;
-  *reinterpret_cast<T4*>(m_out + at) =
-      T4{Elem<T>::from_f32(m[0]), Elem<T>::from_f32(m[1]), Elem<T>::from_f32(m[2]), Elem<T>::from_f32(m[3])};
-  *reinterpret_cast<T4*>(v_out + at) =
-      T4{Elem<T>::from_f32(v[0]), Elem<T>::from_f32(v[1]), Elem<T>::from_f32(v[2]), Elem<T>::from_f32(v[3])};
+    uint32_t mw[kBlocks], vw[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      mw[b] = vw[b] = 0;
+      if (b < blocks) {
+        mw[b] = __builtin_nontemporal_load(as_global<const uint32_t>(rec.mc + start) + b * 64 + lane);
+        vw[b] = __builtin_nontemporal_load(as_global<const uint32_t>(rec.vc + start) + b * 64 + lane);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const int i = b * kQuant + lane * 4;
+      float m[4], v[4];
+      decode_m(mw[b], __builtin_amdgcn_readlane(scale_m, b), m);
+      decode_v(vw[b], __builtin_amdgcn_readlane(scale_v, b), v);
+      T4 mo, vo;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        mo[k] = Elem<T>::from_f32(i + k < left ? m[k] : 0.0f);
+        vo[k] = Elem<T>::from_f32(i + k < left ? v[k] : 0.0f);
+      }
+      const int64_t at = static_cast<int64_t>(place) * kUnitElems + i;
+      __builtin_nontemporal_store(mo, reinterpret_cast<T4*>(m_out + at));
+      __builtin_nontemporal_store(vo, reinterpret_cast<T4*>(v_out + at));
+    }
+  });
+}
+
+// Up to kWaveUnits units a wave has one each; more are split into runs for kRunsPerCu workgroups a CU.
+constexpr int64_t kWaveUnits = int64_t{1} << 15;
+constexpr int kRunsPerCu = 32;
+
+struct Grid8 {
+  unsigned blocks;
+  uint32_t per;
+  bool runs;
+};
+
+Grid8 grid_of(int64_t units) {
+  if (units <= kWaveUnits) return {static_cast<unsigned>((units + kWaves - 1) / kWaves), 0, false};
+  const int64_t most = static_cast<int64_t>(num_cus()) * kRunsPerCu;
+  const int64_t per = (units + most - 1) / most;
+  return {static_cast<unsigned>((units + per - 1) / per), static_cast<uint32_t>(per), true};
 }
 
 int check_table8(const char* fn, const int64_t* table, int64_t n_tensors, int64_t total_blocks) {
@@ -365,17 +494,18 @@ int pt_adamw8_step(const int64_t* table, int64_t n_tensors, int64_t total_blocks
   } else {
     s = scalars_of(lr, beta1, beta2, eps, weight_decay, step, seed);
   }
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(total_blocks)), dim3(kThreads), 0, st,
-                       reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors), s, on_device, grad_scale,
-                       stochastic_params);
+  const Grid8 grid = grid_of(total_blocks);
+  const auto go = [&](auto waves, auto runs) {
+    hipLaunchKernelGGL(grid.runs ? runs : waves, dim3(grid.blocks), dim3(kThreads), 0, st,
+                       reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors),
+                       static_cast<uint32_t>(total_blocks), grid.per, s, on_device, grad_scale, stochastic_params);
   };
   if (dtype == PT_FLOAT32) {
-    go(adamw8_kernel<float>);
+    go(adamw8_kernel<float, false>, adamw8_kernel<float, true>);
   } else if (dtype == PT_FLOAT16) {
-    go(adamw8_kernel<_Float16>);
+    go(adamw8_kernel<_Float16, false>, adamw8_kernel<_Float16, true>);
   } else {
-    go(adamw8_kernel<__bf16>);
+    go(adamw8_kernel<__bf16, false>, adamw8_kernel<__bf16, true>);
   }
   return check_launch(fn);
 }
@@ -389,18 +519,20 @@ int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blo
   if (rc != PT_OK) return rc;
   if (!exp_avg || !exp_avg_sq || !aligned16(exp_avg) || !aligned16(exp_avg_sq))
     return fail(PT_EINVAL, "pt_adamw8_moments: null or misaligned output");
-  const auto go = [&](auto kernel, auto* type) {
+  const Grid8 grid = grid_of(total_blocks);
+  const auto go = [&](auto waves, auto runs, auto* type) {
     typedef std::remove_pointer_t<decltype(type)> T;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(total_blocks)), dim3(kThreads), 0, as_stream(stream),
+    hipLaunchKernelGGL(grid.runs ? runs : waves, dim3(grid.blocks), dim3(kThreads), 0, as_stream(stream),
                        reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors),
-                       static_cast<T*>(exp_avg), static_cast<T*>(exp_avg_sq));
+                       static_cast<uint32_t>(total_blocks), grid.per, static_cast<T*>(exp_avg),
+                       static_cast<T*>(exp_avg_sq));
   };
   if (dtype == PT_FLOAT32) {
-    go(adamw8_moments_kernel<float>, static_cast<float*>(nullptr));
+    go(adamw8_moments_kernel<float, false>, adamw8_moments_kernel<float, true>, static_cast<float*>(nullptr));
   } else if (dtype == PT_FLOAT16) {
-    go(adamw8_moments_kernel<_Float16>, static_cast<_Float16*>(nullptr));
+    go(adamw8_moments_kernel<_Float16, false>, adamw8_moments_kernel<_Float16, true>, static_cast<_Float16*>(nullptr));
   } else {
-    go(adamw8_moments_kernel<__bf16>, static_cast<__bf16*>(nullptr));
+    go(adamw8_moments_kernel<__bf16, false>, adamw8_moments_kernel<__bf16, true>, static_cast<__bf16*>(nullptr));
   }
   return check_launch(fn);
 }
