@@ -115,24 +115,22 @@ __device__ __forceinline__ uint32_t find_record(const Rec8* __restrict__ table, 
   return lo;
 }
 
-// Largest of a wave's values (bits of non-negative floats order as integers, NaN above infinity).
+// Largest of a wave's values (bits of non-negative floats order as integers, NaN above infinity): within rows of 16
+// lanes, then row 0's and 2's last lane to the next row's, and row 1's to the upper half, which leaves it in lane 63.
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-  const auto step = [&](auto ctrl) {
-    const uint32_t o = static_cast<uint32_t>(
-        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, false));
+  const auto step = [&](auto ctrl, auto rows) {
+    const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+        0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));  // 0 where nothing comes
     v = v > o ? v : o;
   };
-  step(std::integral_constant<int, dpp::kQuadSwap1>{});
-  step(std::integral_constant<int, dpp::kQuadSwap2>{});
-  step(std::integral_constant<int, dpp::kRowHalfMirror>{});
-  step(std::integral_constant<int, dpp::kRowMirror>{});
-  uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 0));
-#pragma unroll
-  for (int l = 16; l < 64; l += 16) {
-    const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
-    m = m > o ? m : o;
-  }
-  return m;
+  constexpr std::integral_constant<int, 0xf> all{};
+  step(std::integral_constant<int, dpp::kQuadSwap1>{}, all);
+  step(std::integral_constant<int, dpp::kQuadSwap2>{}, all);
+  step(std::integral_constant<int, dpp::kRowHalfMirror>{}, all);
+  step(std::integral_constant<int, dpp::kRowMirror>{}, all);
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
 __device__ __forceinline__ uint32_t scale_of(uint32_t bits) {
@@ -149,8 +147,7 @@ __device__ __forceinline__ float factor_m(int e) {  // what a first-moment code 
   return e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(e - 134 + 127) << 23);
 }
 
-__device__ __forceinline__ void decode_m(uint32_t word, int e, float (&m)[4]) {
-  const float f = factor_m(e);
+__device__ __forceinline__ void decode_m(uint32_t word, float f, float (&m)[4]) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word), false);
   const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word), true);
   m[0] = lo[0] * f;
@@ -159,15 +156,15 @@ __device__ __forceinline__ void decode_m(uint32_t word, int e, float (&m)[4]) {
   m[3] = hi[1] * f;
 }
 
+// (A block with scale 255 reads as NaN: the callers see to it.)
 __device__ __forceinline__ void decode_v(uint32_t word, int e, float (&v)[4]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     v[k] = __builtin_amdgcn_ldexpf(__uint_as_float(((word >> (8 * k)) & 255u) << 20), e - kTopV);
-  if (e == 255) v[0] = v[1] = v[2] = v[3] = NAN;
 }
 
 __device__ __forceinline__ uint32_t encode_m(const float (&m)[4], int e, const uint32_t (&r)[4]) {
-  const float f = __uint_as_float(static_cast<uint32_t>(134 - e + 127) << 23);
+  const float f = __uint_as_float(static_cast<uint32_t>(134 - e + 127) << 23);  // 2^(134 - e), e up to 255
   int w = 0;
   w = __builtin_amdgcn_cvt_sr_fp8_f32(m[0] * f, static_cast<int>(r[0]), w, 0);
   w = __builtin_amdgcn_cvt_sr_fp8_f32(m[1] * f, static_cast<int>(r[1]), w, 1);
@@ -182,7 +179,8 @@ __device__ __forceinline__ uint32_t encode_v(const float (&v)[4], int e, const u
   for (int k = 0; k < 4; ++k) {
     const uint32_t y = __float_as_uint(__builtin_amdgcn_ldexpf(v[k], kTopV - e));
     const uint32_t code = (y + (__builtin_rotateleft32(r[k], 4) & 0xFFFFFu)) >> 20;
-    const uint32_t least = __float_as_uint(v[k]) < 1u ? __float_as_uint(v[k]) : 1u;  // 1 for any positive value
+    uint32_t least;  // 1 for any positive value (written out: the compiler makes two instructions of this minimum)
+    asm("v_min_u32 %0, 1, %1" : "=v"(least) : "v"(__float_as_uint(v[k])));
     w |= (code > least ? code : least) << (8 * k);
   }
   return w;
@@ -213,11 +211,25 @@ struct Four<float> {
   }
 };
 
-// x in bf16, rounded by 16 random bits; infinities and NaN as they are.
-__device__ __forceinline__ __bf16 stochastic_bf16(float x, uint32_t r) {
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7f800000u) == 0x7f800000u) return static_cast<__bf16>(x);
-  return static_cast<__bf16>(__uint_as_float((u + ((r >> 8) & 0xffffu)) & 0xffff0000u));
+// x[k] in T: to nearest, or (STOCHASTIC, bf16) by 16 random bits below the last kept one, bits 23-8 of r[k].  The sum
+// leaves infinities and NaN what they are: their lower 16 bits are zero here (a bf16 value's, or an operation's own NaN).
+template <typename T, bool STOCHASTIC>
+__device__ __forceinline__ typename Four<T>::type rounded(const float (&x)[4], const uint32_t (&r)[4]) {
+  typename Four<T>::type out;
+  if constexpr (STOCHASTIC) {
+    u32x2 w;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t lo = __float_as_uint(x[2 * k]) + ((r[2 * k] >> 8) & 0xffffu);
+      const uint32_t hi = __float_as_uint(x[2 * k + 1]) + ((r[2 * k + 1] >> 8) & 0xffffu);
+      w[k] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);  // the upper halves
+    }
+    out = __builtin_bit_cast(typename Four<T>::type, w);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = Elem<T>::from_f32(x[k]);
+  }
+  return out;
 }
 
 // Calls f(record, unit of its tensor, unit of the table) for each unit of the wave.  RUNS: workgroup b takes the units
@@ -248,10 +260,9 @@ __device__ __forceinline__ void walk_units(const Rec8* __restrict__ table, uint3
 
 // One block's four elements of a lane: the parameters p and gradients g in, the new parameters out; the codes and the
 // scales replaced.  `place`: the first element's place in the call, over 4.
-template <typename T>
+template <typename T, bool STOCHASTIC>
 __device__ __forceinline__ typename Four<T>::type update(typename Four<T>::type p, const float (&g)[4], const Scalars8& s,
-                                                         uint32_t place, int stochastic, uint32_t* mw, uint32_t* vw,
-                                                         int* em, int* ev) {
+                                                         uint32_t place, uint32_t* mw, uint32_t* vw, int* em, int* ev) {
 #pragma clang fp contract(off)
   uint32_t r[4];
   uint32_t x = place * 0x9E3779B1u + s.seed;
@@ -264,49 +275,45 @@ __device__ __forceinline__ typename Four<T>::type update(typename Four<T>::type 
     x ^= x << 5;
     r[k] = x;
   }
-  float m[4], v[4];
-  decode_m(*mw, *em, m);
+  float m[4], v[4], y[4];
+  // the codes' factor times beta1 is exact, and so the product with either in turn the same
+  decode_m(*mw, factor_m(*em) * s.beta1, m);
   decode_v(*vw, *ev, v);
-  typename Four<T>::type out;
+  const float beta2 = *ev == 255 ? NAN : s.beta2;
   uint32_t top_m = 0, top_v = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    m[k] = m[k] * s.beta1 + g[k] * s.omb1;
-    v[k] = v[k] * s.beta2 + (g[k] * s.omb2) * g[k];
-    const uint32_t am = __float_as_uint(m[k]) & 0x7fffffffu, av = __float_as_uint(v[k]) & 0x7fffffffu;
+    m[k] = m[k] + g[k] * s.omb1;
+    v[k] = v[k] * beta2 + (g[k] * s.omb2) * g[k];
+    const uint32_t am = __float_as_uint(m[k]) & 0x7fffffffu, av = __float_as_uint(v[k]);  // no sign but a NaN's
     top_m = top_m > am ? top_m : am;
     top_v = top_v > av ? top_v : av;
     // one rounding off for the square root and the reciprocal each (the hardware's approximations, 1 ulp): the
     // update is right to 2^-21 of itself
     const float denom = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[k]), s.inv_bc2, s.eps);
-    const float y = __builtin_fmaf(s.neg_step, m[k] * __builtin_amdgcn_rcpf(denom), static_cast<float>(p[k]) * s.decay);
-    if constexpr (std::is_same<T, __bf16>::value) {
-      out[k] = stochastic ? stochastic_bf16(y, r[k]) : static_cast<__bf16>(y);
-    } else {
-      out[k] = Elem<T>::from_f32(y);
-    }
+    y[k] = __builtin_fmaf(s.neg_step, m[k] * __builtin_amdgcn_rcpf(denom), static_cast<float>(p[k]) * s.decay);
   }
   *em = static_cast<int>(scale_of(wave_umax(top_m)));
-  *ev = static_cast<int>(scale_of(wave_umax(top_v)));
+  *ev = static_cast<int>(scale_of(wave_umax(top_v) & 0x7fffffffu));
   // a block with an infinity or NaN: its codes say nothing
-  *mw = *em == 255 ? 0u : encode_m(m, *em, r);
-  *vw = *ev == 255 ? 0u : encode_v(v, *ev, r);
-  return out;
+  const uint32_t mo = encode_m(m, *em, r), vo = encode_v(v, *ev, r);
+  *mw = *em == 255 ? 0u : mo;
+  *vw = *ev == 255 ? 0u : vo;
+  return rounded<T, STOCHASTIC>(y, r);
 }
 
 // A wave's unit: four blocks of 256 elements, four elements a lane of each.  A whole unit of aligned tensors goes through
 // buffer resources (one base a stream and small offsets), all its loads in flight together; another one block by
 // block, element by element.
-template <typename T, bool RUNS>
+template <typename T, bool STOCHASTIC, bool SCALED, bool RUNS>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
                                                           uint32_t units, uint32_t per, Scalars8 by_value,
                                                           const Scalars8* __restrict__ scalars,
-                                                          const float* __restrict__ grad_scale, int stochastic) {
+                                                          const float* __restrict__ grad_scale) {
   typedef typename Four<T>::type T4;
   constexpr int E = static_cast<int>(sizeof(T));
   const Scalars8 s = scalars != nullptr ? *scalars : by_value;
-  const bool scaled = grad_scale != nullptr;
-  const float gs = scaled ? *grad_scale : 1.0f;
+  const float gs = SCALED ? *grad_scale : 1.0f;
   const int lane = threadIdx.x % 64;
   walk_units<RUNS>(table, n_tensors, units, per, [&](const Rec8& rec, int64_t unit, uint32_t place) {
     const int64_t start = unit * kUnitElems, q0 = unit * kBlocks;
@@ -338,13 +345,13 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict
         float g[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[k] = static_cast<float>(gv[b][k]);
-        if (scaled) {
+        if constexpr (SCALED) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) g[k] = g[k] * gs;
         }
         int em = __builtin_amdgcn_readlane(scale_m, b), ev = __builtin_amdgcn_readlane(scale_v, b);
-        const T4 out = update<T>(p[b], g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), stochastic, &mw[b], &vw[b],
-                                 &em, &ev);
+        const T4 out = update<T, STOCHASTIC>(p[b], g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), &mw[b], &vw[b],
+                                             &em, &ev);
         new_m = lane == b ? em : new_m;
         new_v = lane == b ? ev : new_v;
         __builtin_amdgcn_raw_buffer_store_b32(mw[b], mbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
@@ -372,9 +379,9 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict
           const bool in = i + k < n;
           p[k] = in ? P[k] : T{};
           g[k] = in ? static_cast<float>(G[k]) : 0.0f;
-          if (scaled) g[k] = in ? g[k] * gs : 0.0f;  // zero behind the end under an infinite scale too
+          if (SCALED) g[k] = in ? g[k] * gs : 0.0f;  // zero behind the end under an infinite scale too
         }
-        const T4 out = update<T>(p, g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), stochastic, &mw, &vw, &em, &ev);
+        const T4 out = update<T, STOCHASTIC>(p, g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), &mw, &vw, &em, &ev);
         *MC = mw;
         *VC = vw;
 #pragma unroll
@@ -418,13 +425,15 @@ __global__ __launch_bounds__(kThreads) void adamw8_moments_kernel(const Rec8* __
     for (int b = 0; b < kBlocks; ++b) {
       const int i = b * kQuant + lane * 4;
       float m[4], v[4];
-      decode_m(mw[b], __builtin_amdgcn_readlane(scale_m, b), m);
-      decode_v(vw[b], __builtin_amdgcn_readlane(scale_v, b), v);
+      const int ev = __builtin_amdgcn_readlane(scale_v, b);
+      decode_m(mw[b], factor_m(__builtin_amdgcn_readlane(scale_m, b)), m);
+      decode_v(vw[b], ev, v);
+      const float whole = ev == 255 ? NAN : 1.0f;
       T4 mo, vo;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         mo[k] = Elem<T>::from_f32(i + k < left ? m[k] : 0.0f);
-        vo[k] = Elem<T>::from_f32(i + k < left ? v[k] : 0.0f);
+        vo[k] = Elem<T>::from_f32(i + k < left ? v[k] * whole : 0.0f);
       }
       const int64_t at = static_cast<int64_t>(place) * kUnitElems + i;
       __builtin_nontemporal_store(mo, reinterpret_cast<T4*>(m_out + at));
@@ -498,15 +507,24 @@ int pt_adamw8_step(const int64_t* table, int64_t n_tensors, int64_t total_blocks
   const auto go = [&](auto waves, auto runs) {
     hipLaunchKernelGGL(grid.runs ? runs : waves, dim3(grid.blocks), dim3(kThreads), 0, st,
                        reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors),
-                       static_cast<uint32_t>(total_blocks), grid.per, s, on_device, grad_scale, stochastic_params);
+                       static_cast<uint32_t>(total_blocks), grid.per, s, on_device, grad_scale);
   };
-  if (dtype == PT_FLOAT32) {
-    go(adamw8_kernel<float, false>, adamw8_kernel<float, true>);
-  } else if (dtype == PT_FLOAT16) {
-    go(adamw8_kernel<_Float16, false>, adamw8_kernel<_Float16, true>);
-  } else {
-    go(adamw8_kernel<__bf16, false>, adamw8_kernel<__bf16, true>);
+#define PT_ADAMW8(T, STOCHASTIC)                                                              \
+  if (grad_scale) {                                                                           \
+    go(adamw8_kernel<T, STOCHASTIC, true, false>, adamw8_kernel<T, STOCHASTIC, true, true>);   \
+  } else {                                                                                    \
+    go(adamw8_kernel<T, STOCHASTIC, false, false>, adamw8_kernel<T, STOCHASTIC, false, true>); \
   }
+  if (dtype == PT_FLOAT32) {
+    PT_ADAMW8(float, false)
+  } else if (dtype == PT_FLOAT16) {
+    PT_ADAMW8(_Float16, false)
+  } else if (stochastic_params) {
+    PT_ADAMW8(__bf16, true)
+  } else {
+    PT_ADAMW8(__bf16, false)
+  }
+#undef PT_ADAMW8
   return check_launch(fn);
 }
 
