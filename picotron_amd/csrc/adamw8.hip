@@ -141,8 +141,8 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t bits) {
 // Reading and writing codes.  A first-moment code is the hardware's 8-bit float (4 exponent bits, bias 7) in its own
 // right, its block's factor 2^(E - 134): the conversions, stochastic rounding with the top 20 of 32 random bits
 // among them, are one instruction each and give the bits of the integer form in the file's comment (checked over 10^6
-// values of both signs, subnormals and zeros among them).  They took the step of 1.04e9 bf16 elements from XX to YY us.
-// The second moment's format is no hardware one.
+// values of both signs, subnormals and zeros among them): 50 vector operations an element in all instead of 62.  The second
+// moment's format is no hardware one.
 __device__ __forceinline__ float factor_m(int e) {  // what a first-moment code of a block with scale e is multiplied by
   return e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(e - 134 + 127) << 23);
 }
@@ -232,30 +232,19 @@ __device__ __forceinline__ typename Four<T>::type rounded(const float (&x)[4], c
   return out;
 }
 
-// Calls f(record, unit of its tensor, unit of the table) for each unit of the wave.  RUNS: workgroup b takes the units
-// [b * per, (b + 1) * per), a run of each tensor they lie in, its four waves in turn, so that the table is
-// searched once a workgroup; else every wave has the unit of its number.
-template <bool RUNS, typename F>
-__device__ __forceinline__ void walk_units(const Rec8* __restrict__ table, uint32_t n_tensors, uint32_t units,
-                                           uint32_t per, const F& f) {
-  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
-  if constexpr (!RUNS) {
-    const uint32_t u = blockIdx.x * kWaves + wave;
-    if (u >= units) return;
-    const Rec8 rec = table[find_record(table, n_tensors, u)];
-    f(rec, u - rec.first_block, u);
-  } else {
-    uint32_t at = blockIdx.x * per;
-    const uint32_t end = at + per < units ? at + per : units;
-    if (at >= end) return;
-    for (uint32_t row = find_record(table, n_tensors, at); at < end; ++row) {
-      const Rec8 rec = table[row];
-      const uint32_t next = row + 1 < n_tensors ? static_cast<uint32_t>(table[row + 1].first_block) : end;
-      const uint32_t stop = next < end ? next : end;
-      for (uint32_t u = at + wave; u < stop; u += kWaves) f(rec, u - rec.first_block, u);
-      at = stop;
-    }
-  }
+// The unit of this wave, its record and its number in the tensor; false behind the last one.
+struct Unit {
+  Rec8 rec;
+  int64_t index;
+  uint32_t place;  // in the table
+};
+
+__device__ __forceinline__ bool unit_of_wave(const Rec8* __restrict__ table, uint32_t n_tensors, uint32_t units, Unit* w) {
+  w->place = blockIdx.x * kWaves + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
+  if (w->place >= units) return false;
+  w->rec = table[find_record(table, n_tensors, w->place)];
+  w->index = w->place - w->rec.first_block;
+  return true;
 }
 
 // One block's four elements of a lane: the parameters p and gradients g in, the new parameters out; the codes and the
@@ -305,9 +294,9 @@ __device__ __forceinline__ typename Four<T>::type update(typename Four<T>::type 
 // A wave's unit: four blocks of 256 elements, four elements a lane of each.  A whole unit of aligned tensors goes through
 // buffer resources (one base a stream and small offsets), all its loads in flight together; another one block by
 // block, element by element.
-template <typename T, bool STOCHASTIC, bool SCALED, bool RUNS>
+template <typename T, bool STOCHASTIC, bool SCALED>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
-                                                          uint32_t units, uint32_t per, Scalars8 by_value,
+                                                          uint32_t units, Scalars8 by_value,
                                                           const Scalars8* __restrict__ scalars,
                                                           const float* __restrict__ grad_scale) {
   typedef typename Four<T>::type T4;
@@ -315,148 +304,154 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Rec8* __restrict
   const Scalars8 s = scalars != nullptr ? *scalars : by_value;
   const float gs = SCALED ? *grad_scale : 1.0f;
   const int lane = threadIdx.x % 64;
-  walk_units<RUNS>(table, n_tensors, units, per, [&](const Rec8& rec, int64_t unit, uint32_t place) {
-    const int64_t start = unit * kUnitElems, q0 = unit * kBlocks;
-    const int64_t left = rec.n - start;  // elements from here on
-    const gptr<unsigned char> MS = as_global<unsigned char>(rec.ms + q0), VS = as_global<unsigned char>(rec.vs + q0);
-    if (left >= kUnitElems && ((rec.p | rec.g) & (4 * E - 1)) == 0) {
-      const auto pbuf = uniform_buffer(reinterpret_cast<const void*>(rec.p + start * E), kUnitElems * E);
-      const auto gbuf = uniform_buffer(reinterpret_cast<const void*>(rec.g + start * E), kUnitElems * E);
-      const auto mbuf = uniform_buffer(reinterpret_cast<const void*>(rec.mc + start), kUnitElems);
-      const auto vbuf = uniform_buffer(reinterpret_cast<const void*>(rec.vc + start), kUnitElems);
-      // lane k reads and writes block k's scales
-      int scale_m = 0, scale_v = 0;
-      if (lane < kBlocks) {
-        scale_m = MS[lane];
-        scale_v = VS[lane];
-      }
-      T4 p[kBlocks], gv[kBlocks];
-      uint32_t mw[kBlocks], vw[kBlocks];
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        mw[b] = __builtin_amdgcn_raw_buffer_load_b32(mbuf, (b * 64 + lane) * 4, 0, kNonTemporal);
-        vw[b] = __builtin_amdgcn_raw_buffer_load_b32(vbuf, (b * 64 + lane) * 4, 0, kNonTemporal);
-        p[b] = Four<T>::load(pbuf, (b * 64 + lane) * 4 * E);
-        gv[b] = Four<T>::load(gbuf, (b * 64 + lane) * 4 * E);
-      }
-      int new_m = 0, new_v = 0;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        float g[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) g[k] = static_cast<float>(gv[b][k]);
-        if constexpr (SCALED) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) g[k] = g[k] * gs;
-        }
-        int em = __builtin_amdgcn_readlane(scale_m, b), ev = __builtin_amdgcn_readlane(scale_v, b);
-        const T4 out = update<T, STOCHASTIC>(p[b], g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), &mw[b], &vw[b],
-                                             &em, &ev);
-        new_m = lane == b ? em : new_m;
-        new_v = lane == b ? ev : new_v;
-        __builtin_amdgcn_raw_buffer_store_b32(mw[b], mbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
-        __builtin_amdgcn_raw_buffer_store_b32(vw[b], vbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
-        Four<T>::store(out, pbuf, (b * 64 + lane) * 4 * E);
-      }
-      if (lane < kBlocks) {
-        MS[lane] = static_cast<unsigned char>(new_m);
-        VS[lane] = static_cast<unsigned char>(new_v);
-      }
-    } else {
-      const int n = left < kUnitElems ? static_cast<int>(left) : static_cast<int>(kUnitElems);
-#pragma unroll 1
-      for (int b = 0; b * kQuant < n; ++b) {
-        const int i = b * kQuant + lane * 4;
-        const gptr<T> P = as_global<T>(rec.p) + start + i;
-        const gptr<const T> G = as_global<const T>(rec.g) + start + i;
-        const gptr<uint32_t> MC = as_global<uint32_t>(rec.mc + start + i), VC = as_global<uint32_t>(rec.vc + start + i);
-        int em = __builtin_amdgcn_readfirstlane(MS[b]), ev = __builtin_amdgcn_readfirstlane(VS[b]);
-        uint32_t mw = *MC, vw = *VC;  // codes fill their last block
-        T4 p;
-        float g[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool in = i + k < n;
-          p[k] = in ? P[k] : T{};
-          g[k] = in ? static_cast<float>(G[k]) : 0.0f;
-          if (SCALED) g[k] = in ? g[k] * gs : 0.0f;  // zero behind the end under an infinite scale too
-        }
-        const T4 out = update<T, STOCHASTIC>(p, g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), &mw, &vw, &em, &ev);
-        *MC = mw;
-        *VC = vw;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (i + k < n) P[k] = out[k];
-        if (lane == 0) {
-          MS[b] = static_cast<unsigned char>(em);
-          VS[b] = static_cast<unsigned char>(ev);
-        }
-      }
-    }
-  });
-}
-
-// The moments' values: element i of the table's unit b at out[b * 1024 + i], zeros behind a tensor's end.
-template <typename T, bool RUNS>
-__global__ __launch_bounds__(kThreads) void adamw8_moments_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
-                                                                  uint32_t units, uint32_t per, T* __restrict__ m_out,
-                                                                  T* __restrict__ v_out) {
-  typedef typename Four<T>::type T4;
-  const int lane = threadIdx.x % 64;
-  walk_units<RUNS>(table, n_tensors, units, per, [&](const Rec8& rec, int64_t unit, uint32_t place) {
-    const int64_t start = unit * kUnitElems;
-    const int64_t left = rec.n - start;
-    const int blocks = left >= kUnitElems ? kBlocks : static_cast<int>((left + kQuant - 1) / kQuant);
+  Unit w;
+  if (!unit_of_wave(table, n_tensors, units, &w)) return;
+  const Rec8& rec = w.rec;
+  const uint32_t place = w.place;
+  const int64_t start = w.index * kUnitElems, q0 = w.index * kBlocks;
+  const int64_t left = rec.n - start;  // elements from here on
+  const gptr<unsigned char> MS = as_global<unsigned char>(rec.ms + q0), VS = as_global<unsigned char>(rec.vs + q0);
+  if (left >= kUnitElems && ((rec.p | rec.g) & (4 * E - 1)) == 0) {
+    const auto pbuf = uniform_buffer(reinterpret_cast<const void*>(rec.p + start * E), kUnitElems * E);
+    const auto gbuf = uniform_buffer(reinterpret_cast<const void*>(rec.g + start * E), kUnitElems * E);
+    const auto mbuf = uniform_buffer(reinterpret_cast<const void*>(rec.mc + start), kUnitElems);
+    const auto vbuf = uniform_buffer(reinterpret_cast<const void*>(rec.vc + start), kUnitElems);
+    // lane k reads and writes block k's scales
     int scale_m = 0, scale_v = 0;
-    if (lane < blocks) {
-      scale_m = as_global<const unsigned char>(rec.ms + unit * kBlocks)[lane];
-      scale_v = as_global<const unsigned char>(rec.vs + unit * kBlocks)[lane];
+    if (lane < kBlocks) {
+      scale_m = MS[lane];
+      scale_v = VS[lane];
     }
+    T4 p[kBlocks], gv[kBlocks];
     uint32_t mw[kBlocks], vw[kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
-      mw[b] = vw[b] = 0;
-      if (b < blocks) {
-        mw[b] = __builtin_nontemporal_load(as_global<const uint32_t>(rec.mc + start) + b * 64 + lane);
-        vw[b] = __builtin_nontemporal_load(as_global<const uint32_t>(rec.vc + start) + b * 64 + lane);
-      }
+      mw[b] = __builtin_amdgcn_raw_buffer_load_b32(mbuf, (b * 64 + lane) * 4, 0, kNonTemporal);
+      vw[b] = __builtin_amdgcn_raw_buffer_load_b32(vbuf, (b * 64 + lane) * 4, 0, kNonTemporal);
+      p[b] = Four<T>::load(pbuf, (b * 64 + lane) * 4 * E);
+      gv[b] = Four<T>::load(gbuf, (b * 64 + lane) * 4 * E);
     }
+    int new_m = 0, new_v = 0;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
+      float g[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g[k] = static_cast<float>(gv[b][k]);
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[k] = g[k] * gs;
+      }
+      int em = __builtin_amdgcn_readlane(scale_m, b), ev = __builtin_amdgcn_readlane(scale_v, b);
+      const T4 out = update<T, STOCHASTIC>(p[b], g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), &mw[b], &vw[b],
+                                           &em, &ev);
+      new_m = lane == b ? em : new_m;
+      new_v = lane == b ? ev : new_v;
+      __builtin_amdgcn_raw_buffer_store_b32(mw[b], mbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
+      __builtin_amdgcn_raw_buffer_store_b32(vw[b], vbuf, (b * 64 + lane) * 4, 0, kWriteThrough);
+      Four<T>::store(out, pbuf, (b * 64 + lane) * 4 * E);
+    }
+    if (lane < kBlocks) {
+      MS[lane] = static_cast<unsigned char>(new_m);
+      VS[lane] = static_cast<unsigned char>(new_v);
+    }
+  } else {
+    const int n = left < kUnitElems ? static_cast<int>(left) : static_cast<int>(kUnitElems);
+#pragma unroll 1
+    for (int b = 0; b * kQuant < n; ++b) {
       const int i = b * kQuant + lane * 4;
-      float m[4], v[4];
-      const int ev = __builtin_amdgcn_readlane(scale_v, b);
-      decode_m(mw[b], factor_m(__builtin_amdgcn_readlane(scale_m, b)), m);
-      decode_v(vw[b], ev, v);
-      const float whole = ev == 255 ? NAN : 1.0f;
-      T4 mo, vo;
+      const gptr<T> P = as_global<T>(rec.p) + start + i;
+      const gptr<const T> G = as_global<const T>(rec.g) + start + i;
+      const gptr<uint32_t> MC = as_global<uint32_t>(rec.mc + start + i), VC = as_global<uint32_t>(rec.vc + start + i);
+      int em = __builtin_amdgcn_readfirstlane(MS[b]), ev = __builtin_amdgcn_readfirstlane(VS[b]);
+      uint32_t mw = *MC, vw = *VC;  // codes fill their last block
+      T4 p;
+      float g[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        mo[k] = Elem<T>::from_f32(i + k < left ? m[k] : 0.0f);
-        vo[k] = Elem<T>::from_f32(i + k < left ? v[k] * whole : 0.0f);
+        const bool in = i + k < n;
+        p[k] = in ? P[k] : T{};
+        g[k] = in ? static_cast<float>(G[k]) : 0.0f;
+        if (SCALED) g[k] = in ? g[k] * gs : 0.0f;  // zero behind the end under an infinite scale too
       }
-      const int64_t at = static_cast<int64_t>(place) * kUnitElems + i;
-      __builtin_nontemporal_store(mo, reinterpret_cast<T4*>(m_out + at));
-      __builtin_nontemporal_store(vo, reinterpret_cast<T4*>(v_out + at));
+      const T4 out = update<T, STOCHASTIC>(p, g, s, place * 256u + static_cast<uint32_t>(b * 64 + lane), &mw, &vw, &em, &ev);
+      *MC = mw;
+      *VC = vw;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) P[k] = out[k];
+      if (lane == 0) {
+        MS[b] = static_cast<unsigned char>(em);
+        VS[b] = static_cast<unsigned char>(ev);
+      }
     }
-  });
+  }
 }
 
-// Up to kWaveUnits units a wave has one each; more are split into runs for kRunsPerCu workgroups a CU.
-constexpr int64_t kWaveUnits = int64_t{1} << 15;
-constexpr int kRunsPerCu = 32;
+// The moments' values: element i of the table's unit b at out[b * 1024 + i], zeros behind a tensor's end.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void adamw8_moments_kernel(const Rec8* __restrict__ table, uint32_t n_tensors,
+                                                                  uint32_t units, T* __restrict__ m_out,
+                                                                  T* __restrict__ v_out) {
+  typedef typename Four<T>::type T4;
+  const int lane = threadIdx.x % 64;
+  Unit w;
+  if (!unit_of_wave(table, n_tensors, units, &w)) return;
+  const Rec8& rec = w.rec;
+  const int64_t unit = w.index;
+  const uint32_t place = w.place;
+  const int64_t start = unit * kUnitElems;
+  const int64_t left = rec.n - start;
+  const int blocks = left >= kUnitElems ? kBlocks : static_cast<int>((left + kQuant - 1) / kQuant);
+  int scale_m = 0, scale_v = 0;
+  if (lane < blocks) {
+    scale_m = as_global<const unsigned char>(rec.ms + unit * kBlocks)[lane];
+    scale_v = as_global<const unsigned char>(rec.vs + unit * kBlocks)[lane];
+  }
+  uint32_t mw[kBlocks], vw[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    mw[b] = vw[b] = 0;
+    if (b < blocks) {
+      mw[b] = __builtin_nontemporal_load(as_global<const uint32_t>(rec.mc + start) + b * 64 + lane);
+      vw[b] = __builtin_nontemporal_load(as_global<const uint32_t>(rec.vc + start) + b * 64 + lane);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const int i = b * kQuant + lane * 4;
+    float m[4], v[4];
+    const int ev = __builtin_amdgcn_readlane(scale_v, b);
+    decode_m(mw[b], factor_m(__builtin_amdgcn_readlane(scale_m, b)), m);
+    decode_v(vw[b], ev, v);
+    const float whole = ev == 255 ? NAN : 1.0f;
+    T4 mo, vo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      mo[k] = Elem<T>::from_f32(i + k < left ? m[k] : 0.0f);
+      vo[k] = Elem<T>::from_f32(i + k < left ? v[k] * whole : 0.0f);
+    }
+    const int64_t at = static_cast<int64_t>(place) * kUnitElems + i;
+    __builtin_nontemporal_store(mo, reinterpret_cast<T4*>(m_out + at));
+    __builtin_nontemporal_store(vo, reinterpret_cast<T4*>(v_out + at));
+  }
+}
 
-struct Grid8 {
-  unsigned blocks;
-  uint32_t per;
-  bool runs;
-};
+// Resident workgroups per CU.  Each wave reads and writes four streams of one unit; a one-shot grid with few workgroups
+// a CU keeps them in one compact window of each.  1.04e9 bf16 parameters, step / moments, us: 2 a CU 2250 / 1493, 3 1907 /
+// 1125, 4 1805 / 1019, 5 1787 / 984, no limit 1845 / 1079; with workgroups that each walk a run of units (one search
+// of the table a run) 2077 / 1247 with 32 runs a CU, 1932 / 1163 with 256.  1.4e8 fp32 parameters, step: 380, 362, 364, 369,
+// 375, runs 431.
+constexpr int kPerCu = 5;
 
-Grid8 grid_of(int64_t units) {
-  if (units <= kWaveUnits) return {static_cast<unsigned>((units + kWaves - 1) / kWaves), 0, false};
-  const int64_t most = static_cast<int64_t>(num_cus()) * kRunsPerCu;
-  const int64_t per = (units + most - 1) / most;
-  return {static_cast<unsigned>((units + per - 1) / per), static_cast<uint32_t>(per), true};
+template <typename K, typename... Args>
+int launch_units(const char* fn, K kernel, int64_t units, hipStream_t st, const int64_t* table, int64_t n_tensors,
+                 Args... args) {
+  size_t lds = occupancy_lds(kPerCu, 0);
+  if (allow_dynamic_lds(reinterpret_cast<const void*>(kernel), lds) != PT_OK) lds = 0;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((units + kWaves - 1) / kWaves)), dim3(kThreads), lds, st,
+                     reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors), static_cast<uint32_t>(units),
+                     args...);
+  return check_launch(fn);
 }
 
 int check_table8(const char* fn, const int64_t* table, int64_t n_tensors, int64_t total_blocks) {
@@ -503,29 +498,15 @@ int pt_adamw8_step(const int64_t* table, int64_t n_tensors, int64_t total_blocks
   } else {
     s = scalars_of(lr, beta1, beta2, eps, weight_decay, step, seed);
   }
-  const Grid8 grid = grid_of(total_blocks);
-  const auto go = [&](auto waves, auto runs) {
-    hipLaunchKernelGGL(grid.runs ? runs : waves, dim3(grid.blocks), dim3(kThreads), 0, st,
-                       reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors),
-                       static_cast<uint32_t>(total_blocks), grid.per, s, on_device, grad_scale);
+  const auto go = [&](auto kernel) {
+    return launch_units(fn, kernel, total_blocks, st, table, n_tensors, s, static_cast<const Scalars8*>(on_device), grad_scale);
   };
-#define PT_ADAMW8(T, STOCHASTIC)                                                              \
-  if (grad_scale) {                                                                           \
-    go(adamw8_kernel<T, STOCHASTIC, true, false>, adamw8_kernel<T, STOCHASTIC, true, true>);   \
-  } else {                                                                                    \
-    go(adamw8_kernel<T, STOCHASTIC, false, false>, adamw8_kernel<T, STOCHASTIC, false, true>); \
-  }
-  if (dtype == PT_FLOAT32) {
-    PT_ADAMW8(float, false)
-  } else if (dtype == PT_FLOAT16) {
-    PT_ADAMW8(_Float16, false)
-  } else if (stochastic_params) {
-    PT_ADAMW8(__bf16, true)
-  } else {
-    PT_ADAMW8(__bf16, false)
-  }
-#undef PT_ADAMW8
-  return check_launch(fn);
+  if (dtype == PT_FLOAT32) return grad_scale ? go(adamw8_kernel<float, false, true>) : go(adamw8_kernel<float, false, false>);
+  if (dtype == PT_FLOAT16)
+    return grad_scale ? go(adamw8_kernel<_Float16, false, true>) : go(adamw8_kernel<_Float16, false, false>);
+  if (stochastic_params)
+    return grad_scale ? go(adamw8_kernel<__bf16, true, true>) : go(adamw8_kernel<__bf16, true, false>);
+  return grad_scale ? go(adamw8_kernel<__bf16, false, true>) : go(adamw8_kernel<__bf16, false, false>);
 }
 
 int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blocks, void* exp_avg, void* exp_avg_sq,
@@ -537,22 +518,14 @@ int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blo
   if (rc != PT_OK) return rc;
   if (!exp_avg || !exp_avg_sq || !aligned16(exp_avg) || !aligned16(exp_avg_sq))
     return fail(PT_EINVAL, "pt_adamw8_moments: null or misaligned output");
-  const Grid8 grid = grid_of(total_blocks);
-  const auto go = [&](auto waves, auto runs, auto* type) {
-    typedef std::remove_pointer_t<decltype(type)> T;
-    hipLaunchKernelGGL(grid.runs ? runs : waves, dim3(grid.blocks), dim3(kThreads), 0, as_stream(stream),
-                       reinterpret_cast<const Rec8*>(table), static_cast<uint32_t>(n_tensors),
-                       static_cast<uint32_t>(total_blocks), grid.per, static_cast<T*>(exp_avg),
-                       static_cast<T*>(exp_avg_sq));
+  const auto go = [&](auto kernel, auto* m, auto* v) {
+    return launch_units(fn, kernel, total_blocks, as_stream(stream), table, n_tensors, m, v);
   };
-  if (dtype == PT_FLOAT32) {
-    go(adamw8_moments_kernel<float, false>, adamw8_moments_kernel<float, true>, static_cast<float*>(nullptr));
-  } else if (dtype == PT_FLOAT16) {
-    go(adamw8_moments_kernel<_Float16, false>, adamw8_moments_kernel<_Float16, true>, static_cast<_Float16*>(nullptr));
-  } else {
-    go(adamw8_moments_kernel<__bf16, false>, adamw8_moments_kernel<__bf16, true>, static_cast<__bf16*>(nullptr));
-  }
-  return check_launch(fn);
+  if (dtype == PT_FLOAT32)
+    return go(adamw8_moments_kernel<float>, static_cast<float*>(exp_avg), static_cast<float*>(exp_avg_sq));
+  if (dtype == PT_FLOAT16)
+    return go(adamw8_moments_kernel<_Float16>, static_cast<_Float16*>(exp_avg), static_cast<_Float16*>(exp_avg_sq));
+  return go(adamw8_moments_kernel<__bf16>, static_cast<__bf16*>(exp_avg), static_cast<__bf16*>(exp_avg_sq));
 }
 
 }  // extern "C"

@@ -8,12 +8,12 @@
 //
 // g_b needs every token of both sequences of a pair, so no pass over the logits can write the gradient before one
 // has read them all: the kept rows are read twice and every row's gradient written once, which is what bounds both passes.
-//   1. seq_stats: per row (and part of a row, when there are few rows) the maximum and the sum of exp(x - max).
-//   2. seq_finish: joins a row's parts, takes the label's logit, and adds a sequence's tokens (in 64 bits, in a fixed
-//      order; every position's own log-probability is formed in 32 from the row's maximum and sum, without the
-//      cancellation of two large numbers).
-//   3. pair_loss: the loss, the rewards beta * (y - r) and dloss / dy.
-//   4. seq_grad: g * ([j = label] - exp(x - max) / sum), every row's.
+//   1. seq_stats: per row the maximum, the sum of exp(x - max) and the label's log-probability, formed in 32 bits from
+//      these without the cancellation of two large numbers.  Where there are few rows each is split into
+//      parts, which seq_join joins.
+//   2. seq_sum: a sequence's tokens, in 64 bits, in a fixed order.  pair_loss: the loss, the rewards beta * (y - r) and
+//      dloss / dy.  Both in one launch (pair_sum) for calls of few tokens.
+//   3. seq_grad: g * ([j = label] - exp(x - max) / sum), every row's.
 // exp(x - m) is exp2((x - m) * log2(e)) on the hardware's exp2.
 #include <cmath>
 
@@ -70,151 +70,213 @@ constexpr uint32_t kNegInf<__bf16> = 0xff80ff80u;
 // The shift of exps whose maximum is m: m, or 0 where there is nothing above -inf (-inf - -inf would be NaN).
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// Partial (max, sum of exp(x - max)) of each kept row's part blockIdx % parts, by a workgroup of LANES threads.
-// A read-only stream: nothing of the row stays, batches of kBatch vectors a thread in flight, one rescale a batch.
-constexpr int kBatch = 8;
+// What the sums take for a row without a label: no log-probability is above 0.
+constexpr float kLeftOut = 1.0f;
+
+// A label's log-probability, free of the cancellation of a logit and a log-sum-exp: both terms are at most 0.
+__device__ __forceinline__ float log_prob(float xt, float M, float S) { return (xt - M) - logf(S); }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void seq_stats_kernel(Rows d, uint32_t parts, float2* __restrict__ partial) {
+__device__ __forceinline__ float label_logit(const Rows& d, const T* p, int64_t label) {
+  return label >= 0 && label < d.vocab ? Elem<T>::to_f32(p[label]) : NAN;
+}
+
+// Maximum and sum of exp(x - max) of each kept row, LANES threads a row (part: LANES is 256 then), which stay in no
+// register: batches of BATCH 16-byte vectors a thread are in flight together and rescale the sum once.  One part a
+// row: its (max, 1 / sum) goes to stats and its label's log-probability to tokens.  Several: each part's (max, sum)
+// to `partial`, for seq_join.
+template <typename T, int LANES, int BATCH>
+__global__ __launch_bounds__(kThreads) void seq_stats_kernel(Rows d, uint32_t parts, float2* __restrict__ partial,
+                                                             float2* __restrict__ stats, float* __restrict__ tokens) {
   constexpr int V = Elem<T>::VEC;
-  constexpr int kWaves = kThreads / 64;
+  constexpr int kWaves = LANES / 64;
+  constexpr int kGroups = kThreads / LANES;
   __shared__ float red_m[kWaves], red_s[kWaves];
-  const uint32_t row = blockIdx.x / parts, part = blockIdx.x - row * parts;
+  const int slot = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / LANES);
+  const int tid = static_cast<int>(threadIdx.x) % LANES;
+  const uint32_t item = blockIdx.x * static_cast<uint32_t>(kGroups) + slot;
+  const uint32_t row = item / parts, part = item - row * parts;
+  if (row >= d.rows) return;  // spare waves of the last workgroup (no barrier with several rows to one)
   const uint32_t b = row / d.seq, t = row - b * d.seq;
-  if (label_of(d, b, t) == d.ignore) return;
+  const int64_t label = label_of(d, b, t);
+  if (label == d.ignore) {
+    if (tid == 0 && part == 0) tokens[row] = kLeftOut;
+    return;
+  }
   const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
+  float xt = 0.0f;
+  if (tid == 0 && parts == 1) xt = label_logit(d, p, label);  // in flight with the row
   const Split<T> sp(p, d.vocab);
-  const int tid = threadIdx.x;
   // this part's vectors
   const int per = (sp.vecs + static_cast<int>(parts) - 1) / static_cast<int>(parts);
   const int from = static_cast<int>(part) * per < sp.vecs ? static_cast<int>(part) * per : sp.vecs;
   const int n = sp.vecs - from < per ? sp.vecs - from : per;
   const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p) + sp.head + static_cast<int64_t>(from) * V, 0,
                                                      n * 16, kBufferWord3);
+  // the row's head goes with its first part, its tail with its last, an element a thread from either end
   float m = -INFINITY, s = 0.0f;
-  if (part == 0 && tid < sp.head) m = Elem<T>::to_f32(p[tid]);
-  if (part == parts - 1 && tid >= kThreads - V && sp.tail + (kThreads - 1 - tid) < d.vocab) {
-    const float e = Elem<T>::to_f32(p[sp.tail + (kThreads - 1 - tid)]);
-    s = exp_from(m < e ? m : e, shift_of(fmaxf(m, e)));  // of the smaller one (the larger's is added below)
-    m = fmaxf(m, e);
-  }
-  if (m != -INFINITY) s += 1.0f;
-  for (int base = tid; base < n; base += kThreads * kBatch) {
-    Vec16<T> v[kBatch];
+  const int tail = sp.tail + (LANES - 1 - tid);
+  const float head_x = part == 0 && tid < sp.head ? Elem<T>::to_f32(p[tid]) : -INFINITY;
+  const float tail_x = part == parts - 1 && tail < d.vocab ? Elem<T>::to_f32(p[tail]) : -INFINITY;
+  for (int base = tid; base < n; base += LANES * BATCH) {
+    Vec16<T> v[BATCH];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      v[u].raw = __builtin_amdgcn_raw_buffer_load_b128(buf, (base + u * kThreads) * 16, 0, kNonTemporal);
+    for (int u = 0; u < BATCH; ++u)
+      v[u].raw = __builtin_amdgcn_raw_buffer_load_b128(buf, (base + u * LANES) * 16, 0, kNonTemporal);
     float cm = m;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (base + u * kThreads >= n) v[u].raw = u32x4{kNegInf<T>, kNegInf<T>, kNegInf<T>, kNegInf<T>};
+    for (int u = 0; u < BATCH; ++u) {
+      if (base + u * LANES >= n) v[u].raw = u32x4{kNegInf<T>, kNegInf<T>, kNegInf<T>, kNegInf<T>};
 #pragma unroll
       for (int i = 0; i < V; ++i) cm = fmaxf(cm, Elem<T>::to_f32(v[u].e[i]));
     }
     const float ref = shift_of(cm);
     float add = 0.0f;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
+    for (int u = 0; u < BATCH; ++u)
 #pragma unroll
       for (int i = 0; i < V; ++i) add += exp_from(Elem<T>::to_f32(v[u].e[i]), ref);
     s = s * exp_from(m, ref) + add;
     m = cm;
   }
-  const float mw = wave_max(m);
-  const float sw = wave_sum(s * exp_from(m, shift_of(mw)));
-  if (tid % 64 == 0) {
-    red_m[tid / 64] = mw;
-    red_s[tid / 64] = sw;
+  {
+    const float cm = fmaxf(fmaxf(m, head_x), tail_x), ref = shift_of(cm);
+    s = s * exp_from(m, ref) + exp_from(head_x, ref) + exp_from(tail_x, ref);
+    m = cm;
   }
-  __syncthreads();
-  if (tid == 0) {
-    float M = red_m[0];
+  float M = wave_max(m);
+  float S = wave_sum(s * exp_from(m, shift_of(M)));
+  if constexpr (kWaves > 1) {
+    if (tid % 64 == 0) {
+      red_m[tid / 64] = M;
+      red_s[tid / 64] = S;
+    }
+    __syncthreads();
+    if (tid != 0) return;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, red_m[w]);
-    float S = 0.0f;
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_m[w]);
+    S = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) S += red_s[w] * exp_from(red_m[w], shift_of(M));
+  }
+  if (tid != 0) return;
+  if (parts > 1) {
     partial[static_cast<int64_t>(row) * parts + part] = make_float2(M, S);
+  } else {
+    stats[row] = make_float2(M, 1.0f / S);
+    tokens[row] = log_prob(xt, M, S);
   }
 }
 
-// Per sequence: joins the parts of its rows, leaves each row's (max, 1 / sum) in stats, and adds its tokens.
-constexpr int kFinishThreads = 1024;
-
+// Joins the parts of each row, a wave a row.
 template <typename T>
-__global__ __launch_bounds__(kFinishThreads) void seq_finish_kernel(Rows d, uint32_t parts,
-                                                                    const float2* __restrict__ partial,
-                                                                    float2* __restrict__ stats, int average,
-                                                                    float* __restrict__ log_probs,
-                                                                    double* __restrict__ exact_out,
-                                                                    float* __restrict__ weight) {
-  __shared__ double red[kFinishThreads / 64];
-  __shared__ int red_n[kFinishThreads / 64];
-  const uint32_t b = blockIdx.x;
-  double sum = 0.0;
-  int kept = 0;
-  for (uint32_t t = threadIdx.x; t < d.seq; t += kFinishThreads) {
-    const int64_t label = label_of(d, b, t);
-    if (label == d.ignore) continue;
-    const int64_t row = static_cast<int64_t>(b) * d.seq + t;
-    const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
-    const bool inside = label >= 0 && label < d.vocab;
-    const float xt = inside ? Elem<T>::to_f32(p[inside ? label : 0]) : NAN;
-    float M = -INFINITY, S = 0.0f;
-    for (uint32_t k = 0; k < parts; ++k) {
-      const float2 v = partial[row * parts + k];
-      const float nm = fmaxf(M, v.x);
-      S = S * exp_from(M, shift_of(nm)) + v.y * exp_from(v.x, shift_of(nm));
-      M = nm;
-    }
+__global__ __launch_bounds__(kThreads) void seq_join_kernel(Rows d, uint32_t parts, const float2* __restrict__ partial,
+                                                            float2* __restrict__ stats, float* __restrict__ tokens) {
+  const uint32_t row = blockIdx.x * 4u + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
+  if (row >= d.rows) return;
+  const int lane = threadIdx.x % 64;
+  const uint32_t b = row / d.seq, t = row - b * d.seq;
+  const int64_t label = label_of(d, b, t);
+  if (label == d.ignore) return;
+  const float xt = label_logit(d, static_cast<const T*>(d.x) + (b * d.bs + t * d.ss), label);
+  float m = -INFINITY, s = 0.0f;
+  for (uint32_t k = lane; k < parts; k += 64) {
+    const float2 v = partial[static_cast<int64_t>(row) * parts + k];
+    const float cm = fmaxf(m, v.x), ref = shift_of(cm);
+    s = s * exp_from(m, ref) + v.y * exp_from(v.x, ref);
+    m = cm;
+  }
+  const float M = wave_max(m);
+  const float S = wave_sum(s * exp_from(m, shift_of(M)));
+  if (lane == 0) {
     stats[row] = make_float2(M, 1.0f / S);
-    sum += static_cast<double>((xt - M) - logf(S));
-    ++kept;
+    tokens[row] = log_prob(xt, M, S);
+  }
+}
+
+// A sequence's tokens added by one wave, in 64 bits and in a fixed order, eight a lane in flight; every lane has the sum
+// and the number of the kept ones.
+__device__ __forceinline__ double wave_tokens(const float* __restrict__ tokens, uint32_t seq, int* kept) {
+  constexpr int kLoads = 8;
+  const uint32_t lane = threadIdx.x % 64;
+  double sum = 0.0;
+  int n = 0;
+  for (uint32_t base = lane; base < seq; base += 64 * kLoads) {
+    float v[kLoads];
+#pragma unroll
+    for (uint32_t u = 0; u < kLoads; ++u) v[u] = tokens[base + u * 64 < seq ? base + u * 64 : seq - 1];
+#pragma unroll
+    for (uint32_t u = 0; u < kLoads; ++u) {
+      const bool in = base + u * 64 < seq && v[u] != kLeftOut;
+      sum += in ? static_cast<double>(v[u]) : 0.0;
+      n += in ? 1 : 0;
+    }
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) {
     sum += __shfl_xor(sum, k);
-    kept += __shfl_xor(kept, k);
+    n += __shfl_xor(n, k);
   }
+  *kept = n;
+  return sum;
+}
+
+struct SequenceSums {
+  const float* tokens;
+  uint32_t seq, batch;
+  int average;
+  float* log_probs;
+  double* exact;   // for the loss, may be null
+  float* weight;   // of a token in its sequence's value
+};
+
+// One sequence by one wave.
+__device__ __forceinline__ void sum_sequence(const SequenceSums& a, uint32_t b) {
+  int kept;
+  double total = wave_tokens(a.tokens + static_cast<int64_t>(b) * a.seq, a.seq, &kept);
+  const double scale = a.average ? 1.0 / (kept > 0 ? kept : 1) : 1.0;
+  total *= scale;
   if (threadIdx.x % 64 == 0) {
-    red[threadIdx.x / 64] = sum;
-    red_n[threadIdx.x / 64] = kept;
+    a.log_probs[b] = static_cast<float>(total);
+    if (a.exact != nullptr) a.exact[b] = total;
+    a.weight[b] = static_cast<float>(scale);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double total = 0.0;
-    int n = 0;
-#pragma unroll
-    for (int w = 0; w < kFinishThreads / 64; ++w) {
-      total += red[w];
-      n += red_n[w];
-    }
-    const double scale = average ? 1.0 / (n > 0 ? n : 1) : 1.0;
-    total *= scale;
-    log_probs[b] = static_cast<float>(total);
-    if (exact_out != nullptr) exact_out[b] = total;
-    weight[b] = static_cast<float>(scale);
-  }
+}
+
+__global__ __launch_bounds__(kThreads) void seq_sum_kernel(SequenceSums a) {
+  const uint32_t b = blockIdx.x * 4u + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
+  if (b < a.batch) sum_sequence(a, b);
 }
 
 enum LossKind { kSigmoid = 0, kHinge = 1, kIpo = 2 };
 
-// The loss over pairs, by one workgroup; pairs are added in 64 bits in a fixed order.
-__global__ __launch_bounds__(kThreads) void pair_loss_kernel(const double* __restrict__ y, const float* __restrict__ ref,
-                                                             uint32_t pairs, float beta, float smooth, int kind,
-                                                             const float* __restrict__ weight, float* __restrict__ loss,
-                                                             float* __restrict__ rewards, float* __restrict__ slope) {
-  __shared__ double red[kThreads / 64];
+struct PairLoss {
+  const double* y;
+  const float* ref;
+  uint32_t pairs;
+  float beta, smooth;
+  int kind;
+  const float* weight;
+  float* loss;
+  float* rewards;
+  float* slope;
+};
+
+// The loss over pairs, by one workgroup of THREADS; pairs are added in 64 bits in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ void pair_loss(const PairLoss& a) {
+  __shared__ double red[THREADS / 64];
+  const float beta = a.beta, smooth = a.smooth;
   double sum = 0.0;
-  const float inv = 1.0f / static_cast<float>(pairs);
-  for (uint32_t i = threadIdx.x; i < pairs; i += kThreads) {
-    const double c = static_cast<double>(beta) * (y[i] - (ref ? static_cast<double>(ref[i]) : 0.0));
-    const double r = static_cast<double>(beta) * (y[i + pairs] - (ref ? static_cast<double>(ref[i + pairs]) : 0.0));
-    rewards[i] = static_cast<float>(c);
-    rewards[i + pairs] = static_cast<float>(r);
+  const float inv = 1.0f / static_cast<float>(a.pairs);
+  for (uint32_t i = threadIdx.x; i < a.pairs; i += THREADS) {
+    const double rc = a.ref ? static_cast<double>(a.ref[i]) : 0.0, rr = a.ref ? static_cast<double>(a.ref[i + a.pairs]) : 0.0;
+    const double c = static_cast<double>(beta) * (a.y[i] - rc), r = static_cast<double>(beta) * (a.y[i + a.pairs] - rr);
+    a.rewards[i] = static_cast<float>(c);
+    a.rewards[i + a.pairs] = static_cast<float>(r);
     const float h = static_cast<float>(c - r);
     float l, dh;  // L(h) and its derivative
-    if (kind == kSigmoid) {
+    if (a.kind == kSigmoid) {
       // ln(1 + e^-h) = max(-h, 0) + ln(1 + e^-|h|), and that for -h
       const float e = expf(-fabsf(h)), low = log1pf(e), inv1 = 1.0f / (1.0f + e);
       const float neg = h > 0.0f ? e * inv1 : inv1;  // s(-h)
@@ -224,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void pair_loss_kernel(const double* __res
           (smooth > 0.0f ? smooth * (fmaxf(h, 0.0f) + low) : 0.0f);
       dh = smooth * pos - (1.0f - smooth) * neg;
       if (h != h) l = dh = h;
-    } else if (kind == kHinge) {
+    } else if (a.kind == kHinge) {
       l = h < 1.0f ? 1.0f - h : (h == h ? 0.0f : h);
       dh = h < 1.0f ? -1.0f : (h == h ? 0.0f : h);
     } else {
@@ -233,8 +295,8 @@ __global__ __launch_bounds__(kThreads) void pair_loss_kernel(const double* __res
       dh = 2.0f * u / beta;
     }
     sum += static_cast<double>(l);
-    slope[i] = dh * beta * inv * weight[i];
-    slope[i + pairs] = -(dh * beta * inv) * weight[i + pairs];
+    a.slope[i] = dh * beta * inv * a.weight[i];
+    a.slope[i + a.pairs] = -(dh * beta * inv) * a.weight[i + a.pairs];
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
@@ -243,9 +305,20 @@ __global__ __launch_bounds__(kThreads) void pair_loss_kernel(const double* __res
   if (threadIdx.x == 0) {
     double total = 0.0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) total += red[w];
-    *loss = static_cast<float>(total / pairs);
+    for (int w = 0; w < THREADS / 64; ++w) total += red[w];
+    *a.loss = static_cast<float>(total / a.pairs);
   }
+}
+
+__global__ __launch_bounds__(kThreads) void pair_loss_kernel(PairLoss a) { pair_loss<kThreads>(a); }
+
+// Sums and loss in one workgroup, a launch less, for calls of few tokens.
+constexpr int kJoinedThreads = 1024;
+__global__ __launch_bounds__(kJoinedThreads) void pair_sum_kernel(SequenceSums s, PairLoss a) {
+  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
+  for (uint32_t b = wave; b < s.batch; b += kJoinedThreads / 64) sum_sequence(s, b);
+  __syncthreads();  // the sums are this workgroup's own, through global memory
+  pair_loss<kJoinedThreads>(a);
 }
 
 // Gradient rows: item (row, chunk of kVecs * LANES vectors), LANES threads each.  `grad` rows start in the 16-byte phase
@@ -320,10 +393,10 @@ __global__ __launch_bounds__(kThreads) void seq_grad_kernel(Rows d, T* __restric
   if (has_tail) g[tail] = value(tail_v, tail);
 }
 
-// Workspace of a forward call: stats (float2 a row), partials (float2 a row and part), weight (a float a sequence),
-// slope (a float a sequence), 64-bit sums.  stats, weight and slope are what the backward reads.
+// Workspace of a forward call: stats (float2 a row), weight and slope (a float a sequence), which the backward reads;
+// 64-bit sums, tokens (a float a row) and partials (float2 a row and part, when there are several).
 struct Layout {
-  size_t stats, weight, slope, sums, partial, total;
+  size_t stats, weight, slope, sums, tokens, partial, total;
   Layout(int64_t batch, int64_t seq, uint32_t parts) {
     const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
     const size_t rows = static_cast<size_t>(batch) * static_cast<size_t>(seq);
@@ -331,18 +404,25 @@ struct Layout {
     weight = stats + up(rows * 8);
     slope = weight + up(static_cast<size_t>(batch) * 4);
     sums = slope + up(static_cast<size_t>(batch) * 4);
-    partial = sums + up(static_cast<size_t>(batch) * 8);
-    total = partial + up(rows * parts * 8);
+    tokens = sums + up(static_cast<size_t>(batch) * 8);
+    partial = tokens + up(rows * 4);
+    total = partial + (parts > 1 ? up(rows * parts * 8) : 0);
   }
 };
 
-// Parts of a row: one, unless the rows alone leave most of the card idle.
+// Parts of a row: one, unless the rows alone leave most of the card idle; then as many as make kPartGroups workgroups, of
+// kPartVecs vectors at least.
+constexpr int64_t kPartGroups = 512;
+constexpr int64_t kPartVecs = 512;
 uint32_t parts_for(int64_t rows, int64_t vocab, int dtype) {
-  (void)rows;
-  (void)vocab;
-  (void)dtype;
-  return 1;
+  if (rows <= 0 || rows * 2 > kPartGroups) return 1;
+  const int64_t vecs = vocab * dtype_size(dtype) / 16;
+  const int64_t most = vecs / kPartVecs, want = kPartGroups / rows;
+  return static_cast<uint32_t>(most < 2 ? 1 : (want < most ? want : most));
 }
+
+// Rows up to which one workgroup adds all sequences and forms the loss.
+constexpr int64_t kJoinedRows = 16384;
 
 constexpr int64_t kMaxRows = int64_t{1} << 23;
 constexpr int64_t kMaxBatch = int64_t{1} << 21;
@@ -372,24 +452,46 @@ Rows rows_of(const void* logits, int64_t seq, int64_t batch, int64_t bs, int64_t
 }
 
 template <typename T>
-int run_forward(const char* fn, const Rows& d, int64_t batch, uint32_t parts, char* ws, const Layout& at, int average,
-                float* log_probs, double* sums, hipStream_t st) {
-  if (d.rows > 0) {
-    hipLaunchKernelGGL(seq_stats_kernel<T>, dim3(d.rows * parts), dim3(kThreads), 0, st, d, parts,
-                       reinterpret_cast<float2*>(ws + at.partial));
-    if (int rc = check_launch(fn)) return rc;
+int run_rows(const char* fn, const Rows& d, uint32_t parts, char* ws, const Layout& at, hipStream_t st) {
+  float2* partial = reinterpret_cast<float2*>(ws + at.partial);
+  float2* stats = reinterpret_cast<float2*>(ws + at.stats);
+  float* tokens = reinterpret_cast<float*>(ws + at.tokens);
+  const int64_t vecs = (static_cast<int64_t>(d.vocab) + Elem<T>::VEC - 1) / Elem<T>::VEC;
+  const auto go = [&](auto kernel, uint32_t groups) {
+    hipLaunchKernelGGL(kernel, dim3((d.rows * parts + groups - 1) / groups), dim3(kThreads), 0, st, d, parts, partial, stats,
+                       tokens);
+  };
+  if (vecs <= 64) {
+    go(seq_stats_kernel<T, 64, 1>, 4);
+  } else if (vecs <= 512) {
+    go(seq_stats_kernel<T, 64, 4>, 4);
+  } else {
+    go(seq_stats_kernel<T, kThreads, 8>, 1);
   }
-  hipLaunchKernelGGL(seq_finish_kernel<T>, dim3(static_cast<unsigned>(batch)), dim3(kFinishThreads), 0, st, d, parts,
-                     reinterpret_cast<const float2*>(ws + at.partial), reinterpret_cast<float2*>(ws + at.stats), average,
-                     log_probs, sums, reinterpret_cast<float*>(ws + at.weight));
-  return check_launch(fn);
+  if (int rc = check_launch(fn)) return rc;
+  if (parts > 1) {
+    hipLaunchKernelGGL(seq_join_kernel<T>, dim3((d.rows + 3) / 4), dim3(kThreads), 0, st, d, parts, partial, stats, tokens);
+    return check_launch(fn);
+  }
+  return PT_OK;
 }
 
-int forward(const char* fn, const Rows& d, int64_t batch, char* ws, const Layout& at, uint32_t parts, int average,
-            float* log_probs, double* sums, int dtype, hipStream_t st) {
-  if (dtype == PT_FLOAT32) return run_forward<float>(fn, d, batch, parts, ws, at, average, log_probs, sums, st);
-  if (dtype == PT_FLOAT16) return run_forward<_Float16>(fn, d, batch, parts, ws, at, average, log_probs, sums, st);
-  return run_forward<__bf16>(fn, d, batch, parts, ws, at, average, log_probs, sums, st);
+// The rows' statistics and tokens.
+int forward_rows(const char* fn, const Rows& d, uint32_t parts, char* ws, const Layout& at, int dtype, hipStream_t st) {
+  if (d.rows == 0) return PT_OK;
+  if (dtype == PT_FLOAT32) return run_rows<float>(fn, d, parts, ws, at, st);
+  if (dtype == PT_FLOAT16) return run_rows<_Float16>(fn, d, parts, ws, at, st);
+  return run_rows<__bf16>(fn, d, parts, ws, at, st);
+}
+
+SequenceSums sums_of(const Rows& d, int64_t batch, char* ws, const Layout& at, int average, float* log_probs, bool exact) {
+  return SequenceSums{reinterpret_cast<const float*>(ws + at.tokens), d.seq, static_cast<uint32_t>(batch), average, log_probs,
+                      exact ? reinterpret_cast<double*>(ws + at.sums) : nullptr, reinterpret_cast<float*>(ws + at.weight)};
+}
+
+int launch_sums(const char* fn, const SequenceSums& s, hipStream_t st) {
+  hipLaunchKernelGGL(seq_sum_kernel, dim3((s.batch + 3) / 4), dim3(kThreads), 0, st, s);
+  return check_launch(fn);
 }
 
 template <typename T>
@@ -435,8 +537,10 @@ int pt_sequence_log_probs(const void* logits, int64_t batch, int64_t seq, int64_
   const Layout at(batch, seq, parts);
   const Rows d = rows_of(logits, seq, batch, batch_stride, seq_stride, vocab, labels, l_batch_stride, l_seq_stride, shift,
                          ignore_index);
-  return forward(fn, d, batch, static_cast<char*>(workspace), at, parts, average, log_probs, nullptr, dtype,
-                 as_stream(stream));
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t st = as_stream(stream);
+  if (int frc = forward_rows(fn, d, parts, ws, at, dtype, st)) return frc;
+  return launch_sums(fn, sums_of(d, batch, ws, at, average, log_probs, false), st);
 }
 
 int pt_preference_loss(const void* logits, int64_t pairs, int64_t seq, int64_t batch_stride, int64_t seq_stride,
@@ -460,11 +564,16 @@ int pt_preference_loss(const void* logits, int64_t pairs, int64_t seq, int64_t b
   const Rows d = rows_of(logits, seq, batch, batch_stride, seq_stride, vocab, labels, l_batch_stride, l_seq_stride, shift,
                          ignore_index);
   hipStream_t st = as_stream(stream);
-  double* sums = reinterpret_cast<double*>(ws + at.sums);
-  if (int frc = forward(fn, d, batch, ws, at, parts, average, log_probs, sums, dtype, st)) return frc;
-  hipLaunchKernelGGL(pair_loss_kernel, dim3(1), dim3(kThreads), 0, st, sums, reference, static_cast<uint32_t>(pairs), beta,
-                     label_smoothing, kind, reinterpret_cast<const float*>(ws + at.weight), loss, rewards,
-                     reinterpret_cast<float*>(ws + at.slope));
+  if (int frc = forward_rows(fn, d, parts, ws, at, dtype, st)) return frc;
+  const SequenceSums sums = sums_of(d, batch, ws, at, average, log_probs, true);
+  const PairLoss pl{sums.exact, reference, static_cast<uint32_t>(pairs), beta, label_smoothing, kind, sums.weight, loss,
+                    rewards, reinterpret_cast<float*>(ws + at.slope)};
+  if (batch * seq <= kJoinedRows) {
+    hipLaunchKernelGGL(pair_sum_kernel, dim3(1), dim3(kJoinedThreads), 0, st, sums, pl);
+    return check_launch(fn);
+  }
+  if (int frc = launch_sums(fn, sums, st)) return frc;
+  hipLaunchKernelGGL(pair_loss_kernel, dim3(1), dim3(kThreads), 0, st, pl);
   return check_launch(fn);
 }
 
