@@ -12,7 +12,7 @@
 //      these without the cancellation of two large numbers.  Where there are few rows each is split into
 //      parts, which seq_join joins.
 //   2. seq_sum: a sequence's tokens, in 64 bits, in a fixed order.  pair_loss: the loss, the rewards beta * (y - r) and
-//      dloss / dy.  Both in one launch (pair_sum) for calls of few tokens.
+//      dloss / dy.  All of it in one launch (seq_small) for calls of few tokens.
 //   3. seq_grad: g * ([j = label] - exp(x - max) / sum), every row's.
 // exp(x - m) is exp2((x - m) * log2(e)) on the hardware's exp2.
 #include <cmath>
@@ -81,22 +81,183 @@ __device__ __forceinline__ float label_logit(const Rows& d, const T* p, int64_t 
   return label >= 0 && label < d.vocab ? Elem<T>::to_f32(p[label]) : NAN;
 }
 
-// Maximum and sum of exp(x - max) of each kept row, LANES threads a row (part: LANES is 256 then), which stay in no
-// register: batches of BATCH 16-byte vectors a thread are in flight together and rescale the sum once.  One part a
-// row: its (max, 1 / sum) goes to stats and its label's log-probability to tokens.  Several: each part's (max, sum)
-// to `partial`, for seq_join.
-template <typename T, int LANES, int BATCH>
+// Running maximum and sum of exp(x - max) of a thread's elements.
+struct Running {
+  float m = -INFINITY, s = 0.0f;
+
+  // Adds N vectors of T, one rescale for all; elements that are none are -inf.
+  template <typename T, int N>
+  __device__ __forceinline__ void add(const Vec16<T> (&v)[N]) {
+    float cm = m;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int i = 0; i < Elem<T>::VEC; ++i) cm = fmaxf(cm, Elem<T>::to_f32(v[u].e[i]));
+    const float ref = shift_of(cm);
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int i = 0; i < Elem<T>::VEC; ++i) sum += exp_from(Elem<T>::to_f32(v[u].e[i]), ref);
+    s = s * exp_from(m, ref) + sum;
+    m = cm;
+  }
+
+  __device__ __forceinline__ void add(float x, float y) {
+    const float cm = fmaxf(fmaxf(m, x), y), ref = shift_of(cm);
+    s = s * exp_from(m, ref) + exp_from(x, ref) + exp_from(y, ref);
+    m = cm;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ u32x4 lowest_vec() {
+  return u32x4{kNegInf<T>, kNegInf<T>, kNegInf<T>, kNegInf<T>};
+}
+
+// A row (or part of one) as LANES threads read it, of which this is number tid: 16-byte vectors through a buffer
+// resource whose range check drops what lies behind them; the row's head goes with its first part, its tail with its
+// last, an element a thread from either end.
+template <typename T, int LANES>
+struct RowReader {
+  __amdgpu_buffer_rsrc_t buf;
+  int n;  // vectors
+  float head, tail;
+
+  __device__ __forceinline__ RowReader(const T* p, int vocab, int part, int parts, int tid, bool skip) {
+    const Split<T> sp(p, vocab);
+    const int per = (sp.vecs + parts - 1) / parts;
+    const int from = part * per < sp.vecs ? part * per : sp.vecs;
+    n = skip ? 0 : (sp.vecs - from < per ? sp.vecs - from : per);
+    buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p) + sp.head + static_cast<int64_t>(from) * Elem<T>::VEC, 0,
+                                            n * 16, kBufferWord3);
+    const int at = sp.tail + (LANES - 1 - tid);
+    head = !skip && part == 0 && tid < sp.head ? Elem<T>::to_f32(p[tid]) : -INFINITY;
+    tail = !skip && part == parts - 1 && at < vocab ? Elem<T>::to_f32(p[at]) : -INFINITY;
+  }
+
+  template <int N>
+  __device__ __forceinline__ void load(int base, Vec16<T> (&v)[N]) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      v[u].raw = __builtin_amdgcn_raw_buffer_load_b128(buf, (base + u * LANES) * 16, 0, kNonTemporal);
+  }
+
+  // -inf in place of the zeros that were read behind the part
+  template <int N>
+  __device__ __forceinline__ void mask(int base, Vec16<T> (&v)[N]) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (base + u * LANES >= n) v[u].raw = lowest_vec<T>();
+  }
+};
+
+__device__ __forceinline__ uint32_t wave_index() {
+  return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
+}
+
+// Rows of up to 16 * K vectors, of one at least: 16 lanes a row, four rows a wave, so that the reductions and what
+// follows them are paid once for four rows (262000 rows of 260 bf16 logits: a wave a row was bound by them, 85 us).  The
+// last vector of a row that is no whole number of them starts earlier; what it repeats is masked.
+template <typename T, int K>
+struct TinyRow {
+  static constexpr int V = Elem<T>::VEC;
+  uint32_t row, b;
+  int64_t label;
+  bool skip;
+  const T* p;
+  int at[K];  // first element of each vector, or behind the row
+  Vec16<T> v[K];
+
+  __device__ __forceinline__ TinyRow(const Rows& d) {
+    const int lane = threadIdx.x % 16;
+    row = blockIdx.x * (kThreads / 16) + threadIdx.x / 16;
+    const bool in = row < d.rows;
+    b = (in ? row : 0) / d.seq;
+    const uint32_t t = (in ? row : 0) - b * d.seq;
+    label = in ? label_of(d, b, t) : d.ignore;
+    skip = label == d.ignore;
+    p = static_cast<const T*>(d.x) + (static_cast<int64_t>(b) * d.bs + static_cast<int64_t>(t) * d.ss);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = (lane + 16 * k) * V;
+      at[k] = i >= d.vocab ? d.vocab : (i <= d.vocab - V ? i : d.vocab - V);
+      v[k].raw = lowest_vec<T>();
+      if (!skip && at[k] < d.vocab) v[k].raw = load_vec<T, false, true>(p + at[k]);
+    }
+  }
+};
+
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp::move<dpp::kQuadSwap1>(v));
+  v = fmaxf(v, dpp::move<dpp::kQuadSwap2>(v));
+  v = fmaxf(v, dpp::move<dpp::kRowHalfMirror>(v));
+  return fmaxf(v, dpp::move<dpp::kRowMirror>(v));
+}
+
+template <typename T, int K>
+__global__ __launch_bounds__(kThreads) void seq_stats_tiny_kernel(Rows d, float2* __restrict__ stats,
+                                                                  float* __restrict__ tokens) {
+  const int lane = threadIdx.x % 16;
+  TinyRow<T, K> r(d);
+  const float xt = r.skip ? 0.0f : label_logit(d, r.p, r.label);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int again = (lane + 16 * k) * TinyRow<T, K>::V - r.at[k];  // elements that the vector before has
+#pragma unroll
+    for (int i = 0; i < TinyRow<T, K>::V; ++i)
+      if (i < again) r.v[k].e[i] = Elem<T>::from_f32(-INFINITY);
+  }
+  Running run;
+  run.add(r.v);
+  const float M = row16_max(run.m);
+  const float S = row16_sum(run.s * exp_from(run.m, shift_of(M)));
+  if (lane == 0 && r.row < d.rows) {
+    if (!r.skip) stats[r.row] = make_float2(M, 1.0f / S);
+    tokens[r.row] = r.skip ? kLeftOut : log_prob(xt, M, S);
+  }
+}
+
+// Rows of up to 64 * N vectors: a wave a row, all of it in flight together.
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void seq_stats_short_kernel(Rows d, float2* __restrict__ stats,
+                                                                   float* __restrict__ tokens) {
+  const int lane = threadIdx.x % 64;
+  const uint32_t row = blockIdx.x * (kThreads / 64) + wave_index();
+  if (row >= d.rows) return;
+  const uint32_t b = row / d.seq, t = row - b * d.seq;
+  const int64_t label = label_of(d, b, t);
+  if (label == d.ignore) {
+    if (lane == 0) tokens[row] = kLeftOut;
+    return;
+  }
+  const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
+  const RowReader<T, 64> in(p, d.vocab, 0, 1, lane, false);
+  Vec16<T> v[N];
+  in.load(lane, v);
+  const float xt = label_logit(d, p, label);
+  in.mask(lane, v);
+  Running run;
+  run.add(v);
+  run.add(in.head, in.tail);
+  const float M = wave_max(run.m);
+  const float S = wave_sum(run.s * exp_from(run.m, shift_of(M)));
+  if (lane == 0) {
+    stats[row] = make_float2(M, 1.0f / S);
+    tokens[row] = log_prob(xt, M, S);
+  }
+}
+
+// Longer rows: a workgroup a row, or a part of one where there are few: its (max, sum) then goes to `partial`.
+constexpr int kBatch = 8;
+
+template <typename T>
 __global__ __launch_bounds__(kThreads) void seq_stats_kernel(Rows d, uint32_t parts, float2* __restrict__ partial,
                                                              float2* __restrict__ stats, float* __restrict__ tokens) {
-  constexpr int V = Elem<T>::VEC;
-  constexpr int kWaves = LANES / 64;
-  constexpr int kGroups = kThreads / LANES;
+  constexpr int kWaves = kThreads / 64;
   __shared__ float red_m[kWaves], red_s[kWaves];
-  const int slot = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / LANES);
-  const int tid = static_cast<int>(threadIdx.x) % LANES;
-  const uint32_t item = blockIdx.x * static_cast<uint32_t>(kGroups) + slot;
-  const uint32_t row = item / parts, part = item - row * parts;
-  if (row >= d.rows) return;  // spare waves of the last workgroup (no barrier with several rows to one)
+  const int tid = threadIdx.x;
+  const uint32_t row = blockIdx.x / parts, part = blockIdx.x - row * parts;
   const uint32_t b = row / d.seq, t = row - b * d.seq;
   const int64_t label = label_of(d, b, t);
   if (label == d.ignore) {
@@ -104,62 +265,30 @@ __global__ __launch_bounds__(kThreads) void seq_stats_kernel(Rows d, uint32_t pa
     return;
   }
   const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
+  const RowReader<T, kThreads> in(p, d.vocab, static_cast<int>(part), static_cast<int>(parts), tid, false);
   float xt = 0.0f;
   if (tid == 0 && parts == 1) xt = label_logit(d, p, label);  // in flight with the row
-  const Split<T> sp(p, d.vocab);
-  // this part's vectors
-  const int per = (sp.vecs + static_cast<int>(parts) - 1) / static_cast<int>(parts);
-  const int from = static_cast<int>(part) * per < sp.vecs ? static_cast<int>(part) * per : sp.vecs;
-  const int n = sp.vecs - from < per ? sp.vecs - from : per;
-  const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p) + sp.head + static_cast<int64_t>(from) * V, 0,
-                                                     n * 16, kBufferWord3);
-  // the row's head goes with its first part, its tail with its last, an element a thread from either end
-  float m = -INFINITY, s = 0.0f;
-  const int tail = sp.tail + (LANES - 1 - tid);
-  const float head_x = part == 0 && tid < sp.head ? Elem<T>::to_f32(p[tid]) : -INFINITY;
-  const float tail_x = part == parts - 1 && tail < d.vocab ? Elem<T>::to_f32(p[tail]) : -INFINITY;
-  for (int base = tid; base < n; base += LANES * BATCH) {
-    Vec16<T> v[BATCH];
-#pragma unroll
-    for (int u = 0; u < BATCH; ++u)
-      v[u].raw = __builtin_amdgcn_raw_buffer_load_b128(buf, (base + u * LANES) * 16, 0, kNonTemporal);
-    float cm = m;
-#pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      if (base + u * LANES >= n) v[u].raw = u32x4{kNegInf<T>, kNegInf<T>, kNegInf<T>, kNegInf<T>};
-#pragma unroll
-      for (int i = 0; i < V; ++i) cm = fmaxf(cm, Elem<T>::to_f32(v[u].e[i]));
-    }
-    const float ref = shift_of(cm);
-    float add = 0.0f;
-#pragma unroll
-    for (int u = 0; u < BATCH; ++u)
-#pragma unroll
-      for (int i = 0; i < V; ++i) add += exp_from(Elem<T>::to_f32(v[u].e[i]), ref);
-    s = s * exp_from(m, ref) + add;
-    m = cm;
+  Running run;
+  for (int base = tid; base < in.n; base += kThreads * kBatch) {
+    Vec16<T> v[kBatch];
+    in.load(base, v);
+    in.mask(base, v);
+    run.add(v);
   }
-  {
-    const float cm = fmaxf(fmaxf(m, head_x), tail_x), ref = shift_of(cm);
-    s = s * exp_from(m, ref) + exp_from(head_x, ref) + exp_from(tail_x, ref);
-    m = cm;
+  run.add(in.head, in.tail);
+  float M = wave_max(run.m);
+  float S = wave_sum(run.s * exp_from(run.m, shift_of(M)));
+  if (tid % 64 == 0) {
+    red_m[tid / 64] = M;
+    red_s[tid / 64] = S;
   }
-  float M = wave_max(m);
-  float S = wave_sum(s * exp_from(m, shift_of(M)));
-  if constexpr (kWaves > 1) {
-    if (tid % 64 == 0) {
-      red_m[tid / 64] = M;
-      red_s[tid / 64] = S;
-    }
-    __syncthreads();
-    if (tid != 0) return;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_m[w]);
-    S = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) S += red_s[w] * exp_from(red_m[w], shift_of(M));
-  }
+  __syncthreads();
   if (tid != 0) return;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_m[w]);
+  S = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) S += red_s[w] * exp_from(red_m[w], shift_of(M));
   if (parts > 1) {
     partial[static_cast<int64_t>(row) * parts + part] = make_float2(M, S);
   } else {
@@ -168,20 +297,24 @@ __global__ __launch_bounds__(kThreads) void seq_stats_kernel(Rows d, uint32_t pa
   }
 }
 
-// Joins the parts of each row, a wave a row.
+struct Parts {
+  uint32_t parts;
+  const float2* partial;
+  float2* stats;
+  float* tokens;
+};
+
+// Joins the parts of a row, by a wave.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void seq_join_kernel(Rows d, uint32_t parts, const float2* __restrict__ partial,
-                                                            float2* __restrict__ stats, float* __restrict__ tokens) {
-  const uint32_t row = blockIdx.x * 4u + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
-  if (row >= d.rows) return;
+__device__ __forceinline__ void join_row(const Rows& d, const Parts& a, uint32_t row) {
   const int lane = threadIdx.x % 64;
   const uint32_t b = row / d.seq, t = row - b * d.seq;
   const int64_t label = label_of(d, b, t);
   if (label == d.ignore) return;
   const float xt = label_logit(d, static_cast<const T*>(d.x) + (b * d.bs + t * d.ss), label);
   float m = -INFINITY, s = 0.0f;
-  for (uint32_t k = lane; k < parts; k += 64) {
-    const float2 v = partial[static_cast<int64_t>(row) * parts + k];
+  for (uint32_t k = lane; k < a.parts; k += 64) {
+    const float2 v = a.partial[static_cast<int64_t>(row) * a.parts + k];
     const float cm = fmaxf(m, v.x), ref = shift_of(cm);
     s = s * exp_from(m, ref) + v.y * exp_from(v.x, ref);
     m = cm;
@@ -189,25 +322,31 @@ __global__ __launch_bounds__(kThreads) void seq_join_kernel(Rows d, uint32_t par
   const float M = wave_max(m);
   const float S = wave_sum(s * exp_from(m, shift_of(M)));
   if (lane == 0) {
-    stats[row] = make_float2(M, 1.0f / S);
-    tokens[row] = log_prob(xt, M, S);
+    a.stats[row] = make_float2(M, 1.0f / S);
+    a.tokens[row] = log_prob(xt, M, S);
   }
 }
 
-// A sequence's tokens added by one wave, in 64 bits and in a fixed order, eight a lane in flight; every lane has the sum
-// and the number of the kept ones.
-__device__ __forceinline__ double wave_tokens(const float* __restrict__ tokens, uint32_t seq, int* kept) {
-  constexpr int kLoads = 8;
-  const uint32_t lane = threadIdx.x % 64;
+template <typename T>
+__global__ __launch_bounds__(kThreads) void seq_join_kernel(Rows d, Parts a) {
+  const uint32_t row = blockIdx.x * 4u + wave_index();
+  if (row < d.rows) join_row<T>(d, a, row);
+}
+
+// The tokens first, first + step, ... of a sequence of `seq` added by one wave (first: its lane's), in 64 bits and in a
+// fixed order, eight a lane in flight; every lane has the sum and the number of the kept ones.
+__device__ __forceinline__ double wave_tokens(const float* __restrict__ tokens, uint32_t seq, uint32_t first, uint32_t step,
+                                              int* kept) {
+  constexpr uint32_t kLoads = 8;
   double sum = 0.0;
   int n = 0;
-  for (uint32_t base = lane; base < seq; base += 64 * kLoads) {
+  for (uint32_t base = first; base < seq; base += step * kLoads) {
     float v[kLoads];
 #pragma unroll
-    for (uint32_t u = 0; u < kLoads; ++u) v[u] = tokens[base + u * 64 < seq ? base + u * 64 : seq - 1];
+    for (uint32_t u = 0; u < kLoads; ++u) v[u] = tokens[base + u * step < seq ? base + u * step : seq - 1];
 #pragma unroll
     for (uint32_t u = 0; u < kLoads; ++u) {
-      const bool in = base + u * 64 < seq && v[u] != kLeftOut;
+      const bool in = base + u * step < seq && v[u] != kLeftOut;
       sum += in ? static_cast<double>(v[u]) : 0.0;
       n += in ? 1 : 0;
     }
@@ -230,22 +369,54 @@ struct SequenceSums {
   float* weight;   // of a token in its sequence's value
 };
 
-// One sequence by one wave.
-__device__ __forceinline__ void sum_sequence(const SequenceSums& a, uint32_t b) {
-  int kept;
-  double total = wave_tokens(a.tokens + static_cast<int64_t>(b) * a.seq, a.seq, &kept);
-  const double scale = a.average ? 1.0 / (kept > 0 ? kept : 1) : 1.0;
-  total *= scale;
-  if (threadIdx.x % 64 == 0) {
-    a.log_probs[b] = static_cast<float>(total);
-    if (a.exact != nullptr) a.exact[b] = total;
-    a.weight[b] = static_cast<float>(scale);
+// The sequences [first, end) by a workgroup of WAVES waves: `team` (a power of two) waves a sequence, at a time as many
+// sequences as there are teams.
+template <int WAVES>
+__device__ __forceinline__ void sum_sequences(const SequenceSums& a, uint32_t first, uint32_t end, uint32_t team) {
+  __shared__ double red[WAVES];
+  __shared__ int red_n[WAVES];
+  const uint32_t wave = wave_index(), lane = threadIdx.x % 64;
+  const uint32_t teams = WAVES / team, mine = wave / team, member = wave % team;
+  for (uint32_t at = first; at < end; at += teams) {  // the same for every wave
+    const uint32_t b = at + mine;
+    int kept = 0;
+    double sum = 0.0;
+    if (b < end)
+      sum = wave_tokens(a.tokens + static_cast<int64_t>(b) * a.seq, a.seq, member * 64 + lane, team * 64, &kept);
+    if (team > 1) {
+      if (lane == 0) {
+        red[wave] = sum;
+        red_n[wave] = kept;
+      }
+      __syncthreads();
+      if (member == 0) {
+        for (uint32_t w = 1; w < team; ++w) {
+          sum += red[wave + w];
+          kept += red_n[wave + w];
+        }
+      }
+      __syncthreads();
+    }
+    if (b < end && member == 0 && lane == 0) {
+      const double scale = a.average ? 1.0 / (kept > 0 ? kept : 1) : 1.0;
+      a.log_probs[b] = static_cast<float>(sum * scale);
+      if (a.exact != nullptr) a.exact[b] = sum * scale;
+      a.weight[b] = static_cast<float>(scale);
+    }
   }
 }
 
-__global__ __launch_bounds__(kThreads) void seq_sum_kernel(SequenceSums a) {
-  const uint32_t b = blockIdx.x * 4u + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
-  if (b < a.batch) sum_sequence(a, b);
+// Waves for a sequence, of `most`, so that each has up to 512 tokens (its lanes' eight loads).
+__host__ __device__ inline uint32_t team_of(uint32_t seq, uint32_t most) {
+  uint32_t team = 1;
+  while (team < most && team * 512 < seq) team *= 2;
+  return team;
+}
+
+__global__ __launch_bounds__(kThreads) void seq_sum_kernel(SequenceSums a, uint32_t team) {
+  constexpr uint32_t kWaves = kThreads / 64;
+  const uint32_t first = blockIdx.x * (kWaves / team), end = first + kWaves / team;
+  sum_sequences<kWaves>(a, first, end < a.batch ? end : a.batch, team);
 }
 
 enum LossKind { kSigmoid = 0, kHinge = 1, kIpo = 2 };
@@ -312,85 +483,121 @@ __device__ __forceinline__ void pair_loss(const PairLoss& a) {
 
 __global__ __launch_bounds__(kThreads) void pair_loss_kernel(PairLoss a) { pair_loss<kThreads>(a); }
 
-// Sums and loss in one workgroup, a launch less, for calls of few tokens.
-constexpr int kJoinedThreads = 1024;
-__global__ __launch_bounds__(kJoinedThreads) void pair_sum_kernel(SequenceSums s, PairLoss a) {
-  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64));
-  for (uint32_t b = wave; b < s.batch; b += kJoinedThreads / 64) sum_sequence(s, b);
-  __syncthreads();  // the sums are this workgroup's own, through global memory
-  pair_loss<kJoinedThreads>(a);
+// What is left after the rows in one workgroup, for calls of few tokens: the join of the rows' parts, the sums, and the loss
+// (pairs above 0).
+constexpr int kSmallThreads = 1024;
+template <typename T>
+__global__ __launch_bounds__(kSmallThreads) void seq_small_kernel(Rows d, Parts j, SequenceSums s, uint32_t team, PairLoss a) {
+  constexpr uint32_t kWaves = kSmallThreads / 64;
+  if (j.parts > 1) {
+    for (uint32_t row = wave_index(); row < d.rows; row += kWaves) join_row<T>(d, j, row);
+    __syncthreads();  // (what a workgroup's waves read of each other here goes through global memory)
+  }
+  sum_sequences<kWaves>(s, 0, s.batch, team);
+  if (a.pairs > 0) {
+    __syncthreads();
+    pair_loss<kSmallThreads>(a);
+  }
 }
 
-// Gradient rows: item (row, chunk of kVecs * LANES vectors), LANES threads each.  `grad` rows start in the 16-byte phase
-// of their logits rows (checked on the host).
-constexpr int kVecs = 4;
-
-template <typename T, int LANES>
-__global__ __launch_bounds__(kThreads) void seq_grad_kernel(Rows d, T* __restrict__ grad, int64_t gbs, int64_t gss,
-                                                            uint32_t chunks, uint32_t items,
-                                                            const float2* __restrict__ stats,
-                                                            const float* __restrict__ slope,
-                                                            const float* __restrict__ weight,
-                                                            const float* __restrict__ upstream) {
-  constexpr int V = Elem<T>::VEC;
-  constexpr int kGroups = kThreads / LANES;
-  const int slot = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / LANES);
-  const uint32_t item = blockIdx.x * static_cast<uint32_t>(kGroups) + slot;
-  if (item >= items) return;
-  const uint32_t row = item / chunks, c = item - row * chunks;
-  const uint32_t b = row / d.seq, t = row - b * d.seq;
-  const int tid = static_cast<int>(threadIdx.x) % LANES;
-  const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
-  T* g = grad + (b * gbs + t * gss);
-  const int64_t label = label_of(d, b, t);
-  const bool skip = label == d.ignore;
-  const Split<T> sp(p, d.vocab);
-  const int from = static_cast<int>(c) * LANES * kVecs;
-  int n = sp.vecs - from;
-  n = n < 0 ? 0 : (n < LANES * kVecs ? n : LANES * kVecs);
-  const int64_t at = sp.head + static_cast<int64_t>(from) * V;
-  // a row without a label reads nothing
-  const auto in = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p) + at, 0, skip ? 0 : n * 16, kBufferWord3);
-  const auto out = __builtin_amdgcn_make_buffer_rsrc(g + at, 0, n * 16, kBufferWord3);
-  Vec16<T> v[kVecs];
-#pragma unroll
-  for (int k = 0; k < kVecs; ++k)
-    v[k].raw = __builtin_amdgcn_raw_buffer_load_b128(in, (k * LANES + tid) * 16, 0, kNonTemporal);
-  // the row's head goes with its first item, its tail with its last (one element a thread, LANES >= 64 of each)
-  const bool has_head = c == 0 && tid < sp.head;
-  const int tail = sp.tail + tid;
-  const bool has_tail = c == chunks - 1 && tail < d.vocab;
-  T head_v{}, tail_v{};
-  if (!skip && has_head) head_v = p[tid];
-  if (!skip && has_tail) tail_v = p[tail];
-  float coef = 0.0f, m = 0.0f, f = 0.0f;
-  if (!skip) {
-    const float2 st = stats[row];
-    coef = slope[b] * (weight ? weight[b] : 1.0f) * (upstream ? *upstream : 1.0f);
-    m = st.x;
-    f = coef * st.y;
+// What a gradient element is made of: g * ([j == label] - exp(x - max) / sum).
+struct Slope {
+  float coef = 0.0f, m = 0.0f, f = 0.0f;  // g, the maximum, g / sum
+  __device__ __forceinline__ float at(float x, bool target) const {
+    const float y = -(exp_from(x, m) * f);
+    return target ? y + coef : y;
   }
-  const auto value = [&](T x, int64_t j) -> T {
-    if (skip) return Elem<T>::from_f32(0.0f);
-    float y = -(exp_from(Elem<T>::to_f32(x), m) * f);
-    if (j == label) y += coef;
-    return Elem<T>::from_f32(y);
-  };
-  const int64_t rel = label - at;
-  const int target = rel >= 0 && rel < static_cast<int64_t>(LANES) * kVecs * V ? static_cast<int>(rel) : -1;
+};
+
+struct SlopeSource {
+  const float2* stats;
+  const float* slope;
+  const float* weight;
+  const float* upstream;
+  __device__ __forceinline__ Slope of(uint32_t row, uint32_t b) const {
+    const float2 st = stats[row];
+    Slope s;
+    s.coef = slope[b] * (weight ? weight[b] : 1.0f) * (upstream ? *upstream : 1.0f);
+    s.m = st.x;
+    s.f = s.coef * st.y;
+    return s;
+  }
+};
+
+// Rows of up to 16 * K vectors (seq_stats_tiny): what the last vector repeats is written twice, the same.
+template <typename T, int K>
+__global__ __launch_bounds__(kThreads) void seq_grad_tiny_kernel(Rows d, T* __restrict__ grad, int64_t gbs, int64_t gss,
+                                                                 SlopeSource from) {
+  constexpr int V = Elem<T>::VEC;
+  TinyRow<T, K> r(d);
+  if (r.row >= d.rows) return;
+  Slope s;
+  if (!r.skip) s = from.of(r.row, r.b);
+  T* g = grad + (static_cast<int64_t>(r.b) * gbs + static_cast<int64_t>(r.row - r.b * d.seq) * gss);
+  const int target = r.label >= 0 && r.label < d.vocab ? static_cast<int>(r.label) : -1;
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
+  for (int k = 0; k < K; ++k) {
+    if (r.at[k] >= d.vocab) break;
     Vec16<T> o;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float y = -(exp_from(Elem<T>::to_f32(v[k].e[i]), m) * f);
-      if ((k * LANES + tid) * V + i == target) y += coef;
+      const float y = s.at(Elem<T>::to_f32(r.v[k].e[i]), r.at[k] + i == target);
+      o.e[i] = Elem<T>::from_f32(r.skip ? 0.0f : y);
+    }
+    store_vec<T, false, true>(g + r.at[k], o.raw);
+  }
+}
+
+// LANES threads for `per` vectors (whole lines, at most LANES * VECS) of a row: item i is chunk i % chunks of row
+// i / chunks.  All its loads are in flight before the first exp.  `grad` rows start in the 16-byte phase of their logits
+// rows (checked on the host).
+template <typename T, int LANES, int VECS>
+__global__ __launch_bounds__(kThreads) void seq_grad_kernel(Rows d, T* __restrict__ grad, int64_t gbs, int64_t gss,
+                                                            uint32_t chunks, uint32_t items, int per, SlopeSource from) {
+  constexpr int V = Elem<T>::VEC;
+  constexpr int kGroups = kThreads / LANES;
+  const uint32_t item = blockIdx.x * static_cast<uint32_t>(kGroups) + (kGroups == 1 ? 0 : wave_index() / (LANES / 64));
+  if (item >= items) return;
+  const int tid = static_cast<int>(threadIdx.x) % LANES;
+  const uint32_t row = item / chunks, c = item - row * chunks;
+  const uint32_t b = row / d.seq, t = row - b * d.seq;
+  const int64_t label = label_of(d, b, t);
+  const bool skip = label == d.ignore;
+  const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
+  T* g = grad + (b * gbs + t * gss);
+  const Split<T> sp(p, d.vocab);
+  const int begin = static_cast<int>(c) * per;
+  int n = sp.vecs - begin;
+  n = n < 0 ? 0 : (n < per ? n : per);
+  const int64_t at = sp.head + static_cast<int64_t>(begin) * V;
+  // a row without a label reads nothing
+  const auto in = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p) + at, 0, skip ? 0 : n * 16, kBufferWord3);
+  const auto out = __builtin_amdgcn_make_buffer_rsrc(g + at, 0, n * 16, kBufferWord3);
+  Vec16<T> v[VECS];
+#pragma unroll
+  for (int k = 0; k < VECS; ++k)
+    v[k].raw = __builtin_amdgcn_raw_buffer_load_b128(in, (k * LANES + tid) * 16, 0, kNonTemporal);
+  // the row's head goes with its first chunk, its tail with its last (one element a thread)
+  const bool has_head = c == 0 && tid < sp.head, has_tail = c == chunks - 1 && sp.tail + tid < d.vocab;
+  T head_v{}, tail_v{};
+  if (!skip && has_head) head_v = p[tid];
+  if (!skip && has_tail) tail_v = p[sp.tail + tid];
+  Slope s;
+  if (!skip) s = from.of(row, b);
+  const int64_t rel = label - at;
+  const int target = rel >= 0 && rel < static_cast<int64_t>(LANES) * VECS * V ? static_cast<int>(rel) : -1;
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) {
+    Vec16<T> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float y = s.at(Elem<T>::to_f32(v[k].e[i]), (k * LANES + tid) * V + i == target);
       o.e[i] = Elem<T>::from_f32(skip ? 0.0f : y);
     }
-    __builtin_amdgcn_raw_buffer_store_b128(o.raw, out, (k * LANES + tid) * 16, 0, kWriteThrough);
+    __builtin_amdgcn_raw_buffer_store_b128(o.raw, out, (k * LANES + tid) * 16, 0, kWriteThrough);  // dropped behind the chunk
   }
-  if (has_head) g[tid] = value(head_v, tid);
-  if (has_tail) g[tail] = value(tail_v, tail);
+  if (has_head) g[tid] = Elem<T>::from_f32(skip ? 0.0f : s.at(Elem<T>::to_f32(head_v), label == tid));
+  if (has_tail) g[sp.tail + tid] = Elem<T>::from_f32(skip ? 0.0f : s.at(Elem<T>::to_f32(tail_v), label == sp.tail + tid));
 }
 
 // Workspace of a forward call: stats (float2 a row), weight and slope (a float a sequence), which the backward reads;
@@ -421,8 +628,9 @@ uint32_t parts_for(int64_t rows, int64_t vocab, int dtype) {
   return static_cast<uint32_t>(most < 2 ? 1 : (want < most ? want : most));
 }
 
-// Rows up to which one workgroup adds all sequences and forms the loss.
-constexpr int64_t kJoinedRows = 16384;
+// Rows up to which one workgroup does what is left after them: joins their parts, or adds and forms the loss.
+constexpr uint32_t kJoinedRows = 64;
+constexpr uint32_t kSummedRows = 16384;
 
 constexpr int64_t kMaxRows = int64_t{1} << 23;
 constexpr int64_t kMaxBatch = int64_t{1} << 21;
@@ -452,64 +660,96 @@ Rows rows_of(const void* logits, int64_t seq, int64_t batch, int64_t bs, int64_t
 }
 
 template <typename T>
-int run_rows(const char* fn, const Rows& d, uint32_t parts, char* ws, const Layout& at, hipStream_t st) {
-  float2* partial = reinterpret_cast<float2*>(ws + at.partial);
-  float2* stats = reinterpret_cast<float2*>(ws + at.stats);
-  float* tokens = reinterpret_cast<float*>(ws + at.tokens);
+int run_rows(const char* fn, const Rows& d, const Parts& a, hipStream_t st) {
   const int64_t vecs = (static_cast<int64_t>(d.vocab) + Elem<T>::VEC - 1) / Elem<T>::VEC;
-  const auto go = [&](auto kernel, uint32_t groups) {
-    hipLaunchKernelGGL(kernel, dim3((d.rows * parts + groups - 1) / groups), dim3(kThreads), 0, st, d, parts, partial, stats,
-                       tokens);
+  const auto rows_by = [&](auto kernel, uint32_t rows) {
+    hipLaunchKernelGGL(kernel, dim3((d.rows + rows - 1) / rows), dim3(kThreads), 0, st, d, a.stats, a.tokens);
   };
-  if (vecs <= 64) {
-    go(seq_stats_kernel<T, 64, 1>, 4);
+  if (d.vocab >= Elem<T>::VEC && vecs <= 16) {
+    rows_by(seq_stats_tiny_kernel<T, 1>, 16);
+  } else if (d.vocab >= Elem<T>::VEC && vecs <= 48) {
+    rows_by(seq_stats_tiny_kernel<T, 3>, 16);
+  } else if (vecs <= 128) {
+    rows_by(seq_stats_short_kernel<T, 2>, 4);
+  } else if (vecs <= 256) {
+    rows_by(seq_stats_short_kernel<T, 4>, 4);
   } else if (vecs <= 512) {
-    go(seq_stats_kernel<T, 64, 4>, 4);
+    rows_by(seq_stats_short_kernel<T, 8>, 4);
   } else {
-    go(seq_stats_kernel<T, kThreads, 8>, 1);
+    hipLaunchKernelGGL(seq_stats_kernel<T>, dim3(d.rows * a.parts), dim3(kThreads), 0, st, d, a.parts,
+                       const_cast<float2*>(a.partial), a.stats, a.tokens);
   }
-  if (int rc = check_launch(fn)) return rc;
-  if (parts > 1) {
-    hipLaunchKernelGGL(seq_join_kernel<T>, dim3((d.rows + 3) / 4), dim3(kThreads), 0, st, d, parts, partial, stats, tokens);
-    return check_launch(fn);
-  }
-  return PT_OK;
-}
-
-// The rows' statistics and tokens.
-int forward_rows(const char* fn, const Rows& d, uint32_t parts, char* ws, const Layout& at, int dtype, hipStream_t st) {
-  if (d.rows == 0) return PT_OK;
-  if (dtype == PT_FLOAT32) return run_rows<float>(fn, d, parts, ws, at, st);
-  if (dtype == PT_FLOAT16) return run_rows<_Float16>(fn, d, parts, ws, at, st);
-  return run_rows<__bf16>(fn, d, parts, ws, at, st);
-}
-
-SequenceSums sums_of(const Rows& d, int64_t batch, char* ws, const Layout& at, int average, float* log_probs, bool exact) {
-  return SequenceSums{reinterpret_cast<const float*>(ws + at.tokens), d.seq, static_cast<uint32_t>(batch), average, log_probs,
-                      exact ? reinterpret_cast<double*>(ws + at.sums) : nullptr, reinterpret_cast<float*>(ws + at.weight)};
-}
-
-int launch_sums(const char* fn, const SequenceSums& s, hipStream_t st) {
-  hipLaunchKernelGGL(seq_sum_kernel, dim3((s.batch + 3) / 4), dim3(kThreads), 0, st, s);
   return check_launch(fn);
 }
 
 template <typename T>
-int run_grad(const char* fn, const Rows& d, void* grad, int64_t gbs, int64_t gss, const float2* stats, const float* slope,
-             const float* weight, const float* upstream, hipStream_t st) {
+int run_sums(const char* fn, const Rows& d, const Parts& a, const SequenceSums& s, const PairLoss& pl, hipStream_t st) {
+  const bool joins = a.parts > 1;
+  if (joins ? d.rows <= kJoinedRows : (pl.pairs > 0 && d.rows <= kSummedRows)) {
+    hipLaunchKernelGGL(seq_small_kernel<T>, dim3(1), dim3(kSmallThreads), 0, st, d, a, s,
+                       team_of(s.seq, kSmallThreads / 64), pl);
+    return check_launch(fn);
+  }
+  if (joins) {
+    hipLaunchKernelGGL(seq_join_kernel<T>, dim3((d.rows + 3) / 4), dim3(kThreads), 0, st, d, a);
+    if (int rc = check_launch(fn)) return rc;
+  }
+  const uint32_t team = team_of(s.seq, kThreads / 64), per = kThreads / 64 / team;
+  hipLaunchKernelGGL(seq_sum_kernel, dim3((s.batch + per - 1) / per), dim3(kThreads), 0, st, s, team);
+  if (pl.pairs > 0) {
+    if (int rc = check_launch(fn)) return rc;
+    hipLaunchKernelGGL(pair_loss_kernel, dim3(1), dim3(kThreads), 0, st, pl);
+  }
+  return check_launch(fn);
+}
+
+template <typename T>
+int run_forward(const char* fn, const Rows& d, const Parts& a, const SequenceSums& s, const PairLoss& pl, hipStream_t st) {
+  if (d.rows > 0)
+    if (int rc = run_rows<T>(fn, d, a, st)) return rc;
+  return run_sums<T>(fn, d, a, s, pl, st);
+}
+
+int forward(const char* fn, const Rows& d, int64_t batch, uint32_t parts, char* ws, const Layout& at, int average,
+            float* log_probs, PairLoss pl, int dtype, hipStream_t st) {
+  const Parts a{parts, reinterpret_cast<const float2*>(ws + at.partial), reinterpret_cast<float2*>(ws + at.stats),
+                reinterpret_cast<float*>(ws + at.tokens)};
+  const SequenceSums s{a.tokens, d.seq, static_cast<uint32_t>(batch), average, log_probs,
+                       pl.pairs > 0 ? reinterpret_cast<double*>(ws + at.sums) : nullptr,
+                       reinterpret_cast<float*>(ws + at.weight)};
+  pl.y = s.exact;
+  pl.weight = s.weight;
+  pl.slope = reinterpret_cast<float*>(ws + at.slope);
+  if (dtype == PT_FLOAT32) return run_forward<float>(fn, d, a, s, pl, st);
+  if (dtype == PT_FLOAT16) return run_forward<_Float16>(fn, d, a, s, pl, st);
+  return run_forward<__bf16>(fn, d, a, s, pl, st);
+}
+
+template <typename T>
+int run_grad(const char* fn, const Rows& d, void* grad, int64_t gbs, int64_t gss, const SlopeSource& from, hipStream_t st) {
   const int64_t vecs = (static_cast<int64_t>(d.vocab) + Elem<T>::VEC - 1) / Elem<T>::VEC;
-  const auto go = [&](auto kernel, int lanes) {
-    const int64_t per = static_cast<int64_t>(lanes) * kVecs;
-    const int64_t chunks = (vecs + per - 1) / per, items = chunks * d.rows, groups = kThreads / lanes;
+  const auto tiny = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((d.rows + 15) / 16), dim3(kThreads), 0, st, d, static_cast<T*>(grad), gbs, gss, from);
+    return check_launch(fn);
+  };
+  const auto go = [&](auto kernel, int lanes, int each) {
+    // a row's chunks are equally long, whole lines
+    const int64_t most = static_cast<int64_t>(lanes) * each;
+    const int64_t chunks = (vecs + most - 1) / most, per = ((vecs + chunks - 1) / chunks + 7) / 8 * 8;
+    const int64_t items = chunks * d.rows, groups = kThreads / lanes;
     const int64_t blocks = (items + groups - 1) / groups;
     if (items > 0x7fffffffLL || blocks * kThreads > 0xffffffffLL)
       return fail(PT_EUNSUPPORTED, std::string(fn) + ": too many gradient vectors for one launch");
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, d, static_cast<T*>(grad), gbs,
-                       gss, static_cast<uint32_t>(chunks), static_cast<uint32_t>(items), stats, slope, weight, upstream);
+                       gss, static_cast<uint32_t>(chunks), static_cast<uint32_t>(items), static_cast<int>(per), from);
     return check_launch(fn);
   };
-  if (vecs <= 64 * kVecs) return go(seq_grad_kernel<T, 64>, 64);
-  return go(seq_grad_kernel<T, kThreads>, kThreads);
+  if (d.vocab >= Elem<T>::VEC && vecs <= 16) return tiny(seq_grad_tiny_kernel<T, 1>);
+  if (d.vocab >= Elem<T>::VEC && vecs <= 48) return tiny(seq_grad_tiny_kernel<T, 3>);
+  if (vecs <= 128) return go(seq_grad_kernel<T, 64, 2>, 64, 2);
+  if (vecs <= 256) return go(seq_grad_kernel<T, 64, 4>, 64, 4);
+  if (vecs <= 512) return go(seq_grad_kernel<T, kThreads, 2>, kThreads, 2);
+  return go(seq_grad_kernel<T, kThreads, 4>, kThreads, 4);
 }
 
 }  // namespace
@@ -537,10 +777,8 @@ int pt_sequence_log_probs(const void* logits, int64_t batch, int64_t seq, int64_
   const Layout at(batch, seq, parts);
   const Rows d = rows_of(logits, seq, batch, batch_stride, seq_stride, vocab, labels, l_batch_stride, l_seq_stride, shift,
                          ignore_index);
-  char* ws = static_cast<char*>(workspace);
-  hipStream_t st = as_stream(stream);
-  if (int frc = forward_rows(fn, d, parts, ws, at, dtype, st)) return frc;
-  return launch_sums(fn, sums_of(d, batch, ws, at, average, log_probs, false), st);
+  return forward(fn, d, batch, parts, static_cast<char*>(workspace), at, average, log_probs, PairLoss{}, dtype,
+                 as_stream(stream));
 }
 
 int pt_preference_loss(const void* logits, int64_t pairs, int64_t seq, int64_t batch_stride, int64_t seq_stride,
@@ -563,18 +801,9 @@ int pt_preference_loss(const void* logits, int64_t pairs, int64_t seq, int64_t b
   char* ws = static_cast<char*>(workspace);
   const Rows d = rows_of(logits, seq, batch, batch_stride, seq_stride, vocab, labels, l_batch_stride, l_seq_stride, shift,
                          ignore_index);
-  hipStream_t st = as_stream(stream);
-  if (int frc = forward_rows(fn, d, parts, ws, at, dtype, st)) return frc;
-  const SequenceSums sums = sums_of(d, batch, ws, at, average, log_probs, true);
-  const PairLoss pl{sums.exact, reference, static_cast<uint32_t>(pairs), beta, label_smoothing, kind, sums.weight, loss,
-                    rewards, reinterpret_cast<float*>(ws + at.slope)};
-  if (batch * seq <= kJoinedRows) {
-    hipLaunchKernelGGL(pair_sum_kernel, dim3(1), dim3(kJoinedThreads), 0, st, sums, pl);
-    return check_launch(fn);
-  }
-  if (int frc = launch_sums(fn, sums, st)) return frc;
-  hipLaunchKernelGGL(pair_loss_kernel, dim3(1), dim3(kThreads), 0, st, pl);
-  return check_launch(fn);
+  const PairLoss pl{nullptr, reference, static_cast<uint32_t>(pairs), beta, label_smoothing, kind, nullptr, loss, rewards,
+                    nullptr};
+  return forward(fn, d, batch, parts, ws, at, average, log_probs, pl, dtype, as_stream(stream));
 }
 
 int pt_sequence_log_probs_bwd(const void* logits, int64_t batch, int64_t seq, int64_t batch_stride, int64_t seq_stride,
@@ -603,16 +832,14 @@ int pt_sequence_log_probs_bwd(const void* logits, int64_t batch, int64_t seq, in
   const char* ws = static_cast<const char*>(workspace);
   const Rows d = rows_of(logits, seq, batch, batch_stride, seq_stride, vocab, labels, l_batch_stride, l_seq_stride, shift,
                          ignore_index);
-  const float2* stats = reinterpret_cast<const float2*>(ws + at.stats);
   // the pairs' slopes hold the averages' weights already
-  const float* slope = grad_log_probs ? grad_log_probs : reinterpret_cast<const float*>(ws + at.slope);
-  const float* weight = grad_log_probs ? reinterpret_cast<const float*>(ws + at.weight) : nullptr;
+  const SlopeSource from{reinterpret_cast<const float2*>(ws + at.stats),
+                         grad_log_probs ? grad_log_probs : reinterpret_cast<const float*>(ws + at.slope),
+                         grad_log_probs ? reinterpret_cast<const float*>(ws + at.weight) : nullptr, grad_loss};
   hipStream_t st = as_stream(stream);
-  if (dtype == PT_FLOAT32)
-    return run_grad<float>(fn, d, grad, g_batch_stride, g_seq_stride, stats, slope, weight, grad_loss, st);
-  if (dtype == PT_FLOAT16)
-    return run_grad<_Float16>(fn, d, grad, g_batch_stride, g_seq_stride, stats, slope, weight, grad_loss, st);
-  return run_grad<__bf16>(fn, d, grad, g_batch_stride, g_seq_stride, stats, slope, weight, grad_loss, st);
+  if (dtype == PT_FLOAT32) return run_grad<float>(fn, d, grad, g_batch_stride, g_seq_stride, from, st);
+  if (dtype == PT_FLOAT16) return run_grad<_Float16>(fn, d, grad, g_batch_stride, g_seq_stride, from, st);
+  return run_grad<__bf16>(fn, d, grad, g_batch_stride, g_seq_stride, from, st);
 }
 
 }  // extern "C"
