@@ -275,26 +275,47 @@ void launch_at(const AtAngles& an, AtRow row, AtView (&v)[2], hipStream_t st) {
     blocks += t.blocks;
   }
   if (blocks == 0) return;
-  // streams larger than the caches are touched once
+  // Streams larger than the caches are touched once: nontemporal -- but not where an item's two vectors lie in halves that are
+  // no whole lines, whose other parts another access fetches (us: 160 MB of bf16 heads of 96 60.9 nontemporal, 45.0
+  // not; of 80 elements, half of them rotated, in 270 MB 104.6 and 81.1; 128, a quarter, 77.8 and 62.9; whole lines, 128 rotated,
+  // 55.9 and 61.2).
+  constexpr int kLine = 128;
   const int64_t bytes = rows * row.head_dim * static_cast<int64_t>(sizeof(T));
-  const auto kernel = bytes > kNontemporalBytes ? rope_at_kernel<T, LAYOUT, VEC, true, U> : rope_at_kernel<T, LAYOUT, VEC, false, U>;
+  const bool lines = LAYOUT == 0 || (half * static_cast<int>(sizeof(T)) % kLine == 0 &&
+                                     row.head_dim * static_cast<int>(sizeof(T)) % kLine == 0);
+  auto kernel = rope_at_kernel<T, LAYOUT, VEC, false, U>;
+  if constexpr (!VEC || U > 2 - LAYOUT) {  // calls of fewer heads an item are smaller than that
+    if (lines && bytes > kNontemporalBytes) kernel = rope_at_kernel<T, LAYOUT, VEC, true, U>;
+  }
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, an, row, v[0].t, v[1].t);
 }
 
 template <typename T>
 void launch_layout(int layout, const AtAngles& an, const AtRow& row, AtView (&v)[2], hipStream_t st) {
+  // Heads of an item, by the call's vectors.  The angles of an item cost as much arithmetic as the rotation of four heads;
+  // what few items there are of a small call would only lengthen.  us, one / two / four heads: 335 MB of bf16 heads of 128
+  // interleaved 85.3 / 59.7 / 55.9, rotate-half 71.8 / 56.0 / 57.3; 1.3e6 vectors interleaved 13.3 / 11.5 / 10.5, rotate-half
+  // 11.9 / 10.2 / 10.6; 164000 4.5 / 4.4 / 4.8; 10240 3.8 / 4.1 / 4.4.
   constexpr int V = Elem<T>::VEC;
+  constexpr int64_t kTwoHeads = 65536, kFourHeads = int64_t{1} << 20;
   const int rest = row.head_dim - row.rotary;
+  const int64_t vectors = (v[0].rows + v[1].rows) * row.head_dim / V;
   if (layout == 0) {
     if (row.head_dim < V) {
       launch_at<T, 0, false, 1>(an, row, v, st);
-    } else {
+    } else if (vectors < kTwoHeads) {
       launch_at<T, 0, true, 1>(an, row, v, st);
+    } else if (vectors < kFourHeads) {
+      launch_at<T, 0, true, 2>(an, row, v, st);
+    } else {
+      launch_at<T, 0, true, 4>(an, row, v, st);
     }
   } else if (row.rotary / 2 < V || (rest > 0 && rest < V)) {
     launch_at<T, 1, false, 1>(an, row, v, st);
-  } else {
+  } else if (vectors < kTwoHeads) {
     launch_at<T, 1, true, 1>(an, row, v, st);
+  } else {
+    launch_at<T, 1, true, 2>(an, row, v, st);
   }
 }
 
