@@ -262,6 +262,10 @@ def _bind_native(lib: ctypes.CDLL) -> None:
         pt_swiglu_fwd=native.swiglu_fwd,
         pt_swiglu_bwd=native.swiglu_bwd,
         pt_rope=native.rope,
+        pt_rope_at=native.rope_at,
+        pt_sequence_log_probs=native.sequence_log_probs,
+        pt_preference_loss=native.preference_loss,
+        pt_sequence_log_probs_bwd=native.sequence_log_probs_bwd,
         pt_cross_entropy=native.cross_entropy,
         pt_cross_entropy_shifted=native.cross_entropy,
         pt_cross_entropy_scale_grad=native.cross_entropy_scale_grad,

@@ -18,6 +18,7 @@
 #include <ATen/ATen.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -31,7 +32,9 @@ namespace {
   X(pt_residual_rmsnorm_fwd) X(pt_residual_rmsnorm_bwd) X(pt_swiglu_fwd) X(pt_swiglu_bwd)     \
   X(pt_rope) X(pt_cross_entropy_workspace_bytes) X(pt_cross_entropy)                          \
   X(pt_cross_entropy_shifted) X(pt_cross_entropy_scale_grad)                                  \
-  X(pt_cross_entropy_shifted_scale_grad)
+  X(pt_cross_entropy_shifted_scale_grad) X(pt_rope_at)                                        \
+  X(pt_sequence_log_probs_workspace_bytes) X(pt_sequence_log_probs) X(pt_preference_loss)     \
+  X(pt_sequence_log_probs_bwd)
 #define PT_DECLARE(f) decltype(&f) p_##f = nullptr;
 PT_NATIVE_FNS(PT_DECLARE)
 #undef PT_DECLARE
@@ -320,6 +323,52 @@ PT_FN(rope, 7)
   return tuple(y0, y1);
 PT_END
 
+// As ops._rope_at_out.
+at::Tensor rope_at_out(const at::Tensor& x) {
+  at::Tensor y = at::empty_like(x);
+  return y.stride(3) == 1 ? y : at::empty(x.sizes(), x.options());
+}
+
+// (x0, x1 or None, turns, positions or None, offset, scale, layout, inverse, stream) -> (y0, y1 or None)
+PT_FN(rope_at, 9)
+  const at::Tensor *x0 = plain(a[0]), *g = plain(a[2]);
+  const at::Tensor* x1 = a[1] == Py_None ? nullptr : plain(a[1]);
+  const at::Tensor* p = a[3] == Py_None ? nullptr : plain(a[3]);
+  int64_t offset, layout;
+  double scale;
+  if (x0 == nullptr || g == nullptr || x0->dim() != 4 || code_of(*x0) < 0 || !rope_state(x0, *x0, x0->size(3)) ||
+      (a[1] != Py_None && (!rope_state(x1, *x0, x0->size(3)) || x1->size(0) != x0->size(0) || x1->size(2) != x0->size(2))) ||
+      g->dim() != 1 || g->scalar_type() != at::kLong || !g->is_contiguous() || !same_place(*g, *x0) ||
+      g->size(0) * 2 > x0->size(3) || !as_i64(a[4], &offset) || !as_f64(a[5], &scale) || !as_i64(a[6], &layout))
+    return none();
+  int64_t pbs = 0, pss = 0;
+  int width = 0;
+  if (a[3] != Py_None) {
+    if (p == nullptr || !same_place(*p, *x0)) return none();
+    width = p->scalar_type() == at::kLong ? 8 : (p->scalar_type() == at::kInt ? 4 : 0);
+    const int64_t seq = x0->size(2);
+    if (width == 0 || p->dim() < 1 || p->dim() > 2 || p->size(-1) != seq) return none();
+    if (p->dim() == 2 && p->size(0) != 1 && p->size(0) != x0->size(0)) return none();
+    pss = p->stride(-1);
+    if (p->dim() == 2 && p->size(0) > 1) pbs = p->stride(0);
+  }
+  void* const stream = as_stream(a[8]);
+  NoGil nogil;
+  at::Tensor y0 = rope_at_out(*x0);
+  std::optional<at::Tensor> y1;
+  if (x1 != nullptr) y1 = rope_at_out(*x1);
+  int64_t d0[9], d1[9];
+  rope_desc(*x0, y0, d0);
+  if (x1 != nullptr) rope_desc(*x1, *y1, d1);
+  const int rc = p_pt_rope_at(in(*x0), out(y0), d0, x1 ? in(*x1) : nullptr, x1 ? out(*y1) : nullptr,
+                              x1 ? d1 : nullptr, x0->size(3), 2 * g->size(0), p ? in(*p) : nullptr, width, pbs, pss,
+                              offset, static_cast<const uint64_t*>(in(*g)), static_cast<float>(scale),
+                              static_cast<int>(layout), a[7] == Py_True ? 1 : 0, code_of(*x0), stream);
+  nogil.end();
+  if (rc != PT_OK) return PyLong_FromLong(rc);
+  return tuple(y0, y1);
+PT_END
+
 // ------------------------------------------------------------------ cross-entropy
 
 // The rows of a logits tensor and its targets, in the C ABI's terms: outer x inner rows of `vocab`
@@ -482,6 +531,94 @@ PT_FN(cross_entropy_scale_grad, 8)
   Py_RETURN_TRUE;
 PT_END
 
+// ------------------------------------------------------------------ preference loss
+
+// (batch, seq, vocab) logits with a contiguous vocabulary and their (batch, seq) labels.
+bool sequences(const at::Tensor* x, const at::Tensor* y) {
+  return x != nullptr && y != nullptr && x->dim() == 3 && x->stride(2) == 1 && code_of(*x) >= 0 &&
+         y->scalar_type() == at::kLong && y->dim() == 2 && y->size(0) == x->size(0) && y->size(1) == x->size(1) &&
+         same_place(*x, *y);
+}
+
+at::Tensor sequence_workspace(const at::Tensor& x, size_t* bytes) {
+  *bytes = p_pt_sequence_log_probs_workspace_bytes(x.size(0), x.size(1), x.size(2), code_of(x));
+  return at::empty({static_cast<int64_t>(*bytes < 16 ? 16 : *bytes)}, x.options().dtype(at::kByte));
+}
+
+#define PT_SEQUENCES(x, y) \
+  x->size(1), x->stride(0), x->stride(1), x->size(2), static_cast<const int64_t*>(in(*y)), y->stride(0), y->stride(1)
+
+// (logits, labels, shift, ignore_index, average, stream) -> (log_probs, workspace)
+PT_FN(sequence_log_probs, 6)
+  const at::Tensor *x = plain(a[0]), *y = plain(a[1]);
+  int64_t ignore;
+  if (!sequences(x, y) || !as_i64(a[3], &ignore)) return none();
+  void* const stream = as_stream(a[5]);
+  NoGil nogil;
+  size_t bytes;
+  at::Tensor ws = sequence_workspace(*x, &bytes);
+  at::Tensor lp = at::empty({x->size(0)}, x->options().dtype(at::kFloat));
+  const int rc = p_pt_sequence_log_probs(in(*x), x->size(0), PT_SEQUENCES(x, y), a[2] == Py_True ? 1 : 0, ignore,
+                                         a[4] == Py_True ? 1 : 0, static_cast<float*>(out(lp)), out(ws), bytes, code_of(*x),
+                                         stream);
+  nogil.end();
+  if (rc != PT_OK) return PyLong_FromLong(rc);
+  return tuple(lp, ws);
+PT_END
+
+// (logits, labels, reference or None, beta, label_smoothing, kind, shift, ignore_index, average, stream) ->
+// (loss, rewards, log_probs, workspace)
+PT_FN(preference_loss, 10)
+  const at::Tensor *x = plain(a[0]), *y = plain(a[1]);
+  const at::Tensor* r = a[2] == Py_None ? nullptr : plain(a[2]);
+  double beta, smooth;
+  int64_t kind, ignore;
+  if (!sequences(x, y) || x->size(0) % 2 != 0 || !as_f64(a[3], &beta) || !as_f64(a[4], &smooth) || !as_i64(a[5], &kind) ||
+      !as_i64(a[7], &ignore) ||
+      (a[2] != Py_None && (r == nullptr || r->scalar_type() != at::kFloat || r->dim() != 1 || r->size(0) != x->size(0) ||
+                           !r->is_contiguous() || !same_place(*r, *x))))
+    return none();
+  void* const stream = as_stream(a[9]);
+  NoGil nogil;
+  size_t bytes;
+  at::Tensor ws = sequence_workspace(*x, &bytes);
+  const auto f32 = x->options().dtype(at::kFloat);
+  at::Tensor loss = at::empty({}, f32), rewards = at::empty({x->size(0)}, f32), lp = at::empty({x->size(0)}, f32);
+  const int rc = p_pt_preference_loss(in(*x), x->size(0) / 2, PT_SEQUENCES(x, y), a[6] == Py_True ? 1 : 0, ignore,
+                                      a[8] == Py_True ? 1 : 0, r ? static_cast<const float*>(in(*r)) : nullptr,
+                                      static_cast<float>(beta), static_cast<float>(smooth), static_cast<int>(kind),
+                                      static_cast<float*>(out(loss)), static_cast<float*>(out(rewards)),
+                                      static_cast<float*>(out(lp)), out(ws), bytes, code_of(*x), stream);
+  nogil.end();
+  if (rc != PT_OK) return PyLong_FromLong(rc);
+  return tuple(loss, rewards, lp, ws);
+PT_END
+
+// (logits, labels, workspace, gradient of the log-probabilities or the loss, of the loss, shift, ignore_index, stream) ->
+// gradient of the logits
+PT_FN(sequence_log_probs_bwd, 8)
+  const at::Tensor *x = plain(a[0]), *y = plain(a[1]), *ws = plain(a[2]), *up = plain(a[3]);
+  int64_t ignore;
+  const bool of_loss = a[4] == Py_True;
+  if (!sequences(x, y) || !as_i64(a[6], &ignore) || ws == nullptr || !same_place(*ws, *x) || !ws->is_contiguous() ||
+      ws->scalar_type() != at::kByte || up == nullptr || !same_place(*up, *x) || up->scalar_type() != at::kFloat ||
+      !up->is_contiguous() || up->numel() != (of_loss ? 1 : x->size(0)) ||
+      !rows_disjoint(x->size(0), x->stride(0), x->size(1), x->stride(1), x->size(2)))
+    return none();
+  const size_t bytes = p_pt_sequence_log_probs_workspace_bytes(x->size(0), x->size(1), x->size(2), code_of(*x));
+  if (static_cast<size_t>(ws->numel()) < bytes) return none();
+  void* const stream = as_stream(a[7]);
+  NoGil nogil;
+  const at::Tensor grad = grad_buffer(*x);
+  const float* g = static_cast<const float*>(in(*up));
+  const int rc = p_pt_sequence_log_probs_bwd(in(*x), x->size(0), PT_SEQUENCES(x, y), a[5] == Py_True ? 1 : 0, ignore,
+                                             of_loss ? nullptr : g, of_loss ? g : nullptr, out(grad), grad.stride(0),
+                                             grad.stride(1), in(*ws), bytes, code_of(*x), stream);
+  nogil.end();
+  if (rc != PT_OK) return PyLong_FromLong(rc);
+  return wrap(grad);
+PT_END
+
 // ------------------------------------------------------------------ AdamW
 
 // A contiguous fp32 GPU tensor.
@@ -593,6 +730,84 @@ PT_FN(adamw_scan, 3)
                        bytes(grads), list.get());
 PT_END
 
+// Uint8 bytes of a moment: `bytes` of them, contiguous, on p's device; its address, or 0.
+int64_t moment_bytes(PyObject* o, const at::Tensor& p, std::initializer_list<int64_t> shape, int64_t align) {
+  const at::Tensor* t = o != nullptr ? plain(o) : nullptr;
+  if (t == nullptr || t->scalar_type() != at::kByte || !t->is_contiguous() || t->device() != p.device() ||
+      t->sizes() != at::IntArrayRef(shape))
+    return 0;
+  const int64_t address = reinterpret_cast<int64_t>(out(*t));
+  return address % align == 0 ? address : 0;
+}
+
+// adamw8_scan([params, ...] per group, optimizer.state, elements per table block, elements per scale) ->
+// (device index, [(table, rows, blocks, step, steps, dtype code) or None, ...])
+// for parameters with 8-bit moments that all have their state in place, one dtype and one host step count a group: the
+// record table of each group's step as bytes (None for a group without gradients).  None for anything else.
+PT_FN(adamw8_scan, 4)
+  int64_t per, quant;
+  if (!PyList_Check(a[0]) || !PyDict_Check(a[1]) || !as_i64(a[2], &per) || !as_i64(a[3], &quant) || per <= 0 || quant <= 0)
+    return none();
+  THPObjectPtr list{PyList_New(0)};
+  if (!list) return nullptr;
+  c10::Device device(c10::kCPU);
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i) {
+    PyObject* params = PyList_GET_ITEM(a[0], i);
+    if (!PyList_Check(params)) return none();
+    std::vector<int64_t> rows;
+    int64_t blocks = 0;
+    float step = 0.0f;
+    int code = -1;
+    THPObjectPtr steps{PyList_New(0)};
+    if (!steps) return nullptr;
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(params); ++k) {
+      THPObjectPtr held = owned(PyList_GET_ITEM(params, k));  // (the state's lookup runs Python: see adamw_scan)
+      PyObject* o = held.get();
+      if (!THPVariable_CheckExact(o)) return none();
+      const at::Tensor grad = THPVariable_Unpack(o).grad();
+      if (!grad.defined()) continue;
+      const at::Tensor* p = plain(o);
+      if (p == nullptr || code_of(*p) < 0 || !p->is_contiguous() || grad.layout() != at::kStrided ||
+          grad.scalar_type() != p->scalar_type() || !grad.is_contiguous() || !grad.has_storage() ||
+          grad.device() != p->device() || grad.numel() != p->numel() || grad.is_neg() || grad.storage().data() == nullptr)
+        return none();
+      THPObjectPtr entry = owned(PyDict_GetItemWithError(a[1], o));
+      PyObject* state = entry.get();
+      if (state == nullptr || !PyDict_Check(state)) {
+        PyErr_Clear();
+        return none();
+      }
+      const int64_t n = p->numel(), scales = (n + quant - 1) / quant;
+      const int64_t mc = moment_bytes(item(state, "exp_avg"), *p, {scales, quant}, 4);
+      const int64_t ms = moment_bytes(item(state, "exp_avg_scale"), *p, {scales}, 1);
+      const int64_t vc = moment_bytes(item(state, "exp_avg_sq"), *p, {scales, quant}, 4);
+      const int64_t vs = moment_bytes(item(state, "exp_avg_sq_scale"), *p, {scales}, 1);
+      PyObject* so = item(state, "step");
+      const float* count = host_step(so);
+      if (mc == 0 || ms == 0 || vc == 0 || vs == 0 || count == nullptr) return none();
+      if (device.is_cpu()) device = p->device();
+      if (p->device() != device || (!rows.empty() && (*count != step || code_of(*p) != code))) return none();
+      step = *count;
+      code = code_of(*p);
+      if (PyList_Append(steps, so) != 0) return nullptr;
+      rows.insert(rows.end(), {reinterpret_cast<int64_t>(out(*p)), reinterpret_cast<int64_t>(out(grad)), mc, ms, vc, vs, n, blocks});
+      blocks += (n + per - 1) / per;
+    }
+    if (rows.empty()) {
+      if (PyList_Append(list, Py_None) != 0) return nullptr;
+      continue;
+    }
+    THPObjectPtr entry{Py_BuildValue("(NnLdOi)",
+                                     PyBytes_FromStringAndSize(reinterpret_cast<const char*>(rows.data()),
+                                                               static_cast<Py_ssize_t>(rows.size() * sizeof(int64_t))),
+                                     static_cast<Py_ssize_t>(rows.size() / 8), static_cast<long long>(blocks),
+                                     static_cast<double>(step), steps.get(), code)};
+    if (!entry || PyList_Append(list, entry.get()) != 0) return nullptr;
+  }
+  if (device.is_cpu()) return none();
+  return Py_BuildValue("(iO)", static_cast<int>(device.index()), list.get());
+PT_END
+
 // Adds 1 to each fp32 host step tensor of a list, as `step += 1` does.
 PT_FN(advance_steps, 1)
   if (!PyList_Check(a[0])) {
@@ -642,7 +857,12 @@ PyMethodDef methods[] = {PT_METHOD(rmsnorm_fwd),
                          PT_METHOD(ce_grad_buffer),
                          PT_METHOD(cross_entropy),
                          PT_METHOD(cross_entropy_scale_grad),
+                         PT_METHOD(rope_at),
+                         PT_METHOD(sequence_log_probs),
+                         PT_METHOD(preference_loss),
+                         PT_METHOD(sequence_log_probs_bwd),
                          PT_METHOD(adamw_scan),
+                         PT_METHOD(adamw8_scan),
                          PT_METHOD(advance_steps),
                          PT_METHOD(bind),
                          {nullptr, nullptr, 0, nullptr}};

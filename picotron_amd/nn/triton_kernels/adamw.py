@@ -120,7 +120,7 @@ def _check_state(state: dict, p: Tensor, capturable: bool = False) -> None:
                           f"({tuple(m.shape)} for {tuple(p.shape)}, or not contiguous)")
 
 
-_table_cache: dict[tuple, Tensor] = {}
+_table_cache: dict[tuple, tuple[Tensor, int]] = {}  # the table and the stream that it was copied on
 _TABLE_CACHE_SIZE = 16
 _table_lock = threading.Lock()  # optimizers may step from several threads at once
 # Tables used while a stream is being captured into a graph: the graph's kernels read them
@@ -144,8 +144,9 @@ def _device_bytes(table: bytes, shape: tuple[int, ...], device: torch.device) ->
 
     key = (device, table)
     capturing = torch.cuda.is_current_stream_capturing()
+    stream = ops._stream(device)
     with _table_lock:
-        cached = _table_cache.pop(key, None)
+        cached, owner = _table_cache.pop(key, (None, stream))
     if cached is None:
         if capturing:
             raise TritonAdamWUnavailable(
@@ -153,10 +154,12 @@ def _device_bytes(table: bytes, shape: tuple[int, ...], device: torch.device) ->
                 "same call once before capturing it.")
         host = torch.frombuffer(bytearray(table), dtype=torch.int64).reshape(shape)
         cached = host.pin_memory().to(device, non_blocking=True)
+    elif owner != stream and not capturing:
+        cached.record_stream(torch.cuda.current_stream(device))  # not reused after an eviction while this one reads it
     with _table_lock:
         if capturing:
             _captured_tables.append(cached)
-        _table_cache[key] = cached  # most recent last
+        _table_cache[key] = cached, owner  # most recent last
         while len(_table_cache) > _TABLE_CACHE_SIZE:
             del _table_cache[next(iter(_table_cache))]
     return cached
@@ -376,11 +379,7 @@ def _plan_8bit(optimizer: AdamW8bit) -> tuple[list[tuple[dict, list[Tensor]]], t
     groups, device, blocks = [], None, 0
     state_of = optimizer.state
     for group in optimizer.param_groups:
-        for key in ("lr", "eps", "weight_decay"):
-            if isinstance(group[key], Tensor):
-                raise _reject(f"tensor-valued {key}")
-        if any(isinstance(b, Tensor) for b in group["betas"]):
-            raise _reject("tensor-valued betas")
+        _check_group_8bit(group)
         params = [p for p in group["params"] if p.grad is not None]
         for p in params:
             g = p.grad
@@ -423,19 +422,61 @@ def _require_library(device: torch.device) -> None:
         raise _reject("devices other than gfx950")
 
 
+_DTYPES = {code: dtype for dtype, code in ops._DTYPE_CODES.items()}
+
+
+def _scan_8bit(optimizer: AdamW8bit) -> tuple[torch.device, list] | None:
+    """The launches of :func:`_run_8bit` from one native pass, for the usual step (every state in place, host step
+    counts, a dtype and a count a group); None for anything else."""
+
+    native = _lib.extension() if _lib.is_available() else None
+    if native is None:
+        return None
+    groups = optimizer.param_groups
+    for group in groups:
+        _check_group_8bit(group)
+        if group["capturable"]:
+            return None
+    found = native.adamw8_scan([group["params"] for group in groups], optimizer.state, *ops.adamw8_sizes())
+    if found is None:
+        return None
+    index, tables = found
+    kept = [(group, *table) for group, table in zip(groups, tables) if table is not None]
+    if sum(blocks for _, _, _, blocks, *_ in kept) * 256 > 0xFFFFFFFF or not ops.device_supported(index):
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    device = torch.device("cuda", index)
+    return device, [(_device_bytes(table, (rows, 8), device), blocks, _DTYPES[code], steps, group, step,
+                     optimizer.bucket_seed(group, i))
+                    for i, (group, table, rows, blocks, step, steps, code) in enumerate(kept)]
+
+
+def _check_group_8bit(group: dict) -> None:
+    for key in ("lr", "eps", "weight_decay"):
+        if isinstance(group[key], Tensor):
+            raise _reject(f"tensor-valued {key}")
+    if any(isinstance(b, Tensor) for b in group["betas"]):
+        raise _reject("tensor-valued betas")
+
+
 def _run_8bit(optimizer: AdamW8bit, groups, device: torch.device, grad_scale: Tensor | None = None) -> None:
     launches = []
     for group, params, states, step, seed in optimizer.buckets(groups):
         host_table, blocks = ops.adamw8_table(params, [p.grad for p in params], states)
-        launches.append((_device_table(host_table, device), blocks, params[0].dtype, states, group, step, seed))
+        launches.append((_device_table(host_table, device), blocks, params[0].dtype, [state["step"] for state in states],
+                         group, step, seed))
     _committed(_launch_8bit, launches, grad_scale)
 
 
 def _launch_8bit(launches: list, grad_scale: Tensor | None) -> None:
-    for table, blocks, dtype, states, group, step, seed in launches:
+    for table, blocks, dtype, steps, group, step, seed in launches:
         if not isinstance(step, Tensor):
             step = _next_step(step)
-            torch._foreach_add_([state["step"] for state in states], 1.0)
+            if _lib.native is not None and all(s.is_cpu and s.dtype == torch.float32 for s in steps):
+                _lib.native.advance_steps(steps)
+            else:
+                torch._foreach_add_(steps, 1.0)
         beta1, beta2 = group["betas"]
         ops.adamw8_step(table, blocks, dtype, lr=group["lr"], beta1=beta1, beta2=beta2, eps=group["eps"],
                         weight_decay=group["weight_decay"], step=step, seed=seed,
@@ -447,6 +488,10 @@ def triton_adamw_step(optimizer: Optimizer) -> None:
     kernel (or raise unavailable)."""
 
     if isinstance(optimizer, AdamW8bit):
+        scan = _scan_8bit(optimizer)
+        if scan is not None:
+            _committed(_launch_8bit, scan[1], None)
+            return
         groups, device = _plan_8bit(optimizer)
         if device is not None:
             _run_8bit(optimizer, groups, device)
@@ -490,7 +535,11 @@ def triton_clip_grad_norm_and_step(
 
 
 def _clip_and_step_8bit(optimizer: AdamW8bit, max_norm: float, write_back_grads: bool) -> Tensor:
-    groups, device = _plan_8bit(optimizer)
+    scan = _scan_8bit(optimizer)
+    if scan is None:
+        groups, device = _plan_8bit(optimizer)
+    else:
+        groups, device = optimizer._with_gradients(), scan[0]
     grads, _ = _grads_of(p for _, params in groups for p in params)  # fp32 ones, or refused
     if device is None:
         return torch.tensor(0.0)
@@ -499,7 +548,10 @@ def _clip_and_step_8bit(optimizer: AdamW8bit, max_norm: float, write_back_grads:
     if write_back_grads:
         _committed(ops.grad_scale, table, blocks, coef)
         coef = None
-    _run_8bit(optimizer, groups, device, coef)
+    if scan is None:
+        _run_8bit(optimizer, groups, device, coef)
+    else:
+        _committed(_launch_8bit, scan[1], coef)
     return total_norm
 
 

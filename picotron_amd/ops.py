@@ -94,10 +94,21 @@ def _check_cuda(*tensors: Tensor) -> torch.device:
     return device
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch_here(fn: str, first: Tensor, *args):
+    """:func:`_launch`, for tensors on the current device (None for others)."""
+
+    if not first.is_cuda or first.device.index != _current_device():
+        return None
+    return _launch(fn, first, *args)
+
+
 def _call_on(device: torch.device, fn: str, *args) -> None:
     """:func:`_lib.raw_call` with ``device`` the current one, which a launch on its stream needs."""
 
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _current_device():
         _lib.raw_call(fn, *args, _stream(device))
     else:
         with torch.cuda.device(device):
@@ -396,6 +407,13 @@ def rope(
     return outs[0], (outs[1] if x1 is not None else None)
 
 
+def _rope_at_out(x: Tensor) -> Tensor:
+    """A new tensor like ``x`` with a contiguous head_dim (which empty_like moves outwards for windows that overlap)."""
+
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _position_strides(positions: Tensor | None, batch: int, seq: int) -> tuple[int, int]:
     """(batch stride, sequence stride) of (seq,), (1, seq) or (batch, seq) positions."""
 
@@ -437,6 +455,10 @@ def rope_at(
             return torch.ops.picotron_amd.rope_at(x0, turns, positions, offset, scale, layout, bool(inverse)), None
         y0, y1 = torch.ops.picotron_amd.rope_at_pair(x0, x1, turns, positions, offset, scale, layout, bool(inverse))
         return y0, y1
+    if layout in LAYOUTS:
+        out = _launch_here("pt_rope_at", x0, x1, turns, positions, offset, scale, LAYOUTS[layout], bool(inverse))
+        if out is not None:
+            return out
     tensors = [x0] if x1 is None else [x0, x1]
     device = _check_cuda(*tensors, turns, *([] if positions is None else [positions]))
     if layout not in LAYOUTS:
@@ -453,7 +475,7 @@ def rope_at(
     if not -(1 << 63) <= offset < 1 << 63:
         raise ValueError("the RoPE position offset must fit 64 bits")
     pbs, pss = _position_strides(positions, x0.size(0), x0.size(2))
-    outs = [torch.empty_like(t) for t in tensors]
+    outs = [_rope_at_out(t) for t in tensors]
     descs = [_rope_desc(t, o) for t, o in zip(tensors, outs)]
     _call_on(
         device,
@@ -743,6 +765,9 @@ def sequence_log_probs(
 ) -> tuple[Tensor, Tensor]:
     """(log-probability of each sequence's kept labels, fp32; workspace for :func:`sequence_log_probs_bwd`)."""
 
+    out = _launch_here("pt_sequence_log_probs", logits, labels, bool(shift), ignore_index, bool(average))
+    if out is not None:
+        return out
     device = _check_cuda(logits, labels)
     rows = _sequence_rows(logits, labels, shift)
     ws, size = _sequence_workspace(logits)
@@ -759,6 +784,11 @@ def preference_loss(
     """(loss, rewards, log-probabilities, workspace) over logits whose first half of sequences are the chosen ones of
     the pairs and whose second half the rejected ones; ``reference``: fp32 log-probabilities, or None for zeros."""
 
+    if kind in PREFERENCE_LOSSES:
+        out = _launch_here("pt_preference_loss", logits, labels, reference, beta, label_smoothing, PREFERENCE_LOSSES[kind],
+                           bool(shift), ignore_index, bool(average))
+        if out is not None:
+            return out
     device = _check_cuda(logits, labels, *([] if reference is None else [reference]))
     rows = _sequence_rows(logits, labels, shift)
     batch = logits.size(0)
@@ -787,6 +817,10 @@ def sequence_log_probs_bwd(
     forward left ``workspace``."""
 
     up = grad_log_probs if grad_log_probs is not None else grad_loss
+    grad = _launch_here("pt_sequence_log_probs_bwd", logits, labels, workspace, up, grad_log_probs is None, bool(shift),
+                        ignore_index)
+    if grad is not None:
+        return grad
     device = _check_cuda(logits, labels, workspace, up)
     grad = ce_grad_buffer(logits, 2)
     if grad is None:  # rows that overlap in memory (an expanded tensor)
@@ -967,6 +1001,7 @@ def adamw_step_device_step(
 _ADAMW8_STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
 
 
+@functools.lru_cache(maxsize=None)
 @functools.lru_cache(maxsize=None)
 def adamw8_sizes() -> tuple[int, int]:
     """(elements of a table block, elements that share a scale) of the AdamW step with 8-bit moments."""
@@ -1241,7 +1276,7 @@ def _op_rope_at(x: Tensor, turns: Tensor, positions: Tensor | None, offset: int,
 
 @_op_rope_at.register_fake
 def _(x, turns, positions, offset, scale, layout, inverse):
-    return torch.empty_like(x)
+    return _rope_at_out(x)
 
 
 @torch.library.custom_op("picotron_amd::rope_at_pair", mutates_args=())
@@ -1253,4 +1288,4 @@ def _op_rope_at_pair(x0: Tensor, x1: Tensor, turns: Tensor, positions: Tensor | 
 
 @_op_rope_at_pair.register_fake
 def _(x0, x1, turns, positions, offset, scale, layout, inverse):
-    return torch.empty_like(x0), torch.empty_like(x1)
+    return _rope_at_out(x0), _rope_at_out(x1)

@@ -164,8 +164,14 @@ class AdamW8bit(Optimizer):
                 states.append(state)
             for (_, _, step), (ps, states) in shared.items():
                 value = states[0]["step"] if group["capturable"] else step
-                found.append((group, ps, states, value, (group["seed"] + 0x632BE5AB * len(found)) & _MASK))
+                found.append((group, ps, states, value, self.bucket_seed(group, len(found))))
         return found
+
+    @staticmethod
+    def bucket_seed(group: dict, index: int) -> int:
+        """The seed of a step's launch number ``index``: its places start at 0 again."""
+
+        return (group["seed"] + 0x632BE5AB * index) & _MASK
 
     def _with_gradients(self) -> list[tuple[dict, list[Tensor]]]:
         return [(group, [p for p in group["params"] if p.grad is not None]) for group in self.param_groups]

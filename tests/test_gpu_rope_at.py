@@ -75,6 +75,22 @@ def test_parts_of_heads(gpu, dtype, layout, dim, part):
 
 
 @pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+@pytest.mark.parametrize("native", [True, False])
+def test_windows_that_overlap(gpu, monkeypatch, layout, native):
+    """Windows of one row share their elements, so that both dimensions have stride 1; the output's head_dim stays contiguous."""
+
+    if not native:
+        monkeypatch.setattr(ops, "_launch", lambda *args: None)
+    f = RotaryFrequencies(12)
+    for s in (1, 3, 16, 30):
+        q, k = (randn((2, h, 16 + s - 1), torch.float32, gpu, h).unfold(2, 16, 1) for h in (2, 3))
+        a, b = triton_apply_rotary_at(q, k, 9, f, layout=layout)
+        check(a, q, 9, f, layout)
+        check(b, k, 9, f, layout)
+        assert a.stride(-1) == b.stride(-1) == 1
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
 @pytest.mark.parametrize("memory", ["bshd", "bhsd", "slice", "sbhd"])
 @pytest.mark.parametrize("form", ["offset", "seq", "one", "each", "int32", "strided", "broadcast"])
 def test_positions_and_memory(gpu, layout, memory, form):
