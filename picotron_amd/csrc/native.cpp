@@ -740,6 +740,46 @@ int64_t moment_bytes(PyObject* o, const at::Tensor& p, std::initializer_list<int
   return address % align == 0 ? address : 0;
 }
 
+// Appends the record of a parameter with 8-bit moments (p, gradient, the four state tensors, n, first block) and counts its
+// blocks; false if its state cannot be read as it is.
+bool moment_row(const at::Tensor& p, int64_t grad, PyObject* state, int64_t per, int64_t quant, std::vector<int64_t>* rows,
+                int64_t* blocks) {
+  const int64_t n = p.numel(), scales = (n + quant - 1) / quant;
+  const int64_t mc = moment_bytes(item(state, "exp_avg"), p, {scales, quant}, 4);
+  const int64_t ms = moment_bytes(item(state, "exp_avg_scale"), p, {scales}, 1);
+  const int64_t vc = moment_bytes(item(state, "exp_avg_sq"), p, {scales, quant}, 4);
+  const int64_t vs = moment_bytes(item(state, "exp_avg_sq_scale"), p, {scales}, 1);
+  if (mc == 0 || ms == 0 || vc == 0 || vs == 0) return false;
+  rows->insert(rows->end(), {reinterpret_cast<int64_t>(out(p)), grad, mc, ms, vc, vs, n, *blocks});
+  *blocks += (n + per - 1) / per;
+  return true;
+}
+
+// adamw8_table([params], [their states], elements per table block, elements per scale) -> (table, blocks)
+// The record table that the moments are read through, as bytes; None for anything but plain parameters of one device
+// with 8-bit states in place.
+PT_FN(adamw8_table, 4)
+  int64_t per, quant, blocks = 0;
+  if (!PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1]) || !as_i64(a[2], &per) ||
+      !as_i64(a[3], &quant) || per <= 0 || quant <= 0)
+    return none();
+  std::vector<int64_t> rows;
+  c10::Device device(c10::kCPU);
+  for (Py_ssize_t k = 0; k < PyList_GET_SIZE(a[0]); ++k) {
+    const at::Tensor* p = plain(PyList_GET_ITEM(a[0], k));
+    PyObject* state = PyList_GET_ITEM(a[1], k);
+    if (p == nullptr || code_of(*p) < 0 || !p->is_contiguous() || !PyDict_Check(state)) return none();
+    if (device.is_cpu()) device = p->device();
+    if (p->device() != device ||
+        !moment_row(*p, reinterpret_cast<int64_t>(out(*p)), state, per, quant, &rows, &blocks))
+      return none();
+  }
+  return Py_BuildValue("(NL)",
+                       PyBytes_FromStringAndSize(reinterpret_cast<const char*>(rows.data()),
+                                                 static_cast<Py_ssize_t>(rows.size() * sizeof(int64_t))),
+                       static_cast<long long>(blocks));
+PT_END
+
 // adamw8_scan([params, ...] per group, optimizer.state, elements per table block, elements per scale) ->
 // (device index, [(table, rows, blocks, step, steps, dtype code) or None, ...])
 // for parameters with 8-bit moments that all have their state in place, one dtype and one host step count a group: the
@@ -777,21 +817,15 @@ PT_FN(adamw8_scan, 4)
         PyErr_Clear();
         return none();
       }
-      const int64_t n = p->numel(), scales = (n + quant - 1) / quant;
-      const int64_t mc = moment_bytes(item(state, "exp_avg"), *p, {scales, quant}, 4);
-      const int64_t ms = moment_bytes(item(state, "exp_avg_scale"), *p, {scales}, 1);
-      const int64_t vc = moment_bytes(item(state, "exp_avg_sq"), *p, {scales, quant}, 4);
-      const int64_t vs = moment_bytes(item(state, "exp_avg_sq_scale"), *p, {scales}, 1);
       PyObject* so = item(state, "step");
       const float* count = host_step(so);
-      if (mc == 0 || ms == 0 || vc == 0 || vs == 0 || count == nullptr) return none();
+      if (count == nullptr) return none();
       if (device.is_cpu()) device = p->device();
       if (p->device() != device || (!rows.empty() && (*count != step || code_of(*p) != code))) return none();
       step = *count;
       code = code_of(*p);
       if (PyList_Append(steps, so) != 0) return nullptr;
-      rows.insert(rows.end(), {reinterpret_cast<int64_t>(out(*p)), reinterpret_cast<int64_t>(out(grad)), mc, ms, vc, vs, n, blocks});
-      blocks += (n + per - 1) / per;
+      if (!moment_row(*p, reinterpret_cast<int64_t>(out(grad)), state, per, quant, &rows, &blocks)) return none();
     }
     if (rows.empty()) {
       if (PyList_Append(list, Py_None) != 0) return nullptr;
@@ -862,6 +896,7 @@ PyMethodDef methods[] = {PT_METHOD(rmsnorm_fwd),
                          PT_METHOD(preference_loss),
                          PT_METHOD(sequence_log_probs_bwd),
                          PT_METHOD(adamw_scan),
+                         PT_METHOD(adamw8_table),
                          PT_METHOD(adamw8_scan),
                          PT_METHOD(advance_steps),
                          PT_METHOD(bind),

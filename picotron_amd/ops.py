@@ -1025,13 +1025,6 @@ def adamw8_reason(p: Tensor, state: dict) -> str | None:
     return None
 
 
-def adamw8_ready(params: list[Tensor], states: list[dict]) -> bool:
-    """True if the HIP kernels can read these parameters' 8-bit states."""
-
-    return (params[0].is_cuda and _lib.is_available() and device_supported(params[0].device.index)
-            and all(adamw8_reason(p, state) is None for p, state in zip(params, states)))
-
-
 def adamw8_table(params: list[Tensor], grads: list[Tensor], states: list[dict]) -> tuple[Tensor, int]:
     """Host int64 [n, 8] table for :func:`adamw8_step` and its block count (no empty parameters)."""
 
@@ -1083,16 +1076,24 @@ def adamw8_step(
 
 def adamw8_moments(
     params: list[Tensor], states: list[dict], dtype: torch.dtype = torch.float32
-) -> tuple[Tensor, Tensor, list[tuple[Tensor, int]]]:
-    """The values of 8-bit moments, flat: (exp_avg, exp_avg_sq, each parameter's place), zeros between them."""
+) -> tuple[Tensor, Tensor, list[tuple[Tensor, int]]] | None:
+    """The values of the 8-bit moments of parameters on one device, flat: (exp_avg, exp_avg_sq, each parameter's place),
+    zeros between them; None where the kernel cannot read or write them."""
 
-    device = _check_cuda(*params)
-    for p, state in zip(params, states):
-        reason = adamw8_reason(p, state)
-        if reason is not None:
-            raise ValueError(f"AdamW moments: {reason}")
-    table, blocks = adamw8_table(params, params, states)
-    per = adamw8_sizes()[0]
+    device = params[0].device
+    if dtype not in _DTYPE_CODES or device.type != "cuda" or not _lib.is_available() or not device_supported(device.index):
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("AdamW moments: their table is copied to the device, which a graph capture cannot hold")
+    per, scale = adamw8_sizes()
+    native = _lib.extension()
+    found = None if native is None else native.adamw8_table(params, states, per, scale)
+    if found is not None:
+        table, blocks = torch.frombuffer(bytearray(found[0]), dtype=torch.int64).view(-1, 8), found[1]
+    elif all(adamw8_reason(p, state) is None for p, state in zip(params, states)):
+        table, blocks = adamw8_table(params, params, states)
+    else:
+        return None
     m = torch.empty(blocks * per, dtype=dtype, device=device)
     v = torch.empty_like(m)
     places = [(p, first * per) for p, first in zip(params, table[:, 7].tolist())]

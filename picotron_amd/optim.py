@@ -240,8 +240,9 @@ class AdamW8bit(Optimizer):
             return torch.zeros(0, dtype=dtype), torch.zeros(0, dtype=dtype), []
         if any(p.device != held[0][0].device for p, _ in held):
             raise ValueError("AdamW8bit.moments takes parameters on one device")
-        if ops.adamw8_ready([p for p, _ in held], [state for _, state in held]):
-            return ops.adamw8_moments([p for p, _ in held], [state for _, state in held], dtype)
+        found = ops.adamw8_moments([p for p, _ in held], [state for _, state in held], dtype)
+        if found is not None:
+            return found
         total, places = 0, []
         for p, _ in held:
             places.append((p, total))

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from gpu_util import randn
-from picotron_amd import ops
+from picotron_amd import _lib, ops
 from picotron_amd.nn import RotaryFrequencies
 from picotron_amd.nn.triton_kernels import adamw, triton_adamw_step, triton_clip_grad_norm_and_step
 from picotron_amd.optim import AdamW8bit
@@ -133,6 +133,31 @@ def test_scan_takes_the_same_8bit_steps(gpu, monkeypatch, dtype, groups, clip):
         assert all(torch.equal(a[k], b[k]) for k in a)
     for a, b in zip(*(r[2] for r in runs)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_moments_by_either_table(gpu, monkeypatch, dtype):
+    params, opt = _optimizer(gpu, dtype, 3)
+    for i, p in enumerate(params[:-1]):
+        p.grad = randn(p.shape, dtype, gpu, i)
+    triton_adamw_step(opt)
+    m, v, places = opt.moments()
+    with monkeypatch.context() as c:
+        c.setattr(_lib, "extension", lambda: None)
+        general = opt.moments()
+    assert torch.equal(m, general[0]) and torch.equal(v, general[1])
+    assert [(id(p), at) for p, at in places] == [(id(p), at) for p, at in general[2]]
+    wide = opt.moments(torch.float64)  # a type without kernels: in PyTorch
+    for p, at in places:
+        assert torch.equal(m[at:at + p.numel()].double(), wide[0][at:at + p.numel()])
+        assert torch.equal(v[at:at + p.numel()].double(), wide[1][at:at + p.numel()])
+    state = opt.state[params[1]]
+    state["exp_avg"] = torch.cat((state["exp_avg"],) * 2, 1)[:, :256]  # strided: the kernel cannot read it
+    again = opt.moments()
+    assert all(torch.equal(m[at:at + p.numel()], again[0][at:at + p.numel()]) for p, at in places)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capture"), torch.cuda.graph(graph):
+        opt.moments()
 
 
 def test_8bit_scan_leaves_the_unusual_to_the_plan(gpu):
