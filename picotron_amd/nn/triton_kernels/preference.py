@@ -68,11 +68,14 @@ class _PreferenceLoss(torch.autograd.Function):
         ctx.save_for_backward(logits, labels, ws)
         ctx.how = how
         ctx.mark_non_differentiable(rewards, log_probs)
+        ctx.set_materialize_grads(False)  # no zeros for them
         return loss, rewards, log_probs
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad: Tensor, *_):  # type: ignore[override]
+    def backward(ctx, grad: Tensor | None, *_):  # type: ignore[override]
+        if grad is None:
+            return None, None, None, None
         logits, labels, ws = ctx.saved_tensors
         d = ops.sequence_log_probs_bwd(logits, labels, ws, grad_loss=grad, shift=ctx.how["shift"],
                                        ignore_index=ctx.how["ignore_index"])

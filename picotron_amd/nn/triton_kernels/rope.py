@@ -126,6 +126,7 @@ class _RoPEAtFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, how: tuple, turns: Tensor, positions: Tensor | None, *states: Tensor):  # type: ignore[override]
+        ctx.set_materialize_grads(False)
         ctx.how = how  # (offset, scale, layout, inverse)
         ctx.has_positions = positions is not None
         ctx.save_for_backward(turns, *((positions,) if positions is not None else ()))
