@@ -339,7 +339,7 @@ PT_FN(rope_at, 9)
   if (x0 == nullptr || g == nullptr || x0->dim() != 4 || code_of(*x0) < 0 || !rope_state(x0, *x0, x0->size(3)) ||
       (a[1] != Py_None && (!rope_state(x1, *x0, x0->size(3)) || x1->size(0) != x0->size(0) || x1->size(2) != x0->size(2))) ||
       g->dim() != 1 || g->scalar_type() != at::kLong || !g->is_contiguous() || !same_place(*g, *x0) ||
-      g->size(0) * 2 > x0->size(3) || !as_i64(a[4], &offset) || !as_f64(a[5], &scale) || !as_i64(a[6], &layout))
+      x0->size(3) % 2 != 0 || g->size(0) * 2 > x0->size(3) || !as_i64(a[4], &offset) || !as_f64(a[5], &scale) || !as_i64(a[6], &layout))
     return none();
   int64_t pbs = 0, pss = 0;
   int width = 0;

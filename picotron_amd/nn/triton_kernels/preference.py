@@ -121,8 +121,14 @@ def triton_sequence_log_probs(
     """Each sequence's log-probability of its kept labels (their mean with ``average``), fp32 of (batch,); 0 for a
     sequence that keeps none.  Differentiable in the logits."""
 
+    plain = no_graph(logits)
+    if plain:  # what the native launcher takes needs no check here
+        require_hip(TritonPreferenceUnavailable, "preference loss", logits, labels)
+        out = ops._launch_here("pt_sequence_log_probs", logits, labels, bool(shift), ignore_index, bool(average))
+        if out is not None:
+            return out[0]
     _validate(logits, labels, shift)
-    if no_graph(logits):
+    if plain:
         return ops.sequence_log_probs(logits, labels, shift=shift, ignore_index=ignore_index, average=average)[0]
     return _SequenceLogProbs.apply(logits, labels, bool(shift), int(ignore_index), bool(average))
 
