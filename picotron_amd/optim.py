@@ -143,12 +143,14 @@ class AdamW8bit(Optimizer):
     def buckets(self, groups: list[tuple[dict, list[Tensor]]]) -> list[tuple]:
         """The launches of one step over ``groups`` (param_group, its parameters that step): (param_group, params, states, their
         common step before it -- a number, or for a capturable group the device tensor -- and seed).  Creates
-        what state is missing.  Parameters of a bucket share a group, a dtype and a step count."""
+        what state is missing.  Parameters of a bucket share a group, a dtype and a step count; a device count belongs to one bucket,
+        whose launch advances it."""
 
         found = []
+        counted: set[int] = set()
         for group, params in groups:
             shared: dict[tuple, tuple[list, list]] = {}
-            fresh: dict[torch.device, Tensor] = {}
+            fresh: dict[tuple, Tensor] = {}
             for p in params:
                 if p.numel() == 0:
                     continue
@@ -156,14 +158,24 @@ class AdamW8bit(Optimizer):
                 if len(state) == 0:
                     state = self._new_state(p, group["capturable"])
                     if group["capturable"]:  # the parameters that start together count together
-                        state["step"] = fresh.setdefault(p.device, state["step"])
+                        state["step"] = fresh.setdefault((p.dtype, p.device), state["step"])
                 step = state["step"]
                 key = (p.dtype, p.device, id(step) if group["capturable"] else float(step))
                 ps, states = shared.setdefault(key, ([], []))
                 ps.append(p)
                 states.append(state)
             for (_, _, step), (ps, states) in shared.items():
-                value = states[0]["step"] if group["capturable"] else step
+                value = step
+                if group["capturable"]:
+                    value = states[0]["step"]
+                    if id(value) in counted:  # shared with another bucket: a count of its own from here on
+                        if value.is_cuda and torch.cuda.is_current_stream_capturing():
+                            raise RuntimeError("AdamW8bit: parameters that step in several launches share a step count; take one "
+                                               "step before capturing it")
+                        value = value.clone()
+                        for state in states:
+                            state["step"] = value
+                    counted.add(id(value))
                 found.append((group, ps, states, value, self.bucket_seed(group, len(found))))
         return found
 
@@ -265,7 +277,7 @@ class AdamW8bit(Optimizer):
                     raise ValueError(f"AdamW8bit does not take a state of {flag}=True")
         super().load_state_dict(state_dict)
         shared: dict[tuple, Tensor] = {}
-        capturable = {id(p) for group in self.param_groups if group["capturable"] for p in group["params"]}
+        capturable = {id(p): i for i, group in enumerate(self.param_groups) if group["capturable"] for p in group["params"]}
         for p, state in self.state.items():
             for codes, scales, top in zip(_CODES, _SCALES, (TOP_M, TOP_V)):
                 if codes not in state:
@@ -279,8 +291,8 @@ class AdamW8bit(Optimizer):
                 nearest = torch.full((_blocks(p), BLOCK), 1 << 19, dtype=torch.int32, device=p.device)
                 state[codes], state[scales] = encode(values.view(-1, BLOCK), nearest, top)
             if id(p) in capturable and "step" in state:
-                # equal counts of one device share a tensor again, as they did before
-                key = (p.device, float(state["step"]))
+                # equal counts of a launch share a tensor again, as they did before
+                key = (capturable[id(p)], p.dtype, p.device, float(state["step"]))
                 state["step"] = shared.setdefault(key, torch.as_tensor(state["step"], dtype=torch.float32, device=p.device))
 
     def __setstate__(self, state: dict) -> None:

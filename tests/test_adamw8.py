@@ -262,3 +262,42 @@ def test_nothing_to_do():
     empty.param_groups[0]["params"][0].grad = torch.zeros(0)
     empty.step()
     assert empty.moments()[2] == []
+
+
+def _mixed(**options):
+    params = [torch.nn.Parameter(torch.randn(300, dtype=t)) for t in (torch.float32, torch.bfloat16, torch.float32, torch.bfloat16)]
+    return params, AdamW8bit([dict(params=params[:3]), dict(params=params[3:], lr=1e-2)], capturable=True, **options)
+
+
+def _one_count_a_launch(optimizer):
+    buckets = optimizer.buckets(optimizer._with_gradients())
+    steps = [step for _, _, _, step, _ in buckets]
+    assert len({id(step) for step in steps}) == len(steps)
+    for _, _, states, step, _ in buckets:
+        assert all(state["step"] is step for state in states)
+    return buckets
+
+
+def test_launches_do_not_share_a_step_count():
+    """A launch advances its device count, so that two launches of one step must not have the same one: parameters of
+    two dtypes that start together, two groups that a checkpoint restores at one count, and counts that a program shares."""
+
+    params, optimizer = _mixed()
+    for p in params:
+        p.grad = torch.ones_like(p)
+    assert len(_one_count_a_launch(optimizer)) == 3
+    optimizer.step()
+    assert [float(optimizer.state[p]["step"]) for p in params] == [1.0] * 4
+    again, restored = _mixed()
+    restored.load_state_dict(optimizer.state_dict())
+    for p in again:
+        p.grad = torch.ones_like(p)
+    assert len(_one_count_a_launch(restored)) == 3
+    restored.step()
+    assert [float(restored.state[p]["step"]) for p in again] == [2.0] * 4
+    one = torch.tensor(2.0)
+    for p in again:
+        restored.state[p]["step"] = one
+    _one_count_a_launch(restored)
+    restored.step()
+    assert [float(restored.state[p]["step"]) for p in again] == [3.0] * 4

@@ -323,3 +323,28 @@ def test_refusals_change_nothing(gpu, case):
         triton_adamw_step(fused)
     for p, q in zip(a, before):
         assert torch.equal(p, q) and float(fused.state[p]["step"]) == 1.0
+
+
+def test_capturable_launches_of_several_dtypes_and_groups(gpu):
+    """Two dtypes in a group and a second group, restored from a checkpoint: each launch counts for itself."""
+
+    def made():
+        params = [torch.nn.Parameter(randn((n,), t, gpu, n, 0.1)) for n, t in
+                  ((300, torch.float32), (1300, torch.bfloat16), (5000, torch.float32), (700, torch.bfloat16))]
+        return params, AdamW8bit([dict(params=params[:3]), dict(params=params[3:], lr=1e-2)], **HP, capturable=True)
+
+    (a, fused), (b, plain) = made(), made()
+    for step in range(5):
+        if step == 3:
+            (a2, fused2), (b2, plain2) = made(), made()
+            for old, new, before, after in ((a, a2, fused, fused2), (b, b2, plain, plain2)):
+                for p, q in zip(old, new):
+                    q.data.copy_(p.data)
+                after.load_state_dict(before.state_dict())
+            a, b, fused, plain = a2, b2, fused2, plain2
+        gradients(step, a, b)
+        triton_adamw_step(fused)
+        plain.step()
+        assert [float(fused.state[p]["step"]) for p in a] == [step + 1.0] * 4
+        same_codes(a, b, fused, plain)
+    close_parameters(a, b, 5, lr=1e-2)
