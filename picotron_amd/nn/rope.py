@@ -131,6 +131,7 @@ class RotaryFrequencies:
     It is a plan that a model keeps: :meth:`turns` is copied to a device once (before a graph capture
     that uses it there)."""
 
+    @torch.inference_mode(False)  # (a model may be built, or first used, where tensors are another's)
     def __init__(self, rotary_dim: int, theta: float = 10_000.0, *, scaling: Mapping | None = None) -> None:
         if rotary_dim <= 0 or rotary_dim % 2 != 0:
             raise ValueError("RoPE requires an even, positive rotary dimension.")
@@ -138,7 +139,7 @@ class RotaryFrequencies:
             raise ValueError("rope_theta must be positive.")
         self.rotary_dim = rotary_dim
         self.attention_factor = 1.0
-        i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        i = torch.arange(rotary_dim // 2, dtype=torch.float64, device="cpu")
         if scaling is None:
             self.frequencies = theta ** (-2.0 * i / rotary_dim)
         else:
@@ -185,7 +186,8 @@ class RotaryFrequencies:
                     "HIP RoPE: the frequencies are first used on this device during graph capture; run the same call "
                     "once before capturing it.")
             bits = [round(math.fmod(f / (2 * math.pi), 1.0) * 2**64) % 2**64 for f in self.frequencies.tolist()]
-            found = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64).to(device)
+            with torch.inference_mode(False):  # a later pass may keep them for its backward
+                found = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64, device="cpu").to(device)
             self._turns[device] = found
         return found
 

@@ -271,3 +271,16 @@ def test_refusals(gpu, case):
         p = p.cpu()
     with pytest.raises(TritonRoPEUnavailable):
         triton_apply_rotary_at(q, k, p, f, layout=layout)
+
+
+def test_training_after_an_inference_pass(gpu):
+    f = RotaryFrequencies(16)
+    q = randn((1, 2, 5, 16), torch.float32, gpu, 1)
+    with torch.inference_mode():
+        first, _ = triton_apply_rotary_at(q, None, 3, f)
+    q.requires_grad_()
+    out, _ = triton_apply_rotary_at(q, None, 3, f)
+    assert torch.equal(out, first)
+    up = randn(q.shape, torch.float32, gpu, 2)
+    (grad,) = torch.autograd.grad(out, q, up)
+    check(grad, up, 3, f, "interleaved", inverse=True)

@@ -177,3 +177,18 @@ def test_entry_point_refuses(change, code):
 def test_empty_tensors_are_no_ops():
     desc = (ctypes.c_int64 * 9)(2, 0, 3, 8, 8, 8, 8, 8, 8)
     assert _lib.lib().pt_rope_at(None, None, desc, None, None, None, 8, 8, None, 0, 0, 0, 0, 4096, 1.0, 0, 0, 0, None) == _lib.PT_OK
+
+
+def test_frequencies_are_the_hosts_under_another_default_device():
+    want = RotaryFrequencies(16, scaling=dict(type="yarn", factor=4.0, original_max_positions=128))
+    with torch.device("meta"):
+        f = RotaryFrequencies(16, scaling=dict(type="yarn", factor=4.0, original_max_positions=128))
+        turns = f.turns(torch.device("cpu"))
+    assert torch.equal(f.frequencies, want.frequencies) and torch.equal(turns, want.turns(torch.device("cpu")))
+
+
+def test_turns_of_an_inference_pass_serve_training():
+    with torch.inference_mode():
+        f = RotaryFrequencies(16)
+        turns = f.turns(torch.device("cpu"))
+    assert not turns.is_inference() and not f.frequencies.is_inference()
