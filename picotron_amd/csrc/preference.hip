@@ -633,9 +633,13 @@ uint32_t parts_for(int64_t rows, int64_t vocab, int dtype) {
   return static_cast<uint32_t>(most < 2 ? 1 : (want < most ? want : most));
 }
 
-// Rows up to which one workgroup does what is left after them: joins their parts, or adds and forms the loss.
+// What is left after the rows is one workgroup's where it joins the parts of up to kJoinedRows rows, or adds up to
+// kSummedRows rows' tokens and forms the loss with at most kPasses sequences for each team of waves: a second launch costs
+// more than them (16 sequences of 1024 tokens 6.5 us against 4.1 + 4.1 and the gap between, 64 of 256 7.9 against as much;
+// but 128 of 128 12.6, 1024 of 16 79).
 constexpr uint32_t kJoinedRows = 64;
 constexpr uint32_t kSummedRows = 16384;
+constexpr uint32_t kPasses = 4;
 
 constexpr int64_t kMaxRows = int64_t{1} << 23;
 constexpr int64_t kMaxBatch = int64_t{1} << 21;
@@ -690,9 +694,10 @@ int run_rows(const char* fn, const Rows& d, const Parts& a, hipStream_t st) {
 template <typename T>
 int run_sums(const char* fn, const Rows& d, const Parts& a, const SequenceSums& s, const PairLoss& pl, hipStream_t st) {
   const bool joins = a.parts > 1;
-  if (joins ? d.rows <= kJoinedRows : (pl.pairs > 0 && d.rows <= kSummedRows)) {
-    hipLaunchKernelGGL(seq_small_kernel<T>, dim3(1), dim3(kSmallThreads), 0, st, d, a, s,
-                       team_of(s.seq, kSmallThreads / 64), pl);
+  const uint32_t together = team_of(s.seq, kSmallThreads / 64);
+  const bool few = d.rows <= kSummedRows && s.batch * together <= kPasses * (kSmallThreads / 64);
+  if (joins ? d.rows <= kJoinedRows : (pl.pairs > 0 && few)) {
+    hipLaunchKernelGGL(seq_small_kernel<T>, dim3(1), dim3(kSmallThreads), 0, st, d, a, s, together, pl);
     return check_launch(fn);
   }
   if (joins) {

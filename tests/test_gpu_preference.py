@@ -438,3 +438,29 @@ def test_one_step_of_preference_tuning(gpu):
     for p, b in zip((embed, mix), before):
         assert p.isfinite().all() and (p != b).any()
     assert not loss._fallback_warned and not rope._triton_fallback_warned
+
+
+@pytest.mark.parametrize("use", ["loss", "log_probs"])
+def test_under_the_compiler(gpu, use):
+    logits, labels, reference = inputs(4, 9, 300, torch.bfloat16, gpu, 5)
+    logits.requires_grad_()
+
+    def step(x):
+        if use == "loss":
+            return triton_preference_loss(x * 2, labels, reference, beta=0.2).loss * 3
+        return (triton_sequence_log_probs(x * 2, labels) * reference).sum()
+
+    want = step(logits)
+    (grad,) = torch.autograd.grad(want, logits)
+    got = torch.compile(step, backend="aot_eager")(logits)
+    (compiled,) = torch.autograd.grad(got, logits)
+    assert torch.equal(got, want) and torch.equal(compiled, grad)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(step, backend="aot_eager")(logits), want)
+
+
+@pytest.mark.parametrize("batch,seq", [(16384, 1), (5462, 3), (2048, 8), (1022, 16)])
+def test_many_short_sequences(gpu, batch, seq):
+    logits, labels, reference = inputs(batch, seq, 40, torch.float32, gpu, 7)
+    out = triton_preference_loss(logits, labels, reference, beta=0.5, shift=False)
+    check_log_probs(out.log_probs, logits, labels, shift=False)
