@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void seq_stats_tiny_kernel(Rows d, float2
   }
 }
 
-// Rows of up to 64 * N vectors: a wave a row, all of it in flight together.
+// Shorter rows: a wave a row, N vectors a lane in flight together.
 template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void seq_stats_short_kernel(Rows d, float2* __restrict__ stats,
                                                                    float* __restrict__ tokens) {
@@ -233,12 +233,14 @@ __global__ __launch_bounds__(kThreads) void seq_stats_short_kernel(Rows d, float
   }
   const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
   const RowReader<T, 64> in(p, d.vocab, 0, 1, lane, false);
-  Vec16<T> v[N];
-  in.load(lane, v);
-  const float xt = label_logit(d, p, label);
-  in.mask(lane, v);
+  const float xt = label_logit(d, p, label);  // in flight with the row
   Running run;
-  run.add(v);
+  for (int from = 0; from < in.n; from += 64 * N) {
+    Vec16<T> v[N];
+    in.load(from + lane, v);
+    in.mask(from + lane, v);
+    run.add(v);
+  }
   run.add(in.head, in.tail);
   const float M = wave_max(run.m);
   const float S = wave_sum(run.s * exp_from(run.m, shift_of(M)));
@@ -622,22 +624,23 @@ struct Layout {
   }
 };
 
-// Parts of a row: one, unless the rows alone leave most of the card idle; then as many as make kPartGroups workgroups, of
-// kPartVecs vectors at least.
-constexpr int64_t kPartGroups = 512;
-constexpr int64_t kPartVecs = 512;
+// Parts of a row: one, unless the rows alone leave most of the card idle; then one for each batch of loads that a workgroup
+// has in flight, where that is three and more.  Rows and sums, us, whole / in parts: one row of 128256 bf16 logits 16.8 /
+// 8.3, 64 rows 17.5 / 12.0, of 50257 one row 10.2 / 8.4, 64 rows 11.9 / 11.1.  Above kPartRows the join is another launch,
+// which only long rows are worth: 128 rows of 128256 18.1 / 15.5, of 200000 fp32 logits 32.4 / 25.5, of 50257 12.4 / 13.2;
+// 192 of 128256 18.6 / 18.4.
+constexpr int64_t kBatchVecs = kThreads * kBatch;
+constexpr int64_t kPartRows = 64, kLongPartRows = 128, kLongBatches = 8;
 uint32_t parts_for(int64_t rows, int64_t vocab, int dtype) {
-  if (rows <= 0 || rows * 2 > kPartGroups) return 1;
-  const int64_t vecs = vocab * dtype_size(dtype) / 16;
-  const int64_t most = vecs / kPartVecs, want = kPartGroups / rows;
-  return static_cast<uint32_t>(most < 2 ? 1 : (want < most ? want : most));
+  if (rows <= 0 || rows > kLongPartRows) return 1;
+  const int64_t batches = (vocab * dtype_size(dtype) / 16 + kBatchVecs - 1) / kBatchVecs;
+  return batches < (rows <= kPartRows ? 3 : kLongBatches) ? 1 : static_cast<uint32_t>(batches);
 }
 
-// What is left after the rows is one workgroup's where it joins the parts of up to kJoinedRows rows, or adds up to
+// What is left after the rows is one workgroup's where it joins the parts of up to kPartRows rows, or adds up to
 // kSummedRows rows' tokens and forms the loss with at most kPasses sequences for each team of waves: a second launch costs
 // more than them (16 sequences of 1024 tokens 6.5 us against 4.1 + 4.1 and the gap between, 64 of 256 7.9 against as much;
 // but 128 of 128 12.6, 1024 of 16 79).
-constexpr uint32_t kJoinedRows = 64;
 constexpr uint32_t kSummedRows = 16384;
 constexpr uint32_t kPasses = 4;
 
@@ -668,6 +671,12 @@ Rows rows_of(const void* logits, int64_t seq, int64_t batch, int64_t bs, int64_t
               static_cast<uint32_t>(batch * seq), shift};
 }
 
+// Rows by their vectors, us for 16384 rows of bf16 logits: 16 lanes a row where three vectors a lane hold it (48 vectors:
+// 5.0, a wave 9.8); a wave (64: 10.0, a workgroup 39.6; 512: 22.8 and 69; 1024: 44.4 and 66) while the rows' number
+// hides that a wave takes long over one (256 rows of 1024 vectors: 5.3, a workgroup 4.2; 1024 rows 6.0 and 6.6); a
+// workgroup (1536: 68, a wave 64; 2048: 77 and 86; 1024 rows of 1536 7.1 and 8.6).
+constexpr uint32_t kManyRows = 1024;
+
 template <typename T>
 int run_rows(const char* fn, const Rows& d, const Parts& a, hipStream_t st) {
   const int64_t vecs = (static_cast<int64_t>(d.vocab) + Elem<T>::VEC - 1) / Elem<T>::VEC;
@@ -680,10 +689,8 @@ int run_rows(const char* fn, const Rows& d, const Parts& a, hipStream_t st) {
     rows_by(seq_stats_tiny_kernel<T, 3>, 16);
   } else if (vecs <= 128) {
     rows_by(seq_stats_short_kernel<T, 2>, 4);
-  } else if (vecs <= 256) {
+  } else if (vecs <= (d.rows >= kManyRows ? 1024 : 512)) {
     rows_by(seq_stats_short_kernel<T, 4>, 4);
-  } else if (vecs <= 512) {
-    rows_by(seq_stats_short_kernel<T, 8>, 4);
   } else {
     hipLaunchKernelGGL(seq_stats_kernel<T>, dim3(d.rows * a.parts), dim3(kThreads), 0, st, d, a.parts,
                        const_cast<float2*>(a.partial), a.stats, a.tokens);
@@ -696,7 +703,7 @@ int run_sums(const char* fn, const Rows& d, const Parts& a, const SequenceSums& 
   const bool joins = a.parts > 1;
   const uint32_t together = team_of(s.seq, kSmallThreads / 64);
   const bool few = d.rows <= kSummedRows && s.batch * together <= kPasses * (kSmallThreads / 64);
-  if (joins ? d.rows <= kJoinedRows : (pl.pairs > 0 && few)) {
+  if (joins ? d.rows <= kPartRows : (pl.pairs > 0 && few)) {
     hipLaunchKernelGGL(seq_small_kernel<T>, dim3(1), dim3(kSmallThreads), 0, st, d, a, s, together, pl);
     return check_launch(fn);
   }
@@ -763,6 +770,9 @@ int run_grad(const char* fn, const Rows& d, void* grad, int64_t gbs, int64_t gss
                        large ? static_cast<uint32_t>(items / kXcds) : 0u, static_cast<int>(per), from);
     return check_launch(fn);
   };
+  // By a row's vectors, us for 16384 rows of bf16 logits: 16 lanes a row up to 48 (5.5, a wave 9.2), a wave up to 256 (192:
+  // 18.1, a workgroup 27.8; 256: 23.2 and 28.3), a workgroup of two vectors a thread up to 512 (384: 34.8, of four 44.2; 512:
+  // 42.5 and 46.3), of four from there on.
   if (d.vocab >= Elem<T>::VEC && vecs <= 16) return tiny(seq_grad_tiny_kernel<T, 1>);
   if (d.vocab >= Elem<T>::VEC && vecs <= 48) return tiny(seq_grad_tiny_kernel<T, 3>);
   if (vecs <= 128) return go(seq_grad_kernel<T, 64, 2>, 64, 2);

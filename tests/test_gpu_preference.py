@@ -464,3 +464,24 @@ def test_many_short_sequences(gpu, batch, seq):
     logits, labels, reference = inputs(batch, seq, 40, torch.float32, gpu, 7)
     out = triton_preference_loss(logits, labels, reference, beta=0.5, shift=False)
     check_log_probs(out.log_probs, logits, labels, shift=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vecs", [257, 511, 513, 767, 1023, 1024, 1025])
+@pytest.mark.parametrize("rows", [1023, 1024])
+def test_rows_a_wave_or_a_workgroup_takes(gpu, dtype, vecs, rows):
+    per = 128 // torch.finfo(dtype).bits
+    logits, labels, _ = inputs(1, rows, vecs * per - 3, dtype, gpu, 11)
+    got = triton_sequence_log_probs(logits, labels, shift=False)
+    check_log_probs(got, logits, labels, shift=False)
+
+
+@pytest.mark.parametrize("vocab,dtype", [(33_000, torch.bfloat16), (50257, torch.float16), (128256, torch.bfloat16), (70_001, torch.float32)])
+@pytest.mark.parametrize("rows", [64, 65, 128, 129])
+def test_parts_of_rows(gpu, vocab, dtype, rows):
+    logits, labels, _ = inputs(1, rows, vocab, dtype, gpu, 12)
+    logits.requires_grad_()
+    out = triton_sequence_log_probs(logits, labels)
+    check_log_probs(out.detach(), logits.detach(), labels)
+    (grad,) = torch.autograd.grad(out, logits, torch.full((1,), -1.5, device=gpu))
+    check_grad(grad, logits.detach(), labels, torch.full((1,), -1.5, dtype=torch.float64, device=gpu))
