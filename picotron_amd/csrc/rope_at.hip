@@ -9,8 +9,9 @@
 // fraction from p = 2^23 on.  Its upper 32 bits (a resolution of 1.5e-9 rad) are reduced to an eighth of a turn around the
 // nearest quarter; sine and cosine of the rest are polynomials in its square.
 //
-// Work item = for up to U heads of one position, one 16-byte vector of a row (interleaved) or two, from
-// both halves of the rotated part or both parts of the rest (rotate-half).  The heads share the item's angles, and
+// Work item = for up to U heads of one position, one 16-byte vector of a row (interleaved, and large rotate-half
+// calls, whose lanes swap what their pairs need) or two, from both halves of the rotated part or both parts of the
+// rest (rotate-half otherwise).  The heads share the item's angles, and
 // all their vectors are in flight before the first is rotated.  Vectors are moved at the element's
 // alignment (one instruction on gfx950 at any address); where a part is no whole number of them its last one starts
 // earlier and overlaps the one before, both writing the same values, so nothing is done by the element but rows whose
@@ -53,6 +54,7 @@ struct AtRow {
   int head_dim;
   int rotary;      // rotated elements
   uint32_t items;  // per row
+  uint32_t slots;  // rows that a wave takes at once (rope_swap_kernel)
 };
 
 // cos and sin of t / 2^32 turns.  t = q quarter turns + r, |r| <= 1/8 turn.  The polynomials (minimax, degree 7
@@ -88,6 +90,26 @@ __device__ __forceinline__ void rotate(float u, float w, float c, float s, T* a,
   *b = Elem<T>::from_f32(__builtin_fmaf(w, c, u * s));
 }
 
+// Row r of a tensor: its memory, head and position.
+template <typename T>
+struct AtPlace {
+  const T* x;
+  T* y;
+  uint32_t head;
+  int64_t pos;
+  __device__ __forceinline__ AtPlace(const AtAngles& an, const AtTensor& t, uint32_t r) {
+    const uint32_t r1 = r / t.n2;
+    const uint32_t i2 = r - r1 * t.n2;
+    const uint32_t i0 = r1 / t.n1;
+    const uint32_t i1 = r1 - i0 * t.n1;
+    const auto pick = [&](int at) -> uint32_t { return at == 0 ? i0 : (at == 1 ? i1 : i2); };
+    x = static_cast<const T*>(t.x) + (i0 * t.xs[0] + i1 * t.xs[1] + i2 * t.xs[2]);
+    y = static_cast<T*>(t.y) + (i0 * t.ys[0] + i1 * t.ys[1] + i2 * t.ys[2]);
+    head = pick(t.head_at);
+    pos = position_of(an, pick(t.batch_at), pick(t.seq_at));
+  }
+};
+
 // Thread t of block b takes item b * 256 + t of its tensor.  VEC: rows by vectors, else by pairs (U is 1).
 template <typename T, int LAYOUT, bool VEC, bool NT, int U>
 __global__ __launch_bounds__(256) void rope_at_kernel(AtAngles an, AtRow row, AtTensor t0, AtTensor t1) {
@@ -102,15 +124,11 @@ __global__ __launch_bounds__(256) void rope_at_kernel(AtAngles an, AtRow row, At
   if (item >= t->items) return;
   const uint32_t r = item / row.items;
   const int j = static_cast<int>(item - r * row.items);
-  const uint32_t r1 = r / t->n2;
-  const uint32_t i2 = r - r1 * t->n2;
-  const uint32_t i0 = r1 / t->n1;
-  const uint32_t i1 = r1 - i0 * t->n1;
-  const auto pick = [&](int at) -> uint32_t { return at == 0 ? i0 : (at == 1 ? i1 : i2); };
-  const T* x = static_cast<const T*>(t->x) + (i0 * t->xs[0] + i1 * t->xs[1] + i2 * t->xs[2]);
-  T* y = static_cast<T*>(t->y) + (i0 * t->ys[0] + i1 * t->ys[1] + i2 * t->ys[2]);
-  const uint32_t head = pick(t->head_at);
-  const int64_t pos = position_of(an, pick(t->batch_at), pick(t->seq_at));
+  const AtPlace<T> place(an, *t, r);
+  const T* const x = place.x;
+  T* const y = place.y;
+  const uint32_t head = place.head;
+  const int64_t pos = place.pos;
   const int half = row.rotary / 2;
 
   if constexpr (!VEC) {
@@ -191,6 +209,54 @@ __global__ __launch_bounds__(256) void rope_at_kernel(AtAngles an, AtRow row, At
   }
 }
 
+// Rotate-half rows by whole rows of a wave: `slots` rows of `items` vectors, a vector a lane, so that every access is
+// contiguous however short the halves are.  A lane gets the other element of its pairs from the lane that holds
+// it; both work the angles out.  (Host: halves and rows are whole vectors, a row 64 at most.)
+template <typename T, bool NT, int U>
+__global__ __launch_bounds__(256) void rope_swap_kernel(AtAngles an, AtRow row, AtTensor t0, AtTensor t1) {
+  constexpr int V = Elem<T>::VEC;
+  uint32_t blk = blockIdx.x;
+  const AtTensor* t = &t0;
+  if (blk >= t0.blocks) {
+    blk -= t0.blocks;
+    t = &t1;
+  }
+  const uint32_t lane = threadIdx.x % 64u, slot = lane / row.items, j = lane - slot * row.items;
+  const uint32_t r = (blk * 4u + threadIdx.x / 64u) * row.slots + slot;
+  if (slot >= row.slots || r >= t->items) return;  // whole rows: both lanes of a pair go or stay
+  const AtPlace<T> place(an, *t, r);
+  const int at = static_cast<int>(j) * V, half = row.rotary / 2;
+  const bool low = at < half, turns = at < row.rotary;
+  Vec16<T> v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u == 0 || place.head + u * t->chunks < t->heads) v[u].raw = load_vec<T, false, NT>(place.x + u * t->xstep + at);
+  float c[V], s[V];
+  if (turns) {
+    const uint64_t* g = an.turns + (low ? at : at - half);
+#pragma unroll
+    for (int p = 0; p < V; ++p)
+      turn_cos_sin(static_cast<uint32_t>((static_cast<uint64_t>(place.pos) * g[p]) >> 32), an.scale,
+                   low ? -an.sign : an.sign, &c[p], &s[p]);
+  }
+  const int other = (static_cast<int>(lane) + (low ? half : -half) / V) * 4;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (u == 0 || place.head + u * t->chunks < t->heads) {
+      if (turns) {
+        Vec16<T> w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w.raw[k] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(other, static_cast<int>(v[u].raw[k])));
+#pragma unroll
+        for (int p = 0; p < V; ++p)  // as in rotate(), the sine's sign with the half
+          v[u].e[p] = Elem<T>::from_f32(__builtin_fmaf(Elem<T>::to_f32(v[u].e[p]), c[p], Elem<T>::to_f32(w.e[p]) * s[p]));
+      }
+      store_vec<T, false, NT>(place.y + u * t->ystep + at, v[u].raw);
+    }
+  }
+}
+
 struct AtView {
   AtTensor t{};
   int64_t n[3] = {1, 1, 1};
@@ -246,11 +312,15 @@ bool parse_view(const void* x, void* y, const int64_t* d, AtView* v, std::string
 
 constexpr int64_t kNontemporalBytes = int64_t{64} << 20;
 
-template <typename T, int LAYOUT, bool VEC, int U>
+// SWAP: rope_swap_kernel
+template <typename T, int LAYOUT, bool VEC, int U, bool SWAP = false>
 void launch_at(const AtAngles& an, AtRow row, AtView (&v)[2], hipStream_t st) {
   constexpr int V = Elem<T>::VEC;
   const int half = row.rotary / 2, rest = row.head_dim - row.rotary;
-  if (!VEC) {
+  if (SWAP) {
+    row.items = static_cast<uint32_t>(row.head_dim / V);
+    row.slots = 64u / row.items;
+  } else if (!VEC) {
     row.items = static_cast<uint32_t>(row.head_dim / 2);
   } else if (LAYOUT == 0) {
     row.items = static_cast<uint32_t>((row.head_dim + V - 1) / V);
@@ -270,24 +340,26 @@ void launch_at(const AtAngles& an, AtRow row, AtView (&v)[2], hipStream_t st) {
     t.ystep = t.ys[t.head_at] * t.chunks;
     t.n1 = static_cast<uint32_t>(w.n[1]);
     t.n2 = static_cast<uint32_t>(w.n[2]);
-    t.items = static_cast<uint32_t>(w.n[0] * w.n[1] * w.n[2] * row.items);
-    t.blocks = (t.items + 255) / 256;
+    t.items = static_cast<uint32_t>(w.n[0] * w.n[1] * w.n[2] * (SWAP ? 1 : row.items));
+    const uint32_t block = SWAP ? 4 * row.slots : 256;
+    t.blocks = (t.items + block - 1) / block;
     blocks += t.blocks;
   }
   if (blocks == 0) return;
-  // Streams larger than the caches are touched once: nontemporal -- but not where an item's two vectors lie in halves that are
-  // no whole lines, whose other parts another access fetches (us: 160 MB of bf16 heads of 96 60.9 nontemporal, 45.0
-  // not; of 80 elements, half of them rotated, in 270 MB 104.6 and 81.1; 128, a quarter, 77.8 and 62.9; whole lines, 128 rotated,
-  // 55.9 and 61.2).
-  constexpr int kLine = 128;
-  const int64_t bytes = rows * row.head_dim * static_cast<int64_t>(sizeof(T));
-  const bool lines = LAYOUT == 0 || (half * static_cast<int>(sizeof(T)) % kLine == 0 &&
-                                     row.head_dim * static_cast<int>(sizeof(T)) % kLine == 0);
-  auto kernel = rope_at_kernel<T, LAYOUT, VEC, false, U>;
-  if constexpr (!VEC || U > 2 - LAYOUT) {  // calls of fewer heads an item are smaller than that
-    if (lines && bytes > kNontemporalBytes) kernel = rope_at_kernel<T, LAYOUT, VEC, true, U>;
+  // Streams larger than the caches are touched once: nontemporal, where a wave's access covers whole lines -- not the two
+  // halves of rotate-half rows apart (us: 160 MB of bf16 heads of 96 60.0 nontemporal, 50.2 not; 128, a quarter
+  // rotated, 77.0 and 61.3).
+  const bool large = rows * row.head_dim * static_cast<int64_t>(sizeof(T)) > kNontemporalBytes;
+  const auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, an, row, v[0].t, v[1].t);
+  };
+  if constexpr (SWAP) {
+    large ? run(rope_swap_kernel<T, true, U>) : run(rope_swap_kernel<T, false, U>);
+  } else if constexpr (LAYOUT == 0 && (!VEC || U > 2)) {  // calls of fewer heads an item are smaller than that
+    large ? run(rope_at_kernel<T, LAYOUT, VEC, true, U>) : run(rope_at_kernel<T, LAYOUT, VEC, false, U>);
+  } else {
+    run(rope_at_kernel<T, LAYOUT, VEC, false, U>);
   }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, an, row, v[0].t, v[1].t);
 }
 
 template <typename T>
@@ -296,6 +368,10 @@ void launch_layout(int layout, const AtAngles& an, const AtRow& row, AtView (&v)
   // what few items there are of a small call would only lengthen.  us, one / two / four heads: 335 MB of bf16 heads of 128
   // interleaved 85.3 / 59.7 / 55.9, rotate-half 71.8 / 56.0 / 57.3; 1.3e6 vectors interleaved 13.3 / 11.5 / 10.5, rotate-half
   // 11.9 / 10.2 / 10.6; 164000 4.5 / 4.4 / 4.8; 10240 3.8 / 4.1 / 4.4.
+  // Large rotate-half calls swap pairs between lanes, four heads an item (us, vectors of both halves a lane / swapped: bf16
+  // heads of 64 34.4 / 29.1, of 96 51.3 / 43.6, of 80 43.9 / 37.4, of 128, a quarter rotated, 62.2 / 54.5, whole 55.6 / 55.2;
+  // fp32 of 64, half rotated, 49.2 / 44.0; 2^21 vectors 13.1 / 12.6, 2^20 8.2 / 7.8, 2^19 5.4 / 5.4, 2^18 4.3 / 4.3, fewer
+  // 3.5 / 3.8).
   constexpr int V = Elem<T>::VEC;
   constexpr int64_t kTwoHeads = 65536, kFourHeads = int64_t{1} << 20;
   const int rest = row.head_dim - row.rotary;
@@ -314,6 +390,8 @@ void launch_layout(int layout, const AtAngles& an, const AtRow& row, AtView (&v)
     launch_at<T, 1, false, 1>(an, row, v, st);
   } else if (vectors < kTwoHeads) {
     launch_at<T, 1, true, 1>(an, row, v, st);
+  } else if (vectors >= kFourHeads && row.rotary / 2 % V == 0 && row.head_dim % V == 0 && row.head_dim <= 64 * V) {
+    launch_at<T, 1, true, 4, true>(an, row, v, st);
   } else {
     launch_at<T, 1, true, 2>(an, row, v, st);
   }
@@ -356,7 +434,7 @@ extern "C" int pt_rope_at(const void* x0, void* y0, const int64_t* desc0, const 
     return fail(PT_EUNSUPPORTED, "pt_rope_at: too many rows for one launch");
   const AtAngles an{turns, positions, position_batch_stride, position_seq_stride, position_offset,
                     position_bytes == 8 ? 1 : 0, scale, inverse ? -1.0f : 1.0f};
-  const AtRow row{static_cast<int>(head_dim), static_cast<int>(rotary_dim), 0};
+  const AtRow row{static_cast<int>(head_dim), static_cast<int>(rotary_dim), 0, 0};
   hipStream_t st = as_stream(stream);
   if (dtype == PT_FLOAT32) {
     launch_layout<float>(layout, an, row, v, st);

@@ -284,3 +284,21 @@ def test_training_after_an_inference_pass(gpu):
     up = randn(q.shape, torch.float32, gpu, 2)
     (grad,) = torch.autograd.grad(out, q, up)
     check(grad, up, 3, f, "interleaved", inverse=True)
+
+
+@pytest.mark.parametrize("dtype,dim,part", [(torch.bfloat16, 96, 96), (torch.float16, 80, 48), (torch.float32, 64, 32),
+                                            (torch.bfloat16, 128, 16), (torch.float32, 8, 8), (torch.bfloat16, 512, 512),
+                                            (torch.float16, 520, 256), (torch.float16, 72, 40)])
+@pytest.mark.parametrize("heads,memory", [(33, "bshd"), (7, "bhsd"), (6, "slice")])
+def test_large_rotate_half_rows(gpu, dtype, dim, part, heads, memory):
+    """2^20 vectors and more, where lanes swap their pairs' elements: rows that do and do not divide a wave, head counts that
+    are no multiples of four, a head or half that is no whole number of vectors or wider than a wave."""
+
+    per = 16 // torch.empty((), dtype=dtype).element_size()
+    seq = (1 << 20) * per // (2 * (heads + 3) * dim) + 5
+    f = RotaryFrequencies(part, 5e5, scaling=YARN)
+    q, k = states(2, heads, seq, dim, dtype, gpu, 3, memory), states(2, 3, seq, dim, dtype, gpu, 4, memory)
+    positions = torch.randint(0, 1 << 30, (2, seq), device=gpu)
+    a, b = triton_apply_rotary_at(q, k, positions, f, layout="rotate_half")
+    check(a, q, positions, f, "rotate_half")
+    check(b, k, positions, f, "rotate_half")
