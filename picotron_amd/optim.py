@@ -275,25 +275,37 @@ class AdamW8bit(Optimizer):
             for flag in ("amsgrad", "maximize"):
                 if group.get(flag, False):
                     raise ValueError(f"AdamW8bit does not take a state of {flag}=True")
-        super().load_state_dict(state_dict)
+        super().load_state_dict({**state_dict, "state": self._in_codes(state_dict)})
         shared: dict[tuple, Tensor] = {}
         capturable = {id(p): i for i, group in enumerate(self.param_groups) if group["capturable"] for p in group["params"]}
         for p, state in self.state.items():
-            for codes, scales, top in zip(_CODES, _SCALES, (TOP_M, TOP_V)):
-                if codes not in state:
-                    continue
-                if scales in state:  # torch has cast the bytes to the parameter's dtype, which holds them exactly
-                    state[codes] = state[codes].to(torch.uint8).contiguous()
-                    state[scales] = state[scales].to(torch.uint8).contiguous()
-                    continue
-                values = torch.zeros(_blocks(p) * BLOCK, dtype=torch.float32, device=p.device)
-                values[:p.numel()] = state[codes].float().reshape(-1)
-                nearest = torch.full((_blocks(p), BLOCK), 1 << 19, dtype=torch.int32, device=p.device)
-                state[codes], state[scales] = encode(values.view(-1, BLOCK), nearest, top)
+            for key in (*_CODES, *_SCALES):
+                if key in state:  # torch has cast the bytes to the parameter's dtype, which holds them exactly
+                    state[key] = state[key].to(torch.uint8).contiguous()
             if id(p) in capturable and "step" in state:
                 # equal counts of a launch share a tensor again, as they did before
                 key = (capturable[id(p)], p.dtype, p.device, float(state["step"]))
                 state["step"] = shared.setdefault(key, torch.as_tensor(state["step"], dtype=torch.float32, device=p.device))
+
+    def _in_codes(self, state_dict: dict) -> dict:
+        """The parameters' states of ``state_dict``, a torch AdamW's moments as codes.  They are rounded from the values given:
+        torch's loading casts them to the parameter's dtype first, and fp16 has no second moment below 3e-8."""
+
+        loaded = dict(state_dict["state"])
+        names = [name for group in state_dict["param_groups"] for name in group["params"]]
+        for name, p in zip(names, [p for group in self.param_groups for p in group["params"]]):
+            if not all(key in loaded.get(name, ()) for key in _CODES) or _SCALES[0] in loaded[name]:
+                continue
+            state = loaded[name] = dict(loaded[name])
+            for codes, scales, top in zip(_CODES, _SCALES, (TOP_M, TOP_V)):
+                if state[codes].numel() != p.numel():
+                    raise ValueError(f"AdamW8bit cannot take a state whose {codes} has {state[codes].numel()} elements for a "
+                                     f"parameter of {p.numel()}")
+                values = torch.zeros(_blocks(p) * BLOCK, dtype=torch.float32, device=p.device)
+                values[:p.numel()] = state[codes].to(p.device, torch.float32).reshape(-1)
+                nearest = torch.full((_blocks(p), BLOCK), 1 << 19, dtype=torch.int32, device=p.device)
+                state[codes], state[scales] = encode(values.view(-1, BLOCK), nearest, top)
+        return loaded
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)

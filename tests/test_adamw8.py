@@ -301,3 +301,45 @@ def test_launches_do_not_share_a_step_count():
     _one_count_a_launch(restored)
     restored.step()
     assert [float(restored.state[p]["step"]) for p in again] == [3.0] * 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_small_moments_of_torch_adamw_are_taken(dtype):
+    """Second moments far below fp16's smallest number: the codes come from the values given, not from a cast of them."""
+
+    torch.manual_seed(4)
+    p = torch.nn.Parameter(torch.randn(300))
+    theirs = torch.optim.AdamW([p], lr=1e-4)
+    p.grad = torch.randn(300) * 1e-5
+    theirs.step()
+    q = torch.nn.Parameter(p.detach().to(dtype))
+    ours = AdamW8bit([q], lr=1e-4)
+    ours.load_state_dict(theirs.state_dict())
+    m, v, _ = ours.moments()
+    state = theirs.state[p]
+    # half a step of 1/8, or of the lowest code (2^-17 and 2^-33 of the largest); a positive second moment takes that code at least
+    for got, want, low in ((m[:300], state["exp_avg"], 2.0**-17), (v[:300], state["exp_avg_sq"], 2.0**-32)):
+        assert ((got - want).abs() <= want.abs() / 16 + want.abs().max() * low).all()
+    assert (v[:300] > 0).all()
+    before = q.detach().float()
+    q.grad = torch.zeros_like(q)
+    ours.step()
+    # lr * m / sqrt(v) of one earlier gradient, (0.9 * 0.1 / 0.19) / sqrt(0.999 * 0.001 / 0.002) < 1 before the codes' roundings
+    # (1/16 of m, 1/32 of the root, and a step of v's lowest code), the decay of 1e-6, and a step of the type
+    assert ((q.float() - before).abs() <= 2e-4 + 1e-6 * before.abs() + torch.finfo(dtype).eps * before.abs()).all()
+
+
+def test_moments_of_another_size_are_refused():
+    p, q = torch.nn.Parameter(torch.zeros(300)), torch.nn.Parameter(torch.zeros(300))
+    theirs, ours = torch.optim.AdamW([p]), AdamW8bit([q])
+    p.grad = q.grad = torch.ones(300)
+    theirs.step()
+    ours.step()
+    before = copy.deepcopy(ours.state_dict())
+    for key in ("exp_avg", "exp_avg_sq"):
+        bad = copy.deepcopy(theirs.state_dict())
+        bad["state"][0][key] = torch.ones(1)
+        with pytest.raises(ValueError, match=key):
+            ours.load_state_dict(bad)
+    for key, value in before["state"][0].items():
+        assert torch.equal(ours.state[q][key], value)
