@@ -34,6 +34,7 @@ _MIN_SCALE = 16
 _MASK = 0xFFFFFFFF
 _CODES = ("exp_avg", "exp_avg_sq")
 _SCALES = ("exp_avg_scale", "exp_avg_sq_scale")
+_OPTIONS = ("seed", "stochastic_rounding", "capturable")
 
 
 def _signed(x: int) -> int:
@@ -269,13 +270,17 @@ class AdamW8bit(Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Restores a state of this optimizer, or of a ``torch.optim.AdamW`` over the same parameters (its fp32 moments are
-        rounded to the nearest codes)."""
+        rounded to the nearest codes).  Options that its groups lack (seed and rounding, from a torch AdamW) stay as they are."""
 
         for group in state_dict["param_groups"]:
             for flag in ("amsgrad", "maximize"):
                 if group.get(flag, False):
                     raise ValueError(f"AdamW8bit does not take a state of {flag}=True")
-        super().load_state_dict({**state_dict, "state": self._in_codes(state_dict)})
+        # a torch AdamW's groups have no options of this optimizer's own: it keeps the ones it has
+        groups = [{**{key: own[key] for key in _OPTIONS}, **group}
+                  for own, group in zip(self.param_groups, state_dict["param_groups"])]
+        groups += state_dict["param_groups"][len(groups):]  # more of them than here: refused by torch
+        super().load_state_dict({**state_dict, "state": self._in_codes(state_dict), "param_groups": groups})
         shared: dict[tuple, Tensor] = {}
         capturable = {id(p): i for i, group in enumerate(self.param_groups) if group["capturable"] for p in group["params"]}
         for p, state in self.state.items():
@@ -309,7 +314,7 @@ class AdamW8bit(Optimizer):
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
-        for group in self.param_groups:  # a torch AdamW's groups have none of these
+        for group in self.param_groups:  # a torch AdamW's, from a hook of the loading, have none of these
             group.setdefault("seed", 0)
             group.setdefault("stochastic_rounding", True)
             group.setdefault("capturable", False)

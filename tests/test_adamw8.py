@@ -343,3 +343,20 @@ def test_moments_of_another_size_are_refused():
             ours.load_state_dict(bad)
     for key, value in before["state"][0].items():
         assert torch.equal(ours.state[q][key], value)
+
+
+def test_options_stay_where_a_loaded_group_has_none():
+    ps = [torch.nn.Parameter(torch.zeros(3)) for _ in range(4)]
+    ours = AdamW8bit([dict(params=ps[:1], seed=5), dict(params=ps[1:2], stochastic_rounding=True)], lr=1.0, seed=17,
+                     stochastic_rounding=False, capturable=True)
+    theirs = torch.optim.AdamW([dict(params=ps[2:3]), dict(params=ps[3:], lr=3e-3)], lr=2e-3)
+    state = theirs.state_dict()
+    for group in state["param_groups"]:
+        group.pop("capturable", None)
+    ours.load_state_dict(state)
+    assert [(g["seed"], g["stochastic_rounding"], g["capturable"], g["lr"]) for g in ours.param_groups] == [
+        (5, False, True, 2e-3), (17, True, True, 3e-3)]
+    with pytest.raises(ValueError, match="groups"):
+        ours.load_state_dict(torch.optim.AdamW(ps[2:]).state_dict())
+    with pytest.raises(ValueError, match="groups"):
+        ours.load_state_dict(torch.optim.AdamW([dict(params=[p]) for p in ps[1:]]).state_dict())
