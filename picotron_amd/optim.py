@@ -282,15 +282,23 @@ class AdamW8bit(Optimizer):
         groups += state_dict["param_groups"][len(groups):]  # more of them than here: refused by torch
         super().load_state_dict({**state_dict, "state": self._in_codes(state_dict), "param_groups": groups})
         shared: dict[tuple, Tensor] = {}
-        capturable = {id(p): i for i, group in enumerate(self.param_groups) if group["capturable"] for p in group["params"]}
+        group_of = {id(p): i for i, group in enumerate(self.param_groups) for p in group["params"]}
         for p, state in self.state.items():
             for key in (*_CODES, *_SCALES):
                 if key in state:  # torch has cast the bytes to the parameter's dtype, which holds them exactly
                     state[key] = state[key].to(torch.uint8).contiguous()
-            if id(p) in capturable and "step" in state:
-                # equal counts of a launch share a tensor again, as they did before
-                key = (capturable[id(p)], p.dtype, p.device, float(state["step"]))
-                state["step"] = shared.setdefault(key, torch.as_tensor(state["step"], dtype=torch.float32, device=p.device))
+            if "step" not in state or id(p) not in group_of:
+                continue
+            # torch hands a count over as it is, or on the device (of a fused AdamW): it becomes this optimizer's own, on the host
+            # or, where it is to be captured, one for each launch again, as before
+            step = float(state["step"])
+            if self.param_groups[group_of[id(p)]]["capturable"]:
+                key = (group_of[id(p)], p.dtype, p.device, step)
+                if key not in shared:
+                    shared[key] = torch.tensor(step, dtype=torch.float32, device=p.device)
+                state["step"] = shared[key]
+            else:
+                state["step"] = torch.tensor(step, dtype=torch.float32, device="cpu")
 
     def _in_codes(self, state_dict: dict) -> dict:
         """The parameters' states of ``state_dict``, a torch AdamW's moments as codes.  They are rounded from the values given:

@@ -360,3 +360,33 @@ def test_options_stay_where_a_loaded_group_has_none():
         ours.load_state_dict(torch.optim.AdamW(ps[2:]).state_dict())
     with pytest.raises(ValueError, match="groups"):
         ours.load_state_dict(torch.optim.AdamW([dict(params=[p]) for p in ps[1:]]).state_dict())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("mine", [True, False])
+def test_loaded_counts_are_the_optimizers_own(capturable, mine):
+    """The count of the optimizer that the state came from does not move with this one's."""
+
+    p, q = torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(5))
+    first = AdamW8bit([p], capturable=capturable) if mine else torch.optim.AdamW([p])
+    p.grad = q.grad = torch.ones(5)
+    first.step()
+    second = AdamW8bit([q], capturable=capturable)
+    second.load_state_dict(first.state_dict())
+    second.step()
+    assert float(first.state[p]["step"]) == 1.0 and float(second.state[q]["step"]) == 2.0
+
+
+def test_loaded_counts_are_fp32_scalars():
+
+    p = torch.nn.Parameter(torch.ones(5))
+    theirs = torch.optim.AdamW([p])
+    p.grad = torch.ones(5)
+    theirs.step()
+    state = theirs.state_dict()
+    state["param_groups"][0]["fused"] = True
+    state["state"][0]["step"] = torch.tensor(1.0, dtype=torch.float64)
+    ours = AdamW8bit([p])
+    ours.load_state_dict(state)
+    step = ours.state[p]["step"]
+    assert step.device.type == "cpu" and step.dtype == torch.float32 and step.shape == () and float(step) == 1.0
