@@ -462,10 +462,15 @@ def _check_group_8bit(group: dict) -> None:
 
 def _run_8bit(optimizer: AdamW8bit, groups, device: torch.device, grad_scale: Tensor | None = None) -> None:
     launches = []
+    counted: set[int] = set()  # a count that parameters share (as those of a capturable group do) advances once
     for group, params, states, step, seed in optimizer.buckets(groups):
         host_table, blocks = ops.adamw8_table(params, [p.grad for p in params], states)
-        launches.append((_device_table(host_table, device), blocks, params[0].dtype, [state["step"] for state in states],
-                         group, step, seed))
+        steps = []
+        for state in states:
+            if id(state["step"]) not in counted:
+                counted.add(id(state["step"]))
+                steps.append(state["step"])
+        launches.append((_device_table(host_table, device), blocks, params[0].dtype, steps, group, step, seed))
     _committed(_launch_8bit, launches, grad_scale)
 
 
@@ -475,7 +480,7 @@ def _launch_8bit(launches: list, grad_scale: Tensor | None) -> None:
             step = _next_step(step)
             if _lib.native is not None and all(s.is_cpu and s.dtype == torch.float32 for s in steps):
                 _lib.native.advance_steps(steps)
-            else:
+            elif steps:
                 torch._foreach_add_(steps, 1.0)
         beta1, beta2 = group["betas"]
         ops.adamw8_step(table, blocks, dtype, lr=group["lr"], beta1=beta1, beta2=beta2, eps=group["eps"],

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from picotron_amd import _lib, ops
+from picotron_amd.nn.triton_kernels import adamw
 from picotron_amd.nn.triton_kernels import AdamWStepWithFallback, TritonAdamWUnavailable, triton_adamw_step, triton_clip_grad_norm_and_step
 from picotron_amd.optim import BLOCK, TOP_M, TOP_V, AdamW8bit, decode, encode, mixed_seed, random_bits
 
@@ -390,3 +391,26 @@ def test_loaded_counts_are_fp32_scalars():
     ours.load_state_dict(state)
     step = ours.state[p]["step"]
     assert step.device.type == "cpu" and step.dtype == torch.float32 and step.shape == () and float(step) == 1.0
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_shared_count_advances_once(monkeypatch, native):
+    """A capturable group's parameters share one count, and still do when the group is no longer capturable.  (The launches
+    themselves are left out.)"""
+
+    params, optimizer = _trained(capturable=True)
+    other, plain = _trained(capturable=True)
+    steps = []
+    monkeypatch.setattr(adamw, "_device_table", lambda table, device: table)
+    monkeypatch.setattr(ops, "adamw8_step", lambda *args, step, **options: steps.append(step))
+    if not native:
+        monkeypatch.setattr(_lib, "native", None)
+    for o, ps in ((optimizer, params), (plain, other)):
+        o.param_groups[0]["capturable"] = False
+        o.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(3))], lr=0.5))
+        last = o.param_groups[1]["params"][0]
+        last.grad = torch.ones(3)
+        o._new_state(last, False)["step"] = o.state[ps[0]]["step"]  # a program may share it between groups
+    adamw._run_8bit(optimizer, optimizer._with_gradients(), torch.device("cpu"))
+    plain.step()
+    assert steps == [4.0, 4.0] and float(optimizer.state[params[0]]["step"]) == float(plain.state[other[0]]["step"]) == 4.0

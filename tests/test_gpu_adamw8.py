@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from gpu_util import randn
-from picotron_amd import ops
+from picotron_amd import _lib, ops
 from picotron_amd.nn.triton_kernels import (
     AdamWStepWithFallback,
     TritonAdamWUnavailable,
@@ -372,3 +372,27 @@ def test_scaled_loops_take_the_pytorch_step(gpu):
         assert torch.equal(p, q)
     with pytest.raises(TritonAdamWUnavailable):
         triton_unscale_clip_and_step(fused, 4.0, 1.0, parameters=a)
+
+
+@pytest.mark.parametrize("count", ["host", "device"])
+@pytest.mark.parametrize("native", [True, False])
+def test_a_shared_count_advances_once(gpu, monkeypatch, count, native):
+    """Parameters of a capturable group share their count, also when the group stops being capturable, and a program may share
+    one between its host counts: the fused step advances it as the plain form does."""
+
+    if not native:
+        monkeypatch.setattr(_lib, "extension", lambda: None)
+        monkeypatch.setattr(_lib, "native", None)
+    (a, fused), (b, plain) = pair([(300,), (1000,), (7,)], torch.float32, gpu, capturable=count == "device")
+    for step in range(4):
+        gradients(step, a, b)
+        triton_adamw_step(fused)
+        plain.step()
+        if step == 0:
+            for optimizer, ps in ((fused, a), (plain, b)):
+                optimizer.param_groups[0]["capturable"] = False
+                for p in ps:
+                    optimizer.state[p]["step"] = optimizer.state[ps[0]]["step"]
+        assert float(fused.state[a[0]]["step"]) == step + 1.0
+        same_codes(a, b, fused, plain)
+        close_parameters(a, b, step + 1)
