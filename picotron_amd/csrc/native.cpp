@@ -295,6 +295,12 @@ void rope_desc(const at::Tensor& x, const at::Tensor& y, int64_t (&d)[9]) {
   }
 }
 
+// As ops._rope_out.
+at::Tensor rope_out(const at::Tensor& x) {
+  at::Tensor y = at::empty_like(x);
+  return y.stride(3) == 1 ? y : at::empty(x.sizes(), x.options());
+}
+
 // (x0, x1 or None, cos, sin, layout, inverse, stream) -> (y0, y1 or None)
 PT_FN(rope, 7)
   const at::Tensor *x0 = plain(a[0]), *c = plain(a[2]), *s = plain(a[3]);
@@ -308,10 +314,9 @@ PT_FN(rope, 7)
     return none();
   void* const stream = as_stream(a[6]);
   NoGil nogil;
-  // empty_like keeps a dense input's stride order
-  at::Tensor y0 = at::empty_like(*x0);
+  at::Tensor y0 = rope_out(*x0);
   std::optional<at::Tensor> y1;
-  if (x1 != nullptr) y1 = at::empty_like(*x1);
+  if (x1 != nullptr) y1 = rope_out(*x1);
   int64_t d0[9], d1[9];
   rope_desc(*x0, y0, d0);
   if (x1 != nullptr) rope_desc(*x1, *y1, d1);
@@ -323,12 +328,6 @@ PT_FN(rope, 7)
   if (rc != PT_OK) return PyLong_FromLong(rc);
   return tuple(y0, y1);
 PT_END
-
-// As ops._rope_at_out.
-at::Tensor rope_at_out(const at::Tensor& x) {
-  at::Tensor y = at::empty_like(x);
-  return y.stride(3) == 1 ? y : at::empty(x.sizes(), x.options());
-}
 
 // (x0, x1 or None, turns, positions or None, offset, scale, layout, inverse, stream) -> (y0, y1 or None)
 PT_FN(rope_at, 9)
@@ -355,9 +354,9 @@ PT_FN(rope_at, 9)
   }
   void* const stream = as_stream(a[8]);
   NoGil nogil;
-  at::Tensor y0 = rope_at_out(*x0);
+  at::Tensor y0 = rope_out(*x0);
   std::optional<at::Tensor> y1;
-  if (x1 != nullptr) y1 = rope_at_out(*x1);
+  if (x1 != nullptr) y1 = rope_out(*x1);
   int64_t d0[9], d1[9];
   rope_desc(*x0, y0, d0);
   if (x1 != nullptr) rope_desc(*x1, *y1, d1);

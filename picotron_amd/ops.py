@@ -352,6 +352,14 @@ def _rope_desc(x: Tensor, y: Tensor) -> ctypes.Array:
     )
 
 
+def _rope_out(x: Tensor) -> Tensor:
+    """A new tensor like ``x`` with a contiguous head_dim: empty_like keeps a dense input's stride order, so that a
+    (B, S, H, D)-memory view comes back as one, but moves head_dim outwards for windows that overlap."""
+
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def rope(
     x0: Tensor,
     cos: Tensor,
@@ -392,9 +400,7 @@ def rope(
     sin = sin.contiguous()
     if cos.dim() != 2 or cos.shape != sin.shape or cos.size(1) * 2 != head_dim:
         raise ValueError("RoPE tables must be [seq, head_dim/2]")
-    # empty_like keeps the input's stride order (dense inputs), so a (B,S,H,D)-memory view
-    # comes back with the same memory layout.
-    outs = [torch.empty_like(t) for t in tensors]
+    outs = [_rope_out(t) for t in tensors]
     descs = [_rope_desc(t, o) for t, o in zip(tensors, outs)]
     _lib.raw_call(
         "pt_rope",
@@ -405,13 +411,6 @@ def rope(
         dtype_code(x0.dtype), _stream(device),
     )
     return outs[0], (outs[1] if x1 is not None else None)
-
-
-def _rope_at_out(x: Tensor) -> Tensor:
-    """A new tensor like ``x`` with a contiguous head_dim (which empty_like moves outwards for windows that overlap)."""
-
-    y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _position_strides(positions: Tensor | None, batch: int, seq: int) -> tuple[int, int]:
@@ -475,7 +474,7 @@ def rope_at(
     if not -(1 << 63) <= offset < 1 << 63:
         raise ValueError("the RoPE position offset must fit 64 bits")
     pbs, pss = _position_strides(positions, x0.size(0), x0.size(2))
-    outs = [_rope_at_out(t) for t in tensors]
+    outs = [_rope_out(t) for t in tensors]
     descs = [_rope_desc(t, o) for t, o in zip(tensors, outs)]
     _call_on(
         device,
@@ -1253,7 +1252,7 @@ def _op_rope(x: Tensor, cos: Tensor, sin: Tensor, layout: str, inverse: bool) ->
 
 @_op_rope.register_fake
 def _(x, cos, sin, layout, inverse):
-    return torch.empty_like(x)
+    return _rope_out(x)
 
 
 @torch.library.custom_op("picotron_amd::rope_pair", mutates_args=())
@@ -1266,7 +1265,7 @@ def _op_rope_pair(
 
 @_op_rope_pair.register_fake
 def _(x0, x1, cos, sin, layout, inverse):
-    return torch.empty_like(x0), torch.empty_like(x1)
+    return _rope_out(x0), _rope_out(x1)
 
 
 @torch.library.custom_op("picotron_amd::rope_at", mutates_args=())
@@ -1277,7 +1276,7 @@ def _op_rope_at(x: Tensor, turns: Tensor, positions: Tensor | None, offset: int,
 
 @_op_rope_at.register_fake
 def _(x, turns, positions, offset, scale, layout, inverse):
-    return _rope_at_out(x)
+    return _rope_out(x)
 
 
 @torch.library.custom_op("picotron_amd::rope_at_pair", mutates_args=())
@@ -1289,4 +1288,4 @@ def _op_rope_at_pair(x0: Tensor, x1: Tensor, turns: Tensor, positions: Tensor | 
 
 @_op_rope_at_pair.register_fake
 def _(x0, x1, turns, positions, offset, scale, layout, inverse):
-    return _rope_at_out(x0), _rope_at_out(x1)
+    return _rope_out(x0), _rope_out(x1)

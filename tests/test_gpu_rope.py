@@ -231,3 +231,35 @@ def test_one_and_two_heads_per_item_agree(gpu, dtype, heads, kv_heads, memory):
             close(z, y[:, :, :cut], dtype)
             ref = o_rope.rotate(x, cos, -sin if inverse else sin, "interleaved")
             close(y, ref, dtype, scale=float(x.abs().max()) * float(cos.abs().max()))
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("native", [True, False])
+def test_windows_that_overlap(gpu, monkeypatch, layout, native):
+    """Windows of one row share their elements, so that both dimensions have stride 1; the outputs' head_dim stays contiguous."""
+
+    if not native:
+        monkeypatch.setattr(ops, "_launch", lambda *args: None)
+    for s in (1, 3, 16, 30):
+        q, k = (randn((2, h, 16 + s - 1), torch.float32, gpu, h).unfold(2, 16, 1) for h in (2, 3))
+        cos, sin = o_rope.tables(s, 16, 10_000.0, device=gpu)
+        outs = ops.rope(q, cos, sin, layout=layout, x1=k)
+        single, none = ops.rope(q, cos, sin, layout=layout)
+        assert none is None and torch.equal(single, outs[0])
+        for y, x in zip(outs, (q, k)):
+            assert y.stride(-1) == 1
+            # three roundings of |u| + |w|, each element below 6
+            torch.testing.assert_close(y.double(), o_rope.rotate(x.double(), cos.double(), sin.double(), layout, compute=torch.float64),
+                                       rtol=0, atol=3 * 2.0**-24 * 12)
+
+
+def test_windows_that_overlap_compile(gpu):
+    q = randn((2, 3, 20), torch.float32, gpu, 1).unfold(2, 16, 1)
+    cos, sin = o_rope.tables(5, 16, 10_000.0, device=gpu)
+
+    def turn(x, y):
+        a, b = ops.rope(x, cos, sin, x1=y)
+        return a + 1, b.flatten(), ops.rope(x, cos, sin)[0] + 1
+
+    for got, want in zip(torch.compile(turn, backend="aot_eager", fullgraph=True)(q, q), turn(q, q)):
+        assert torch.equal(got, want) and got.stride() == want.stride()
