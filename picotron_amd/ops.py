@@ -482,7 +482,7 @@ def rope_at(
         x0.data_ptr(), outs[0].data_ptr(), descs[0],
         None if x1 is None else x1.data_ptr(), None if x1 is None else outs[1].data_ptr(),
         None if x1 is None else descs[1],
-        x0.size(-1), 2 * turns.numel(), _ptr(positions) if x0.numel() else None,
+        x0.size(-1), 2 * turns.numel(), _ptr(positions),
         0 if positions is None else positions.element_size(), pbs, pss, int(offset), turns.data_ptr(), float(scale),
         LAYOUTS[layout], int(inverse), dtype_code(x0.dtype),
     )

@@ -302,3 +302,19 @@ def test_large_rotate_half_rows(gpu, dtype, dim, part, heads, memory):
     a, b = triton_apply_rotary_at(q, k, positions, f, layout="rotate_half")
     check(a, q, positions, f, "rotate_half")
     check(b, k, positions, f, "rotate_half")
+
+
+@pytest.mark.parametrize("form", ["each", "one", "int32"])
+def test_a_query_without_heads(gpu, form):
+    """The key is turned at the positions given all the same."""
+
+    f = RotaryFrequencies(16)
+    q, k = torch.empty(2, 0, 5, 16, device=gpu), states(2, 3, 5, 16, torch.float32, gpu, 1)
+    p = torch.randint(0, 1 << 20, (2, 5), device=gpu)
+    p = {"each": p, "one": p[:1], "int32": p.int()}[form]
+    a, b = triton_apply_rotary_at(q, k, p, f)
+    assert a.shape == q.shape
+    check(b, k, p, f, "interleaved")
+    b, a = triton_apply_rotary_at(k, q, p, f)
+    assert a.shape == q.shape
+    check(b, k, p, f, "interleaved")
