@@ -180,6 +180,26 @@ class HipKernelError(RuntimeError):
         self.code = code
 
 
+# entry point -> function of the extension that takes tensors for it, and the extension's other functions
+_LAUNCHERS = {
+    "pt_rmsnorm_fwd": "rmsnorm_fwd",
+    "pt_rmsnorm_bwd": "rmsnorm_bwd",
+    "pt_residual_rmsnorm_fwd": "residual_rmsnorm_fwd",
+    "pt_residual_rmsnorm_bwd": "residual_rmsnorm_bwd",
+    "pt_swiglu_fwd": "swiglu_fwd",
+    "pt_swiglu_bwd": "swiglu_bwd",
+    "pt_rope": "rope",
+    "pt_rope_at": "rope_at",
+    "pt_sequence_log_probs": "sequence_log_probs",
+    "pt_preference_loss": "preference_loss",
+    "pt_sequence_log_probs_bwd": "sequence_log_probs_bwd",
+    "pt_cross_entropy": "cross_entropy",
+    "pt_cross_entropy_shifted": "cross_entropy",
+    "pt_cross_entropy_scale_grad": "cross_entropy_scale_grad",
+    "pt_cross_entropy_shifted_scale_grad": "cross_entropy_scale_grad",
+}
+_NATIVE_PASSES = ("ENTRY_POINTS", "adamw8_scan", "adamw8_table", "adamw_scan", "advance_steps", "bind", "ce_grad_buffer")
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 # entry point -> native launcher taking tensors; filled with the extension
@@ -251,26 +271,14 @@ def _bind_native(lib: ctypes.CDLL) -> None:
     version = getattr(found, "PT_ABI_VERSION", None)
     if version != ABI_VERSION:
         raise HipLibraryUnavailable(f"{found.__file__} has ABI version {version}, expected {ABI_VERSION}; rebuild it")
+    # an older build of the same ABI version lacks what was added since
+    missing = sorted({*_LAUNCHERS.values(), *_NATIVE_PASSES}.difference(dir(found)))
+    if missing:
+        raise HipLibraryUnavailable(f"{found.__file__} lacks {', '.join(missing)}; rebuild it")
     for name in found.ENTRY_POINTS:
         found.bind(name, ctypes.cast(getattr(lib, name), c_void_p).value)
     native = found
-    _launchers.update(
-        pt_rmsnorm_fwd=native.rmsnorm_fwd,
-        pt_rmsnorm_bwd=native.rmsnorm_bwd,
-        pt_residual_rmsnorm_fwd=native.residual_rmsnorm_fwd,
-        pt_residual_rmsnorm_bwd=native.residual_rmsnorm_bwd,
-        pt_swiglu_fwd=native.swiglu_fwd,
-        pt_swiglu_bwd=native.swiglu_bwd,
-        pt_rope=native.rope,
-        pt_rope_at=native.rope_at,
-        pt_sequence_log_probs=native.sequence_log_probs,
-        pt_preference_loss=native.preference_loss,
-        pt_sequence_log_probs_bwd=native.sequence_log_probs_bwd,
-        pt_cross_entropy=native.cross_entropy,
-        pt_cross_entropy_shifted=native.cross_entropy,
-        pt_cross_entropy_scale_grad=native.cross_entropy_scale_grad,
-        pt_cross_entropy_shifted_scale_grad=native.cross_entropy_scale_grad,
-    )
+    _launchers.update((entry, getattr(found, name)) for entry, name in _LAUNCHERS.items())
     _native_tried = True
 
 

@@ -244,3 +244,23 @@ def test_extension_is_bound_when_torch_comes_after_the_library():
            "assert 'torch' not in sys.modules and _lib.native is None\n"
            "import torch\n"
            "assert _lib.extension() is not None and _lib.native is _lib.extension()")
+
+
+def test_an_older_extension_of_the_same_abi_version_is_refused():
+    """One from before a launcher was added: the reason says so, for every operator, and nothing is bound."""
+
+    for name in ("rope_at", "adamw8_scan"):
+        _child("import torch\n"
+               "from picotron_amd import _native, _lib\n"
+               f"del _native.{name}\n"
+               "_native.bind = None  # nothing may be bound\n"
+               "for _ in range(2):\n"
+               f"    assert not _lib.is_available() and 'lacks {name}; rebuild it' in _lib.unavailable_reason()\n"
+               "assert _lib.native is None and not _lib._launchers")
+
+
+def test_extension_has_every_function_that_is_called():
+    used = set()
+    for path in (ROOT / "picotron_amd").rglob("*.py"):
+        used |= set(re.findall(r"\bnative\.([a-z]\w+)\(", path.read_text()))
+    assert used and used <= {*_lib._LAUNCHERS.values(), *_lib._NATIVE_PASSES}
