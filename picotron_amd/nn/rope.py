@@ -23,6 +23,7 @@ from __future__ import annotations
 import math
 import warnings
 from collections.abc import Mapping
+from fractions import Fraction
 
 import torch
 from torch import Tensor, nn
@@ -116,6 +117,19 @@ def _checked_scaling(scaling: Mapping) -> dict:
     return values
 
 
+# pi to 50 digits: a frequency is a binary fraction, and its turns per position are rounded once
+_PI_DIGITS = 31415926535897932384626433832795028841971693993751
+_PI_SCALE = 10**49
+
+
+def _turn_bits(frequency: float) -> int:
+    """``frequency / (2 pi)`` turns as a 64-bit fraction of a turn, right to half its last bit (formed in 64 bits it would
+    be right to 2^-56 of a turn, 1e-4 rad at position 2^40)."""
+
+    numerator, denominator = frequency.as_integer_ratio()
+    return round(Fraction((numerator * _PI_SCALE) << 63, denominator * _PI_DIGITS)) % 2**64
+
+
 class RotaryFrequencies:
     """Radians per position of each rotated pair (``frequencies``, fp64 on the CPU) and the factor on cosine and sine
     (``attention_factor``): ``theta^(-2i/rotary_dim)``, scaled to contexts longer than those of training by ``scaling``:
@@ -185,7 +199,7 @@ class RotaryFrequencies:
                 raise TritonRoPEUnavailable(
                     "HIP RoPE: the frequencies are first used on this device during graph capture; run the same call "
                     "once before capturing it.")
-            bits = [round(math.fmod(f / (2 * math.pi), 1.0) * 2**64) % 2**64 for f in self.frequencies.tolist()]
+            bits = [_turn_bits(f) for f in self.frequencies.tolist()]
             with torch.inference_mode(False):  # a later pass may keep them for its backward
                 found = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64, device="cpu").to(device)
             self._turns[device] = found

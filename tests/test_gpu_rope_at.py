@@ -3,7 +3,9 @@ vectors, positions of every form and size, strided views, its gradients, other s
 
 from __future__ import annotations
 
+import math
 import random
+from fractions import Fraction
 
 import pytest
 import torch
@@ -318,3 +320,24 @@ def test_a_query_without_heads(gpu, form):
     b, a = triton_apply_rotary_at(k, q, p, f)
     assert a.shape == q.shape
     check(b, k, p, f, "interleaved")
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+@pytest.mark.parametrize("far", [2**20, 2**31, 2**40, 2**48])
+def test_far_positions_against_rational_angles(gpu, layout, far):
+    """The angle itself, from the frequencies: position * f / 2 pi modulo 1 in rational numbers."""
+
+    pi = Fraction(31415926535897932384626433832795028841971693993751, 10**49)
+    f = RotaryFrequencies(32, 5e5, scaling=YARN)
+    positions = [far, far - 1, far // 3, -far + 7]
+    x = torch.ones(1, 1, 4, 32, device=gpu)
+    y = triton_apply_rotary_at(x, None, torch.tensor(positions, device=gpu), f, layout=layout)[0][0, 0].double().cpu()
+    a = f.attention_factor
+    for row, p in zip(y, positions):
+        for i, freq in enumerate(f.frequencies.tolist()):
+            angle = 2 * math.pi * float(p * Fraction(freq) / (2 * pi) % 1)
+            u, w = (row[2 * i], row[2 * i + 1]) if layout == "interleaved" else (row[i], row[i + 16])
+            # as check() for |u| + |w| = 2, and the turns' rounding of 2^-65 a position in each of the two terms
+            bound = 2 * a * (3e-7 + 2 * math.pi * abs(p) * 2.0**-65) + 2.0**-24 * 2 * a
+            assert abs(float(u) - a * (math.cos(angle) - math.sin(angle))) <= bound, (p, i)
+            assert abs(float(w) - a * (math.cos(angle) + math.sin(angle))) <= bound, (p, i)

@@ -192,3 +192,12 @@ def test_turns_of_an_inference_pass_serve_training():
         f = RotaryFrequencies(16)
         turns = f.turns(torch.device("cpu"))
     assert not turns.is_inference() and not f.frequencies.is_inference()
+
+
+@pytest.mark.parametrize("dim,theta", [(2, 1e4), (64, 1e4), (128, 5e5), (128, 0.5), (256, 1e9)])
+@pytest.mark.parametrize("scaling", [None, dict(type="linear", factor=3.0), YARN, LLAMA3])
+def test_turns_are_rounded_once(dim, theta, scaling):
+    f = RotaryFrequencies(dim, theta, scaling=scaling)
+    for bits, freq in zip(f.turns(torch.device("cpu")).tolist(), f.frequencies.tolist()):
+        off = (Fraction(bits % 2**64, 2**64) - exact_turns(1, freq)) % 1
+        assert min(off, 1 - off) <= Fraction(1, 2**65)  # PI has as many digits as the turns were formed with
