@@ -153,21 +153,24 @@ class RotaryFrequencies:
             raise ValueError("rope_theta must be positive.")
         self.rotary_dim = rotary_dim
         self.attention_factor = 1.0
-        i = torch.arange(rotary_dim // 2, dtype=torch.float64, device="cpu")
-        if scaling is None:
-            self.frequencies = theta ** (-2.0 * i / rotary_dim)
-        else:
-            self._scale(_checked_scaling(scaling), theta, i)
+        # Python numbers, whatever device or mode torch makes tensors in here; the bits before any tracing of turns()
+        values = self._scaled(_checked_scaling(scaling), theta) if scaling is not None else self._base(theta)
+        self.frequencies = torch.tensor(values, dtype=torch.float64, device="cpu")
+        bits = [_turn_bits(f) for f in values]
+        self._bits = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64, device="cpu")
         self._turns: dict[torch.device, Tensor] = {}
 
-    def _scale(self, s: dict, theta: float, i: Tensor) -> None:
+    def _base(self, theta: float) -> list[float]:
+        return [theta ** (-2.0 * i / self.rotary_dim) for i in range(self.rotary_dim // 2)]
+
+    def _scaled(self, s: dict, theta: float) -> list[float]:
         dim, factor = self.rotary_dim, s["factor"]
         if s["type"] == "ntk":
             theta = theta * factor ** (dim / max(dim - 2, 1))
-        f = theta ** (-2.0 * i / dim)
+        base = self._base(theta)
         if s["type"] == "linear":
-            f = f / factor
-        elif s["type"] == "yarn":
+            return [f / factor for f in base]
+        if s["type"] == "yarn":
             length = s["original_max_positions"]
             if theta == 1.0:
                 raise ValueError("rotary scaling 'yarn' needs a theta other than 1.")
@@ -177,31 +180,30 @@ class RotaryFrequencies:
 
             low = max(math.floor(pair_with(s["beta_fast"])), 0)
             high = min(math.ceil(pair_with(s["beta_slow"])), dim - 1)
-            ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
-            f = f * (1 - ramp) + f / factor * ramp
             given = s["attention_factor"]
             self.attention_factor = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
-        elif s["type"] == "llama3":
+            ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(len(base))]
+            return [f * (1 - t) + f / factor * t for f, t in zip(base, ramp)]
+        if s["type"] == "llama3":
             low, high = s["low_freq_factor"], s["high_freq_factor"]
             if high <= low:
                 raise ValueError("rotary scaling 'llama3' needs high_freq_factor above low_freq_factor.")
-            turns = s["original_max_positions"] * f / (2 * math.pi)
-            keep = ((turns - low) / (high - low)).clamp(0, 1)
-            f = f / factor * (1 - keep) + f * keep
-        self.frequencies = f
+            turns = [s["original_max_positions"] * f / (2 * math.pi) for f in base]
+            keep = [min(max((t - low) / (high - low), 0.0), 1.0) for t in turns]
+            return [f / factor * (1 - k) + f * k for f, k in zip(base, keep)]
+        return base
 
     def turns(self, device: torch.device) -> Tensor:
         """int64 on ``device``: the bits of each frequency as a fraction of a turn per position, times 2^64."""
 
         found = self._turns.get(device)
         if found is None:
-            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            if device.type == "cuda" and not torch.compiler.is_compiling() and torch.cuda.is_current_stream_capturing():
                 raise TritonRoPEUnavailable(
                     "HIP RoPE: the frequencies are first used on this device during graph capture; run the same call "
                     "once before capturing it.")
-            bits = [_turn_bits(f) for f in self.frequencies.tolist()]
             with torch.inference_mode(False):  # a later pass may keep them for its backward
-                found = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64, device="cpu").to(device)
+                found = self._bits.to(device)
             self._turns[device] = found
         return found
 

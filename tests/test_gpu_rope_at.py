@@ -341,3 +341,16 @@ def test_far_positions_against_rational_angles(gpu, layout, far):
             bound = 2 * a * (3e-7 + 2 * math.pi * abs(p) * 2.0**-65) + 2.0**-24 * 2 * a
             assert abs(float(u) - a * (math.cos(angle) - math.sin(angle))) <= bound, (p, i)
             assert abs(float(w) - a * (math.cos(angle) + math.sin(angle))) <= bound, (p, i)
+
+
+def test_first_use_compiles_into_one_graph(gpu):
+    """Nothing has run the module before it is compiled."""
+
+    rope = RotaryEmbedding(64, 1e4, use_triton_rope=True, rotary_dim=32, scaling=YARN)
+    q, k = (states(2, h, 6, 64, torch.float32, gpu, h).requires_grad_() for h in (4, 2))
+    p = torch.arange(6, device=gpu).repeat(2, 1)
+    out = torch.compile(rope, backend="aot_eager", fullgraph=True)(q, k, p)
+    assert not rope._triton_fallback_warned
+    eager = rope(q, k, p)
+    assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+    check(out[0].detach(), q.detach(), p, rope.frequencies, "interleaved")

@@ -201,3 +201,22 @@ def test_turns_are_rounded_once(dim, theta, scaling):
     for bits, freq in zip(f.turns(torch.device("cpu")).tolist(), f.frequencies.tolist()):
         off = (Fraction(bits % 2**64, 2**64) - exact_turns(1, freq)) % 1
         assert min(off, 1 - off) <= Fraction(1, 2**65)  # PI has as many digits as the turns were formed with
+
+
+@pytest.mark.parametrize("scaling", [None, YARN, LLAMA3])
+def test_first_use_compiles(scaling):
+    """Nothing has asked for the turns before the module is traced."""
+
+    torch._dynamo.reset()
+    q = torch.randn(1, 2, 3, 8)
+    rope = RotaryEmbedding(8, rotary_dim=4, scaling=scaling)
+    turns = torch.compile(lambda x: rope.frequencies.turns(x.device) + x.sum().long() * 0, backend="aot_eager", fullgraph=True)
+    assert torch.equal(turns(q), RotaryFrequencies(4, scaling=scaling).turns(q.device))
+    assert torch.equal(rope.frequencies.turns(q.device), RotaryFrequencies(4, scaling=scaling).turns(q.device))
+
+
+def test_modules_are_built_without_data():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        RotaryEmbedding(8, rotary_dim=4, scaling=YARN)
