@@ -122,16 +122,17 @@ def triton_apply_rotary_embedding_pair(
 
 
 class _RoPEAtFunction(torch.autograd.Function):
-    """Rotate one or two (B, H, S, D) views at their positions; the backward is the rotation the other way."""
+    """Rotate one or two (B, H, S, D) views at their positions; the backward is the rotation the other way.  (Two named
+    states, the second one None or not: torch.compile calls a forward with variable arguments without its ctx where no input asks for
+    a gradient.)"""
 
     @staticmethod
-    def forward(ctx, how: tuple, turns: Tensor, positions: Tensor | None, *states: Tensor):  # type: ignore[override]
+    def forward(ctx, how: tuple, turns: Tensor, positions: Tensor | None, x0: Tensor, x1: Tensor | None):  # type: ignore[override]
         ctx.set_materialize_grads(False)
         ctx.how = how  # (offset, scale, layout, inverse)
-        ctx.has_positions = positions is not None
         ctx.save_for_backward(turns, *((positions,) if positions is not None else ()))
-        out0, out1 = _rotate_at(how, turns, positions, states)
-        return (out0,) if out1 is None else (out0, out1)
+        out0, out1 = _rotate_at(how, turns, positions, x0, x1)
+        return out0 if out1 is None else (out0, out1)
 
     @staticmethod
     def backward(ctx, *grads: Tensor):  # type: ignore[override]
@@ -139,22 +140,25 @@ class _RoPEAtFunction(torch.autograd.Function):
         offset, scale, layout, inverse = ctx.how
         how = (offset, scale, layout, not inverse)
         present = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
-        results: list[Tensor | None] = [None] * len(grads)
+        results: list[Tensor | None] = [None, None]
         if present:
             g = [_last_dim_contiguous(grads[i]) for i in present]
+            g0, g1 = g[0], g[1] if len(g) > 1 else None
             if torch.is_grad_enabled() and not ops._compiling():
-                d = _RoPEAtFunction.apply(how, turns, positions, *g)  # create_graph=True
+                d = _RoPEAtFunction.apply(how, turns, positions, g0, g1)  # create_graph=True
+                d = (d, None) if g1 is None else d
             else:
-                d = _rotate_at(how, turns, positions, g)
+                d = _rotate_at(how, turns, positions, g0, g1)
             for i, x in zip(present, d):
                 results[i] = x
         return (None, None, None, *results)
 
 
-def _rotate_at(how: tuple, turns: Tensor, positions: Tensor | None, states) -> tuple[Tensor, Tensor | None]:
+def _rotate_at(
+    how: tuple, turns: Tensor, positions: Tensor | None, x0: Tensor, x1: Tensor | None
+) -> tuple[Tensor, Tensor | None]:
     offset, scale, layout, inverse = how
-    return ops.rope_at(states[0], turns, positions=positions, offset=offset, scale=scale, layout=layout, inverse=inverse,
-                       x1=states[1] if len(states) > 1 else None)
+    return ops.rope_at(x0, turns, positions=positions, offset=offset, scale=scale, layout=layout, inverse=inverse, x1=x1)
 
 
 def triton_apply_rotary_at(
@@ -206,6 +210,6 @@ def triton_apply_rotary_at(
     turns, scale = frequencies.turns(query.device), frequencies.attention_factor
     how = (offset, scale, layout, False)
     if plain:
-        return _rotate_at(how, turns, positions, states)
-    out = _RoPEAtFunction.apply(how, turns, positions, *states)
-    return out[0], (out[1] if key is not None else None)
+        return _rotate_at(how, turns, positions, query, key)
+    out = _RoPEAtFunction.apply(how, turns, positions, query, key)
+    return (out, None) if key is None else out

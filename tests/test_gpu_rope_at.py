@@ -354,3 +354,35 @@ def test_first_use_compiles_into_one_graph(gpu):
     eager = rope(q, k, p)
     assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
     check(out[0].detach(), q.detach(), p, rope.frequencies, "interleaved")
+
+
+@pytest.mark.parametrize("how", ["inputs", "no_grad", "one"])
+@pytest.mark.parametrize("pair", [True, False])
+def test_compiles_into_one_graph_without_gradients(gpu, how, pair):
+    """Inference: no input asks for a gradient, or none is recorded, or only one of two asks."""
+
+    f = RotaryFrequencies(32, 1e4, scaling=YARN)
+    q, k = (states(2, h, 6, 64, torch.float32, gpu, h) for h in (4, 2))
+    if how != "inputs":
+        (k if pair else q).requires_grad_()
+    if not pair:
+        k = None
+    p = torch.arange(6, device=gpu).repeat(2, 1)
+
+    def turn(x, y):
+        return triton_apply_rotary_at(x, y, p, f)
+
+    with torch.set_grad_enabled(how != "no_grad"):
+        out = torch.compile(turn, backend="aot_eager", fullgraph=True)(q, k)
+        eager = turn(q, k)
+    check(out[0].detach(), q.detach(), p, f, "interleaved")
+    if pair:
+        check(out[1].detach(), k.detach(), p, f, "interleaved")
+    else:
+        assert out[1] is None
+    if how == "one":
+        leaf, i = (k, 1) if pair else (q, 0)
+        up = randn(leaf.shape, torch.float32, gpu, 5)
+        got, want = (torch.autograd.grad(o[i], leaf, up)[0] for o in (out, eager))
+        assert torch.equal(got, want)
+        check(got, up, p, f, "interleaved", inverse=True)
