@@ -25,40 +25,35 @@ class TritonRoPEUnavailable(RuntimeError):
 
 class _RoPEFunction(torch.autograd.Function):
     """Rotate one or two (B, H, S, D) views by fp32 angle tables (by minus the angles when
-    ``inverse``); the backward is the rotation the other way."""
+    ``inverse``); the backward is the rotation the other way.  (Two named states, the second one
+    None or not: torch.compile calls a forward with variable arguments without its ctx where no
+    input asks for a gradient.)"""
 
     @staticmethod
-    def forward(ctx, layout: str, inverse: bool, cosine: Tensor, sine: Tensor, *states: Tensor):  # type: ignore[override]
+    def forward(ctx, layout: str, inverse: bool, cosine: Tensor, sine: Tensor, x0: Tensor, x1: Tensor | None):  # type: ignore[override]
         ctx.layout = layout
         ctx.inverse = inverse
         ctx.save_for_backward(cosine, sine)
-        ctx.count = len(states)
-        out0, out1 = ops.rope(
-            states[0], cosine, sine, layout=layout, inverse=inverse,
-            x1=states[1] if len(states) > 1 else None,
-        )
-        return (out0,) if out1 is None else (out0, out1)
+        out0, out1 = ops.rope(x0, cosine, sine, layout=layout, inverse=inverse, x1=x1)
+        return out0 if out1 is None else (out0, out1)
 
     @staticmethod
     def backward(ctx, *grads: Tensor):  # type: ignore[override]
         cosine, sine = ctx.saved_tensors
         present = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[4 + i]]
-        results: list[Tensor | None] = [None] * ctx.count
+        results: list[Tensor | None] = [None, None]
         if present:
             g = [_last_dim_contiguous(grads[i]) for i in present]
+            g0, g1 = g[0], g[1] if len(g) > 1 else None
             if torch.is_grad_enabled() and not ops._compiling():
                 # create_graph=True: the backward rotation as this Function again, so that
                 # autograd can differentiate it to any order
-                d = _RoPEFunction.apply(ctx.layout, not ctx.inverse, cosine, sine, *g)
-                d0, d1 = d[0], (d[1] if len(d) > 1 else None)
+                d = _RoPEFunction.apply(ctx.layout, not ctx.inverse, cosine, sine, g0, g1)
+                d = (d, None) if g1 is None else d
             else:
-                d0, d1 = ops.rope(
-                    g[0], cosine, sine, layout=ctx.layout, inverse=not ctx.inverse,
-                    x1=g[1] if len(g) > 1 else None,
-                )
-            results[present[0]] = d0
-            if len(present) > 1:
-                results[present[1]] = d1
+                d = ops.rope(g0, cosine, sine, layout=ctx.layout, inverse=not ctx.inverse, x1=g1)
+            for i, x in zip(present, d):
+                results[i] = x
         return (None, None, None, None, *results)
 
 
@@ -106,7 +101,7 @@ def triton_apply_rotary_embedding(
     _validate([states], cosine, sine)
     if no_graph(states, cosine, sine):
         return ops.rope(states, cosine.float(), sine.float(), layout=layout)[0]
-    return _RoPEFunction.apply(layout, False, cosine.float(), sine.float(), states)[0]
+    return _RoPEFunction.apply(layout, False, cosine.float(), sine.float(), states, None)
 
 
 def triton_apply_rotary_embedding_pair(

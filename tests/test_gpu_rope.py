@@ -263,3 +263,31 @@ def test_windows_that_overlap_compile(gpu):
 
     for got, want in zip(torch.compile(turn, backend="aot_eager", fullgraph=True)(q, q), turn(q, q)):
         assert torch.equal(got, want) and got.stride() == want.stride()
+
+
+@pytest.mark.parametrize("how", ["inputs", "no_grad", "one"])
+@pytest.mark.parametrize("pair", [True, False])
+def test_compiles_into_one_graph_without_gradients(gpu, how, pair):
+    """Inference: no input asks for a gradient, or none is recorded, or only one of two asks."""
+
+    from picotron_amd.nn.triton_kernels import triton_apply_rotary_embedding, triton_apply_rotary_embedding_pair
+
+    q, k = (_bhsd_view(2, 6, h, 64, torch.float32, gpu, h) for h in (4, 2))
+    cos, sin = o_rope.tables(6, 64, 10_000.0, device=gpu)
+    leaf = k if pair else q
+    leaf.requires_grad_(how != "inputs")
+
+    def turn(x, y):
+        return triton_apply_rotary_embedding_pair(x, y, cos, sin) if pair else (triton_apply_rotary_embedding(x, cos, sin),)
+
+    with torch.set_grad_enabled(how != "no_grad"):
+        out = torch.compile(turn, backend="aot_eager", fullgraph=True)(q, k)
+        eager = turn(q, k)
+    for y, e, x in zip(out, eager, (q, k)):
+        assert torch.equal(y, e)
+        close_fp32(y.detach(), o_rope.rotate(x.detach(), cos, sin, compute=torch.float32))
+    if how == "one":
+        up = randn(leaf.shape, torch.float32, gpu, 5)
+        got, want = (torch.autograd.grad(o[-1], leaf, up)[0] for o in (out, eager))
+        assert torch.equal(got, want)
+        close_fp32(got, o_rope.rotate(up, cos, sin, inverse=True, compute=torch.float32))
