@@ -211,8 +211,9 @@ class RotaryFrequencies:
 def apply_rotary_at(
     states: Tensor, positions: Tensor | int | None, frequencies: RotaryFrequencies, *, layout: str = "interleaved"
 ) -> Tensor:
-    """The rotation of ``triton_apply_rotary_at`` in PyTorch: angles in fp64, the rotation in fp32 (fp64 for fp64
-    states), one rounding to the states' type."""
+    """The rotation of ``triton_apply_rotary_at`` in PyTorch: angles as the kernel forms them, position times turns modulo 2^64
+    (a product in fp64 is off by 1e-4 rad at position 2^40), then fp64; the rotation in fp32 (fp64 for fp64 states), one
+    rounding to the states' type."""
 
     seq, dim = states.size(-2), frequencies.rotary_dim
     if dim > states.size(-1):
@@ -221,7 +222,7 @@ def apply_rotary_at(
         positions = torch.arange(seq, device=states.device) + int(positions or 0)
     ops._position_strides(positions, states.size(0), seq)
     positions = positions if positions.dim() == 2 else positions[None]
-    angles = positions[:, None, :, None].double() * frequencies.frequencies.to(states.device)
+    angles = (positions[:, None, :, None].long() * frequencies.turns(states.device)).double() * (math.pi * 2.0**-63)
     compute = torch.promote_types(states.dtype, torch.float32)
     cosine, sine = ((f(angles) * frequencies.attention_factor).to(compute) for f in (torch.cos, torch.sin))
     part = states[..., :dim].to(compute)

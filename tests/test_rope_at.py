@@ -220,3 +220,24 @@ def test_modules_are_built_without_data():
 
     with FakeTensorMode():
         RotaryEmbedding(8, rotary_dim=4, scaling=YARN)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "rotate_half"])
+@pytest.mark.parametrize("far", [2**20, 2**31, 2**40, 2**48])
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32])
+def test_plain_form_at_far_positions(layout, far, dtype):
+    f = RotaryFrequencies(16, 5e5, scaling=YARN)
+    positions = [far, far - 1, far // 3, -far + 7]
+    y = apply_rotary_at(torch.ones(1, 1, 4, 16, dtype=dtype), torch.tensor(positions), f, layout=layout)[0, 0].double()
+    a = f.attention_factor
+    for row, p in zip(y, positions):
+        for i, freq in enumerate(f.frequencies.tolist()):
+            angle = 2 * math.pi * float(exact_turns(p, freq))
+            u, w = (row[2 * i], row[2 * i + 1]) if layout == "interleaved" else (row[i], row[i + 8])
+            # for |u| + |w| = 2: the turns' rounding of 2^-65 a position, the angle's in 64 bits (2^-51), and four roundings of
+            # the type: cosine, its factor, the product, the sum
+            bound = 2 * a * (2 * math.pi * abs(p) * 2.0**-65 + 2.0**-51 + 4 * torch.finfo(dtype).eps / 2)
+            assert abs(float(u) - a * (math.cos(angle) - math.sin(angle))) <= bound, (p, i)
+            assert abs(float(w) - a * (math.cos(angle) + math.sin(angle))) <= bound, (p, i)
+    whole = apply_rotary_at(torch.ones(1, 1, 2, 16), torch.tensor([2**63 - 1, -(2**63)]), f, layout=layout)
+    assert whole.isfinite().all()
