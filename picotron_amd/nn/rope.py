@@ -204,7 +204,8 @@ class RotaryFrequencies:
                     "once before capturing it.")
             with torch.inference_mode(False):  # a later pass may keep them for its backward
                 found = self._bits.to(device)
-            self._turns[device] = found
+            if type(found) is Tensor:  # not a dry run's
+                self._turns[device] = found
         return found
 
 

@@ -351,6 +351,7 @@ def test_first_use_compiles_into_one_graph(gpu):
     p = torch.arange(6, device=gpu).repeat(2, 1)
     out = torch.compile(rope, backend="aot_eager", fullgraph=True)(q, k, p)
     assert not rope._triton_fallback_warned
+    assert [type(t) for t in rope.frequencies._turns.values()] == [torch.Tensor]  # copied once, and kept
     eager = rope(q, k, p)
     assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
     check(out[0].detach(), q.detach(), p, rope.frequencies, "interleaved")

@@ -241,3 +241,13 @@ def test_plain_form_at_far_positions(layout, far, dtype):
             assert abs(float(w) - a * (math.cos(angle) + math.sin(angle))) <= bound, (p, i)
     whole = apply_rotary_at(torch.ones(1, 1, 2, 16), torch.tensor([2**63 - 1, -(2**63)]), f, layout=layout)
     assert whole.isfinite().all()
+
+
+def test_turns_of_a_dry_run_are_not_kept(monkeypatch):
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    f = RotaryFrequencies(8)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        assert isinstance(f.turns(torch.device("cuda", 0)), FakeTensor)
+    assert not f._turns
