@@ -216,6 +216,8 @@ def apply_rotary_at(
     (a product in fp64 is off by 1e-4 rad at position 2^40), then fp64; the rotation in fp32 (fp64 for fp64 states), one
     rounding to the states' type."""
 
+    if layout not in LAYOUTS:
+        raise ValueError(f"RoPE layout must be one of {LAYOUTS}.")
     seq, dim = states.size(-2), frequencies.rotary_dim
     if dim > states.size(-1):
         raise ValueError("RoPE frequencies cover more than the attention head dimension.")

@@ -251,3 +251,8 @@ def test_turns_of_a_dry_run_are_not_kept(monkeypatch):
     with FakeTensorMode(allow_non_fake_inputs=True):
         assert isinstance(f.turns(torch.device("cuda", 0)), FakeTensor)
     assert not f._turns
+
+
+def test_plain_form_refuses_another_layout():
+    with pytest.raises(ValueError, match="layout"):
+        apply_rotary_at(torch.randn(1, 1, 3, 8), 0, RotaryFrequencies(8), layout="half")
