@@ -222,7 +222,7 @@ def apply_rotary_at(
     if dim > states.size(-1):
         raise ValueError("RoPE frequencies cover more than the attention head dimension.")
     if not isinstance(positions, Tensor):
-        positions = torch.arange(seq, device=states.device) + int(positions or 0)
+        positions = torch.arange(seq, device=states.device) + ops._first_position(positions)
     ops._position_strides(positions, states.size(0), seq)
     positions = positions if positions.dim() == 2 else positions[None]
     angles = (positions[:, None, :, None].long() * frequencies.turns(states.device)).double() * (math.pi * 2.0**-63)

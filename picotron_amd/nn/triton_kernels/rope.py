@@ -174,7 +174,7 @@ def triton_apply_rotary_at(
     if isinstance(positions, Tensor):
         require_hip(TritonRoPEUnavailable, "RoPE", *states, positions)
     else:
-        offset, positions = int(positions or 0), None
+        offset, positions = ops._first_position(positions), None
         require_hip(TritonRoPEUnavailable, "RoPE", *states)
     if layout not in ops.LAYOUTS:
         raise TritonRoPEUnavailable(f"RoPE layout must be one of {sorted(ops.LAYOUTS)}.")

@@ -413,6 +413,15 @@ def rope(
     return outs[0], (outs[1] if x1 is not None else None)
 
 
+def _first_position(position) -> int:
+    """The position of a call's first token, from an integer or None (0)."""
+
+    first = int(position or 0)
+    if first != (position or 0):
+        raise ValueError(f"a RoPE position must be an integer, got {position!r}")
+    return first
+
+
 def _position_strides(positions: Tensor | None, batch: int, seq: int) -> tuple[int, int]:
     """(batch stride, sequence stride) of (seq,), (1, seq) or (batch, seq) positions."""
 

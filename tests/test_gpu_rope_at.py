@@ -387,3 +387,20 @@ def test_compiles_into_one_graph_without_gradients(gpu, how, pair):
         got, want = (torch.autograd.grad(o[i], leaf, up)[0] for o in (out, eager))
         assert torch.equal(got, want)
         check(got, up, p, f, "interleaved", inverse=True)
+
+
+def test_a_position_that_is_no_integer_is_refused(gpu):
+    x, f = randn((1, 2, 3, 8), torch.float32, gpu, 1), RotaryFrequencies(8)
+    for state in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="integer"):
+            triton_apply_rotary_at(state, None, 2.7, f)
+
+
+def test_compiled_with_a_moving_position(gpu):
+    """A decode loop that passes the position as a number, which a compiled graph may take as a symbol."""
+
+    f = RotaryFrequencies(8, 5e5)
+    x = randn((2, 3, 1, 8), torch.float32, gpu, 1)
+    turn = torch.compile(lambda x, p: triton_apply_rotary_at(x, None, p, f)[0], backend="aot_eager", fullgraph=True)
+    for p in (0, 1, 17, 2**20, 2**40):
+        assert torch.equal(turn(x, p), triton_apply_rotary_at(x, None, p, f)[0]), p

@@ -256,3 +256,18 @@ def test_turns_of_a_dry_run_are_not_kept(monkeypatch):
 def test_plain_form_refuses_another_layout():
     with pytest.raises(ValueError, match="layout"):
         apply_rotary_at(torch.randn(1, 1, 3, 8), 0, RotaryFrequencies(8), layout="half")
+
+
+@pytest.mark.parametrize("position", [2.7, -0.5, float("nan"), "3"])
+def test_a_position_that_is_no_integer_is_refused(position):
+    x, f = torch.randn(1, 1, 3, 8), RotaryFrequencies(8)
+    for call in (lambda: apply_rotary_at(x, position, f), lambda: RotaryEmbedding(8)(x, x, position), lambda: ops._first_position(position)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_positions_that_are_integers():
+    import numpy as np
+
+    for position in (None, 0, 5, -3, 2**62, True, 4.0, np.int64(7), np.int32(-1)):
+        assert ops._first_position(position) == int(position or 0)
