@@ -245,6 +245,10 @@ class RotaryEmbedding(nn.Module):
     :class:`RotaryFrequencies`'s.  With either, or with positions given to :meth:`forward`, the angles come from the
     positions themselves; without them from fp32 tables, as in the reference."""
 
+    # Of a module whose arguments only the tables take (a theta that is infinite), or that was stored before it had them.
+    frequencies: RotaryFrequencies | None = None
+    _plain = True
+
     def __init__(
         self,
         head_dim: int,
@@ -269,8 +273,13 @@ class RotaryEmbedding(nn.Module):
         self._triton_fallback_warned = False
         if rotary_dim is not None and not 0 < rotary_dim <= head_dim:
             raise ValueError("rotary_dim must be positive and at most head_dim.")
-        self.frequencies = RotaryFrequencies(head_dim if rotary_dim is None else rotary_dim, theta, scaling=scaling)
-        self._plain = scaling is None and self.frequencies.rotary_dim == head_dim
+        try:
+            self.frequencies = RotaryFrequencies(head_dim if rotary_dim is None else rotary_dim, theta, scaling=scaling)
+        except (ValueError, OverflowError):
+            if rotary_dim is not None or scaling is not None:
+                raise
+        else:
+            self._plain = scaling is None and self.frequencies.rotary_dim == head_dim
         # One fp32 table pair per device, as long as the longest sequence seen: position p's
         # angles do not depend on the table length, and the kernel reads rows 0..seq-1 of a
         # longer table, so variable sequence lengths share one pair instead of one each.
@@ -286,6 +295,8 @@ class RotaryEmbedding(nn.Module):
         return tables
 
     def _at(self, query: Tensor, key: Tensor, positions: Tensor | int | None) -> tuple[Tensor, Tensor]:
+        if self.frequencies is None:
+            self.frequencies = RotaryFrequencies(self.head_dim, self.theta)  # or refused
         if self.use_triton_rope:
             try:
                 return triton_apply_rotary_at(query, key, positions, self.frequencies, layout=self.layout)

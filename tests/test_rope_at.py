@@ -271,3 +271,22 @@ def test_positions_that_are_integers():
 
     for position in (None, 0, 5, -3, 2**62, True, 4.0, np.int64(7), np.int32(-1)):
         assert ops._first_position(position) == int(position or 0)
+
+
+@pytest.mark.parametrize("arguments", [(8, float("inf")), (0,), (128, 1e-320)])
+def test_modules_without_positions_take_what_the_tables_take(arguments):
+    q = torch.randn(1, 2, 3, arguments[0])
+    rope = RotaryEmbedding(*arguments)
+    assert rope(q, q)[0].shape == q.shape
+    with pytest.raises((ValueError, OverflowError)):
+        rope(q, q, 5)
+    with pytest.raises((ValueError, OverflowError)):
+        RotaryEmbedding(*arguments, scaling=dict(type="linear", factor=2.0))
+
+
+def test_a_module_stored_before_it_had_frequencies():
+    rope, q = RotaryEmbedding(8), torch.randn(1, 2, 3, 8)
+    want = rope(q, q)[0], rope(q, q, 5)[0]
+    for name in ("frequencies", "_plain"):
+        rope.__dict__.pop(name, None)
+    assert torch.equal(rope(q, q)[0], want[0]) and torch.equal(rope(q, q, 5)[0], want[1])
