@@ -173,6 +173,7 @@ def sequence_log_probs_with_pytorch(
     if shift:
         logits, labels = logits[:, :-1], labels[:, 1:]
     keep = labels != ignore_index
+    logits = logits.masked_fill(~keep.unsqueeze(-1), 0.0)  # what is left out may be no numbers, and asks for no gradient
     logits = logits.to(torch.promote_types(logits.dtype, torch.float32))
     token = F.log_softmax(logits, dim=-1).gather(-1, labels.masked_fill(~keep, 0).unsqueeze(-1)).squeeze(-1)
     total = torch.where(keep, token, 0.0).sum(-1)

@@ -165,3 +165,17 @@ def test_nothing_to_do():
         assert getattr(_lib.lib(), fn)(*arguments.values()) == _lib.PT_OK
     assert _lib.lib().pt_sequence_log_probs_workspace_bytes(-1, 3, 8, 0) == 0
     assert _lib.lib().pt_sequence_log_probs_workspace_bytes(2, 1 << 40, 8, 0) == 0
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_left_out_rows_may_hold_anything(value):
+    logits, labels, reference = inputs()
+    want = preference_loss_with_pytorch(logits.requires_grad_(), labels, reference)
+    (grad,) = torch.autograd.grad(want.loss, logits)
+    other = logits.detach().clone()
+    keep = torch.zeros(4, 6, dtype=torch.bool)
+    keep[:, :-1] = labels[:, 1:] != -100
+    other[~keep] = value
+    out = preference_loss_with_pytorch(other.requires_grad_(), labels, reference)
+    assert torch.equal(out.loss, want.loss) and torch.equal(torch.autograd.grad(out.loss, other)[0], grad)
+    assert not grad[~keep].any()
