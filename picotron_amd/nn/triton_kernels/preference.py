@@ -168,15 +168,17 @@ def triton_preference_loss(
 def sequence_log_probs_with_pytorch(
     logits: Tensor, labels: Tensor, *, shift: bool = True, ignore_index: int = IGNORE_INDEX, average: bool = False
 ) -> Tensor:
-    """:func:`triton_sequence_log_probs` in PyTorch."""
+    """:func:`triton_sequence_log_probs` in PyTorch, NaN for a label outside the vocabulary among the rest (a gather there
+    is an error, on a GPU one that ends the process)."""
 
     if shift:
         logits, labels = logits[:, :-1], labels[:, 1:]
     keep = labels != ignore_index
     logits = logits.masked_fill(~keep.unsqueeze(-1), 0.0)  # what is left out may be no numbers, and asks for no gradient
     logits = logits.to(torch.promote_types(logits.dtype, torch.float32))
-    token = F.log_softmax(logits, dim=-1).gather(-1, labels.masked_fill(~keep, 0).unsqueeze(-1)).squeeze(-1)
-    total = torch.where(keep, token, 0.0).sum(-1)
+    inside = (labels >= 0) & (labels < logits.size(-1))
+    token = F.log_softmax(logits, dim=-1).gather(-1, labels.masked_fill(~(keep & inside), 0).unsqueeze(-1)).squeeze(-1)
+    total = torch.where(keep, token.masked_fill(~inside, math.nan), 0.0).sum(-1)
     return total / keep.sum(-1).clamp_min(1) if average else total
 
 

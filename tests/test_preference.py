@@ -179,3 +179,20 @@ def test_left_out_rows_may_hold_anything(value):
     out = preference_loss_with_pytorch(other.requires_grad_(), labels, reference)
     assert torch.equal(out.loss, want.loss) and torch.equal(torch.autograd.grad(out.loss, other)[0], grad)
     assert not grad[~keep].any()
+
+
+@pytest.mark.parametrize("label", [-1, 11, 2**40, -(2**40)])
+def test_labels_outside_the_vocabulary_give_nan(label):
+    logits, labels, reference = inputs()
+    want = sequence_log_probs_with_pytorch(logits, labels)
+    labels[0, 3] = label
+    got = sequence_log_probs_with_pytorch(logits.requires_grad_(), labels)
+    assert got[0].isnan() and torch.equal(got[1:], want[1:])
+    (grad,) = torch.autograd.grad(got.sum(), logits)
+    assert grad[1:].isfinite().all()
+    assert preference_loss_with_pytorch(logits, labels, reference).loss.isnan()
+    # the label that leaves positions out may be one of the vocabulary, or far from it
+    for ignored in (3, 2**40):
+        other = labels.clamp(0, 10)
+        assert torch.equal(sequence_log_probs_with_pytorch(logits, other.masked_fill(other == 3, ignored), ignore_index=ignored),
+                           sequence_log_probs_with_pytorch(logits, other.masked_fill(other == 3, -100)))
