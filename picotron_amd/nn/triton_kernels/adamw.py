@@ -460,7 +460,9 @@ def _check_group_8bit(group: dict) -> None:
         raise _reject("tensor-valued betas")
 
 
-def _run_8bit(optimizer: AdamW8bit, groups, device: torch.device, grad_scale: Tensor | None = None) -> None:
+def _prepare_8bit(optimizer: AdamW8bit, groups, device: torch.device) -> list:
+    """:func:`_prepare` for 8-bit moments: the launches, with what state is missing and no count advanced."""
+
     launches = []
     counted: set[int] = set()  # a count that parameters share (as those of a capturable group do) advances once
     for group, params, states, step, seed in optimizer.buckets(groups):
@@ -471,7 +473,11 @@ def _run_8bit(optimizer: AdamW8bit, groups, device: torch.device, grad_scale: Te
                 counted.add(id(state["step"]))
                 steps.append(state["step"])
         launches.append((_device_table(host_table, device), blocks, params[0].dtype, steps, group, step, seed))
-    _committed(_launch_8bit, launches, grad_scale)
+    return launches
+
+
+def _run_8bit(optimizer: AdamW8bit, groups, device: torch.device) -> None:
+    _committed(_launch_8bit, _prepare_8bit(optimizer, groups, device), None)
 
 
 def _launch_8bit(launches: list, grad_scale: Tensor | None) -> None:
@@ -549,14 +555,13 @@ def _clip_and_step_8bit(optimizer: AdamW8bit, max_norm: float, write_back_grads:
     if device is None:
         return torch.tensor(0.0)
     table, blocks = _grad_table(grads, device)
+    # all that can fail comes before the gradients are written, so that a fallback never clips them a second time
+    launches = scan[1] if scan is not None else _prepare_8bit(optimizer, groups, device)
     total_norm, coef = ops.clip_grad_norm(table, blocks, float(max_norm))
     if write_back_grads:
         _committed(ops.grad_scale, table, blocks, coef)
         coef = None
-    if scan is None:
-        _run_8bit(optimizer, groups, device, coef)
-    else:
-        _committed(_launch_8bit, scan[1], coef)
+    _committed(_launch_8bit, launches, coef)
     return total_norm
 
 

@@ -414,3 +414,26 @@ def test_a_shared_count_advances_once(monkeypatch, native):
     adamw._run_8bit(optimizer, optimizer._with_gradients(), torch.device("cpu"))
     plain.step()
     assert steps == [4.0, 4.0] and float(optimizer.state[params[0]]["step"]) == float(plain.state[other[0]]["step"]) == 4.0
+
+
+def test_clipping_writes_no_gradient_before_the_step_is_prepared(monkeypatch):
+    """A step that cannot be prepared (its table is first needed during a capture, say) is left to the fallback, whose clipping
+    reads the gradients as they were."""
+
+    params, optimizer = _trained()
+    done = []
+
+    def prepare(table, device):
+        done.append("table")
+        raise TritonAdamWUnavailable("first built during graph capture")
+
+    monkeypatch.setattr(adamw, "_scan_8bit", lambda optimizer: None)
+    monkeypatch.setattr(adamw, "_plan_8bit", lambda optimizer: (optimizer._with_gradients(), torch.device("cpu")))
+    monkeypatch.setattr(adamw, "_grads_of", lambda params: ([p.grad for p in params], torch.device("cpu")))
+    monkeypatch.setattr(adamw, "_grad_table", lambda grads, device: (None, 1))
+    monkeypatch.setattr(adamw, "_device_table", prepare)
+    monkeypatch.setattr(ops, "clip_grad_norm", lambda *args: (torch.tensor(1.0), torch.tensor(0.5)))
+    monkeypatch.setattr(ops, "grad_scale", lambda *args: done.append("written"))
+    with pytest.raises(TritonAdamWUnavailable):
+        triton_clip_grad_norm_and_step(optimizer, 1.0)
+    assert done == ["table"] and float(optimizer.state[params[0]]["step"]) == 3.0
