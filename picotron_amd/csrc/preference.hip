@@ -653,7 +653,8 @@ int check_call(const char* fn, const void* logits, int64_t batch, int64_t seq, i
   if (!valid_dtype(dtype)) return fail(PT_EINVAL, name + ": unknown dtype code");
   if (batch < 0 || seq < 0 || vocab < 1) return fail(PT_EINVAL, name + ": negative size, or no vocabulary");
   if (shift != 0 && shift != 1) return fail(PT_EINVAL, name + ": shift must be 0 or 1");
-  if (vocab * dtype_size(dtype) > 0x7fffffffLL - (1 << 20)) return fail(PT_EUNSUPPORTED, name + ": rows of 2 GB and more");
+  if (vocab > 0x7fffffffLL || vocab * dtype_size(dtype) > 0x7fffffffLL - (1 << 20))
+    return fail(PT_EUNSUPPORTED, name + ": rows of 2 GB and more");
   // a launch has fewer than 2^32 threads: 256 a row and part, 1024 a sequence
   if (batch > kMaxBatch || seq > kMaxRows || batch * seq > kMaxRows)
     return fail(PT_EUNSUPPORTED, name + ": more than 2^23 rows or 2^21 sequences");
@@ -789,7 +790,7 @@ using namespace pt;
 extern "C" {
 
 size_t pt_sequence_log_probs_workspace_bytes(int64_t batch, int64_t seq, int64_t vocab, int dtype) {
-  if (batch < 0 || seq < 0 || batch > kMaxBatch || seq > kMaxRows || batch * seq > kMaxRows) return 0;
+  if (batch < 0 || seq < 0 || batch > kMaxBatch || seq > kMaxRows || batch * seq > kMaxRows || vocab > 0x7fffffffLL) return 0;
   return Layout(batch, seq, parts_for(batch * seq, vocab, dtype)).total;
 }
 

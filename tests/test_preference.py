@@ -196,3 +196,14 @@ def test_labels_outside_the_vocabulary_give_nan(label):
         other = labels.clamp(0, 10)
         assert torch.equal(sequence_log_probs_with_pytorch(logits, other.masked_fill(other == 3, ignored), ignore_index=ignored),
                            sequence_log_probs_with_pytorch(logits, other.masked_fill(other == 3, -100)))
+
+
+@pytest.mark.parametrize("vocab", [1 << 31, 1 << 33, 1 << 61, 1 << 62, (1 << 63) - 1])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_vocabularies_beyond_any_row_are_refused(vocab, dtype):
+    """Also where their bytes pass 64 bits."""
+
+    for make in (_logp, _loss, _bwd):
+        fn, arguments = make(vocab=vocab, dtype=dtype)
+        assert getattr(_lib.lib(), fn)(*arguments.values()) == _lib.PT_EUNSUPPORTED
+    assert _lib.lib().pt_sequence_log_probs_workspace_bytes(2, 3, vocab, dtype) == 0
