@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from gpu_util import randn
-from picotron_amd import ops
+from picotron_amd import _lib, ops
 from picotron_amd.nn import RotaryEmbedding
 from picotron_amd.nn.triton_kernels import (
     PreferenceLossWithFallback,
@@ -485,3 +485,80 @@ def test_parts_of_rows(gpu, vocab, dtype, rows):
     check_log_probs(out.detach(), logits.detach(), labels)
     (grad,) = torch.autograd.grad(out, logits, torch.full((1,), -1.5, device=gpu))
     check_grad(grad, logits.detach(), labels, torch.full((1,), -1.5, dtype=torch.float64, device=gpu))
+
+
+# What follows the rows, by route: one launch for few tokens (one wave a sequence, several waves a sequence); sums and loss in
+# launches of their own (many sequences, more than 256 pairs; few long sequences of more than 16384 tokens); rows in parts joined in
+# the one launch (up to 64 rows) and in one of their own (up to 128).
+ROUTES = [
+    *[(6, 13, 1003, torch.float32), (4, 600, 130, torch.float32), (2, 1025, 65, torch.float16), (4, 3000, 130, torch.bfloat16)],
+    *[(16384, 1, 40, torch.float32), (5462, 3, 40, torch.float32), (1022, 16, 77, torch.bfloat16), (514, 40, 260, torch.float16)],
+    *[(2, 9000, 65, torch.float32), (4, 8200, 33, torch.bfloat16)],
+    *[(2, 32, 33_000, torch.bfloat16), (4, 16, 70_001, torch.float32), (2, 31, 128256, torch.float16)],
+    *[(2, 33, 128256, torch.bfloat16), (4, 32, 200_001, torch.float32), (2, 64, 128257, torch.float16), (6, 30, 128256, torch.bfloat16)],
+]
+
+
+@pytest.mark.parametrize("batch,seq,vocab,dtype", ROUTES)
+@pytest.mark.parametrize("loss,average", [("sigmoid", False), ("sigmoid", True), ("ipo", True), ("hinge", False)])
+def test_losses_on_every_route(gpu, batch, seq, vocab, dtype, loss, average):
+    """Each step against the one before it: log-probabilities against 64 bits, rewards against them, and loss, slopes and gradient
+    against the rewards."""
+
+    beta, pairs, shift = 0.25, batch // 2, seq > 1
+    logits, labels, reference = inputs(batch, seq, vocab, dtype, gpu, batch + seq)
+    token, keep, _, _ = token_log_probs(logits, labels, shift)
+    n = keep.sum(1).clamp_min(1).double() if average else torch.ones(batch, dtype=torch.float64, device=gpu)
+    reference = (token.sum(1) / n + reference.double()).float()  # margins of a few, however long the sequences
+    logits.requires_grad_()
+    out = triton_preference_loss(logits, labels, reference, beta=beta, loss=loss, average=average, shift=shift)
+    check_log_probs(out.log_probs, logits, labels, shift, average)
+    rewards = torch.cat((out.chosen_rewards, out.rejected_rewards)).double()
+    # the log-probability's one rounding, the reward's own
+    off = beta * 2.0**-24 * out.log_probs.double().abs() + 2.0**-24 * rewards.abs()
+    assert ((rewards - beta * (out.log_probs.double() - reference.double())).abs() <= off * (1 + 2.0**-20) + 1e-30).all()
+    c, r = rewards.chunk(2)
+    h = c - r
+    dh = 2.0**-23 * (c.abs() + r.abs())  # one rounding of each reward, and h's
+    u = h / beta - 0.5 / beta
+    each = {"sigmoid": -torch.nn.functional.logsigmoid(h), "hinge": torch.relu(1 - h), "ipo": u.square()}[loss]
+    # a few roundings of an fp32 function (2^-21), the margin's error by a slope of 1, or of 2 u / beta
+    du = dh / beta + 2.0**-22 * (h.abs() + 0.5) / beta
+    error = dh + 2.0**-21 * each if loss != "ipo" else 2 * u.abs() * du + du.square() + 2.0**-21 * each
+    assert abs(float(out.loss.detach()) - float(each.mean())) <= float(error.mean()) + 2.0**-23 * float(each.mean()) + 1e-30
+    (grad,) = torch.autograd.grad(out.loss, logits)
+    # sigmoid: ln of the slope moves by the margin's error; ipo's by that of u; hinge's not at all (no margin lies that near 1)
+    rel = {"sigmoid": dh, "hinge": torch.zeros_like(h), "ipo": du / u.abs()}[loss] + 2.0**-20
+    assert loss != "hinge" or ((h - 1).abs() > dh).all()
+    slope = slope_of(rewards, beta, loss, 0.0) / n
+    rel = rel.repeat(2)
+    for at in range(0, batch, max(1, 8_000_000 // (seq * vocab))):
+        part = slice(at, at + max(1, 8_000_000 // (seq * vocab)))
+        check_grad(grad[part], logits.detach()[part], labels[part], slope[part], shift, slope_rel=rel[part][:, None, None])
+
+
+@pytest.mark.parametrize("dtype,batch,seq,vocab", [(torch.bfloat16, 7, 1201, 65_537), (torch.float32, 3, 700, 128_256),
+                                                   (torch.float16, 2, 11_003, 25_000)])
+def test_every_row_of_a_large_gradient(gpu, dtype, batch, seq, vocab):
+    """1 GB and more, whose rows are dealt to the XCDs in ranges: every element is written, the items behind the last
+    whole range among them, into a buffer of NaN."""
+
+    logits, labels, _ = inputs(batch, seq, vocab, dtype, gpu, 43)
+    assert logits.nbytes >= 1 << 30
+    up = torch.linspace(0.5, 2.0, batch, device=gpu)
+    _, ws = ops.sequence_log_probs(logits, labels)
+    grad = torch.full_like(logits, float("nan"))
+    _lib.raw_call("pt_sequence_log_probs_bwd", logits.data_ptr(), batch, *ops._sequence_rows(logits, labels, True), -100,
+                  up.data_ptr(), None, grad.data_ptr(), grad.stride(0), grad.stride(1), ws.data_ptr(), ws.numel(),
+                  ops.dtype_code(dtype), ops._stream(logits.device))
+    assert torch.equal(grad, ops.sequence_log_probs_bwd(logits, labels, ws, grad_log_probs=up))
+    for b in range(batch):
+        # 64 bits of a few hundred rows at a time; a slice's last label is the next one's first
+        for at in range(0, seq - 1, 500):
+            rows = slice(at, min(at + 501, seq))
+            g = grad[b:b + 1, rows].clone()
+            x, y = logits[b:b + 1, rows], labels[b:b + 1, rows]
+            if rows.stop < seq:
+                g[:, -1] = 0.0  # has its label in the next slice
+            check_grad(g, x, y, up[b:b + 1].double())
+    assert not grad[:, -1].any()
