@@ -124,16 +124,16 @@ struct RowReader {
   int n;  // vectors
   float head, tail;
 
-  __device__ __forceinline__ RowReader(const T* p, int vocab, int part, int parts, int tid, bool skip) {
+  __device__ __forceinline__ RowReader(const T* p, int vocab, int part, int parts, int tid) {
     const Split<T> sp(p, vocab);
     const int per = (sp.vecs + parts - 1) / parts;
     const int from = part * per < sp.vecs ? part * per : sp.vecs;
-    n = skip ? 0 : (sp.vecs - from < per ? sp.vecs - from : per);
+    n = sp.vecs - from < per ? sp.vecs - from : per;
     buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p) + sp.head + static_cast<int64_t>(from) * Elem<T>::VEC, 0,
                                             n * 16, kBufferWord3);
     const int at = sp.tail + (LANES - 1 - tid);
-    head = !skip && part == 0 && tid < sp.head ? Elem<T>::to_f32(p[tid]) : -INFINITY;
-    tail = !skip && part == parts - 1 && at < vocab ? Elem<T>::to_f32(p[at]) : -INFINITY;
+    head = part == 0 && tid < sp.head ? Elem<T>::to_f32(p[tid]) : -INFINITY;
+    tail = part == parts - 1 && at < vocab ? Elem<T>::to_f32(p[at]) : -INFINITY;
   }
 
   template <int N>
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void seq_stats_short_kernel(Rows d, float
     return;
   }
   const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
-  const RowReader<T, 64> in(p, d.vocab, 0, 1, lane, false);
+  const RowReader<T, 64> in(p, d.vocab, 0, 1, lane);
   const float xt = label_logit(d, p, label);  // in flight with the row
   Running run;
   for (int from = 0; from < in.n; from += 64 * N) {
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void seq_stats_kernel(Rows d, uint32_t pa
     return;
   }
   const T* p = static_cast<const T*>(d.x) + (b * d.bs + t * d.ss);
-  const RowReader<T, kThreads> in(p, d.vocab, static_cast<int>(part), static_cast<int>(parts), tid, false);
+  const RowReader<T, kThreads> in(p, d.vocab, static_cast<int>(part), static_cast<int>(parts), tid);
   float xt = 0.0f;
   if (tid == 0 && parts == 1) xt = label_logit(d, p, label);  // in flight with the row
   Running run;

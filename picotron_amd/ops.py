@@ -1010,7 +1010,6 @@ _ADAMW8_STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
 
 
 @functools.lru_cache(maxsize=None)
-@functools.lru_cache(maxsize=None)
 def adamw8_sizes() -> tuple[int, int]:
     """(elements of a table block, elements that share a scale) of the AdamW step with 8-bit moments."""
 
