@@ -17,10 +17,10 @@
 
 #include <ATen/ATen.h>
 
+#include <algorithm>
 #include <cstring>
 #include <initializer_list>
 #include <optional>
-#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -783,8 +783,8 @@ PT_END
 // adamw8_scan([params, ...] per group, optimizer.state, elements per table block, elements per scale) ->
 // (device index, [(table, rows, blocks, step, steps, dtype code) or None, ...])
 // for parameters with 8-bit moments that all have their state in place, one dtype and one host step count a group: the
-// record table of each group's step as bytes (None for a group without gradients), and the counts that it advances -- each once,
-// also where parameters share one.  None for anything else.
+// record table of each group's step as bytes (None for a group without gradients).  None for anything else, a count that
+// parameters share among it.
 PT_FN(adamw8_scan, 4)
   int64_t per, quant;
   if (!PyList_Check(a[0]) || !PyDict_Check(a[1]) || !as_i64(a[2], &per) || !as_i64(a[3], &quant) || per <= 0 || quant <= 0)
@@ -792,7 +792,7 @@ PT_FN(adamw8_scan, 4)
   THPObjectPtr list{PyList_New(0)};
   if (!list) return nullptr;
   c10::Device device(c10::kCPU);
-  std::unordered_set<PyObject*> counted;  // step tensors, held by the lists below
+  std::vector<PyObject*> counts;  // step tensors, held by the lists below
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i) {
     PyObject* params = PyList_GET_ITEM(a[0], i);
     if (!PyList_Check(params)) return none();
@@ -826,7 +826,8 @@ PT_FN(adamw8_scan, 4)
       if (p->device() != device || (!rows.empty() && (*count != step || code_of(*p) != code))) return none();
       step = *count;
       code = code_of(*p);
-      if (counted.insert(so).second && PyList_Append(steps, so) != 0) return nullptr;
+      if (PyList_Append(steps, so) != 0) return nullptr;
+      counts.push_back(so);
       if (!moment_row(*p, reinterpret_cast<int64_t>(out(grad)), state, per, quant, &rows, &blocks)) return none();
     }
     if (rows.empty()) {
@@ -841,6 +842,8 @@ PT_FN(adamw8_scan, 4)
     if (!entry || PyList_Append(list, entry.get()) != 0) return nullptr;
   }
   if (device.is_cpu()) return none();
+  std::sort(counts.begin(), counts.end());
+  if (std::adjacent_find(counts.begin(), counts.end()) != counts.end()) return none();  // it would be advanced twice
   return Py_BuildValue("(iO)", static_cast<int>(device.index()), list.get());
 PT_END
 
