@@ -130,6 +130,17 @@ def _turn_bits(frequency: float) -> int:
     return round(Fraction((numerator * _PI_SCALE) << 63, denominator * _PI_DIGITS)) % 2**64
 
 
+def _bits_of(frequencies: list[float]) -> Tensor:
+    bits = [_turn_bits(f) for f in frequencies]
+    return torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64, device="cpu")
+
+
+def _elsewhere(t: Tensor, device: torch.device) -> bool:
+    """True for what was kept for ``device`` and is on another: a module that was loaded with a map_location."""
+
+    return t.device != device and (t.device.type != device.type or device.index is not None)
+
+
 class RotaryFrequencies:
     """Radians per position of each rotated pair (``frequencies``, fp64 on the CPU) and the factor on cosine and sine
     (``attention_factor``): ``theta^(-2i/rotary_dim)``, scaled to contexts longer than those of training by ``scaling``:
@@ -156,8 +167,7 @@ class RotaryFrequencies:
         # Python numbers, whatever device or mode torch makes tensors in here; the bits before any tracing of turns()
         values = self._scaled(_checked_scaling(scaling), theta) if scaling is not None else self._base(theta)
         self.frequencies = torch.tensor(values, dtype=torch.float64, device="cpu")
-        bits = [_turn_bits(f) for f in values]
-        self._bits = torch.tensor([b - 2**64 if b >= 2**63 else b for b in bits], dtype=torch.int64, device="cpu")
+        self._bits = _bits_of(values)
         self._turns: dict[torch.device, Tensor] = {}
 
     def _base(self, theta: float) -> list[float]:
@@ -197,7 +207,7 @@ class RotaryFrequencies:
         """int64 on ``device``: the bits of each frequency as a fraction of a turn per position, times 2^64."""
 
         found = self._turns.get(device)
-        if found is None:
+        if found is None or _elsewhere(found, device):
             if device.type == "cuda" and not torch.compiler.is_compiling() and torch.cuda.is_current_stream_capturing():
                 raise TritonRoPEUnavailable(
                     "HIP RoPE: the frequencies are first used on this device during graph capture; run the same call "
@@ -287,7 +297,7 @@ class RotaryEmbedding(nn.Module):
 
     def _tables_fp32(self, sequence_length: int, device: torch.device) -> tuple[Tensor, Tensor]:
         tables = self._fp32_tables.get(device)
-        if tables is None or tables[0].size(0) < sequence_length:
+        if tables is None or tables[0].size(0) < sequence_length or _elsewhere(tables[0], device):
             tables = rotary_cos_sin(
                 sequence_length, self.head_dim, self.theta, device=device, dtype=torch.float32
             )

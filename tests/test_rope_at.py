@@ -290,3 +290,18 @@ def test_a_module_stored_before_it_had_frequencies():
     for name in ("frequencies", "_plain"):
         rope.__dict__.pop(name, None)
     assert torch.equal(rope(q, q)[0], want[0]) and torch.equal(rope(q, q, 5)[0], want[1])
+
+
+@pytest.mark.parametrize("rotary_dim", [None, 4])
+def test_a_module_loaded_onto_another_device(rotary_dim):
+    """What it kept for its device lies elsewhere after a load with a map_location (the meta device stands in for it)."""
+
+    rope, q = RotaryEmbedding(8, rotary_dim=rotary_dim), torch.randn(1, 2, 3, 8)
+    want = rope(q, q)[0], rope(q, q, 5)[0]
+    cpu = q.device
+    rope._fp32_tables[cpu] = tuple(t.to("meta") for t in rope._tables_fp32(9, cpu))
+    rope.frequencies._turns[cpu] = rope.frequencies.turns(cpu).to("meta")
+    assert torch.equal(rope(q, q, 5)[0], want[1]) and torch.equal(rope(q, q)[0], want[0])
+    assert {t.device for t in (rope.frequencies.turns(cpu), *rope._tables_fp32(3, cpu))} == {cpu}
+    kept = rope.frequencies.turns(cpu)
+    assert rope.frequencies.turns(cpu) is kept
