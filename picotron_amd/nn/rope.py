@@ -170,6 +170,11 @@ class RotaryFrequencies:
         self._bits = _bits_of(values)
         self._turns: dict[torch.device, Tensor] = {}
 
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        if "_bits" not in state:  # stored when they were formed on first use
+            self._bits = _bits_of(self.frequencies.tolist())
+
     def _base(self, theta: float) -> list[float]:
         return [theta ** (-2.0 * i / self.rotary_dim) for i in range(self.rotary_dim // 2)]
 

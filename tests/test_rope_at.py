@@ -305,3 +305,14 @@ def test_a_module_loaded_onto_another_device(rotary_dim):
     assert {t.device for t in (rope.frequencies.turns(cpu), *rope._tables_fp32(3, cpu))} == {cpu}
     kept = rope.frequencies.turns(cpu)
     assert rope.frequencies.turns(cpu) is kept
+
+
+def test_frequencies_stored_before_they_had_their_bits():
+    import copy
+
+    f = RotaryFrequencies(8, scaling=YARN)
+    old = copy.copy(f)
+    state = {key: value for key, value in f.__dict__.items() if key != "_bits"}
+    old.__dict__.clear()
+    old.__setstate__({**state, "_turns": {}})
+    assert torch.equal(old.turns(torch.device("cpu")), f.turns(torch.device("cpu")))
