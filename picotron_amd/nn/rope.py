@@ -114,7 +114,7 @@ def _checked_scaling(scaling: Mapping) -> dict:
     for key, value in values.items():
         if key != "type" and value is not None and not (math.isfinite(value) and value > 0):
             raise ValueError(f"rotary scaling {key} must be a positive number; got {value!r}.")
-    return values
+    return {key: value if key == "type" or value is None else float(value) for key, value in values.items()}
 
 
 # pi to 50 digits: a frequency is a binary fraction, and its turns per position are rounded once
@@ -162,6 +162,7 @@ class RotaryFrequencies:
             raise ValueError("RoPE requires an even, positive rotary dimension.")
         if not (math.isfinite(theta) and theta > 0):
             raise ValueError("rope_theta must be positive.")
+        theta = float(theta)
         self.rotary_dim = rotary_dim
         self.attention_factor = 1.0
         # Python numbers, whatever device or mode torch makes tensors in here; the bits before any tracing of turns()
@@ -196,7 +197,7 @@ class RotaryFrequencies:
             low = max(math.floor(pair_with(s["beta_fast"])), 0)
             high = min(math.ceil(pair_with(s["beta_slow"])), dim - 1)
             given = s["attention_factor"]
-            self.attention_factor = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+            self.attention_factor = given if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
             ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(len(base))]
             return [f * (1 - t) + f / factor * t for f, t in zip(base, ramp)]
         if s["type"] == "llama3":

@@ -316,3 +316,15 @@ def test_frequencies_stored_before_they_had_their_bits():
     old.__dict__.clear()
     old.__setstate__({**state, "_turns": {}})
     assert torch.equal(old.turns(torch.device("cpu")), f.turns(torch.device("cpu")))
+
+
+def test_numbers_of_any_kind():
+    import numpy as np
+
+    want = RotaryFrequencies(16, 5e5, scaling=dict(type="yarn", factor=4.0, original_max_positions=128, beta_fast=32.0))
+    for number in (np.float64, lambda x: np.float32(x), lambda x: torch.tensor(x, dtype=torch.float64), int):
+        f = RotaryFrequencies(16, number(5e5), scaling=dict(type="yarn", factor=number(4), original_max_positions=number(128),
+                                                            beta_fast=number(32)))
+        assert torch.equal(f.turns(torch.device("cpu")), want.turns(torch.device("cpu"))) and f.attention_factor == want.attention_factor
+        q = torch.randn(1, 2, 3, 16)
+        assert torch.equal(RotaryEmbedding(16, number(5e5))(q, q, 3)[0], RotaryEmbedding(16, 5e5)(q, q, 3)[0])
