@@ -432,6 +432,38 @@ int pt_adamw8_step(const int64_t* table, int64_t n_tensors, int64_t total_blocks
 int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blocks, void* exp_avg,
                       void* exp_avg_sq, int dtype, void* stream);
 
+/* ---------------------------------------------------------------- Cross-entropy of a head, without its logits
+ * l[n, :] = x[n, :] weight^T over `vocab` rows of weight (weight_stride elements apart) of `hidden` elements, x
+ * [outer, inner, hidden] at the given strides; loss[n] = logsumexp(l[n, :]) - l[n, label[n]] for the rows whose label
+ * is not ignore_index: their mean (NaN of none) or sum as one fp32 value, or with PT_REDUCTION_NONE each row's, fp32
+ * [outer, inner], 0 at ignored rows.  A label outside the vocabulary gives NaN, in the loss and in every gradient it
+ * enters.  The logits are never held whole: exponentials of at most 2 GiB (chunk_rows rows, where that is fewer;
+ * 0: as many as fit) are.  x and weight share `dtype`; fp32 operands are multiplied in three bf16 planes (24 bits).
+ * Gradients, where dx or dw is non-NULL: dx [outer, dx_inner, hidden] contiguous (rows inner.. and ignored rows zero),
+ * dw [vocab, hidden] contiguous, of grad_dtype (dtype or fp32), for an incoming gradient of 1 of the mean or sum; of the
+ * loss without a reduction for dloss (fp32, the given strides).  16 bytes (of fp32; 8 of two-byte types) aligned.
+ * loss may be NULL where gradients are asked for.  workspace: 256-byte aligned, _workspace_bytes for the same arguments.
+ *   pt_scale_gradient: to = from * scale (fp32 device scalar), rounded once: in place, or from fp32 to another
+ *     type.  Nothing is touched in place for a scale of 1.
+ * Replaces the head's product and F.cross_entropy behind it (src/picotron/training/train_loop.py:136-145). */
+#define PT_REDUCTION_MEAN 0
+#define PT_REDUCTION_SUM 1
+#define PT_REDUCTION_NONE 2
+size_t pt_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden,
+                                               const void* weight, int64_t weight_stride, int dtype,
+                                               int want_dx, int want_dw, int64_t chunk_rows);
+int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inner_stride,
+                            int64_t outer, int64_t inner, const void* weight,
+                            int64_t weight_stride, int64_t vocab, int64_t hidden,
+                            const int64_t* labels, int64_t label_outer_stride,
+                            int64_t label_inner_stride, int64_t ignore_index, int reduction,
+                            float* loss, const float* dloss, int64_t dloss_outer_stride,
+                            int64_t dloss_inner_stride, void* dx, int64_t dx_inner, void* dw,
+                            int grad_dtype, void* workspace, size_t workspace_bytes,
+                            int64_t chunk_rows, int dtype, void* stream);
+int pt_scale_gradient(const void* from, int from_dtype, void* to, int to_dtype, int64_t elements,
+                      const float* scale, void* stream);
+
 /* ---------------------------------------------------------------- Utility
  * Device-to-device copy of `bytes` (multiple of 16, 16-byte aligned pointers) with the
  * same 128-bit load/store pattern as the streaming kernels.  No reference counterpart:

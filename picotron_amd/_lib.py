@@ -163,6 +163,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_void_p, c_void_p, c_uint32, c_int, c_int, c_void_p],
     ),
     "pt_adamw8_moments": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "pt_linear_cross_entropy_workspace_bytes": (
+        c_size_t, [c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int64]
+    ),
+    "pt_linear_cross_entropy": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
+         c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_size_t,
+         c_int64, c_int, c_void_p],
+    ),
+    "pt_scale_gradient": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p]),
     "pt_copy": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

@@ -1,0 +1,830 @@
+// Cross-entropy of a language model's head without its logits: hidden states x (N, H) and the head's weight w (V, H) in,
+// the loss and the gradients of both out.
+//
+//   l = x w^T,  z_n = ln sum_v exp l_nv,  loss_n = z_n - l_{n, t_n}
+//   G = c_n (softmax(l) - onehot(t)),  dx = G w,  dw = G^T x        (c_n the weight that arrives at token n)
+//
+// Three matrix products bound it: 2 N H V operations each, 8.6e12 at 8192 tokens, 4096 wide, 128256 words.
+//
+// - Tokens whose label is ignored take no part: the kept rows of x are gathered first, and their number stays on the device.
+// - The first product's workgroups, a tile of 256 tokens by 256 words each, leave exp(l - m) with m the largest logit
+//   of the token in the tile, and m and the sum of the tile: one pass, no logits.  From z a second pass makes G of it
+//   in place: an exp for each token and tile, a product for each element, and at the label expm1(l_t - z), which
+//   keeps its accuracy where the softmax is close to 1.
+// - With 16-bit inputs exp(l - m) is held as fp16 scaled by 2^14: 11 bits where the largest bf16 error below is 8,
+//   down to 2^-28 of the tile's largest.  G is rounded to the inputs' type, as the matrix cores take it, scaled by 2^14
+//   too (fp16 keeps softmax values down to 2^-28 normal), and the scale is taken out of the fp32 sums.
+// - With 32-bit inputs every operand is the sum of three bf16 planes of 8 bits (see Planes): 6 products of 16-bit operands
+//   run 2.6 times as fast as one of the fp32 matrix instructions would at its peak.
+// - Tokens are taken in chunks, so that G takes at most 2 GiB; with more than one, dw is summed in fp32 over them.
+// - The gradients are formed in the forward call, where G is at hand; the backward only multiplies them by what arrives
+//   from above.  fp16's stay in fp32 until then, as a loss scale arrives only there.
+//   Where each token has its own weight (no reduction), the backward forms G itself, with one product more.
+#include "tile_product.hpp"
+
+namespace pt {
+namespace {
+
+constexpr float kScale = 16384.0f;  // of exp(l - m) and G in 16 bits
+constexpr int kTile = 256;
+constexpr int64_t kChunkBytes = int64_t{1} << 31;
+constexpr int64_t kScoreRows = 65536;  // rows of a chunk that only leaves sums
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+struct Meta {
+  int count;        // kept rows
+  float alpha;      // of the gradients' sums
+  float inv_weight; // of the rows' own weights
+  int pad;
+};
+
+struct Rows {  // labels, and the rows of x, by (outer, inner)
+  const void* x;
+  int64_t xso, xsi;
+  const int64_t* t;
+  int64_t tso, tsi;
+  int64_t outer, inner, ignore;
+  const float* c;  // weights, or null
+  int64_t cso, csi;
+  int64_t dx_inner;  // rows of dx an outer index has
+};
+
+// ------------------------------------------------------------------ rows
+
+// Which rows are kept, in order: their row of dx, label (-1 for one outside the vocabulary) and weight; how many; the
+// gradients' factor.  One workgroup: a scan of 1024 labels a round (8192 take 10 us).
+__global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int reduction, int* __restrict__ row_of,
+                                                    int* __restrict__ label_of, float* __restrict__ weight_of,
+                                                    Meta* __restrict__ meta, float* __restrict__ losses) {
+  __shared__ int counts[16];
+  __shared__ float tops[16];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int64_t n = r.outer * r.inner;
+  int base = 0;
+  float top = 0.f;
+  for (int64_t first = 0; first < n; first += 1024) {
+    const int64_t i = first + threadIdx.x;
+    int64_t o = 0, s = 0, t = r.ignore;
+    if (i < n) {
+      o = i / r.inner;
+      s = i - o * r.inner;
+      t = r.t[o * r.tso + s * r.tsi];
+    }
+    const bool keep = i < n && t != r.ignore;
+    const unsigned long long mask = __ballot(keep);
+    if (lane == 0) counts[wave] = __popcll(mask);
+    __syncthreads();
+    int before = base, all = base;
+    for (int k = 0; k < 16; ++k) {
+      if (k < wave) before += counts[k];
+      all += counts[k];
+    }
+    if (keep) {
+      const int at = before + __popcll(mask & ((1ull << lane) - 1));
+      row_of[at] = static_cast<int>(o * r.dx_inner + s);
+      label_of[at] = t >= 0 && t < vocab ? static_cast<int>(t) : -1;
+      if (r.c != nullptr) {
+        const float c = r.c[o * r.cso + s * r.csi];
+        weight_of[at] = c;
+        if (fabsf(c) <= 3.4e38f) top = fmaxf(top, fabsf(c));
+      }
+    } else if (i < n && losses != nullptr) {
+      losses[i] = 0.f;
+    }
+    base = all;
+    __syncthreads();
+  }
+  top = wave_max(top);
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < 16; ++k) top = fmaxf(top, tops[k]);
+    // the rows' weights are taken relative to a power of two near the largest, which G's 16 bits then hold
+    unsigned e = __builtin_bit_cast(unsigned, top) & 0x7f800000u;
+    e = e < 0x00800000u ? 0x00800000u : e;
+    const float unit = __builtin_bit_cast(float, e);
+    Meta m{base, 0.f, 1.f, 0};
+    if (reduction == PT_REDUCTION_NONE) {
+      m.alpha = unit / kScale;
+      m.inv_weight = 1.f / unit;
+    } else if (base > 0) {
+      m.alpha = (reduction == PT_REDUCTION_MEAN ? 1.f / static_cast<float>(base) : 1.f) / kScale;
+    }
+    *meta = m;
+  }
+}
+
+// A value as planes of 16 bits: itself, or three bf16 whose sum it is.
+template <typename T>
+struct Split {
+  typedef T plane;
+  static __device__ __forceinline__ void put(T* p, int64_t, T v) { *p = v; }
+};
+template <>
+struct Split<float> {
+  typedef __bf16 plane;
+  static __device__ __forceinline__ void put(__bf16* p, int64_t plane, float v) {
+    const __bf16 a = static_cast<__bf16>(v);
+    const float r = v - static_cast<float>(a);
+    const __bf16 b = static_cast<__bf16>(r);
+    p[0] = a;
+    p[plane] = b;
+    p[2 * plane] = static_cast<__bf16>(r - static_cast<float>(b));
+  }
+};
+
+// One wave a row: the kept rows of x, one behind the other, `width` (a multiple of 64) elements each with zeros
+// behind the H-th, and zero rows up to a whole tile; and zeros in the rows of dx that are not kept.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void gather_kernel(Rows r, const int* __restrict__ row_of, const Meta* __restrict__ meta,
+                                                     typename Split<T>::plane* __restrict__ to, int64_t plane, int64_t width,
+                                                     int64_t hidden, int64_t gathered, char* __restrict__ dx, int dx_size) {
+  const int lane = threadIdx.x % 64;
+  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
+  if (wave < gathered) {
+    const int count = meta->count;
+    if (wave >= (static_cast<int64_t>(count) + kTile - 1) / kTile * kTile) return;
+    const T* from = nullptr;
+    if (wave < count) {
+      const int64_t row = row_of[wave], o = row / r.dx_inner, s = row - o * r.dx_inner;
+      from = static_cast<const T*>(r.x) + o * r.xso + s * r.xsi;
+    }
+    typename Split<T>::plane* p = to + wave * width;
+    if constexpr (VEC) {  // 16-bit elements, H a multiple of 64
+      const u32x4 zero = {0, 0, 0, 0};
+      for (int64_t c = lane * 8; c < width; c += 512)
+        *reinterpret_cast<u32x4*>(p + c) = from != nullptr ? *reinterpret_cast<const u32x4*>(from + c) : zero;
+    } else {
+      for (int64_t c = lane; c < width; c += 64)
+        Split<T>::put(p + c, plane, from != nullptr && c < hidden ? from[c] : static_cast<T>(0.f));
+    }
+    return;
+  }
+  const int64_t row = wave - gathered;
+  if (dx == nullptr || row >= r.outer * r.dx_inner) return;
+  const int64_t o = row / r.dx_inner, s = row - o * r.dx_inner;
+  if (s < r.inner && r.t[o * r.tso + s * r.tsi] != r.ignore) return;
+  char* p = dx + row * hidden * dx_size;
+  if (dx_size == 4) {
+    for (int64_t c = lane; c < hidden; c += 64) reinterpret_cast<float*>(p)[c] = 0.f;
+  } else {
+    for (int64_t c = lane; c < hidden; c += 64) reinterpret_cast<unsigned short*>(p)[c] = 0;
+  }
+}
+
+// The weight with rows of `width` elements, in planes: for one whose rows the products cannot read in place.
+template <typename T>
+__global__ __launch_bounds__(256) void weight_kernel(const T* __restrict__ w, int64_t ld, typename Split<T>::plane* __restrict__ to,
+                                                     int64_t plane, int64_t width, int64_t hidden, int64_t vocab) {
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; row < vocab;
+       row += static_cast<int64_t>(gridDim.x) * 4)
+    for (int64_t c = threadIdx.x % 64; c < width; c += 64)
+      Split<T>::put(to + row * width + c, plane, c < hidden ? w[row * ld + c] : static_cast<T>(0.f));
+}
+
+// ------------------------------------------------------------------ the three products
+
+template <typename T, bool A_COLUMNS, bool B_COLUMNS>
+using Product = TileProduct<T, kTile, kTile, 2, 4, A_COLUMNS, B_COLUMNS>;
+
+__device__ __forceinline__ int rows_here(const Meta* meta, int64_t first, int64_t chunk) {
+  const int64_t n = meta->count - first;
+  return static_cast<int>(n < 0 ? 0 : (n > chunk ? chunk : n));
+}
+
+struct Scores {
+  Operand x, w;
+  Planes planes;
+  const Meta* meta;
+  const int* label_of;
+  int64_t first, chunk, vocab;
+  int tiles_n, steps;
+  void* e;           // exp(l - m), (chunk, tiles_n * 256), or null
+  f32x2* sums;       // m and the sum of exp(l - m), (tiles_n, padded)
+  int64_t padded;
+  float* target;     // the label's logit of each kept row
+};
+
+// E: how exp(l - m) is held (fp16 scaled by 2^14, or float).
+template <typename T, typename E>
+__global__ __launch_bounds__(512) void scores_kernel(Scores s) {
+  extern __shared__ char lds_raw[];
+  typedef Product<T, false, false> P;
+  const int rows = rows_here(s.meta, s.first, s.chunk);
+  int tm, tn;
+  if (!tile_of(blockIdx.x, (rows + kTile - 1) / kTile, s.tiles_n, 4, &tm, &tn)) return;
+  P p;
+  p.run((lds_char*)lds_raw, s.x, s.w, s.planes, s.first + static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, 0,
+        s.steps);
+
+  float* red = reinterpret_cast<float*>(lds_raw);  // (4, 256): the waves' parts of a row
+  const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
+  const int col = p.wn * P::TN + 4 * g;  // of the lane's first element in the tile
+  const int valid = static_cast<int>(s.vocab - static_cast<int64_t>(tn) * kTile < kTile ? s.vocab - static_cast<int64_t>(tn) * kTile : kTile);
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f) {
+    const int m = p.wm * P::TM + f * 16 + i;
+    const int row = tm * kTile + m;
+    const int label = row < rows ? s.label_of[s.first + row] - tn * kTile - col : -1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < P::FN; ++h)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (col + h * 16 + k < valid) {
+          top = fmaxf(top, p.sums[f][h][k]);
+          if (label == h * 16 + k) s.target[s.first + row] = p.sums[f][h][k];
+        }
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (g == 0) red[p.wn * kTile + m] = top;
+  }
+  __syncthreads();
+  float tops[P::FM];
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f) {
+    const int m = p.wm * P::TM + f * 16 + i;
+    tops[f] = fmaxf(fmaxf(red[m], red[kTile + m]), fmaxf(red[2 * kTile + m], red[3 * kTile + m]));
+  }
+  __syncthreads();
+  const int64_t width = static_cast<int64_t>(s.tiles_n) * kTile;
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f) {
+    const int m = p.wm * P::TM + f * 16 + i;
+    const int row = tm * kTile + m;
+    const float top = tops[f] == -INFINITY ? 0.f : tops[f];
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < P::FN; ++h) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float v = col + h * 16 + k < valid ? __expf(p.sums[f][h][k] - top) : 0.f;
+        sum += v;
+        p.sums[f][h][k] = row < rows ? v : 0.f;
+      }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (g == 0) red[p.wn * kTile + m] = sum;
+  }
+  if (s.e != nullptr) {
+#pragma unroll
+    for (int f = 0; f < P::FM; ++f) {
+      const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
+      E* at = static_cast<E*>(s.e) + row * width + static_cast<int64_t>(tn) * kTile + col;
+#pragma unroll
+      for (int h = 0; h < P::FN; ++h) {
+        typedef E E4 __attribute__((ext_vector_type(4)));
+        E4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = static_cast<E>(sizeof(E) == 2 ? p.sums[f][h][k] * kScale : p.sums[f][h][k]);
+        *reinterpret_cast<E4*>(at + h * 16) = v;
+      }
+    }
+  }
+  __syncthreads();
+  const int m = threadIdx.x;
+  if (m < kTile && tm * kTile + m < rows) {
+    // the sum's own maximum is not kept beside it: every thread of the row holds the same one
+    const float sum = (red[m] + red[kTile + m]) + (red[2 * kTile + m] + red[3 * kTile + m]);
+    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * kTile + m)[1] = sum;
+  }
+  if (p.wn == 0 && g == 0) {
+#pragma unroll
+    for (int f = 0; f < P::FM; ++f) {
+      const int row = tm * kTile + p.wm * P::TM + f * 16 + i;
+      if (row < rows) reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + row)[0] = tops[f];
+    }
+  }
+}
+
+// z of each row from its tiles' sums, and the row's loss.  32 rows a workgroup, eight threads a row, in tile order.
+__global__ __launch_bounds__(256) void join_kernel(const f32x2* __restrict__ sums, int64_t padded, int tiles,
+                                                   const Meta* __restrict__ meta, int64_t first, int64_t chunk,
+                                                   const int* __restrict__ row_of, const int* __restrict__ label_of,
+                                                   const float* __restrict__ target, float* __restrict__ z,
+                                                   float* __restrict__ row_loss, float* __restrict__ losses, int64_t inner,
+                                                   int64_t dx_inner) {
+  __shared__ float tops[8][32], parts[8][32];
+  const int rows = rows_here(meta, first, chunk);
+  const int c = threadIdx.x % 32, part = threadIdx.x / 32;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + c;
+  if (static_cast<int64_t>(blockIdx.x) * 32 >= rows) return;
+  float top = -INFINITY, sum = 0.f;
+  if (row < rows)
+    for (int t = part; t < tiles; t += 8) {
+      const f32x2 v = sums[t * padded + row];
+      if (v[0] > top) {
+        sum = sum * __expf(top - v[0]) + v[1];
+        top = v[0];
+      } else if (v[0] == -INFINITY) {
+        sum += v[1];  // 0, or NaN
+      } else {
+        sum += v[1] * __expf(v[0] - top);
+      }
+    }
+  tops[part][c] = top;
+  parts[part][c] = sum;
+  __syncthreads();
+  if (part != 0 || row >= rows) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) top = fmaxf(top, tops[k][c]);
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum += tops[k][c] == -INFINITY ? parts[k][c] : parts[k][c] * __expf(tops[k][c] - top);
+  const float lse = top + logf(sum);
+  const float loss = label_of[first + row] < 0 ? NAN : lse - target[first + row];
+  z[first + row] = lse;
+  row_loss[first + row] = loss;
+  if (losses != nullptr) {
+    const int64_t d = row_of[first + row], o = d / dx_inner;
+    losses[o * inner + (d - o * dx_inner)] = loss;
+  }
+}
+
+// The sum (or mean) of the kept rows' losses, one workgroup, in a fixed order and 64 bits.
+__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss, const Meta* __restrict__ meta, int mean,
+                                                    float* __restrict__ loss) {
+  __shared__ double parts[16];
+  const int n = meta->count;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) sum += row_loss[i];
+  for (int d = 32; d > 0; d /= 2) sum += __shfl_down(sum, d);
+  if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 16; ++k) sum += parts[k];
+    *loss = static_cast<float>(mean ? sum / n : sum);
+  }
+}
+
+// G from exp(l - m), 16 bytes a thread: 16-bit values in place, or float ones to three planes.
+template <typename T, typename E>
+__global__ __launch_bounds__(256) void slope_kernel(void* __restrict__ e, typename Split<T>::plane* __restrict__ planes, int64_t plane,
+                                                    int64_t width, const f32x2* __restrict__ sums, int64_t padded,
+                                                    const Meta* __restrict__ meta, int64_t first, int64_t chunk,
+                                                    const int* __restrict__ label_of, const float* __restrict__ weight_of,
+                                                    const float* __restrict__ target, const float* __restrict__ z) {
+  constexpr int V = 16 / sizeof(E);
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
+  if (col >= width) return;
+  const int rows = rows_here(meta, first, chunk);
+  const int all = (rows + kStep - 1) / kStep * kStep;  // the last product takes rows 64 by 64: zeros there
+  for (int64_t row = blockIdx.y; row < all; row += gridDim.y) {
+    float out[V];
+    Vec16<E> v;
+    E* at = static_cast<E*>(e) + row * width + col;
+    if (row < rows) {
+      v.raw = *reinterpret_cast<const u32x4*>(at);
+      const float lse = z[first + row];
+      const int label = label_of[first + row];
+      const float weight = weight_of == nullptr ? 1.f : weight_of[first + row] * meta->inv_weight;
+      const float m = sums[(col / kTile) * padded + row][0];
+      const float unit = sizeof(E) == 2 ? 1.f : kScale;
+      // a label outside the vocabulary leaves a NaN, as its loss
+      const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight * unit;
+      const int64_t place = label - col;
+#pragma unroll
+      for (int k = 0; k < V; ++k) out[k] = static_cast<float>(v.e[k]) * factor;
+      if (place >= 0 && place < V) {
+        const float d = expm1f(target[first + row] - lse) * weight * kScale;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (k == place) out[k] = d;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) out[k] = 0.f;
+    }
+    if constexpr (sizeof(E) == 2) {
+      Vec16<T> w;
+#pragma unroll
+      for (int k = 0; k < V; ++k) w.e[k] = static_cast<T>(out[k]);
+      *reinterpret_cast<u32x4*>(at) = w.raw;
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) Split<T>::put(planes + row * width + col + k, plane, out[k]);
+    }
+  }
+}
+
+enum { kFinal = 0, kPart = 1, kAdd = 2, kAddFinal = 3 };
+
+// Where a product's sums go: times alpha to rows of `p`, (rows, cols), or as they are to a part of their own, to be
+// joined; with more than one chunk added to, and from, an fp32 buffer.
+struct Out {
+  void* p;
+  int dtype;
+  int how;
+  int64_t rows, cols;
+  const int* row_of;  // rows of p, or null for their own
+  float* parts;       // (splits, rows padded, cols padded) or the chunks' sum
+  int64_t part_ld, part_size;
+};
+
+__device__ __forceinline__ void put4(void* p, int dtype, int64_t at, f32x4 v, int valid, bool vec) {
+  if (vec && valid >= 4) {
+    if (dtype == PT_FLOAT32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p) + at) = v;
+    } else if (dtype == PT_BFLOAT16) {
+      typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+      b4 w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = static_cast<__bf16>(v[k]);
+      *reinterpret_cast<b4*>(static_cast<__bf16*>(p) + at) = w;
+    } else {
+      typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+      h4 w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = static_cast<_Float16>(v[k]);
+      *reinterpret_cast<h4*>(static_cast<_Float16*>(p) + at) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < valid) store_any(p, at + k, dtype, v[k]);
+}
+
+struct Gradient {
+  Operand a, b;
+  Planes planes;
+  const Meta* meta;
+  int64_t first, chunk;
+  int tiles_m, tiles_n;  // tiles_m < 0: as many as the chunk's rows take
+  int steps;             // < 0: as many as the chunk's rows take
+  int splits;
+  Out out;
+};
+
+template <typename T, bool A_COLUMNS>
+__global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
+  extern __shared__ char lds_raw[];
+  typedef Product<T, A_COLUMNS, true> P;
+  const int rows = rows_here(s.meta, s.first, s.chunk);
+  const int tiles_m = s.tiles_m < 0 ? (rows + kTile - 1) / kTile : s.tiles_m;
+  const int steps = s.steps < 0 ? (rows + kStep - 1) / kStep : s.steps;
+  int tm, tn;
+  // the splits of a tile lie side by side
+  if (!tile_of(blockIdx.x, tiles_m, s.tiles_n * s.splits, 4, &tm, &tn)) return;
+  const int split = tn % s.splits;
+  tn /= s.splits;
+  const int each = (steps + s.splits - 1) / s.splits;
+  const int from = split * each, to = from + each < steps ? from + each : steps;
+  P p;
+  p.run((lds_char*)lds_raw, s.a, s.b, s.planes, static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, from, to);
+
+  const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
+  const Out& o = s.out;
+  const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
+  const float alpha = s.meta->alpha;
+  const bool vec = o.cols % 4 == 0;
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f) {
+    const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
+    if (row >= limit) continue;
+    const int64_t col0 = static_cast<int64_t>(tn) * kTile + p.wn * P::TN + 4 * g;
+    float* part = o.parts + split * o.part_size + row * o.part_ld + col0;
+    const int64_t at = (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col0;
+#pragma unroll
+    for (int h = 0; h < P::FN; ++h) {
+      f32x4 v = p.sums[f][h];
+      const int64_t left = o.cols - (col0 + h * 16);
+      if (left <= 0) continue;
+      if (o.how == kPart) {
+        *reinterpret_cast<f32x4*>(part + h * 16) = v;
+        continue;
+      }
+      v *= alpha;
+      if (o.how == kAdd || o.how == kAddFinal) {
+        if (s.first > 0) v += *reinterpret_cast<f32x4*>(part + h * 16);
+        if (o.how == kAdd) {
+          *reinterpret_cast<f32x4*>(part + h * 16) = v;
+          continue;
+        }
+      }
+      put4(o.p, o.dtype, at + h * 16, v, left < 4 ? static_cast<int>(left) : 4, vec);
+    }
+  }
+}
+
+// Joins the parts of a split product, in their order.
+__global__ __launch_bounds__(256) void parts_kernel(Out o, int splits, const Meta* __restrict__ meta, int64_t first, int64_t chunk,
+                                                    int by_rows) {
+  const int rows = rows_here(meta, first, chunk);
+  const int64_t limit = by_rows ? rows : o.rows;
+  const int64_t quads = (o.cols + 3) / 4;
+  const float alpha = meta->alpha;
+  const bool vec = o.cols % 4 == 0;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < limit * quads; q += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = q / quads, col = (q - row * quads) * 4;
+    const float* p = o.parts + row * o.part_ld + col;
+    f32x4 v = *reinterpret_cast<const f32x4*>(p);
+    for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * o.part_size);
+    v *= alpha;
+    const int64_t left = o.cols - col;
+    put4(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
+  }
+}
+
+// to = from * scale, rounded once; nothing at all where that changes nothing.
+template <typename S, typename D>
+__global__ __launch_bounds__(256) void rescale_kernel(const S* __restrict__ from, D* __restrict__ to, int64_t n,
+                                                      const float* __restrict__ scale) {
+  const float c = *scale;
+  if (sizeof(S) == sizeof(D) && c == 1.f) return;
+  const int64_t quads = n / 4;
+  typedef S S4 __attribute__((ext_vector_type(4)));
+  typedef D D4 __attribute__((ext_vector_type(4)));
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < quads; q += static_cast<int64_t>(gridDim.x) * 256) {
+    const S4 v = reinterpret_cast<const S4*>(from)[q];
+    D4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = static_cast<D>(static_cast<float>(v[k]) * c);
+    reinterpret_cast<D4*>(to)[q] = w;
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n % 4)
+    to[quads * 4 + threadIdx.x] = static_cast<D>(static_cast<float>(from[quads * 4 + threadIdx.x]) * c);
+}
+
+// ------------------------------------------------------------------ sizes
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Plan {
+  bool fp32, copy_weight, grads;
+  int64_t rows, width, words, chunk, chunks, padded;  // width: of x and w; words: of G
+  int planes;
+  int splits_x, splits_w;
+  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, g, sums, parts, total;
+};
+
+// How many parts to split a product of `tiles` tiles and `steps` steps into: a workgroup takes a step in 0.9 us (256 CUs
+// take one tile each), and a part costs its write and read at 4 TB/s.
+int splits_for(int64_t tiles, int64_t steps, double part_bytes) {
+  const int cus = num_cus();
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && s <= steps; ++s) {
+    const double rounds = static_cast<double>((tiles * s + cus - 1) / cus);
+    const double t = rounds * static_cast<double>((steps + s - 1) / s) * 0.9e-6 + (s > 1 ? 3e-6 + s * part_bytes * 2 / 4e12 : 0.0);
+    if (t < least * 0.97) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_t ldw, int dtype, bool want_dx, bool want_dw,
+              int64_t chunk_rows) {
+  Plan p{};
+  p.fp32 = dtype == PT_FLOAT32;
+  p.grads = want_dx || want_dw;
+  p.planes = p.fp32 ? 3 : 1;
+  p.rows = rows;
+  p.width = up(hidden, kStep);
+  p.words = up(vocab, kTile);
+  p.copy_weight = p.fp32 || hidden % kStep != 0 || ldw % 8 != 0 || !aligned16(w);
+  const int64_t each = p.grads ? (p.fp32 ? 10 : 2) * p.words : 0;
+  int64_t most = p.grads ? kChunkBytes / each / kTile * kTile : kScoreRows;
+  if (most < kTile) most = kTile;
+  if (chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
+  p.chunks = rows > 0 ? (rows + most - 1) / most : 1;
+  p.chunk = up((rows + p.chunks - 1) / p.chunks, kTile);
+  if (p.chunk < kTile) p.chunk = kTile;
+  p.padded = p.chunk;
+  const int64_t all = up(rows > 0 ? rows : 1, kTile);
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  p.meta = take(sizeof(Meta));
+  p.row_of = take(all * 4);
+  p.label_of = take(all * 4);
+  p.weight_of = take(all * 4);
+  p.target = take(all * 4);
+  p.z = take(all * 4);
+  p.row_loss = take(all * 4);
+  p.x = take(all * p.width * 2 * p.planes);
+  p.w = take(p.copy_weight ? vocab * p.width * 2 * p.planes : 0);
+  p.sums = take(p.words / kTile * p.padded * sizeof(f32x2));
+  p.e = take(p.grads ? p.chunk * p.words * (p.fp32 ? 4 : 2) : 0);
+  p.g = take(p.grads && p.fp32 ? p.chunk * p.words * 2 * p.planes : 0);
+  const int64_t pairs = p.fp32 ? 6 : 1, cols = up(hidden, kTile);
+  const int64_t tiles_h = cols / kTile, tiles_v = p.words / kTile, tiles_r = p.chunk / kTile;
+  p.splits_x = want_dx ? splits_for(tiles_r * tiles_h, p.words / kStep * pairs, 4.0 * p.chunk * cols) : 1;
+  p.splits_w = want_dw && p.chunks == 1 ? splits_for(tiles_v * tiles_h, p.chunk / kStep * pairs, 4.0 * p.words * cols) : 1;
+  if (p.splits_x > p.words / kStep) p.splits_x = static_cast<int>(p.words / kStep);
+  if (p.splits_w > p.chunk / kStep) p.splits_w = static_cast<int>(p.chunk / kStep);
+  size_t parts = p.splits_x > 1 ? static_cast<size_t>(p.splits_x) * p.chunk * cols * 4 : 0;
+  const size_t parts_w = want_dw && (p.splits_w > 1 || p.chunks > 1) ? static_cast<size_t>(p.splits_w) * p.words * cols * 4 : 0;
+  // the parts of dx are joined before dw begins, but a sum over chunks stays
+  const size_t kept = p.chunks > 1 ? parts_w : 0;
+  p.parts = take((kept > 0 ? 0 : (parts > parts_w ? parts : parts_w)) + kept + (kept > 0 ? parts : 0));
+  p.total = at;
+  return p;
+}
+
+const Planes kOne{1, {0}, {0}};
+const Planes kSix{6, {2, 1, 0, 1, 0, 0}, {0, 1, 2, 0, 1, 0}};
+
+template <typename K>
+int allow(K kernel, size_t bytes) {
+  return allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+}
+
+template <typename T>  // of the inputs
+int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden, int reduction, float* loss, void* dx, void* dw,
+        int grad_dtype, char* ws, const Plan& p, hipStream_t st) {
+  typedef typename Split<T>::plane P;
+  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type E;
+  Meta* meta = reinterpret_cast<Meta*>(ws + p.meta);
+  int* row_of = reinterpret_cast<int*>(ws + p.row_of);
+  int* label_of = reinterpret_cast<int*>(ws + p.label_of);
+  float* weight_of = r.c != nullptr ? reinterpret_cast<float*>(ws + p.weight_of) : nullptr;
+  float* target = reinterpret_cast<float*>(ws + p.target);
+  float* z = reinterpret_cast<float*>(ws + p.z);
+  float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
+  f32x2* sums = reinterpret_cast<f32x2*>(ws + p.sums);
+  float* parts = reinterpret_cast<float*>(ws + p.parts);
+  P* x = reinterpret_cast<P*>(ws + p.x);
+  float* losses = reduction == PT_REDUCTION_NONE ? loss : nullptr;
+
+  hipLaunchKernelGGL(keep_kernel, dim3(1), dim3(1024), 0, st, r, vocab, reduction, row_of, label_of,
+                     reinterpret_cast<float*>(ws + p.weight_of), meta, losses);
+  const int64_t all = up(p.rows, kTile);
+  const int64_t waves = all + (dx != nullptr ? r.outer * r.dx_inner : 0);
+  const unsigned gather_grid = static_cast<unsigned>(waves > 0 ? (waves + 3) / 4 : 1);
+  const int grad_size = dtype_size(grad_dtype);
+  bool vec = false;
+  if constexpr (sizeof(T) == 2) vec = hidden % kStep == 0 && r.xso % 8 == 0 && r.xsi % 8 == 0 && aligned16(r.x);
+  if (vec) {
+    if constexpr (sizeof(T) == 2)
+      hipLaunchKernelGGL((gather_kernel<T, true>), dim3(gather_grid), dim3(256), 0, st, r, row_of, meta, x, all * p.width, p.width,
+                         hidden, all, static_cast<char*>(dx), grad_size);
+  } else {
+    hipLaunchKernelGGL((gather_kernel<T, false>), dim3(gather_grid), dim3(256), 0, st, r, row_of, meta, x, all * p.width, p.width,
+                       hidden, all, static_cast<char*>(dx), grad_size);
+  }
+  Operand ow{w, ldw, 0, ((vocab - 1) * ldw + hidden) * 2};
+  if (p.copy_weight) {
+    P* to = reinterpret_cast<P*>(ws + p.w);
+    const int64_t blocks = (vocab + 3) / 4;
+    hipLaunchKernelGGL(weight_kernel<T>, dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st,
+                       static_cast<const T*>(w), ldw, to, vocab * p.width, p.width, hidden, vocab);
+    ow = Operand{to, p.width, vocab * p.width, vocab * p.width * 2};
+  }
+  if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
+
+  const Planes& planes = p.fp32 ? kSix : kOne;
+  const Operand ox{x, p.width, all * p.width, all * p.width * 2};
+  const int tiles_v = static_cast<int>(p.words / kTile), tiles_h = static_cast<int>(up(hidden, kTile) / kTile);
+  const int tiles_r = static_cast<int>(p.chunk / kTile);
+  constexpr size_t lds = Product<P, false, false>::kLds;
+  if (int rc = allow(scores_kernel<P, E>, lds)) return rc;
+  if (int rc = allow(gradient_kernel<P, false>, lds)) return rc;
+  if (int rc = allow(gradient_kernel<P, true>, lds)) return rc;
+  auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>(up(tiles, 8))); };
+
+  for (int64_t c = 0; c < p.chunks; ++c) {
+    const int64_t first = c * p.chunk;
+    void* e = p.grads ? ws + p.e : nullptr;
+    Scores s{ox, ow, planes, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, sums, p.padded, target};
+    hipLaunchKernelGGL((scores_kernel<P, E>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
+    hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(256), 0, st, sums, p.padded, tiles_v, meta, first,
+                       p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
+    if (!p.grads) continue;
+    P* g = reinterpret_cast<P*>(p.fp32 ? ws + p.g : ws + p.e);
+    const int64_t vectors = p.words * static_cast<int64_t>(sizeof(E)) / 16;
+    hipLaunchKernelGGL((slope_kernel<T, E>), dim3(static_cast<unsigned>((vectors + 255) / 256), static_cast<unsigned>(p.chunk < 16384 ? p.chunk : 16384)),
+                       dim3(256), 0, st, e, g, p.chunk * p.words, p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of,
+                       target, z);
+    const Operand og{g, p.words, p.chunk * p.words, p.chunk * p.words * 2};
+    const int64_t cols = up(hidden, kTile);
+    if (dx != nullptr) {
+      Gradient d{og, ow, planes, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), p.splits_x, {}};
+      // a sum of dw over chunks stays behind the parts
+      d.out = Out{dx, grad_dtype, p.splits_x > 1 ? kPart : kFinal, p.chunk, hidden, row_of, parts, cols, p.chunk * cols};
+      hipLaunchKernelGGL((gradient_kernel<P, false>), grid(static_cast<int64_t>(tiles_r) * tiles_h * p.splits_x), dim3(512), lds, st, d);
+      if (p.splits_x > 1)
+        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_x, meta, first, p.chunk, 1);
+    }
+    if (dw != nullptr) {
+      const Operand oxc{x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2};
+      Gradient d{og, oxc, planes, meta, first, p.chunk, tiles_v, tiles_h, -1, p.splits_w, {}};
+      float* own = p.chunks > 1 && p.splits_x > 1 ? parts + static_cast<int64_t>(p.splits_x) * p.chunk * cols : parts;
+      const int how = p.chunks > 1 ? (c + 1 == p.chunks ? kAddFinal : kAdd) : (p.splits_w > 1 ? kPart : kFinal);
+      d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, own, cols, p.words * cols};
+      hipLaunchKernelGGL((gradient_kernel<P, true>), grid(static_cast<int64_t>(tiles_v) * tiles_h * p.splits_w), dim3(512), lds, st, d);
+      if (how == kPart)
+        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_w, meta, first, p.chunk, 0);
+    }
+    if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
+  }
+  if (loss != nullptr && reduction != PT_REDUCTION_NONE)
+    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, meta, reduction == PT_REDUCTION_MEAN ? 1 : 0, loss);
+  return check_launch("pt_linear_cross_entropy");
+}
+
+int check_sizes(const char* fn, int64_t rows, int64_t vocab, int64_t hidden, int64_t ldw, int dtype) {
+  const std::string name(fn);
+  if (!valid_dtype(dtype)) return fail(PT_EUNSUPPORTED, name + ": dtype must be fp32, fp16 or bf16");
+  if (rows < 0 || vocab < 1 || hidden < 1) return fail(PT_EINVAL, name + ": bad sizes");
+  if (ldw < hidden) return fail(PT_EINVAL, name + ": the weight's rows overlap");
+  // byte offsets inside a tile are 32-bit
+  if (rows > (int64_t{1} << 30) || vocab > (int64_t{1} << 21) || hidden > (int64_t{1} << 20) || ldw > (int64_t{1} << 21))
+    return fail(PT_EUNSUPPORTED, name + ": at most 2^30 rows, 2^21 words, 2^20 wide, 2^21 elements between the weight's rows");
+  return PT_OK;
+}
+
+}  // namespace
+}  // namespace pt
+
+extern "C" {
+
+size_t pt_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, const void* weight, int64_t weight_stride,
+                                               int dtype, int want_dx, int want_dw, int64_t chunk_rows) {
+  if (pt::check_sizes("pt_linear_cross_entropy_workspace_bytes", rows, vocab, hidden, weight_stride, dtype)) return 0;
+  return pt::plan_for(rows, vocab, hidden, weight, weight_stride, dtype, want_dx != 0, want_dw != 0, chunk_rows).total;
+}
+
+int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inner_stride, int64_t outer, int64_t inner,
+                            const void* weight, int64_t weight_stride, int64_t vocab, int64_t hidden, const int64_t* labels,
+                            int64_t label_outer_stride, int64_t label_inner_stride, int64_t ignore_index, int reduction, float* loss,
+                            const float* dloss, int64_t dloss_outer_stride, int64_t dloss_inner_stride, void* dx, int64_t dx_inner,
+                            void* dw, int grad_dtype, void* workspace, size_t workspace_bytes, int64_t chunk_rows, int dtype,
+                            void* stream) {
+  const char* fn = "pt_linear_cross_entropy";
+  const std::string name(fn);
+  if (outer < 0 || inner < 0) return pt::fail(PT_EINVAL, name + ": bad sizes");
+  if (outer > (int64_t{1} << 30) || inner > (int64_t{1} << 30) || outer * inner > (int64_t{1} << 30) || dx_inner > (int64_t{1} << 30))
+    return pt::fail(PT_EUNSUPPORTED, name + ": at most 2^30 rows");
+  const int64_t rows = outer * inner;
+  if (int rc = pt::check_sizes(fn, rows, vocab, hidden, weight_stride, dtype)) return rc;
+  if (reduction != PT_REDUCTION_MEAN && reduction != PT_REDUCTION_SUM && reduction != PT_REDUCTION_NONE)
+    return pt::fail(PT_EINVAL, name + ": unknown reduction");
+  const bool grads = dx != nullptr || dw != nullptr;
+  if (grads && grad_dtype != dtype && grad_dtype != PT_FLOAT32)
+    return pt::fail(PT_EINVAL, name + ": gradients are of the inputs' type, or fp32");
+  if (grads && (reduction == PT_REDUCTION_NONE) != (dloss != nullptr))
+    return pt::fail(PT_EINVAL, name + ": the tokens' weights belong to the gradients of a loss without a reduction");
+  if (!grads && dloss != nullptr) return pt::fail(PT_EINVAL, name + ": weights without gradients");
+  if (dx_inner < inner || outer * dx_inner > (int64_t{1} << 30)) return pt::fail(PT_EINVAL, name + ": dx has too few rows, or over 2^30");
+  if (weight == nullptr || (rows > 0 && (x == nullptr || labels == nullptr)) || workspace == nullptr || (loss == nullptr && !grads && rows > 0))
+    return pt::fail(PT_EINVAL, name + ": null pointer");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return pt::fail(PT_EINVAL, name + ": the workspace must be aligned to 256 bytes");
+  const int size = pt::dtype_size(dtype), grad_size = pt::dtype_size(grad_dtype);
+  if (reinterpret_cast<uintptr_t>(x) % size != 0 || reinterpret_cast<uintptr_t>(weight) % size != 0 ||
+      (grads && (reinterpret_cast<uintptr_t>(dx) % (4 * grad_size) != 0 || reinterpret_cast<uintptr_t>(dw) % (4 * grad_size) != 0)))
+    return pt::fail(PT_EINVAL, name + ": misaligned pointer");
+  const pt::Plan plan = pt::plan_for(rows, vocab, hidden, weight, weight_stride, dtype, dx != nullptr, dw != nullptr, chunk_rows);
+  if (workspace_bytes < plan.total) return pt::fail(PT_EINVAL, name + ": workspace too small");
+  if (rows == 0 && outer * dx_inner == 0 && dw == nullptr && (loss == nullptr || reduction == PT_REDUCTION_NONE)) return pt::ok();
+  const pt::Rows r{x, x_outer_stride, x_inner_stride, labels, label_outer_stride, label_inner_stride, outer, inner, ignore_index,
+                   dloss, dloss_outer_stride, dloss_inner_stride, dx_inner > 0 ? dx_inner : 1};
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t st = pt::as_stream(stream);
+  switch (dtype) {
+    case PT_FLOAT32:
+      return pt::run<float>(r, weight, weight_stride, vocab, hidden, reduction, loss, dx, dw, grad_dtype, ws, plan, st);
+    case PT_FLOAT16:
+      return pt::run<_Float16>(r, weight, weight_stride, vocab, hidden, reduction, loss, dx, dw, grad_dtype, ws, plan, st);
+    default:
+      return pt::run<__bf16>(r, weight, weight_stride, vocab, hidden, reduction, loss, dx, dw, grad_dtype, ws, plan, st);
+  }
+}
+
+int pt_scale_gradient(const void* from, int from_dtype, void* to, int to_dtype, int64_t elements, const float* scale, void* stream) {
+  const std::string name("pt_scale_gradient");
+  if (!pt::valid_dtype(from_dtype) || !pt::valid_dtype(to_dtype)) return pt::fail(PT_EUNSUPPORTED, name + ": dtype must be fp32, fp16 or bf16");
+  if (from_dtype != to_dtype && from_dtype != PT_FLOAT32) return pt::fail(PT_EUNSUPPORTED, name + ": only fp32 changes its type");
+  if (elements < 0) return pt::fail(PT_EINVAL, name + ": negative size");
+  if (elements == 0) return pt::ok();
+  if (from == nullptr || to == nullptr || scale == nullptr) return pt::fail(PT_EINVAL, name + ": null pointer");
+  if (from_dtype == to_dtype && from != to) return pt::fail(PT_EINVAL, name + ": gradients of one type are scaled in place");
+  if (!pt::aligned16(from) || !pt::aligned16(to)) return pt::fail(PT_EINVAL, name + ": pointers must be 16-byte aligned");
+  int64_t blocks = (elements / 4 + 255) / 256;
+  blocks = blocks < 1 ? 1 : (blocks > 8192 ? 8192 : blocks);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  hipStream_t st = pt::as_stream(stream);
+#define PT_SCALE(S, D) \
+  hipLaunchKernelGGL((pt::rescale_kernel<S, D>), grid, dim3(256), 0, st, static_cast<const S*>(from), static_cast<D*>(to), elements, scale)
+  if (from_dtype == PT_FLOAT32) {
+    if (to_dtype == PT_FLOAT32) PT_SCALE(float, float);
+    else if (to_dtype == PT_FLOAT16) PT_SCALE(float, _Float16);
+    else PT_SCALE(float, __bf16);
+  } else if (from_dtype == PT_FLOAT16) {
+    PT_SCALE(_Float16, _Float16);
+  } else {
+    PT_SCALE(__bf16, __bf16);
+  }
+#undef PT_SCALE
+  return pt::check_launch("pt_scale_gradient");
+}
+
+}  // extern "C"

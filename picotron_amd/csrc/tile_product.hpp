@@ -1,0 +1,221 @@
+// Matrix products on the matrix cores: C[m][n] = sum over k of A[m][k] * B[n][k], 16-bit operands, fp32 sums.
+//
+// An operand lies in memory either with k contiguous ("rows": row m holds its k values) or with m contiguous
+// ("columns": row k holds the values of all m).  Either kind goes to LDS as it lies in memory, by loads that
+// write LDS directly; what the matrix instruction wants (8 consecutive k of one m in a lane) is then one
+// 16-byte LDS read of a row tile, or two of gfx950's transposing LDS reads of a column tile.
+#pragma once
+
+#include "pt_common.hpp"
+
+namespace pt {
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStep = 64;  // k of one step: 128 bytes of a row
+
+// One operand.  Element (m, k) of plane s is at p + s * plane + m * ld + k (rows) or + k * ld + m (columns); ld and the
+// planes are multiples of 8 elements and p is aligned to 16 bytes.  A plane has `bytes` bytes: what lies behind is
+// read as zero.
+struct Operand {
+  const void* p;
+  int64_t ld;
+  int64_t plane;
+  int64_t bytes;
+};
+
+// Which planes of the operands a product sums over, in order.  A 32-bit value is the sum of three bf16 planes of 8
+// significant bits each; the six products of planes whose magnitudes lie within 2^-16 of the largest carry 24 bits.
+// The small ones come first, so that they are not lost one by one against a large sum.
+struct Planes {
+  int count;
+  signed char a[6], b[6];
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mfma16<__bf16>(s16x8 a, s16x8 b, f32x4 c) {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mfma16<_Float16>(s16x8 a, s16x8 b, f32x4 c) {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+// A tile of SIZE m by 64 k of one operand in LDS, and its loads by THREADS threads.
+//
+// Rows: 128 bytes of k for each m, its eight 16-byte chunks permuted by XOR with the low bits of m, so that 16 lanes that
+// read the same chunk of 16 consecutive rows touch every bank.  Columns: SIZE * 2 bytes for each k, whose chunks are
+// permuted by bits of k: a transposing read takes two chunks of four consecutive k.
+template <int SIZE, bool COLUMNS, int THREADS>
+struct Tile {
+  static constexpr int kBytes = SIZE * kStep * 2;
+  static constexpr int kLoads = kBytes / (THREADS * 16);
+  static_assert(kLoads * THREADS * 16 == kBytes, "whole loads");
+  static_assert(!COLUMNS || SIZE == 256, "32 chunks a row of k");
+
+  int voffset[kLoads];  // bytes from the tile's first element
+
+  static __device__ __forceinline__ int row_swizzle(int m) { return (m >> 1) & 7; }
+  static __device__ __forceinline__ int column_swizzle(int k) { return ((k & 3) << 1) | (((k >> 3) & 3) << 3); }
+
+  __device__ __forceinline__ void init(int64_t ld) {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int piece = j * THREADS + t;  // 16-byte place in the tile
+      if constexpr (COLUMNS) {
+        const int k = piece / 32, c = (piece % 32) ^ column_swizzle(k);
+        voffset[j] = static_cast<int>(k * ld * 2) + c * 16;
+      } else {
+        const int m = piece / 8, c = (piece % 8) ^ row_swizzle(m);
+        voffset[j] = static_cast<int>(m * ld * 2) + c * 16;
+      }
+    }
+  }
+
+  // Starts the loads of a step's tile: `at` bytes into the plane at `p`, which has `bytes` bytes.
+  __device__ __forceinline__ void load(lds_char* lds, const char* p, int64_t at, int64_t bytes) const {
+    int64_t left = bytes - at;
+    left = left < 0 ? 0 : (left > 0x7ffffff0 ? 0x7ffffff0 : left);
+    const __amdgpu_buffer_rsrc_t r = uniform_buffer(p + at, static_cast<int>(left));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (__attribute__((address_space(3))) void*)(lds + (j * (THREADS / 64) + wave) * 1024), 16, voffset[j], 0, 0, 0);
+  }
+};
+
+// The reads of one wave's fragments of a tile: fragment f is 16 m from `first` + 16 f on.
+template <int SIZE, bool COLUMNS>
+struct Fragments {
+  int base;
+  int chunk, twist;
+
+  __device__ __forceinline__ void init(int first) {
+    const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
+    if constexpr (COLUMNS) {
+      base = (g * 8 + i / 4) * SIZE * 2 + (i & 1) * 8;
+      chunk = first / 8 + ((i & 3) >> 1);
+      twist = ((i / 4) << 1) | (g << 3);
+    } else {
+      base = (first + i) * 128;
+      chunk = g;
+      twist = ((first + i) >> 1) & 7;
+    }
+  }
+
+  // k from 32 * half on, as lane (i, g) of the instruction holds it: 8 consecutive k from 8 g on, of m = i.
+  __device__ __forceinline__ s16x8 read(const lds_char* lds, int f, int half) const {
+    if constexpr (COLUMNS) {
+      typedef __attribute__((address_space(3))) s16x4* lds4;
+      const lds_char* p = lds + base + (((chunk + 2 * f) ^ twist) * 16) + half * 32 * SIZE * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * SIZE * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const lds_char* p = lds + base + f * 16 * 128 + (((half * 4 + chunk) ^ twist) * 16);
+      return *(const __attribute__((address_space(3))) s16x8*)p;
+    }
+  }
+};
+
+// The sums of one workgroup's tile, BM by BN, over the steps [first, last) of 64 k of every plane pair.  WM by WN waves
+// hold TM by TN each; in sums[f][h] lane (i, g) has m = 16 f + i and the four n = 16 h + 4 g + (0..3) of its wave's part.
+template <typename T, int BM, int BN, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS>
+struct TileProduct {
+  static constexpr int kThreads = WM * WN * 64;
+  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  typedef Tile<BM, A_COLUMNS, kThreads> TileA;
+  typedef Tile<BN, B_COLUMNS, kThreads> TileB;
+  static constexpr int kStage = TileA::kBytes + TileB::kBytes;
+  static constexpr int kLds = 2 * kStage;
+
+  f32x4 sums[FM][FN];
+  int wm, wn;
+
+  __device__ __forceinline__ void run(lds_char* lds, const Operand& a, const Operand& b, const Planes& planes, int64_t m0,
+                                      int64_t n0, int first, int last) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    wm = wave / WN;
+    wn = wave % WN;
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int h = 0; h < FN; ++h) sums[f][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (last <= first) return;
+
+    TileA ta;
+    TileB tb;
+    ta.init(a.ld);
+    tb.init(b.ld);
+    Fragments<BM, A_COLUMNS> fa;
+    Fragments<BN, B_COLUMNS> fb;
+    fa.init(wm * TM);
+    fb.init(wn * TN);
+
+    // bytes from one step to the next, and to the tile's first element
+    const int64_t step_a = A_COLUMNS ? a.ld * kStep * 2 : kStep * 2, step_b = B_COLUMNS ? b.ld * kStep * 2 : kStep * 2;
+    const int64_t tile_a = (A_COLUMNS ? m0 : m0 * a.ld) * 2, tile_b = (B_COLUMNS ? n0 : n0 * b.ld) * 2;
+    int pair = 0, step = first;
+    const char* pa = static_cast<const char*>(a.p) + planes.a[0] * a.plane * 2;
+    const char* pb = static_cast<const char*>(b.p) + planes.b[0] * b.plane * 2;
+    auto load = [&](int stage) {
+      lds_char* to = lds + stage * kStage;
+      ta.load(to, pa, tile_a + step * step_a, a.bytes);
+      tb.load(to + TileA::kBytes, pb, tile_b + step * step_b, b.bytes);
+      if (++step == last && ++pair < planes.count) {
+        step = first;
+        pa = static_cast<const char*>(a.p) + planes.a[pair] * a.plane * 2;
+        pb = static_cast<const char*>(b.p) + planes.b[pair] * b.plane * 2;
+      }
+    };
+
+    load(0);
+    __syncthreads();
+    const int total = (last - first) * planes.count;
+    for (int t = 0; t < total; ++t) {
+      if (t + 1 < total) load((t + 1) & 1);
+      const lds_char* la = lds + (t & 1) * kStage;
+      const lds_char* lb = la + TileA::kBytes;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        s16x8 av[FM], bv[FN];
+#pragma unroll
+        for (int h = 0; h < FN; ++h) bv[h] = fb.read(lb, h, half);
+#pragma unroll
+        for (int f = 0; f < FM; ++f) av[f] = fa.read(la, f, half);
+#pragma unroll
+        for (int f = 0; f < FM; ++f)
+#pragma unroll
+          for (int h = 0; h < FN; ++h) sums[f][h] = mfma16<T>(bv[h], av[f], sums[f][h]);
+      }
+      __syncthreads();
+    }
+  }
+};
+
+// The tile (m, n) that workgroup `id` of a grid of at least `tiles_m * tiles_n` takes, or false.  Workgroups go to the eight
+// XCDs in turn; each XCD gets a contiguous run of tiles, and walks it in bands of `band` tiles of m, so that the 32 tiles
+// that run on it together share operands in its L2.
+__device__ __forceinline__ bool tile_of(int64_t id, int tiles_m, int tiles_n, int band, int* tm, int* tn) {
+  const int64_t tiles = static_cast<int64_t>(tiles_m) * tiles_n;
+  const int64_t each = (tiles + 7) / 8;
+  const int64_t place = (id % 8) * each + id / 8;
+  if (id / 8 >= each || place >= tiles) return false;
+  const int64_t per_band = static_cast<int64_t>(band) * tiles_n;
+  const int b = static_cast<int>(place / per_band);
+  const int64_t in = place - b * per_band;
+  const int height = tiles_m - b * band < band ? tiles_m - b * band : band;
+  *tn = static_cast<int>(in / height);
+  *tm = b * band + static_cast<int>(in % height);
+  return true;
+}
+
+}  // namespace pt

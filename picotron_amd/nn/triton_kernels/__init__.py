@@ -25,6 +25,12 @@ from picotron_amd.nn.triton_kernels.cross_entropy import (
     TritonCrossEntropyUnavailable,
     triton_cross_entropy,
 )
+from picotron_amd.nn.triton_kernels.linear_cross_entropy import (
+    LinearCrossEntropyWithFallback,
+    TritonLinearCrossEntropyUnavailable,
+    linear_cross_entropy_with_pytorch,
+    triton_linear_cross_entropy,
+)
 from picotron_amd.nn.triton_kernels.preference import (
     PreferenceLoss,
     PreferenceLossWithFallback,
@@ -70,9 +76,12 @@ __all__ = [
     "rms_norm_with_pytorch_forward",
     # additions beyond the reference surface
     "FusedAdamWStepFailed",
+    "LinearCrossEntropyWithFallback",
     "PreferenceLoss",
     "PreferenceLossWithFallback",
+    "TritonLinearCrossEntropyUnavailable",
     "TritonPreferenceUnavailable",
+    "linear_cross_entropy_with_pytorch",
     "preference_loss_with_pytorch",
     "sequence_log_probs_with_pytorch",
     "triton_adamw_step",
@@ -80,6 +89,7 @@ __all__ = [
     "triton_apply_rotary_embedding_pair",
     "triton_clip_grad_norm_and_step",
     "triton_grad_scaler_step",
+    "triton_linear_cross_entropy",
     "triton_preference_loss",
     "triton_residual_rms_norm",
     "triton_sequence_log_probs",

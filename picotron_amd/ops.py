@@ -744,6 +744,105 @@ def cross_entropy_shifted_scale_grad(
     )
 
 
+# ------------------------------------------------------------------ cross-entropy of a head
+
+REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+def head_rows(hidden: Tensor, weight: Tensor, labels: Tensor, shift: bool) -> tuple[int, int, int]:
+    """(outer, inner, rows of an outer index) of (batch, seq, hidden) or (tokens, hidden) states with labels of their leading
+    shape; with ``shift`` position t belongs to label t + 1, and the last one to none."""
+
+    if hidden.dim() not in (2, 3) or hidden.size(-1) < 1:
+        raise ValueError("hidden states must be (batch, seq, hidden) or (tokens, hidden)")
+    if weight.dim() != 2 or weight.size(1) != hidden.size(-1) or weight.size(0) < 1:
+        raise ValueError("the head's weight must be (vocab, hidden)")
+    if hidden.dtype != weight.dtype or hidden.dtype not in _DTYPE_CODES:
+        raise ValueError("hidden states and the head's weight must be float32, float16 or bfloat16, both of one type")
+    if labels.dtype != torch.int64 or labels.shape != hidden.shape[:-1]:
+        raise ValueError("labels must be int64, one a hidden state")
+    if shift and hidden.dim() != 3:
+        raise ValueError("shifted labels need (batch, seq, hidden) states")
+    if hidden.dim() == 2:
+        return 1, hidden.size(0), hidden.size(0)
+    seq = hidden.size(1)
+    return hidden.size(0), (max(seq - 1, 0) if shift else seq), seq
+
+
+def linear_cross_entropy(
+    hidden: Tensor,
+    weight: Tensor,
+    labels: Tensor,
+    *,
+    shift: bool = False,
+    ignore_index: int = -100,
+    reduction: str = "mean",
+    want_loss: bool = True,
+    want_dx: bool = False,
+    want_dw: bool = False,
+    grad_losses: Tensor | None = None,
+    grad_dtype: torch.dtype | None = None,
+    chunk_tokens: int = 0,
+) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """Cross-entropy of ``hidden @ weight.T`` against ``labels`` without those logits, and its gradients: (loss, dx, dw).
+
+    The loss is an fp32 scalar, or with reduction ``"none"`` fp32 of the labels' shape (seq - 1 with ``shift``).  The
+    gradients (of ``grad_dtype``: the inputs' type or fp32) are those of the mean or sum for an incoming gradient of 1;
+    with ``"none"`` for ``grad_losses``.  At most ``chunk_tokens`` tokens are worked on at a time (0: as many as keep the
+    exponentials within 2 GiB)."""
+
+    device = _check_cuda(hidden, weight, labels)
+    outer, inner, dx_inner = head_rows(hidden, weight, labels, shift)
+    if hidden.stride(-1) != 1:
+        hidden = hidden.contiguous()
+    vocab, width = weight.shape
+    if weight.stride(1) != 1 or weight.stride(0) < width:
+        weight = weight.contiguous()
+    xs = (hidden.stride(0), hidden.stride(1)) if hidden.dim() == 3 else (0, hidden.stride(0))
+    ts = (labels.stride(0), labels.stride(1)) if labels.dim() == 2 else (0, labels.stride(0))
+    shape = labels.shape[:-1] + (inner,) if shift else labels.shape
+    if shift:
+        labels = labels[:, 1:]
+    gs = (0, 0)
+    if grad_losses is not None:
+        if grad_losses.shape != shape or grad_losses.device != device:
+            raise ValueError("the losses' gradients must have the losses' shape")
+        grad_losses = grad_losses.to(torch.float32)
+        gs = (grad_losses.stride(0), grad_losses.stride(1)) if grad_losses.dim() == 2 else (0, grad_losses.stride(0))
+    dtype = grad_dtype or hidden.dtype
+    loss = None
+    if want_loss:
+        loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=device)
+    dx = torch.empty(hidden.shape, dtype=dtype, device=device) if want_dx else None
+    dw = torch.empty(weight.shape, dtype=dtype, device=device) if want_dw else None
+    if outer * inner == 0:
+        if loss is not None:
+            loss.fill_(float("nan") if reduction == "mean" else 0.0)
+        return loss, None if dx is None else dx.zero_(), None if dw is None else dw.zero_()
+    code = dtype_code(hidden.dtype)
+    ws_bytes = _lib.lib().pt_linear_cross_entropy_workspace_bytes(
+        outer * inner, vocab, width, weight.data_ptr(), weight.stride(0), code, int(want_dx), int(want_dw), int(chunk_tokens))
+    ws = torch.empty(max(int(ws_bytes), 16), dtype=torch.uint8, device=device)
+    _call_on(
+        device, "pt_linear_cross_entropy", hidden.data_ptr(), *xs, outer, inner, weight.data_ptr(), weight.stride(0), vocab, width,
+        labels.data_ptr(), *ts, int(ignore_index), REDUCTIONS[reduction], _ptr(loss), _ptr(grad_losses), *gs, _ptr(dx), dx_inner,
+        _ptr(dw), dtype_code(dtype), ws.data_ptr(), ws.numel(), int(chunk_tokens), code,
+    )
+    return loss, dx, dw
+
+
+def scale_gradient(grad: Tensor, scale: Tensor, dtype: torch.dtype | None = None) -> Tensor:
+    """``grad`` (contiguous) times the device scalar ``scale``, rounded once: in place, left alone where the scale is 1, or from
+    fp32 to a new tensor of ``dtype``."""
+
+    device = _check_cuda(grad, scale)
+    scale = scale.detach().to(torch.float32).reshape(())
+    to = grad if dtype in (None, grad.dtype) else torch.empty(grad.shape, dtype=dtype, device=device)
+    _call_on(device, "pt_scale_gradient", grad.data_ptr(), dtype_code(grad.dtype), to.data_ptr(), dtype_code(to.dtype),
+             grad.numel(), scale.data_ptr())
+    return to
+
+
 # ------------------------------------------------------------------ preference loss
 
 PREFERENCE_LOSSES = {"sigmoid": 0, "hinge": 1, "ipo": 2}
