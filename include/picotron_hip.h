@@ -464,6 +464,34 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
 int pt_scale_gradient(const void* from, int from_dtype, void* to, int to_dtype, int64_t elements,
                       const float* scale, void* stream);
 
+/* ---------------------------------------------------------------- Activations kept in 8 bits
+ * What the backward of SwiGLU and RMSNorm reads of their inputs, held as whole numbers of a step that
+ * pt_block8_elems() = 128 consecutive elements share:
+ *   top = max|x|, step = top / 127, code = 128 + round(x * (127 / top)), value = (code - 128) * step
+ * in fp32, every operation correctly rounded, halves to even.  A block whose top is below 2^-100 is held as zeros; one with
+ * an infinity or a NaN has a NaN step.  The last block of the elements (SwiGLU: of the n; RMSNorm: of each row) is
+ * filled up with zeros.
+ *   pt_swiglu8_fwd: pt_swiglu_fwd, and of gate and up codes [blocks, 16, 2, 8] (bytes; per 8 elements those of gate, then
+ *     those of up; 16-byte aligned) and steps [blocks, 2] (8-byte aligned), blocks = ceil(n / 128).
+ *   pt_swiglu8_bwd: pt_swiglu_bwd from them.  dgate or dup may be NULL.
+ *   pt_rmsnorm8_fwd: y and rstd of x, or of h = x + residual (both non-NULL, or both NULL), rounded to the type, and
+ *     codes [rows, blocks, 128] (8-byte aligned) and steps [rows, blocks], blocks = ceil(cols / 128); contiguous rows.
+ *   pt_rmsnorm8_bwd: dx and dweight from them; dh (may be NULL) is added to dx.  dx or dweight may be NULL; the
+ *     workspace belongs to dweight, which is summed in a fixed order. */
+int64_t pt_block8_elems(void);
+int pt_swiglu8_fwd(const void* gate, const void* up, void* out, void* codes, float* steps, int64_t n,
+                   int dtype, void* stream);
+int pt_swiglu8_bwd(const void* dout, const void* codes, const float* steps, void* dgate, void* dup,
+                   int64_t n, int dtype, void* stream);
+int pt_rmsnorm8_fwd(const void* x, const void* residual, const void* weight, void* h, void* y,
+                    float* rstd, void* codes, float* steps, int64_t rows, int64_t cols, float eps,
+                    int x_dtype, int w_dtype, void* stream);
+size_t pt_rmsnorm8_bwd_workspace_bytes(int64_t rows, int64_t cols);
+int pt_rmsnorm8_bwd(const void* dy, const void* dh, const void* weight, const float* rstd,
+                    const void* codes, const float* steps, void* dx, void* dweight, void* workspace,
+                    size_t workspace_bytes, int64_t rows, int64_t cols, int x_dtype, int w_dtype,
+                    void* stream);
+
 /* ---------------------------------------------------------------- Utility
  * Device-to-device copy of `bytes` (multiple of 16, 16-byte aligned pointers) with the
  * same 128-bit load/store pattern as the streaming kernels.  No reference counterpart:

@@ -42,6 +42,7 @@ from picotron_amd.nn.triton_kernels.preference import (
 )
 from picotron_amd.nn.triton_kernels.rmsnorm import (
     TritonRMSNormUnavailable,
+    residual_rms_norm_with_pytorch,
     rms_norm_with_pytorch_forward,
     triton_residual_rms_norm,
     triton_rms_norm,
@@ -83,6 +84,7 @@ __all__ = [
     "TritonPreferenceUnavailable",
     "linear_cross_entropy_with_pytorch",
     "preference_loss_with_pytorch",
+    "residual_rms_norm_with_pytorch",
     "sequence_log_probs_with_pytorch",
     "triton_adamw_step",
     "triton_apply_rotary_at",

@@ -15,6 +15,10 @@ add with the norm that follows it (reference src/picotron/models/picotron_decode
 ``h = x + residual`` and ``y = RMSNorm(h)`` from one pass, and its backward adds the
 gradient arriving at ``h`` from the block's final residual add into the norm's input
 gradient in the same pass.
+
+With ``checkpoint_8bit`` the norm's input is kept for the backward in 8 bits (1.03 bytes an element,
+in place of 2 or 4): blocks of 128 elements of a row share a step, an element is kept to within 1/254 of its block's
+largest, and the gradients are those at the kept values, with the row's exact inverse RMS.
 """
 
 from __future__ import annotations
@@ -25,6 +29,7 @@ import torch
 from torch import Tensor
 
 from picotron_amd import _lib, ops
+from picotron_amd.nn.triton_kernels import _block8
 from picotron_amd.nn.triton_kernels._gate import no_graph, require_hip
 
 
@@ -126,6 +131,41 @@ class _RMSNormAutogradFunction(torch.autograd.Function):
         return (grad_x if need_x else None), (grad_w if need_w else None), None, None
 
 
+class _RMSNorm8Function(torch.autograd.Function):
+    """RMSNorm that keeps its input in 8 bits, by the HIP kernels or in PyTorch: (h, y) with ``residual``, else y."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float, use_hip: bool):  # type: ignore[override]
+        ctx.use_hip = bool(use_hip)
+        ctx.dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        if ctx.use_hip:
+            h, y, rstd, codes, steps = ops.rmsnorm8_fwd(x, weight, eps, residual)
+        else:
+            h = x if residual is None else x + residual
+            inverse_rms = _inverse_rms(h, eps)
+            y, rstd, (codes, steps) = _pytorch_forward(h, weight, inverse_rms), inverse_rms, _block8.encode(h)
+        ctx.save_for_backward(weight, rstd, codes, steps)
+        return y if residual is None else (h, y)
+
+    @staticmethod
+    def backward(ctx, *grads: Tensor | None):  # type: ignore[override]
+        if torch.is_grad_enabled() and not ops._compiling():
+            raise RuntimeError(_block8.NO_SECOND_DERIVATIVE)
+        weight, rstd, codes, steps = ctx.saved_tensors
+        need_x, need_r, need_w = ctx.needs_input_grad[:3]
+        grad_h, grad_y = grads if len(grads) == 2 else (None, grads[0])
+        grad, grad_w = grad_h, None
+        if grad_y is not None:
+            if ctx.use_hip:
+                grad, grad_w = ops.rmsnorm8_bwd(grad_y, weight, rstd, codes, steps, ctx.dtype, grad_h, need_x or need_r, need_w)
+            else:
+                kept = _block8.decode(codes, steps, weight.numel())
+                grad, grad_w = _pytorch_backward(kept, weight, rstd, grad_y)
+                grad = (grad if grad_h is None else grad + grad_h.float()).to(ctx.dtype)
+        return (grad if need_x else None), (grad if need_r else None), (grad_w if need_w else None), None, None
+
+
 def _validate_triton_inputs(hidden_states: Tensor, weight: Tensor) -> None:
     """Launch constraints of the fused path (reference rmsnorm.py:137-149)."""
 
@@ -142,8 +182,8 @@ def _validate_triton_inputs(hidden_states: Tensor, weight: Tensor) -> None:
         raise TritonRMSNormUnavailable("HIP RMSNorm requires contiguous inputs.")
 
 
-def triton_rms_norm(hidden_states: Tensor, weight: Tensor, eps: float) -> Tensor:
-    """Fused RMSNorm (HIP forward and backward).
+def triton_rms_norm(hidden_states: Tensor, weight: Tensor, eps: float, *, checkpoint_8bit: bool = False) -> Tensor:
+    """Fused RMSNorm (HIP forward and backward).  ``checkpoint_8bit``: the backward reads the input from 8 bits.
 
     Callers should catch :class:`TritonRMSNormUnavailable` and use their native RMSNorm
     when the GPU requirements are unmet (reference rmsnorm.py:152-160).
@@ -152,13 +192,17 @@ def triton_rms_norm(hidden_states: Tensor, weight: Tensor, eps: float) -> Tensor
     _validate_triton_inputs(hidden_states, weight)
     if no_graph(hidden_states, weight):
         return ops.rmsnorm_fwd(hidden_states, weight, eps)[0]
+    if checkpoint_8bit:
+        return _RMSNorm8Function.apply(hidden_states, None, weight, eps, True)
     return _RMSNormAutogradFunction.apply(hidden_states, weight, eps, True)
 
 
-def rms_norm_with_pytorch_forward(hidden_states: Tensor, weight: Tensor, eps: float) -> Tensor:
+def rms_norm_with_pytorch_forward(hidden_states: Tensor, weight: Tensor, eps: float, *, checkpoint_8bit: bool = False) -> Tensor:
     """The reference's CPU-verifiable entry point: PyTorch forward and backward through the
     same autograd Function (reference rmsnorm.py:163-171)."""
 
+    if checkpoint_8bit:
+        return _RMSNorm8Function.apply(hidden_states, None, weight, eps, False)
     return _RMSNormAutogradFunction.apply(hidden_states, weight, eps, False)
 
 
@@ -194,9 +238,10 @@ class _ResidualRMSNormFunction(torch.autograd.Function):
 
 
 def triton_residual_rms_norm(
-    hidden_states: Tensor, residual: Tensor, weight: Tensor, eps: float
+    hidden_states: Tensor, residual: Tensor, weight: Tensor, eps: float, *, checkpoint_8bit: bool = False
 ) -> tuple[Tensor, Tensor]:
-    """``h = hidden_states + residual`` and ``RMSNorm(h)`` fused; returns ``(h, y)``.
+    """``h = hidden_states + residual`` and ``RMSNorm(h)`` fused; returns ``(h, y)``.  ``checkpoint_8bit``: the backward
+    reads h from 8 bits.
 
     Raises :class:`TritonRMSNormUnavailable` when the fused path cannot run (callers then
     add and normalise with PyTorch).
@@ -210,4 +255,17 @@ def triton_residual_rms_norm(
         raise TritonRMSNormUnavailable("HIP RMSNorm requires contiguous inputs.")
     if no_graph(hidden_states, residual, weight):
         return ops.residual_rmsnorm_fwd(hidden_states, residual, weight, eps)[:2]
+    if checkpoint_8bit:
+        return _RMSNorm8Function.apply(hidden_states, residual, weight, eps, True)
     return _ResidualRMSNormFunction.apply(hidden_states, residual, weight, eps)
+
+
+def residual_rms_norm_with_pytorch(
+    hidden_states: Tensor, residual: Tensor, weight: Tensor, eps: float, *, checkpoint_8bit: bool = False
+) -> tuple[Tensor, Tensor]:
+    """:func:`triton_residual_rms_norm` in PyTorch."""
+
+    if checkpoint_8bit:
+        return _RMSNorm8Function.apply(hidden_states, residual, weight, eps, False)
+    h = hidden_states + residual
+    return h, _RMSNormAutogradFunction.apply(h, weight, eps, False)

@@ -6,6 +6,10 @@ src/picotron/nn/triton_kernels/swiglu.py): same public names, autograd Function 
 ``apply(gate, up, use_fast_forward)``, exception type and validation.  The reference has a
 Triton forward and an eager backward in the input dtype; here both are one-pass HIP
 kernels computing in fp32 (``pt_swiglu_fwd`` / ``pt_swiglu_bwd``).
+
+With ``checkpoint_8bit`` gate and up are kept for the backward in 8 bits (1.03 bytes an element each, in
+place of 2 or 4): blocks of 128 elements share a step, an element is kept to within 1/254 of its block's largest, and
+the gradients are those at the kept values.
 """
 
 from __future__ import annotations
@@ -15,6 +19,7 @@ from torch import Tensor
 from torch.nn import functional as F
 
 from picotron_amd import ops
+from picotron_amd.nn.triton_kernels import _block8
 from picotron_amd.nn.triton_kernels._gate import no_graph, require_hip
 
 
@@ -59,6 +64,39 @@ class _SwiGLUAutogradFunction(torch.autograd.Function):
         return grad_gate, grad_up, None
 
 
+class _SwiGLU8Function(torch.autograd.Function):
+    """silu(gate) * up that keeps its inputs in 8 bits, by the HIP kernels or in PyTorch."""
+
+    @staticmethod
+    def forward(ctx, gate: Tensor, up: Tensor, use_hip: bool) -> Tensor:  # type: ignore[override]
+        ctx.use_hip = bool(use_hip)
+        ctx.dtype = gate.dtype
+        if ctx.use_hip:
+            output, codes, steps = ops.swiglu8_fwd(gate, up)
+            ctx.save_for_backward(codes, steps)
+            return output
+        ctx.shape = gate.shape
+        ctx.save_for_backward(*_block8.encode(gate.reshape(-1)), *_block8.encode(up.reshape(-1)))
+        return F.silu(gate) * up
+
+    @staticmethod
+    def backward(ctx, grad_output: Tensor):  # type: ignore[override]
+        if torch.is_grad_enabled() and not ops._compiling():
+            raise RuntimeError(_block8.NO_SECOND_DERIVATIVE)
+        need_gate, need_up = ctx.needs_input_grad[:2]
+        if ctx.use_hip:
+            codes, steps = ctx.saved_tensors
+            grad_gate, grad_up = ops.swiglu8_bwd(grad_output, codes, steps, ctx.dtype, need_gate, need_up)
+            return grad_gate, grad_up, None
+        kept = ctx.saved_tensors
+        gate, up = (_block8.decode(*kept[k:k + 2], grad_output.numel()).view(ctx.shape) for k in (0, 2))
+        grad = grad_output.float()
+        sigmoid_gate = torch.sigmoid(gate)
+        grad_gate = grad * up * (sigmoid_gate * (1 + gate * (1 - sigmoid_gate)))
+        grad_up = grad * (gate * sigmoid_gate)
+        return (grad_gate.to(ctx.dtype) if need_gate else None), (grad_up.to(ctx.dtype) if need_up else None), None
+
+
 def _validate_triton_inputs(gate: Tensor, up: Tensor) -> None:
     """Launch constraints of the fused path (reference swiglu.py:84-94)."""
 
@@ -69,16 +107,16 @@ def _validate_triton_inputs(gate: Tensor, up: Tensor) -> None:
         raise TritonSwiGLUUnavailable("HIP SwiGLU requires float32, float16 or bfloat16 inputs of one dtype.")
 
 
-def triton_swiglu(gate: Tensor, up: Tensor) -> Tensor:
-    """Fused SwiGLU activation (HIP forward and backward)."""
+def triton_swiglu(gate: Tensor, up: Tensor, *, checkpoint_8bit: bool = False) -> Tensor:
+    """Fused SwiGLU activation (HIP forward and backward).  ``checkpoint_8bit``: the backward reads gate and up from 8 bits."""
 
     _validate_triton_inputs(gate, up)
     if no_graph(gate, up):
         return ops.swiglu_fwd(gate, up)
-    return _SwiGLUAutogradFunction.apply(gate, up, True)
+    return (_SwiGLU8Function if checkpoint_8bit else _SwiGLUAutogradFunction).apply(gate, up, True)
 
 
-def swiglu_with_pytorch_forward(gate: Tensor, up: Tensor) -> Tensor:
+def swiglu_with_pytorch_forward(gate: Tensor, up: Tensor, *, checkpoint_8bit: bool = False) -> Tensor:
     """The reference's CPU-verifiable entry point (swiglu.py:104-107)."""
 
-    return _SwiGLUAutogradFunction.apply(gate, up, False)
+    return (_SwiGLU8Function if checkpoint_8bit else _SwiGLUAutogradFunction).apply(gate, up, False)

@@ -342,6 +342,128 @@ def swiglu_bwd(
     return dg, du
 
 
+# ------------------------------------------------------------------ activations kept in 8 bits
+
+BLOCK8 = 128  # elements that share a step (pt_block8_elems)
+
+
+def swiglu8_fwd(gate: Tensor, up: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """:func:`swiglu_fwd`, and what :func:`swiglu8_bwd` reads of ``gate`` and ``up``: (out, codes, steps), uint8
+    (blocks, 16, 2, 8) and fp32 (blocks, 2) over blocks of 128 elements of the flat tensors."""
+
+    if _compiling():
+        return torch.ops.picotron_amd.swiglu8_fwd(gate, up)
+    device = _check_cuda(gate, up)
+    if gate.shape != up.shape or gate.dtype != up.dtype:
+        raise ValueError("SwiGLU gate and up must match in shape and dtype")
+    gate, up = _flat(gate), _flat(up)
+    out = torch.empty_like(gate)
+    blocks = (gate.numel() + BLOCK8 - 1) // BLOCK8
+    codes = torch.empty((blocks, 16, 2, 8), dtype=torch.uint8, device=device)
+    steps = torch.empty((blocks, 2), dtype=torch.float32, device=device)
+    _call_on(device, "pt_swiglu8_fwd", gate.data_ptr(), up.data_ptr(), out.data_ptr(), codes.data_ptr(), steps.data_ptr(),
+             gate.numel(), dtype_code(gate.dtype))
+    return out, codes, steps
+
+
+def swiglu8_bwd(
+    dout: Tensor, codes: Tensor, steps: Tensor, dtype: torch.dtype, need_dgate: bool = True, need_dup: bool = True
+) -> tuple[Tensor | None, Tensor | None]:
+    """Gradients of ``dtype`` of SwiGLU's inputs from what :func:`swiglu8_fwd` kept of them."""
+
+    if _compiling():
+        dg, du = torch.ops.picotron_amd.swiglu8_bwd(dout, codes, steps, dtype)
+        return (dg if need_dgate else None), (du if need_dup else None)
+    device = _check_cuda(dout, codes, steps)
+    if dout.dtype != dtype:
+        dout = dout.to(dtype)
+    dout, codes, steps = _flat(dout), _flat(codes), _flat(steps)
+    blocks = (dout.numel() + BLOCK8 - 1) // BLOCK8
+    if (codes.dtype != torch.uint8 or steps.dtype != torch.float32 or codes.shape != (blocks, 16, 2, 8)
+            or steps.shape != (blocks, 2)):
+        raise ValueError("SwiGLU codes and steps must be those of swiglu8_fwd for this many elements")
+    dg = torch.empty_like(dout) if need_dgate else None
+    du = torch.empty_like(dout) if need_dup else None
+    _call_on(device, "pt_swiglu8_bwd", dout.data_ptr(), codes.data_ptr(), steps.data_ptr(), _ptr(dg), _ptr(du), dout.numel(),
+             dtype_code(dtype))
+    return dg, du
+
+
+def rmsnorm8_fwd(
+    x: Tensor, weight: Tensor, eps: float, residual: Tensor | None = None
+) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(h, y, rstd, codes, steps): :func:`rmsnorm_fwd` of x (h is x itself), or :func:`residual_rmsnorm_fwd` of x and
+    ``residual``, and what :func:`rmsnorm8_bwd` reads of h: uint8 (rows, blocks, 128) and fp32 (rows, blocks)."""
+
+    if _compiling():
+        if residual is None:
+            return x, *torch.ops.picotron_amd.rmsnorm8_fwd(x, weight, float(eps))
+        return torch.ops.picotron_amd.residual_rmsnorm8_fwd(x, residual, weight, float(eps))
+    device = _check_cuda(x, weight) if residual is None else _check_cuda(x, weight, residual)
+    cols = x.size(-1)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must match x in shape and dtype")
+    if weight.dim() != 1 or weight.numel() != cols:
+        raise ValueError("RMSNorm weight must be 1-D with hidden-size elements")
+    weight, flat = weight.contiguous(), _flat(x)
+    rows = x.numel() // cols if cols else 0
+    blocks = (cols + BLOCK8 - 1) // BLOCK8
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    residual = None if residual is None else _flat(residual)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+    codes = torch.empty((rows, blocks, BLOCK8), dtype=torch.uint8, device=device)
+    steps = torch.empty((rows, blocks), dtype=torch.float32, device=device)
+    _call_on(
+        device, "pt_rmsnorm8_fwd", flat.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(h), y.data_ptr(), rstd.data_ptr(),
+        codes.data_ptr(), steps.data_ptr(), rows, cols, float(eps), dtype_code(x.dtype), dtype_code(weight.dtype),
+    )
+    return (x if h is None else h), y, rstd, codes, steps
+
+
+def rmsnorm8_bwd(
+    dy: Tensor,
+    weight: Tensor,
+    rstd: Tensor,
+    codes: Tensor,
+    steps: Tensor,
+    dtype: torch.dtype,
+    dh_in: Tensor | None = None,
+    need_dx: bool = True,
+    need_dw: bool = True,
+) -> tuple[Tensor | None, Tensor | None]:
+    """Gradients of the norm's input (of ``dtype``, ``dh_in`` added) and weight, from what :func:`rmsnorm8_fwd` kept."""
+
+    if _compiling():
+        dx, dw = torch.ops.picotron_amd.rmsnorm8_bwd(dy, weight, rstd, codes, steps, dtype, dh_in)
+        return (dx if need_dx else None), (dw if need_dw else None)
+    device = _check_cuda(dy, weight, rstd, codes, steps)
+    cols = weight.numel()
+    if dy.dtype != dtype:
+        dy = dy.to(dtype)
+    dy, weight, rstd, codes, steps = _flat(dy), weight.contiguous(), _flat(rstd), _flat(codes), _flat(steps)
+    rows = dy.numel() // cols if cols else 0
+    blocks = (cols + BLOCK8 - 1) // BLOCK8
+    if (dy.size(-1) != cols or rstd.numel() != rows or rstd.dtype != torch.float32 or codes.dtype != torch.uint8
+            or codes.shape != (rows, blocks, BLOCK8) or steps.dtype != torch.float32 or steps.shape != (rows, blocks)):
+        raise ValueError("RMSNorm rstd, codes and steps must be those of rmsnorm8_fwd for these rows")
+    if dh_in is not None:
+        _check_cuda(dy, dh_in)
+        if dh_in.shape != dy.shape:
+            raise ValueError("dh_in must match dy")
+        dh_in = _flat(dh_in.to(dtype))
+    dx = torch.empty(dy.shape, dtype=dtype, device=device) if need_dx else None
+    dw = torch.empty(cols, dtype=weight.dtype, device=device) if need_dw else None
+    ws = None
+    if need_dw:
+        ws = torch.empty(max(int(_lib.lib().pt_rmsnorm8_bwd_workspace_bytes(rows, cols)), 16), dtype=torch.uint8, device=device)
+    _call_on(
+        device, "pt_rmsnorm8_bwd", dy.data_ptr(), _ptr(dh_in), weight.data_ptr(), rstd.data_ptr(), codes.data_ptr(), steps.data_ptr(),
+        _ptr(dx), _ptr(dw), _ptr(ws), 0 if ws is None else ws.numel(), rows, cols, dtype_code(dtype), dtype_code(weight.dtype),
+    )
+    return dx, dw
+
+
 # ------------------------------------------------------------------ RoPE
 
 
@@ -1396,3 +1518,65 @@ def _op_rope_at_pair(x0: Tensor, x1: Tensor, turns: Tensor, positions: Tensor | 
 @_op_rope_at_pair.register_fake
 def _(x0, x1, turns, positions, offset, scale, layout, inverse):
     return _rope_out(x0), _rope_out(x1)
+
+
+@torch.library.custom_op("picotron_amd::swiglu8_fwd", mutates_args=())
+def _op_swiglu8_fwd(gate: Tensor, up: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    return swiglu8_fwd(gate, up)
+
+
+@_op_swiglu8_fwd.register_fake
+def _(gate, up):
+    blocks = (gate.numel() + BLOCK8 - 1) // BLOCK8
+    return (gate.new_empty(gate.shape), gate.new_empty((blocks, 16, 2, 8), dtype=torch.uint8),
+            gate.new_empty((blocks, 2), dtype=torch.float32))
+
+
+@torch.library.custom_op("picotron_amd::swiglu8_bwd", mutates_args=())
+def _op_swiglu8_bwd(dout: Tensor, codes: Tensor, steps: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    return swiglu8_bwd(dout, codes, steps, dtype)
+
+
+@_op_swiglu8_bwd.register_fake
+def _(dout, codes, steps, dtype):
+    return dout.new_empty(dout.shape, dtype=dtype), dout.new_empty(dout.shape, dtype=dtype)
+
+
+def _fake_rmsnorm8(x):
+    rows, blocks = x.numel() // x.size(-1), (x.size(-1) + BLOCK8 - 1) // BLOCK8
+    return (x.new_empty(x.shape), x.new_empty(x.shape[:-1], dtype=torch.float32),
+            x.new_empty((rows, blocks, BLOCK8), dtype=torch.uint8), x.new_empty((rows, blocks), dtype=torch.float32))
+
+
+@torch.library.custom_op("picotron_amd::rmsnorm8_fwd", mutates_args=())
+def _op_rmsnorm8_fwd(x: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    return rmsnorm8_fwd(x, weight, eps)[1:]
+
+
+@_op_rmsnorm8_fwd.register_fake
+def _(x, weight, eps):
+    return _fake_rmsnorm8(x)
+
+
+@torch.library.custom_op("picotron_amd::residual_rmsnorm8_fwd", mutates_args=())
+def _op_residual_rmsnorm8_fwd(
+    x: Tensor, residual: Tensor, weight: Tensor, eps: float
+) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    return rmsnorm8_fwd(x, weight, eps, residual)
+
+
+@_op_residual_rmsnorm8_fwd.register_fake
+def _(x, residual, weight, eps):
+    return x.new_empty(x.shape), *_fake_rmsnorm8(x)
+
+
+@torch.library.custom_op("picotron_amd::rmsnorm8_bwd", mutates_args=())
+def _op_rmsnorm8_bwd(
+    dy: Tensor, weight: Tensor, rstd: Tensor, codes: Tensor, steps: Tensor, dtype: torch.dtype, dh_in: Tensor | None
+) -> tuple[Tensor, Tensor]:
+    return rmsnorm8_bwd(dy, weight, rstd, codes, steps, dtype, dh_in)
+
+
+@_op_rmsnorm8_bwd.register_fake
+def _(dy, weight, rstd, codes, steps, dtype, dh_in):
+    return dy.new_empty(dy.shape, dtype=dtype), weight.new_empty(weight.shape)

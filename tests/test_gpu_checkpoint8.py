@@ -1,0 +1,334 @@
+"""SwiGLU and RMSNorm that keep their inputs in 8 bits, against the formulas in 64 bits at the kept values."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from gpu_util import randn
+from picotron_amd import ops
+from picotron_amd.nn import RMSNorm, SwiGLU
+from picotron_amd.nn.triton_kernels import (
+    _block8,
+    triton_residual_rms_norm,
+    triton_rms_norm,
+    triton_swiglu,
+)
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+EPS = 1e-5
+
+
+def near(got, want, dtype, total=None, terms=16):
+    """A rounding of the result, and ``terms`` of 2^-23 of ``total`` (the terms' magnitudes) in fp32."""
+
+    total = want.abs() if total is None else total
+    floor = 2.0**-24 if dtype == torch.float16 else 1e-36
+    limit = torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2.0**-10) + terms * 2.0**-23 * total + floor
+    off = (got.double() - want).abs()
+    assert torch.all(off <= limit), float((off / limit).max())
+
+
+def kept_flat(t):
+    return _block8.decode(*_block8.encode(t.detach().reshape(-1)), t.numel()).view(t.shape).double()
+
+
+SIZES = [1, 7, 8, 127, 128, 129, 2047, 2048, 5003, 128 * 300 + 5]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", SIZES)
+def test_swiglu(gpu, dtype, n):
+    g, u, d = (randn((n,), dtype, gpu, seed, scale) for seed, scale in ((1, 3.0), (2, 1.0), (3, 0.5)))
+    g.requires_grad_()
+    u.requires_grad_()
+    y = triton_swiglu(g, u, checkpoint_8bit=True)
+    # the same operations as without the option, but for the last elements of fp16 (one rounding there, or two)
+    assert torch.equal(y[: n // 8 * 8], triton_swiglu(g, u)[: n // 8 * 8])
+    exact = g.detach().double() * torch.sigmoid(g.detach().double()) * u.detach().double()
+    near(y.detach(), exact, dtype, exact.abs() * (1 + g.detach().double().abs()))
+    dg, du = torch.autograd.grad(y, [g, u], d)
+    a, b, e = kept_flat(g), kept_flat(u), d.double()
+    s = torch.sigmoid(a)
+    # the exponential's argument is rounded: |g| * 2^-23 of the sigmoid; 1 + g (1 - s) has terms of that size
+    near(dg, e * b * (s * (1 + a * (1 - s))), dtype, (e * b).abs() * s * (1 + a.abs()) * (1 + a.abs()))
+    near(du, e * a * s, dtype, (e * a * s).abs() * (1 + a.abs()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", SIZES)
+def test_swiglu_codes(gpu, dtype, n):
+    """The codes and steps, to the bit."""
+
+    g, u = (randn((n,), dtype, gpu, seed, 2.0) for seed in (4, 5))
+    g[: n // 3] = 0
+    if n > 256:
+        u[200], u[140], g[n - 1] = math.inf, math.nan, -math.inf
+        g[256:384] = randn((128,), torch.float32, gpu, 6, 1e-33).to(dtype)[: g[256:384].numel()]
+    _, codes, steps = ops.swiglu8_fwd(g, u)
+    for k, t in enumerate((g, u)):
+        want, step = _block8.encode(t)
+        got, mine = codes[:, :, k].reshape(-1, 128), steps[:, k]
+        assert torch.equal(mine.isnan(), step[:, 0].isnan())
+        held = ~step[:, 0].isnan()
+        assert torch.equal(mine[held], step[held, 0]) and torch.equal(got[held], want[held])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rounding_of_halves(gpu, dtype):
+    """Elements half-way between two codes (half of the largest among them) go to the even one, as in PyTorch."""
+
+    x = (torch.arange(-127, 129, device=gpu) / 2).repeat(8).to(dtype)
+    x[::128] = 127 * 2.0 ** (torch.arange(16, device=gpu) % 5).to(dtype)
+    _, codes, steps = ops.swiglu8_fwd(x, x.flip(0))
+    for k, t in enumerate((x, x.flip(0))):
+        want, step = _block8.encode(t)
+        assert torch.equal(codes[:, :, k].reshape(-1, 128), want) and torch.equal(steps[:, k], step[:, 0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_swiglu_at_any_address(gpu, dtype):
+    n = 1000
+    wide = [randn((n + 3,), dtype, gpu, seed) for seed in (1, 2, 3)]
+    for off in (1, 2, 3):
+        g, u, d = (t[off:off + n] for t in wide)
+        out, codes, steps = ops.swiglu8_fwd(g, u)
+        again, c2, s2 = ops.swiglu8_fwd(g.clone(), u.clone())
+        assert torch.equal(out, again) and torch.equal(codes, c2) and torch.equal(steps, s2)
+        for a, b in zip(ops.swiglu8_bwd(d, codes, steps, dtype), ops.swiglu8_bwd(d.clone(), codes, steps, dtype)):
+            assert torch.equal(a, b)
+
+
+def test_swiglu_not_finite(gpu):
+    """A block with an infinity or a NaN has NaN gradients, its neighbours their own."""
+
+    for bad in (math.inf, -math.inf, math.nan):
+        g, u = randn((512,), torch.bfloat16, gpu, 1), randn((512,), torch.bfloat16, gpu, 2)
+        g[130] = bad
+        g.requires_grad_()
+        u.requires_grad_()
+        dg, du = torch.autograd.grad(triton_swiglu(g, u, checkpoint_8bit=True).sum(), [g, u])
+        for d in (dg, du):
+            assert d[128:256].isnan().all() and d[:128].isfinite().all() and d[256:].isfinite().all()
+
+
+SHAPES = [(1, 1), (3, 7), (5, 32), (300, 128), (17, 129), (33, 500), (9, 512), (40, 513), (7, 1090), (600, 1024), (5, 2047), (4, 4096),
+          (3, 8200), (1100, 256), (2, 16384), (3, 16385), (70, 20001)]
+
+
+def norm_oracle(h, w, d, dh, dtype):
+    h64 = h.double()
+    rstd = (h64.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    hat = _block8.decode(*_block8.encode(h), h.size(-1)).double() * rstd
+    gw = d.double() * w.double()
+    dot = (gw * hat).mean(-1, keepdim=True)
+    dx = rstd * (gw - hat * dot)
+    total = rstd * (gw.abs() + hat.abs() * (gw * hat).abs().mean(-1, keepdim=True) * 4)
+    if dh is not None:
+        dx, total = dx + dh.double(), total + dh.double().abs()
+    return h64 * rstd * w.double(), dx, total, (d.double() * hat).sum(0), (d.double() * hat).abs().sum(0)
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype,w_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                           (torch.bfloat16, torch.float16), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_norm(gpu, dtype, w_dtype, rows, cols, residual):
+    x, r, d, dh = (randn((rows, cols), dtype, gpu, seed, scale) for seed, scale in ((1, 1.0), (2, 3.0), (3, 0.5), (4, 0.5)))
+    w = randn((cols,), w_dtype, gpu, 5, 0.3, 1.0).requires_grad_()
+    x.requires_grad_()
+    r.requires_grad_()
+    if residual:
+        h, y = triton_residual_rms_norm(x, r, w, EPS, checkpoint_8bit=True)
+        assert torch.equal(h, x + r)
+        dx, dr, dw = torch.autograd.grad([h, y], [x, r, w], [dh, d])
+        assert torch.equal(dx, dr)
+    else:
+        h, y, dh = x, triton_rms_norm(x, w, EPS, checkpoint_8bit=True), None
+        dx, dw = torch.autograd.grad([y], [x, w], [d])
+    assert y.dtype == dx.dtype == dtype and dw.dtype == w_dtype
+    y64, dx64, total, dw64, dw_total = norm_oracle(h.detach(), w.detach(), d, dh, dtype)
+    # sums of a row in fp32 by at most 64 additions one after the other, of dw by rows
+    near(y.detach(), y64, dtype, terms=64)
+    near(dx, dx64, dtype, total, terms=64)
+    near(dw, dw64, w_dtype, dw_total, terms=64 + rows)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 7), (17, 129), (9, 512), (7, 1090), (4, 4096), (3, 16385)])
+def test_norm_codes(gpu, dtype, rows, cols):
+    x = randn((rows, cols), dtype, gpu, 1, 2.0)
+    x[0] = 0
+    if cols > 300:
+        x[1, 200], x[2, 5], x[1, 270] = math.inf, math.nan, -math.inf
+    _, _, _, codes, steps = ops.rmsnorm8_fwd(x, torch.ones(cols, device=gpu), EPS)
+    want, step = _block8.encode(x)
+    held = ~step[..., 0].isnan()
+    assert torch.equal(steps.isnan(), ~held) and torch.equal(steps[held], step[..., 0][held]) and torch.equal(codes[held], want[held])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_at_any_address(gpu, dtype):
+    rows, cols = 6, 640
+    wide = [randn((rows * cols + 3,), dtype, gpu, seed) for seed in (1, 2, 3)]
+    w = randn((cols + 1,), dtype, gpu, 4)[1:]
+    for off in (1, 2, 3):
+        x, r, d = (t[off:off + rows * cols].view(rows, cols) for t in wide)
+        got = ops.rmsnorm8_fwd(x, w, EPS, r)
+        want = ops.rmsnorm8_fwd(x.clone(), w.clone(), EPS, r.clone())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        a = ops.rmsnorm8_bwd(d, w, *got[2:], dtype, x)
+        b = ops.rmsnorm8_bwd(d.clone(), w.clone(), *got[2:], dtype, x.clone())
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 128), (40, 640), (70, 20001)])
+def test_norm_parts_alone(gpu, rows, cols):
+    x, d, dh = (randn((rows, cols), torch.bfloat16, gpu, seed) for seed in (1, 2, 3))
+    w = randn((cols,), torch.float32, gpu, 4)
+    _, _, rstd, codes, steps = ops.rmsnorm8_fwd(x, w, EPS)
+    dx, dw = ops.rmsnorm8_bwd(d, w, rstd, codes, steps, torch.bfloat16, dh)
+    assert torch.equal(ops.rmsnorm8_bwd(d, w, rstd, codes, steps, torch.bfloat16, dh, need_dw=False)[0], dx)
+    assert torch.equal(ops.rmsnorm8_bwd(d, w, rstd, codes, steps, torch.bfloat16, dh, need_dx=False)[1], dw)
+    for _ in range(2):
+        assert torch.equal(ops.rmsnorm8_bwd(d, w, rstd, codes, steps, torch.bfloat16, dh)[1], dw)
+
+
+def test_empty(gpu):
+    x = torch.empty(0, 64, device=gpu, requires_grad=True)
+    w = torch.ones(64, device=gpu, requires_grad=True)
+    dx, dw = torch.autograd.grad(triton_rms_norm(x, w, EPS, checkpoint_8bit=True).sum(), [x, w])
+    assert dx.shape == x.shape and not dw.any()
+    y = triton_swiglu(x, x, checkpoint_8bit=True)
+    assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape
+
+
+def test_only_the_sum_is_used(gpu):
+    x, r, w = randn((4, 64), torch.float32, gpu, 1).requires_grad_(), randn((4, 64), torch.float32, gpu, 2), torch.ones(64, device=gpu)
+    h, _ = triton_residual_rms_norm(x, r, w, EPS, checkpoint_8bit=True)
+    assert torch.equal(torch.autograd.grad(h.sum(), x)[0], torch.ones_like(x))
+    _, y = triton_residual_rms_norm(x, r, w, EPS, checkpoint_8bit=True)
+    want = triton_rms_norm(h.detach().requires_grad_(), w, EPS, checkpoint_8bit=True)
+    assert torch.equal(y, want)
+
+
+def test_no_second_derivative(gpu):
+    x = randn((2, 64), torch.float32, gpu, 1).requires_grad_()
+    with pytest.raises(RuntimeError, match="checkpoint_8bit"):
+        torch.autograd.grad(triton_swiglu(x, x, checkpoint_8bit=True).sum(), x, create_graph=True)
+
+
+class Block(nn.Module):
+    """The pieces of a decoder block around its attention, as the decoder uses them."""
+
+    def __init__(self, hidden, inner, **options):
+        super().__init__()
+        self.first = RMSNorm(hidden, use_triton_rmsnorm=True, **options)
+        self.mix = nn.Linear(hidden, hidden, bias=False)
+        self.second = RMSNorm(hidden, use_triton_rmsnorm=True, **options)
+        self.feed = SwiGLU(hidden, inner, use_triton_swiglu=True, **options)
+
+    def forward(self, x):
+        h, y = self.second.add_and_norm(self.mix(self.first(x)), x)
+        return h + self.feed(y)
+
+
+def blocks(gpu, dtype, seed=0):
+    torch.manual_seed(seed)
+    plain = nn.Sequential(Block(96, 200), Block(96, 200)).to(gpu)
+    kept = nn.Sequential(Block(96, 200, checkpoint_8bit=True), Block(96, 200, checkpoint_8bit=True)).to(gpu)
+    kept.load_state_dict(plain.state_dict())
+    return plain.to(dtype), kept.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_block(gpu, dtype):
+    plain, kept = blocks(gpu, dtype)
+    x = randn((3, 50, 96), dtype, gpu, 7)
+    want, got = plain(x), kept(x)
+    torch.testing.assert_close(got, want, rtol=0 if dtype == torch.bfloat16 else 1e-5, atol=2e-2 if dtype == torch.bfloat16 else 1e-5)
+    want.square().sum().backward()
+    got.square().sum().backward()
+    for (name, p), q in zip(plain.named_parameters(), kept.parameters()):
+        # values kept to 1/254 of the largest of 128, about 1/85 of their size, in at most four operators on the way
+        assert float((p.grad - q.grad).float().norm() / p.grad.float().norm()) < 4 / 85, name
+    assert not any(getattr(m, "_triton_fallback_warned", False) for m in kept.modules())
+
+
+def test_block_keeps_less(gpu):
+    plain, kept = blocks(gpu, torch.bfloat16)
+    x = randn((8, 512, 96), torch.bfloat16, gpu, 7).requires_grad_()
+
+    def saved(model):
+        total = {}
+
+        def pack(t):
+            total[t.data_ptr()] = t.untyped_storage().nbytes()
+            return t
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            model(x)
+        return sum(total.values())
+
+    assert saved(kept) < 0.8 * saved(plain)
+
+
+def test_compiled(gpu):
+    plain, kept = blocks(gpu, torch.bfloat16)
+    x = randn((3, 50, 96), torch.bfloat16, gpu, 7)
+    torch._dynamo.reset()
+    compiled = torch.compile(kept, fullgraph=True, backend="aot_eager")
+    outs = []
+    for model in (kept, compiled):
+        model.zero_grad()
+        y = model(x)
+        y.square().sum().backward()
+        outs.append([y.detach(), *(p.grad.clone() for p in kept.parameters())])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_captured(gpu):
+    _, kept = blocks(gpu, torch.bfloat16)
+    params = list(kept.parameters())
+    x = randn((3, 50, 96), torch.bfloat16, gpu, 7)
+
+    def step():
+        y = kept(x)
+        return [y.detach(), *torch.autograd.grad(y.square().sum(), params)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        x.copy_(randn((3, 50, 96), torch.bfloat16, gpu, 30 + seed))
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_large_swiglu(gpu):
+    """More than 2^31 elements."""
+
+    n = (1 << 31) + 8 * 127 + 3
+    g = torch.empty(n, dtype=torch.bfloat16, device=gpu)
+    g[: 1 << 31].view(-1, 1 << 20).copy_(randn((1 << 20,), torch.bfloat16, gpu, 1))
+    g[1 << 31:] = randn((n - (1 << 31),), torch.bfloat16, gpu, 2)
+    y, codes, steps = ops.swiglu8_fwd(g, g)
+    dg, du = ops.swiglu8_bwd(g, codes, steps, torch.bfloat16)
+    for part in (slice(0, 1024), slice((1 << 31) - 1024, n)):
+        a, c, s = ops.swiglu8_fwd(g[part].clone(), g[part].clone())
+        assert torch.equal(a, y[part])
+        for p, q in zip(ops.swiglu8_bwd(g[part].clone(), c, s, torch.bfloat16), (dg, du)):
+            assert torch.equal(p, q[part])
