@@ -438,7 +438,8 @@ int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blo
  * is not ignore_index: their mean (NaN of none) or sum as one fp32 value, or with PT_REDUCTION_NONE each row's, fp32
  * [outer, inner], 0 at ignored rows.  A label outside the vocabulary gives NaN, in the loss and in every gradient it
  * enters.  The logits are never held whole: exponentials of at most 2 GiB (chunk_rows rows, where that is fewer;
- * 0: as many as fit) are.  x and weight share `dtype`; fp32 operands are multiplied in three bf16 planes (24 bits).
+ * 0: as many as fit) are.  x and weight share `dtype`; fp32 operands are multiplied as two fp16 planes
+ * each (22 bits and a sign, relative to the tensor's largest element down to 2^-28 of it).
  * Gradients, where dx or dw is non-NULL: dx [outer, dx_inner, hidden] contiguous (rows inner.. and ignored rows zero),
  * dw [vocab, hidden] contiguous, of grad_dtype (dtype or fp32), for an incoming gradient of 1 of the mean or sum; of the
  * loss without a reduction for dloss (fp32, the given strides).  16 bytes (of fp32; 8 of two-byte types) aligned.

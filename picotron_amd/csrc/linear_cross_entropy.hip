@@ -14,8 +14,8 @@
 // - With 16-bit inputs exp(l - m) is held as fp16 scaled by 2^14: 11 bits where the largest bf16 error below is 8,
 //   down to 2^-28 of the tile's largest.  G is rounded to the inputs' type, as the matrix cores take it, scaled by 2^14
 //   too (fp16 keeps softmax values down to 2^-28 normal), and the scale is taken out of the fp32 sums.
-// - With 32-bit inputs every operand is the sum of three bf16 planes of 8 bits (see Planes): 6 products of 16-bit operands
-//   run 2.6 times as fast as one of the fp32 matrix instructions would at its peak.
+// - With 32-bit inputs every operand is two fp16 planes (see kLow), and a product is three of 16-bit operands: 5 times the
+//   rate that the fp32 matrix instructions have at their peak.
 // - Tokens are taken in chunks, so that G takes at most 2 GiB; with more than one, dw is summed in fp32 over them.
 // - The gradients are formed in the forward call, where G is at hand; the backward only multiplies them by what arrives
 //   from above.  fp16's stay in fp32 until then, as a loss scale arrives only there.
@@ -31,12 +31,13 @@ constexpr int64_t kChunkBytes = int64_t{1} << 31;
 constexpr int64_t kScoreRows = 65536;  // rows of a chunk that only leaves sums
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 struct Meta {
   int count;        // kept rows
   float alpha;      // of the gradients' sums
   float inv_weight; // of the rows' own weights
-  int pad;
+  unsigned top_x, top_w;  // bits of the largest finite magnitudes (32-bit inputs)
 };
 
 struct Rows {  // labels, and the rows of x, by (outer, inner)
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int r
     unsigned e = __builtin_bit_cast(unsigned, top) & 0x7f800000u;
     e = e < 0x00800000u ? 0x00800000u : e;
     const float unit = __builtin_bit_cast(float, e);
-    Meta m{base, 0.f, 1.f, 0};
+    Meta m{base, 0.f, 1.f, 0, 0};
     if (reduction == PT_REDUCTION_NONE) {
       m.alpha = unit / kScale;
       m.inv_weight = 1.f / unit;
@@ -115,24 +116,62 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int r
   }
 }
 
-// A value as planes of 16 bits: itself, or three bf16 whose sum it is.
+// The power of two that takes a magnitude, given by its bits, to between 2^13 and 2^14.
+__device__ __forceinline__ int shift_of(unsigned top) {
+  if (top == 0) return 0;
+  int e;
+  (void)frexpf(__builtin_bit_cast(float, top), &e);
+  return 14 - e;
+}
+
+// A value as planes of 16 bits: itself, or two fp16 (see kLow), whose power of two has been taken.
 template <typename T>
 struct Split {
   typedef T plane;
+  static constexpr bool kSplit = false;
   static __device__ __forceinline__ void put(T* p, int64_t, T v) { *p = v; }
 };
 template <>
 struct Split<float> {
-  typedef __bf16 plane;
-  static __device__ __forceinline__ void put(__bf16* p, int64_t plane, float v) {
-    const __bf16 a = static_cast<__bf16>(v);
-    const float r = v - static_cast<float>(a);
-    const __bf16 b = static_cast<__bf16>(r);
-    p[0] = a;
-    p[plane] = b;
-    p[2 * plane] = static_cast<__bf16>(r - static_cast<float>(b));
+  typedef _Float16 plane;
+  static constexpr bool kSplit = true;
+  static __device__ __forceinline__ void parts(float v, _Float16* hi, _Float16* lo) {
+    *hi = static_cast<_Float16>(v);
+    *lo = static_cast<_Float16>((v - static_cast<float>(*hi)) * kLow);
   }
+  static __device__ __forceinline__ void put(_Float16* p, int64_t plane, float v) { parts(v, p, p + plane); }
 };
+
+// The largest finite magnitude of 32-bit rows: the kept ones of x, or those of the weight.  The maximum does not depend on
+// the order in which waves give theirs.
+__global__ __launch_bounds__(256) void top_kernel(const float* __restrict__ p, int64_t ld, int64_t rows, int64_t cols,
+                                                  unsigned* __restrict__ top) {
+  unsigned t = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 4;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; row < rows; row += step)
+    for (int64_t c = threadIdx.x % 64; c < cols; c += 64) {
+      const unsigned b = __builtin_bit_cast(unsigned, p[row * ld + c]) & 0x7fffffffu;
+      if (b < 0x7f800000u && b > t) t = b;
+    }
+  const float all = wave_max(__builtin_bit_cast(float, t));  // finite magnitudes order as their bits
+  if (threadIdx.x % 64 == 0) atomicMax(top, __builtin_bit_cast(unsigned, all));
+}
+
+__global__ __launch_bounds__(256) void top_rows_kernel(Rows r, const int* __restrict__ row_of, Meta* __restrict__ meta, int64_t hidden) {
+  float t = 0.f;
+  const int count = meta->count;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 4;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; i < count; i += step) {
+    const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
+    const float* p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
+    for (int64_t c = threadIdx.x % 64; c < hidden; c += 64) {
+      const float v = fabsf(p[c]);
+      if (v < INFINITY && v > t) t = v;
+    }
+  }
+  t = wave_max(t);
+  if (threadIdx.x % 64 == 0) atomicMax(&meta->top_x, __builtin_bit_cast(unsigned, t));
+}
 
 // One wave a row: the kept rows of x, one behind the other, `width` (a multiple of 64) elements each with zeros
 // behind the H-th, and zero rows up to a whole tile; and zeros in the rows of dx that are not kept.
@@ -156,8 +195,12 @@ __global__ __launch_bounds__(256) void gather_kernel(Rows r, const int* __restri
       for (int64_t c = lane * 8; c < width; c += 512)
         *reinterpret_cast<u32x4*>(p + c) = from != nullptr ? *reinterpret_cast<const u32x4*>(from + c) : zero;
     } else {
-      for (int64_t c = lane; c < width; c += 64)
-        Split<T>::put(p + c, plane, from != nullptr && c < hidden ? from[c] : static_cast<T>(0.f));
+      const int shift = Split<T>::kSplit ? shift_of(meta->top_x) : 0;
+      for (int64_t c = lane; c < width; c += 64) {
+        T v = from != nullptr && c < hidden ? from[c] : static_cast<T>(0.f);
+        if constexpr (Split<T>::kSplit) v = ldexpf(v, shift);
+        Split<T>::put(p + c, plane, v);
+      }
     }
     return;
   }
@@ -176,17 +219,22 @@ __global__ __launch_bounds__(256) void gather_kernel(Rows r, const int* __restri
 // The weight with rows of `width` elements, in planes: for one whose rows the products cannot read in place.
 template <typename T>
 __global__ __launch_bounds__(256) void weight_kernel(const T* __restrict__ w, int64_t ld, typename Split<T>::plane* __restrict__ to,
-                                                     int64_t plane, int64_t width, int64_t hidden, int64_t vocab) {
+                                                     int64_t plane, int64_t width, int64_t hidden, int64_t vocab,
+                                                     const Meta* __restrict__ meta) {
+  const int shift = Split<T>::kSplit ? shift_of(meta->top_w) : 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; row < vocab;
        row += static_cast<int64_t>(gridDim.x) * 4)
-    for (int64_t c = threadIdx.x % 64; c < width; c += 64)
-      Split<T>::put(to + row * width + c, plane, c < hidden ? w[row * ld + c] : static_cast<T>(0.f));
+    for (int64_t c = threadIdx.x % 64; c < width; c += 64) {
+      T v = c < hidden ? w[row * ld + c] : static_cast<T>(0.f);
+      if constexpr (Split<T>::kSplit) v = ldexpf(v, shift);
+      Split<T>::put(to + row * width + c, plane, v);
+    }
 }
 
 // ------------------------------------------------------------------ the three products
 
-template <typename T, bool A_COLUMNS, bool B_COLUMNS>
-using Product = TileProduct<T, kTile, kTile, 2, 4, A_COLUMNS, B_COLUMNS>;
+template <typename T, bool A_COLUMNS, bool B_COLUMNS>  // T of the inputs
+using Product = TileProduct<typename Split<T>::plane, Split<T>::kSplit, kTile, kTile, 2, 4, A_COLUMNS, B_COLUMNS>;
 
 __device__ __forceinline__ int rows_here(const Meta* meta, int64_t first, int64_t chunk) {
   const int64_t n = meta->count - first;
@@ -195,19 +243,18 @@ __device__ __forceinline__ int rows_here(const Meta* meta, int64_t first, int64_
 
 struct Scores {
   Operand x, w;
-  Planes planes;
   const Meta* meta;
   const int* label_of;
   int64_t first, chunk, vocab;
   int tiles_n, steps;
-  void* e;           // exp(l - m), (chunk, tiles_n * 256), or null
+  _Float16* e;       // exp(l - m) * 2^14, (chunk, tiles_n * 256), in one plane or two, or null
+  int64_t e_plane;
   f32x2* sums;       // m and the sum of exp(l - m), (tiles_n, padded)
   int64_t padded;
   float* target;     // the label's logit of each kept row
 };
 
-// E: how exp(l - m) is held (fp16 scaled by 2^14, or float).
-template <typename T, typename E>
+template <typename T>
 __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
   extern __shared__ char lds_raw[];
   typedef Product<T, false, false> P;
@@ -215,9 +262,18 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
   int tm, tn;
   if (!tile_of(blockIdx.x, (rows + kTile - 1) / kTile, s.tiles_n, 4, &tm, &tn)) return;
   P p;
-  p.run((lds_char*)lds_raw, s.x, s.w, s.planes, s.first + static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, 0,
+  p.run((lds_char*)lds_raw, s.x, s.w, s.first + static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, 0,
         s.steps);
 
+  if constexpr (Split<T>::kSplit) {
+    const int shift = -shift_of(s.meta->top_x) - shift_of(s.meta->top_w);
+#pragma unroll
+    for (int f = 0; f < P::FM; ++f)
+#pragma unroll
+      for (int h = 0; h < P::FN; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p.sums[f][h][k] = ldexpf(p.sums[f][h][k], shift);
+  }
   float* red = reinterpret_cast<float*>(lds_raw);  // (4, 256): the waves' parts of a row
   const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
   const int col = p.wn * P::TN + 4 * g;  // of the lane's first element in the tile
@@ -273,14 +329,18 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
 #pragma unroll
     for (int f = 0; f < P::FM; ++f) {
       const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
-      E* at = static_cast<E*>(s.e) + row * width + static_cast<int64_t>(tn) * kTile + col;
+      _Float16* at = s.e + row * width + static_cast<int64_t>(tn) * kTile + col;
 #pragma unroll
       for (int h = 0; h < P::FN; ++h) {
-        typedef E E4 __attribute__((ext_vector_type(4)));
-        E4 v;
+        f16x4 v, low;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = static_cast<E>(sizeof(E) == 2 ? p.sums[f][h][k] * kScale : p.sums[f][h][k]);
-        *reinterpret_cast<E4*>(at + h * 16) = v;
+        for (int k = 0; k < 4; ++k) {
+          const float e = p.sums[f][h][k] * kScale;
+          v[k] = static_cast<_Float16>(e);
+          low[k] = static_cast<_Float16>((e - static_cast<float>(v[k])) * kLow);
+        }
+        *reinterpret_cast<f16x4*>(at + h * 16) = v;
+        if constexpr (Split<T>::kSplit) *reinterpret_cast<f16x4*>(at + s.e_plane + h * 16) = low;
       }
     }
   }
@@ -360,53 +420,56 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
   }
 }
 
-// G from exp(l - m), 16 bytes a thread: 16-bit values in place, or float ones to three planes.
-template <typename T, typename E>
-__global__ __launch_bounds__(256) void slope_kernel(void* __restrict__ e, typename Split<T>::plane* __restrict__ planes, int64_t plane,
-                                                    int64_t width, const f32x2* __restrict__ sums, int64_t padded,
-                                                    const Meta* __restrict__ meta, int64_t first, int64_t chunk,
-                                                    const int* __restrict__ label_of, const float* __restrict__ weight_of,
-                                                    const float* __restrict__ target, const float* __restrict__ z) {
-  constexpr int V = 16 / sizeof(E);
-  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
+// G from exp(l - m), in place, eight elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, int64_t width,
+                                                    const f32x2* __restrict__ sums, int64_t padded, const Meta* __restrict__ meta,
+                                                    int64_t first, int64_t chunk, const int* __restrict__ label_of,
+                                                    const float* __restrict__ weight_of, const float* __restrict__ target,
+                                                    const float* __restrict__ z) {
+  typedef typename Split<T>::plane P;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
   if (col >= width) return;
   const int rows = rows_here(meta, first, chunk);
   const int all = (rows + kStep - 1) / kStep * kStep;  // the last product takes rows 64 by 64: zeros there
   for (int64_t row = blockIdx.y; row < all; row += gridDim.y) {
-    float out[V];
-    Vec16<E> v;
-    E* at = static_cast<E*>(e) + row * width + col;
+    float out[8];
+    _Float16* at = e + row * width + col;
     if (row < rows) {
+      Vec16<_Float16> v, low;
       v.raw = *reinterpret_cast<const u32x4*>(at);
+      if constexpr (Split<T>::kSplit) low.raw = *reinterpret_cast<const u32x4*>(at + plane);
       const float lse = z[first + row];
       const int label = label_of[first + row];
       const float weight = weight_of == nullptr ? 1.f : weight_of[first + row] * meta->inv_weight;
       const float m = sums[(col / kTile) * padded + row][0];
-      const float unit = sizeof(E) == 2 ? 1.f : kScale;
       // a label outside the vocabulary leaves a NaN, as its loss
-      const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight * unit;
+      const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
       const int64_t place = label - col;
 #pragma unroll
-      for (int k = 0; k < V; ++k) out[k] = static_cast<float>(v.e[k]) * factor;
-      if (place >= 0 && place < V) {
+      for (int k = 0; k < 8; ++k) {
+        out[k] = static_cast<float>(v.e[k]);
+        if constexpr (Split<T>::kSplit) out[k] += static_cast<float>(low.e[k]) * (1.0f / kLow);
+        out[k] *= factor;
+      }
+      if (place >= 0 && place < 8) {
         const float d = expm1f(target[first + row] - lse) * weight * kScale;
 #pragma unroll
-        for (int k = 0; k < V; ++k)
+        for (int k = 0; k < 8; ++k)
           if (k == place) out[k] = d;
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k) out[k] = 0.f;
+      for (int k = 0; k < 8; ++k) out[k] = 0.f;
     }
-    if constexpr (sizeof(E) == 2) {
-      Vec16<T> w;
+    Vec16<P> w, low;
 #pragma unroll
-      for (int k = 0; k < V; ++k) w.e[k] = static_cast<T>(out[k]);
-      *reinterpret_cast<u32x4*>(at) = w.raw;
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) Split<T>::put(planes + row * width + col + k, plane, out[k]);
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (Split<T>::kSplit) Split<T>::parts(out[k], &w.e[k], &low.e[k]);
+      else w.e[k] = static_cast<P>(out[k]);
     }
+    *reinterpret_cast<u32x4*>(at) = w.raw;
+    if constexpr (Split<T>::kSplit) *reinterpret_cast<u32x4*>(at + plane) = low.raw;
   }
 }
 
@@ -450,12 +513,12 @@ __device__ __forceinline__ void put4(void* p, int dtype, int64_t at, f32x4 v, in
 
 struct Gradient {
   Operand a, b;
-  Planes planes;
   const Meta* meta;
   int64_t first, chunk;
   int tiles_m, tiles_n;  // tiles_m < 0: as many as the chunk's rows take
   int steps;             // < 0: as many as the chunk's rows take
   int splits;
+  const unsigned* top_b;  // of b's magnitudes (32-bit inputs)
   Out out;
 };
 
@@ -474,13 +537,14 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   const int each = (steps + s.splits - 1) / s.splits;
   const int from = split * each, to = from + each < steps ? from + each : steps;
   P p;
-  p.run((lds_char*)lds_raw, s.a, s.b, s.planes, static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, from, to);
+  p.run((lds_char*)lds_raw, s.a, s.b, static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, from, to);
 
   const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
   const Out& o = s.out;
   const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
   const float alpha = s.meta->alpha;
   const bool vec = o.cols % 4 == 0;
+  const int shift = Split<T>::kSplit ? -shift_of(*s.top_b) : 0;
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
@@ -498,6 +562,10 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
         continue;
       }
       v *= alpha;
+      if constexpr (Split<T>::kSplit) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], shift);
+      }
       if (o.how == kAdd || o.how == kAddFinal) {
         if (s.first > 0) v += *reinterpret_cast<f32x4*>(part + h * 16);
         if (o.how == kAdd) {
@@ -512,7 +580,7 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
 
 // Joins the parts of a split product, in their order.
 __global__ __launch_bounds__(256) void parts_kernel(Out o, int splits, const Meta* __restrict__ meta, int64_t first, int64_t chunk,
-                                                    int by_rows) {
+                                                    int by_rows, const unsigned* __restrict__ top_b) {
   const int rows = rows_here(meta, first, chunk);
   const int64_t limit = by_rows ? rows : o.rows;
   const int64_t quads = (o.cols + 3) / 4;
@@ -524,6 +592,11 @@ __global__ __launch_bounds__(256) void parts_kernel(Out o, int splits, const Met
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
     for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * o.part_size);
     v *= alpha;
+    if (top_b != nullptr) {
+      const int shift = -shift_of(*top_b);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], shift);
+    }
     const int64_t left = o.cols - col;
     put4(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
   }
@@ -558,7 +631,7 @@ struct Plan {
   int64_t rows, width, words, chunk, chunks, padded;  // width: of x and w; words: of G
   int planes;
   int splits_x, splits_w;
-  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, g, sums, parts, total;
+  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, total;
 };
 
 // How many parts to split a product of `tiles` tiles and `steps` steps into: a workgroup takes a step in 0.9 us (256 CUs
@@ -583,12 +656,12 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   Plan p{};
   p.fp32 = dtype == PT_FLOAT32;
   p.grads = want_dx || want_dw;
-  p.planes = p.fp32 ? 3 : 1;
+  p.planes = p.fp32 ? 2 : 1;
   p.rows = rows;
   p.width = up(hidden, kStep);
   p.words = up(vocab, kTile);
   p.copy_weight = p.fp32 || hidden % kStep != 0 || ldw % 8 != 0 || !aligned16(w);
-  const int64_t each = p.grads ? (p.fp32 ? 10 : 2) * p.words : 0;
+  const int64_t each = p.grads ? 2 * p.planes * p.words : 0;
   int64_t most = p.grads ? kChunkBytes / each / kTile * kTile : kScoreRows;
   if (most < kTile) most = kTile;
   if (chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
@@ -613,9 +686,8 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.x = take(all * p.width * 2 * p.planes);
   p.w = take(p.copy_weight ? vocab * p.width * 2 * p.planes : 0);
   p.sums = take(p.words / kTile * p.padded * sizeof(f32x2));
-  p.e = take(p.grads ? p.chunk * p.words * (p.fp32 ? 4 : 2) : 0);
-  p.g = take(p.grads && p.fp32 ? p.chunk * p.words * 2 * p.planes : 0);
-  const int64_t pairs = p.fp32 ? 6 : 1, cols = up(hidden, kTile);
+  p.e = take(p.grads ? p.chunk * p.words * 2 * p.planes : 0);
+  const int64_t pairs = p.fp32 ? 3 : 1, cols = up(hidden, kTile);
   const int64_t tiles_h = cols / kTile, tiles_v = p.words / kTile, tiles_r = p.chunk / kTile;
   p.splits_x = want_dx ? splits_for(tiles_r * tiles_h, p.words / kStep * pairs, 4.0 * p.chunk * cols) : 1;
   p.splits_w = want_dw && p.chunks == 1 ? splits_for(tiles_v * tiles_h, p.chunk / kStep * pairs, 4.0 * p.words * cols) : 1;
@@ -630,9 +702,6 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   return p;
 }
 
-const Planes kOne{1, {0}, {0}};
-const Planes kSix{6, {2, 1, 0, 1, 0, 0}, {0, 1, 2, 0, 1, 0}};
-
 template <typename K>
 int allow(K kernel, size_t bytes) {
   return allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
@@ -642,7 +711,6 @@ template <typename T>  // of the inputs
 int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden, int reduction, float* loss, void* dx, void* dw,
         int grad_dtype, char* ws, const Plan& p, hipStream_t st) {
   typedef typename Split<T>::plane P;
-  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type E;
   Meta* meta = reinterpret_cast<Meta*>(ws + p.meta);
   int* row_of = reinterpret_cast<int*>(ws + p.row_of);
   int* label_of = reinterpret_cast<int*>(ws + p.label_of);
@@ -657,6 +725,13 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
 
   hipLaunchKernelGGL(keep_kernel, dim3(1), dim3(1024), 0, st, r, vocab, reduction, row_of, label_of,
                      reinterpret_cast<float*>(ws + p.weight_of), meta, losses);
+  const int64_t w_blocks = (vocab + 3) / 4 < 8192 ? (vocab + 3) / 4 : 8192;
+  if constexpr (Split<T>::kSplit) {
+    const int64_t x_blocks = (p.rows + 3) / 4 < 4096 ? (p.rows + 3) / 4 : 4096;
+    hipLaunchKernelGGL(top_rows_kernel, dim3(static_cast<unsigned>(x_blocks > 0 ? x_blocks : 1)), dim3(256), 0, st, r, row_of, meta, hidden);
+    hipLaunchKernelGGL(top_kernel, dim3(static_cast<unsigned>(w_blocks)), dim3(256), 0, st, static_cast<const float*>(w), ldw, vocab, hidden,
+                       &meta->top_w);
+  }
   const int64_t all = up(p.rows, kTile);
   const int64_t waves = all + (dx != nullptr ? r.outer * r.dx_inner : 0);
   const unsigned gather_grid = static_cast<unsigned>(waves > 0 ? (waves + 3) / 4 : 1);
@@ -674,55 +749,53 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   Operand ow{w, ldw, 0, ((vocab - 1) * ldw + hidden) * 2};
   if (p.copy_weight) {
     P* to = reinterpret_cast<P*>(ws + p.w);
-    const int64_t blocks = (vocab + 3) / 4;
-    hipLaunchKernelGGL(weight_kernel<T>, dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st,
-                       static_cast<const T*>(w), ldw, to, vocab * p.width, p.width, hidden, vocab);
+    hipLaunchKernelGGL(weight_kernel<T>, dim3(static_cast<unsigned>(w_blocks)), dim3(256), 0, st, static_cast<const T*>(w), ldw, to,
+                       vocab * p.width, p.width, hidden, vocab, meta);
     ow = Operand{to, p.width, vocab * p.width, vocab * p.width * 2};
   }
   if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
 
-  const Planes& planes = p.fp32 ? kSix : kOne;
+  const unsigned* top_x = p.fp32 ? &meta->top_x : nullptr;
+  const unsigned* top_w = p.fp32 ? &meta->top_w : nullptr;
   const Operand ox{x, p.width, all * p.width, all * p.width * 2};
   const int tiles_v = static_cast<int>(p.words / kTile), tiles_h = static_cast<int>(up(hidden, kTile) / kTile);
   const int tiles_r = static_cast<int>(p.chunk / kTile);
-  constexpr size_t lds = Product<P, false, false>::kLds;
-  if (int rc = allow(scores_kernel<P, E>, lds)) return rc;
-  if (int rc = allow(gradient_kernel<P, false>, lds)) return rc;
-  if (int rc = allow(gradient_kernel<P, true>, lds)) return rc;
+  constexpr size_t lds = Product<T, false, false>::kLds;
+  if (int rc = allow(scores_kernel<T>, lds)) return rc;
+  if (int rc = allow(gradient_kernel<T, false>, lds)) return rc;
+  if (int rc = allow(gradient_kernel<T, true>, lds)) return rc;
   auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>(up(tiles, 8))); };
 
   for (int64_t c = 0; c < p.chunks; ++c) {
     const int64_t first = c * p.chunk;
-    void* e = p.grads ? ws + p.e : nullptr;
-    Scores s{ox, ow, planes, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, sums, p.padded, target};
-    hipLaunchKernelGGL((scores_kernel<P, E>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
+    _Float16* e = p.grads ? reinterpret_cast<_Float16*>(ws + p.e) : nullptr;
+    Scores s{ox,    ow, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, p.chunk * p.words,
+             sums,  p.padded, target};
+    hipLaunchKernelGGL((scores_kernel<T>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
     hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(256), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
-    P* g = reinterpret_cast<P*>(p.fp32 ? ws + p.g : ws + p.e);
-    const int64_t vectors = p.words * static_cast<int64_t>(sizeof(E)) / 16;
-    hipLaunchKernelGGL((slope_kernel<T, E>), dim3(static_cast<unsigned>((vectors + 255) / 256), static_cast<unsigned>(p.chunk < 16384 ? p.chunk : 16384)),
-                       dim3(256), 0, st, e, g, p.chunk * p.words, p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of,
-                       target, z);
-    const Operand og{g, p.words, p.chunk * p.words, p.chunk * p.words * 2};
+    hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>((p.words / 8 + 255) / 256), static_cast<unsigned>(p.chunk < 16384 ? p.chunk : 16384)),
+                       dim3(256), 0, st, e, p.chunk * p.words, p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
+    const Operand og{e, p.words, p.chunk * p.words, p.chunk * p.words * 2};
     const int64_t cols = up(hidden, kTile);
     if (dx != nullptr) {
-      Gradient d{og, ow, planes, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), p.splits_x, {}};
+      Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), p.splits_x, top_w, {}};
       // a sum of dw over chunks stays behind the parts
       d.out = Out{dx, grad_dtype, p.splits_x > 1 ? kPart : kFinal, p.chunk, hidden, row_of, parts, cols, p.chunk * cols};
-      hipLaunchKernelGGL((gradient_kernel<P, false>), grid(static_cast<int64_t>(tiles_r) * tiles_h * p.splits_x), dim3(512), lds, st, d);
+      hipLaunchKernelGGL((gradient_kernel<T, false>), grid(static_cast<int64_t>(tiles_r) * tiles_h * p.splits_x), dim3(512), lds, st, d);
       if (p.splits_x > 1)
-        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_x, meta, first, p.chunk, 1);
+        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_x, meta, first, p.chunk, 1, top_w);
     }
     if (dw != nullptr) {
       const Operand oxc{x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2};
-      Gradient d{og, oxc, planes, meta, first, p.chunk, tiles_v, tiles_h, -1, p.splits_w, {}};
+      Gradient d{og, oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, p.splits_w, top_x, {}};
       float* own = p.chunks > 1 && p.splits_x > 1 ? parts + static_cast<int64_t>(p.splits_x) * p.chunk * cols : parts;
       const int how = p.chunks > 1 ? (c + 1 == p.chunks ? kAddFinal : kAdd) : (p.splits_w > 1 ? kPart : kFinal);
       d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, own, cols, p.words * cols};
-      hipLaunchKernelGGL((gradient_kernel<P, true>), grid(static_cast<int64_t>(tiles_v) * tiles_h * p.splits_w), dim3(512), lds, st, d);
+      hipLaunchKernelGGL((gradient_kernel<T, true>), grid(static_cast<int64_t>(tiles_v) * tiles_h * p.splits_w), dim3(512), lds, st, d);
       if (how == kPart)
-        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_w, meta, first, p.chunk, 0);
+        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_w, meta, first, p.chunk, 0, top_x);
     }
     if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
   }

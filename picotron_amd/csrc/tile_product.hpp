@@ -22,17 +22,15 @@ constexpr int kStep = 64;  // k of one step: 128 bytes of a row
 struct Operand {
   const void* p;
   int64_t ld;
-  int64_t plane;
+  int64_t plane;  // from the first plane to the second
   int64_t bytes;
 };
 
-// Which planes of the operands a product sums over, in order.  A 32-bit value is the sum of three bf16 planes of 8
-// significant bits each; the six products of planes whose magnitudes lie within 2^-16 of the largest carry 24 bits.
-// The small ones come first, so that they are not lost one by one against a large sum.
-struct Planes {
-  int count;
-  signed char a[6], b[6];
-};
+// 32-bit operands are two fp16 planes: with v the value times the operand's power of two (its largest magnitude then lies
+// between 2^13 and 2^14), hi = fp16(v) and lo = fp16((v - hi) * 2^11), 22 bits and the sign of lo, down to 2^-28 of the largest.
+// The product is hi hi + 2^-11 (hi lo + lo hi); lo lo, at most 2^-24 of a term, is left out.  The small sums come
+// first, so that their terms are not lost one by one against a large one.
+constexpr float kLow = 2048.0f;
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c);
@@ -126,9 +124,10 @@ struct Fragments {
   }
 };
 
-// The sums of one workgroup's tile, BM by BN, over the steps [first, last) of 64 k of every plane pair.  WM by WN waves
+// The sums of one workgroup's tile, BM by BN, over the steps [first, last) of 64 k, of SPLIT operands in
+// three rounds.  WM by WN waves
 // hold TM by TN each; in sums[f][h] lane (i, g) has m = 16 f + i and the four n = 16 h + 4 g + (0..3) of its wave's part.
-template <typename T, int BM, int BN, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS>
+template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, bool A_COLUMNS, bool B_COLUMNS>
 struct TileProduct {
   static constexpr int kThreads = WM * WN * 64;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
@@ -140,8 +139,8 @@ struct TileProduct {
   f32x4 sums[FM][FN];
   int wm, wn;
 
-  __device__ __forceinline__ void run(lds_char* lds, const Operand& a, const Operand& b, const Planes& planes, int64_t m0,
-                                      int64_t n0, int first, int last) {
+  __device__ __forceinline__ void run(lds_char* lds, const Operand& a, const Operand& b, int64_t m0, int64_t n0,
+                                      int first, int last) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     wm = wave / WN;
     wn = wave % WN;
@@ -163,25 +162,33 @@ struct TileProduct {
     // bytes from one step to the next, and to the tile's first element
     const int64_t step_a = A_COLUMNS ? a.ld * kStep * 2 : kStep * 2, step_b = B_COLUMNS ? b.ld * kStep * 2 : kStep * 2;
     const int64_t tile_a = (A_COLUMNS ? m0 : m0 * a.ld) * 2, tile_b = (B_COLUMNS ? n0 : n0 * b.ld) * 2;
-    int pair = 0, step = first;
-    const char* pa = static_cast<const char*>(a.p) + planes.a[0] * a.plane * 2;
-    const char* pb = static_cast<const char*>(b.p) + planes.b[0] * b.plane * 2;
+    int round = 0, step = first;
+    const char* pa = static_cast<const char*>(a.p) + (SPLIT ? a.plane * 2 : 0);
+    const char* pb = static_cast<const char*>(b.p);
     auto load = [&](int stage) {
       lds_char* to = lds + stage * kStage;
       ta.load(to, pa, tile_a + step * step_a, a.bytes);
       tb.load(to + TileA::kBytes, pb, tile_b + step * step_b, b.bytes);
-      if (++step == last && ++pair < planes.count) {
+      ++step;
+      if (SPLIT && step == last) {  // lo hi, hi lo, hi hi
         step = first;
-        pa = static_cast<const char*>(a.p) + planes.a[pair] * a.plane * 2;
-        pb = static_cast<const char*>(b.p) + planes.b[pair] * b.plane * 2;
+        pa = static_cast<const char*>(a.p);
+        pb = static_cast<const char*>(b.p) + (round == 0 ? b.plane * 2 : 0);
+        ++round;
       }
     };
 
     load(0);
     __syncthreads();
-    const int total = (last - first) * planes.count;
+    const int total = (last - first) * (SPLIT ? 3 : 1);
     for (int t = 0; t < total; ++t) {
       if (t + 1 < total) load((t + 1) & 1);
+      if (SPLIT && t == 2 * (last - first)) {
+#pragma unroll
+        for (int f = 0; f < FM; ++f)
+#pragma unroll
+          for (int h = 0; h < FN; ++h) sums[f][h] *= 1.0f / kLow;
+      }
       const lds_char* la = lds + (t & 1) * kStage;
       const lds_char* lb = la + TileA::kBytes;
 #pragma unroll

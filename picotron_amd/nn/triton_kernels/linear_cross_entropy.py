@@ -105,7 +105,7 @@ def triton_linear_cross_entropy(
     the leading shape; with ``shift`` the state at t is scored against label t + 1 (the last position of each
     sequence against none).  ``reduction``: ``"mean"`` over the labels != ``ignore_index`` (NaN of none), ``"sum"``, or
     ``"none"`` for every token's loss, 0 at ignored ones.  ``chunk_tokens`` bounds how many tokens are worked on at a
-    time, and so the memory of the call: about ``2 * vocab`` bytes a token in 16 bits, ``10 * vocab`` in fp32, 2 GiB at
+    time, and so the memory of the call: about ``2 * vocab`` bytes a token in 16 bits, ``4 * vocab`` in fp32, 2 GiB at
     most in any case.  Differentiable once in ``hidden`` and ``weight``."""
 
     _check_options(reduction, chunk_tokens)

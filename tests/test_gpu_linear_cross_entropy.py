@@ -289,6 +289,21 @@ def test_far_logits(gpu, dtype):
     check(loss.detach(), dx, dw, x.detach(), w.detach(), t, factors)
 
 
+@pytest.mark.parametrize("power", [-90, -60, -20, 20, 60, 100])
+def test_magnitudes_of_32_bits(gpu, power):
+    """States and weights far from one in opposite directions; rows of one tensor 2^20 apart."""
+
+    x, w, t = make(200, 64, 500, torch.float32, gpu)
+    factors = torch.ones(200, device=gpu)
+    spread = torch.where(torch.arange(200, device=gpu) % 2 == 0, 1.0, 2.0**-20)[:, None]
+    x = (x * spread * 2.0**power).requires_grad_()
+    w = (w * 2.0**-power).requires_grad_()
+    loss = triton_linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad([loss], [x, w], [factors])
+    unit = 2.0**power
+    check(loss.detach(), dx * unit, dw / unit, (x / unit).detach(), (w * unit).detach(), t, factors)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_side_alone(gpu, dtype):
     x, w, t = make(90, 64, 300, dtype, gpu)
