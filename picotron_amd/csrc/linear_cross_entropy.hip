@@ -54,46 +54,60 @@ struct Rows {  // labels, and the rows of x, by (outer, inner)
 // ------------------------------------------------------------------ rows
 
 // Which rows are kept, in order: their row of dx, label (-1 for one outside the vocabulary) and weight; how many; the
-// gradients' factor.  One workgroup: a scan of 1024 labels a round (8192 take 10 us).
+// gradients' factor.  One workgroup, a round of whose threads reads eight labels each before the scan.
 __global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int reduction, int* __restrict__ row_of,
                                                     int* __restrict__ label_of, float* __restrict__ weight_of,
                                                     Meta* __restrict__ meta, float* __restrict__ losses) {
-  __shared__ int counts[16];
+  constexpr int kPer = 8;
+  __shared__ int counts[kPer][16];
   __shared__ float tops[16];
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   const int64_t n = r.outer * r.inner;
   int base = 0;
   float top = 0.f;
-  for (int64_t first = 0; first < n; first += 1024) {
-    const int64_t i = first + threadIdx.x;
-    int64_t o = 0, s = 0, t = r.ignore;
-    if (i < n) {
-      o = i / r.inner;
-      s = i - o * r.inner;
-      t = r.t[o * r.tso + s * r.tsi];
-    }
-    const bool keep = i < n && t != r.ignore;
-    const unsigned long long mask = __ballot(keep);
-    if (lane == 0) counts[wave] = __popcll(mask);
-    __syncthreads();
-    int before = base, all = base;
-    for (int k = 0; k < 16; ++k) {
-      if (k < wave) before += counts[k];
-      all += counts[k];
-    }
-    if (keep) {
-      const int at = before + __popcll(mask & ((1ull << lane) - 1));
-      row_of[at] = static_cast<int>(o * r.dx_inner + s);
-      label_of[at] = t >= 0 && t < vocab ? static_cast<int>(t) : -1;
-      if (r.c != nullptr) {
-        const float c = r.c[o * r.cso + s * r.csi];
-        weight_of[at] = c;
-        if (fabsf(c) <= 3.4e38f) top = fmaxf(top, fabsf(c));
+  for (int64_t first = 0; first < n; first += kPer * 1024) {
+    int64_t t[kPer];
+    int row[kPer];
+    unsigned long long mask[kPer];
+    float c[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t i = first + k * 1024 + threadIdx.x;
+      t[k] = r.ignore;
+      c[k] = 0.f;
+      if (i < n) {
+        const int64_t o = i / r.inner, s = i - o * r.inner;
+        t[k] = r.t[o * r.tso + s * r.tsi];
+        if (r.c != nullptr) c[k] = r.c[o * r.cso + s * r.csi];
+        row[k] = static_cast<int>(o * r.dx_inner + s);
       }
-    } else if (i < n && losses != nullptr) {
-      losses[i] = 0.f;
     }
-    base = all;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t i = first + k * 1024 + threadIdx.x;
+      mask[k] = __ballot(t[k] != r.ignore);
+      if (lane == 0) counts[k][wave] = __popcll(mask[k]);
+      if (t[k] == r.ignore && i < n && losses != nullptr) losses[i] = 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      int before = base, all = base;
+      for (int w = 0; w < 16; ++w) {
+        if (w < wave) before += counts[k][w];
+        all += counts[k][w];
+      }
+      base = all;
+      if (t[k] != r.ignore) {
+        const int at = before + __popcll(mask[k] & ((1ull << lane) - 1));
+        row_of[at] = row[k];
+        label_of[at] = t[k] >= 0 && t[k] < vocab ? static_cast<int>(t[k]) : -1;
+        if (r.c != nullptr) {
+          weight_of[at] = c[k];
+          if (fabsf(c[k]) < INFINITY) top = fmaxf(top, fabsf(c[k]));
+        }
+      }
+    }
     __syncthreads();
   }
   top = wave_max(top);
@@ -142,35 +156,35 @@ struct Split<float> {
   static __device__ __forceinline__ void put(_Float16* p, int64_t plane, float v) { parts(v, p, p + plane); }
 };
 
-// The largest finite magnitude of 32-bit rows: the kept ones of x, or those of the weight.  The maximum does not depend on
-// the order in which waves give theirs.
-__global__ __launch_bounds__(256) void top_kernel(const float* __restrict__ p, int64_t ld, int64_t rows, int64_t cols,
-                                                  unsigned* __restrict__ top) {
-  unsigned t = 0;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 4;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; row < rows; row += step)
-    for (int64_t c = threadIdx.x % 64; c < cols; c += 64) {
-      const unsigned b = __builtin_bit_cast(unsigned, p[row * ld + c]) & 0x7fffffffu;
-      if (b < 0x7f800000u && b > t) t = b;
-    }
-  const float all = wave_max(__builtin_bit_cast(float, t));  // finite magnitudes order as their bits
-  if (threadIdx.x % 64 == 0) atomicMax(top, __builtin_bit_cast(unsigned, all));
-}
-
-__global__ __launch_bounds__(256) void top_rows_kernel(Rows r, const int* __restrict__ row_of, Meta* __restrict__ meta, int64_t hidden) {
+// The largest finite magnitudes of 32-bit inputs: workgroups below `x_blocks` take the kept rows of x, the others the weight's.
+// One atomic a workgroup, whose order a maximum does not depend on.
+__global__ __launch_bounds__(256) void top_kernel(Rows r, const int* __restrict__ row_of, Meta* __restrict__ meta, int64_t hidden,
+                                                  int x_blocks, const float* __restrict__ w, int64_t ld, int64_t vocab) {
+  __shared__ float tops[4];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const bool of_x = static_cast<int>(blockIdx.x) < x_blocks;
+  const int64_t blocks = of_x ? x_blocks : gridDim.x - x_blocks, block = of_x ? blockIdx.x : blockIdx.x - x_blocks;
+  const int64_t rows = of_x ? meta->count : vocab;
   float t = 0.f;
-  const int count = meta->count;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 4;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; i < count; i += step) {
-    const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
-    const float* p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
-    for (int64_t c = threadIdx.x % 64; c < hidden; c += 64) {
+  for (int64_t i = block * 4 + wave; i < rows; i += blocks * 4) {
+    const float* p = w + i * ld;
+    if (of_x) {
+      const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
+      p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
+    }
+#pragma unroll 8
+    for (int64_t c = lane; c < hidden; c += 64) {
       const float v = fabsf(p[c]);
-      if (v < INFINITY && v > t) t = v;
+      t = v < INFINITY ? fmaxf(t, v) : t;
     }
   }
   t = wave_max(t);
-  if (threadIdx.x % 64 == 0) atomicMax(&meta->top_x, __builtin_bit_cast(unsigned, t));
+  if (lane == 0) tops[wave] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    atomicMax(of_x ? &meta->top_x : &meta->top_w, __builtin_bit_cast(unsigned, t));  // magnitudes order as their bits
+  }
 }
 
 // One wave a row: the kept rows of x, one behind the other, `width` (a multiple of 64) elements each with zeros
@@ -276,26 +290,39 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
   }
   float* red = reinterpret_cast<float*>(lds_raw);  // (4, 256): the waves' parts of a row
   const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
-  const int col = p.wn * P::TN + 4 * g;  // of the lane's first element in the tile
-  const int valid = static_cast<int>(s.vocab - static_cast<int64_t>(tn) * kTile < kTile ? s.vocab - static_cast<int64_t>(tn) * kTile : kTile);
+  const int col = p.wn * P::TN + 16 * g;  // of the lane's 16 elements in the tile
+  const int64_t left = s.vocab - static_cast<int64_t>(tn) * kTile;
+  if (left < kTile) {  // words that are none
+#pragma unroll
+    for (int f = 0; f < P::FM; ++f)
+#pragma unroll
+      for (int h = 0; h < P::FN; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (col + h * 4 + k >= left) p.sums[f][h][k] = -INFINITY;
+  }
+  // Rows behind the last are zeros of x; what they leave in their tile is not used.
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     const int m = p.wm * P::TM + f * 16 + i;
     const int row = tm * kTile + m;
-    const int label = row < rows ? s.label_of[s.first + row] - tn * kTile - col : -1;
     float top = -INFINITY;
 #pragma unroll
     for (int h = 0; h < P::FN; ++h)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (col + h * 16 + k < valid) {
-          top = fmaxf(top, p.sums[f][h][k]);
-          if (label == h * 16 + k) s.target[s.first + row] = p.sums[f][h][k];
-        }
-      }
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, p.sums[f][h][k]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     if (g == 0) red[p.wn * kTile + m] = top;
+    const int label = (row < rows ? s.label_of[s.first + row] : -1) - tn * kTile - col;
+    if (label >= 0 && label < 16) {
+      float t = 0.f;
+#pragma unroll
+      for (int h = 0; h < P::FN; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t = label == h * 4 + k ? p.sums[f][h][k] : t;
+      s.target[s.first + row] = t;
+    }
   }
   __syncthreads();
   float tops[P::FM];
@@ -306,50 +333,53 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
   }
   __syncthreads();
   const int64_t width = static_cast<int64_t>(s.tiles_n) * kTile;
+  _Float16* to = s.e == nullptr ? nullptr
+                                : s.e + (static_cast<int64_t>(tm) * kTile + p.wm * P::TM + i) * width + static_cast<int64_t>(tn) * kTile + col;
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
-    const int m = p.wm * P::TM + f * 16 + i;
-    const int row = tm * kTile + m;
+    constexpr float kLog2e = 1.44269504088896340736f, kShift = 14.f;  // 2^14 is kScale
     const float top = tops[f] == -INFINITY ? 0.f : tops[f];
+    const float start = kShift - top * kLog2e;
     float sum = 0.f;
 #pragma unroll
-    for (int h = 0; h < P::FN; ++h) {
+    for (int h = 0; h < P::FN; ++h)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float v = col + h * 16 + k < valid ? __expf(p.sums[f][h][k] - top) : 0.f;
-        sum += v;
-        p.sums[f][h][k] = row < rows ? v : 0.f;
+        // 32-bit inputs: the difference first, which is the more exact by the bits of the logit in front of the point
+        const float v = p.sums[f][h][k];
+        const float e = __builtin_amdgcn_exp2f(Split<T>::kSplit ? __builtin_fmaf(v - top, kLog2e, kShift) : __builtin_fmaf(v, kLog2e, start));
+        sum += e;
+        p.sums[f][h][k] = e;
       }
-    }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (g == 0) red[p.wn * kTile + m] = sum;
-  }
-  if (s.e != nullptr) {
+    if (g == 0) red[p.wn * kTile + p.wm * P::TM + f * 16 + i] = sum;
+    if (to != nullptr) {
+      Vec16<_Float16> v[2], low[2];
 #pragma unroll
-    for (int f = 0; f < P::FM; ++f) {
-      const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
-      _Float16* at = s.e + row * width + static_cast<int64_t>(tn) * kTile + col;
-#pragma unroll
-      for (int h = 0; h < P::FN; ++h) {
-        f16x4 v, low;
+      for (int h = 0; h < P::FN; ++h)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float e = p.sums[f][h][k] * kScale;
-          v[k] = static_cast<_Float16>(e);
-          low[k] = static_cast<_Float16>((e - static_cast<float>(v[k])) * kLow);
+          const float e = p.sums[f][h][k];
+          const _Float16 hi = static_cast<_Float16>(e);
+          v[h / 2].e[(h % 2) * 4 + k] = hi;
+          low[h / 2].e[(h % 2) * 4 + k] = static_cast<_Float16>((e - static_cast<float>(hi)) * kLow);
         }
-        *reinterpret_cast<f16x4*>(at + h * 16) = v;
-        if constexpr (Split<T>::kSplit) *reinterpret_cast<f16x4*>(at + s.e_plane + h * 16) = low;
+      u32x4* at = reinterpret_cast<u32x4*>(to + f * 16 * width);
+      at[0] = v[0].raw;
+      at[1] = v[1].raw;
+      if constexpr (Split<T>::kSplit) {
+        at = reinterpret_cast<u32x4*>(to + s.e_plane + f * 16 * width);
+        at[0] = low[0].raw;
+        at[1] = low[1].raw;
       }
     }
   }
   __syncthreads();
   const int m = threadIdx.x;
   if (m < kTile && tm * kTile + m < rows) {
-    // the sum's own maximum is not kept beside it: every thread of the row holds the same one
     const float sum = (red[m] + red[kTile + m]) + (red[2 * kTile + m] + red[3 * kTile + m]);
-    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * kTile + m)[1] = sum;
+    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * kTile + m)[1] = sum * (1.0f / kScale);
   }
   if (p.wn == 0 && g == 0) {
 #pragma unroll
@@ -360,40 +390,36 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
   }
 }
 
-// z of each row from its tiles' sums, and the row's loss.  32 rows a workgroup, eight threads a row, in tile order.
-__global__ __launch_bounds__(256) void join_kernel(const f32x2* __restrict__ sums, int64_t padded, int tiles,
-                                                   const Meta* __restrict__ meta, int64_t first, int64_t chunk,
-                                                   const int* __restrict__ row_of, const int* __restrict__ label_of,
-                                                   const float* __restrict__ target, float* __restrict__ z,
-                                                   float* __restrict__ row_loss, float* __restrict__ losses, int64_t inner,
-                                                   int64_t dx_inner) {
-  __shared__ float tops[8][32], parts[8][32];
+// z of each row from its tiles' sums, and the row's loss.  32 rows a workgroup, 32 threads a row, in a fixed order.
+__global__ __launch_bounds__(1024) void join_kernel(const f32x2* __restrict__ sums, int64_t padded, int tiles,
+                                                    const Meta* __restrict__ meta, int64_t first, int64_t chunk,
+                                                    const int* __restrict__ row_of, const int* __restrict__ label_of,
+                                                    const float* __restrict__ target, float* __restrict__ z,
+                                                    float* __restrict__ row_loss, float* __restrict__ losses, int64_t inner,
+                                                    int64_t dx_inner) {
+  __shared__ float tops[32][33], parts[32][33];
   const int rows = rows_here(meta, first, chunk);
   const int c = threadIdx.x % 32, part = threadIdx.x / 32;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + c;
   if (static_cast<int64_t>(blockIdx.x) * 32 >= rows) return;
   float top = -INFINITY, sum = 0.f;
-  if (row < rows)
-    for (int t = part; t < tiles; t += 8) {
+  if (row < rows) {
+#pragma unroll 4
+    for (int t = part; t < tiles; t += 32) {
       const f32x2 v = sums[t * padded + row];
-      if (v[0] > top) {
-        sum = sum * __expf(top - v[0]) + v[1];
-        top = v[0];
-      } else if (v[0] == -INFINITY) {
-        sum += v[1];  // 0, or NaN
-      } else {
-        sum += v[1] * __expf(v[0] - top);
-      }
+      const float next = fmaxf(top, v[0]);
+      // a tile without a finite logit has a sum of 0, or NaN
+      sum = next == -INFINITY ? sum + v[1] : sum * __expf(top - next) + v[1] * __expf(v[0] - next);
+      top = next;
     }
+  }
   tops[part][c] = top;
   parts[part][c] = sum;
   __syncthreads();
   if (part != 0 || row >= rows) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) top = fmaxf(top, tops[k][c]);
+  for (int k = 1; k < 32; ++k) top = fmaxf(top, tops[k][c]);
   sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) sum += tops[k][c] == -INFINITY ? parts[k][c] : parts[k][c] * __expf(tops[k][c] - top);
+  for (int k = 0; k < 32; ++k) sum += tops[k][c] == -INFINITY ? parts[k][c] : parts[k][c] * __expf(tops[k][c] - top);
   const float lse = top + logf(sum);
   const float loss = label_of[first + row] < 0 ? NAN : lse - target[first + row];
   z[first + row] = lse;
@@ -727,10 +753,9 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
                      reinterpret_cast<float*>(ws + p.weight_of), meta, losses);
   const int64_t w_blocks = (vocab + 3) / 4 < 8192 ? (vocab + 3) / 4 : 8192;
   if constexpr (Split<T>::kSplit) {
-    const int64_t x_blocks = (p.rows + 3) / 4 < 4096 ? (p.rows + 3) / 4 : 4096;
-    hipLaunchKernelGGL(top_rows_kernel, dim3(static_cast<unsigned>(x_blocks > 0 ? x_blocks : 1)), dim3(256), 0, st, r, row_of, meta, hidden);
-    hipLaunchKernelGGL(top_kernel, dim3(static_cast<unsigned>(w_blocks)), dim3(256), 0, st, static_cast<const float*>(w), ldw, vocab, hidden,
-                       &meta->top_w);
+    const int64_t x_blocks = p.rows < 1024 ? (p.rows + 3) / 4 : 256, tops_w = w_blocks < 1024 ? w_blocks : 1024;
+    hipLaunchKernelGGL(top_kernel, dim3(static_cast<unsigned>(x_blocks + tops_w)), dim3(256), 0, st, r, row_of, meta, hidden,
+                       static_cast<int>(x_blocks), static_cast<const float*>(w), ldw, vocab);
   }
   const int64_t all = up(p.rows, kTile);
   const int64_t waves = all + (dx != nullptr ? r.outer * r.dx_inner : 0);
@@ -768,11 +793,12 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
 
   for (int64_t c = 0; c < p.chunks; ++c) {
     const int64_t first = c * p.chunk;
+    const int64_t rows_most = p.rows - first < p.chunk ? p.rows - first : p.chunk;
     _Float16* e = p.grads ? reinterpret_cast<_Float16*>(ws + p.e) : nullptr;
     Scores s{ox,    ow, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, p.chunk * p.words,
              sums,  p.padded, target};
     hipLaunchKernelGGL((scores_kernel<T>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
-    hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(256), 0, st, sums, p.padded, tiles_v, meta, first,
+    hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows_most + 31) / 32)), dim3(1024), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
     hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>((p.words / 8 + 255) / 256), static_cast<unsigned>(p.chunk < 16384 ? p.chunk : 16384)),

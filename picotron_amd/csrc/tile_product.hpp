@@ -47,10 +47,10 @@ __device__ __forceinline__ f32x4 mfma16<_Float16>(s16x8 a, s16x8 b, f32x4 c) {
 
 // A tile of SIZE m by 64 k of one operand in LDS, and its loads by THREADS threads.
 //
-// Rows: 128 bytes of k for each m, its eight 16-byte chunks permuted by XOR with the low bits of m, so that 16 lanes that
-// read the same chunk of 16 consecutive rows touch every bank.  Columns: SIZE * 2 bytes for each k, whose chunks are
+// Rows: 128 bytes of k for each m, its eight 16-byte chunks permuted by XOR with bits of m, so that the 16 lanes that
+// read one chunk of the rows of a fragment (see Fragments) touch every bank.  Columns: SIZE * 2 bytes for each k, whose chunks are
 // permuted by bits of k: a transposing read takes two chunks of four consecutive k.
-template <int SIZE, bool COLUMNS, int THREADS>
+template <int SIZE, bool COLUMNS, bool SPREAD, int THREADS>
 struct Tile {
   static constexpr int kBytes = SIZE * kStep * 2;
   static constexpr int kLoads = kBytes / (THREADS * 16);
@@ -59,7 +59,7 @@ struct Tile {
 
   int voffset[kLoads];  // bytes from the tile's first element
 
-  static __device__ __forceinline__ int row_swizzle(int m) { return (m >> 1) & 7; }
+  static __device__ __forceinline__ int row_swizzle(int m) { return SPREAD ? ((m >> 1) & 1) | (((m >> 4) & 3) << 1) : (m >> 1) & 7; }
   static __device__ __forceinline__ int column_swizzle(int k) { return ((k & 3) << 1) | (((k >> 3) & 3) << 3); }
 
   __device__ __forceinline__ void init(int64_t ld) {
@@ -90,9 +90,11 @@ struct Tile {
   }
 };
 
-// The reads of one wave's fragments of a tile: fragment f is 16 m from `first` + 16 f on.
-template <int SIZE, bool COLUMNS>
+// The reads of one wave's fragments of a tile.  Fragment f is 16 m from `first` + 16 f on; of SPREAD ones the quads of 4 m
+// lie 16 apart, from `first` + 4 f on, so that four fragments give a lane 16 consecutive m of the result.
+template <int SIZE, bool COLUMNS, bool SPREAD>
 struct Fragments {
+  static_assert(!(COLUMNS && SPREAD), "rows only");
   int base;
   int chunk, twist;
 
@@ -103,9 +105,10 @@ struct Fragments {
       chunk = first / 8 + ((i & 3) >> 1);
       twist = ((i / 4) << 1) | (g << 3);
     } else {
-      base = (first + i) * 128;
+      const int m = SPREAD ? first + (i / 4) * 16 + i % 4 : first + i;
+      base = m * 128;
       chunk = g;
-      twist = ((first + i) >> 1) & 7;
+      twist = Tile<SIZE, false, SPREAD, 64>::row_swizzle(m);
     }
   }
 
@@ -118,7 +121,8 @@ struct Fragments {
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * SIZE * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const lds_char* p = lds + base + f * 16 * 128 + (((half * 4 + chunk) ^ twist) * 16);
+      // m moves by 16 (or 4) a fragment, which leaves the bits of the permutation as they are
+      const lds_char* p = lds + base + f * (SPREAD ? 4 : 16) * 128 + (((half * 4 + chunk) ^ twist) * 16);
       return *(const __attribute__((address_space(3))) s16x8*)p;
     }
   }
@@ -126,7 +130,7 @@ struct Fragments {
 
 // The sums of one workgroup's tile, BM by BN, over the steps [first, last) of 64 k, of SPLIT operands in
 // three rounds.  WM by WN waves hold TM by TN each; in sums[f][h] lane (i, g) has m = 16 f + i and the four
-// n = 16 h + 4 g + (0..3) of its wave's part.
+// n = 16 h + 4 g + (0..3) of its wave's part; where both operands lie as rows n = 16 g + 4 h + (0..3).
 //
 // LDS holds two steps, and the registers two halves of one: while one half is multiplied the other one is read, so that no
 // product waits for LDS, and there is one barrier a step, between the halves: every wave has then read the step
@@ -140,8 +144,10 @@ template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, bool A_COLUMNS
 struct TileProduct {
   static constexpr int kThreads = WM * WN * 64;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  typedef Tile<BM, A_COLUMNS, kThreads> TileA;
-  typedef Tile<BN, B_COLUMNS, kThreads> TileB;
+  static constexpr bool kSpread = !A_COLUMNS && !B_COLUMNS;
+  static_assert(!kSpread || FN == 4, "four quads of 16");
+  typedef Tile<BM, A_COLUMNS, false, kThreads> TileA;
+  typedef Tile<BN, B_COLUMNS, kSpread, kThreads> TileB;
   static constexpr int kStage = TileA::kBytes + TileB::kBytes;
   static constexpr int kLds = 2 * kStage;
 
@@ -163,8 +169,8 @@ struct TileProduct {
     TileB tb;
     ta.init(a.ld);
     tb.init(b.ld);
-    Fragments<BM, A_COLUMNS> fa;
-    Fragments<BN, B_COLUMNS> fb;
+    Fragments<BM, A_COLUMNS, false> fa;
+    Fragments<BN, B_COLUMNS, kSpread> fb;
     fa.init(wm * TM);
     fb.init(wn * TN);
 
