@@ -499,7 +499,27 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
   }
 }
 
-enum { kFinal = 0, kPart = 1, kAdd = 2, kAddFinal = 3 };
+// How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each,
+// a workgroup a step in 1.9 us, and each tile of a part costs 0.13 us for its way to memory and back.  The number of
+// tiles follows from the number of kept rows, so this is decided on the device; `most` bounds the tiles of all parts (0: no
+// split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps, 1025 us in one part.
+constexpr int64_t kMostParts = 1024;
+__host__ __device__ inline int splits_for(int64_t tiles, int64_t steps, int64_t most) {
+  constexpr int kTry[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
+  int best = 1;
+  int64_t least = (tiles + 255) / 256 * steps * 1900;
+  for (int s : kTry) {
+    if (s > steps || s * tiles > most) break;
+    const int64_t t = (tiles * s + 255) / 256 * ((steps + s - 1) / s) * 1900 + 5000 + tiles * s * 130;
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+enum { kFinal = 0, kAdd = 1, kAddFinal = 2 };
 
 // Where a product's sums go: times alpha to rows of `p`, (rows, cols), or as they are to a part of their own, to be
 // joined; with more than one chunk added to, and from, an fp32 buffer.
@@ -509,8 +529,7 @@ struct Out {
   int how;
   int64_t rows, cols;
   const int* row_of;  // rows of p, or null for their own
-  float* parts;       // (splits, rows padded, cols padded) or the chunks' sum
-  int64_t part_ld, part_size;
+  float* parts;       // (splits, tiles_m * 256, tiles_n * 256) or the chunks' sum
 };
 
 __device__ __forceinline__ void put4(void* p, int dtype, int64_t at, f32x4 v, int valid, bool vec) {
@@ -543,7 +562,8 @@ struct Gradient {
   int64_t first, chunk;
   int tiles_m, tiles_n;  // tiles_m < 0: as many as the chunk's rows take
   int steps;             // < 0: as many as the chunk's rows take
-  int splits;
+  int rounds;            // of the steps (32-bit inputs: 3)
+  int64_t most_parts;
   const unsigned* top_b;  // of b's magnitudes (32-bit inputs)
   Out out;
 };
@@ -555,12 +575,13 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   const int rows = rows_here(s.meta, s.first, s.chunk);
   const int tiles_m = s.tiles_m < 0 ? (rows + kTile - 1) / kTile : s.tiles_m;
   const int steps = s.steps < 0 ? (rows + kStep - 1) / kStep : s.steps;
+  const int splits = splits_for(static_cast<int64_t>(tiles_m) * s.tiles_n, static_cast<int64_t>(steps) * s.rounds, s.most_parts);
   int tm, tn;
   // the splits of a tile lie side by side
-  if (!tile_of(blockIdx.x, tiles_m, s.tiles_n * s.splits, 4, &tm, &tn)) return;
-  const int split = tn % s.splits;
-  tn /= s.splits;
-  const int each = (steps + s.splits - 1) / s.splits;
+  if (!tile_of(blockIdx.x, tiles_m, s.tiles_n * splits, 4, &tm, &tn)) return;
+  const int split = tn % splits;
+  tn /= splits;
+  const int each = (steps + splits - 1) / splits;
   const int from = split * each, to = from + each < steps ? from + each : steps;
   P p;
   p.run((lds_char*)lds_raw, s.a, s.b, static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, from, to);
@@ -576,14 +597,14 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
     const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
     if (row >= limit) continue;
     const int64_t col0 = static_cast<int64_t>(tn) * kTile + p.wn * P::TN + 4 * g;
-    float* part = o.parts + split * o.part_size + row * o.part_ld + col0;
+    float* part = o.parts + (static_cast<int64_t>(split) * tiles_m * kTile + row) * s.tiles_n * kTile + col0;
     const int64_t at = (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col0;
 #pragma unroll
     for (int h = 0; h < P::FN; ++h) {
       f32x4 v = p.sums[f][h];
       const int64_t left = o.cols - (col0 + h * 16);
       if (left <= 0) continue;
-      if (o.how == kPart) {
+      if (splits > 1) {
         *reinterpret_cast<f32x4*>(part + h * 16) = v;
         continue;
       }
@@ -605,26 +626,31 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
 }
 
 // Joins the parts of a split product, in their order.
-__global__ __launch_bounds__(256) void parts_kernel(Out o, int splits, const Meta* __restrict__ meta, int64_t first, int64_t chunk,
-                                                    int by_rows, const unsigned* __restrict__ top_b) {
-  const int rows = rows_here(meta, first, chunk);
-  const int64_t limit = by_rows ? rows : o.rows;
-  const int64_t quads = (o.cols + 3) / 4;
-  const float alpha = meta->alpha;
+__global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
+  const Out& o = s.out;
+  const int rows = rows_here(s.meta, s.first, s.chunk);
+  const int tiles_m = s.tiles_m < 0 ? (rows + kTile - 1) / kTile : s.tiles_m;
+  const int steps = s.steps < 0 ? (rows + kStep - 1) / kStep : s.steps;
+  const int splits = splits_for(static_cast<int64_t>(tiles_m) * s.tiles_n, static_cast<int64_t>(steps) * s.rounds, s.most_parts);
+  if (splits == 1) return;
+  const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
+  const int64_t quads = (o.cols + 3) / 4, ld = static_cast<int64_t>(s.tiles_n) * kTile, size = ld * tiles_m * kTile;
+  const float alpha = s.meta->alpha;
   const bool vec = o.cols % 4 == 0;
+  const int shift = s.top_b != nullptr ? -shift_of(*s.top_b) : 0;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < limit * quads; q += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t row = q / quads, col = (q - row * quads) * 4;
-    const float* p = o.parts + row * o.part_ld + col;
+    const float* p = o.parts + row * ld + col;
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
-    for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * o.part_size);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * size);
     v *= alpha;
-    if (top_b != nullptr) {
-      const int shift = -shift_of(*top_b);
+    if (s.top_b != nullptr) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], shift);
     }
     const int64_t left = o.cols - col;
-    put4(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
+    put4(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
   }
 }
 
@@ -656,26 +682,10 @@ struct Plan {
   bool fp32, copy_weight, grads;
   int64_t rows, width, words, chunk, chunks, padded;  // width: of x and w; words: of G
   int planes;
-  int splits_x, splits_w;
-  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, total;
+  int64_t grid_x, grid_w;    // workgroups of the gradients, and the tiles of the parts they may be split into
+  int64_t parts_x, parts_w;
+  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, sum_w, total;
 };
-
-// How many parts to split a product of `tiles` tiles and `steps` steps into: a workgroup takes a step in 0.9 us (256 CUs
-// take one tile each), and a part costs its write and read at 4 TB/s.
-int splits_for(int64_t tiles, int64_t steps, double part_bytes) {
-  const int cus = num_cus();
-  int best = 1;
-  double least = 1e30;
-  for (int s = 1; s <= 64 && s <= steps; ++s) {
-    const double rounds = static_cast<double>((tiles * s + cus - 1) / cus);
-    const double t = rounds * static_cast<double>((steps + s - 1) / s) * 0.9e-6 + (s > 1 ? 3e-6 + s * part_bytes * 2 / 4e12 : 0.0);
-    if (t < least * 0.97) {
-      least = t;
-      best = s;
-    }
-  }
-  return best;
-}
 
 Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_t ldw, int dtype, bool want_dx, bool want_dw,
               int64_t chunk_rows) {
@@ -713,17 +723,32 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.w = take(p.copy_weight ? vocab * p.width * 2 * p.planes : 0);
   p.sums = take(p.words / kTile * p.padded * sizeof(f32x2));
   p.e = take(p.grads ? p.chunk * p.words * 2 * p.planes : 0);
-  const int64_t pairs = p.fp32 ? 3 : 1, cols = up(hidden, kTile);
+  const int64_t rounds = p.fp32 ? 3 : 1, cols = up(hidden, kTile);
   const int64_t tiles_h = cols / kTile, tiles_v = p.words / kTile, tiles_r = p.chunk / kTile;
-  p.splits_x = want_dx ? splits_for(tiles_r * tiles_h, p.words / kStep * pairs, 4.0 * p.chunk * cols) : 1;
-  p.splits_w = want_dw && p.chunks == 1 ? splits_for(tiles_v * tiles_h, p.chunk / kStep * pairs, 4.0 * p.words * cols) : 1;
-  if (p.splits_x > p.words / kStep) p.splits_x = static_cast<int>(p.words / kStep);
-  if (p.splits_w > p.chunk / kStep) p.splits_w = static_cast<int>(p.chunk / kStep);
-  size_t parts = p.splits_x > 1 ? static_cast<size_t>(p.splits_x) * p.chunk * cols * 4 : 0;
-  const size_t parts_w = want_dw && (p.splits_w > 1 || p.chunks > 1) ? static_cast<size_t>(p.splits_w) * p.words * cols * 4 : 0;
-  // the parts of dx are joined before dw begins, but a sum over chunks stays
-  const size_t kept = p.chunks > 1 ? parts_w : 0;
-  p.parts = take((kept > 0 ? 0 : (parts > parts_w ? parts : parts_w)) + kept + (kept > 0 ? parts : 0));
+  // the kept rows are known on the device alone: as many workgroups and parts as any number of them takes
+  if (want_dx) {
+    p.grid_x = tiles_r * tiles_h;
+    for (int64_t t = 1; t <= tiles_r && t * tiles_h * 2 <= kMostParts; ++t) {
+      const int64_t tiles = t * tiles_h, parts = tiles * splits_for(tiles, p.words / kStep * rounds, kMostParts);
+      if (parts > p.grid_x) p.grid_x = parts;
+      if (parts > tiles && parts > p.parts_x) p.parts_x = parts;
+    }
+  }
+  if (want_dw) {
+    const int64_t tiles = tiles_v * tiles_h;
+    p.grid_w = tiles;
+    for (int64_t t = 1; p.chunks == 1 && t <= p.chunk / kStep && tiles * 2 <= kMostParts; ++t) {
+      // beyond 1024 steps the host does not look at each number
+      const int64_t parts = t > 1024 ? kMostParts / tiles * tiles : tiles * splits_for(tiles, t * rounds, kMostParts);
+      if (parts > tiles && parts > p.parts_w) p.parts_w = parts;
+      if (t > 1024) break;
+    }
+    if (p.parts_w > p.grid_w) p.grid_w = p.parts_w;
+  }
+  // the parts of dx are joined before dw begins, but a sum of dw over chunks stays
+  const size_t tile_bytes = static_cast<size_t>(kTile) * kTile * 4;
+  p.sum_w = p.chunks > 1 && want_dw ? tiles_v * tiles_h * tile_bytes : 0;
+  p.parts = take(p.sum_w + (p.parts_x > p.parts_w ? p.parts_x : p.parts_w) * tile_bytes);
   p.total = at;
   return p;
 }
@@ -745,7 +770,6 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   float* z = reinterpret_cast<float*>(ws + p.z);
   float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
   f32x2* sums = reinterpret_cast<f32x2*>(ws + p.sums);
-  float* parts = reinterpret_cast<float*>(ws + p.parts);
   P* x = reinterpret_cast<P*>(ws + p.x);
   float* losses = reduction == PT_REDUCTION_NONE ? loss : nullptr;
 
@@ -804,24 +828,21 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>((p.words / 8 + 255) / 256), static_cast<unsigned>(p.chunk < 16384 ? p.chunk : 16384)),
                        dim3(256), 0, st, e, p.chunk * p.words, p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
     const Operand og{e, p.words, p.chunk * p.words, p.chunk * p.words * 2};
-    const int64_t cols = up(hidden, kTile);
+    const int rounds = p.fp32 ? 3 : 1;
+    float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);
     if (dx != nullptr) {
-      Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), p.splits_x, top_w, {}};
-      // a sum of dw over chunks stays behind the parts
-      d.out = Out{dx, grad_dtype, p.splits_x > 1 ? kPart : kFinal, p.chunk, hidden, row_of, parts, cols, p.chunk * cols};
-      hipLaunchKernelGGL((gradient_kernel<T, false>), grid(static_cast<int64_t>(tiles_r) * tiles_h * p.splits_x), dim3(512), lds, st, d);
-      if (p.splits_x > 1)
-        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_x, meta, first, p.chunk, 1, top_w);
+      Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), rounds, p.parts_x, top_w, {}};
+      d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
+      hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
+      if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, dim3(2048), dim3(256), 0, st, d);
     }
     if (dw != nullptr) {
       const Operand oxc{x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2};
-      Gradient d{og, oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, p.splits_w, top_x, {}};
-      float* own = p.chunks > 1 && p.splits_x > 1 ? parts + static_cast<int64_t>(p.splits_x) * p.chunk * cols : parts;
-      const int how = p.chunks > 1 ? (c + 1 == p.chunks ? kAddFinal : kAdd) : (p.splits_w > 1 ? kPart : kFinal);
-      d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, own, cols, p.words * cols};
-      hipLaunchKernelGGL((gradient_kernel<T, true>), grid(static_cast<int64_t>(tiles_v) * tiles_h * p.splits_w), dim3(512), lds, st, d);
-      if (how == kPart)
-        hipLaunchKernelGGL(parts_kernel, dim3(1024), dim3(256), 0, st, d.out, p.splits_w, meta, first, p.chunk, 0, top_x);
+      const int how = p.chunks == 1 ? kFinal : (c + 1 == p.chunks ? kAddFinal : kAdd);
+      Gradient d{og, oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, rounds, p.parts_w, top_x, {}};
+      d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts)};
+      hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
+      if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel, dim3(2048), dim3(256), 0, st, d);
     }
     if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
   }
