@@ -221,6 +221,9 @@ _LAUNCHERS = {
     "pt_cross_entropy_shifted": "cross_entropy",
     "pt_cross_entropy_scale_grad": "cross_entropy_scale_grad",
     "pt_cross_entropy_shifted_scale_grad": "cross_entropy_scale_grad",
+    "pt_swiglu8_fwd": "swiglu8_node",
+    "pt_rmsnorm8_fwd": "rmsnorm8_node",
+    "pt_linear_cross_entropy": "linear_cross_entropy_node",
 }
 _NATIVE_PASSES = ("ENTRY_POINTS", "adamw8_scan", "adamw8_table", "adamw_scan", "advance_steps", "bind", "ce_grad_buffer")
 

@@ -8,10 +8,16 @@
 // that does not match), untouched, so that the general route in ops.py copies, converts or raises
 // as it always did.  A nonzero code of the library comes back as an int, for _lib.call to raise.
 //
+// Three operators come as nodes of the autograd graph too (the functions that end in _node): a training pass through SwiGLU or
+// RMSNorm with 8-bit checkpoints, or through the head's cross-entropy, then runs no Python between the call and its
+// gradients ([32, 64] fp32 SwiGLU, forward and gradients: 94 us through Python functions).  A node's backward runs on
+// the stream of its forward, as the engine runs every node.
+//
 // Entry points come in by address (bind), from the library that _lib loaded.  Nothing is kept
 // between calls.  Allocations and the library call run without the GIL, as they do through torch and
 // ctypes.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
@@ -35,7 +41,9 @@ namespace {
   X(pt_cross_entropy_shifted) X(pt_cross_entropy_scale_grad)                                  \
   X(pt_cross_entropy_shifted_scale_grad) X(pt_rope_at)                                        \
   X(pt_sequence_log_probs_workspace_bytes) X(pt_sequence_log_probs) X(pt_preference_loss)     \
-  X(pt_sequence_log_probs_bwd)
+  X(pt_sequence_log_probs_bwd) X(pt_last_error) X(pt_swiglu8_fwd) X(pt_swiglu8_bwd)           \
+  X(pt_rmsnorm8_fwd) X(pt_rmsnorm8_bwd_workspace_bytes) X(pt_rmsnorm8_bwd)                    \
+  X(pt_linear_cross_entropy_workspace_bytes) X(pt_linear_cross_entropy) X(pt_scale_gradient)
 #define PT_DECLARE(f) decltype(&f) p_##f = nullptr;
 PT_NATIVE_FNS(PT_DECLARE)
 #undef PT_DECLARE
@@ -867,6 +875,239 @@ PT_FN(advance_steps, 1)
   return none();
 PT_END
 
+// ------------------------------------------------------------------ nodes of the autograd graph
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr const char* kNoSecondDerivative =
+    "the backward of an operator that keeps its inputs in 8 bits has no derivative of its own (create_graph=True); "
+    "use it without checkpoint_8bit";
+
+void checked(const char* fn, int rc) { TORCH_CHECK(rc == PT_OK, fn, " failed (code ", rc, "): ", p_pt_last_error()); }
+
+// A gradient as the kernels read it.
+at::Tensor as_dense(const at::Tensor& t, at::ScalarType type) { return t.to(type).contiguous(); }
+
+at::Tensor bytes_like(const at::Tensor& t, size_t n) {
+  return at::empty({static_cast<int64_t>(n < 16 ? 16 : n)}, t.options().dtype(at::kByte));
+}
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+struct Swiglu8 : torch::autograd::Function<Swiglu8> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& g, const at::Tensor& u, int64_t stream) {
+    at::Tensor o = at::empty(g.sizes(), g.options());
+    at::Tensor codes = at::empty({blocks_of(g.numel()), 16, 2, 8}, g.options().dtype(at::kByte));
+    at::Tensor steps = at::empty({blocks_of(g.numel()), 2}, g.options().dtype(at::kFloat));
+    checked("pt_swiglu8_fwd", p_pt_swiglu8_fwd(in(g), in(u), out(o), out(codes), static_cast<float*>(out(steps)), g.numel(), code_of(g),
+                                               reinterpret_cast<void*>(stream)));
+    ctx->save_for_backward({codes, steps});
+    ctx->saved_data["stream"] = stream;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), kNoSecondDerivative);
+    const variable_list kept = ctx->get_saved_variables();
+    const at::Tensor d = grads[0].contiguous();
+    at::Tensor dg, du;
+    if (ctx->needs_input_grad(0)) dg = at::empty(d.sizes(), d.options());
+    if (ctx->needs_input_grad(1)) du = at::empty(d.sizes(), d.options());
+    checked("pt_swiglu8_bwd", p_pt_swiglu8_bwd(in(d), in(kept[0]), static_cast<const float*>(in(kept[1])), dg.defined() ? out(dg) : nullptr,
+                                               du.defined() ? out(du) : nullptr, d.numel(), code_of(d),
+                                               reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())));
+    return {dg, du, at::Tensor()};
+  }
+};
+
+// (gate, up, stream) -> out
+PT_FN(swiglu8_node, 3)
+  const at::Tensor *g = plain(a[0]), *u = plain(a[1]);
+  if (g == nullptr || !g->is_contiguous() || code_of(*g) < 0 || !twin(u, *g)) return none();
+  const int64_t stream = reinterpret_cast<int64_t>(as_stream(a[2]));
+  NoGil nogil;
+  const at::Tensor o = Swiglu8::apply(*g, *u, stream);
+  nogil.end();
+  return wrap(o);
+PT_END
+
+// y, or h and y with a residual.
+struct Norm8 : torch::autograd::Function<Norm8> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& res, const at::Tensor& w,
+                               double eps, int64_t stream) {
+    const int64_t cols = x.size(-1), rows = x.numel() / cols, blocks = blocks_of(cols);
+    at::Tensor h, y = at::empty(x.sizes(), x.options()), rstd = empty_rstd(x);
+    if (res) h = at::empty(x.sizes(), x.options());
+    at::Tensor codes = at::empty({rows, blocks, 128}, x.options().dtype(at::kByte));
+    at::Tensor steps = at::empty({rows, blocks}, x.options().dtype(at::kFloat));
+    checked("pt_rmsnorm8_fwd",
+            p_pt_rmsnorm8_fwd(in(x), res ? in(*res) : nullptr, in(w), res ? out(h) : nullptr, out(y),
+                              static_cast<float*>(out(rstd)), out(codes), static_cast<float*>(out(steps)), rows, cols,
+                              static_cast<float>(eps), code_of(x), code_of(w), reinterpret_cast<void*>(stream)));
+    ctx->save_for_backward({w, rstd, codes, steps});
+    ctx->saved_data["stream"] = stream;
+    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+    ctx->set_materialize_grads(false);
+    if (h.defined()) return {h, y};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), kNoSecondDerivative);
+    const at::Tensor dh = grads.size() == 2 ? grads[0] : at::Tensor();
+    // counted over the inputs that are tensors
+    const bool add = grads.size() == 2, need_x = ctx->needs_input_grad(0), need_r = add && ctx->needs_input_grad(1);
+    const bool need_w = ctx->needs_input_grad(add ? 2 : 1);
+    at::Tensor dx = dh, dw;
+    if (grads.back().defined()) {
+      const variable_list kept = ctx->get_saved_variables();
+      const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+      const at::Tensor &w = kept[0], dy = as_dense(grads.back(), type);
+      at::Tensor extra, ws;
+      if (dh.defined()) extra = as_dense(dh, type);
+      const int64_t cols = w.numel(), rows = dy.numel() / cols;
+      dx = need_x || need_r ? at::empty(dy.sizes(), dy.options()) : at::Tensor();
+      size_t bytes = 0;
+      if (need_w) {
+        dw = at::empty({cols}, w.options());
+        bytes = p_pt_rmsnorm8_bwd_workspace_bytes(rows, cols);
+        ws = bytes_like(dy, bytes);
+      }
+      checked("pt_rmsnorm8_bwd",
+              p_pt_rmsnorm8_bwd(in(dy), extra.defined() ? in(extra) : nullptr, in(w), static_cast<const float*>(in(kept[1])), in(kept[2]),
+                                static_cast<const float*>(in(kept[3])), dx.defined() ? out(dx) : nullptr, need_w ? out(dw) : nullptr,
+                                need_w ? out(ws) : nullptr, bytes, rows, cols, code_of(dy), code_of(w),
+                                reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())));
+    }
+    return {need_x ? dx : at::Tensor(), need_r ? dx : at::Tensor(), dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+// (x, residual or None, weight, eps, stream) -> y, or (h, y)
+PT_FN(rmsnorm8_node, 5)
+  const at::Tensor *x = plain(a[0]), *w = plain(a[2]);
+  const at::Tensor* res = a[1] == Py_None ? nullptr : plain(a[1]);
+  Rows r;
+  double eps;
+  if (!norm_rows(x, w, &r) || (a[1] != Py_None && !twin(res, *x)) || !as_f64(a[3], &eps)) return none();
+  const int64_t stream = reinterpret_cast<int64_t>(as_stream(a[4]));
+  NoGil nogil;
+  const variable_list o = Norm8::apply(*x, res != nullptr ? std::optional<at::Tensor>(*res) : std::nullopt, *w, eps, stream);
+  nogil.end();
+  return o.size() == 1 ? wrap(o[0]) : tuple(o[0], o[1]);
+PT_END
+
+// The head's cross-entropy: what a call says beside its tensors.
+struct HeadCall {
+  bool shift;
+  int64_t ignore, reduction, chunk, stream;
+};
+
+struct HeadOut {
+  at::Tensor loss, dx, dw;
+};
+
+HeadOut head_call(const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const HeadCall& c, bool want_loss, bool want_dx, bool want_dw,
+                  const at::Tensor& grad, at::ScalarType type) {
+  const bool deep = x.dim() == 3;
+  const int64_t outer = deep ? x.size(0) : 1, seq = deep ? x.size(1) : x.size(0), inner = c.shift ? seq - 1 : seq;
+  const int64_t tso = deep ? t.stride(0) : 0, tsi = t.stride(t.dim() - 1);
+  HeadOut o;
+  if (want_loss) {
+    const auto options = x.options().dtype(at::kFloat);
+    if (c.reduction != PT_REDUCTION_NONE) o.loss = at::empty({}, options);
+    else o.loss = deep ? at::empty({outer, inner}, options) : at::empty({inner}, options);
+  }
+  if (want_dx) o.dx = at::empty(x.sizes(), x.options().dtype(type));
+  if (want_dw) o.dw = at::empty(w.sizes(), w.options().dtype(type));
+  const int64_t vocab = w.size(0), hidden = w.size(1);
+  const size_t bytes = p_pt_linear_cross_entropy_workspace_bytes(outer * inner, vocab, hidden, in(w), w.stride(0), code_of(x), want_dx, want_dw, c.chunk);
+  const at::Tensor ws = bytes_like(x, bytes);
+  checked("pt_linear_cross_entropy",
+          p_pt_linear_cross_entropy(
+              in(x), deep ? x.stride(0) : 0, x.stride(x.dim() - 2), outer, inner, in(w), w.stride(0), vocab, hidden,
+              static_cast<const int64_t*>(in(t)) + (c.shift ? tsi : 0), tso, tsi, c.ignore, static_cast<int>(c.reduction),
+              want_loss ? static_cast<float*>(out(o.loss)) : nullptr, grad.defined() ? static_cast<const float*>(in(grad)) : nullptr,
+              grad.defined() && deep ? grad.stride(0) : 0, grad.defined() ? grad.stride(grad.dim() - 1) : 0, want_dx ? out(o.dx) : nullptr, seq,
+              want_dw ? out(o.dw) : nullptr, type == at::kFloat ? PT_FLOAT32 : code_of(x), out(ws), static_cast<size_t>(ws.numel()), c.chunk, code_of(x),
+              reinterpret_cast<void*>(c.stream)));
+  return o;
+}
+
+struct HeadLoss : torch::autograd::Function<HeadLoss> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const HeadCall& c) {
+    // fp16 gradients stay in fp32 until a loss scale arrives
+    const at::ScalarType type = x.scalar_type() == at::kHalf ? at::kFloat : x.scalar_type();
+    const HeadOut o = head_call(x, w, t, c, true, x.requires_grad(), w.requires_grad(), at::Tensor(), type);
+    if (o.dx.defined()) ctx->saved_data["dx"] = o.dx;
+    if (o.dw.defined()) ctx->saved_data["dw"] = o.dw;
+    ctx->saved_data["stream"] = c.stream;
+    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+    return o.loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the fused head's cross-entropy is differentiable once (create_graph=True)");
+    auto& kept = ctx->saved_data;
+    TORCH_CHECK(kept.count("dx") + kept.count("dw") > 0,
+                "the gradients of the fused head's cross-entropy were handed out by an earlier backward through this graph "
+                "(retain_graph=True); backpropagate through the loss once, or use reduction='none'");
+    const auto type = static_cast<at::ScalarType>(kept["type"].toInt());
+    void* const stream = reinterpret_cast<void*>(kept["stream"].toInt());
+    const at::Tensor scale = as_dense(grads[0], at::kFloat);
+    auto take = [&](const char* name) {
+      if (kept.count(name) == 0) return at::Tensor();
+      const at::Tensor from = kept[name].toTensor();
+      kept.erase(name);
+      const at::Tensor to = from.scalar_type() == type ? from : at::empty(from.sizes(), from.options().dtype(type));
+      checked("pt_scale_gradient", p_pt_scale_gradient(in(from), code_of(from), out(to), code_of(to), from.numel(),
+                                                       static_cast<const float*>(in(scale)), stream));
+      return to;
+    };
+    const at::Tensor dx = take("dx"), dw = take("dw");
+    return {dx, dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+struct HeadTokens : torch::autograd::Function<HeadTokens> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const HeadCall& c) {
+    ctx->save_for_backward({x, w, t});
+    auto& kept = ctx->saved_data;
+    kept["shift"] = c.shift;
+    kept["ignore"] = c.ignore;
+    kept["chunk"] = c.chunk;
+    kept["stream"] = c.stream;
+    return head_call(x, w, t, c, true, false, false, at::Tensor(), x.scalar_type()).loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the fused head's cross-entropy is differentiable once (create_graph=True)");
+    const variable_list saved = ctx->get_saved_variables();
+    auto& kept = ctx->saved_data;
+    const HeadCall c{kept["shift"].toBool(), kept["ignore"].toInt(), PT_REDUCTION_NONE, kept["chunk"].toInt(), kept["stream"].toInt()};
+    const at::Tensor grad = grads[0].to(at::kFloat);
+    const HeadOut o = head_call(saved[0], saved[1], saved[2], c, false, ctx->needs_input_grad(0), ctx->needs_input_grad(1), grad, saved[0].scalar_type());
+    return {o.dx, o.dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+// (hidden, weight, labels, shift, ignore_index, reduction, chunk_tokens, graph, stream) -> loss, in the graph or without one
+PT_FN(linear_cross_entropy_node, 9)
+  const at::Tensor *x = plain(a[0]), *w = plain(a[1]), *t = plain(a[2]);
+  HeadCall c;
+  c.shift = a[3] == Py_True;
+  if (x == nullptr || w == nullptr || t == nullptr || code_of(*x) < 0 || x->scalar_type() != w->scalar_type() || t->scalar_type() != at::kLong ||
+      !same_place(*x, *w) || !same_place(*x, *t) || (x->dim() != 2 && x->dim() != 3) || w->dim() != 2 || w->size(1) != x->size(-1) ||
+      x->stride(-1) != 1 || w->stride(1) != 1 || w->stride(0) < w->size(1) || t->sizes() != x->sizes().slice(0, x->dim() - 1) ||
+      (c.shift && (x->dim() != 3 || x->size(1) < 2)) || !as_i64(a[4], &c.ignore) || !as_i64(a[5], &c.reduction) || !as_i64(a[6], &c.chunk))
+    return none();
+  c.stream = reinterpret_cast<int64_t>(as_stream(a[8]));
+  const bool graph = a[7] == Py_True;
+  NoGil nogil;
+  const at::Tensor o = !graph ? head_call(*x, *w, *t, c, true, false, false, at::Tensor(), x->scalar_type()).loss
+                       : c.reduction == PT_REDUCTION_NONE ? HeadTokens::apply(*x, *w, *t, c)
+                                                          : HeadLoss::apply(*x, *w, *t, c);
+  nogil.end();
+  return wrap(o);
+PT_END
+
 // ------------------------------------------------------------------ module
 
 // bind(name, address): the address of an entry point of the loaded library.
@@ -904,6 +1145,9 @@ PyMethodDef methods[] = {PT_METHOD(rmsnorm_fwd),
                          PT_METHOD(adamw8_table),
                          PT_METHOD(adamw8_scan),
                          PT_METHOD(advance_steps),
+                         PT_METHOD(swiglu8_node),
+                         PT_METHOD(rmsnorm8_node),
+                         PT_METHOD(linear_cross_entropy_node),
                          PT_METHOD(bind),
                          {nullptr, nullptr, 0, nullptr}};
 

@@ -65,6 +65,14 @@ def no_graph(*tensors: Tensor) -> bool:
             and not torch.compiler.is_compiling())
 
 
+def native_graph() -> bool:
+    """True when a node that native code adds to the autograd graph does what an autograd Function would: nothing looks at
+    the call as more than a node (see :func:`no_graph`)."""
+
+    return (_CAN_SKIP_FUNCTION and forward_ad._current_level < 0 and _tracing_state() is None and not _functorch_active()
+            and not torch.compiler.is_compiling())
+
+
 def require_hip(exc: type[RuntimeError], op: str, *tensors: Tensor) -> None:
     reason = _process_reason()
     if reason:

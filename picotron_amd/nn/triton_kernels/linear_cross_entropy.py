@@ -27,7 +27,7 @@ from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from picotron_amd import ops
-from picotron_amd.nn.triton_kernels._gate import no_graph, require_hip
+from picotron_amd.nn.triton_kernels._gate import native_graph, no_graph, require_hip
 from picotron_amd.nn.triton_kernels.cross_entropy import IGNORE_INDEX, TritonCrossEntropyUnavailable, _check_targets
 
 
@@ -122,7 +122,13 @@ def triton_linear_cross_entropy(
     except TritonCrossEntropyUnavailable as error:
         raise TritonLinearCrossEntropyUnavailable(str(error)) from error
     how = dict(shift=bool(shift), ignore_index=int(ignore_index), reduction=reduction, chunk_tokens=chunk_tokens or 0)
-    if no_graph(hidden, weight):
+    plain = no_graph(hidden, weight)
+    if plain or native_graph():
+        loss = ops._launch_here("pt_linear_cross_entropy", hidden, weight, labels, how["shift"], how["ignore_index"],
+                                ops.REDUCTIONS[reduction], how["chunk_tokens"], not plain)
+        if loss is not None:
+            return loss
+    if plain:
         return ops.linear_cross_entropy(hidden, weight, labels, **how)[0]
     return (_TokenLosses if reduction == "none" else _ReducedLoss).apply(hidden, weight, labels, how)
 

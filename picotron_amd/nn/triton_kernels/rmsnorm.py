@@ -30,7 +30,7 @@ from torch import Tensor
 
 from picotron_amd import _lib, ops
 from picotron_amd.nn.triton_kernels import _block8
-from picotron_amd.nn.triton_kernels._gate import no_graph, require_hip
+from picotron_amd.nn.triton_kernels._gate import native_graph, no_graph, require_hip
 
 
 class TritonRMSNormUnavailable(RuntimeError):
@@ -193,7 +193,8 @@ def triton_rms_norm(hidden_states: Tensor, weight: Tensor, eps: float, *, checkp
     if no_graph(hidden_states, weight):
         return ops.rmsnorm_fwd(hidden_states, weight, eps)[0]
     if checkpoint_8bit:
-        return _RMSNorm8Function.apply(hidden_states, None, weight, eps, True)
+        out = ops._launch_here("pt_rmsnorm8_fwd", hidden_states, None, weight, eps) if native_graph() else None
+        return _RMSNorm8Function.apply(hidden_states, None, weight, eps, True) if out is None else out
     return _RMSNormAutogradFunction.apply(hidden_states, weight, eps, True)
 
 
@@ -256,7 +257,8 @@ def triton_residual_rms_norm(
     if no_graph(hidden_states, residual, weight):
         return ops.residual_rmsnorm_fwd(hidden_states, residual, weight, eps)[:2]
     if checkpoint_8bit:
-        return _RMSNorm8Function.apply(hidden_states, residual, weight, eps, True)
+        out = ops._launch_here("pt_rmsnorm8_fwd", hidden_states, residual, weight, eps) if native_graph() else None
+        return _RMSNorm8Function.apply(hidden_states, residual, weight, eps, True) if out is None else out
     return _ResidualRMSNormFunction.apply(hidden_states, residual, weight, eps)
 
 

@@ -20,7 +20,7 @@ from torch.nn import functional as F
 
 from picotron_amd import ops
 from picotron_amd.nn.triton_kernels import _block8
-from picotron_amd.nn.triton_kernels._gate import no_graph, require_hip
+from picotron_amd.nn.triton_kernels._gate import native_graph, no_graph, require_hip
 
 
 class TritonSwiGLUUnavailable(RuntimeError):
@@ -113,7 +113,10 @@ def triton_swiglu(gate: Tensor, up: Tensor, *, checkpoint_8bit: bool = False) ->
     _validate_triton_inputs(gate, up)
     if no_graph(gate, up):
         return ops.swiglu_fwd(gate, up)
-    return (_SwiGLU8Function if checkpoint_8bit else _SwiGLUAutogradFunction).apply(gate, up, True)
+    if checkpoint_8bit:
+        out = ops._launch_here("pt_swiglu8_fwd", gate, up) if native_graph() else None
+        return _SwiGLU8Function.apply(gate, up, True) if out is None else out
+    return _SwiGLUAutogradFunction.apply(gate, up, True)
 
 
 def swiglu_with_pytorch_forward(gate: Tensor, up: Tensor, *, checkpoint_8bit: bool = False) -> Tensor:

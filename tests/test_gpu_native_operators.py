@@ -9,7 +9,15 @@ import torch
 from gpu_util import randn
 from picotron_amd import _lib, ops
 from picotron_amd.nn import RotaryFrequencies
-from picotron_amd.nn.triton_kernels import adamw, triton_adamw_step, triton_clip_grad_norm_and_step
+from picotron_amd.nn.triton_kernels import (
+    adamw,
+    triton_adamw_step,
+    triton_clip_grad_norm_and_step,
+    triton_linear_cross_entropy,
+    triton_residual_rms_norm,
+    triton_rms_norm,
+    triton_swiglu,
+)
 from picotron_amd.optim import AdamW8bit
 from test_gpu_native import DTYPES, _both
 
@@ -200,3 +208,90 @@ def test_8bit_scan_leaves_the_unusual_to_the_plan(gpu):
     version = state["step"]._version
     triton_adamw_step(opt)
     assert state["step"]._version > version
+
+
+def _by_python(monkeypatch, call):
+    """``call`` with the nodes that native code adds to the graph, and through the Python functions: the same bits."""
+
+    out = [call()]
+    with monkeypatch.context() as m:
+        for entry in ("pt_swiglu8_fwd", "pt_rmsnorm8_fwd", "pt_linear_cross_entropy"):
+            m.setitem(_lib._launchers, entry, lambda *a: None)
+        out.append(call())
+    for a, b in zip(*out):
+        assert (a is None) == (b is None) and (a is None or (a.dtype == b.dtype and torch.equal(a, b)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_swiglu8_node(gpu, monkeypatch, dtype):
+    d = randn((5, 300), dtype, gpu, 3)
+    for needs in ((True, True), (True, False), (False, True)):
+        for grad in (d, d[:, :1].expand(5, 300), randn((300, 5), dtype, gpu, 4).t()):
+            def call():
+                g, u = (randn((5, 300), dtype, gpu, k).requires_grad_(n) for k, n in zip((1, 2), needs))
+                y = triton_swiglu(g, u, checkpoint_8bit=True)
+                return [y.detach(), *torch.autograd.grad(y, [t for t in (g, u) if t.requires_grad], grad)]
+
+            _by_python(monkeypatch, call)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm8_node(gpu, monkeypatch, dtype, residual):
+    d, dh = randn((5, 300), dtype, gpu, 3), randn((5, 300), dtype, gpu, 4)
+    for needs in ((True, True, True), (True, False, False), (False, True, True), (False, False, True)):
+        for grads in ([dh, d], [dh, None], [None, d], [dh[:, :1].expand(5, 300), d[:1].expand(5, 300)]):
+            def call():
+                x, r, w = (randn(s, dtype, gpu, k).requires_grad_(n) for k, s, n in zip((1, 2, 5), ((5, 300), (5, 300), (300,)), needs))
+                if residual:
+                    outs = list(triton_residual_rms_norm(x, r, w, 1e-5, checkpoint_8bit=True))
+                    inputs, gs = [x, r, w], grads
+                else:
+                    outs = [triton_rms_norm(x, w, 1e-5, checkpoint_8bit=True)]
+                    inputs, gs = [x, w], grads[1:]
+                inputs = [t for t in inputs if t.requires_grad]
+                used = [(o, g) for o, g in zip(outs, gs) if g is not None and o.requires_grad]
+                if not used or not inputs:
+                    return [o.detach() for o in outs]
+                got = torch.autograd.grad([o for o, _ in used], inputs, [g for _, g in used], allow_unused=True)
+                return [*(o.detach() for o in outs), *got]
+
+            _by_python(monkeypatch, call)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_linear_cross_entropy_node(gpu, monkeypatch, dtype, reduction):
+    t = torch.randint(0, 90, (3, 20), device=gpu, generator=torch.Generator(device=gpu).manual_seed(0))
+    t[0, 4:9] = -100
+    for needs in ((True, True), (True, False), (False, True)):
+        for shift in (False, True):
+            def call():
+                x, w = (randn(s, dtype, gpu, k, 0.3).requires_grad_(n) for k, s, n in zip((1, 2), ((3, 20, 64), (90, 64)), needs))
+                loss = triton_linear_cross_entropy(x, w, t, shift=shift, reduction=reduction, chunk_tokens=30)
+                grad = randn(loss.shape, torch.float32, gpu, 7)
+                got = torch.autograd.grad(loss, [p for p in (x, w) if p.requires_grad], grad)
+                with torch.no_grad():
+                    plain = triton_linear_cross_entropy(x, w, t, shift=shift, reduction=reduction, chunk_tokens=30)
+                return [loss.detach(), plain, *got]
+
+            _by_python(monkeypatch, call)
+
+
+def test_nodes_raise_what_the_functions_raise(gpu, monkeypatch):
+    x = randn((4, 64), torch.float32, gpu, 1).requires_grad_()
+    w, t = randn((9, 64), torch.float32, gpu, 2), torch.arange(4, device=gpu)
+    for route in range(2):
+        with monkeypatch.context() as m:
+            if route:
+                for entry in ("pt_swiglu8_fwd", "pt_rmsnorm8_fwd", "pt_linear_cross_entropy"):
+                    m.setitem(_lib._launchers, entry, lambda *a: None)
+            for y in (triton_swiglu(x, x, checkpoint_8bit=True), triton_rms_norm(x, w[0].clone(), 1e-5, checkpoint_8bit=True)):
+                with pytest.raises(RuntimeError, match="checkpoint_8bit"):
+                    torch.autograd.grad(y.sum(), x, create_graph=True)
+            loss = triton_linear_cross_entropy(x, w, t)
+            torch.autograd.grad(loss, x, retain_graph=True)
+            with pytest.raises(RuntimeError, match="handed out"):
+                torch.autograd.grad(loss, x)
+            with torch.inference_mode():
+                triton_linear_cross_entropy(x, w, t)
