@@ -16,10 +16,12 @@
 //   too (fp16 keeps softmax values down to 2^-28 normal), and the scale is taken out of the fp32 sums.
 // - With 32-bit inputs every operand is two fp16 planes (see kLow), and a product is three of 16-bit operands: 5 times the
 //   rate that the fp32 matrix instructions have at their peak.
+// - Models of up to 128 elements go another way, without exp(l - m) in memory (narrow_head.hpp).
 // - Tokens are taken in chunks, so that G takes at most 2 GiB; with more than one, dw is summed in fp32 over them.
 // - The gradients are formed in the forward call, where G is at hand; the backward only multiplies them by what arrives
 //   from above.  fp16's stay in fp32 until then, as a loss scale arrives only there.
 //   Where each token has its own weight (no reduction), the backward forms G itself, with one product more.
+#include "narrow_head.hpp"
 #include "tile_product.hpp"
 
 namespace pt {
@@ -391,16 +393,18 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
 }
 
 // z of each row from its tiles' sums, and the row's loss.  32 rows a workgroup, 32 threads a row, in a fixed order.
-__global__ __launch_bounds__(1024) void join_kernel(const f32x2* __restrict__ sums, int64_t padded, int tiles,
+__device__ __forceinline__ void join_rows(const f32x2* __restrict__ sums, int64_t padded, int tiles,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
                                                     const int* __restrict__ row_of, const int* __restrict__ label_of,
                                                     const float* __restrict__ target, float* __restrict__ z,
                                                     float* __restrict__ row_loss, float* __restrict__ losses, int64_t inner,
-                                                    int64_t dx_inner) {
+                                                    int64_t dx_inner, float* __restrict__ exponent) {
   __shared__ float tops[32][33], parts[32][33];
   const int rows = rows_here(meta, first, chunk);
   const int c = threadIdx.x % 32, part = threadIdx.x / 32;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + c;
+  if (exponent != nullptr && part == 0 && row >= rows && row < (rows + kNarrowOuter - 1) / kNarrowOuter * kNarrowOuter)
+    exponent[row] = -INFINITY;  // rows that fill up a tile
   if (static_cast<int64_t>(blockIdx.x) * 32 >= rows) return;
   float top = -INFINITY, sum = 0.f;
   if (row < rows) {
@@ -424,10 +428,30 @@ __global__ __launch_bounds__(1024) void join_kernel(const f32x2* __restrict__ su
   const float loss = label_of[first + row] < 0 ? NAN : lse - target[first + row];
   z[first + row] = lse;
   row_loss[first + row] = loss;
+  // the softmax times kScale is exp2(l * log2(e) + exponent); a label outside the vocabulary leaves a NaN, as its loss
+  if (exponent != nullptr) exponent[row] = label_of[row] < 0 ? NAN : 14.f - lse * 1.44269504088896340736f;
   if (losses != nullptr) {
     const int64_t d = row_of[first + row], o = d / dx_inner;
     losses[o * inner + (d - o * dx_inner)] = loss;
   }
+}
+
+__global__ __launch_bounds__(1024) void join_kernel(const f32x2* __restrict__ sums, int64_t padded, int tiles, const Meta* __restrict__ meta,
+                                                    int64_t first, int64_t chunk, const int* __restrict__ row_of,
+                                                    const int* __restrict__ label_of, const float* __restrict__ target,
+                                                    float* __restrict__ z, float* __restrict__ row_loss, float* __restrict__ losses,
+                                                    int64_t inner, int64_t dx_inner) {
+  join_rows(sums, padded, tiles, meta, first, chunk, row_of, label_of, target, z, row_loss, losses, inner, dx_inner, nullptr);
+}
+
+__global__ __launch_bounds__(1024) void narrow_join_kernel(const f32x2* __restrict__ sums, int64_t vocab, const Meta* __restrict__ meta, const int* __restrict__ row_of,
+                                                           const int* __restrict__ label_of, const float* __restrict__ target,
+                                                           float* __restrict__ z, float* __restrict__ row_loss, float* __restrict__ losses,
+                                                           int64_t inner, int64_t dx_inner, float* __restrict__ exponent) {
+  const int64_t rows = meta->count;
+  const int64_t tiles = (rows + kNarrowOuter - 1) / kNarrowOuter;
+  const int splits = narrow_splits(tiles, (vocab + kNarrowInner - 1) / kNarrowInner);
+  join_rows(sums, tiles * kNarrowOuter, splits, meta, 0, rows, row_of, label_of, target, z, row_loss, losses, inner, dx_inner, exponent);
 }
 
 // The sum (or mean) of the kept rows' losses, one workgroup, in a fixed order and 64 bits.
@@ -625,6 +649,246 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   }
 }
 
+// ------------------------------------------------------------------ narrow models
+
+struct Narrow {
+  Operand outer, inner;
+  const Meta* meta;
+  const int* label_of;
+  const float* weight_of;  // or null
+  int64_t vocab;
+  f32x2* sums;  // (splits, outer tiles * 256)
+  float* target;
+  const float* exponent;
+  const float* z;
+  Out out;
+};
+
+template <typename T, int HP, int PASS>
+__device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
+  typedef NarrowTile<HP> Step;
+  constexpr int KK = HP / 32, HF = HP / 16, OF = 4;
+  constexpr float kLog2e = 1.44269504088896340736f;
+  const int rows = s.meta->count;
+  const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows, inner_rows = PASS == kNarrowDw ? rows : s.vocab;
+  const int outer_tiles = static_cast<int>((outer_rows + kNarrowOuter - 1) / kNarrowOuter);
+  const int steps = static_cast<int>((inner_rows + kNarrowInner - 1) / kNarrowInner);
+  const int splits = narrow_splits(outer_tiles, steps);
+  const int tile = blockIdx.x / splits, split = blockIdx.x % splits;
+  if (tile >= outer_tiles) return;
+  const int each = (steps + splits - 1) / splits, from = split * each, to = from + each < steps ? from + each : steps;
+
+  const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16, wave = threadIdx.x / 64;
+  const int64_t o0 = static_cast<int64_t>(tile) * kNarrowOuter + wave * 64;  // the wave's first outer row
+  s16x8 outer[OF][KK];
+  {
+    const int64_t left = s.outer.bytes - static_cast<int64_t>(tile) * kNarrowOuter * s.outer.ld * 2;
+    const __amdgpu_buffer_rsrc_t r =
+        uniform_buffer(static_cast<const char*>(s.outer.p) + static_cast<int64_t>(tile) * kNarrowOuter * s.outer.ld * 2,
+                       left > 0x7ffffff0 ? 0x7ffffff0 : static_cast<int>(left));
+#pragma unroll
+    for (int f = 0; f < OF; ++f)
+#pragma unroll
+      for (int k = 0; k < KK; ++k)
+        outer[f][k] = __builtin_bit_cast(s16x8, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    r, static_cast<int>((wave * 64 + f * 16 + i) * s.outer.ld * 2) + k * 64 + g * 16, 0, 0));
+  }
+  f32x4 acc[OF][HF];
+  float top[OF], sum[OF], add[OF], at_label[OF];
+  int label[OF];
+#pragma unroll
+  for (int f = 0; f < OF; ++f) {
+#pragma unroll
+    for (int h = 0; h < HF; ++h) acc[f][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t o = o0 + f * 16 + i;
+    top[f] = -INFINITY;
+    sum[f] = 0.f;
+    label[f] = PASS != kNarrowDw && o < rows ? s.label_of[o] : -1;
+    if constexpr (PASS == kNarrowDx) {
+      add[f] = s.exponent[o];
+      at_label[f] = o < rows ? expm1f(s.target[o] - s.z[o]) * kScale : 0.f;
+    }
+  }
+
+  Step step;
+  step.init(s.inner.ld);
+  f32x4 adds[4];  // of the step's tokens: a lane's quads of four fragments
+  if (from < to) step.load(lds + (from & 1) * Step::kBytes, s.inner, static_cast<int64_t>(from) * kNarrowInner);
+  for (int t = from; t < to; ++t) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < to) step.load(lds + ((t + 1) & 1) * Step::kBytes, s.inner, static_cast<int64_t>(t + 1) * kNarrowInner);
+    const lds_char* p = lds + (t & 1) * Step::kBytes;
+    const int64_t first = static_cast<int64_t>(t) * kNarrowInner;
+    const bool whole = PASS == kNarrowDw || first + kNarrowInner <= s.vocab;
+    if constexpr (PASS == kNarrowDw) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) adds[b] = *reinterpret_cast<const f32x4*>(s.exponent + first + b * 16 + 4 * g);
+    }
+#pragma unroll
+    for (int pair = 0; pair < 2; ++pair) {
+      f32x4 l[2][OF];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int row = pair * 32 + b * 16 + i;
+#pragma unroll
+        for (int f = 0; f < OF; ++f) l[b][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KK; ++k) {
+          const s16x8 in = Step::row(p, row, k * 4 + g);
+#pragma unroll
+          for (int f = 0; f < OF; ++f) l[b][f] = mfma16<T>(in, outer[f][k], l[b][f]);
+        }
+      }
+      const int64_t base = first + pair * 32 + 4 * g;  // of the lane's quads: base + 16 b + k
+      if (!whole) {  // words that are none
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int f = 0; f < OF; ++f)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (base + b * 16 + k >= s.vocab) l[b][f][k] = -INFINITY;
+      }
+      if constexpr (PASS == kNarrowSums) {
+#pragma unroll
+        for (int f = 0; f < OF; ++f) {
+          float most = top[f];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = fmaxf(most, l[b][f][k]);
+          const float level = most == -INFINITY ? 0.f : most;
+          sum[f] *= __builtin_amdgcn_exp2f((top[f] - level) * kLog2e);
+          top[f] = most;
+          const float start = -level * kLog2e;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, start));
+          const int64_t place = label[f] - base;
+          if (place >= 0 && place < 20 && (place & 15) < 4) {
+            float v = 0.f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v = place == b * 16 + k ? l[b][f][k] : v;
+            s.target[o0 + f * 16 + i] = v;
+          }
+        }
+      } else {
+        s16x8 grad[OF];
+#pragma unroll
+        for (int f = 0; f < OF; ++f) {
+          float e[8];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float start = PASS == kNarrowDw ? adds[pair * 2 + b][k] : add[f];
+              e[b * 4 + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, start));
+            }
+          if constexpr (PASS == kNarrowDx) {
+            const int64_t place = label[f] - base;
+            if (place >= 0 && place < 20 && (place & 15) < 4) {
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[b * 4 + k] = place == b * 16 + k ? at_label[f] : e[b * 4 + k];
+            }
+          }
+          Vec16<T> v;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v.e[k] = static_cast<T>(e[k]);
+          grad[f] = __builtin_bit_cast(s16x8, v.raw);
+        }
+        if constexpr (PASS == kNarrowDw) {
+          // labels among the wave's words, and the tokens' own weights
+          const int64_t token = first + pair * 32 + lane % 32;
+          const int64_t word = (token < rows ? s.label_of[token] : -1) - o0;
+          if (s.weight_of != nullptr || __any(word >= 0 && word < 64)) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int64_t at = base + b * 16 + k;
+                const bool in = at < rows;
+                const int64_t w = in ? s.label_of[at] - o0 : -1;
+                const float d = in && w >= 0 && w < 64 ? expm1f(s.target[at] - s.z[at]) * kScale : 0.f;
+                const float c = in && s.weight_of != nullptr ? s.weight_of[at] * s.meta->inv_weight : 1.f;
+#pragma unroll
+                for (int f = 0; f < OF; ++f) {
+                  float e = __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, adds[pair * 2 + b][k]));
+                  if (w == f * 16 + i) e = d;
+                  grad[f][b * 4 + k] = __builtin_bit_cast(short, static_cast<T>(e * c));
+                }
+              }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < HF; ++h) {
+          const s16x8 in = Step::columns(p, pair * 32 + 4 * g + i / 4, h * 2 + ((i & 3) >> 1), i & 1);
+#pragma unroll
+          for (int f = 0; f < OF; ++f) acc[f][h] = mfma16<T>(in, grad[f], acc[f][h]);
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int f = 0; f < OF; ++f) {
+    const int64_t o = o0 + f * 16 + i;
+    if constexpr (PASS == kNarrowSums) {
+      float most = fmaxf(top[f], __shfl_xor(top[f], 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      float all = top[f] == -INFINITY ? sum[f] : sum[f] * __builtin_amdgcn_exp2f((top[f] - most) * kLog2e);
+      all += __shfl_xor(all, 16);
+      all += __shfl_xor(all, 32);
+      if (g == 0 && o < rows) s.sums[static_cast<int64_t>(split) * outer_tiles * kNarrowOuter + o] = f32x2{most, all};
+    } else if (o < outer_rows) {
+      const float alpha = s.meta->alpha * (PASS == kNarrowDx && s.weight_of != nullptr ? s.weight_of[o] * s.meta->inv_weight : 1.f);
+      const int64_t to_row = s.out.row_of != nullptr ? s.out.row_of[o] : o;
+#pragma unroll
+      for (int h = 0; h < HF; ++h) {
+        const int col = h * 16 + 4 * g;
+        const f32x4 v = acc[f][h] * alpha;
+        if (splits > 1) {
+          *reinterpret_cast<f32x4*>(s.out.parts + ((static_cast<int64_t>(split) * outer_tiles * kNarrowOuter + o) * HP + col)) = v;
+        } else {
+          const int64_t left = s.out.cols - col;
+          if (left > 0) put4(s.out.p, s.out.dtype, to_row * s.out.cols + col, v, left < 4 ? static_cast<int>(left) : 4, s.out.cols % 4 == 0);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int HP, int PASS>
+__global__ __launch_bounds__(256) void narrow_kernel(Narrow s) {
+  __shared__ __attribute__((aligned(16))) char raw[2 * NarrowTile<HP>::kBytes];
+  narrow_pass<T, HP, PASS>(s, (lds_char*)raw);
+}
+
+// Joins the parts of a narrow gradient, in their order.
+template <int HP, int PASS>
+__global__ __launch_bounds__(256) void narrow_parts_kernel(Narrow s) {
+  const int rows = s.meta->count;
+  const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows, inner_rows = PASS == kNarrowDw ? rows : s.vocab;
+  const int64_t outer_tiles = (outer_rows + kNarrowOuter - 1) / kNarrowOuter;
+  const int splits = narrow_splits(outer_tiles, (inner_rows + kNarrowInner - 1) / kNarrowInner);
+  if (splits == 1) return;
+  const int64_t size = outer_tiles * kNarrowOuter * HP;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < outer_rows * (HP / 4); q += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t o = q / (HP / 4), col = (q % (HP / 4)) * 4, left = s.out.cols - col;
+    if (left <= 0) continue;
+    const float* p = s.out.parts + o * HP + col;
+    f32x4 v = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 8
+    for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * size);
+    put4(s.out.p, s.out.dtype, (s.out.row_of != nullptr ? s.out.row_of[o] : o) * s.out.cols + col, v, left < 4 ? static_cast<int>(left) : 4,
+         s.out.cols % 4 == 0);
+  }
+}
+
 // Joins the parts of a split product, in their order.
 __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
   const Out& o = s.out;
@@ -679,12 +943,12 @@ __global__ __launch_bounds__(256) void rescale_kernel(const S* __restrict__ from
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 struct Plan {
-  bool fp32, copy_weight, grads;
+  bool fp32, copy_weight, grads, narrow;
   int64_t rows, width, words, chunk, chunks, padded;  // width: of x and w; words: of G
   int planes;
   int64_t grid_x, grid_w;    // workgroups of the gradients, and the tiles of the parts they may be split into
   int64_t parts_x, parts_w;
-  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, sum_w, total;
+  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, sum_w, exponent, total;
 };
 
 Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_t ldw, int dtype, bool want_dx, bool want_dw,
@@ -696,16 +960,17 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.rows = rows;
   p.width = up(hidden, kStep);
   p.words = up(vocab, kTile);
+  p.narrow = !p.fp32 && p.width <= 128;
   p.copy_weight = p.fp32 || hidden % kStep != 0 || ldw % 8 != 0 || !aligned16(w);
   const int64_t each = p.grads ? 2 * p.planes * p.words : 0;
-  int64_t most = p.grads ? kChunkBytes / each / kTile * kTile : kScoreRows;
+  const int64_t all = up(rows > 0 ? rows : 1, kTile);
+  int64_t most = p.narrow ? all : p.grads ? kChunkBytes / each / kTile * kTile : kScoreRows;
   if (most < kTile) most = kTile;
-  if (chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
+  if (!p.narrow && chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
   p.chunks = rows > 0 ? (rows + most - 1) / most : 1;
   p.chunk = up((rows + p.chunks - 1) / p.chunks, kTile);
   if (p.chunk < kTile) p.chunk = kTile;
   p.padded = p.chunk;
-  const int64_t all = up(rows > 0 ? rows : 1, kTile);
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -721,6 +986,18 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.row_loss = take(all * 4);
   p.x = take(all * p.width * 2 * p.planes);
   p.w = take(p.copy_weight ? vocab * p.width * 2 * p.planes : 0);
+  if (p.narrow) {
+    const int64_t tiles_x = all / kNarrowOuter, tiles_w = up(vocab, kNarrowOuter) / kNarrowOuter, least = kNarrowGroups;
+    p.exponent = take(all * 4);
+    // a tile fewer may be split more often, but all parts together are at most the workgroups wanted, or one a tile
+    p.grid_x = tiles_x > least ? tiles_x : least;
+    p.grid_w = tiles_w > least ? tiles_w : least;
+    p.sums = take(static_cast<size_t>(p.grid_x) * kNarrowOuter * sizeof(f32x2));
+    const int64_t parts = want_dw && p.grid_w > p.grid_x ? p.grid_w : p.grid_x;
+    p.parts = take(p.grads ? static_cast<size_t>(parts) * kNarrowOuter * p.width * 4 : 0);
+    p.total = at;
+    return p;
+  }
   p.sums = take(p.words / kTile * p.padded * sizeof(f32x2));
   p.e = take(p.grads ? p.chunk * p.words * 2 * p.planes : 0);
   const int64_t rounds = p.fp32 ? 3 : 1, cols = up(hidden, kTile);
@@ -756,6 +1033,36 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
 template <typename K>
 int allow(K kernel, size_t bytes) {
   return allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+}
+
+template <typename T, int HP>
+int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t vocab, int64_t hidden, const Plan& p, char* ws, const int* row_of,
+               const float* weight_of, float* losses, void* dx, void* dw, int grad_dtype, hipStream_t st) {
+  const Meta* meta = reinterpret_cast<const Meta*>(ws + p.meta);
+  const int* label_of = reinterpret_cast<const int*>(ws + p.label_of);
+  float* target = reinterpret_cast<float*>(ws + p.target);
+  float* z = reinterpret_cast<float*>(ws + p.z);
+  float* exponent = reinterpret_cast<float*>(ws + p.exponent);
+  f32x2* sums = reinterpret_cast<f32x2*>(ws + p.sums);
+  float* parts = reinterpret_cast<float*>(ws + p.parts);
+  Narrow s{ox, ow, meta, label_of, weight_of, vocab, sums, target, exponent, z, {}};
+  const dim3 grid_x(static_cast<unsigned>(p.grid_x)), grid_w(static_cast<unsigned>(p.grid_w));
+  hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowSums>), grid_x, dim3(256), 0, st, s);
+  hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, vocab, meta, row_of, label_of,
+                     target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent);
+  if (dx != nullptr) {
+    s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
+    hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDx>), grid_x, dim3(256), 0, st, s);
+    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDx>), dim3(1024), dim3(256), 0, st, s);
+  }
+  if (dw != nullptr) {
+    s.outer = ow;
+    s.inner = ox;
+    s.out = Out{dw, grad_dtype, kFinal, vocab, hidden, nullptr, parts};
+    hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDw>), grid_w, dim3(256), 0, st, s);
+    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDw>), dim3(1024), dim3(256), 0, st, s);
+  }
+  return check_launch("pt_linear_cross_entropy");
 }
 
 template <typename T>  // of the inputs
@@ -807,6 +1114,16 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   const unsigned* top_x = p.fp32 ? &meta->top_x : nullptr;
   const unsigned* top_w = p.fp32 ? &meta->top_w : nullptr;
   const Operand ox{x, p.width, all * p.width, all * p.width * 2};
+  if constexpr (!Split<T>::kSplit) {
+    if (p.narrow) {
+      const int rc = p.width == 64 ? run_narrow<T, 64>(r, ox, ow, vocab, hidden, p, ws, row_of, weight_of, losses, dx, dw, grad_dtype, st)
+                                   : run_narrow<T, 128>(r, ox, ow, vocab, hidden, p, ws, row_of, weight_of, losses, dx, dw, grad_dtype, st);
+      if (rc != PT_OK) return rc;
+      if (loss != nullptr && reduction != PT_REDUCTION_NONE)
+        hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, meta, reduction == PT_REDUCTION_MEAN ? 1 : 0, loss);
+      return check_launch("pt_linear_cross_entropy");
+    }
+  }
   const int tiles_v = static_cast<int>(p.words / kTile), tiles_h = static_cast<int>(up(hidden, kTile) / kTile);
   const int tiles_r = static_cast<int>(p.chunk / kTile);
   constexpr size_t lds = Product<T, false, false>::kLds;

@@ -19,6 +19,7 @@ instead, at the cost of a host sync).  Under autocast the inputs are cast as ``F
 
 from __future__ import annotations
 
+import os
 import warnings
 
 import torch
@@ -28,7 +29,7 @@ from torch.nn import functional as F
 
 from picotron_amd import ops
 from picotron_amd.nn.triton_kernels._gate import native_graph, no_graph, require_hip
-from picotron_amd.nn.triton_kernels.cross_entropy import IGNORE_INDEX, TritonCrossEntropyUnavailable, _check_targets
+from picotron_amd.nn.triton_kernels.cross_entropy import _CHECK_ENV, IGNORE_INDEX, TritonCrossEntropyUnavailable, _check_targets
 
 
 class TritonLinearCrossEntropyUnavailable(RuntimeError):
@@ -85,6 +86,10 @@ def _check_options(reduction: str, chunk_tokens: int | None) -> None:
         raise ValueError("chunk_tokens must be a positive integer or None.")
 
 
+def _checks_targets() -> bool:
+    return os.environ.get(_CHECK_ENV, "") not in ("", "0")
+
+
 def _autocast(*tensors: Tensor) -> tuple[Tensor, ...]:
     """As F.linear under autocast casts its inputs."""
 
@@ -94,7 +99,6 @@ def _autocast(*tensors: Tensor) -> tuple[Tensor, ...]:
     return tuple(t.to(dtype) if t.is_floating_point() and t.is_cuda and t.dtype != torch.float64 else t for t in tensors)
 
 
-@torch.compiler.disable
 def triton_linear_cross_entropy(
     hidden: Tensor, weight: Tensor, labels: Tensor, *, shift: bool = False, ignore_index: int = IGNORE_INDEX,
     reduction: str = "mean", chunk_tokens: int | None = None,
@@ -108,11 +112,25 @@ def triton_linear_cross_entropy(
     time, and so the memory of the call: about ``2 * vocab`` bytes a token in 16 bits, ``4 * vocab`` in fp32, 2 GiB at
     most in any case.  Differentiable once in ``hidden`` and ``weight``."""
 
+    if torch.compiler.is_compiling():  # runs between a compiled model's graphs
+        return _outside_graphs(hidden, weight, labels, shift, ignore_index, reduction, chunk_tokens)
+    return _linear_cross_entropy(hidden, weight, labels, shift, ignore_index, reduction, chunk_tokens)
+
+
+def _linear_cross_entropy(
+    hidden: Tensor, weight: Tensor, labels: Tensor, shift: bool, ignore_index: int, reduction: str, chunk_tokens: int | None
+) -> Tensor:
     _check_options(reduction, chunk_tokens)
     require_hip(TritonLinearCrossEntropyUnavailable, "linear cross-entropy", hidden, weight, labels)
+    hidden, weight = _autocast(hidden, weight)
+    plain = no_graph(hidden, weight)
+    if (plain or native_graph()) and not _checks_targets():  # what the native code takes needs no check here
+        loss = ops._launch_here("pt_linear_cross_entropy", hidden, weight, labels, bool(shift), ignore_index,
+                                ops.REDUCTIONS[reduction], chunk_tokens or 0, not plain)
+        if loss is not None:
+            return loss
     if weight.device != hidden.device or labels.device != hidden.device:
         raise TritonLinearCrossEntropyUnavailable("HIP linear cross-entropy needs its inputs on one device.")
-    hidden, weight = _autocast(hidden, weight)
     try:
         ops.head_rows(hidden, weight, labels, shift)
     except ValueError as error:
@@ -122,15 +140,12 @@ def triton_linear_cross_entropy(
     except TritonCrossEntropyUnavailable as error:
         raise TritonLinearCrossEntropyUnavailable(str(error)) from error
     how = dict(shift=bool(shift), ignore_index=int(ignore_index), reduction=reduction, chunk_tokens=chunk_tokens or 0)
-    plain = no_graph(hidden, weight)
-    if plain or native_graph():
-        loss = ops._launch_here("pt_linear_cross_entropy", hidden, weight, labels, how["shift"], how["ignore_index"],
-                                ops.REDUCTIONS[reduction], how["chunk_tokens"], not plain)
-        if loss is not None:
-            return loss
     if plain:
         return ops.linear_cross_entropy(hidden, weight, labels, **how)[0]
     return (_TokenLosses if reduction == "none" else _ReducedLoss).apply(hidden, weight, labels, how)
+
+
+_outside_graphs = torch.compiler.disable(_linear_cross_entropy)
 
 
 def linear_cross_entropy_with_pytorch(

@@ -189,12 +189,16 @@ def triton_rms_norm(hidden_states: Tensor, weight: Tensor, eps: float, *, checkp
     when the GPU requirements are unmet (reference rmsnorm.py:152-160).
     """
 
+    if checkpoint_8bit and not no_graph(hidden_states, weight) and native_graph():
+        require_hip(TritonRMSNormUnavailable, "RMSNorm", hidden_states, weight)
+        out = ops._launch_here("pt_rmsnorm8_fwd", hidden_states, None, weight, eps)  # what it takes needs no check here
+        if out is not None:
+            return out
     _validate_triton_inputs(hidden_states, weight)
     if no_graph(hidden_states, weight):
         return ops.rmsnorm_fwd(hidden_states, weight, eps)[0]
     if checkpoint_8bit:
-        out = ops._launch_here("pt_rmsnorm8_fwd", hidden_states, None, weight, eps) if native_graph() else None
-        return _RMSNorm8Function.apply(hidden_states, None, weight, eps, True) if out is None else out
+        return _RMSNorm8Function.apply(hidden_states, None, weight, eps, True)
     return _RMSNormAutogradFunction.apply(hidden_states, weight, eps, True)
 
 
@@ -248,6 +252,11 @@ def triton_residual_rms_norm(
     add and normalise with PyTorch).
     """
 
+    if checkpoint_8bit and not no_graph(hidden_states, residual, weight) and native_graph():
+        require_hip(TritonRMSNormUnavailable, "RMSNorm", hidden_states, residual, weight)
+        out = ops._launch_here("pt_rmsnorm8_fwd", hidden_states, residual, weight, eps)
+        if out is not None:
+            return out
     _validate_triton_inputs(hidden_states, weight)
     require_hip(TritonRMSNormUnavailable, "RMSNorm", residual)
     if residual.shape != hidden_states.shape or residual.dtype != hidden_states.dtype:
@@ -257,8 +266,7 @@ def triton_residual_rms_norm(
     if no_graph(hidden_states, residual, weight):
         return ops.residual_rmsnorm_fwd(hidden_states, residual, weight, eps)[:2]
     if checkpoint_8bit:
-        out = ops._launch_here("pt_rmsnorm8_fwd", hidden_states, residual, weight, eps) if native_graph() else None
-        return _RMSNorm8Function.apply(hidden_states, residual, weight, eps, True) if out is None else out
+        return _RMSNorm8Function.apply(hidden_states, residual, weight, eps, True)
     return _ResidualRMSNormFunction.apply(hidden_states, residual, weight, eps)
 
 

@@ -110,13 +110,15 @@ def _validate_triton_inputs(gate: Tensor, up: Tensor) -> None:
 def triton_swiglu(gate: Tensor, up: Tensor, *, checkpoint_8bit: bool = False) -> Tensor:
     """Fused SwiGLU activation (HIP forward and backward).  ``checkpoint_8bit``: the backward reads gate and up from 8 bits."""
 
+    if checkpoint_8bit and not no_graph(gate, up) and native_graph():
+        require_hip(TritonSwiGLUUnavailable, "SwiGLU", gate, up)
+        out = ops._launch_here("pt_swiglu8_fwd", gate, up)  # what it takes needs no check here
+        if out is not None:
+            return out
     _validate_triton_inputs(gate, up)
     if no_graph(gate, up):
         return ops.swiglu_fwd(gate, up)
-    if checkpoint_8bit:
-        out = ops._launch_here("pt_swiglu8_fwd", gate, up) if native_graph() else None
-        return _SwiGLU8Function.apply(gate, up, True) if out is None else out
-    return _SwiGLUAutogradFunction.apply(gate, up, True)
+    return (_SwiGLU8Function if checkpoint_8bit else _SwiGLUAutogradFunction).apply(gate, up, True)
 
 
 def swiglu_with_pytorch_forward(gate: Tensor, up: Tensor, *, checkpoint_8bit: bool = False) -> Tensor:

@@ -75,7 +75,7 @@ def check(loss, dx, dw, x, w, t, factors, scale=1.0, reduction="none", ignore=-1
 
 
 SIZES = [(1, 1, 1), (1, 64, 260), (2, 20, 257), (33, 32, 64), (255, 64, 256), (256, 128, 255), (300, 100, 1000), (513, 200, 1027),
-         (1100, 72, 3001), (700, 520, 130)]
+         (1100, 72, 3001), (700, 520, 130), (5, 192, 64), (1030, 160, 2100), (70, 129, 70000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -165,8 +165,9 @@ def test_shift(gpu, dtype, reduction):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 @pytest.mark.parametrize("ignored", [0.0, 0.6])
-def test_chunks_of_tokens(gpu, dtype, reduction, ignored):
-    n, h, v = 1300, 72, 519
+@pytest.mark.parametrize("h", [72, 200])
+def test_chunks_of_tokens(gpu, dtype, reduction, ignored, h):
+    n, v = 1300, 519
     x, w, t = make(n, h, v, dtype, gpu, seed=8, ignored=ignored)
     factors = torch.randn(n, device=gpu, generator=torch.Generator(device=gpu).manual_seed(3))
     x.requires_grad_()
@@ -214,8 +215,9 @@ def test_layouts(gpu, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
-def test_nothing_kept(gpu, dtype, reduction):
-    x, w, _ = make(40, 64, 300, dtype, gpu)
+@pytest.mark.parametrize("h", [64, 192])
+def test_nothing_kept(gpu, dtype, reduction, h):
+    x, w, _ = make(40, h, 300, dtype, gpu)
     t = torch.full((40,), 7, device=gpu)
     x.requires_grad_()
     w.requires_grad_()
@@ -240,8 +242,9 @@ def test_no_tokens(gpu, shape, reduction):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_ignored_rows_may_hold_anything(gpu, dtype):
-    x, w, t = make(300, 64, 500, dtype, gpu, ignored=0.5)
+@pytest.mark.parametrize("h", [64, 192])
+def test_ignored_rows_may_hold_anything(gpu, dtype, h):
+    x, w, t = make(300, h, 500, dtype, gpu, ignored=0.5)
     dirty = torch.where((t == -100)[:, None], math.nan, x)
     dirty[(t == -100).nonzero()[0]] = math.inf
     out = []
@@ -255,8 +258,9 @@ def test_ignored_rows_may_hold_anything(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_not_finite(gpu, dtype):
-    x, w, t = make(300, 64, 500, dtype, gpu, ignored=0)
+@pytest.mark.parametrize("h", [64, 192])
+def test_not_finite(gpu, dtype, h):
+    x, w, t = make(300, h, 500, dtype, gpu, ignored=0)
     for bad in (math.nan, math.inf):
         y = x.clone()
         y[5, 3] = bad
@@ -274,10 +278,11 @@ def test_not_finite(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_far_logits(gpu, dtype):
+@pytest.mark.parametrize("h", [64, 128, 192])
+def test_far_logits(gpu, dtype, h):
     """Rows far apart in level (the tiles' largest differ by hundreds), and labels of nearly all the weight."""
 
-    x, w, t = make(64, 64, 1000, dtype, gpu, ignored=0, spread=1.0)
+    x, w, t = make(64, h, 1000, dtype, gpu, ignored=0, spread=1.0)
     w[:, 0] = torch.linspace(-30, 30, 1000, device=gpu).to(dtype)
     x[:, 0] = torch.linspace(-16, 16, 64, device=gpu).to(dtype)
     t[::2] = (x.double() @ w.double().t()).argmax(1)[::2]
@@ -305,8 +310,9 @@ def test_magnitudes_of_32_bits(gpu, power):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_one_side_alone(gpu, dtype):
-    x, w, t = make(90, 64, 300, dtype, gpu)
+@pytest.mark.parametrize("h", [64, 192])
+def test_one_side_alone(gpu, dtype, h):
+    x, w, t = make(90, h, 300, dtype, gpu)
     both = [x.clone().requires_grad_(), w.clone().requires_grad_()]
     dx, dw = torch.autograd.grad(triton_linear_cross_entropy(*both, t), both)
     a = x.clone().requires_grad_()
@@ -327,8 +333,9 @@ def test_gradients_are_handed_out_once(gpu):
     assert torch.equal(torch.autograd.grad(losses.sum(), x)[0], first)
 
 
-def test_runs_repeat_to_the_bit(gpu):
-    x, w, t = make(600, 192, 3000, torch.bfloat16, gpu)
+@pytest.mark.parametrize("h", [64, 192])
+def test_runs_repeat_to_the_bit(gpu, h):
+    x, w, t = make(600, h, 3000, torch.bfloat16, gpu)
     x.requires_grad_()
     w.requires_grad_()
     runs = []
@@ -367,9 +374,9 @@ def test_tied_weights_add_up(gpu):
     assert torch.all((got.double() - want).abs() <= (4 * 72 * 2.0**-24 * 150 + 2.0**-18) * want.abs().max())
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_captured(gpu, dtype):
-    x, w, t = make(300, 64, 700, dtype, gpu)
+@pytest.mark.parametrize("dtype,h", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 192)])
+def test_captured(gpu, dtype, h):
+    x, w, t = make(300, h, 700, dtype, gpu)
     x.requires_grad_()
     w.requires_grad_()
 
@@ -387,7 +394,7 @@ def test_captured(gpu, dtype):
     with torch.cuda.graph(graph):
         out = step()
     for seed in range(3):
-        y, v, s = make(300, 64, 700, dtype, gpu, seed=seed + 20, ignored=0.2 * seed)
+        y, v, s = make(300, h, 700, dtype, gpu, seed=seed + 20, ignored=0.2 * seed)
         with torch.no_grad():
             x.copy_(y)
             w.copy_(v)
