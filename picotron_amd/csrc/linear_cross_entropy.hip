@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void gather_kernel(Rows r, const int* __restri
       from = static_cast<const T*>(r.x) + o * r.xso + s * r.xsi;
     }
     typename Split<T>::plane* p = to + wave * width;
-    if constexpr (VEC) {  // 16-bit elements, H a multiple of 64
+    if constexpr (VEC) {  // 16-bit elements, rows of whole vectors
       const u32x4 zero = {0, 0, 0, 0};
       for (int64_t c = lane * 8; c < width; c += 512)
         *reinterpret_cast<u32x4*>(p + c) = from != nullptr ? *reinterpret_cast<const u32x4*>(from + c) : zero;
@@ -249,8 +249,12 @@ __global__ __launch_bounds__(256) void weight_kernel(const T* __restrict__ w, in
 
 // ------------------------------------------------------------------ the three products
 
-template <typename T, bool A_COLUMNS, bool B_COLUMNS>  // T of the inputs
-using Product = TileProduct<typename Split<T>::plane, Split<T>::kSplit, kTile, kTile, 2, 4, A_COLUMNS, B_COLUMNS>;
+template <typename T, bool A_COLUMNS, bool B_COLUMNS, int BM = kTile>  // T of the inputs
+using Product = TileProduct<typename Split<T>::plane, Split<T>::kSplit, BM, kTile, (BM < 128 ? 1 : BM / 128), 4, A_COLUMNS, B_COLUMNS>;
+
+// Calls with at most 64 rows take tiles of 64 tokens by 256 words, of which two run on a CU: what bounds them is the weight's
+// way from memory.  One token of 4096 at 128256 words: 247 us in tiles of 256.
+constexpr int kFewRows = 64;
 
 __device__ __forceinline__ int rows_here(const Meta* meta, int64_t first, int64_t chunk) {
   const int64_t n = meta->count - first;
@@ -270,15 +274,15 @@ struct Scores {
   float* target;     // the label's logit of each kept row
 };
 
-template <typename T>
-__global__ __launch_bounds__(512) void scores_kernel(Scores s) {
+template <typename T, int BM>
+__global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Scores s) {
   extern __shared__ char lds_raw[];
-  typedef Product<T, false, false> P;
+  typedef Product<T, false, false, BM> P;
   const int rows = rows_here(s.meta, s.first, s.chunk);
   int tm, tn;
-  if (!tile_of(blockIdx.x, (rows + kTile - 1) / kTile, s.tiles_n, 4, &tm, &tn)) return;
+  if (!tile_of(blockIdx.x, (rows + BM - 1) / BM, s.tiles_n, 4, &tm, &tn)) return;
   P p;
-  p.run((lds_char*)lds_raw, s.x, s.w, s.first + static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * kTile, 0,
+  p.run((lds_char*)lds_raw, s.x, s.w, s.first + static_cast<int64_t>(tm) * BM, static_cast<int64_t>(tn) * kTile, 0,
         s.steps);
 
   if constexpr (Split<T>::kSplit) {
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) p.sums[f][h][k] = ldexpf(p.sums[f][h][k], shift);
   }
-  float* red = reinterpret_cast<float*>(lds_raw);  // (4, 256): the waves' parts of a row
+  float* red = reinterpret_cast<float*>(lds_raw);  // (4, BM): the waves' parts of a row
   const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
   const int col = p.wn * P::TN + 16 * g;  // of the lane's 16 elements in the tile
   const int64_t left = s.vocab - static_cast<int64_t>(tn) * kTile;
@@ -307,7 +311,7 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     const int m = p.wm * P::TM + f * 16 + i;
-    const int row = tm * kTile + m;
+    const int row = tm * BM + m;
     float top = -INFINITY;
 #pragma unroll
     for (int h = 0; h < P::FN; ++h)
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
       for (int k = 0; k < 4; ++k) top = fmaxf(top, p.sums[f][h][k]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    if (g == 0) red[p.wn * kTile + m] = top;
+    if (g == 0) red[p.wn * BM + m] = top;
     const int label = (row < rows ? s.label_of[s.first + row] : -1) - tn * kTile - col;
     if (label >= 0 && label < 16) {
       float t = 0.f;
@@ -331,12 +335,12 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     const int m = p.wm * P::TM + f * 16 + i;
-    tops[f] = fmaxf(fmaxf(red[m], red[kTile + m]), fmaxf(red[2 * kTile + m], red[3 * kTile + m]));
+    tops[f] = fmaxf(fmaxf(red[m], red[BM + m]), fmaxf(red[2 * BM + m], red[3 * BM + m]));
   }
   __syncthreads();
   const int64_t width = static_cast<int64_t>(s.tiles_n) * kTile;
   _Float16* to = s.e == nullptr ? nullptr
-                                : s.e + (static_cast<int64_t>(tm) * kTile + p.wm * P::TM + i) * width + static_cast<int64_t>(tn) * kTile + col;
+                                : s.e + (static_cast<int64_t>(tm) * BM + p.wm * P::TM + i) * width + static_cast<int64_t>(tn) * kTile + col;
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     constexpr float kLog2e = 1.44269504088896340736f, kShift = 14.f;  // 2^14 is kScale
@@ -355,7 +359,7 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
       }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (g == 0) red[p.wn * kTile + p.wm * P::TM + f * 16 + i] = sum;
+    if (g == 0) red[p.wn * BM + p.wm * P::TM + f * 16 + i] = sum;
     if (to != nullptr) {
       Vec16<_Float16> v[2], low[2];
 #pragma unroll
@@ -379,14 +383,14 @@ __global__ __launch_bounds__(512) void scores_kernel(Scores s) {
   }
   __syncthreads();
   const int m = threadIdx.x;
-  if (m < kTile && tm * kTile + m < rows) {
-    const float sum = (red[m] + red[kTile + m]) + (red[2 * kTile + m] + red[3 * kTile + m]);
-    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * kTile + m)[1] = sum * (1.0f / kScale);
+  if (m < BM && tm * BM + m < rows) {
+    const float sum = (red[m] + red[BM + m]) + (red[2 * BM + m] + red[3 * BM + m]);
+    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * BM + m)[1] = sum * (1.0f / kScale);
   }
   if (p.wn == 0 && g == 0) {
 #pragma unroll
     for (int f = 0; f < P::FM; ++f) {
-      const int row = tm * kTile + p.wm * P::TM + f * 16 + i;
+      const int row = tm * BM + p.wm * P::TM + f * 16 + i;
       if (row < rows) reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + row)[0] = tops[f];
     }
   }
@@ -408,22 +412,48 @@ __device__ __forceinline__ void join_rows(const f32x2* __restrict__ sums, int64_
   if (static_cast<int64_t>(blockIdx.x) * 32 >= rows) return;
   float top = -INFINITY, sum = 0.f;
   if (row < rows) {
-#pragma unroll 4
-    for (int t = part; t < tiles; t += 32) {
-      const f32x2 v = sums[t * padded + row];
-      const float next = fmaxf(top, v[0]);
+    for (int t = part; t < tiles; t += 32 * 8) {
+      f32x2 v[8];  // eight tiles' loads at once
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = t + k * 32 < tiles ? sums[(t + k * 32) * padded + row] : f32x2{-INFINITY, 0.f};
+      float next = top;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) next = fmaxf(next, v[k][0]);
       // a tile without a finite logit has a sum of 0, or NaN
-      sum = next == -INFINITY ? sum + v[1] : sum * __expf(top - next) + v[1] * __expf(v[0] - next);
+      const float level = next == -INFINITY ? 0.f : next;
+      sum *= __expf(top - level);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += v[k][0] == -INFINITY ? v[k][1] : v[k][1] * __expf(v[k][0] - level);
       top = next;
     }
   }
   tops[part][c] = top;
   parts[part][c] = sum;
   __syncthreads();
+  // four threads a row join eight parts each, then one the four
+  if (part < 4) {
+    top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, tops[part * 8 + k][c]);
+    const float level = top == -INFINITY ? 0.f : top;
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float m = tops[part * 8 + k][c], v = parts[part * 8 + k][c];
+      sum += m == -INFINITY ? v : v * __expf(m - level);
+    }
+  }
+  __syncthreads();
+  if (part < 4) {
+    tops[part][c] = top;
+    parts[part][c] = sum;
+  }
+  __syncthreads();
   if (part != 0 || row >= rows) return;
-  for (int k = 1; k < 32; ++k) top = fmaxf(top, tops[k][c]);
+  top = fmaxf(fmaxf(tops[0][c], tops[1][c]), fmaxf(tops[2][c], tops[3][c]));
   sum = 0.f;
-  for (int k = 0; k < 32; ++k) sum += tops[k][c] == -INFINITY ? parts[k][c] : parts[k][c] * __expf(tops[k][c] - top);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sum += tops[k][c] == -INFINITY ? parts[k][c] : parts[k][c] * __expf(tops[k][c] - top);
   const float lse = top + logf(sum);
   const float loss = label_of[first + row] < 0 ? NAN : lse - target[first + row];
   z[first + row] = lse;
@@ -447,10 +477,10 @@ __global__ __launch_bounds__(1024) void join_kernel(const f32x2* __restrict__ su
 __global__ __launch_bounds__(1024) void narrow_join_kernel(const f32x2* __restrict__ sums, int64_t vocab, const Meta* __restrict__ meta, const int* __restrict__ row_of,
                                                            const int* __restrict__ label_of, const float* __restrict__ target,
                                                            float* __restrict__ z, float* __restrict__ row_loss, float* __restrict__ losses,
-                                                           int64_t inner, int64_t dx_inner, float* __restrict__ exponent) {
+                                                           int64_t inner, int64_t dx_inner, float* __restrict__ exponent, int hp) {
   const int64_t rows = meta->count;
   const int64_t tiles = (rows + kNarrowOuter - 1) / kNarrowOuter;
-  const int splits = narrow_splits(tiles, (vocab + kNarrowInner - 1) / kNarrowInner);
+  const int splits = narrow_splits(tiles, (vocab + kNarrowInner - 1) / kNarrowInner, hp);
   join_rows(sums, tiles * kNarrowOuter, splits, meta, 0, rows, row_of, label_of, target, z, row_loss, losses, inner, dx_inner, exponent);
 }
 
@@ -523,18 +553,21 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
   }
 }
 
-// How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each,
-// a workgroup a step in 1.9 us, and each tile of a part costs 0.13 us for its way to memory and back.  The number of
+// How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each, a
+// workgroup a step in 1 us while it is alone and in 1.9 beside 255 others, the join 8 us more, and each tile of a part 0.13 us for
+// its way to memory and back.  The number of
 // tiles follows from the number of kept rows, so this is decided on the device; `most` bounds the tiles of all parts (0: no
 // split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps, 1025 us in one part.
 constexpr int64_t kMostParts = 1024;
 __host__ __device__ inline int splits_for(int64_t tiles, int64_t steps, int64_t most) {
-  constexpr int kTry[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
+  constexpr int kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
   int best = 1;
-  int64_t least = (tiles + 255) / 256 * steps * 1900;
+  int64_t least = int64_t{1} << 62;
   for (int s : kTry) {
-    if (s > steps || s * tiles > most) break;
-    const int64_t t = (tiles * s + 255) / 256 * ((steps + s - 1) / s) * 1900 + 5000 + tiles * s * 130;
+    const int64_t groups = tiles * s;
+    if (s > 1 && (s > steps || groups > most)) break;
+    const int64_t step = 1000 + (groups < 256 ? groups : 256) * 900 / 256;
+    const int64_t t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 8000 + groups * 130 : 0);
     if (t < least) {
       least = t;
       best = s;
@@ -673,7 +706,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
   const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows, inner_rows = PASS == kNarrowDw ? rows : s.vocab;
   const int outer_tiles = static_cast<int>((outer_rows + kNarrowOuter - 1) / kNarrowOuter);
   const int steps = static_cast<int>((inner_rows + kNarrowInner - 1) / kNarrowInner);
-  const int splits = narrow_splits(outer_tiles, steps);
+  const int splits = narrow_splits(outer_tiles, steps, HP);
   const int tile = blockIdx.x / splits, split = blockIdx.x % splits;
   if (tile >= outer_tiles) return;
   const int each = (steps + splits - 1) / splits, from = split * each, to = from + each < steps ? from + each : steps;
@@ -712,18 +745,41 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
 
   Step step;
   step.init(s.inner.ld);
-  f32x4 adds[4];  // of the step's tokens: a lane's quads of four fragments
+  // of a step's tokens: a lane's quads of four fragments, and a label a lane; a step ahead, so that no product waits for them
+  f32x4 adds[4] = {}, next_adds[4];
+  int words = -1, next_words;
+  if constexpr (PASS == kNarrowDw) {
+    if (from < to) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) next_adds[b] = *reinterpret_cast<const f32x4*>(s.exponent + from * kNarrowInner + b * 16 + 4 * g);
+      const int token = from * kNarrowInner + lane;
+      next_words = token < rows ? s.label_of[token] : -1;
+    }
+  }
   if (from < to) step.load(lds + (from & 1) * Step::kBytes, s.inner, static_cast<int64_t>(from) * kNarrowInner);
   for (int t = from; t < to; ++t) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < to) step.load(lds + ((t + 1) & 1) * Step::kBytes, s.inner, static_cast<int64_t>(t + 1) * kNarrowInner);
-    const lds_char* p = lds + (t & 1) * Step::kBytes;
-    const int64_t first = static_cast<int64_t>(t) * kNarrowInner;
+    const int first = t * kNarrowInner;
     const bool whole = PASS == kNarrowDw || first + kNarrowInner <= s.vocab;
+    bool hit = false;  // a label of the wave's tokens among the step's words, or of the step's tokens among the wave's
     if constexpr (PASS == kNarrowDw) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) adds[b] = *reinterpret_cast<const f32x4*>(s.exponent + first + b * 16 + 4 * g);
+      for (int b = 0; b < 4; ++b) adds[b] = next_adds[b];
+      words = next_words;
+      hit = static_cast<unsigned>(words - static_cast<int>(o0)) < 64u;
+      if (t + 1 < to) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) next_adds[b] = *reinterpret_cast<const f32x4*>(s.exponent + first + kNarrowInner + b * 16 + 4 * g);
+        const int token = first + kNarrowInner + lane;
+        next_words = token < rows ? s.label_of[token] : -1;
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < OF; ++f) hit = hit || static_cast<unsigned>(label[f] - first) < static_cast<unsigned>(kNarrowInner);
     }
+    hit = __any(hit);
+    if (t + 1 < to) step.load(lds + ((t + 1) & 1) * Step::kBytes, s.inner, static_cast<int64_t>(t + 1) * kNarrowInner);
+    const lds_char* p = lds + (t & 1) * Step::kBytes;
 #pragma unroll
     for (int pair = 0; pair < 2; ++pair) {
       f32x4 l[2][OF];
@@ -739,7 +795,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
           for (int f = 0; f < OF; ++f) l[b][f] = mfma16<T>(in, outer[f][k], l[b][f]);
         }
       }
-      const int64_t base = first + pair * 32 + 4 * g;  // of the lane's quads: base + 16 b + k
+      const int base = first + pair * 32 + 4 * g;  // of the lane's quads: base + 16 b + k
       if (!whole) {  // words that are none
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -765,8 +821,8 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int k = 0; k < 4; ++k) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, start));
-          const int64_t place = label[f] - base;
-          if (place >= 0 && place < 20 && (place & 15) < 4) {
+          const int place = label[f] - base;
+          if (hit && place >= 0 && place < 20 && (place & 15) < 4) {
             float v = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -788,8 +844,8 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
               e[b * 4 + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, start));
             }
           if constexpr (PASS == kNarrowDx) {
-            const int64_t place = label[f] - base;
-            if (place >= 0 && place < 20 && (place & 15) < 4) {
+            const int place = label[f] - base;
+            if (hit && place >= 0 && place < 20 && (place & 15) < 4) {
 #pragma unroll
               for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -802,17 +858,14 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
           grad[f] = __builtin_bit_cast(s16x8, v.raw);
         }
         if constexpr (PASS == kNarrowDw) {
-          // labels among the wave's words, and the tokens' own weights
-          const int64_t token = first + pair * 32 + lane % 32;
-          const int64_t word = (token < rows ? s.label_of[token] : -1) - o0;
-          if (s.weight_of != nullptr || __any(word >= 0 && word < 64)) {
+          if (hit || s.weight_of != nullptr) {  // the labels' own entries, and the tokens' own weights
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const int64_t at = base + b * 16 + k;
+                const int at = base + b * 16 + k;
                 const bool in = at < rows;
-                const int64_t w = in ? s.label_of[at] - o0 : -1;
+                const int w = in ? s.label_of[at] - static_cast<int>(o0) : -1;
                 const float d = in && w >= 0 && w < 64 ? expm1f(s.target[at] - s.z[at]) * kScale : 0.f;
                 const float c = in && s.weight_of != nullptr ? s.weight_of[at] * s.meta->inv_weight : 1.f;
 #pragma unroll
@@ -874,7 +927,7 @@ __global__ __launch_bounds__(256) void narrow_parts_kernel(Narrow s) {
   const int rows = s.meta->count;
   const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows, inner_rows = PASS == kNarrowDw ? rows : s.vocab;
   const int64_t outer_tiles = (outer_rows + kNarrowOuter - 1) / kNarrowOuter;
-  const int splits = narrow_splits(outer_tiles, (inner_rows + kNarrowInner - 1) / kNarrowInner);
+  const int splits = narrow_splits(outer_tiles, (inner_rows + kNarrowInner - 1) / kNarrowInner, HP);
   if (splits == 1) return;
   const int64_t size = outer_tiles * kNarrowOuter * HP;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < outer_rows * (HP / 4); q += static_cast<int64_t>(gridDim.x) * 256) {
@@ -958,10 +1011,10 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.grads = want_dx || want_dw;
   p.planes = p.fp32 ? 2 : 1;
   p.rows = rows;
-  p.width = up(hidden, kStep);
+  p.narrow = dtype != PT_FLOAT32 && hidden <= 128;
+  p.width = p.narrow && hidden <= 32 ? 32 : up(hidden, kStep);
   p.words = up(vocab, kTile);
-  p.narrow = !p.fp32 && p.width <= 128;
-  p.copy_weight = p.fp32 || hidden % kStep != 0 || ldw % 8 != 0 || !aligned16(w);
+  p.copy_weight = p.fp32 || hidden != p.width || ldw % 8 != 0 || !aligned16(w);
   const int64_t each = p.grads ? 2 * p.planes * p.words : 0;
   const int64_t all = up(rows > 0 ? rows : 1, kTile);
   int64_t most = p.narrow ? all : p.grads ? kChunkBytes / each / kTile * kTile : kScoreRows;
@@ -987,9 +1040,9 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.x = take(all * p.width * 2 * p.planes);
   p.w = take(p.copy_weight ? vocab * p.width * 2 * p.planes : 0);
   if (p.narrow) {
-    const int64_t tiles_x = all / kNarrowOuter, tiles_w = up(vocab, kNarrowOuter) / kNarrowOuter, least = kNarrowGroups;
+    const int64_t tiles_x = all / kNarrowOuter, tiles_w = up(vocab, kNarrowOuter) / kNarrowOuter, least = kNarrowParts;
     p.exponent = take(all * 4);
-    // a tile fewer may be split more often, but all parts together are at most the workgroups wanted, or one a tile
+    // fewer tiles may be split more often, but not into more parts in all, or one a tile
     p.grid_x = tiles_x > least ? tiles_x : least;
     p.grid_w = tiles_w > least ? tiles_w : least;
     p.sums = take(static_cast<size_t>(p.grid_x) * kNarrowOuter * sizeof(f32x2));
@@ -1035,6 +1088,12 @@ int allow(K kernel, size_t bytes) {
   return allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 }
 
+// Workgroups that join parts: a thread takes four elements, or several fours.
+dim3 join_grid(int64_t rows, int64_t cols) {
+  const int64_t blocks = (rows * ((cols + 3) / 4) + 255) / 256;
+  return dim3(static_cast<unsigned>(blocks < 1 ? 1 : (blocks < 2048 ? blocks : 2048)));
+}
+
 template <typename T, int HP>
 int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t vocab, int64_t hidden, const Plan& p, char* ws, const int* row_of,
                const float* weight_of, float* losses, void* dx, void* dw, int grad_dtype, hipStream_t st) {
@@ -1049,18 +1108,18 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
   const dim3 grid_x(static_cast<unsigned>(p.grid_x)), grid_w(static_cast<unsigned>(p.grid_w));
   hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowSums>), grid_x, dim3(256), 0, st, s);
   hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, vocab, meta, row_of, label_of,
-                     target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent);
+                     target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent, HP);
   if (dx != nullptr) {
     s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDx>), grid_x, dim3(256), 0, st, s);
-    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDx>), dim3(1024), dim3(256), 0, st, s);
+    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDx>), join_grid(p.rows, hidden), dim3(256), 0, st, s);
   }
   if (dw != nullptr) {
     s.outer = ow;
     s.inner = ox;
     s.out = Out{dw, grad_dtype, kFinal, vocab, hidden, nullptr, parts};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDw>), grid_w, dim3(256), 0, st, s);
-    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDw>), dim3(1024), dim3(256), 0, st, s);
+    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDw>), join_grid(vocab, hidden), dim3(256), 0, st, s);
   }
   return check_launch("pt_linear_cross_entropy");
 }
@@ -1093,7 +1152,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   const unsigned gather_grid = static_cast<unsigned>(waves > 0 ? (waves + 3) / 4 : 1);
   const int grad_size = dtype_size(grad_dtype);
   bool vec = false;
-  if constexpr (sizeof(T) == 2) vec = hidden % kStep == 0 && r.xso % 8 == 0 && r.xsi % 8 == 0 && aligned16(r.x);
+  if constexpr (sizeof(T) == 2) vec = hidden == p.width && r.xso % 8 == 0 && r.xsi % 8 == 0 && aligned16(r.x);
   if (vec) {
     if constexpr (sizeof(T) == 2)
       hipLaunchKernelGGL((gather_kernel<T, true>), dim3(gather_grid), dim3(256), 0, st, r, row_of, meta, x, all * p.width, p.width,
@@ -1116,8 +1175,8 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   const Operand ox{x, p.width, all * p.width, all * p.width * 2};
   if constexpr (!Split<T>::kSplit) {
     if (p.narrow) {
-      const int rc = p.width == 64 ? run_narrow<T, 64>(r, ox, ow, vocab, hidden, p, ws, row_of, weight_of, losses, dx, dw, grad_dtype, st)
-                                   : run_narrow<T, 128>(r, ox, ow, vocab, hidden, p, ws, row_of, weight_of, losses, dx, dw, grad_dtype, st);
+      auto f = p.width == 32 ? run_narrow<T, 32> : (p.width == 64 ? run_narrow<T, 64> : run_narrow<T, 128>);
+      const int rc = f(r, ox, ow, vocab, hidden, p, ws, row_of, weight_of, losses, dx, dw, grad_dtype, st);
       if (rc != PT_OK) return rc;
       if (loss != nullptr && reduction != PT_REDUCTION_NONE)
         hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, meta, reduction == PT_REDUCTION_MEAN ? 1 : 0, loss);
@@ -1127,7 +1186,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   const int tiles_v = static_cast<int>(p.words / kTile), tiles_h = static_cast<int>(up(hidden, kTile) / kTile);
   const int tiles_r = static_cast<int>(p.chunk / kTile);
   constexpr size_t lds = Product<T, false, false>::kLds;
-  if (int rc = allow(scores_kernel<T>, lds)) return rc;
+  if (int rc = allow(scores_kernel<T, kTile>, lds)) return rc;
   if (int rc = allow(gradient_kernel<T, false>, lds)) return rc;
   if (int rc = allow(gradient_kernel<T, true>, lds)) return rc;
   auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>(up(tiles, 8))); };
@@ -1138,7 +1197,13 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     _Float16* e = p.grads ? reinterpret_cast<_Float16*>(ws + p.e) : nullptr;
     Scores s{ox,    ow, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, p.chunk * p.words,
              sums,  p.padded, target};
-    hipLaunchKernelGGL((scores_kernel<T>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
+    if (p.rows <= kFewRows) {
+      constexpr size_t few = Product<T, false, false, kFewRows>::kLds;
+      if (int rc = allow(scores_kernel<T, kFewRows>, few)) return rc;
+      hipLaunchKernelGGL((scores_kernel<T, kFewRows>), grid(tiles_v), dim3(256), few, st, s);
+    } else {
+      hipLaunchKernelGGL((scores_kernel<T, kTile>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
+    }
     hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows_most + 31) / 32)), dim3(1024), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
@@ -1151,7 +1216,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), rounds, p.parts_x, top_w, {}};
       d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
       hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
-      if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, dim3(2048), dim3(256), 0, st, d);
+      if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
     }
     if (dw != nullptr) {
       const Operand oxc{x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2};
@@ -1159,7 +1224,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       Gradient d{og, oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, rounds, p.parts_w, top_x, {}};
       d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts)};
       hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
-      if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel, dim3(2048), dim3(256), 0, st, d);
+      if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel, join_grid(vocab, hidden), dim3(256), 0, st, d);
     }
     if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
   }

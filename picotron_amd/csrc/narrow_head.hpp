@@ -19,14 +19,21 @@ enum NarrowPass { kNarrowSums = 0, kNarrowDx = 1, kNarrowDw = 2 };
 
 constexpr int kNarrowOuter = 256;   // rows of the outer side a workgroup holds, 64 a wave
 constexpr int kNarrowInner = 64;    // rows of the inner side a step
-constexpr int64_t kNarrowGroups = 512;  // workgroups wanted: two a CU
-
-// How many parts the inner rows are split into.
-__host__ __device__ inline int narrow_splits(int64_t outer_tiles, int64_t inner_steps) {
-  if (outer_tiles < 1) return 1;
-  int64_t s = kNarrowGroups / outer_tiles;
-  if (s > inner_steps / 4) s = inner_steps / 4;
-  return s < 1 ? 1 : static_cast<int>(s);
+// How many parts the inner rows are split into: such that whole rounds of the workgroups that run at once (two a CU, four where
+// rows are short) take the fewest steps, a part counting for two more.  All parts together are at most kNarrowParts tiles.
+constexpr int64_t kNarrowParts = 1024;
+__host__ __device__ inline int narrow_splits(int64_t outer_tiles, int64_t inner_steps, int hp) {
+  const int64_t at_once = hp == 32 ? 1024 : 512;
+  int best = 1;
+  int64_t least = (outer_tiles + at_once - 1) / at_once * inner_steps;
+  for (int s = 2; s <= 1024 && s * outer_tiles <= kNarrowParts && s * 4 <= inner_steps; s = s < 8 ? s + 1 : s * 5 / 4) {
+    const int64_t t = (outer_tiles * s + at_once - 1) / at_once * ((inner_steps + s - 1) / s + 2);
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
 }
 
 // The steps of a tile of the inner side, HP elements a row, in LDS: 16-byte chunks permuted by bits of the row.
@@ -36,7 +43,7 @@ struct NarrowTile {
   static constexpr int kLoads = kBytes / 4096;
   static constexpr int kChunks = HP / 8;
 
-  static __device__ __forceinline__ int key(int row) { return HP == 64 ? (row >> 1) & 7 : row & 15; }
+  static __device__ __forceinline__ int key(int row) { return HP == 32 ? (row >> 2) & 3 : (HP == 64 ? (row >> 1) & 7 : row & 15); }
   static __device__ __forceinline__ int place(int row, int chunk) { return row * HP * 2 + ((chunk ^ key(row)) * 16); }
 
   // Eight consecutive elements of a row; and of the lane's column four rows from `row`'s quad on and four from 16 behind it on
