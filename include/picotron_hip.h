@@ -444,8 +444,8 @@ int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blo
  * dw [vocab, hidden] contiguous, of grad_dtype (dtype or fp32), for an incoming gradient of 1 of the mean or sum; of the
  * loss without a reduction for dloss (fp32, the given strides).  16 bytes (of fp32; 8 of two-byte types) aligned.
  * loss may be NULL where gradients are asked for.  workspace: 256-byte aligned, _workspace_bytes for the same arguments.
- *   pt_scale_gradient: to = from * scale (fp32 device scalar), rounded once: in place, or from fp32 to another
- *     type.  Nothing is touched in place for a scale of 1.
+ *   pt_scale_gradients: to = from * scale (fp32 device scalar), rounded once, of up to two arrays: in place, or from fp32 to
+ *     another type.  Nothing is touched in place for a scale of 1.
  * Replaces the head's product and F.cross_entropy behind it (src/picotron/training/train_loop.py:136-145). */
 #define PT_REDUCTION_MEAN 0
 #define PT_REDUCTION_SUM 1
@@ -462,8 +462,9 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
                             int64_t dloss_inner_stride, void* dx, int64_t dx_inner, void* dw,
                             int grad_dtype, void* workspace, size_t workspace_bytes,
                             int64_t chunk_rows, int dtype, void* stream);
-int pt_scale_gradient(const void* from, int from_dtype, void* to, int to_dtype, int64_t elements,
-                      const float* scale, void* stream);
+int pt_scale_gradients(const void* from, void* to, int64_t elements, const void* from2, void* to2,
+                       int64_t elements2, int from_dtype, int to_dtype, const float* scale,
+                       void* stream);
 
 /* ---------------------------------------------------------------- Activations kept in 8 bits
  * What the backward of SwiGLU and RMSNorm reads of their inputs, held as whole numbers of a step that

@@ -172,7 +172,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_size_t,
          c_int64, c_int, c_void_p],
     ),
-    "pt_scale_gradient": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p]),
+    "pt_scale_gradients": (
+        c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]
+    ),
     "pt_block8_elems": (c_int64, []),
     "pt_swiglu8_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "pt_swiglu8_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),

@@ -55,9 +55,138 @@ struct Rows {  // labels, and the rows of x, by (outer, inner)
 
 // ------------------------------------------------------------------ rows
 
+// The power of two that takes a magnitude, given by its bits, to between 2^13 and 2^14.
+__device__ __forceinline__ int shift_of(unsigned top) {
+  if (top == 0) return 0;
+  int e;
+  (void)frexpf(__builtin_bit_cast(float, top), &e);
+  return 14 - e;
+}
+
+// A value as planes of 16 bits: itself, or two fp16 (see kLow), whose power of two has been taken.
+template <typename T>
+struct Split {
+  typedef T plane;
+  static constexpr bool kSplit = false;
+  static __device__ __forceinline__ void put(T* p, int64_t, T v) { *p = v; }
+};
+template <>
+struct Split<float> {
+  typedef _Float16 plane;
+  static constexpr bool kSplit = true;
+  static __device__ __forceinline__ void parts(float v, _Float16* hi, _Float16* lo) {
+    *hi = static_cast<_Float16>(v);
+    *lo = static_cast<_Float16>((v - static_cast<float>(*hi)) * kLow);
+  }
+  static __device__ __forceinline__ void put(_Float16* p, int64_t plane, float v) { parts(v, p, p + plane); }
+};
+
+// The largest finite magnitudes of 32-bit inputs: workgroups below `x_blocks` take the kept rows of x, the others the weight's.
+// One atomic a workgroup, whose order a maximum does not depend on.
+__global__ __launch_bounds__(256) void top_kernel(Rows r, const int* __restrict__ row_of, Meta* __restrict__ meta, int64_t hidden,
+                                                  int x_blocks, const float* __restrict__ w, int64_t ld, int64_t vocab) {
+  __shared__ float tops[4];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const bool of_x = static_cast<int>(blockIdx.x) < x_blocks;
+  const int64_t blocks = of_x ? x_blocks : gridDim.x - x_blocks, block = of_x ? blockIdx.x : blockIdx.x - x_blocks;
+  const int64_t rows = of_x ? meta->count : vocab;
+  float t = 0.f;
+  for (int64_t i = block * 4 + wave; i < rows; i += blocks * 4) {
+    const float* p = w + i * ld;
+    if (of_x) {
+      const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
+      p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
+    }
+#pragma unroll 8
+    for (int64_t c = lane; c < hidden; c += 64) {
+      const float v = fabsf(p[c]);
+      t = v < INFINITY ? fmaxf(t, v) : t;
+    }
+  }
+  t = wave_max(t);
+  if (lane == 0) tops[wave] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    atomicMax(of_x ? &meta->top_x : &meta->top_w, __builtin_bit_cast(unsigned, t));  // magnitudes order as their bits
+  }
+}
+
+// What a call lays out for its products, a row a wave: the kept rows of x, one behind the other, `width` elements each with zeros
+// behind the H-th, and zero rows up to a whole tile; zeros in the rows of dx that are not kept; and the weight's rows
+// likewise, where the products cannot read them in place.
+struct Lay {
+  void* x;         // (x_rows, width)
+  int64_t x_rows;
+  void* dx;        // (dx_rows, hidden), or null
+  int64_t dx_rows;
+  int dx_size;
+  const void* w;
+  int64_t ldw;
+  void* to_w;      // (w_rows, width)
+  int64_t w_rows;  // 0: the weight is read in place
+  int64_t width, hidden;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void lay_row(const Rows& r, const Lay& a, const int* row_of, int count, int shift_x, int shift_w, int64_t wave) {
+  typedef typename Split<T>::plane P;
+  const int lane = threadIdx.x % 64;
+  if (wave < a.x_rows) {
+    if (wave >= (static_cast<int64_t>(count) + kTile - 1) / kTile * kTile) return;
+    const T* from = nullptr;
+    if (wave < count) {
+      const int64_t row = row_of[wave], o = row / r.dx_inner, s = row - o * r.dx_inner;
+      from = static_cast<const T*>(r.x) + o * r.xso + s * r.xsi;
+    }
+    P* p = static_cast<P*>(a.x) + wave * a.width;
+    if constexpr (VEC) {  // 16-bit elements, rows of whole vectors
+      const u32x4 zero = {0, 0, 0, 0};
+      for (int64_t c = lane * 8; c < a.width; c += 512)
+        *reinterpret_cast<u32x4*>(p + c) = from != nullptr ? *reinterpret_cast<const u32x4*>(from + c) : zero;
+    } else {
+      for (int64_t c = lane; c < a.width; c += 64) {
+        T v = from != nullptr && c < a.hidden ? from[c] : static_cast<T>(0.f);
+        if constexpr (Split<T>::kSplit) v = ldexpf(v, shift_x);
+        Split<T>::put(p + c, a.x_rows * a.width, v);
+      }
+    }
+    return;
+  }
+  wave -= a.x_rows;
+  if (wave < a.dx_rows) {
+    const int64_t o = wave / r.dx_inner, s = wave - o * r.dx_inner;
+    if (s < r.inner && r.t[o * r.tso + s * r.tsi] != r.ignore) return;
+    char* p = static_cast<char*>(a.dx) + wave * a.hidden * a.dx_size;
+    if (a.dx_size == 4) {
+      for (int64_t c = lane; c < a.hidden; c += 64) reinterpret_cast<float*>(p)[c] = 0.f;
+    } else {
+      for (int64_t c = lane; c < a.hidden; c += 64) reinterpret_cast<unsigned short*>(p)[c] = 0;
+    }
+    return;
+  }
+  wave -= a.dx_rows;
+  if (wave >= a.w_rows) return;
+  const T* from = static_cast<const T*>(a.w) + wave * a.ldw;
+  P* p = static_cast<P*>(a.to_w) + wave * a.width;
+  for (int64_t c = lane; c < a.width; c += 64) {
+    T v = c < a.hidden ? from[c] : static_cast<T>(0.f);
+    if constexpr (Split<T>::kSplit) v = ldexpf(v, shift_w);
+    Split<T>::put(p + c, a.w_rows * a.width, v);
+  }
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void lay_kernel(Rows r, Lay a, const int* __restrict__ row_of, const Meta* __restrict__ meta) {
+  const int shift_x = Split<T>::kSplit ? shift_of(meta->top_x) : 0, shift_w = Split<T>::kSplit ? shift_of(meta->top_w) : 0;
+  lay_row<T, VEC>(r, a, row_of, meta->count, shift_x, shift_w, static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64);
+}
+
 // Which rows are kept, in order: their row of dx, label (-1 for one outside the vocabulary) and weight; how many; the
-// gradients' factor.  One workgroup, a round of whose threads reads eight labels each before the scan.
-__global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int reduction, int* __restrict__ row_of,
+// gradients' factor.  One workgroup, a round of whose threads reads eight labels each before the scan.  Of a small call (`lay`
+// has rows) it does everything in front of the first product, where a launch more would cost more than the work.
+template <typename T>
+__global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, int64_t vocab, int reduction, int* __restrict__ row_of,
                                                     int* __restrict__ label_of, float* __restrict__ weight_of,
                                                     Meta* __restrict__ meta, float* __restrict__ losses) {
   constexpr int kPer = 8;
@@ -121,7 +250,7 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int r
     unsigned e = __builtin_bit_cast(unsigned, top) & 0x7f800000u;
     e = e < 0x00800000u ? 0x00800000u : e;
     const float unit = __builtin_bit_cast(float, e);
-    Meta m{base, 0.f, 1.f, 0, 0};
+    Meta m{base, 0.f, 1.f, 0u, 0u};
     if (reduction == PT_REDUCTION_NONE) {
       m.alpha = unit / kScale;
       m.inv_weight = 1.f / unit;
@@ -130,121 +259,38 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, int64_t vocab, int r
     }
     *meta = m;
   }
-}
-
-// The power of two that takes a magnitude, given by its bits, to between 2^13 and 2^14.
-__device__ __forceinline__ int shift_of(unsigned top) {
-  if (top == 0) return 0;
-  int e;
-  (void)frexpf(__builtin_bit_cast(float, top), &e);
-  return 14 - e;
-}
-
-// A value as planes of 16 bits: itself, or two fp16 (see kLow), whose power of two has been taken.
-template <typename T>
-struct Split {
-  typedef T plane;
-  static constexpr bool kSplit = false;
-  static __device__ __forceinline__ void put(T* p, int64_t, T v) { *p = v; }
-};
-template <>
-struct Split<float> {
-  typedef _Float16 plane;
-  static constexpr bool kSplit = true;
-  static __device__ __forceinline__ void parts(float v, _Float16* hi, _Float16* lo) {
-    *hi = static_cast<_Float16>(v);
-    *lo = static_cast<_Float16>((v - static_cast<float>(*hi)) * kLow);
-  }
-  static __device__ __forceinline__ void put(_Float16* p, int64_t plane, float v) { parts(v, p, p + plane); }
-};
-
-// The largest finite magnitudes of 32-bit inputs: workgroups below `x_blocks` take the kept rows of x, the others the weight's.
-// One atomic a workgroup, whose order a maximum does not depend on.
-__global__ __launch_bounds__(256) void top_kernel(Rows r, const int* __restrict__ row_of, Meta* __restrict__ meta, int64_t hidden,
-                                                  int x_blocks, const float* __restrict__ w, int64_t ld, int64_t vocab) {
-  __shared__ float tops[4];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const bool of_x = static_cast<int>(blockIdx.x) < x_blocks;
-  const int64_t blocks = of_x ? x_blocks : gridDim.x - x_blocks, block = of_x ? blockIdx.x : blockIdx.x - x_blocks;
-  const int64_t rows = of_x ? meta->count : vocab;
-  float t = 0.f;
-  for (int64_t i = block * 4 + wave; i < rows; i += blocks * 4) {
-    const float* p = w + i * ld;
-    if (of_x) {
-      const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
-      p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
-    }
-#pragma unroll 8
-    for (int64_t c = lane; c < hidden; c += 64) {
-      const float v = fabsf(p[c]);
-      t = v < INFINITY ? fmaxf(t, v) : t;
-    }
-  }
-  t = wave_max(t);
-  if (lane == 0) tops[wave] = t;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    t = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    atomicMax(of_x ? &meta->top_x : &meta->top_w, __builtin_bit_cast(unsigned, t));  // magnitudes order as their bits
-  }
-}
-
-// One wave a row: the kept rows of x, one behind the other, `width` (a multiple of 64) elements each with zeros
-// behind the H-th, and zero rows up to a whole tile; and zeros in the rows of dx that are not kept.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void gather_kernel(Rows r, const int* __restrict__ row_of, const Meta* __restrict__ meta,
-                                                     typename Split<T>::plane* __restrict__ to, int64_t plane, int64_t width,
-                                                     int64_t hidden, int64_t gathered, char* __restrict__ dx, int dx_size) {
-  const int lane = threadIdx.x % 64;
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
-  if (wave < gathered) {
-    const int count = meta->count;
-    if (wave >= (static_cast<int64_t>(count) + kTile - 1) / kTile * kTile) return;
-    const T* from = nullptr;
-    if (wave < count) {
-      const int64_t row = row_of[wave], o = row / r.dx_inner, s = row - o * r.dx_inner;
-      from = static_cast<const T*>(r.x) + o * r.xso + s * r.xsi;
-    }
-    typename Split<T>::plane* p = to + wave * width;
-    if constexpr (VEC) {  // 16-bit elements, rows of whole vectors
-      const u32x4 zero = {0, 0, 0, 0};
-      for (int64_t c = lane * 8; c < width; c += 512)
-        *reinterpret_cast<u32x4*>(p + c) = from != nullptr ? *reinterpret_cast<const u32x4*>(from + c) : zero;
-    } else {
-      const int shift = Split<T>::kSplit ? shift_of(meta->top_x) : 0;
-      for (int64_t c = lane; c < width; c += 64) {
-        T v = from != nullptr && c < hidden ? from[c] : static_cast<T>(0.f);
-        if constexpr (Split<T>::kSplit) v = ldexpf(v, shift);
-        Split<T>::put(p + c, plane, v);
+  if (lay.width == 0) return;
+  float most[2] = {0.f, 0.f};  // x and the weight
+  if constexpr (Split<T>::kSplit) {
+    __syncthreads();
+    for (int64_t i = wave; i < base + lay.w_rows; i += 16) {
+      const float* p = static_cast<const float*>(lay.w) + (i - base) * lay.ldw;
+      if (i < base) {
+        const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
+        p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
+      }
+      for (int64_t c = lane; c < lay.hidden; c += 64) {
+        const float v = fabsf(p[c]);
+        if (v < INFINITY) most[i < base ? 0 : 1] = fmaxf(most[i < base ? 0 : 1], v);
       }
     }
-    return;
-  }
-  const int64_t row = wave - gathered;
-  if (dx == nullptr || row >= r.outer * r.dx_inner) return;
-  const int64_t o = row / r.dx_inner, s = row - o * r.dx_inner;
-  if (s < r.inner && r.t[o * r.tso + s * r.tsi] != r.ignore) return;
-  char* p = dx + row * hidden * dx_size;
-  if (dx_size == 4) {
-    for (int64_t c = lane; c < hidden; c += 64) reinterpret_cast<float*>(p)[c] = 0.f;
-  } else {
-    for (int64_t c = lane; c < hidden; c += 64) reinterpret_cast<unsigned short*>(p)[c] = 0;
-  }
-}
-
-// The weight with rows of `width` elements, in planes: for one whose rows the products cannot read in place.
-template <typename T>
-__global__ __launch_bounds__(256) void weight_kernel(const T* __restrict__ w, int64_t ld, typename Split<T>::plane* __restrict__ to,
-                                                     int64_t plane, int64_t width, int64_t hidden, int64_t vocab,
-                                                     const Meta* __restrict__ meta) {
-  const int shift = Split<T>::kSplit ? shift_of(meta->top_w) : 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64; row < vocab;
-       row += static_cast<int64_t>(gridDim.x) * 4)
-    for (int64_t c = threadIdx.x % 64; c < width; c += 64) {
-      T v = c < hidden ? w[row * ld + c] : static_cast<T>(0.f);
-      if constexpr (Split<T>::kSplit) v = ldexpf(v, shift);
-      Split<T>::put(to + row * width + c, plane, v);
+    for (int k = 0; k < 2; ++k) {
+      most[k] = wave_max(most[k]);
+      __syncthreads();
+      if (lane == 0) tops[wave] = most[k];
+      __syncthreads();
+      for (int w = 0; w < 16; ++w) most[k] = fmaxf(most[k], tops[w]);
     }
+    if (threadIdx.x == 0) {
+      meta->top_x = __builtin_bit_cast(unsigned, most[0]);
+      meta->top_w = __builtin_bit_cast(unsigned, most[1]);
+    }
+  } else {
+    __syncthreads();
+  }
+  const int shift_x = shift_of(__builtin_bit_cast(unsigned, most[0])), shift_w = shift_of(__builtin_bit_cast(unsigned, most[1]));
+  for (int64_t i = wave; i < lay.x_rows + lay.dx_rows + lay.w_rows; i += 16)
+    lay_row<T, false>(r, lay, row_of, base, shift_x, shift_w, i);
 }
 
 // ------------------------------------------------------------------ the three products
@@ -554,7 +600,7 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
 }
 
 // How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each, a
-// workgroup a step in 1 us while it is alone and in 1.9 beside 255 others, the join 8 us more, and each tile of a part 0.13 us for
+// workgroup a step in 1 us while it is alone and in 1.9 beside 255 others, the join 12 us more, and each tile of a part 0.13 us for
 // its way to memory and back.  The number of
 // tiles follows from the number of kept rows, so this is decided on the device; `most` bounds the tiles of all parts (0: no
 // split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps, 1025 us in one part.
@@ -567,7 +613,7 @@ __host__ __device__ inline int splits_for(int64_t tiles, int64_t steps, int64_t 
     const int64_t groups = tiles * s;
     if (s > 1 && (s > steps || groups > most)) break;
     const int64_t step = 1000 + (groups < 256 ? groups : 256) * 900 / 256;
-    const int64_t t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 8000 + groups * 130 : 0);
+    const int64_t t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
     if (t < least) {
       least = t;
       best = s;
@@ -971,27 +1017,46 @@ __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
   }
 }
 
-// to = from * scale, rounded once; nothing at all where that changes nothing.
+// to = from * scale, rounded once, of up to two arrays; nothing at all where that changes nothing.
 template <typename S, typename D>
-__global__ __launch_bounds__(256) void rescale_kernel(const S* __restrict__ from, D* __restrict__ to, int64_t n,
-                                                      const float* __restrict__ scale) {
+struct Scaled {
+  const S* from;
+  D* to;
+  int64_t n;
+};
+
+template <typename S, typename D>
+__global__ __launch_bounds__(256) void rescale_kernel(Scaled<S, D> first, Scaled<S, D> second, int blocks, const float* __restrict__ scale) {
   const float c = *scale;
   if (sizeof(S) == sizeof(D) && c == 1.f) return;
-  const int64_t quads = n / 4;
+  const bool one = static_cast<int>(blockIdx.x) < blocks;
+  const Scaled<S, D> a = one ? first : second;
+  const int64_t block = one ? blockIdx.x : blockIdx.x - blocks, grid = one ? blocks : gridDim.x - blocks;
+  const int64_t quads = a.n / 4;
   typedef S S4 __attribute__((ext_vector_type(4)));
   typedef D D4 __attribute__((ext_vector_type(4)));
-  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < quads; q += static_cast<int64_t>(gridDim.x) * 256) {
-    const S4 v = reinterpret_cast<const S4*>(from)[q];
+  for (int64_t q = block * 256 + threadIdx.x; q < quads; q += grid * 256) {
+    const S4 v = reinterpret_cast<const S4*>(a.from)[q];
     D4 w;
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[k] = static_cast<D>(static_cast<float>(v[k]) * c);
-    reinterpret_cast<D4*>(to)[q] = w;
+    reinterpret_cast<D4*>(a.to)[q] = w;
   }
-  if (blockIdx.x == 0 && threadIdx.x < n % 4)
-    to[quads * 4 + threadIdx.x] = static_cast<D>(static_cast<float>(from[quads * 4 + threadIdx.x]) * c);
+  if (block == 0 && threadIdx.x < a.n % 4) a.to[quads * 4 + threadIdx.x] = static_cast<D>(static_cast<float>(a.from[quads * 4 + threadIdx.x]) * c);
+}
+
+template <typename S, typename D>
+int rescale(const void* from, void* to, int64_t n, const void* from2, void* to2, int64_t n2, const float* scale, hipStream_t st) {
+  auto blocks = [](int64_t k) { return k == 0 ? int64_t{0} : ((k / 4 + 255) / 256 < 1 ? int64_t{1} : ((k / 4 + 255) / 256 > 8192 ? int64_t{8192} : (k / 4 + 255) / 256)); };
+  const Scaled<S, D> a{static_cast<const S*>(from), static_cast<D*>(to), n}, b{static_cast<const S*>(from2), static_cast<D*>(to2), n2};
+  hipLaunchKernelGGL((rescale_kernel<S, D>), dim3(static_cast<unsigned>(blocks(n) + blocks(n2))), dim3(256), 0, st, a, b, static_cast<int>(blocks(n)), scale);
+  return check_launch("pt_scale_gradients");
 }
 
 // ------------------------------------------------------------------ sizes
+
+// Calls that lay out no more are laid out by the workgroup that reads the labels.
+constexpr int64_t kSmallRows = 1024, kSmallElements = 32768;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -1139,34 +1204,31 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
   P* x = reinterpret_cast<P*>(ws + p.x);
   float* losses = reduction == PT_REDUCTION_NONE ? loss : nullptr;
 
-  hipLaunchKernelGGL(keep_kernel, dim3(1), dim3(1024), 0, st, r, vocab, reduction, row_of, label_of,
-                     reinterpret_cast<float*>(ws + p.weight_of), meta, losses);
-  const int64_t w_blocks = (vocab + 3) / 4 < 8192 ? (vocab + 3) / 4 : 8192;
-  if constexpr (Split<T>::kSplit) {
-    const int64_t x_blocks = p.rows < 1024 ? (p.rows + 3) / 4 : 256, tops_w = w_blocks < 1024 ? w_blocks : 1024;
-    hipLaunchKernelGGL(top_kernel, dim3(static_cast<unsigned>(x_blocks + tops_w)), dim3(256), 0, st, r, row_of, meta, hidden,
-                       static_cast<int>(x_blocks), static_cast<const float*>(w), ldw, vocab);
-  }
   const int64_t all = up(p.rows, kTile);
-  const int64_t waves = all + (dx != nullptr ? r.outer * r.dx_inner : 0);
-  const unsigned gather_grid = static_cast<unsigned>(waves > 0 ? (waves + 3) / 4 : 1);
-  const int grad_size = dtype_size(grad_dtype);
-  bool vec = false;
-  if constexpr (sizeof(T) == 2) vec = hidden == p.width && r.xso % 8 == 0 && r.xsi % 8 == 0 && aligned16(r.x);
-  if (vec) {
-    if constexpr (sizeof(T) == 2)
-      hipLaunchKernelGGL((gather_kernel<T, true>), dim3(gather_grid), dim3(256), 0, st, r, row_of, meta, x, all * p.width, p.width,
-                         hidden, all, static_cast<char*>(dx), grad_size);
-  } else {
-    hipLaunchKernelGGL((gather_kernel<T, false>), dim3(gather_grid), dim3(256), 0, st, r, row_of, meta, x, all * p.width, p.width,
-                       hidden, all, static_cast<char*>(dx), grad_size);
-  }
+  Lay lay{x, all, dx, dx != nullptr ? r.outer * r.dx_inner : 0, dtype_size(grad_dtype), w, ldw, nullptr, 0, p.width, hidden};
   Operand ow{w, ldw, 0, ((vocab - 1) * ldw + hidden) * 2};
   if (p.copy_weight) {
-    P* to = reinterpret_cast<P*>(ws + p.w);
-    hipLaunchKernelGGL(weight_kernel<T>, dim3(static_cast<unsigned>(w_blocks)), dim3(256), 0, st, static_cast<const T*>(w), ldw, to,
-                       vocab * p.width, p.width, hidden, vocab, meta);
-    ow = Operand{to, p.width, vocab * p.width, vocab * p.width * 2};
+    lay.to_w = ws + p.w;
+    lay.w_rows = vocab;
+    ow = Operand{lay.to_w, p.width, vocab * p.width, vocab * p.width * 2};
+  }
+  const int64_t lay_rows = lay.x_rows + lay.dx_rows + lay.w_rows;
+  const bool small = lay_rows <= kSmallRows && lay_rows * p.width <= kSmallElements;
+  hipLaunchKernelGGL(keep_kernel<T>, dim3(1), dim3(1024), 0, st, r, small ? lay : Lay{}, vocab, reduction, row_of, label_of,
+                     reinterpret_cast<float*>(ws + p.weight_of), meta, losses);
+  if (!small) {
+    if constexpr (Split<T>::kSplit) {
+      const int64_t tops_x = p.rows < 1024 ? (p.rows + 3) / 4 : 256, tops_w = vocab < 4096 ? (vocab + 3) / 4 : 1024;
+      hipLaunchKernelGGL(top_kernel, dim3(static_cast<unsigned>(tops_x + tops_w)), dim3(256), 0, st, r, row_of, meta, hidden,
+                         static_cast<int>(tops_x), static_cast<const float*>(w), ldw, vocab);
+    }
+    const dim3 lay_grid(static_cast<unsigned>(lay_rows > 0 ? (lay_rows + 3) / 4 : 1));
+    bool vec = false;
+    if constexpr (sizeof(T) == 2) {
+      vec = hidden == p.width && r.xso % 8 == 0 && r.xsi % 8 == 0 && aligned16(r.x);
+      if (vec) hipLaunchKernelGGL((lay_kernel<T, true>), lay_grid, dim3(256), 0, st, r, lay, row_of, meta);
+    }
+    if (!vec) hipLaunchKernelGGL((lay_kernel<T, false>), lay_grid, dim3(256), 0, st, r, lay, row_of, meta);
   }
   if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
 
@@ -1301,32 +1363,27 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
   }
 }
 
-int pt_scale_gradient(const void* from, int from_dtype, void* to, int to_dtype, int64_t elements, const float* scale, void* stream) {
-  const std::string name("pt_scale_gradient");
+int pt_scale_gradients(const void* from, void* to, int64_t elements, const void* from2, void* to2, int64_t elements2, int from_dtype,
+                       int to_dtype, const float* scale, void* stream) {
+  const std::string name("pt_scale_gradients");
   if (!pt::valid_dtype(from_dtype) || !pt::valid_dtype(to_dtype)) return pt::fail(PT_EUNSUPPORTED, name + ": dtype must be fp32, fp16 or bf16");
   if (from_dtype != to_dtype && from_dtype != PT_FLOAT32) return pt::fail(PT_EUNSUPPORTED, name + ": only fp32 changes its type");
-  if (elements < 0) return pt::fail(PT_EINVAL, name + ": negative size");
-  if (elements == 0) return pt::ok();
-  if (from == nullptr || to == nullptr || scale == nullptr) return pt::fail(PT_EINVAL, name + ": null pointer");
-  if (from_dtype == to_dtype && from != to) return pt::fail(PT_EINVAL, name + ": gradients of one type are scaled in place");
-  if (!pt::aligned16(from) || !pt::aligned16(to)) return pt::fail(PT_EINVAL, name + ": pointers must be 16-byte aligned");
-  int64_t blocks = (elements / 4 + 255) / 256;
-  blocks = blocks < 1 ? 1 : (blocks > 8192 ? 8192 : blocks);
-  const dim3 grid(static_cast<unsigned>(blocks));
+  if (elements < 0 || elements2 < 0) return pt::fail(PT_EINVAL, name + ": negative size");
+  if (elements == 0 && elements2 == 0) return pt::ok();
+  if ((elements > 0 && (from == nullptr || to == nullptr)) || (elements2 > 0 && (from2 == nullptr || to2 == nullptr)) || scale == nullptr)
+    return pt::fail(PT_EINVAL, name + ": null pointer");
+  if (from_dtype == to_dtype && ((elements > 0 && from != to) || (elements2 > 0 && from2 != to2)))
+    return pt::fail(PT_EINVAL, name + ": gradients of one type are scaled in place");
+  if (!pt::aligned16(from) || !pt::aligned16(to) || !pt::aligned16(from2) || !pt::aligned16(to2))
+    return pt::fail(PT_EINVAL, name + ": pointers must be 16-byte aligned");
   hipStream_t st = pt::as_stream(stream);
-#define PT_SCALE(S, D) \
-  hipLaunchKernelGGL((pt::rescale_kernel<S, D>), grid, dim3(256), 0, st, static_cast<const S*>(from), static_cast<D*>(to), elements, scale)
   if (from_dtype == PT_FLOAT32) {
-    if (to_dtype == PT_FLOAT32) PT_SCALE(float, float);
-    else if (to_dtype == PT_FLOAT16) PT_SCALE(float, _Float16);
-    else PT_SCALE(float, __bf16);
-  } else if (from_dtype == PT_FLOAT16) {
-    PT_SCALE(_Float16, _Float16);
-  } else {
-    PT_SCALE(__bf16, __bf16);
+    if (to_dtype == PT_FLOAT32) return pt::rescale<float, float>(from, to, elements, from2, to2, elements2, scale, st);
+    if (to_dtype == PT_FLOAT16) return pt::rescale<float, _Float16>(from, to, elements, from2, to2, elements2, scale, st);
+    return pt::rescale<float, __bf16>(from, to, elements, from2, to2, elements2, scale, st);
   }
-#undef PT_SCALE
-  return pt::check_launch("pt_scale_gradient");
+  if (from_dtype == PT_FLOAT16) return pt::rescale<_Float16, _Float16>(from, to, elements, from2, to2, elements2, scale, st);
+  return pt::rescale<__bf16, __bf16>(from, to, elements, from2, to2, elements2, scale, st);
 }
 
 }  // extern "C"

@@ -43,7 +43,7 @@ namespace {
   X(pt_sequence_log_probs_workspace_bytes) X(pt_sequence_log_probs) X(pt_preference_loss)     \
   X(pt_sequence_log_probs_bwd) X(pt_last_error) X(pt_swiglu8_fwd) X(pt_swiglu8_bwd)           \
   X(pt_rmsnorm8_fwd) X(pt_rmsnorm8_bwd_workspace_bytes) X(pt_rmsnorm8_bwd)                    \
-  X(pt_linear_cross_entropy_workspace_bytes) X(pt_linear_cross_entropy) X(pt_scale_gradient)
+  X(pt_linear_cross_entropy_workspace_bytes) X(pt_linear_cross_entropy) X(pt_scale_gradients)
 #define PT_DECLARE(f) decltype(&f) p_##f = nullptr;
 PT_NATIVE_FNS(PT_DECLARE)
 #undef PT_DECLARE
@@ -1053,16 +1053,21 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     const auto type = static_cast<at::ScalarType>(kept["type"].toInt());
     void* const stream = reinterpret_cast<void*>(kept["stream"].toInt());
     const at::Tensor scale = as_dense(grads[0], at::kFloat);
-    auto take = [&](const char* name) {
-      if (kept.count(name) == 0) return at::Tensor();
-      const at::Tensor from = kept[name].toTensor();
+    at::Tensor from[2], to[2];
+    for (int k = 0; k < 2; ++k) {
+      const char* name = k == 0 ? "dx" : "dw";
+      if (kept.count(name) == 0) continue;
+      from[k] = kept[name].toTensor();
       kept.erase(name);
-      const at::Tensor to = from.scalar_type() == type ? from : at::empty(from.sizes(), from.options().dtype(type));
-      checked("pt_scale_gradient", p_pt_scale_gradient(in(from), code_of(from), out(to), code_of(to), from.numel(),
-                                                       static_cast<const float*>(in(scale)), stream));
-      return to;
-    };
-    const at::Tensor dx = take("dx"), dw = take("dw");
+      to[k] = from[k].scalar_type() == type ? from[k] : at::empty(from[k].sizes(), from[k].options().dtype(type));
+    }
+    auto n = [](const at::Tensor& t) { return t.defined() ? t.numel() : int64_t{0}; };
+    auto code = [](const at::Tensor (&t)[2]) { return code_of(t[0].defined() ? t[0] : t[1]); };
+    checked("pt_scale_gradients",
+            p_pt_scale_gradients(from[0].defined() ? in(from[0]) : nullptr, to[0].defined() ? out(to[0]) : nullptr, n(from[0]),
+                                 from[1].defined() ? in(from[1]) : nullptr, to[1].defined() ? out(to[1]) : nullptr, n(from[1]), code(from),
+                                 code(to), static_cast<const float*>(in(scale)), stream));
+    const at::Tensor dx = to[0], dw = to[1];
     return {dx, dw, at::Tensor(), at::Tensor()};
   }
 };

@@ -57,8 +57,8 @@ class _ReducedLoss(torch.autograd.Function):
     def backward(ctx, grad: Tensor):  # type: ignore[override]
         if ctx.gradients is None:
             raise RuntimeError(_REPEATED_BACKWARD)
-        (dx, dw), ctx.gradients = ctx.gradients, None
-        dx, dw = (None if d is None else ops.scale_gradient(d, grad, ctx.dtype) for d in (dx, dw))
+        gradients, ctx.gradients = ctx.gradients, None
+        dx, dw = ops.scale_gradients(gradients, grad, ctx.dtype)
         return dx, dw, None, None
 
 

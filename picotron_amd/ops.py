@@ -953,16 +953,17 @@ def linear_cross_entropy(
     return loss, dx, dw
 
 
-def scale_gradient(grad: Tensor, scale: Tensor, dtype: torch.dtype | None = None) -> Tensor:
-    """``grad`` (contiguous) times the device scalar ``scale``, rounded once: in place, left alone where the scale is 1, or from
-    fp32 to a new tensor of ``dtype``."""
+def scale_gradients(grads: tuple[Tensor | None, Tensor | None], scale: Tensor, dtype: torch.dtype) -> tuple[Tensor | None, Tensor | None]:
+    """Up to two contiguous gradients of one type times the device scalar ``scale``, rounded once: in place, left alone where the
+    scale is 1, or from fp32 to new tensors of ``dtype``."""
 
-    device = _check_cuda(grad, scale)
+    given = [g for g in grads if g is not None]
+    device = _check_cuda(scale, *given)
     scale = scale.detach().to(torch.float32).reshape(())
-    to = grad if dtype in (None, grad.dtype) else torch.empty(grad.shape, dtype=dtype, device=device)
-    _call_on(device, "pt_scale_gradient", grad.data_ptr(), dtype_code(grad.dtype), to.data_ptr(), dtype_code(to.dtype),
-             grad.numel(), scale.data_ptr())
-    return to
+    to = [None if g is None else (g if g.dtype == dtype else torch.empty(g.shape, dtype=dtype, device=device)) for g in grads]
+    args = [a for g, t in zip(grads, to) for a in (_ptr(g), _ptr(t), 0 if g is None else g.numel())]
+    _call_on(device, "pt_scale_gradients", *args, dtype_code(given[0].dtype), dtype_code(dtype), scale.data_ptr())
+    return to[0], to[1]
 
 
 # ------------------------------------------------------------------ preference loss

@@ -124,14 +124,15 @@ def test_entry_point_refuses(change, code):
 
 
 def test_scale_entry_point_refuses():
-    f = _lib.lib().pt_scale_gradient
-    assert f(256, 0, 256, 9, 4, 256, None) == _lib.PT_EUNSUPPORTED
-    assert f(256, 1, 512, 0, 4, 256, None) == _lib.PT_EUNSUPPORTED
-    assert f(256, 0, 512, 0, 4, 256, None) == _lib.PT_EINVAL
-    assert f(None, 0, 256, 1, 4, 256, None) == _lib.PT_EINVAL
-    assert f(264, 0, 512, 1, 4, 256, None) == _lib.PT_EINVAL
-    assert f(256, 0, 512, 1, -1, 256, None) == _lib.PT_EINVAL
-    assert f(None, 0, None, 1, 0, None, None) == _lib.PT_OK
+    def call(from_=256, to=256, n=4, from2=None, to2=None, n2=0, a=0, b=0, scale=256):
+        return _lib.lib().pt_scale_gradients(from_, to, n, from2, to2, n2, a, b, scale, None)
+
+    assert call(b=9) == _lib.PT_EUNSUPPORTED
+    assert call(to=512, a=1) == _lib.PT_EUNSUPPORTED
+    for bad in (dict(to=512), dict(from_=None, b=1), dict(from_=264, to=512, b=1), dict(to=512, b=1, n=-1), dict(n2=4), dict(scale=None),
+                dict(from2=256, to2=512, n2=4), dict(from2=264, to2=264, n2=4)):
+        assert call(**bad) == _lib.PT_EINVAL
+    assert call(from_=None, to=None, n=0, scale=None) == _lib.PT_OK
 
 
 def test_workspace_holds_at_most_two_gib_of_exponentials():
