@@ -1124,7 +1124,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   if (want_dx) {
     p.grid_x = tiles_r * tiles_h;
     for (int64_t t = 1; t <= tiles_r && t * tiles_h * 2 <= kMostParts; ++t) {
-      const int64_t tiles = t * tiles_h, parts = tiles * splits_for(tiles, p.words / kStep * rounds, kMostParts);
+      const int64_t tiles = t * tiles_h, parts = tiles * splits_for(tiles, up(vocab, kStep) / kStep * rounds, kMostParts);
       if (parts > p.grid_x) p.grid_x = parts;
       if (parts > tiles && parts > p.parts_x) p.parts_x = parts;
     }
@@ -1273,9 +1273,10 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
                        dim3(256), 0, st, e, p.chunk * p.words, p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
     const Operand og{e, p.words, p.chunk * p.words, p.chunk * p.words * 2};
     const int rounds = p.fp32 ? 3 : 1;
+    const int64_t word_steps = up(vocab, kStep) / kStep;
     float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);
     if (dx != nullptr) {
-      Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(p.words / kStep), rounds, p.parts_x, top_w, {}};
+      Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), rounds, p.parts_x, top_w, {}};
       d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
       hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
       if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
