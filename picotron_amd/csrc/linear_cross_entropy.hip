@@ -313,7 +313,7 @@ struct Scores {
   const int* label_of;
   int64_t first, chunk, vocab;
   int tiles_n, steps;
-  _Float16* e;       // exp(l - m) * 2^14, (chunk, tiles_n * 256), in one plane or two, or null
+  _Float16* e;       // exp(l - m) * 2^14, (chunk, tiles_n * 256) in blocks, in one plane or two, or null
   int64_t e_plane;
   f32x2* sums;       // m and the sum of exp(l - m), (tiles_n, padded)
   int64_t padded;
@@ -384,9 +384,10 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
     tops[f] = fmaxf(fmaxf(red[m], red[BM + m]), fmaxf(red[2 * BM + m], red[3 * BM + m]));
   }
   __syncthreads();
-  const int64_t width = static_cast<int64_t>(s.tiles_n) * kTile;
-  _Float16* to = s.e == nullptr ? nullptr
-                                : s.e + (static_cast<int64_t>(tm) * BM + p.wm * P::TM + i) * width + static_cast<int64_t>(tn) * kTile + col;
+  // the block's rows from the wave's first on: one block in m for a tile of 256, a part of it for one of 64
+  const int block_row = (tm * BM) % kBlockSide + p.wm * P::TM + i;
+  const int64_t block = static_cast<int64_t>(tm * BM / kBlockSide) * s.tiles_n + tn;
+  _Float16* to = s.e == nullptr ? nullptr : s.e + (block * kBlockSide + block_row) * kBlockSide + col;
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     constexpr float kLog2e = 1.44269504088896340736f, kShift = 14.f;  // 2^14 is kScale
@@ -417,11 +418,11 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
           v[h / 2].e[(h % 2) * 4 + k] = hi;
           low[h / 2].e[(h % 2) * 4 + k] = static_cast<_Float16>((e - static_cast<float>(hi)) * kLow);
         }
-      u32x4* at = reinterpret_cast<u32x4*>(to + f * 16 * width);
+      u32x4* at = reinterpret_cast<u32x4*>(to + f * 16 * kBlockSide);
       at[0] = v[0].raw;
       at[1] = v[1].raw;
       if constexpr (Split<T>::kSplit) {
-        at = reinterpret_cast<u32x4*>(to + s.e_plane + f * 16 * width);
+        at = reinterpret_cast<u32x4*>(to + s.e_plane + f * 16 * kBlockSide);
         at[0] = low[0].raw;
         at[1] = low[1].raw;
       }
@@ -546,21 +547,24 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
   }
 }
 
-// G from exp(l - m), in place, eight elements a thread.
+// G from exp(l - m), in place: a workgroup takes 64 rows of a block, eight elements a thread at a time.
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, int64_t width,
-                                                    const f32x2* __restrict__ sums, int64_t padded, const Meta* __restrict__ meta,
-                                                    int64_t first, int64_t chunk, const int* __restrict__ label_of,
-                                                    const float* __restrict__ weight_of, const float* __restrict__ target,
-                                                    const float* __restrict__ z) {
+__global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, const f32x2* __restrict__ sums, int64_t padded,
+                                                    const Meta* __restrict__ meta, int64_t first, int64_t chunk,
+                                                    const int* __restrict__ label_of, const float* __restrict__ weight_of,
+                                                    const float* __restrict__ target, const float* __restrict__ z) {
   typedef typename Split<T>::plane P;
-  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
-  if (col >= width) return;
   const int rows = rows_here(meta, first, chunk);
-  const int all = (rows + kStep - 1) / kStep * kStep;  // the last product takes rows 64 by 64: zeros there
-  for (int64_t row = blockIdx.y; row < all; row += gridDim.y) {
+  const int row0 = static_cast<int>(blockIdx.y) * 64 + threadIdx.x / 32;  // 64 rows lie in one block
+  const int all = (rows + kStep - 1) / kStep * kStep;                     // the last product takes rows 64 by 64: zeros there
+  if (static_cast<int>(blockIdx.y) * 64 >= all) return;
+  const int col = threadIdx.x % 32 * 8;
+  const int64_t block = static_cast<int64_t>(row0 / kBlockSide) * gridDim.x + blockIdx.x;
+  _Float16* at = e + (block * kBlockSide + row0 % kBlockSide) * kBlockSide + col;
+#pragma unroll 4
+  for (int k8 = 0; k8 < 8; ++k8, at += 8 * kBlockSide) {
+    const int row = row0 + k8 * 8;
     float out[8];
-    _Float16* at = e + row * width + col;
     if (row < rows) {
       Vec16<_Float16> v, low;
       v.raw = *reinterpret_cast<const u32x4*>(at);
@@ -568,10 +572,10 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
       const float lse = z[first + row];
       const int label = label_of[first + row];
       const float weight = weight_of == nullptr ? 1.f : weight_of[first + row] * meta->inv_weight;
-      const float m = sums[(col / kTile) * padded + row][0];
+      const float m = sums[blockIdx.x * padded + row][0];
       // a label outside the vocabulary leaves a NaN, as its loss
       const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
-      const int64_t place = label - col;
+      const int place = label - static_cast<int>(blockIdx.x) * kTile - col;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         out[k] = static_cast<float>(v.e[k]);
@@ -1206,11 +1210,11 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
 
   const int64_t all = up(p.rows, kTile);
   Lay lay{x, all, dx, dx != nullptr ? r.outer * r.dx_inner : 0, dtype_size(grad_dtype), w, ldw, nullptr, 0, p.width, hidden};
-  Operand ow{w, ldw, 0, ((vocab - 1) * ldw + hidden) * 2};
+  Operand ow = rows_operand(w, ldw, 0, ((vocab - 1) * ldw + hidden) * 2);
   if (p.copy_weight) {
     lay.to_w = ws + p.w;
     lay.w_rows = vocab;
-    ow = Operand{lay.to_w, p.width, vocab * p.width, vocab * p.width * 2};
+    ow = rows_operand(lay.to_w, p.width, vocab * p.width, vocab * p.width * 2);
   }
   const int64_t lay_rows = lay.x_rows + lay.dx_rows + lay.w_rows;
   const bool small = lay_rows <= kSmallRows && lay_rows * p.width <= kSmallElements;
@@ -1234,7 +1238,8 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
 
   const unsigned* top_x = p.fp32 ? &meta->top_x : nullptr;
   const unsigned* top_w = p.fp32 ? &meta->top_w : nullptr;
-  const Operand ox{x, p.width, all * p.width, all * p.width * 2};
+  const Operand ox = rows_operand(x, p.width, all * p.width, all * p.width * 2);
+  const Operand ow_columns = columns_operand(ow.p, ow.ld, ow.plane, ow.bytes);
   if constexpr (!Split<T>::kSplit) {
     if (p.narrow) {
       auto f = p.width == 32 ? run_narrow<T, 32> : (p.width == 64 ? run_narrow<T, 64> : run_narrow<T, 128>);
@@ -1269,22 +1274,23 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows_most + 31) / 32)), dim3(1024), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
-    hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>((p.words / 8 + 255) / 256), static_cast<unsigned>(p.chunk < 16384 ? p.chunk : 16384)),
-                       dim3(256), 0, st, e, p.chunk * p.words, p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
-    const Operand og{e, p.words, p.chunk * p.words, p.chunk * p.words * 2};
+    const int64_t slope_rows = (rows_most + 63) / 64;
+    hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>(tiles_v), static_cast<unsigned>(slope_rows)), dim3(256), 0, st, e,
+                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
+    const int64_t plane = p.chunk * p.words;
     const int rounds = p.fp32 ? 3 : 1;
     const int64_t word_steps = up(vocab, kStep) / kStep;
     float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);
     if (dx != nullptr) {
-      Gradient d{og, ow, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), rounds, p.parts_x, top_w, {}};
+      Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), rounds, p.parts_x, top_w, {}};
       d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
       hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
       if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
     }
     if (dw != nullptr) {
-      const Operand oxc{x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2};
+      const Operand oxc = columns_operand(x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2);
       const int how = p.chunks == 1 ? kFinal : (c + 1 == p.chunks ? kAddFinal : kAdd);
-      Gradient d{og, oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, rounds, p.parts_w, top_x, {}};
+      Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, rounds, p.parts_w, top_x, {}};
       d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts)};
       hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
       if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel, join_grid(vocab, hidden), dim3(256), 0, st, d);

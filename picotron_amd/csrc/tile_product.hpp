@@ -19,12 +19,29 @@ constexpr int kStep = 64;  // k of one step: 128 bytes of a row
 // One operand.  Element (m, k) of plane s is at p + s * plane + m * ld + k (rows) or + k * ld + m (columns); ld and the
 // planes are multiples of 8 elements and p is aligned to 16 bytes.  A plane has `bytes` bytes: what lies behind is
 // read as zero.
+//
+// A blocked operand lies in blocks of 256 by 256 elements, each contiguous, so that a step of a tile stays within one: with rows of
+// 128256 words a tile's 256 rows would lie 256 KB apart, and its loads wait for address translation.
 struct Operand {
   const void* p;
   int64_t ld;
   int64_t plane;  // from the first plane to the second
   int64_t bytes;
+  int64_t per_m;  // bytes from one m to the next tile's, over the m of a tile
+  int64_t jump;   // bytes more after every fourth step
 };
+
+constexpr int kBlockSide = 256;
+
+inline Operand rows_operand(const void* p, int64_t ld, int64_t plane, int64_t bytes) { return Operand{p, ld, plane, bytes, ld * 2, 0}; }
+inline Operand columns_operand(const void* p, int64_t ld, int64_t plane, int64_t bytes) { return Operand{p, ld, plane, bytes, 2, 0}; }
+// (rows, `words`) in blocks, row blocks one behind the other: its rows along m and words along k, or the other way round.
+inline Operand blocked_rows(const void* p, int64_t words, int64_t plane, int64_t bytes) {
+  return Operand{p, kBlockSide, plane, bytes, words * 2, (kBlockSide - 1) * kBlockSide * 2};
+}
+inline Operand blocked_columns(const void* p, int64_t words, int64_t plane, int64_t bytes) {
+  return Operand{p, kBlockSide, plane, bytes, kBlockSide * 2, (words - kBlockSide) * kBlockSide * 2};
+}
 
 // 32-bit operands are two fp16 planes: with v the value times the operand's power of two (its largest magnitude then lies
 // between 2^13 and 2^14), hi = fp16(v) and lo = fp16((v - hi) * 2^11), 22 bits and the sign of lo, down to 2^-28 of the largest.
@@ -176,21 +193,22 @@ struct TileProduct {
 
     // bytes from one step to the next, and to the first
     const int64_t step_a = A_COLUMNS ? a.ld * kStep * 2 : kStep * 2, step_b = B_COLUMNS ? b.ld * kStep * 2 : kStep * 2;
-    const int64_t from_a = (A_COLUMNS ? m0 : m0 * a.ld) * 2 + first * step_a;
-    const int64_t from_b = (B_COLUMNS ? n0 : n0 * b.ld) * 2 + first * step_b;
+    const int64_t from_a = m0 * a.per_m + first * step_a + first / 4 * a.jump, from_b = n0 * b.per_m + first * step_b + first / 4 * b.jump;
     const int steps = last - first, total = steps * (SPLIT ? 3 : 1);
     const char* pa = static_cast<const char*>(a.p) + (SPLIT ? a.plane * 2 : 0);
     const char* pb = static_cast<const char*>(b.p);
     int64_t at_a = from_a, at_b = from_b, bytes_a = a.bytes, bytes_b = b.bytes;
-    int loaded = 0;
+    int loaded = 0, step = first;
     auto load = [&]() {
       lds_char* to = lds + (loaded & 1) * kStage;
       ta.load(to, pa, at_a, bytes_a);
       tb.load(to + TileA::kBytes, pb, at_b, bytes_b);
-      at_a += step_a;
-      at_b += step_b;
       ++loaded;
-      if (SPLIT && (loaded == steps || loaded == 2 * steps)) {  // lo hi, hi lo, hi hi
+      ++step;
+      at_a += step_a + (step % 4 == 0 ? a.jump : 0);
+      at_b += step_b + (step % 4 == 0 ? b.jump : 0);
+      if (SPLIT && step == last && loaded < total) {  // lo hi, hi lo, hi hi
+        step = first;
         at_a = from_a;
         at_b = from_b;
         pa = static_cast<const char*>(a.p);
