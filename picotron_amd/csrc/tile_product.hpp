@@ -259,18 +259,16 @@ struct TileProduct {
 #undef PT_ARRIVED
   }
 
-  // The reads of one half, and the loads of a step to come, among the products of the other half.  Loads before reads where both
-  // operands lie as rows (8192 x 32768 x 4096: 1.78 against 1.81 ms), behind them where one lies as columns, which is
-  // read in twice as many pieces (8192 x 4096 x 64256: 3.82 and 3.64 ms; both as columns, 65536 x 4096 x 8192: 4.07 and 3.97).
+  // The reads of one half, and the loads of a step to come, among the products of the other half: the loads as early as the
+  // reads let them, which the next half waits for.  With the loads behind the reads 8192 x 4096 x 64256 (the second operand as
+  // columns) took 4.05 ms and 65536 x 4096 x 8192 (both) 4.19; so, 3.89 and 4.16; all loads first, 3.95 and 4.14.
   template <int LOADS>
   static __device__ __forceinline__ void interleave() {
     constexpr int kReads = FN * (B_COLUMNS ? 2 : 1) + FM * (A_COLUMNS ? 2 : 1);
-    constexpr bool kLoadsFirst = !A_COLUMNS && !B_COLUMNS;
 #pragma unroll
-    for (int k = 0; k < LOADS + kReads; ++k) {
-      const bool is_load = kLoadsFirst ? k < LOADS : k >= kReads;
-      if (is_load) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-      else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    for (int k = 0; k < (LOADS > kReads ? LOADS : kReads); ++k) {
+      if (k < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      if (k < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, FM * FN, 0);
