@@ -35,12 +35,61 @@ constexpr int64_t kScoreRows = 65536;  // rows of a chunk that only leaves sums
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
+// How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each, a
+// workgroup a step in 1 us while it is alone and in 1.9 beside 255 others, the join 12 us more, and each tile of a part 0.13 us for
+// its way to memory and back.  The number of
+// tiles follows from the number of kept rows, so this is decided on the device; `most` bounds the tiles of all parts (0: no
+// split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps, 1025 us in one part.
+constexpr int64_t kMostParts = 1024;
+__host__ __device__ inline int splits_for(int64_t all_tiles, int64_t all_steps, int64_t most) {
+  if (all_tiles * 2 > most || all_tiles < 1) return 1;
+  constexpr unsigned kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
+  const unsigned tiles = static_cast<unsigned>(all_tiles), steps = static_cast<unsigned>(all_steps);
+  unsigned best = 1, least = ~0u;  // ns
+#pragma unroll
+  for (unsigned s : kTry) {
+    const unsigned groups = tiles * s, step = 1000 + (groups < 256 ? groups : 256) * 900 / 256;
+    const unsigned t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
+    if ((s == 1 || (s <= steps && groups <= most)) && t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return static_cast<int>(best);
+}
+
+// What the splits follow from beside the kept rows (see Plan); found once, by the kernel that counts the rows.
+struct Splits {
+  int narrow;                           // the width of a narrow model, or 0
+  int64_t chunk;
+  int few, tiles_v, tiles_h, steps_s, steps_x, rounds;
+  int64_t vocab, most_s, most_x, most_w;
+};
+enum { kSplitS = 0, kSplitX = 1, kSplitW = 2 };
+
+__host__ __device__ inline int split_of(const Splits& p, int64_t rows, int which) {
+  if (p.narrow > 0) {
+    const int64_t tiles_r = (rows + kNarrowOuter - 1) / kNarrowOuter, tiles_v = (p.vocab + kNarrowOuter - 1) / kNarrowOuter;
+    return which == kSplitW ? narrow_splits(tiles_v, (rows + kNarrowInner - 1) / kNarrowInner, p.narrow)
+                            : narrow_splits(tiles_r, (p.vocab + kNarrowInner - 1) / kNarrowInner, p.narrow);
+  }
+  const int64_t tiles_r = (rows + kTile - 1) / kTile;
+  if (which == kSplitS) return splits_for((rows + p.few - 1) / p.few * p.tiles_v, static_cast<int64_t>(p.steps_s) * p.rounds, p.most_s);
+  if (which == kSplitX) return splits_for(tiles_r * p.tiles_h, static_cast<int64_t>(p.steps_x) * p.rounds, p.most_x);
+  return splits_for(static_cast<int64_t>(p.tiles_v) * p.tiles_h, (rows + kStep - 1) / kStep * p.rounds, p.most_w);
+}
+
 struct Meta {
   int count;        // kept rows
   float alpha;      // of the gradients' sums
   float inv_weight; // of the rows' own weights
   unsigned top_x, top_w;  // bits of the largest finite magnitudes (32-bit inputs)
+  int splits[2][3];       // of a whole chunk's products, and of the last one's
 };
+
+__device__ __forceinline__ int splits_here(const Meta* meta, int rows, int64_t chunk, int which) {
+  return meta->splits[rows == chunk ? 0 : 1][which];
+}
 
 struct Rows {  // labels, and the rows of x, by (outer, inner)
   const void* x;
@@ -51,6 +100,7 @@ struct Rows {  // labels, and the rows of x, by (outer, inner)
   const float* c;  // weights, or null
   int64_t cso, csi;
   int64_t dx_inner;  // rows of dx an outer index has
+  const float* scale;  // of the gradients of a mean or sum, or null
 };
 
 // ------------------------------------------------------------------ rows
@@ -186,7 +236,7 @@ __global__ __launch_bounds__(256) void lay_kernel(Rows r, Lay a, const int* __re
 // gradients' factor.  One workgroup, a round of whose threads reads eight labels each before the scan.  Of a small call (`lay`
 // has rows) it does everything in front of the first product, where a launch more would cost more than the work.
 template <typename T>
-__global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, int64_t vocab, int reduction, int* __restrict__ row_of,
+__global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits splits, int64_t vocab, int reduction, int* __restrict__ row_of,
                                                     int* __restrict__ label_of, float* __restrict__ weight_of,
                                                     Meta* __restrict__ meta, float* __restrict__ losses) {
   constexpr int kPer = 8;
@@ -250,14 +300,22 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, int64_t voc
     unsigned e = __builtin_bit_cast(unsigned, top) & 0x7f800000u;
     e = e < 0x00800000u ? 0x00800000u : e;
     const float unit = __builtin_bit_cast(float, e);
-    Meta m{base, 0.f, 1.f, 0u, 0u};
+    float alpha = 0.f, inv_weight = 1.f;
     if (reduction == PT_REDUCTION_NONE) {
-      m.alpha = unit / kScale;
-      m.inv_weight = 1.f / unit;
+      alpha = unit / kScale;
+      inv_weight = 1.f / unit;
     } else if (base > 0) {
-      m.alpha = (reduction == PT_REDUCTION_MEAN ? 1.f / static_cast<float>(base) : 1.f) / kScale;
+      alpha = (reduction == PT_REDUCTION_MEAN ? 1.f / static_cast<float>(base) : 1.f) / kScale * (r.scale != nullptr ? *r.scale : 1.f);
     }
-    *meta = m;
+    meta->count = base;
+    meta->alpha = alpha;
+    meta->inv_weight = inv_weight;
+    meta->top_x = meta->top_w = 0u;
+  }
+  if (threadIdx.x >= 64 && threadIdx.x < 70) {
+    const int k = threadIdx.x - 64;
+    const int64_t rows = k < 3 ? splits.chunk : base % splits.chunk;
+    meta->splits[k / 3][k % 3] = rows > 0 ? split_of(splits, rows, k % 3) : 1;
   }
   if (lay.width == 0) return;
   float most[2] = {0.f, 0.f};  // x and the weight
@@ -318,6 +376,7 @@ struct Scores {
   f32x2* sums;       // m and the sum of exp(l - m), (tiles_n, padded)
   int64_t padded;
   float* target;     // the label's logit of each kept row
+  float* parts;      // (splits, tiles of rows * BM, tiles_n * 256)
 };
 
 template <typename T, int BM>
@@ -326,11 +385,10 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
   typedef Product<T, false, false, BM> P;
   const int rows = rows_here(s.meta, s.first, s.chunk);
   int tm, tn;
+  if (splits_here(s.meta, rows, s.chunk, kSplitS) > 1) return;  // parts_scores_kernel and finish_kernel
   if (!tile_of(blockIdx.x, (rows + BM - 1) / BM, s.tiles_n, 4, &tm, &tn)) return;
   P p;
-  p.run((lds_char*)lds_raw, s.x, s.w, s.first + static_cast<int64_t>(tm) * BM, static_cast<int64_t>(tn) * kTile, 0,
-        s.steps);
-
+  p.run((lds_char*)lds_raw, s.x, s.w, s.first + static_cast<int64_t>(tm) * BM, static_cast<int64_t>(tn) * kTile, 0, s.steps);
   if constexpr (Split<T>::kSplit) {
     const int shift = -shift_of(s.meta->top_x) - shift_of(s.meta->top_w);
 #pragma unroll
@@ -443,6 +501,92 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
   }
 }
 
+// Where there are few tiles and many steps, a product's parts (kept apart from scores_kernel, whose registers they would spill).
+template <typename T, int BM>
+__device__ __forceinline__ void parts_scores(const Scores& s, lds_char* lds) {
+  typedef Product<T, false, false, BM> P;
+  const int rows = rows_here(s.meta, s.first, s.chunk), tiles_m = (rows + BM - 1) / BM;
+  const int splits = splits_here(s.meta, rows, s.chunk, kSplitS);
+  int tm, tn;
+  if (splits == 1 || !tile_of(blockIdx.x, tiles_m, s.tiles_n * splits, 4, &tm, &tn)) return;
+  const int split = tn % splits;
+  tn /= splits;
+  const int each = (s.steps + splits - 1) / splits;
+  const int from = split * each, until = from + each < s.steps ? from + each : s.steps;
+  P p;
+  p.run(lds, s.x, s.w, s.first + static_cast<int64_t>(tm) * BM, static_cast<int64_t>(tn) * kTile, from, until);
+  const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+  const int64_t ld = static_cast<int64_t>(s.tiles_n) * kTile;
+  float* to = s.parts + (static_cast<int64_t>(split) * tiles_m * BM + tm * BM + p.wm * P::TM + i) * ld + tn * kTile + p.wn * P::TN + 16 * g;
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f)
+#pragma unroll
+    for (int h = 0; h < P::FN; ++h) *reinterpret_cast<f32x4*>(to + f * 16 * ld + h * 4) = p.sums[f][h];
+}
+
+template <typename T, int BM>
+__global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void parts_scores_kernel(Scores s) {
+  extern __shared__ char lds_raw[];
+  parts_scores<T, BM>(s, (lds_char*)lds_raw);
+}
+
+// What scores_kernel leaves, from the parts of split products: 16 rows of a tile a workgroup, 16 lanes a row, 16 words a lane.
+template <typename T, int BM>
+__global__ __launch_bounds__(256) void finish_kernel(Scores s) {
+  const int rows = rows_here(s.meta, s.first, s.chunk), tiles_m = (rows + BM - 1) / BM;
+  const int splits = splits_here(s.meta, rows, s.chunk, kSplitS);
+  const int row = blockIdx.y * 16 + threadIdx.x / 16, tn = blockIdx.x, col = threadIdx.x % 16 * 16;
+  if (splits == 1 || static_cast<int>(blockIdx.y) * 16 >= rows) return;
+  const int64_t ld = static_cast<int64_t>(s.tiles_n) * kTile, size = static_cast<int64_t>(tiles_m) * BM * ld;
+  const float* from = s.parts + row * ld + tn * kTile + col;  // rows behind the last lie in the same tile
+  f32x4 v[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    v[h] = *reinterpret_cast<const f32x4*>(from + h * 4);
+#pragma unroll 8
+    for (int k = 1; k < splits; ++k) v[h] += *reinterpret_cast<const f32x4*>(from + k * size + h * 4);
+  }
+  const int shift = Split<T>::kSplit ? -shift_of(s.meta->top_x) - shift_of(s.meta->top_w) : 0;
+  const int64_t left = s.vocab - static_cast<int64_t>(tn) * kTile - col;
+  const int label = (row < rows ? s.label_of[s.first + row] : -1) - tn * kTile - col;
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    float l = v[k / 4][k % 4];
+    if constexpr (Split<T>::kSplit) l = ldexpf(l, shift);
+    if (k >= left) l = -INFINITY;
+    if (k == label) s.target[s.first + row] = l;
+    v[k / 4][k % 4] = l;
+    top = fmaxf(top, l);
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  constexpr float kLog2e = 1.44269504088896340736f, kShift = 14.f;
+  const float level = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  Vec16<_Float16> hi[2], low[2];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k / 4][k % 4] - level, kLog2e, kShift));
+    sum += e;
+    hi[k / 8].e[k % 8] = static_cast<_Float16>(e);
+    low[k / 8].e[k % 8] = static_cast<_Float16>((e - static_cast<float>(hi[k / 8].e[k % 8])) * kLow);
+  }
+  sum = row16_sum(sum);
+  if (row >= rows) return;
+  if (col == 0) s.sums[static_cast<int64_t>(tn) * s.padded + row] = f32x2{top, sum * (1.0f / kScale)};
+  if (s.e == nullptr) return;
+  const int64_t block = static_cast<int64_t>(row / kBlockSide) * s.tiles_n + tn;
+  u32x4* at = reinterpret_cast<u32x4*>(s.e + (block * kBlockSide + row % kBlockSide) * kBlockSide + col);
+  at[0] = hi[0].raw;
+  at[1] = hi[1].raw;
+  if constexpr (Split<T>::kSplit) {
+    at = reinterpret_cast<u32x4*>(reinterpret_cast<_Float16*>(at) + s.e_plane);
+    at[0] = low[0].raw;
+    at[1] = low[1].raw;
+  }
+}
+
 // z of each row from its tiles' sums, and the row's loss.  32 rows a workgroup, 32 threads a row, in a fixed order.
 __device__ __forceinline__ void join_rows(const f32x2* __restrict__ sums, int64_t padded, int tiles,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
@@ -521,13 +665,13 @@ __global__ __launch_bounds__(1024) void join_kernel(const f32x2* __restrict__ su
   join_rows(sums, padded, tiles, meta, first, chunk, row_of, label_of, target, z, row_loss, losses, inner, dx_inner, nullptr);
 }
 
-__global__ __launch_bounds__(1024) void narrow_join_kernel(const f32x2* __restrict__ sums, int64_t vocab, const Meta* __restrict__ meta, const int* __restrict__ row_of,
+__global__ __launch_bounds__(1024) void narrow_join_kernel(const f32x2* __restrict__ sums, int64_t chunk, const Meta* __restrict__ meta, const int* __restrict__ row_of,
                                                            const int* __restrict__ label_of, const float* __restrict__ target,
                                                            float* __restrict__ z, float* __restrict__ row_loss, float* __restrict__ losses,
-                                                           int64_t inner, int64_t dx_inner, float* __restrict__ exponent, int hp) {
+                                                           int64_t inner, int64_t dx_inner, float* __restrict__ exponent) {
   const int64_t rows = meta->count;
   const int64_t tiles = (rows + kNarrowOuter - 1) / kNarrowOuter;
-  const int splits = narrow_splits(tiles, (vocab + kNarrowInner - 1) / kNarrowInner, hp);
+  const int splits = splits_here(meta, static_cast<int>(rows), chunk, kSplitX);
   join_rows(sums, tiles * kNarrowOuter, splits, meta, 0, rows, row_of, label_of, target, z, row_loss, losses, inner, dx_inner, exponent);
 }
 
@@ -603,29 +747,6 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
   }
 }
 
-// How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each, a
-// workgroup a step in 1 us while it is alone and in 1.9 beside 255 others, the join 12 us more, and each tile of a part 0.13 us for
-// its way to memory and back.  The number of
-// tiles follows from the number of kept rows, so this is decided on the device; `most` bounds the tiles of all parts (0: no
-// split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps, 1025 us in one part.
-constexpr int64_t kMostParts = 1024;
-__host__ __device__ inline int splits_for(int64_t tiles, int64_t steps, int64_t most) {
-  constexpr int kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
-  int best = 1;
-  int64_t least = int64_t{1} << 62;
-  for (int s : kTry) {
-    const int64_t groups = tiles * s;
-    if (s > 1 && (s > steps || groups > most)) break;
-    const int64_t step = 1000 + (groups < 256 ? groups : 256) * 900 / 256;
-    const int64_t t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
-    if (t < least) {
-      least = t;
-      best = s;
-    }
-  }
-  return best;
-}
-
 enum { kFinal = 0, kAdd = 1, kAddFinal = 2 };
 
 // Where a product's sums go: times alpha to rows of `p`, (rows, cols), or as they are to a part of their own, to be
@@ -669,8 +790,7 @@ struct Gradient {
   int64_t first, chunk;
   int tiles_m, tiles_n;  // tiles_m < 0: as many as the chunk's rows take
   int steps;             // < 0: as many as the chunk's rows take
-  int rounds;            // of the steps (32-bit inputs: 3)
-  int64_t most_parts;
+  int which;             // of the splits
   const unsigned* top_b;  // of b's magnitudes (32-bit inputs)
   Out out;
 };
@@ -682,7 +802,7 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   const int rows = rows_here(s.meta, s.first, s.chunk);
   const int tiles_m = s.tiles_m < 0 ? (rows + kTile - 1) / kTile : s.tiles_m;
   const int steps = s.steps < 0 ? (rows + kStep - 1) / kStep : s.steps;
-  const int splits = splits_for(static_cast<int64_t>(tiles_m) * s.tiles_n, static_cast<int64_t>(steps) * s.rounds, s.most_parts);
+  const int splits = splits_here(s.meta, rows, s.chunk, s.which);
   int tm, tn;
   // the splits of a tile lie side by side
   if (!tile_of(blockIdx.x, tiles_m, s.tiles_n * splits, 4, &tm, &tn)) return;
@@ -697,6 +817,39 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   const Out& o = s.out;
   const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
   const float alpha = s.meta->alpha;
+  if (!Split<T>::kSplit && splits == 1 && o.how == kFinal && o.dtype != PT_FLOAT32 && o.cols % 8 == 0) {
+    // 16-bit results go through LDS, a row's 512 bytes contiguous (chunks of 16 permuted by bits of the row), and leave in whole
+    // lines: 40 rows of 4096, 118914 words, whose dw is 1 GB: 438 us by 8 bytes a lane, 303 so
+    lds_char* lds = (lds_char*)lds_raw;
+#pragma unroll
+    for (int f = 0; f < P::FM; ++f) {
+      const int row = p.wm * P::TM + f * 16 + i;
+#pragma unroll
+      for (int h = 0; h < P::FN; ++h) {
+        const int chunk = p.wn * (P::TN / 8) + h * 2 + g / 2;
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+        s16x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          typename Split<T>::plane e = static_cast<typename Split<T>::plane>(p.sums[f][h][k] * alpha);
+          v[k] = __builtin_bit_cast(short, e);
+        }
+        *(lds4)(lds + row * 512 + ((chunk ^ (row & 15)) * 16) + (g & 1) * 8) = v;
+      }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int k = 0; k < 16; ++k) {
+      const int row = k * 16 + threadIdx.x / 32, chunk = threadIdx.x % 32;
+      const int64_t at = static_cast<int64_t>(tm) * kTile + row, col = static_cast<int64_t>(tn) * kTile + chunk * 8;
+      if (at >= limit || col >= o.cols) continue;
+      typedef __attribute__((address_space(3))) u32x4* lds16;
+      const u32x4 v = *(lds16)(lds + row * 512 + ((chunk ^ (row & 15)) * 16));
+      const int64_t to_row = o.row_of != nullptr ? o.row_of[s.first + at] : at;
+      *reinterpret_cast<u32x4*>(static_cast<char*>(o.p) + (to_row * o.cols + col) * 2) = v;
+    }
+    return;
+  }
   const bool vec = o.cols % 4 == 0;
   const int shift = Split<T>::kSplit ? -shift_of(*s.top_b) : 0;
 #pragma unroll
@@ -739,7 +892,7 @@ struct Narrow {
   const Meta* meta;
   const int* label_of;
   const float* weight_of;  // or null
-  int64_t vocab;
+  int64_t vocab, chunk;
   f32x2* sums;  // (splits, outer tiles * 256)
   float* target;
   const float* exponent;
@@ -756,7 +909,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
   const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows, inner_rows = PASS == kNarrowDw ? rows : s.vocab;
   const int outer_tiles = static_cast<int>((outer_rows + kNarrowOuter - 1) / kNarrowOuter);
   const int steps = static_cast<int>((inner_rows + kNarrowInner - 1) / kNarrowInner);
-  const int splits = narrow_splits(outer_tiles, steps, HP);
+  const int splits = splits_here(s.meta, rows, s.chunk, PASS == kNarrowDw ? kSplitW : kSplitX);
   const int tile = blockIdx.x / splits, split = blockIdx.x % splits;
   if (tile >= outer_tiles) return;
   const int each = (steps + splits - 1) / splits, from = split * each, to = from + each < steps ? from + each : steps;
@@ -975,9 +1128,9 @@ __global__ __launch_bounds__(256) void narrow_kernel(Narrow s) {
 template <int HP, int PASS>
 __global__ __launch_bounds__(256) void narrow_parts_kernel(Narrow s) {
   const int rows = s.meta->count;
-  const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows, inner_rows = PASS == kNarrowDw ? rows : s.vocab;
+  const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows;
   const int64_t outer_tiles = (outer_rows + kNarrowOuter - 1) / kNarrowOuter;
-  const int splits = narrow_splits(outer_tiles, (inner_rows + kNarrowInner - 1) / kNarrowInner, HP);
+  const int splits = splits_here(s.meta, rows, s.chunk, PASS == kNarrowDw ? kSplitW : kSplitX);
   if (splits == 1) return;
   const int64_t size = outer_tiles * kNarrowOuter * HP;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < outer_rows * (HP / 4); q += static_cast<int64_t>(gridDim.x) * 256) {
@@ -997,8 +1150,7 @@ __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
   const Out& o = s.out;
   const int rows = rows_here(s.meta, s.first, s.chunk);
   const int tiles_m = s.tiles_m < 0 ? (rows + kTile - 1) / kTile : s.tiles_m;
-  const int steps = s.steps < 0 ? (rows + kStep - 1) / kStep : s.steps;
-  const int splits = splits_for(static_cast<int64_t>(tiles_m) * s.tiles_n, static_cast<int64_t>(steps) * s.rounds, s.most_parts);
+  const int splits = splits_here(s.meta, rows, s.chunk, s.which);
   if (splits == 1) return;
   const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
   const int64_t quads = (o.cols + 3) / 4, ld = static_cast<int64_t>(s.tiles_n) * kTile, size = ld * tiles_m * kTile;
@@ -1068,8 +1220,8 @@ struct Plan {
   bool fp32, copy_weight, grads, narrow;
   int64_t rows, width, words, chunk, chunks, padded;  // width: of x and w; words: of G
   int planes;
-  int64_t grid_x, grid_w;    // workgroups of the gradients, and the tiles of the parts they may be split into
-  int64_t parts_x, parts_w;
+  int64_t grid_x, grid_w;    // workgroups of the products, and the tiles of the parts they may be split into
+  int64_t parts_s, parts_x, parts_w;
   size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, sum_w, exponent, total;
 };
 
@@ -1125,6 +1277,11 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   const int64_t rounds = p.fp32 ? 3 : 1, cols = up(hidden, kTile);
   const int64_t tiles_h = cols / kTile, tiles_v = p.words / kTile, tiles_r = p.chunk / kTile;
   // the kept rows are known on the device alone: as many workgroups and parts as any number of them takes
+  const int64_t few = rows <= kFewRows ? kFewRows : kTile, tiles_s = p.chunk / few;
+  for (int64_t t = 1; t <= tiles_s && t * tiles_v * 2 <= kMostParts; ++t) {
+    const int64_t tiles = t * tiles_v, parts = tiles * splits_for(tiles, p.width / kStep * rounds, kMostParts);
+    if (parts > tiles && parts > p.parts_s) p.parts_s = parts;
+  }
   if (want_dx) {
     p.grid_x = tiles_r * tiles_h;
     for (int64_t t = 1; t <= tiles_r && t * tiles_h * 2 <= kMostParts; ++t) {
@@ -1144,10 +1301,13 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
     }
     if (p.parts_w > p.grid_w) p.grid_w = p.parts_w;
   }
-  // the parts of dx are joined before dw begins, but a sum of dw over chunks stays
+  // parts are joined before the next product begins, but a sum of dw over chunks stays
   const size_t tile_bytes = static_cast<size_t>(kTile) * kTile * 4;
   p.sum_w = p.chunks > 1 && want_dw ? tiles_v * tiles_h * tile_bytes : 0;
-  p.parts = take(p.sum_w + (p.parts_x > p.parts_w ? p.parts_x : p.parts_w) * tile_bytes);
+  size_t parts = p.parts_s * few * kTile * 4;
+  if (parts < p.parts_x * tile_bytes) parts = p.parts_x * tile_bytes;
+  if (parts < p.parts_w * tile_bytes) parts = p.parts_w * tile_bytes;
+  p.parts = take(p.sum_w + parts);
   p.total = at;
   return p;
 }
@@ -1173,11 +1333,11 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
   float* exponent = reinterpret_cast<float*>(ws + p.exponent);
   f32x2* sums = reinterpret_cast<f32x2*>(ws + p.sums);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
-  Narrow s{ox, ow, meta, label_of, weight_of, vocab, sums, target, exponent, z, {}};
+  Narrow s{ox, ow, meta, label_of, weight_of, vocab, p.chunk, sums, target, exponent, z, {}};
   const dim3 grid_x(static_cast<unsigned>(p.grid_x)), grid_w(static_cast<unsigned>(p.grid_w));
   hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowSums>), grid_x, dim3(256), 0, st, s);
-  hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, vocab, meta, row_of, label_of,
-                     target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent, HP);
+  hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, p.chunk, meta, row_of, label_of,
+                     target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent);
   if (dx != nullptr) {
     s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDx>), grid_x, dim3(256), 0, st, s);
@@ -1191,6 +1351,20 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
     hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDw>), join_grid(vocab, hidden), dim3(256), 0, st, s);
   }
   return check_launch("pt_linear_cross_entropy");
+}
+
+template <typename T, int BM>
+int scores(const Scores& s, dim3 grid, dim3 parts, dim3 finish, bool may_split, hipStream_t st) {
+  constexpr size_t lds = Product<T, false, false, BM>::kLds;
+  constexpr int threads = Product<T, false, false, BM>::kThreads;
+  if (int rc = allow(scores_kernel<T, BM>, lds)) return rc;
+  hipLaunchKernelGGL((scores_kernel<T, BM>), grid, dim3(threads), lds, st, s);
+  if (may_split) {
+    if (int rc = allow(parts_scores_kernel<T, BM>, lds)) return rc;
+    hipLaunchKernelGGL((parts_scores_kernel<T, BM>), parts, dim3(threads), lds, st, s);
+    hipLaunchKernelGGL((finish_kernel<T, BM>), finish, dim3(256), 0, st, s);
+  }
+  return PT_OK;
 }
 
 template <typename T>  // of the inputs
@@ -1216,9 +1390,14 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     lay.w_rows = vocab;
     ow = rows_operand(lay.to_w, p.width, vocab * p.width, vocab * p.width * 2);
   }
+  const int tiles_v = static_cast<int>(p.words / kTile), tiles_h = static_cast<int>(up(hidden, kTile) / kTile);
+  const int rounds = p.fp32 ? 3 : 1, few_rows = p.rows <= kFewRows ? kFewRows : kTile;
+  const int64_t word_steps = up(vocab, kStep) / kStep;
+  const Splits splits{p.narrow ? static_cast<int>(p.width) : 0, p.chunk, few_rows, tiles_v, tiles_h, static_cast<int>(p.width / kStep),
+                      static_cast<int>(word_steps), rounds, vocab, p.parts_s, p.parts_x, p.parts_w};
   const int64_t lay_rows = lay.x_rows + lay.dx_rows + lay.w_rows;
   const bool small = lay_rows <= kSmallRows && lay_rows * p.width <= kSmallElements;
-  hipLaunchKernelGGL(keep_kernel<T>, dim3(1), dim3(1024), 0, st, r, small ? lay : Lay{}, vocab, reduction, row_of, label_of,
+  hipLaunchKernelGGL(keep_kernel<T>, dim3(1), dim3(1024), 0, st, r, small ? lay : Lay{}, splits, vocab, reduction, row_of, label_of,
                      reinterpret_cast<float*>(ws + p.weight_of), meta, losses);
   if (!small) {
     if constexpr (Split<T>::kSplit) {
@@ -1250,12 +1429,10 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       return check_launch("pt_linear_cross_entropy");
     }
   }
-  const int tiles_v = static_cast<int>(p.words / kTile), tiles_h = static_cast<int>(up(hidden, kTile) / kTile);
-  const int tiles_r = static_cast<int>(p.chunk / kTile);
   constexpr size_t lds = Product<T, false, false>::kLds;
-  if (int rc = allow(scores_kernel<T, kTile>, lds)) return rc;
   if (int rc = allow(gradient_kernel<T, false>, lds)) return rc;
   if (int rc = allow(gradient_kernel<T, true>, lds)) return rc;
+  float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);
   auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>(up(tiles, 8))); };
 
   for (int64_t c = 0; c < p.chunks; ++c) {
@@ -1263,14 +1440,13 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     const int64_t rows_most = p.rows - first < p.chunk ? p.rows - first : p.chunk;
     _Float16* e = p.grads ? reinterpret_cast<_Float16*>(ws + p.e) : nullptr;
     Scores s{ox,    ow, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, p.chunk * p.words,
-             sums,  p.padded, target};
-    if (p.rows <= kFewRows) {
-      constexpr size_t few = Product<T, false, false, kFewRows>::kLds;
-      if (int rc = allow(scores_kernel<T, kFewRows>, few)) return rc;
-      hipLaunchKernelGGL((scores_kernel<T, kFewRows>), grid(tiles_v), dim3(256), few, st, s);
-    } else {
-      hipLaunchKernelGGL((scores_kernel<T, kTile>), grid(static_cast<int64_t>(tiles_r) * tiles_v), dim3(512), lds, st, s);
-    }
+             sums,  p.padded, target, parts};
+    const bool few = p.rows <= kFewRows;
+    const int64_t tiles_s = p.chunk / few_rows * tiles_v;
+    const dim3 finish(static_cast<unsigned>(tiles_v), static_cast<unsigned>((rows_most + 15) / 16));
+    if (int rc = few ? scores<T, kFewRows>(s, grid(tiles_s), grid(p.parts_s), finish, p.parts_s > 0, st)
+                     : scores<T, kTile>(s, grid(tiles_s), grid(p.parts_s), finish, p.parts_s > 0, st))
+      return rc;
     hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows_most + 31) / 32)), dim3(1024), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
@@ -1278,11 +1454,8 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>(tiles_v), static_cast<unsigned>(slope_rows)), dim3(256), 0, st, e,
                        p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
     const int64_t plane = p.chunk * p.words;
-    const int rounds = p.fp32 ? 3 : 1;
-    const int64_t word_steps = up(vocab, kStep) / kStep;
-    float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);
     if (dx != nullptr) {
-      Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), rounds, p.parts_x, top_w, {}};
+      Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), kSplitX, top_w, {}};
       d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
       hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
       if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
@@ -1290,7 +1463,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     if (dw != nullptr) {
       const Operand oxc = columns_operand(x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2);
       const int how = p.chunks == 1 ? kFinal : (c + 1 == p.chunks ? kAddFinal : kAdd);
-      Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, rounds, p.parts_w, top_x, {}};
+      Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, kSplitW, top_x, {}};
       d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts)};
       hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
       if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel, join_grid(vocab, hidden), dim3(256), 0, st, d);
@@ -1342,8 +1515,8 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
   const bool grads = dx != nullptr || dw != nullptr;
   if (grads && grad_dtype != dtype && grad_dtype != PT_FLOAT32)
     return pt::fail(PT_EINVAL, name + ": gradients are of the inputs' type, or fp32");
-  if (grads && (reduction == PT_REDUCTION_NONE) != (dloss != nullptr))
-    return pt::fail(PT_EINVAL, name + ": the tokens' weights belong to the gradients of a loss without a reduction");
+  if (grads && reduction == PT_REDUCTION_NONE && dloss == nullptr)
+    return pt::fail(PT_EINVAL, name + ": the gradients of a loss without a reduction need the tokens' weights");
   if (!grads && dloss != nullptr) return pt::fail(PT_EINVAL, name + ": weights without gradients");
   if (dx_inner < inner || outer * dx_inner > (int64_t{1} << 30)) return pt::fail(PT_EINVAL, name + ": dx has too few rows, or over 2^30");
   if (weight == nullptr || (rows > 0 && (x == nullptr || labels == nullptr)) || workspace == nullptr || (loss == nullptr && !grads && rows > 0))
@@ -1356,8 +1529,9 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
   const pt::Plan plan = pt::plan_for(rows, vocab, hidden, weight, weight_stride, dtype, dx != nullptr, dw != nullptr, chunk_rows);
   if (workspace_bytes < plan.total) return pt::fail(PT_EINVAL, name + ": workspace too small");
   if (rows == 0 && outer * dx_inner == 0 && dw == nullptr && (loss == nullptr || reduction == PT_REDUCTION_NONE)) return pt::ok();
+  const bool each = reduction == PT_REDUCTION_NONE;
   const pt::Rows r{x, x_outer_stride, x_inner_stride, labels, label_outer_stride, label_inner_stride, outer, inner, ignore_index,
-                   dloss, dloss_outer_stride, dloss_inner_stride, dx_inner > 0 ? dx_inner : 1};
+                   each ? dloss : nullptr, dloss_outer_stride, dloss_inner_stride, dx_inner > 0 ? dx_inner : 1, each ? nullptr : dloss};
   char* ws = static_cast<char*>(workspace);
   hipStream_t st = pt::as_stream(stream);
   switch (dtype) {

@@ -23,17 +23,20 @@ constexpr int kNarrowInner = 64;    // rows of the inner side a step
 // rows are short) take the fewest steps, a part counting for two more.  All parts together are at most kNarrowParts tiles.
 constexpr int64_t kNarrowParts = 1024;
 __host__ __device__ inline int narrow_splits(int64_t outer_tiles, int64_t inner_steps, int hp) {
-  const int64_t at_once = hp == 32 ? 1024 : 512;
-  int best = 1;
-  int64_t least = (outer_tiles + at_once - 1) / at_once * inner_steps;
-  for (int s = 2; s <= 1024 && s * outer_tiles <= kNarrowParts && s * 4 <= inner_steps; s = s < 8 ? s + 1 : s * 5 / 4) {
-    const int64_t t = (outer_tiles * s + at_once - 1) / at_once * ((inner_steps + s - 1) / s + 2);
-    if (t < least) {
+  if (outer_tiles * 2 > kNarrowParts || outer_tiles < 1) return 1;
+  const unsigned tiles = static_cast<unsigned>(outer_tiles), steps = static_cast<unsigned>(inner_steps);
+  const unsigned at_once = hp == 32 ? 1024 : 512;
+  constexpr unsigned kTry[] = {2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 26, 32, 40, 52, 64, 80, 104, 128, 160, 208, 256, 320, 416, 512, 1024};
+  unsigned best = 1, least = (tiles + at_once - 1) / at_once * steps;
+#pragma unroll
+  for (unsigned s : kTry) {
+    const unsigned t = (tiles * s + at_once - 1) / at_once * ((steps + s - 1) / s + 2);
+    if (s * tiles <= kNarrowParts && s * 4 <= steps && t < least) {
       least = t;
       best = s;
     }
   }
-  return best;
+  return static_cast<int>(best);
 }
 
 // The steps of a tile of the inner side, HP elements a row, in LDS: 16-byte chunks permuted by bits of the row.

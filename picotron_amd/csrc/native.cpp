@@ -1027,7 +1027,7 @@ HeadOut head_call(const at::Tensor& x, const at::Tensor& w, const at::Tensor& t,
               in(x), deep ? x.stride(0) : 0, x.stride(x.dim() - 2), outer, inner, in(w), w.stride(0), vocab, hidden,
               static_cast<const int64_t*>(in(t)) + (c.shift ? tsi : 0), tso, tsi, c.ignore, static_cast<int>(c.reduction),
               want_loss ? static_cast<float*>(out(o.loss)) : nullptr, grad.defined() ? static_cast<const float*>(in(grad)) : nullptr,
-              grad.defined() && deep ? grad.stride(0) : 0, grad.defined() ? grad.stride(grad.dim() - 1) : 0, want_dx ? out(o.dx) : nullptr, seq,
+              grad.defined() && grad.dim() == 2 ? grad.stride(0) : 0, grad.defined() && grad.dim() > 0 ? grad.stride(grad.dim() - 1) : 0, want_dx ? out(o.dx) : nullptr, seq,
               want_dw ? out(o.dw) : nullptr, type == at::kFloat ? PT_FLOAT32 : code_of(x), out(ws), static_cast<size_t>(ws.numel()), c.chunk, code_of(x),
               reinterpret_cast<void*>(c.stream)));
   return o;
@@ -1072,12 +1072,18 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
   }
 };
 
-struct HeadTokens : torch::autograd::Function<HeadTokens> {
+// As ops.head_defers.
+bool head_defers(const at::Tensor& x, const HeadCall& c) {
+  return c.reduction == PT_REDUCTION_NONE || (x.scalar_type() == at::kHalf && x.numel() / x.size(-1) <= 512);
+}
+
+struct HeadDeferred : torch::autograd::Function<HeadDeferred> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& t, const HeadCall& c) {
     ctx->save_for_backward({x, w, t});
     auto& kept = ctx->saved_data;
     kept["shift"] = c.shift;
     kept["ignore"] = c.ignore;
+    kept["reduction"] = c.reduction;
     kept["chunk"] = c.chunk;
     kept["stream"] = c.stream;
     return head_call(x, w, t, c, true, false, false, at::Tensor(), x.scalar_type()).loss;
@@ -1086,7 +1092,7 @@ struct HeadTokens : torch::autograd::Function<HeadTokens> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the fused head's cross-entropy is differentiable once (create_graph=True)");
     const variable_list saved = ctx->get_saved_variables();
     auto& kept = ctx->saved_data;
-    const HeadCall c{kept["shift"].toBool(), kept["ignore"].toInt(), PT_REDUCTION_NONE, kept["chunk"].toInt(), kept["stream"].toInt()};
+    const HeadCall c{kept["shift"].toBool(), kept["ignore"].toInt(), kept["reduction"].toInt(), kept["chunk"].toInt(), kept["stream"].toInt()};
     const at::Tensor grad = grads[0].to(at::kFloat);
     const HeadOut o = head_call(saved[0], saved[1], saved[2], c, false, ctx->needs_input_grad(0), ctx->needs_input_grad(1), grad, saved[0].scalar_type());
     return {o.dx, o.dw, at::Tensor(), at::Tensor()};
@@ -1107,8 +1113,8 @@ PT_FN(linear_cross_entropy_node, 9)
   const bool graph = a[7] == Py_True;
   NoGil nogil;
   const at::Tensor o = !graph ? head_call(*x, *w, *t, c, true, false, false, at::Tensor(), x->scalar_type()).loss
-                       : c.reduction == PT_REDUCTION_NONE ? HeadTokens::apply(*x, *w, *t, c)
-                                                          : HeadLoss::apply(*x, *w, *t, c);
+                       : head_defers(*x, c) ? HeadDeferred::apply(*x, *w, *t, c)
+                                            : HeadLoss::apply(*x, *w, *t, c);
   nogil.end();
   return wrap(o);
 PT_END

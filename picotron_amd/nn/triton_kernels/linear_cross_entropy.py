@@ -10,7 +10,7 @@ backward).  The backward multiplies them by what arrives from above, on the devi
 They are handed out once: a second backward through the same graph raises.
 
 With ``reduction="none"`` each token's loss comes back and takes a gradient of its own; the forward then keeps its inputs,
-and the backward forms the softmax again.
+and the backward forms the softmax again.  So does the loss of up to 512 fp16 states.
 
 Ignored tokens cost nothing: their rows take no part in any product, may hold anything, and get zeros as their gradient.
 A label outside the vocabulary gives NaN, in the loss and the gradients it enters (PICOTRON_HIP_CE_CHECK=1 raises
@@ -62,7 +62,7 @@ class _ReducedLoss(torch.autograd.Function):
         return dx, dw, None, None
 
 
-class _TokenLosses(torch.autograd.Function):
+class _DeferredLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden: Tensor, weight: Tensor, labels: Tensor, how: dict):  # type: ignore[override]
         ctx.save_for_backward(hidden, weight, labels)
@@ -142,7 +142,7 @@ def _linear_cross_entropy(
     how = dict(shift=bool(shift), ignore_index=int(ignore_index), reduction=reduction, chunk_tokens=chunk_tokens or 0)
     if plain:
         return ops.linear_cross_entropy(hidden, weight, labels, **how)[0]
-    return (_TokenLosses if reduction == "none" else _ReducedLoss).apply(hidden, weight, labels, how)
+    return (_DeferredLoss if ops.head_defers(hidden, reduction) else _ReducedLoss).apply(hidden, weight, labels, how)
 
 
 _outside_graphs = torch.compiler.disable(_linear_cross_entropy)

@@ -75,7 +75,7 @@ def check(loss, dx, dw, x, w, t, factors, scale=1.0, reduction="none", ignore=-1
 
 
 SIZES = [(1, 1, 1), (1, 64, 260), (2, 20, 257), (33, 32, 64), (255, 64, 256), (256, 128, 255), (300, 100, 1000), (513, 200, 1027),
-         (1100, 72, 3001), (700, 520, 130), (5, 192, 64), (1030, 160, 2100), (70, 129, 70000)]
+         (1100, 72, 3001), (700, 520, 130), (5, 192, 64), (1030, 160, 2100), (70, 129, 70000), (12, 2000, 168), (300, 1100, 90)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

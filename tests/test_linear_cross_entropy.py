@@ -110,7 +110,6 @@ def call(**change):
     (dict(dx=256, grad_dtype=1), _lib.PT_EINVAL),
     (dict(dx=264), _lib.PT_EINVAL),
     (dict(dx=256, reduction=2), _lib.PT_EINVAL),
-    (dict(dx=256, dloss=256), _lib.PT_EINVAL),
     (dict(dloss=256, reduction=2), _lib.PT_EINVAL),
     (dict(x=258), _lib.PT_EINVAL),
     (dict(outer=1 << 20, inner=1 << 20, dx_inner=1 << 20), _lib.PT_EUNSUPPORTED),
