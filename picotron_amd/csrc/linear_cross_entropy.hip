@@ -30,7 +30,8 @@ namespace {
 constexpr float kScale = 16384.0f;  // of exp(l - m) and G in 16 bits
 constexpr int kTile = 256;
 constexpr int64_t kChunkBytes = int64_t{1} << 31;
-constexpr int64_t kScoreRows = 65536;  // rows of a chunk that only leaves sums
+constexpr int64_t kSumsBytes = int64_t{1} << 28;  // of the tiles' sums of a chunk that leaves nothing else
+constexpr int64_t kMostRows = int64_t{1} << 24;   // a launch has fewer than 2^32 work-items, and a row is a wave's
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -1238,7 +1239,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   p.copy_weight = p.fp32 || hidden != p.width || ldw % 8 != 0 || !aligned16(w);
   const int64_t each = p.grads ? 2 * p.planes * p.words : 0;
   const int64_t all = up(rows > 0 ? rows : 1, kTile);
-  int64_t most = p.narrow ? all : p.grads ? kChunkBytes / each / kTile * kTile : kScoreRows;
+  int64_t most = p.narrow ? all : p.grads ? kChunkBytes / each / kTile * kTile : kSumsBytes / (p.words / kTile * static_cast<int64_t>(sizeof(f32x2))) / kTile * kTile;
   if (most < kTile) most = kTile;
   if (!p.narrow && chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
   p.chunks = rows > 0 ? (rows + most - 1) / most : 1;
@@ -1481,8 +1482,8 @@ int check_sizes(const char* fn, int64_t rows, int64_t vocab, int64_t hidden, int
   if (rows < 0 || vocab < 1 || hidden < 1) return fail(PT_EINVAL, name + ": bad sizes");
   if (ldw < hidden) return fail(PT_EINVAL, name + ": the weight's rows overlap");
   // byte offsets inside a tile are 32-bit
-  if (rows > (int64_t{1} << 30) || vocab > (int64_t{1} << 21) || hidden > (int64_t{1} << 20) || ldw > (int64_t{1} << 21))
-    return fail(PT_EUNSUPPORTED, name + ": at most 2^30 rows, 2^21 words, 2^20 wide, 2^21 elements between the weight's rows");
+  if (rows > kMostRows || vocab > (int64_t{1} << 21) || hidden > (int64_t{1} << 20) || ldw > (int64_t{1} << 21))
+    return fail(PT_EUNSUPPORTED, name + ": at most 2^24 rows, 2^21 words, 2^20 wide, 2^21 elements between the weight's rows");
   return PT_OK;
 }
 
@@ -1506,8 +1507,8 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
   const char* fn = "pt_linear_cross_entropy";
   const std::string name(fn);
   if (outer < 0 || inner < 0) return pt::fail(PT_EINVAL, name + ": bad sizes");
-  if (outer > (int64_t{1} << 30) || inner > (int64_t{1} << 30) || outer * inner > (int64_t{1} << 30) || dx_inner > (int64_t{1} << 30))
-    return pt::fail(PT_EUNSUPPORTED, name + ": at most 2^30 rows");
+  if (outer > pt::kMostRows || inner > pt::kMostRows || outer * inner > pt::kMostRows || dx_inner > pt::kMostRows)
+    return pt::fail(PT_EUNSUPPORTED, name + ": at most 2^24 rows");
   const int64_t rows = outer * inner;
   if (int rc = pt::check_sizes(fn, rows, vocab, hidden, weight_stride, dtype)) return rc;
   if (reduction != PT_REDUCTION_MEAN && reduction != PT_REDUCTION_SUM && reduction != PT_REDUCTION_NONE)
@@ -1518,13 +1519,13 @@ int pt_linear_cross_entropy(const void* x, int64_t x_outer_stride, int64_t x_inn
   if (grads && reduction == PT_REDUCTION_NONE && dloss == nullptr)
     return pt::fail(PT_EINVAL, name + ": the gradients of a loss without a reduction need the tokens' weights");
   if (!grads && dloss != nullptr) return pt::fail(PT_EINVAL, name + ": weights without gradients");
-  if (dx_inner < inner || outer * dx_inner > (int64_t{1} << 30)) return pt::fail(PT_EINVAL, name + ": dx has too few rows, or over 2^30");
+  if (dx_inner < inner || outer * dx_inner > pt::kMostRows) return pt::fail(PT_EINVAL, name + ": dx has too few rows, or over 2^24");
   if (weight == nullptr || (rows > 0 && (x == nullptr || labels == nullptr)) || workspace == nullptr || (loss == nullptr && !grads && rows > 0))
     return pt::fail(PT_EINVAL, name + ": null pointer");
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return pt::fail(PT_EINVAL, name + ": the workspace must be aligned to 256 bytes");
-  const int size = pt::dtype_size(dtype), grad_size = pt::dtype_size(grad_dtype);
+  const int size = pt::dtype_size(dtype);
   if (reinterpret_cast<uintptr_t>(x) % size != 0 || reinterpret_cast<uintptr_t>(weight) % size != 0 ||
-      (grads && (reinterpret_cast<uintptr_t>(dx) % (4 * grad_size) != 0 || reinterpret_cast<uintptr_t>(dw) % (4 * grad_size) != 0)))
+      (grads && (!pt::aligned16(dx) || !pt::aligned16(dw))))
     return pt::fail(PT_EINVAL, name + ": misaligned pointer");
   const pt::Plan plan = pt::plan_for(rows, vocab, hidden, weight, weight_stride, dtype, dx != nullptr, dw != nullptr, chunk_rows);
   if (workspace_bytes < plan.total) return pt::fail(PT_EINVAL, name + ": workspace too small");

@@ -338,28 +338,54 @@ inline int64_t part_rows(int64_t rows, int64_t cols) {
   return bwd_grid(rows, s) * (kThreads / s.lanes);
 }
 
+// A launch has fewer than 2^32 work-items: 2^22 rows at a time of kernels with a grid over all rows.
+constexpr int64_t kMostRows = int64_t{1} << 22;
+
+// The rows from `first` on, as many as a launch takes.
+template <typename T>
+Norm8 rows_of(const Norm8& whole, int64_t first) {
+  Norm8 a = whole;
+  const int64_t bytes = first * a.cols * static_cast<int64_t>(sizeof(T));
+  a.x = static_cast<const char*>(a.x) + bytes;
+  if (a.extra != nullptr) a.extra = static_cast<const char*>(a.extra) + bytes;
+  if (a.h != nullptr) a.h = static_cast<char*>(a.h) + bytes;
+  if (a.y != nullptr) a.y = static_cast<char*>(a.y) + bytes;
+  a.rstd += first;
+  a.codes += first * a.blocks * 16;
+  a.steps += first * a.blocks;
+  a.rows = whole.rows - first < kMostRows ? whole.rows - first : kMostRows;
+  return a;
+}
+
 template <typename T, bool ADD, bool ALIGNED, bool NT>
-int launch_fwd8(const Norm8& a, hipStream_t st) {
-  const Shape s = shape_of(a.cols);
-  const int64_t per = kThreads / s.lanes;
-  const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per));
+int launch_fwd8(const Norm8& whole, hipStream_t st) {
+  const Shape s = shape_of(whole.cols);
+  for (int64_t first = 0; first < whole.rows; first += kMostRows) {
+    const Norm8 a = rows_of<T>(whole, first);
+    const int64_t per = kThreads / s.lanes;
+    const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per));
 #define PT_NORM8(L, V) hipLaunchKernelGGL((norm8_fwd_kernel<T, L, V, ADD, ALIGNED, NT>), grid, dim3(kThreads), 0, st, a)
-  if (s.vpl == 0) hipLaunchKernelGGL((norm8_long_fwd_kernel<T, ADD>), grid, dim3(kThreads), 0, st, a);
-  else if (s.lanes == 16) PT_NORM8(16, 1);
-  else if (s.lanes == 64) PT_NORM8(64, 1);
-  else if (s.vpl == 1) PT_NORM8(kThreads, 1);
-  else if (s.vpl == 2) PT_NORM8(kThreads, 2);
-  else if (s.vpl == 4) PT_NORM8(kThreads, 4);
-  else PT_NORM8(kThreads, 8);
+    if (s.vpl == 0) hipLaunchKernelGGL((norm8_long_fwd_kernel<T, ADD>), grid, dim3(kThreads), 0, st, a);
+    else if (s.lanes == 16) PT_NORM8(16, 1);
+    else if (s.lanes == 64) PT_NORM8(64, 1);
+    else if (s.vpl == 1) PT_NORM8(kThreads, 1);
+    else if (s.vpl == 2) PT_NORM8(kThreads, 2);
+    else if (s.vpl == 4) PT_NORM8(kThreads, 4);
+    else PT_NORM8(kThreads, 8);
 #undef PT_NORM8
-  return check_launch("pt_rmsnorm8_fwd");
+    if (int rc = check_launch("pt_rmsnorm8_fwd")) return rc;
+  }
+  return ok();
 }
 
 template <typename T, bool ADD, bool ALIGNED, bool NT>
 int launch_bwd8(const Norm8& a, void* dw, hipStream_t st) {
   const Shape s = shape_of(a.cols);
   if (s.vpl == 0) {
-    if (a.y != nullptr) hipLaunchKernelGGL((norm8_long_bwd_kernel<T, ADD>), dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, st, a);
+    for (int64_t first = 0; a.y != nullptr && first < a.rows; first += kMostRows) {
+      const Norm8 part = rows_of<T>(a, first);
+      hipLaunchKernelGGL((norm8_long_bwd_kernel<T, ADD>), dim3(static_cast<unsigned>(part.rows)), dim3(kThreads), 0, st, part);
+    }
     if (dw != nullptr) {
       const int parts = static_cast<int>(part_rows(a.rows, a.cols));
       hipLaunchKernelGGL(norm8_long_dw_kernel<T>, dim3(static_cast<unsigned>((a.cols + kThreads * kUnit - 1) / (kThreads * kUnit)), parts),

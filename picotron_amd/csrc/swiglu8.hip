@@ -82,6 +82,9 @@ __global__ __launch_bounds__(256) void swiglu8_bwd_kernel(const T* __restrict__ 
   }
 }
 
+// A launch has fewer than 2^32 work-items: 2^30 units, 2^33 elements, at a time.
+constexpr int64_t kMostElements = int64_t{1} << 33;
+
 template <typename T>
 int fwd8(const void* g, const void* u, void* o, void* codes, float* steps, int64_t n, hipStream_t st) {
   const bool aligned = aligned16(g) && aligned16(u) && aligned16(o);
@@ -149,11 +152,17 @@ int pt_swiglu8_fwd(const void* gate, const void* up, void* out, void* codes, flo
   if (n == 0) return pt::ok();
   if (gate == nullptr || up == nullptr || out == nullptr) return pt::fail(PT_EINVAL, std::string(fn) + ": null pointer");
   hipStream_t st = pt::as_stream(stream);
-  switch (dtype) {
-    case PT_FLOAT32: return pt::fwd8<float>(gate, up, out, codes, steps, n, st);
-    case PT_FLOAT16: return pt::fwd8<_Float16>(gate, up, out, codes, steps, n, st);
-    default: return pt::fwd8<__bf16>(gate, up, out, codes, steps, n, st);
+  for (int64_t at = 0; at < n; at += pt::kMostElements) {
+    const int64_t part = n - at < pt::kMostElements ? n - at : pt::kMostElements, bytes = at * pt::dtype_size(dtype);
+    const char *g = static_cast<const char*>(gate) + bytes, *u = static_cast<const char*>(up) + bytes;
+    char *o = static_cast<char*>(out) + bytes, *c = static_cast<char*>(codes) + at * 2;
+    float* s = steps + at / pt::block8::kBlock * 2;
+    const int rc = dtype == PT_FLOAT32 ? pt::fwd8<float>(g, u, o, c, s, part, st)
+                   : dtype == PT_FLOAT16 ? pt::fwd8<_Float16>(g, u, o, c, s, part, st)
+                                         : pt::fwd8<__bf16>(g, u, o, c, s, part, st);
+    if (rc != PT_OK) return rc;
   }
+  return pt::ok();
 }
 
 int pt_swiglu8_bwd(const void* dout, const void* codes, const float* steps, void* dgate, void* dup, int64_t n, int dtype, void* stream) {
@@ -162,11 +171,17 @@ int pt_swiglu8_bwd(const void* dout, const void* codes, const float* steps, void
   if (n == 0 || (dgate == nullptr && dup == nullptr)) return pt::ok();
   if (dout == nullptr) return pt::fail(PT_EINVAL, std::string(fn) + ": null pointer");
   hipStream_t st = pt::as_stream(stream);
-  switch (dtype) {
-    case PT_FLOAT32: return pt::bwd8<float>(dout, codes, steps, dgate, dup, n, st);
-    case PT_FLOAT16: return pt::bwd8<_Float16>(dout, codes, steps, dgate, dup, n, st);
-    default: return pt::bwd8<__bf16>(dout, codes, steps, dgate, dup, n, st);
+  for (int64_t at = 0; at < n; at += pt::kMostElements) {
+    const int64_t part = n - at < pt::kMostElements ? n - at : pt::kMostElements, bytes = at * pt::dtype_size(dtype);
+    const char *d = static_cast<const char*>(dout) + bytes, *c = static_cast<const char*>(codes) + at * 2;
+    char *g = dgate == nullptr ? nullptr : static_cast<char*>(dgate) + bytes, *u = dup == nullptr ? nullptr : static_cast<char*>(dup) + bytes;
+    const float* s = steps + at / pt::block8::kBlock * 2;
+    const int rc = dtype == PT_FLOAT32 ? pt::bwd8<float>(d, c, s, g, u, part, st)
+                   : dtype == PT_FLOAT16 ? pt::bwd8<_Float16>(d, c, s, g, u, part, st)
+                                         : pt::bwd8<__bf16>(d, c, s, g, u, part, st);
+    if (rc != PT_OK) return rc;
   }
+  return pt::ok();
 }
 
 }  // extern "C"

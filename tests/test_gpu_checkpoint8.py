@@ -332,3 +332,22 @@ def test_large_swiglu(gpu):
         assert torch.equal(a, y[part])
         for p, q in zip(ops.swiglu8_bwd(g[part].clone(), c, s, torch.bfloat16), (dg, du)):
             assert torch.equal(p, q[part])
+
+
+def test_many_rows(gpu):
+    """More rows than one launch of the forward takes."""
+
+    rows, cols = (1 << 22) + 5, 24
+    x = randn((rows, cols), torch.bfloat16, gpu, 1)
+    w = randn((cols,), torch.float32, gpu, 2)
+    _, y, rstd, codes, steps = ops.rmsnorm8_fwd(x, w, EPS, x)
+    dx, dw = ops.rmsnorm8_bwd(x, w, rstd, codes, steps, torch.bfloat16, x)
+    for part in (slice(0, 40), slice((1 << 22) - 20, rows)):
+        p = x[part].clone()
+        _, y1, r1, c1, s1 = ops.rmsnorm8_fwd(p, w, EPS, p)
+        assert torch.equal(y1, y[part]) and torch.equal(r1, rstd[part]) and torch.equal(c1, codes[part]) and torch.equal(s1, steps[part])
+        assert torch.equal(ops.rmsnorm8_bwd(p, w, r1, c1, s1, torch.bfloat16, p)[0], dx[part])
+    kept = _block8.decode(codes[:, :, None].view(rows, 1, 128), steps[..., None], cols).double() * rstd.double()[:, None]
+    want, total = (x.double() * kept).sum(0), (x.double() * kept).abs().sum(0)
+    # each slot adds up some thousands of rows one after the other, in fp32
+    assert torch.all((dw.double() - want).abs() <= 2.0**-24 * (rows // 8192 + 40) * total)

@@ -459,3 +459,33 @@ def test_refusals(gpu):
         triton_linear_cross_entropy(x, w, t, shift=True)
     with pytest.raises(ValueError):
         ops.linear_cross_entropy(x, w, t, reduction="none", want_dx=True, grad_losses=torch.ones(9, device=gpu))
+
+
+def test_between_the_graphs_of_a_compiled_model(gpu):
+    x, w, t = make(90, 64, 300, torch.float32, gpu)
+    layer = torch.nn.Linear(64, 64, bias=False).to(gpu)
+
+    def loss_of():
+        return triton_linear_cross_entropy(layer(x).relu(), w, t)
+
+    outs = []
+    torch._dynamo.reset()
+    for f in (loss_of, torch.compile(loss_of, backend="aot_eager")):
+        layer.zero_grad()
+        loss = f()
+        loss.backward()
+        outs.append((loss.detach(), layer.weight.grad.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_many_tokens_without_gradients(gpu):
+    """More tokens than a chunk of sums takes, at a vocabulary whose tiles make that few."""
+
+    n, h, v = 700, 160, 300000
+    x, w, t = make(n, h, v, torch.bfloat16, gpu, ignored=0.2)
+    whole = triton_linear_cross_entropy(x, w, t, reduction="none")
+    parts = triton_linear_cross_entropy(x, w, t, reduction="none", chunk_tokens=256)
+    assert torch.equal(whole, parts)
+    want = torch.nn.functional.cross_entropy(x.double() @ w.double().t(), t, reduction="none")
+    slack = (h + 8) * 2.0**-24 * float((x.double().abs() @ w.double().abs().t()).max()) + 2.0**-22
+    assert torch.all((whole.double() - want).abs() <= 2 * slack + 2.0**-20 * (1 + want.abs()))

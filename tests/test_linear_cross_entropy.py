@@ -113,6 +113,7 @@ def call(**change):
     (dict(dloss=256, reduction=2), _lib.PT_EINVAL),
     (dict(x=258), _lib.PT_EINVAL),
     (dict(outer=1 << 20, inner=1 << 20, dx_inner=1 << 20), _lib.PT_EUNSUPPORTED),
+    (dict(inner=(1 << 24) + 1, dx_inner=(1 << 24) + 1), _lib.PT_EUNSUPPORTED),
     (dict(vocab=(1 << 21) + 1), _lib.PT_EUNSUPPORTED),
     (dict(hidden=(1 << 20) + 1, ldw=(1 << 20) + 1), _lib.PT_EUNSUPPORTED),
     (dict(ldw=(1 << 21) + 1), _lib.PT_EUNSUPPORTED),
