@@ -1,6 +1,7 @@
 // Activations held in 8 bits: blocks of 128 elements that share a step.
 //
-//   top = max |x|,  inv = 127 / top,  code = 128 + round(x * inv),  step = top / 127,  value = (code - 128) * step
+//   top = max |x|,  inv = 127 / top,  code = 128 + round(x * inv),  step = top / 127 (of the largest float, one ulp less, so that
+//   127 steps are finite),  value = (code - 128) * step
 //
 // A block whose top is below 2^-100 is held as zeros, one with an infinity or a NaN comes back as NaN (its step is).
 // Every quotient and product is the correctly rounded one of 32 bits, so that the codes of given elements are the same
@@ -95,11 +96,12 @@ __device__ __forceinline__ unsigned row16_max(unsigned v) {
 struct Step {
   float step, inv;
 };
+constexpr float kMostStep = 0x1.020406p+121f;  // the largest whose 127th multiple is finite
 __device__ __forceinline__ Step step_of(unsigned top_bits) {
   const float top = __builtin_bit_cast(float, top_bits);
   if (top_bits >= 0x7f800000u) return {NAN, 0.f};
   if (top < 0x1p-100f) return {0.f, 0.f};
-  return {top / 127.f, 127.f / top};
+  return {fminf(top / 127.f, kMostStep), 127.f / top};
 }
 
 // The codes of a unit, a byte each.  Adding 1.5 * 2^23 + 128 rounds to the nearest whole number (ties to even) and leaves
@@ -122,10 +124,11 @@ __device__ __forceinline__ u32x2 encode(const Unit<T>& x, float inv) {
   return out;
 }
 
-// Element i of a unit: code * step - 128 * step, whose fused form is the product of the code less 128 and the step, rounded once.
+// Element i of a unit.  Not as one multiply-add of the code and -128 steps, which overflow where the block's largest is within
+// 1/128 of the largest float, as a mask of the type's lowest value is.
 __device__ __forceinline__ float decode(u32x2 codes, int i, float step) {
   const unsigned b = (codes[i / 4] >> (8 * (i % 4))) & 255u;
-  return __builtin_fmaf(static_cast<float>(b), step, -128.f * step);
+  return (static_cast<float>(b) - 128.f) * step;
 }
 
 }  // namespace block8

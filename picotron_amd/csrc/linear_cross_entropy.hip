@@ -32,6 +32,7 @@ constexpr int kTile = 256;
 constexpr int64_t kChunkBytes = int64_t{1} << 31;
 constexpr int64_t kSumsBytes = int64_t{1} << 28;  // of the tiles' sums of a chunk that leaves nothing else
 constexpr int64_t kMostRows = int64_t{1} << 24;   // a launch has fewer than 2^32 work-items, and a row is a wave's
+constexpr int64_t kMostChunk = int64_t{1} << 19;  // rows of a chunk: a grid's y ends at 65535, and finish_kernel takes 16 rows each
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -1241,6 +1242,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   const int64_t all = up(rows > 0 ? rows : 1, kTile);
   int64_t most = p.narrow ? all : p.grads ? kChunkBytes / each / kTile * kTile : kSumsBytes / (p.words / kTile * static_cast<int64_t>(sizeof(f32x2))) / kTile * kTile;
   if (most < kTile) most = kTile;
+  if (!p.narrow && most > kMostChunk) most = kMostChunk;
   if (!p.narrow && chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
   p.chunks = rows > 0 ? (rows + most - 1) / most : 1;
   p.chunk = up((rows + p.chunks - 1) / p.chunks, kTile);
@@ -1438,7 +1440,8 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
 
   for (int64_t c = 0; c < p.chunks; ++c) {
     const int64_t first = c * p.chunk;
-    const int64_t rows_most = p.rows - first < p.chunk ? p.rows - first : p.chunk;
+    const int64_t rows_left = p.rows > first ? p.rows - first : 1;  // a call without rows launches its grids too
+    const int64_t rows_most = rows_left < p.chunk ? rows_left : p.chunk;
     _Float16* e = p.grads ? reinterpret_cast<_Float16*>(ws + p.e) : nullptr;
     Scores s{ox,    ow, meta, label_of, first, p.chunk, vocab, tiles_v, static_cast<int>(p.width / kStep), e, p.chunk * p.words,
              sums,  p.padded, target, parts};

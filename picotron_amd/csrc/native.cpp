@@ -145,7 +145,7 @@ struct Rows {
 // x contiguous rows and a contiguous 1-D weight of their length.
 bool norm_rows(const at::Tensor* x, const at::Tensor* w, Rows* r) {
   if (x == nullptr || w == nullptr || x->dim() < 1 || w->dim() != 1 || !x->is_contiguous() ||
-      !w->is_contiguous() || !same_place(*x, *w))
+      !w->is_contiguous() || !same_place(*x, *w) || x->size(-1) < 1)
     return false;
   r->cols = x->size(-1);
   r->rows = x->numel() / r->cols;
@@ -1106,7 +1106,7 @@ PT_FN(linear_cross_entropy_node, 9)
   c.shift = a[3] == Py_True;
   if (x == nullptr || w == nullptr || t == nullptr || code_of(*x) < 0 || x->scalar_type() != w->scalar_type() || t->scalar_type() != at::kLong ||
       !same_place(*x, *w) || !same_place(*x, *t) || (x->dim() != 2 && x->dim() != 3) || w->dim() != 2 || w->size(1) != x->size(-1) ||
-      x->stride(-1) != 1 || w->stride(1) != 1 || w->stride(0) < w->size(1) || t->sizes() != x->sizes().slice(0, x->dim() - 1) ||
+      w->size(0) < 1 || w->size(1) < 1 || x->stride(-1) != 1 || w->stride(1) != 1 || w->stride(0) < w->size(1) || t->sizes() != x->sizes().slice(0, x->dim() - 1) ||
       (c.shift && (x->dim() != 3 || x->size(1) < 2)) || !as_i64(a[4], &c.ignore) || !as_i64(a[5], &c.reduction) || !as_i64(a[6], &c.chunk))
     return none();
   c.stream = reinterpret_cast<int64_t>(as_stream(a[8]));

@@ -15,6 +15,8 @@ from torch.nn import functional as F
 
 from picotron_amd.ops import BLOCK8
 
+_MOST_STEP = float.fromhex("0x1.020406p+121")  # the largest whose 127th multiple is finite in fp32
+
 NO_SECOND_DERIVATIVE = (
     "the backward of an operator that keeps its inputs in 8 bits has no derivative of its own (create_graph=True); "
     "use it without checkpoint_8bit"
@@ -30,7 +32,7 @@ def encode(x: Tensor) -> tuple[Tensor, Tensor]:
     most = torch.full_like(top, 127.0)  # a tensor: by a number, torch multiplies with a rounded reciprocal on the GPU
     finite = top.isfinite()
     held = finite & (top >= 2.0**-100)
-    steps = torch.where(held, top / most, torch.where(finite, 0.0, math.nan))
+    steps = torch.where(held, (top / most).clamp_max(_MOST_STEP), torch.where(finite, 0.0, math.nan))
     codes = torch.where(held, (x * (most / top)).round(), 0.0)
     return (codes + 128).to(torch.uint8), steps
 

@@ -50,6 +50,14 @@ def test_special_blocks():
     assert not values[:2].any() and values[2:5].isnan().all() and values[5].isfinite().all()
 
 
+def test_the_largest_values_stay_finite():
+    x = randn(3, 128)
+    for row, dtype in enumerate((torch.float32, torch.float16, torch.bfloat16)):
+        x[row, 5], x[row, 77] = torch.finfo(dtype).min, torch.finfo(dtype).max
+    values = _block8.decode(*_block8.encode(x), 128)
+    assert values.isfinite().all() and torch.all((values[:, 5] / x[:, 5] - 1).abs() <= 2.0**-22)
+
+
 def test_swiglu_gradients_are_those_at_the_kept_values():
     g, u, d = randn(3, 100, seed=1).requires_grad_(), randn(3, 100, seed=2).requires_grad_(), randn(3, 100, seed=3)
     y = swiglu_with_pytorch_forward(g, u, checkpoint_8bit=True)

@@ -117,6 +117,26 @@ def test_swiglu_not_finite(gpu):
             assert d[128:256].isnan().all() and d[:128].isfinite().all() and d[256:].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_swiglu_lowest_values(gpu, dtype):
+    """The type's lowest and highest values are held as such, and their blocks' gradients are finite."""
+
+    g, u = randn((512,), dtype, gpu, 1), randn((512,), dtype, gpu, 2)
+    info = torch.finfo(dtype)
+    g[130], u[300], u[301] = info.min, info.min, info.max
+    _, codes, steps = ops.swiglu8_fwd(g, u)
+    d = torch.full_like(g, info.tiny * 8)
+    got = ops.swiglu8_bwd(d, codes, steps, dtype)
+    a, b, e = kept_flat(g), kept_flat(u), d.double()
+    s = torch.sigmoid(a)
+    assert all(t.isfinite().all() for t in (a, b, *got))
+    near(got[0], e * b * (s * (1 + a * (1 - s))), dtype, (e * b).abs() * s * (1 + a.abs()) * (1 + a.abs()))
+    near(got[1], e * a * s, dtype, (e * a * s).abs() * (1 + a.abs()))
+    wide = u.clone().requires_grad_()
+    dg, du = torch.autograd.grad(triton_swiglu(g.requires_grad_(), wide, checkpoint_8bit=True), [g, wide], torch.zeros_like(g))
+    assert not dg.any() and not du.any()
+
+
 SHAPES = [(1, 1), (3, 7), (5, 32), (300, 128), (17, 129), (33, 500), (9, 512), (40, 513), (7, 1090), (600, 1024), (5, 2047), (4, 4096),
           (3, 8200), (1100, 256), (2, 16384), (3, 16385), (70, 20001)]
 

@@ -452,7 +452,7 @@ def test_fallback_class_runs_the_kernels(gpu):
 def test_refusals(gpu):
     x, w, t = make(8, 64, 30, torch.float32, gpu)
     for args in ((x.half(), w, t), (x.double(), w.double(), t), (x, w[:, :32], t), (x, w, t[:4]), (x, w, t.int()), (x, w[0], t),
-                 (x[0], w, t[0]), (x, w, t.cpu())):
+                 (x[0], w, t[0]), (x, w, t.cpu()), (x[:, :0], w[:, :0], t), (x.half()[:, :0], w.half()[:, :0], t), (x, w[:0], t)):
         with pytest.raises(TritonLinearCrossEntropyUnavailable):
             triton_linear_cross_entropy(*args)
     with pytest.raises(TritonLinearCrossEntropyUnavailable):
@@ -489,3 +489,30 @@ def test_many_tokens_without_gradients(gpu):
     want = torch.nn.functional.cross_entropy(x.double() @ w.double().t(), t, reduction="none")
     slack = (h + 8) * 2.0**-24 * float((x.double().abs() @ w.double().abs().t()).max()) + 2.0**-22
     assert torch.all((whole.double() - want).abs() <= 2 * slack + 2.0**-20 * (1 + want.abs()))
+
+
+def test_more_tokens_than_a_chunk_of_a_small_vocabulary(gpu):
+    """A million rows: a chunk's exponentials would fit, its grids would not."""
+
+    n, h, v = 1_100_000, 136, 10
+    x, w, t = make(n, h, v, torch.bfloat16, gpu)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = triton_linear_cross_entropy(x, w, t, reduction="none")
+    factors = torch.rand(n, device=gpu)
+    dx, dw = torch.autograd.grad(loss, [x, w], factors)
+    part = slice(n - 3000, n)
+    check(loss.detach()[part], dx[part], None, x.detach()[part], w.detach(), t[part], factors[part])
+    with torch.no_grad():
+        assert torch.equal(triton_linear_cross_entropy(x, w, t, reduction="none"), loss)
+    want = torch.zeros(v, h, dtype=torch.float64, device=gpu)
+    size = torch.zeros_like(want)
+    slack = 0.0
+    for i in range(0, n, 100_000):
+        p = slice(i, i + 100_000)
+        _, _, dw64, _, aw, more = oracle(x.detach()[p], w.detach(), t[p], factors[p])
+        want, size, slack = want + dw64, size + aw, max(slack, more)
+    # as in check, with the fp32 sums' errors over the kept rows: at worst one rounding of the running sum for each, of which the
+    # signs of a million do not agree: sqrt(n) of them
+    limit = (2.0**-9 + 2.0**-11 + 4 * slack + 2.0**-18 + math.sqrt(n) * 2.0**-24) * size + 2.0**-8 * want.abs()
+    assert torch.all((dw.double() - want).abs() <= limit)
