@@ -444,10 +444,7 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
     tops[f] = fmaxf(fmaxf(red[m], red[BM + m]), fmaxf(red[2 * BM + m], red[3 * BM + m]));
   }
   __syncthreads();
-  // the block's rows from the wave's first on: one block in m for a tile of 256, a part of it for one of 64
-  const int block_row = (tm * BM) % kBlockSide + p.wm * P::TM + i;
-  const int64_t block = static_cast<int64_t>(tm * BM / kBlockSide) * s.tiles_n + tn;
-  _Float16* to = s.e == nullptr ? nullptr : s.e + (block * kBlockSide + block_row) * kBlockSide + col;
+  _Float16* to = s.e == nullptr ? nullptr : s.e + blocked_at(tm * BM + p.wm * P::TM + i, static_cast<int64_t>(tn) * kTile + col, static_cast<int64_t>(s.tiles_n) * kTile);
 #pragma unroll
   for (int f = 0; f < P::FM; ++f) {
     constexpr float kLog2e = 1.44269504088896340736f, kShift = 14.f;  // 2^14 is kScale
@@ -478,11 +475,11 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
           v[h / 2].e[(h % 2) * 4 + k] = hi;
           low[h / 2].e[(h % 2) * 4 + k] = static_cast<_Float16>((e - static_cast<float>(hi)) * kLow);
         }
-      u32x4* at = reinterpret_cast<u32x4*>(to + f * 16 * kBlockSide);
+      u32x4* at = reinterpret_cast<u32x4*>(to + f * 16 * kBlockWords);
       at[0] = v[0].raw;
       at[1] = v[1].raw;
       if constexpr (Split<T>::kSplit) {
-        at = reinterpret_cast<u32x4*>(to + s.e_plane + f * 16 * kBlockSide);
+        at = reinterpret_cast<u32x4*>(to + s.e_plane + f * 16 * kBlockWords);
         at[0] = low[0].raw;
         at[1] = low[1].raw;
       }
@@ -578,8 +575,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Scores s) {
   if (row >= rows) return;
   if (col == 0) s.sums[static_cast<int64_t>(tn) * s.padded + row] = f32x2{top, sum * (1.0f / kScale)};
   if (s.e == nullptr) return;
-  const int64_t block = static_cast<int64_t>(row / kBlockSide) * s.tiles_n + tn;
-  u32x4* at = reinterpret_cast<u32x4*>(s.e + (block * kBlockSide + row % kBlockSide) * kBlockSide + col);
+  u32x4* at = reinterpret_cast<u32x4*>(s.e + blocked_at(row, static_cast<int64_t>(tn) * kTile + col, ld));
   at[0] = hi[0].raw;
   at[1] = hi[1].raw;
   if constexpr (Split<T>::kSplit) {
@@ -693,7 +689,8 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
   }
 }
 
-// G from exp(l - m), in place: a workgroup takes 64 rows of a block, eight elements a thread at a time.
+// G from exp(l - m), in place: a workgroup takes 64 rows of a tile, 32 of them at a time, eight elements a thread in each of its four
+// blocks.
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, const f32x2* __restrict__ sums, int64_t padded,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
@@ -701,51 +698,47 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
                                                     const float* __restrict__ target, const float* __restrict__ z) {
   typedef typename Split<T>::plane P;
   const int rows = rows_here(meta, first, chunk);
-  const int row0 = static_cast<int>(blockIdx.y) * 64 + threadIdx.x / 32;  // 64 rows lie in one block
-  const int all = (rows + kStep - 1) / kStep * kStep;                     // the last product takes rows 64 by 64: zeros there
+  const int row0 = static_cast<int>(blockIdx.y) * 64 + threadIdx.x / 8;
+  const int all = (rows + kStep - 1) / kStep * kStep;  // the last product takes rows 64 by 64: zeros there
   if (static_cast<int>(blockIdx.y) * 64 >= all) return;
-  const int col = threadIdx.x % 32 * 8;
-  const int64_t block = static_cast<int64_t>(row0 / kBlockSide) * gridDim.x + blockIdx.x;
-  _Float16* at = e + (block * kBlockSide + row0 % kBlockSide) * kBlockSide + col;
-#pragma unroll 4
-  for (int k8 = 0; k8 < 8; ++k8, at += 8 * kBlockSide) {
-    const int row = row0 + k8 * 8;
-    float out[8];
-    if (row < rows) {
-      Vec16<_Float16> v, low;
-      v.raw = *reinterpret_cast<const u32x4*>(at);
-      if constexpr (Split<T>::kSplit) low.raw = *reinterpret_cast<const u32x4*>(at + plane);
-      const float lse = z[first + row];
-      const int label = label_of[first + row];
-      const float weight = weight_of == nullptr ? 1.f : weight_of[first + row] * meta->inv_weight;
-      const float m = sums[blockIdx.x * padded + row][0];
-      // a label outside the vocabulary leaves a NaN, as its loss
-      const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
-      const int place = label - static_cast<int>(blockIdx.x) * kTile - col;
+  const int col = threadIdx.x % 8 * 8;
+  _Float16* const at0 = e + blocked_at(row0, static_cast<int64_t>(blockIdx.x) * kTile + col, static_cast<int64_t>(gridDim.x) * kTile);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = row0 + half * 32;
+    _Float16* at = at0 + half * 32 * kBlockWords;
+    const bool in = row < rows;
+    Vec16<_Float16> v[4], low[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      v[b].raw = low[b].raw = u32x4{0, 0, 0, 0};
+      if (in) {
+        v[b].raw = *reinterpret_cast<const u32x4*>(at + b * kBlockElements);
+        if constexpr (Split<T>::kSplit) low[b].raw = *reinterpret_cast<const u32x4*>(at + b * kBlockElements + plane);
+      }
+    }
+    const float lse = in ? z[first + row] : 0.f;
+    const int label = in ? label_of[first + row] : -1;
+    const float weight = weight_of == nullptr || !in ? 1.f : weight_of[first + row] * meta->inv_weight;
+    const float m = in ? sums[blockIdx.x * padded + row][0] : 0.f;
+    // a label outside the vocabulary leaves a NaN, as its loss
+    const float factor = !in ? 0.f : label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
+    const int place = label - static_cast<int>(blockIdx.x) * kTile - col;  // in 64 b + (0..7) of a block b
+    const float at_label = place >= 0 && place < kTile && place % kBlockWords < 8 ? expm1f(target[first + row] - lse) * weight * kScale : 0.f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      Vec16<P> w, w_low;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        out[k] = static_cast<float>(v.e[k]);
-        if constexpr (Split<T>::kSplit) out[k] += static_cast<float>(low.e[k]) * (1.0f / kLow);
-        out[k] *= factor;
+        float out = static_cast<float>(v[b].e[k]);
+        if constexpr (Split<T>::kSplit) out += static_cast<float>(low[b].e[k]) * (1.0f / kLow);
+        out = place == b * kBlockWords + k ? at_label : out * factor;
+        if constexpr (Split<T>::kSplit) Split<T>::parts(out, &w.e[k], &w_low.e[k]);
+        else w.e[k] = static_cast<P>(out);
       }
-      if (place >= 0 && place < 8) {
-        const float d = expm1f(target[first + row] - lse) * weight * kScale;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k == place) out[k] = d;
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) out[k] = 0.f;
+      *reinterpret_cast<u32x4*>(at + b * kBlockElements) = w.raw;
+      if constexpr (Split<T>::kSplit) *reinterpret_cast<u32x4*>(at + b * kBlockElements + plane) = w_low.raw;
     }
-    Vec16<P> w, low;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if constexpr (Split<T>::kSplit) Split<T>::parts(out[k], &w.e[k], &low.e[k]);
-      else w.e[k] = static_cast<P>(out[k]);
-    }
-    *reinterpret_cast<u32x4*>(at) = w.raw;
-    if constexpr (Split<T>::kSplit) *reinterpret_cast<u32x4*>(at + plane) = low.raw;
   }
 }
 

@@ -20,27 +20,41 @@ constexpr int kStep = 64;  // k of one step: 128 bytes of a row
 // planes are multiples of 8 elements and p is aligned to 16 bytes.  A plane has `bytes` bytes: what lies behind is
 // read as zero.
 //
-// A blocked operand lies in blocks of 256 by 256 elements, each contiguous, so that a step of a tile stays within one: with rows of
-// 128256 words a tile's 256 rows would lie 256 KB apart, and its loads wait for address translation.
+// A blocked operand lies in blocks of 256 rows by 64 words, each contiguous, those of 256 rows one behind the other: the tile of a
+// step is then one block, or a quarter of four.  With rows of 128256 words a tile's 256 rows would lie 256 KB apart, and its
+// loads wait for address translation.
 struct Operand {
   const void* p;
   int64_t ld;
   int64_t plane;  // from the first plane to the second
   int64_t bytes;
-  int64_t per_m;  // bytes from one m to the next tile's, over the m of a tile
-  int64_t jump;   // bytes more after every fourth step
+  int64_t step;   // bytes from one step to the next
+  int64_t jump;   // and more after every fourth
+  int64_t per_m;  // bytes from one tile of m to the next, over the m of a tile
+  int wide;       // columns: bytes from 64 values of m to the next 64
 };
 
-constexpr int kBlockSide = 256;
+constexpr int kBlockRows = 256, kBlockWords = 64;
+constexpr int kBlockElements = kBlockRows * kBlockWords;
 
-inline Operand rows_operand(const void* p, int64_t ld, int64_t plane, int64_t bytes) { return Operand{p, ld, plane, bytes, ld * 2, 0}; }
-inline Operand columns_operand(const void* p, int64_t ld, int64_t plane, int64_t bytes) { return Operand{p, ld, plane, bytes, 2, 0}; }
-// (rows, `words`) in blocks, row blocks one behind the other: its rows along m and words along k, or the other way round.
+// Where element (row, word) of a blocked array of `words` words a row lies.
+__device__ __forceinline__ int64_t blocked_at(int64_t row, int64_t word, int64_t words) {
+  return (row / kBlockRows * (words / kBlockWords) + word / kBlockWords) * kBlockElements + row % kBlockRows * kBlockWords + word % kBlockWords;
+}
+
+inline Operand rows_operand(const void* p, int64_t ld, int64_t plane, int64_t bytes) {
+  return Operand{p, ld, plane, bytes, kStep * 2, 0, ld * 2, 0};
+}
+inline Operand columns_operand(const void* p, int64_t ld, int64_t plane, int64_t bytes) {
+  return Operand{p, ld, plane, bytes, ld * kStep * 2, 0, 2, 128};
+}
+// Its rows along m and words along k, or the other way round.
 inline Operand blocked_rows(const void* p, int64_t words, int64_t plane, int64_t bytes) {
-  return Operand{p, kBlockSide, plane, bytes, words * 2, (kBlockSide - 1) * kBlockSide * 2};
+  return Operand{p, kBlockWords, plane, bytes, kBlockElements * 2, 0, words * 2, 0};
 }
 inline Operand blocked_columns(const void* p, int64_t words, int64_t plane, int64_t bytes) {
-  return Operand{p, kBlockSide, plane, bytes, kBlockSide * 2, (words - kBlockSide) * kBlockSide * 2};
+  constexpr int step = kStep * kBlockWords * 2;
+  return Operand{p, kBlockWords, plane, bytes, step, words * kBlockRows * 2 - 4 * step, kBlockRows * 2, kBlockElements * 2};
 }
 
 // 32-bit operands are two fp16 planes: with v the value times the operand's power of two (its largest magnitude then lies
@@ -79,14 +93,14 @@ struct Tile {
   static __device__ __forceinline__ int row_swizzle(int m) { return SPREAD ? ((m >> 1) & 1) | (((m >> 4) & 3) << 1) : (m >> 1) & 7; }
   static __device__ __forceinline__ int column_swizzle(int k) { return ((k & 3) << 1) | (((k >> 3) & 3) << 3); }
 
-  __device__ __forceinline__ void init(int64_t ld) {
+  __device__ __forceinline__ void init(int64_t ld, int wide) {
     const int t = threadIdx.x;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int piece = j * THREADS + t;  // 16-byte place in the tile
       if constexpr (COLUMNS) {
         const int k = piece / 32, c = (piece % 32) ^ column_swizzle(k);
-        voffset[j] = static_cast<int>(k * ld * 2) + c * 16;
+        voffset[j] = static_cast<int>(k * ld * 2) + c / 8 * wide + c % 8 * 16;
       } else {
         const int m = piece / 8, c = (piece % 8) ^ row_swizzle(m);
         voffset[j] = static_cast<int>(m * ld * 2) + c * 16;
@@ -184,16 +198,15 @@ struct TileProduct {
 
     TileA ta;
     TileB tb;
-    ta.init(a.ld);
-    tb.init(b.ld);
+    ta.init(a.ld, a.wide);
+    tb.init(b.ld, b.wide);
     Fragments<BM, A_COLUMNS, false> fa;
     Fragments<BN, B_COLUMNS, kSpread> fb;
     fa.init(wm * TM);
     fb.init(wn * TN);
 
-    // bytes from one step to the next, and to the first
-    const int64_t step_a = A_COLUMNS ? a.ld * kStep * 2 : kStep * 2, step_b = B_COLUMNS ? b.ld * kStep * 2 : kStep * 2;
-    const int64_t from_a = m0 * a.per_m + first * step_a + first / 4 * a.jump, from_b = n0 * b.per_m + first * step_b + first / 4 * b.jump;
+    // bytes to the first step
+    const int64_t from_a = m0 * a.per_m + first * a.step + first / 4 * a.jump, from_b = n0 * b.per_m + first * b.step + first / 4 * b.jump;
     const int steps = last - first, total = steps * (SPLIT ? 3 : 1);
     const char* pa = static_cast<const char*>(a.p) + (SPLIT ? a.plane * 2 : 0);
     const char* pb = static_cast<const char*>(b.p);
@@ -205,8 +218,8 @@ struct TileProduct {
       tb.load(to + TileA::kBytes, pb, at_b, bytes_b);
       ++loaded;
       ++step;
-      at_a += step_a + (step % 4 == 0 ? a.jump : 0);
-      at_b += step_b + (step % 4 == 0 ? b.jump : 0);
+      at_a += a.step + (step % 4 == 0 ? a.jump : 0);
+      at_b += b.step + (step % 4 == 0 ? b.jump : 0);
       if (SPLIT && step == last && loaded < total) {  // lo hi, hi lo, hi hi
         step = first;
         at_a = from_a;
