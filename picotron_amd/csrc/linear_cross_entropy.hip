@@ -1425,7 +1425,8 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       return check_launch("pt_linear_cross_entropy");
     }
   }
-  constexpr size_t lds = Product<T, false, false>::kLds;
+  constexpr size_t lds = Product<T, false, true>::kLds;
+  static_assert(lds == Product<T, true, true>::kLds, "one size for both gradients");
   if (int rc = allow(gradient_kernel<T, false>, lds)) return rc;
   if (int rc = allow(gradient_kernel<T, true>, lds)) return rc;
   float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);

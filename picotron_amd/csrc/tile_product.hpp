@@ -179,8 +179,9 @@ struct TileProduct {
   static_assert(!kSpread || FN == 4, "four quads of 16");
   typedef Tile<BM, A_COLUMNS, false, kThreads> TileA;
   typedef Tile<BN, B_COLUMNS, kSpread, kThreads> TileB;
-  static constexpr int kStage = TileA::kBytes + TileB::kBytes;
-  static constexpr int kLds = 2 * kStage;
+  static constexpr bool kDeep = BM == 256 && B_COLUMNS;
+  static constexpr int kSlotsB = kDeep ? 3 : 2;
+  static constexpr int kLds = 2 * TileA::kBytes + kSlotsB * TileB::kBytes;
 
   f32x4 sums[FM][FN];
   int wm, wn;
@@ -205,35 +206,42 @@ struct TileProduct {
     fa.init(wm * TM);
     fb.init(wn * TN);
 
-    // bytes to the first step
-    const int64_t from_a = m0 * a.per_m + first * a.step + first / 4 * a.jump, from_b = n0 * b.per_m + first * b.step + first / 4 * b.jump;
-    const int steps = last - first, total = steps * (SPLIT ? 3 : 1);
-    const char* pa = static_cast<const char*>(a.p) + (SPLIT ? a.plane * 2 : 0);
-    const char* pb = static_cast<const char*>(b.p);
-    int64_t at_a = from_a, at_b = from_b, bytes_a = a.bytes, bytes_b = b.bytes;
-    int loaded = 0, step = first;
-    auto load = [&]() {
-      lds_char* to = lds + (loaded & 1) * kStage;
-      ta.load(to, pa, at_a, bytes_a);
-      tb.load(to + TileA::kBytes, pb, at_b, bytes_b);
-      ++loaded;
-      ++step;
-      at_a += a.step + (step % 4 == 0 ? a.jump : 0);
-      at_b += b.step + (step % 4 == 0 ? b.jump : 0);
-      if (SPLIT && step == last && loaded < total) {  // lo hi, hi lo, hi hi
-        step = first;
-        at_a = from_a;
-        at_b = from_b;
-        pa = static_cast<const char*>(a.p);
-        pb = static_cast<const char*>(b.p) + (loaded == steps ? b.plane * 2 : 0);
-      }
-      if (loaded == total) bytes_a = bytes_b = 0;
+    // one operand's loads: the step's place, its slot, how many are under way or done
+    struct Stream {
+      const char* p;
+      int64_t at, bytes;
+      int loaded, step, slot;
     };
+    const int64_t from_a = m0 * a.per_m + first * a.step + first / 4 * a.jump, from_b = n0 * b.per_m + first * b.step + first / 4 * b.jump;
+    Stream sa, sb;
+    int total;
+    auto advance = [&](Stream& s, const Operand& o, int64_t from, int slots) {
+      ++s.loaded;
+      ++s.step;
+      s.slot = s.slot + 1 == slots ? 0 : s.slot + 1;
+      s.at += o.step + (s.step % 4 == 0 ? o.jump : 0);
+      if (SPLIT && s.step == last && s.loaded < total) {  // the second round of lo hi, hi lo: the other plane of each
+        s.step = first;
+        s.at = from;
+        s.p = static_cast<const char*>(o.p) + (s.p == o.p ? o.plane * 2 : 0);
+      }
+      if (s.loaded == total) s.bytes = 0;
+    };
+    lds_char* const lds_b = lds + 2 * TileA::kBytes;
+    auto load_a = [&](lds_char* to) {
+      ta.load(to, sa.p, sa.at, sa.bytes);
+      advance(sa, a, from_a, 2);
+    };
+    auto load_b = [&](lds_char* to) {
+      tb.load(to, sb.p, sb.at, sb.bytes);
+      advance(sb, b, from_b, kSlotsB);
+    };
+    auto to_a = [&]() { return lds + sa.slot * TileA::kBytes; };
+    auto to_b = [&]() { return lds_b + sb.slot * TileB::kBytes; };
     s16x8 av[2][FM], bv[2][FN];
-    auto read = [&](int t, int half) {
-      const lds_char* la = lds + (t & 1) * kStage;
+    auto read = [&](const lds_char* la, const lds_char* lb, int half) {
 #pragma unroll
-      for (int h = 0; h < FN; ++h) bv[half][h] = fb.read(la + TileA::kBytes, h, half);
+      for (int h = 0; h < FN; ++h) bv[half][h] = fb.read(lb, h, half);
 #pragma unroll
       for (int f = 0; f < FM; ++f) av[half][f] = fa.read(la, f, half);
     };
@@ -243,32 +251,55 @@ struct TileProduct {
 #pragma unroll
         for (int h = 0; h < FN; ++h) sums[f][h] = mfma16<T>(bv[half][h], av[half][f], sums[f][h]);
     };
-    // every wave's loads have arrived, and its reads
-#define PT_ARRIVED() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+    // every wave's loads of the step to come have arrived, and its reads; those of B behind it are under way
+#define PT_ARRIVED() \
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kDeep ? TileB::kLoads : 0) : "memory")
+    // From the second half of a step to the first of the next one.  The compiler would have the transposing reads wait for every load
+    // that may write LDS; these pointers tell it that the loads under way write elsewhere.
+    auto turn = [&](const lds_char* __restrict__ from_a, const lds_char* __restrict__ from_b, lds_char* __restrict__ into_a,
+                    lds_char* __restrict__ into_b) __attribute__((always_inline)) {
+      load_a(into_a);
+      load_b(into_b);
+      read(from_a, from_b, 0);
+      multiply(1);
+      interleave<TileA::kLoads + TileB::kLoads>();
+      __builtin_amdgcn_sched_barrier(0);
+      read(from_a, from_b, 1);
+      multiply(0);
+      interleave<0>();
+    };
 
-    load();
-    PT_ARRIVED();
-    load();
-    read(0, 0);
-    for (int t = 0; t < total; ++t) {
-      if (SPLIT && t == 2 * steps) {
+    // 32-bit operands: lo hi and hi lo, their sums scaled, then hi hi
+    for (int phase = 0; phase < (SPLIT ? 2 : 1); ++phase) {
+      total = (last - first) * (SPLIT && phase == 0 ? 2 : 1);
+      sa = Stream{static_cast<const char*>(a.p) + (SPLIT && phase == 0 ? a.plane * 2 : 0), from_a, a.bytes, 0, first, 0};
+      sb = Stream{static_cast<const char*>(b.p), from_b, b.bytes, 0, first, 0};
+      load_a(to_a());
+      load_b(to_b());
+      if (kDeep) load_b(to_b());
+      PT_ARRIVED();
+      load_a(to_a());
+      load_b(to_b());
+      read(lds, lds_b, 0);
+      read(lds, lds_b, 1);
+      multiply(0);
+      int slot_b = 0;
+      for (int t = 1; t < total; ++t) {
+        slot_b = slot_b + 1 == kSlotsB ? 0 : slot_b + 1;
+        __builtin_amdgcn_sched_barrier(0);
+        PT_ARRIVED();
+        __builtin_amdgcn_sched_barrier(0);
+        turn(lds + (t & 1) * TileA::kBytes, lds_b + slot_b * TileB::kBytes, to_a(), to_b());
+      }
+      multiply(1);
+      if (SPLIT && phase == 0) {
 #pragma unroll
         for (int f = 0; f < FM; ++f)
 #pragma unroll
           for (int h = 0; h < FN; ++h) sums[f][h] *= 1.0f / kLow;
       }
-      read(t, 1);
-      multiply(0);
-      interleave<0>();
-      __builtin_amdgcn_sched_barrier(0);
-      PT_ARRIVED();
-      __builtin_amdgcn_sched_barrier(0);
-      load();
-      read(t + 1, 0);  // behind the last step: what is there, and not used
-      multiply(1);
-      interleave<TileA::kLoads + TileB::kLoads>();
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
-    PT_ARRIVED();
 #undef PT_ARRIVED
   }
 
