@@ -689,56 +689,68 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
   }
 }
 
-// G from exp(l - m), in place: a workgroup takes 64 rows of a tile, 32 of them at a time, eight elements a thread in each of its four
-// blocks.
+// G from exp(l - m), in place: a workgroup takes half of a block, eight elements a thread of each 32 rows.
+constexpr int kSlopeRows = 128;
+
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, const f32x2* __restrict__ sums, int64_t padded,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
                                                     const int* __restrict__ label_of, const float* __restrict__ weight_of,
                                                     const float* __restrict__ target, const float* __restrict__ z) {
   typedef typename Split<T>::plane P;
+  constexpr int kPer = kSlopeRows / 32;
   const int rows = rows_here(meta, first, chunk);
-  const int row0 = static_cast<int>(blockIdx.y) * 64 + threadIdx.x / 8;
   const int all = (rows + kStep - 1) / kStep * kStep;  // the last product takes rows 64 by 64: zeros there
-  if (static_cast<int>(blockIdx.y) * 64 >= all) return;
+  const int row0 = static_cast<int>(blockIdx.y) * kSlopeRows + threadIdx.x / 8;
+  if (static_cast<int>(blockIdx.y) * kSlopeRows >= all) return;
   const int col = threadIdx.x % 8 * 8;
-  _Float16* const at0 = e + blocked_at(row0, static_cast<int64_t>(blockIdx.x) * kTile + col, static_cast<int64_t>(gridDim.x) * kTile);
+  const int half = blockIdx.y % (kBlockRows / kSlopeRows);
+  _Float16* const at = e + (static_cast<int64_t>(blockIdx.y / (kBlockRows / kSlopeRows)) * gridDim.x + blockIdx.x) * kBlockElements +
+                       half * (kSlopeRows * kBlockWords) + threadIdx.x * 8;
+  Vec16<_Float16> v[kPer], low[kPer];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int row = row0 + half * 32;
-    _Float16* at = at0 + half * 32 * kBlockWords;
-    const bool in = row < rows;
-    Vec16<_Float16> v[4], low[4];
+  for (int k = 0; k < kPer; ++k) {
+    v[k].raw = low[k].raw = u32x4{0, 0, 0, 0};
+    if (row0 + k * 32 < rows) {
+      v[k].raw = *reinterpret_cast<const u32x4*>(at + k * 2048);
+      if constexpr (Split<T>::kSplit) low[k].raw = *reinterpret_cast<const u32x4*>(at + k * 2048 + plane);
+    }
+  }
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      v[b].raw = low[b].raw = u32x4{0, 0, 0, 0};
-      if (in) {
-        v[b].raw = *reinterpret_cast<const u32x4*>(at + b * kBlockElements);
-        if constexpr (Split<T>::kSplit) low[b].raw = *reinterpret_cast<const u32x4*>(at + b * kBlockElements + plane);
+  for (int k = 0; k < kPer; ++k) {
+    const int row = row0 + k * 32;
+    if (row >= all) break;
+    Vec16<P> w, w_low;
+    w.raw = w_low.raw = u32x4{0, 0, 0, 0};
+    if (row < rows) {
+      const float lse = z[first + row];
+      const int label = label_of[first + row];
+      const float weight = weight_of == nullptr ? 1.f : weight_of[first + row] * meta->inv_weight;
+      const float m = sums[blockIdx.x / (kTile / kBlockWords) * padded + row][0];
+      // a label outside the vocabulary leaves a NaN, as its loss
+      const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
+      const int place = label - static_cast<int>(blockIdx.x) * kBlockWords - col;
+      float out[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        out[i] = static_cast<float>(v[k].e[i]);
+        if constexpr (Split<T>::kSplit) out[i] += static_cast<float>(low[k].e[i]) * (1.0f / kLow);
+        out[i] *= factor;
+      }
+      if (place >= 0 && place < 8) {
+        const float d = expm1f(target[first + row] - lse) * weight * kScale;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i == place) out[i] = d;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (Split<T>::kSplit) Split<T>::parts(out[i], &w.e[i], &w_low.e[i]);
+        else w.e[i] = static_cast<P>(out[i]);
       }
     }
-    const float lse = in ? z[first + row] : 0.f;
-    const int label = in ? label_of[first + row] : -1;
-    const float weight = weight_of == nullptr || !in ? 1.f : weight_of[first + row] * meta->inv_weight;
-    const float m = in ? sums[blockIdx.x * padded + row][0] : 0.f;
-    // a label outside the vocabulary leaves a NaN, as its loss
-    const float factor = !in ? 0.f : label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
-    const int place = label - static_cast<int>(blockIdx.x) * kTile - col;  // in 64 b + (0..7) of a block b
-    const float at_label = place >= 0 && place < kTile && place % kBlockWords < 8 ? expm1f(target[first + row] - lse) * weight * kScale : 0.f;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      Vec16<P> w, w_low;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float out = static_cast<float>(v[b].e[k]);
-        if constexpr (Split<T>::kSplit) out += static_cast<float>(low[b].e[k]) * (1.0f / kLow);
-        out = place == b * kBlockWords + k ? at_label : out * factor;
-        if constexpr (Split<T>::kSplit) Split<T>::parts(out, &w.e[k], &w_low.e[k]);
-        else w.e[k] = static_cast<P>(out);
-      }
-      *reinterpret_cast<u32x4*>(at + b * kBlockElements) = w.raw;
-      if constexpr (Split<T>::kSplit) *reinterpret_cast<u32x4*>(at + b * kBlockElements + plane) = w_low.raw;
-    }
+    *reinterpret_cast<u32x4*>(at + k * 2048) = w.raw;
+    if constexpr (Split<T>::kSplit) *reinterpret_cast<u32x4*>(at + k * 2048 + plane) = w_low.raw;
   }
 }
 
@@ -1448,8 +1460,8 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows_most + 31) / 32)), dim3(1024), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
-    const int64_t slope_rows = (rows_most + 63) / 64;
-    hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>(tiles_v), static_cast<unsigned>(slope_rows)), dim3(256), 0, st, e,
+    const dim3 slope(static_cast<unsigned>(p.words / kBlockWords), static_cast<unsigned>((rows_most + kSlopeRows - 1) / kSlopeRows));
+    hipLaunchKernelGGL(slope_kernel<T>, slope, dim3(256), 0, st, e,
                        p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
     const int64_t plane = p.chunk * p.words;
     if (dx != nullptr) {

@@ -165,7 +165,7 @@ struct Fragments {
 //
 // LDS holds two steps, and the registers two halves of one: while one half is multiplied the other one is read, so that no
 // product waits for LDS, and there is one barrier a step, between the halves: every wave has then read the step
-// that is done, and the next one has arrived.  With a barrier between steps and the reads just ahead of their
+// that is done, and the next one has arrived.  A third slot for B, whose loads then have two steps' time, changed nothing.  With a barrier between steps and the reads just ahead of their
 // products, 8192 x 32768 x 4096 took 1.91 ms; with the loads under a branch, not among the products, 1.81; so, 1.78 (1232
 // TFLOP/s with an fp32 result of 1 GB, which alone takes 0.18 ms).  Loads three half steps ahead in four slots of 32 k, a
 // barrier each: 2.17.  A higher priority around the products: 1.87.
@@ -179,9 +179,7 @@ struct TileProduct {
   static_assert(!kSpread || FN == 4, "four quads of 16");
   typedef Tile<BM, A_COLUMNS, false, kThreads> TileA;
   typedef Tile<BN, B_COLUMNS, kSpread, kThreads> TileB;
-  static constexpr bool kDeep = BM == 256 && B_COLUMNS;
-  static constexpr int kSlotsB = kDeep ? 3 : 2;
-  static constexpr int kLds = 2 * TileA::kBytes + kSlotsB * TileB::kBytes;
+  static constexpr int kLds = 2 * (TileA::kBytes + TileB::kBytes);
 
   f32x4 sums[FM][FN];
   int wm, wn;
@@ -215,10 +213,10 @@ struct TileProduct {
     const int64_t from_a = m0 * a.per_m + first * a.step + first / 4 * a.jump, from_b = n0 * b.per_m + first * b.step + first / 4 * b.jump;
     Stream sa, sb;
     int total;
-    auto advance = [&](Stream& s, const Operand& o, int64_t from, int slots) {
+    auto advance = [&](Stream& s, const Operand& o, int64_t from) {
       ++s.loaded;
       ++s.step;
-      s.slot = s.slot + 1 == slots ? 0 : s.slot + 1;
+      s.slot ^= 1;
       s.at += o.step + (s.step % 4 == 0 ? o.jump : 0);
       if (SPLIT && s.step == last && s.loaded < total) {  // the second round of lo hi, hi lo: the other plane of each
         s.step = first;
@@ -230,11 +228,11 @@ struct TileProduct {
     lds_char* const lds_b = lds + 2 * TileA::kBytes;
     auto load_a = [&](lds_char* to) {
       ta.load(to, sa.p, sa.at, sa.bytes);
-      advance(sa, a, from_a, 2);
+      advance(sa, a, from_a);
     };
     auto load_b = [&](lds_char* to) {
       tb.load(to, sb.p, sb.at, sb.bytes);
-      advance(sb, b, from_b, kSlotsB);
+      advance(sb, b, from_b);
     };
     auto to_a = [&]() { return lds + sa.slot * TileA::kBytes; };
     auto to_b = [&]() { return lds_b + sb.slot * TileB::kBytes; };
@@ -251,11 +249,11 @@ struct TileProduct {
 #pragma unroll
         for (int h = 0; h < FN; ++h) sums[f][h] = mfma16<T>(bv[half][h], av[half][f], sums[f][h]);
     };
-    // every wave's loads of the step to come have arrived, and its reads; those of B behind it are under way
-#define PT_ARRIVED() \
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kDeep ? TileB::kLoads : 0) : "memory")
-    // From the second half of a step to the first of the next one.  The compiler would have the transposing reads wait for every load
-    // that may write LDS; these pointers tell it that the loads under way write elsewhere.
+    // every wave's loads have arrived, and its reads
+#define PT_ARRIVED() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+    // From the second half of a step to the first of the next one.  The compiler has transposing reads wait for every load that may
+    // write what they read, which is all of them, just issued: these pointers tell it that they write elsewhere (8192 x 4096 x
+    // 128256 and its transpose, 7.70 and 7.98 ms with the waits, 6.13 and 6.49 without).
     auto turn = [&](const lds_char* __restrict__ from_a, const lds_char* __restrict__ from_b, lds_char* __restrict__ into_a,
                     lds_char* __restrict__ into_b) __attribute__((always_inline)) {
       load_a(into_a);
@@ -276,7 +274,6 @@ struct TileProduct {
       sb = Stream{static_cast<const char*>(b.p), from_b, b.bytes, 0, first, 0};
       load_a(to_a());
       load_b(to_b());
-      if (kDeep) load_b(to_b());
       PT_ARRIVED();
       load_a(to_a());
       load_b(to_b());
@@ -285,7 +282,7 @@ struct TileProduct {
       multiply(0);
       int slot_b = 0;
       for (int t = 1; t < total; ++t) {
-        slot_b = slot_b + 1 == kSlotsB ? 0 : slot_b + 1;
+        slot_b ^= 1;
         __builtin_amdgcn_sched_barrier(0);
         PT_ARRIVED();
         __builtin_amdgcn_sched_barrier(0);
@@ -298,7 +295,7 @@ struct TileProduct {
 #pragma unroll
           for (int h = 0; h < FN; ++h) sums[f][h] *= 1.0f / kLow;
       }
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      PT_ARRIVED();
     }
 #undef PT_ARRIVED
   }
