@@ -38,10 +38,10 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 // How many parts the steps of a product of `tiles` tiles are split into, where that takes less time: 256 CUs take a tile each, a
-// workgroup a step in 1 us while it is alone and in 1.9 beside 255 others, the join 12 us more, and each tile of a part 0.13 us for
-// its way to memory and back.  The number of
-// tiles follows from the number of kept rows, so this is decided on the device; `most` bounds the tiles of all parts (0: no
-// split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps, 1025 us in one part.
+// workgroup a step in 1 us while it is alone and in 1.5 beside 255 others, the join 12 us more, and each tile of a part 0.13 us for
+// its way to memory and back.  The number of tiles follows from the number of kept rows, so this is decided on the device; `most`
+// bounds the tiles of all parts (0: no split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps,
+// takes 549 us in parts, and their join 37.
 constexpr int64_t kMostParts = 1024;
 __host__ __device__ inline int splits_for(int64_t all_tiles, int64_t all_steps, int64_t most) {
   if (all_tiles * 2 > most || all_tiles < 1) return 1;
@@ -50,7 +50,7 @@ __host__ __device__ inline int splits_for(int64_t all_tiles, int64_t all_steps, 
   unsigned best = 1, least = ~0u;  // ns
 #pragma unroll
   for (unsigned s : kTry) {
-    const unsigned groups = tiles * s, step = 1000 + (groups < 256 ? groups : 256) * 900 / 256;
+    const unsigned groups = tiles * s, step = 1000 + (groups < 256 ? groups : 256) * 500 / 256;
     const unsigned t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
     if ((s == 1 || (s <= steps && groups <= most)) && t < least) {
       least = t;
