@@ -8,7 +8,8 @@
 //
 // What a wave's first product leaves, inner index along the registers of a lane, is what its second one takes as its
 // operand, so that G never leaves the registers.  What bounds each pass is the vector unit: an fma, an exp (four cycles of its
-// quarter-rate unit) and half a conversion for each word of each token.
+// quarter-rate unit) and half a conversion for each word of each token.  8160 tokens, 20 wide, 50257 words in fp16: 98, 115 and 159
+// us; with the softmax held, as wider models have it, the whole call took 1.13 ms, so 0.40.
 #pragma once
 
 #include "tile_product.hpp"

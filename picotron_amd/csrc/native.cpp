@@ -10,7 +10,7 @@
 //
 // Three operators come as nodes of the autograd graph too (the functions that end in _node): a training pass through SwiGLU or
 // RMSNorm with 8-bit checkpoints, or through the head's cross-entropy, then runs no Python between the call and its
-// gradients ([32, 64] fp32 SwiGLU, forward and gradients: 94 us through Python functions).  A node's backward runs on
+// gradients ([32, 64] fp32 SwiGLU, forward and gradients: 94 us through Python functions, 57 so).  A node's backward runs on
 // the stream of its forward, as the engine runs every node.
 //
 // Entry points come in by address (bind), from the library that _lib loaded.  Nothing is kept

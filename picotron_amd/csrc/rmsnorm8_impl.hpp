@@ -8,6 +8,8 @@
 // has its units of eight elements l, l + LANES, ... in registers from the load to the store, so the sixteen lanes of a
 // block of 128 are a DPP row.  Rows of more than 16384 elements go through a workgroup in pieces and are read twice.
 //
+// [16384, 4096] bf16 with the residual add: 606 MB in 96 us forward, 472 MB in 78 backward, 6.3 and 6.1 TB/s.
+//
 // dw: a row slot of the backward adds up its rows in fp32 registers and writes one partial row; a second kernel adds the
 // partial rows in a fixed order.
 //
@@ -194,7 +196,7 @@ __device__ __forceinline__ void norm8_row(const Norm8& a, int l, int t, bool act
 }
 
 // A slot takes rows slot, slot + slots, ..., the next one's loads under way while a row is worked on ([16384, 4096] bf16 with the
-// gradient of h, 470 MB: 92 us without, 81 with; a copy of these bytes takes 74).
+// gradient of h, 472 MB: 92 us without, 78 with; a copy of these bytes takes 74).
 template <typename T, int LANES, int VPL, bool ADD, bool ALIGNED, bool NT>
 __global__ __launch_bounds__(kThreads) void norm8_bwd_kernel(Norm8 a, int iterations) {
   __shared__ float red[8];

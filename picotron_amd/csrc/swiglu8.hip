@@ -5,7 +5,8 @@
 //
 // HBM streams: the forward reads 2 elements and writes 1 and 2.06 bytes, the backward reads 1 and 2.06 bytes and writes 2.  A unit
 // of eight elements a lane: its codes of gate and up lie side by side, so that a lane stores and loads them as
-// 16 bytes, and a block's two steps are 8 bytes.
+// 16 bytes, and a block's two steps are 8 bytes.  bf16 [16384, 14336]: 1.89 GB each way, 310 and 301 us, 6.1 and 6.3 TB/s,
+// where a copy of 4 GiB reaches 6.57.
 #include "block8.hpp"
 
 namespace pt {

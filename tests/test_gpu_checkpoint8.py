@@ -13,6 +13,8 @@ from picotron_amd import ops
 from picotron_amd.nn import RMSNorm, SwiGLU
 from picotron_amd.nn.triton_kernels import (
     _block8,
+    linear_cross_entropy_with_pytorch,
+    triton_linear_cross_entropy,
     triton_residual_rms_norm,
     triton_rms_norm,
     triton_swiglu,
@@ -336,6 +338,53 @@ def test_captured(gpu):
         got = [t.clone() for t in out]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_training_step_of_all(gpu, dtype):
+    """Blocks, the norm behind them and the head, whose weight the embedding shares: eager, against the plain operators, and as a graph."""
+
+    plain, kept = blocks(gpu, dtype)
+    vocab = 700
+    steps = []
+    for body, options in ((plain, {}), (kept, dict(checkpoint_8bit=True))):
+        norm = RMSNorm(96, use_triton_rmsnorm=True, **options).to(gpu, dtype)
+        table = nn.Parameter(randn((vocab, 96), dtype, gpu, 5, 0.3))
+        params = [table, norm.weight, *body.parameters()]
+
+        def step(ids, body=body, norm=norm, table=table, params=params, fused=bool(options)):
+            loss_of = triton_linear_cross_entropy if fused else linear_cross_entropy_with_pytorch
+            loss = loss_of(norm(body(nn.functional.embedding(ids, table))), table, ids, shift=True)
+            return [loss.detach(), *torch.autograd.grad(loss, params)]
+
+        steps.append(step)
+    ids = torch.randint(0, vocab, (4, 60), device=gpu, generator=torch.Generator(gpu).manual_seed(3))
+    want, got = (step(ids) for step in steps)
+    # the loss: bf16 logits of up to 10 are rounded to 8 bits in the plain form; fp32 sums in another order
+    assert abs(float(got[0] - want[0])) <= (10 * 2.0**-8 if dtype == torch.bfloat16 else 1e-5 * float(want[0]))
+    for a, b in zip(got[1:], want[1:]):
+        # values kept to 1/254 of the largest of 128, about 1/85 of their size, in at most seven operators on the way
+        assert float((a - b).float().norm() / b.float().norm()) < 7 / 85
+    del want, got
+    step = steps[1]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(ids)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(ids)
+    for seed in range(3):
+        ids.copy_(torch.randint(0, vocab, ids.shape, device=gpu, generator=torch.Generator(gpu).manual_seed(40 + seed)))
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        want = step(ids)
+        # the embedding's own backward may add with atomics: its table to rounding, the rest to the bit
+        assert all(torch.equal(a, b) for a, b in zip(got[:1] + got[2:], want[:1] + want[2:]))
+        torch.testing.assert_close(got[1], want[1], rtol=2.0**-6 if dtype == torch.bfloat16 else 1e-5, atol=1e-4)
 
 
 def test_large_swiglu(gpu):
