@@ -46,10 +46,10 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 constexpr int64_t kMostParts = 1024;
 __host__ __device__ inline int splits_for(int64_t all_tiles, int64_t all_steps, int64_t most) {
   if (all_tiles * 2 > most || all_tiles < 1) return 1;
-  constexpr unsigned kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
+  static constexpr unsigned kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
   const unsigned tiles = static_cast<unsigned>(all_tiles), steps = static_cast<unsigned>(all_steps);
   unsigned best = 1, least = ~0u;  // ns
-#pragma unroll
+#pragma unroll 1  // the kernel that calls this is one workgroup, whose time is that of fetching its code
   for (unsigned s : kTry) {
     const unsigned groups = tiles * s, step = 1000 + (groups < 256 ? groups : 256) * 500 / 256;
     const unsigned t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
@@ -60,6 +60,9 @@ __host__ __device__ inline int splits_for(int64_t all_tiles, int64_t all_steps, 
   }
   return static_cast<int>(best);
 }
+
+// Of numbers of rows, which are below 2^32.
+__host__ __device__ inline int64_t quotient(int64_t a, int64_t b) { return static_cast<unsigned>(a) / static_cast<unsigned>(b); }
 
 // What the splits follow from beside the kept rows (see Plan); found once, by the kernel that counts the rows.
 struct Splits {
@@ -77,7 +80,7 @@ __host__ __device__ inline int split_of(const Splits& p, int64_t rows, int which
                             : narrow_splits(tiles_r, (p.vocab + kNarrowInner - 1) / kNarrowInner, p.narrow);
   }
   const int64_t tiles_r = (rows + kTile - 1) / kTile;
-  if (which == kSplitS) return splits_for((rows + p.few - 1) / p.few * p.tiles_v, static_cast<int64_t>(p.steps_s) * p.rounds, p.most_s);
+  if (which == kSplitS) return splits_for(quotient(rows + p.few - 1, p.few) * p.tiles_v, static_cast<int64_t>(p.steps_s) * p.rounds, p.most_s);
   if (which == kSplitX) return splits_for(tiles_r * p.tiles_h, static_cast<int64_t>(p.steps_x) * p.rounds, p.most_x);
   return splits_for(static_cast<int64_t>(p.tiles_v) * p.tiles_h, (rows + kStep - 1) / kStep * p.rounds, p.most_w);
 }
@@ -107,6 +110,7 @@ struct Rows {  // labels, and the rows of x, by (outer, inner)
 };
 
 // ------------------------------------------------------------------ rows
+
 
 // The power of two that takes a magnitude, given by its bits, to between 2^13 and 2^14.
 __device__ __forceinline__ int shift_of(unsigned top) {
@@ -147,7 +151,7 @@ __global__ __launch_bounds__(256) void top_kernel(Rows r, const int* __restrict_
   for (int64_t i = block * 4 + wave; i < rows; i += blocks * 4) {
     const float* p = w + i * ld;
     if (of_x) {
-      const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
+      const int64_t row = row_of[i], o = quotient(row, r.dx_inner), s = row - o * r.dx_inner;
       p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
     }
 #pragma unroll 8
@@ -189,7 +193,7 @@ __device__ __forceinline__ void lay_row(const Rows& r, const Lay& a, const int* 
     if (wave >= (static_cast<int64_t>(count) + kTile - 1) / kTile * kTile) return;
     const T* from = nullptr;
     if (wave < count) {
-      const int64_t row = row_of[wave], o = row / r.dx_inner, s = row - o * r.dx_inner;
+      const int64_t row = row_of[wave], o = quotient(row, r.dx_inner), s = row - o * r.dx_inner;
       from = static_cast<const T*>(r.x) + o * r.xso + s * r.xsi;
     }
     P* p = static_cast<P*>(a.x) + wave * a.width;
@@ -208,7 +212,7 @@ __device__ __forceinline__ void lay_row(const Rows& r, const Lay& a, const int* 
   }
   wave -= a.x_rows;
   if (wave < a.dx_rows) {
-    const int64_t o = wave / r.dx_inner, s = wave - o * r.dx_inner;
+    const int64_t o = quotient(wave, r.dx_inner), s = wave - o * r.dx_inner;
     if (s < r.inner && r.t[o * r.tso + s * r.tsi] != r.ignore) return;
     char* p = static_cast<char*>(a.dx) + wave * a.hidden * a.dx_size;
     if (a.dx_size == 4) {
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits spli
       t[k] = r.ignore;
       c[k] = 0.f;
       if (i < n) {
-        const int64_t o = i / r.inner, s = i - o * r.inner;
+        const int64_t o = quotient(i, r.inner), s = i - o * r.inner;
         t[k] = r.t[o * r.tso + s * r.tsi];
         if (r.c != nullptr) c[k] = r.c[o * r.cso + s * r.csi];
         row[k] = static_cast<int>(o * r.dx_inner + s);
@@ -317,7 +321,7 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits spli
   }
   if (threadIdx.x >= 64 && threadIdx.x < 70) {
     const int k = threadIdx.x - 64;
-    const int64_t rows = k < 3 ? splits.chunk : base % splits.chunk;
+    const int64_t rows = k < 3 ? splits.chunk : base - quotient(base, splits.chunk) * splits.chunk;
     meta->splits[k / 3][k % 3] = rows > 0 ? split_of(splits, rows, k % 3) : 1;
   }
   if (lay.width == 0) return;
@@ -327,7 +331,7 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits spli
     for (int64_t i = wave; i < base + lay.w_rows; i += 16) {
       const float* p = static_cast<const float*>(lay.w) + (i - base) * lay.ldw;
       if (i < base) {
-        const int64_t row = row_of[i], o = row / r.dx_inner, s = row - o * r.dx_inner;
+        const int64_t row = row_of[i], o = quotient(row, r.dx_inner), s = row - o * r.dx_inner;
         p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
       }
       for (int64_t c = lane; c < lay.hidden; c += 64) {
@@ -651,7 +655,7 @@ __device__ __forceinline__ void join_rows(const f32x2* __restrict__ sums, int64_
   // the softmax times kScale is exp2(l * log2(e) + exponent); a label outside the vocabulary leaves a NaN, as its loss
   if (exponent != nullptr) exponent[row] = label_of[row] < 0 ? NAN : 14.f - lse * 1.44269504088896340736f;
   if (losses != nullptr) {
-    const int64_t d = row_of[first + row], o = d / dx_inner;
+    const int64_t d = row_of[first + row], o = quotient(d, dx_inner);
     losses[o * inner + (d - o * dx_inner)] = loss;
   }
 }
@@ -768,28 +772,26 @@ struct Out {
   float* parts;       // (splits, tiles_m * 256, tiles_n * 256) or the chunks' sum
 };
 
-__device__ __forceinline__ void put4(void* p, int dtype, int64_t at, f32x4 v, int valid, bool vec) {
+template <typename T>
+__device__ __forceinline__ void put4_as(T* p, f32x4 v, int valid, bool vec) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 w;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = static_cast<T>(v[k]);
   if (vec && valid >= 4) {
-    if (dtype == PT_FLOAT32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(p) + at) = v;
-    } else if (dtype == PT_BFLOAT16) {
-      typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-      b4 w;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = static_cast<__bf16>(v[k]);
-      *reinterpret_cast<b4*>(static_cast<__bf16*>(p) + at) = w;
-    } else {
-      typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-      h4 w;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = static_cast<_Float16>(v[k]);
-      *reinterpret_cast<h4*>(static_cast<_Float16*>(p) + at) = w;
-    }
+    *reinterpret_cast<T4*>(p) = w;
     return;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (k < valid) store_any(p, at + k, dtype, v[k]);
+    if (k < valid) p[k] = w[k];
+}
+
+// Of an array of T or fp32.
+template <typename T>
+__device__ __forceinline__ void put4(void* p, int dtype, int64_t at, f32x4 v, int valid, bool vec) {
+  if (sizeof(T) == 4 || dtype == PT_FLOAT32) put4_as(static_cast<float*>(p) + at, v, valid, vec);
+  else put4_as(static_cast<T*>(p) + at, v, valid, vec);
 }
 
 struct Gradient {
@@ -888,7 +890,7 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
           continue;
         }
       }
-      put4(o.p, o.dtype, at + h * 16, v, left < 4 ? static_cast<int>(left) : 4, vec);
+      put4<T>(o.p, o.dtype, at + h * 16, v, left < 4 ? static_cast<int>(left) : 4, vec);
     }
   }
 }
@@ -1119,7 +1121,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
           *reinterpret_cast<f32x4*>(s.out.parts + ((static_cast<int64_t>(split) * outer_tiles * kNarrowOuter + o) * HP + col)) = v;
         } else {
           const int64_t left = s.out.cols - col;
-          if (left > 0) put4(s.out.p, s.out.dtype, to_row * s.out.cols + col, v, left < 4 ? static_cast<int>(left) : 4, s.out.cols % 4 == 0);
+          if (left > 0) put4<T>(s.out.p, s.out.dtype, to_row * s.out.cols + col, v, left < 4 ? static_cast<int>(left) : 4, s.out.cols % 4 == 0);
         }
       }
     }
@@ -1133,7 +1135,7 @@ __global__ __launch_bounds__(256) void narrow_kernel(Narrow s) {
 }
 
 // Joins the parts of a narrow gradient, in their order.
-template <int HP, int PASS>
+template <typename T, int HP, int PASS>
 __global__ __launch_bounds__(256) void narrow_parts_kernel(Narrow s) {
   const int rows = s.meta->count;
   const int64_t outer_rows = PASS == kNarrowDw ? s.vocab : rows;
@@ -1148,12 +1150,13 @@ __global__ __launch_bounds__(256) void narrow_parts_kernel(Narrow s) {
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll 8
     for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * size);
-    put4(s.out.p, s.out.dtype, (s.out.row_of != nullptr ? s.out.row_of[o] : o) * s.out.cols + col, v, left < 4 ? static_cast<int>(left) : 4,
+    put4<T>(s.out.p, s.out.dtype, (s.out.row_of != nullptr ? s.out.row_of[o] : o) * s.out.cols + col, v, left < 4 ? static_cast<int>(left) : 4,
          s.out.cols % 4 == 0);
   }
 }
 
 // Joins the parts of a split product, in their order.
+template <typename T>
 __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
   const Out& o = s.out;
   const int rows = rows_here(s.meta, s.first, s.chunk);
@@ -1177,7 +1180,7 @@ __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
       for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], shift);
     }
     const int64_t left = o.cols - col;
-    put4(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
+    put4<T>(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
   }
 }
 
@@ -1350,14 +1353,14 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
   if (dx != nullptr) {
     s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDx>), grid_x, dim3(256), 0, st, s);
-    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDx>), join_grid(p.rows, hidden), dim3(256), 0, st, s);
+    hipLaunchKernelGGL((narrow_parts_kernel<T, HP, kNarrowDx>), join_grid(p.rows, hidden), dim3(256), 0, st, s);
   }
   if (dw != nullptr) {
     s.outer = ow;
     s.inner = ox;
     s.out = Out{dw, grad_dtype, kFinal, vocab, hidden, nullptr, parts};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDw>), grid_w, dim3(256), 0, st, s);
-    hipLaunchKernelGGL((narrow_parts_kernel<HP, kNarrowDw>), join_grid(vocab, hidden), dim3(256), 0, st, s);
+    hipLaunchKernelGGL((narrow_parts_kernel<T, HP, kNarrowDw>), join_grid(vocab, hidden), dim3(256), 0, st, s);
   }
   return check_launch("pt_linear_cross_entropy");
 }
@@ -1469,7 +1472,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), kSplitX, top_w, {}};
       d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
       hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
-      if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
+      if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel<T>, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
     }
     if (dw != nullptr) {
       const Operand oxc = columns_operand(x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2);
@@ -1477,7 +1480,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, kSplitW, top_x, {}};
       d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts)};
       hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
-      if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel, join_grid(vocab, hidden), dim3(256), 0, st, d);
+      if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel<T>, join_grid(vocab, hidden), dim3(256), 0, st, d);
     }
     if (int rc = check_launch("pt_linear_cross_entropy")) return rc;
   }

@@ -27,9 +27,9 @@ __host__ __device__ inline int narrow_splits(int64_t outer_tiles, int64_t inner_
   if (outer_tiles * 2 > kNarrowParts || outer_tiles < 1) return 1;
   const unsigned tiles = static_cast<unsigned>(outer_tiles), steps = static_cast<unsigned>(inner_steps);
   const unsigned at_once = hp == 32 ? 1024 : 512;
-  constexpr unsigned kTry[] = {2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 26, 32, 40, 52, 64, 80, 104, 128, 160, 208, 256, 320, 416, 512, 1024};
+  static constexpr unsigned kTry[] = {2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 26, 32, 40, 52, 64, 80, 104, 128, 160, 208, 256, 320, 416, 512, 1024};
   unsigned best = 1, least = (tiles + at_once - 1) / at_once * steps;
-#pragma unroll
+#pragma unroll 1
   for (unsigned s : kTry) {
     const unsigned t = (tiles * s + at_once - 1) / at_once * ((steps + s - 1) / s + 2);
     if (s * tiles <= kNarrowParts && s * 4 <= steps && t < least) {
