@@ -239,6 +239,85 @@ __global__ __launch_bounds__(256) void lay_kernel(Rows r, Lay a, const int* __re
   lay_row<T, VEC>(r, a, row_of, meta->count, shift_x, shift_w, static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64);
 }
 
+// What a small call lays out (see Lay), by the workgroup of keep_kernel: four rows of each wave at a time, whose loads are under way
+// together (32 tokens and 64 words of 32 in fp32, forward and backward: 78.7 us row by row, 75 so).
+template <typename T>
+__device__ __forceinline__ void lay_small(const Rows& r, const Lay& a, const int* row_of, int count, Meta* meta, int wave, float* tops) {
+  typedef typename Split<T>::plane P;
+  constexpr int kAtOnce = 4, kWaves = 16;
+  const int lane = threadIdx.x % 64;
+  const int x_rows = (count + kTile - 1) / kTile * kTile, all = x_rows + static_cast<int>(a.w_rows);
+  auto sources = [&](int first, const T* (&from)[kAtOnce]) {  // of rows first, first + 16, ... of x and the weight behind it; null: zeros
+    int row[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) row[u] = first + u * kWaves < count ? row_of[first + u * kWaves] : 0;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = first + u * kWaves;
+      const int64_t o = quotient(row[u], r.dx_inner), s = row[u] - o * r.dx_inner;
+      from[u] = i < count ? static_cast<const T*>(r.x) + o * r.xso + s * r.xsi
+                          : (i < x_rows || i >= all ? nullptr : static_cast<const T*>(a.w) + (i - x_rows) * a.ldw);
+    }
+  };
+  int shift[2] = {0, 0};  // of x and the weight
+  if constexpr (Split<T>::kSplit) {
+    float most[2] = {0.f, 0.f};
+#pragma unroll 1
+    for (int first = wave; first < all; first += kWaves * kAtOnce) {
+      if (first >= count && first + (kAtOnce - 1) * kWaves < x_rows) continue;  // zeros
+      const float* from[kAtOnce];
+      sources(first, from);
+#pragma unroll 1
+      for (int c = lane; c < a.hidden; c += 64) {
+        float v[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) v[u] = from[u] != nullptr ? fabsf(from[u][c]) : 0.f;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const float finite = v[u] < INFINITY ? v[u] : 0.f;
+          const bool of_x = first + u * kWaves < x_rows;
+          most[0] = fmaxf(most[0], of_x ? finite : 0.f);
+          most[1] = fmaxf(most[1], of_x ? 0.f : finite);
+        }
+      }
+    }
+    for (int k = 0; k < 2; ++k) {
+      most[k] = wave_max(most[k]);
+      __syncthreads();
+      if (lane == 0) tops[wave] = most[k];
+      __syncthreads();
+      most[k] = tops[lane % kWaves];
+      most[k] = wave_max(most[k]);
+      shift[k] = shift_of(__builtin_bit_cast(unsigned, most[k]));
+    }
+    if (threadIdx.x == 0) {
+      meta->top_x = __builtin_bit_cast(unsigned, most[0]);
+      meta->top_w = __builtin_bit_cast(unsigned, most[1]);
+    }
+  }
+#pragma unroll 1
+  for (int first = wave; first < all; first += kWaves * kAtOnce) {
+    const T* from[kAtOnce];
+    sources(first, from);
+#pragma unroll 1
+    for (int c = lane; c < a.width; c += 64) {
+      T v[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) v[u] = from[u] != nullptr && c < a.hidden ? from[u][c] : static_cast<T>(0.f);
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = first + u * kWaves;
+        if (i >= all) break;
+        const bool of_x = i < x_rows;
+        if constexpr (Split<T>::kSplit) v[u] = ldexpf(v[u], shift[of_x ? 0 : 1]);
+        P* to = static_cast<P*>(of_x ? a.x : a.to_w) + (of_x ? i : i - x_rows) * a.width + c;
+        Split<T>::put(to, (of_x ? a.x_rows : a.w_rows) * a.width, v[u]);
+      }
+    }
+  }
+  for (int i = wave; i < a.dx_rows; i += kWaves) lay_row<T, false>(r, a, row_of, count, 0, 0, a.x_rows + i);
+}
+
 // Which rows are kept, in order: their row of dx, label (-1 for one outside the vocabulary) and weight; how many; the
 // gradients' factor.  One workgroup, a round of whose threads reads eight labels each before the scan.  Of a small call (`lay`
 // has rows) it does everything in front of the first product, where a launch more would cost more than the work.
@@ -325,37 +404,8 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits spli
     meta->splits[k / 3][k % 3] = rows > 0 ? split_of(splits, rows, k % 3) : 1;
   }
   if (lay.width == 0) return;
-  float most[2] = {0.f, 0.f};  // x and the weight
-  if constexpr (Split<T>::kSplit) {
-    __syncthreads();
-    for (int64_t i = wave; i < base + lay.w_rows; i += 16) {
-      const float* p = static_cast<const float*>(lay.w) + (i - base) * lay.ldw;
-      if (i < base) {
-        const int64_t row = row_of[i], o = quotient(row, r.dx_inner), s = row - o * r.dx_inner;
-        p = static_cast<const float*>(r.x) + o * r.xso + s * r.xsi;
-      }
-      for (int64_t c = lane; c < lay.hidden; c += 64) {
-        const float v = fabsf(p[c]);
-        if (v < INFINITY) most[i < base ? 0 : 1] = fmaxf(most[i < base ? 0 : 1], v);
-      }
-    }
-    for (int k = 0; k < 2; ++k) {
-      most[k] = wave_max(most[k]);
-      __syncthreads();
-      if (lane == 0) tops[wave] = most[k];
-      __syncthreads();
-      for (int w = 0; w < 16; ++w) most[k] = fmaxf(most[k], tops[w]);
-    }
-    if (threadIdx.x == 0) {
-      meta->top_x = __builtin_bit_cast(unsigned, most[0]);
-      meta->top_w = __builtin_bit_cast(unsigned, most[1]);
-    }
-  } else {
-    __syncthreads();
-  }
-  const int shift_x = shift_of(__builtin_bit_cast(unsigned, most[0])), shift_w = shift_of(__builtin_bit_cast(unsigned, most[1]));
-  for (int64_t i = wave; i < lay.x_rows + lay.dx_rows + lay.w_rows; i += 16)
-    lay_row<T, false>(r, lay, row_of, base, shift_x, shift_w, i);
+  __syncthreads();
+  lay_small<T>(r, lay, row_of, base, meta, wave, tops);
 }
 
 // ------------------------------------------------------------------ the three products

@@ -516,3 +516,41 @@ def test_more_tokens_than_a_chunk_of_a_small_vocabulary(gpu):
     # signs of a million do not agree: sqrt(n) of them
     limit = (2.0**-9 + 2.0**-11 + 4 * slack + 2.0**-18 + math.sqrt(n) * 2.0**-24) * size + 2.0**-8 * want.abs()
     assert torch.all((dw.double() - want).abs() <= limit)
+
+
+def test_calls_of_two_threads(gpu):
+    """Each on a stream of its own: the same bits as one after the other."""
+
+    import threading
+
+    cases = [make(*size, dtype, gpu, seed) for seed, (size, dtype) in enumerate(
+        [((300, 72, 1000), torch.float32), ((300, 192, 2000), torch.bfloat16), ((20, 64, 500), torch.float16), ((700, 40, 900), torch.bfloat16)])]
+
+    def run(x, w, t):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = triton_linear_cross_entropy(x, w, t, reduction="sum")
+        return [loss.detach(), *torch.autograd.grad(loss, [x, w])]
+
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(order):
+        try:
+            stream = torch.cuda.Stream(gpu)
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    for i in order:
+                        got = run(*cases[i])
+                        stream.synchronize()
+                        if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                            wrong.append(i)
+        except Exception as error:  # noqa: BLE001
+            wrong.append(error)
+
+    threads = [threading.Thread(target=work, args=(order,)) for order in ((0, 1, 2, 3), (3, 2, 1, 0))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong
