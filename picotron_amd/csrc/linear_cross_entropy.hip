@@ -44,21 +44,35 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 // bounds the tiles of all parts (0: no split).  8 x 1024 answers of 5100 kept tokens, 2048 x 32000: dx, 160 tiles of 500 steps,
 // takes 549 us in parts, and their join 37.
 constexpr int64_t kMostParts = 1024;
-__host__ __device__ inline int splits_for(int64_t all_tiles, int64_t all_steps, int64_t most) {
-  if (all_tiles * 2 > most || all_tiles < 1) return 1;
-  static constexpr unsigned kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
-  const unsigned tiles = static_cast<unsigned>(all_tiles), steps = static_cast<unsigned>(all_steps);
-  unsigned best = 1, least = ~0u;  // ns
-#pragma unroll 1  // the kernel that calls this is one workgroup, whose time is that of fetching its code
-  for (unsigned s : kTry) {
-    const unsigned groups = tiles * s, step = 1000 + (groups < 256 ? groups : 256) * 500 / 256;
-    const unsigned t = (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
-    if ((s == 1 || (s <= steps && groups <= most)) && t < least) {
+constexpr int kTries = 14;
+__host__ __device__ inline unsigned try_of(int k) {
+  static constexpr unsigned all[kTries] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
+  return all[k];
+}
+// ns in s parts, or ~0 where that is not possible.
+__host__ __device__ inline unsigned split_time(unsigned s, unsigned tiles, unsigned steps, int64_t most) {
+  const unsigned groups = tiles * s, step = 1000 + (groups < 256 ? groups : 256) * 500 / 256;
+  if (s > 1 && (s > steps || groups > most)) return ~0u;
+  return (groups + 255) / 256 * ((steps + s - 1) / s) * step + (s > 1 ? 12000 + groups * 130 : 0);
+}
+inline int splits_for(int64_t tiles, int64_t steps, int64_t most) {
+  if (tiles * 2 > most || tiles < 1) return 1;
+  unsigned best = 1, least = ~0u;
+  for (int k = 0; k < kTries; ++k) {
+    const unsigned t = split_time(try_of(k), static_cast<unsigned>(tiles), static_cast<unsigned>(steps), most);
+    if (t < least) {
       least = t;
-      best = s;
+      best = try_of(k);
     }
   }
   return static_cast<int>(best);
+}
+// As splits_for, a possibility a lane of a wave.
+__device__ inline int splits_by_lanes(int64_t tiles, int64_t steps, int64_t most) {
+  if (tiles * 2 > most || tiles < 1) return 1;
+  const int lane = threadIdx.x % 64;
+  const unsigned t = lane < kTries ? split_time(try_of(lane), static_cast<unsigned>(tiles), static_cast<unsigned>(steps), most) : ~0u;
+  return static_cast<int>(try_of(least_lane(t)));
 }
 
 // Of numbers of rows, which are below 2^32.
@@ -73,16 +87,17 @@ struct Splits {
 };
 enum { kSplitS = 0, kSplitX = 1, kSplitW = 2 };
 
-__host__ __device__ inline int split_of(const Splits& p, int64_t rows, int which) {
+// By a whole wave.
+__device__ inline int split_of(const Splits& p, int64_t rows, int which) {
   if (p.narrow > 0) {
     const int64_t tiles_r = (rows + kNarrowOuter - 1) / kNarrowOuter, tiles_v = (p.vocab + kNarrowOuter - 1) / kNarrowOuter;
     return which == kSplitW ? narrow_splits(tiles_v, (rows + kNarrowInner - 1) / kNarrowInner, p.narrow)
                             : narrow_splits(tiles_r, (p.vocab + kNarrowInner - 1) / kNarrowInner, p.narrow);
   }
   const int64_t tiles_r = (rows + kTile - 1) / kTile;
-  if (which == kSplitS) return splits_for(quotient(rows + p.few - 1, p.few) * p.tiles_v, static_cast<int64_t>(p.steps_s) * p.rounds, p.most_s);
-  if (which == kSplitX) return splits_for(tiles_r * p.tiles_h, static_cast<int64_t>(p.steps_x) * p.rounds, p.most_x);
-  return splits_for(static_cast<int64_t>(p.tiles_v) * p.tiles_h, (rows + kStep - 1) / kStep * p.rounds, p.most_w);
+  if (which == kSplitS) return splits_by_lanes(quotient(rows + p.few - 1, p.few) * p.tiles_v, static_cast<int64_t>(p.steps_s) * p.rounds, p.most_s);
+  if (which == kSplitX) return splits_by_lanes(tiles_r * p.tiles_h, static_cast<int64_t>(p.steps_x) * p.rounds, p.most_x);
+  return splits_by_lanes(static_cast<int64_t>(p.tiles_v) * p.tiles_h, (rows + kStep - 1) / kStep * p.rounds, p.most_w);
 }
 
 struct Meta {
@@ -398,10 +413,11 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits spli
     meta->inv_weight = inv_weight;
     meta->top_x = meta->top_w = 0u;
   }
-  if (threadIdx.x >= 64 && threadIdx.x < 70) {
-    const int k = threadIdx.x - 64;
+  if (wave >= 1 && wave < 7) {
+    const int k = wave - 1;
     const int64_t rows = k < 3 ? splits.chunk : base - quotient(base, splits.chunk) * splits.chunk;
-    meta->splits[k / 3][k % 3] = rows > 0 ? split_of(splits, rows, k % 3) : 1;
+    const int parts = rows > 0 ? split_of(splits, rows, k % 3) : 1;
+    if (lane == 0) meta->splits[k / 3][k % 3] = parts;
   }
   if (lay.width == 0) return;
   __syncthreads();

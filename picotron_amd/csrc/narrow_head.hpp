@@ -23,21 +23,31 @@ constexpr int kNarrowInner = 64;    // rows of the inner side a step
 // How many parts the inner rows are split into: such that whole rounds of the workgroups that run at once (two a CU, four where
 // rows are short) take the fewest steps, a part counting for two more.  All parts together are at most kNarrowParts tiles.
 constexpr int64_t kNarrowParts = 1024;
-__host__ __device__ inline int narrow_splits(int64_t outer_tiles, int64_t inner_steps, int hp) {
+// By a whole wave, a possibility a lane.
+__device__ inline int least_lane(unsigned t) {  // the first lane with the least
+  uint64_t key = static_cast<uint64_t>(t) << 32 | threadIdx.x % 64;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t other = __shfl_xor(static_cast<unsigned long long>(key), d);
+    key = other < key ? other : key;
+  }
+  return static_cast<int>(key & 63);
+}
+__device__ inline int narrow_splits(int64_t outer_tiles, int64_t inner_steps, int hp) {
   if (outer_tiles * 2 > kNarrowParts || outer_tiles < 1) return 1;
   const unsigned tiles = static_cast<unsigned>(outer_tiles), steps = static_cast<unsigned>(inner_steps);
   const unsigned at_once = hp == 32 ? 1024 : 512;
-  static constexpr unsigned kTry[] = {2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 26, 32, 40, 52, 64, 80, 104, 128, 160, 208, 256, 320, 416, 512, 1024};
-  unsigned best = 1, least = (tiles + at_once - 1) / at_once * steps;
-#pragma unroll 1
-  for (unsigned s : kTry) {
-    const unsigned t = (tiles * s + at_once - 1) / at_once * ((steps + s - 1) / s + 2);
-    if (s * tiles <= kNarrowParts && s * 4 <= steps && t < least) {
-      least = t;
-      best = s;
-    }
+  constexpr int kTries = 27;
+  static constexpr unsigned all[kTries] = {1,  2,  3,  4,  5,  6,   7,   8,   10,  12,  16,  20,  26, 32,
+                                           40, 52, 64, 80, 104, 128, 160, 208, 256, 320, 416, 512, 1024};
+  const int lane = threadIdx.x % 64;
+  unsigned t = ~0u;
+  if (lane < kTries) {
+    const unsigned s = all[lane], rounds = (tiles * s + at_once - 1) / at_once;
+    if (s == 1) t = rounds * steps;
+    else if (s * tiles <= kNarrowParts && s * 4 <= steps) t = rounds * ((steps + s - 1) / s + 2);
   }
-  return static_cast<int>(best);
+  return static_cast<int>(all[least_lane(t)]);
 }
 
 // The steps of a tile of the inner side, HP elements a row, in LDS: 16-byte chunks permuted by bits of the row.
