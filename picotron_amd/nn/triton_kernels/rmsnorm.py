@@ -137,7 +137,7 @@ class _RMSNorm8Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float, use_hip: bool):  # type: ignore[override]
         ctx.use_hip = bool(use_hip)
-        ctx.dtype = x.dtype
+        ctx.dtypes = x.dtype, x.dtype if residual is None else residual.dtype
         ctx.set_materialize_grads(False)
         if ctx.use_hip:
             h, y, rstd, codes, steps = ops.rmsnorm8_fwd(x, weight, eps, residual)
@@ -158,12 +158,14 @@ class _RMSNorm8Function(torch.autograd.Function):
         grad, grad_w = grad_h, None
         if grad_y is not None:
             if ctx.use_hip:
-                grad, grad_w = ops.rmsnorm8_bwd(grad_y, weight, rstd, codes, steps, ctx.dtype, grad_h, need_x or need_r, need_w)
+                grad, grad_w = ops.rmsnorm8_bwd(grad_y, weight, rstd, codes, steps, ctx.dtypes[0], grad_h, need_x or need_r, need_w)
             else:
                 kept = _block8.decode(codes, steps, weight.numel())
                 grad, grad_w = _pytorch_backward(kept, weight, rstd, grad_y)
-                grad = (grad if grad_h is None else grad + grad_h.float()).to(ctx.dtype)
-        return (grad if need_x else None), (grad if need_r else None), (grad_w if need_w else None), None, None
+                grad = grad if grad_h is None else grad + grad_h.float()
+        # in PyTorch h may be wider than either: each input's gradient is rounded to its own type
+        grad_x, grad_r = (grad.to(dtype) if need and grad is not None else None for need, dtype in zip((need_x, need_r), ctx.dtypes))
+        return grad_x, grad_r, (grad_w if need_w else None), None, None
 
 
 def _validate_triton_inputs(hidden_states: Tensor, weight: Tensor) -> None:

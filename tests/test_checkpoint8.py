@@ -95,6 +95,31 @@ def test_norm_gradients_are_those_at_the_kept_values(residual):
     torch.testing.assert_close(got[1].double(), (d.double() * hat).sum(0), rtol=2e-6, atol=2e-6)
 
 
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("dtype,scale", [(torch.bfloat16, 1.0), (torch.float16, 1e-9)])
+def test_a_residual_stream_of_32_bits_keeps_its_gradient(dtype, scale, fused):
+    """A 16-bit branch added to an fp32 stream, as under autocast: the sum and its gradient are fp32."""
+
+    x, r, d, dh = randn(4, 200, seed=1).to(dtype), randn(4, 200, seed=2), randn(4, 200, seed=3, scale=scale), randn(4, 200, seed=4, scale=scale)
+    norm = RMSNorm(200, 1e-5, use_triton_rmsnorm=fused, checkpoint_8bit=True)
+    norm._triton_fallback_warned = True
+    x.requires_grad_()
+    r.requires_grad_()
+    h, y = norm.add_and_norm(x, r)
+    assert h.dtype == y.dtype == torch.float32
+    dx, dr = torch.autograd.grad([h, y], [x, r], [dh, d])
+    assert dx.dtype == dtype and dr.dtype == torch.float32
+    h64 = h.detach().double()
+    rstd = (h64.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    hat = _block8.decode(*_block8.encode(h.detach()), 200).double() * rstd
+    want = rstd * (d.double() - hat * (d.double() * hat).mean(-1, keepdim=True)) + dh.double()
+    # a few roundings to 24 bits of terms of up to 4 * 4 * 4 of the gradients' scale, and a mean of 200 of them
+    assert torch.all((dr.double() - want).abs() <= 64 * 16 * 2.0**-24 * scale)
+    # and one to the branch's type, or to half its smallest step
+    assert torch.all((dx.double() - want).abs() <= 64 * 16 * 2.0**-24 * scale + want.abs() * torch.finfo(dtype).eps / 2
+                     + (2.0**-25 if dtype == torch.float16 else 0))
+
+
 def test_gradients_are_near_the_exact_ones():
     """Within what half a step of each block, 1/254 of its largest, makes of them."""
 
