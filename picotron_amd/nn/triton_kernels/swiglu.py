@@ -70,7 +70,7 @@ class _SwiGLU8Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate: Tensor, up: Tensor, use_hip: bool) -> Tensor:  # type: ignore[override]
         ctx.use_hip = bool(use_hip)
-        ctx.dtype = gate.dtype
+        ctx.dtypes = gate.dtype, up.dtype
         if ctx.use_hip:
             output, codes, steps = ops.swiglu8_fwd(gate, up)
             ctx.save_for_backward(codes, steps)
@@ -86,7 +86,7 @@ class _SwiGLU8Function(torch.autograd.Function):
         need_gate, need_up = ctx.needs_input_grad[:2]
         if ctx.use_hip:
             codes, steps = ctx.saved_tensors
-            grad_gate, grad_up = ops.swiglu8_bwd(grad_output, codes, steps, ctx.dtype, need_gate, need_up)
+            grad_gate, grad_up = ops.swiglu8_bwd(grad_output, codes, steps, ctx.dtypes[0], need_gate, need_up)
             return grad_gate, grad_up, None
         kept = ctx.saved_tensors
         gate, up = (_block8.decode(*kept[k:k + 2], grad_output.numel()).view(ctx.shape) for k in (0, 2))
@@ -94,7 +94,7 @@ class _SwiGLU8Function(torch.autograd.Function):
         sigmoid_gate = torch.sigmoid(gate)
         grad_gate = grad * up * (sigmoid_gate * (1 + gate * (1 - sigmoid_gate)))
         grad_up = grad * (gate * sigmoid_gate)
-        return (grad_gate.to(ctx.dtype) if need_gate else None), (grad_up.to(ctx.dtype) if need_up else None), None
+        return (grad_gate.to(ctx.dtypes[0]) if need_gate else None), (grad_up.to(ctx.dtypes[1]) if need_up else None), None
 
 
 def _validate_triton_inputs(gate: Tensor, up: Tensor) -> None:

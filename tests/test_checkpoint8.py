@@ -69,6 +69,25 @@ def test_swiglu_gradients_are_those_at_the_kept_values():
         torch.testing.assert_close(a.double(), b, rtol=2e-6, atol=1e-6)
 
 
+@pytest.mark.parametrize("narrow", [0, 1])
+@pytest.mark.parametrize("dtype,scale", [(torch.bfloat16, 1.0), (torch.float16, 1e-9)])
+def test_swiglu_gradients_of_two_types(dtype, scale, narrow):
+    """gate and up of different types: each gradient in its own."""
+
+    inputs = [randn(3, 100, seed=1), randn(3, 100, seed=2)]
+    inputs[narrow] = inputs[narrow].to(dtype)
+    inputs = [t.requires_grad_() for t in inputs]
+    d = randn(3, 100, seed=3, scale=scale)
+    got = torch.autograd.grad(swiglu_with_pytorch_forward(*inputs, checkpoint_8bit=True), inputs, d)
+    kept = [_block8.decode(*_block8.encode(t.detach().view(-1)), 300).view(3, 100).double().requires_grad_() for t in inputs]
+    want = torch.autograd.grad(torch.nn.functional.silu(kept[0]) * kept[1], kept, d.double())
+    for a, b, t in zip(got, want, inputs):
+        assert a.dtype == t.dtype
+        # a dozen roundings to 24 bits of factors of up to 4, 4 and 4; and one to 16, or to half the smallest step there
+        own = 0 if t.dtype == torch.float32 else torch.finfo(t.dtype).eps / 2 * b.abs() + (2.0**-25 if t.dtype == torch.float16 else 0)
+        assert torch.all((a.double() - b).abs() <= 12 * 64 * 2.0**-24 * scale + own)
+
+
 @pytest.mark.parametrize("residual", [False, True])
 def test_norm_gradients_are_those_at_the_kept_values(residual):
     x, r, w, d, dh = (randn(4, 200, seed=k) for k in (1, 2, 3, 4, 5))
