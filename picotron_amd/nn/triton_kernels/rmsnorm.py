@@ -137,12 +137,13 @@ class _RMSNorm8Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float, use_hip: bool):  # type: ignore[override]
         ctx.use_hip = bool(use_hip)
-        ctx.dtypes = x.dtype, x.dtype if residual is None else residual.dtype
+        ctx.dtype = x.dtype
         ctx.set_materialize_grads(False)
         if ctx.use_hip:
             h, y, rstd, codes, steps = ops.rmsnorm8_fwd(x, weight, eps, residual)
         else:
             h = x if residual is None else x + residual
+            ctx.inputs = tuple((t.shape, t.dtype) for t in (x, x if residual is None else residual))
             inverse_rms = _inverse_rms(h, eps)
             y, rstd, (codes, steps) = _pytorch_forward(h, weight, inverse_rms), inverse_rms, _block8.encode(h)
         ctx.save_for_backward(weight, rstd, codes, steps)
@@ -158,13 +159,15 @@ class _RMSNorm8Function(torch.autograd.Function):
         grad, grad_w = grad_h, None
         if grad_y is not None:
             if ctx.use_hip:
-                grad, grad_w = ops.rmsnorm8_bwd(grad_y, weight, rstd, codes, steps, ctx.dtypes[0], grad_h, need_x or need_r, need_w)
+                grad, grad_w = ops.rmsnorm8_bwd(grad_y, weight, rstd, codes, steps, ctx.dtype, grad_h, need_x or need_r, need_w)
             else:
                 kept = _block8.decode(codes, steps, weight.numel())
                 grad, grad_w = _pytorch_backward(kept, weight, rstd, grad_y)
                 grad = grad if grad_h is None else grad + grad_h.float()
-        # in PyTorch h may be wider than either: each input's gradient is rounded to its own type
-        grad_x, grad_r = (grad.to(dtype) if need and grad is not None else None for need, dtype in zip((need_x, need_r), ctx.dtypes))
+        grad_x = grad if need_x else None
+        grad_r = grad if need_r else None
+        if not ctx.use_hip:  # h may be of a wider type than either, and of more elements: summed first, then rounded to each one's type
+            grad_x, grad_r = (None if g is None else g.sum_to_size(shape).to(dtype) for g, (shape, dtype) in zip((grad_x, grad_r), ctx.inputs))
         return grad_x, grad_r, (grad_w if need_w else None), None, None
 
 

@@ -70,12 +70,12 @@ class _SwiGLU8Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate: Tensor, up: Tensor, use_hip: bool) -> Tensor:  # type: ignore[override]
         ctx.use_hip = bool(use_hip)
-        ctx.dtypes = gate.dtype, up.dtype
+        ctx.dtype = gate.dtype
         if ctx.use_hip:
             output, codes, steps = ops.swiglu8_fwd(gate, up)
             ctx.save_for_backward(codes, steps)
             return output
-        ctx.shape = gate.shape
+        ctx.inputs = (gate.shape, gate.dtype), (up.shape, up.dtype)
         ctx.save_for_backward(*_block8.encode(gate.reshape(-1)), *_block8.encode(up.reshape(-1)))
         return F.silu(gate) * up
 
@@ -86,15 +86,15 @@ class _SwiGLU8Function(torch.autograd.Function):
         need_gate, need_up = ctx.needs_input_grad[:2]
         if ctx.use_hip:
             codes, steps = ctx.saved_tensors
-            grad_gate, grad_up = ops.swiglu8_bwd(grad_output, codes, steps, ctx.dtypes[0], need_gate, need_up)
+            grad_gate, grad_up = ops.swiglu8_bwd(grad_output, codes, steps, ctx.dtype, need_gate, need_up)
             return grad_gate, grad_up, None
         kept = ctx.saved_tensors
-        gate, up = (_block8.decode(*kept[k:k + 2], grad_output.numel()).view(ctx.shape) for k in (0, 2))
+        gate, up = (_block8.decode(*kept[2 * k:2 * k + 2], shape.numel()).view(shape) for k, (shape, _) in enumerate(ctx.inputs))
         grad = grad_output.float()
         sigmoid_gate = torch.sigmoid(gate)
-        grad_gate = grad * up * (sigmoid_gate * (1 + gate * (1 - sigmoid_gate)))
-        grad_up = grad * (gate * sigmoid_gate)
-        return (grad_gate.to(ctx.dtypes[0]) if need_gate else None), (grad_up.to(ctx.dtypes[1]) if need_up else None), None
+        grad_gate = grad * up * (sigmoid_gate * (1 + gate * (1 - sigmoid_gate))) if need_gate else None
+        grad_up = grad * (gate * sigmoid_gate) if need_up else None
+        return *(None if g is None else g.sum_to_size(shape).to(dtype) for g, (shape, dtype) in zip((grad_gate, grad_up), ctx.inputs)), None
 
 
 def _validate_triton_inputs(gate: Tensor, up: Tensor) -> None:

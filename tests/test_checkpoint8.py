@@ -88,6 +88,39 @@ def test_swiglu_gradients_of_two_types(dtype, scale, narrow):
         assert torch.all((a.double() - b).abs() <= 12 * 64 * 2.0**-24 * scale + own)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shapes", [((3, 5, 16), (16,)), ((16,), (3, 5, 16)), ((3, 1, 16), (5, 1))])
+def test_swiglu_of_shapes_that_broadcast(shapes, dtype):
+    inputs = [randn(*shape, seed=k).to(dtype).requires_grad_() for k, shape in enumerate(shapes)]
+    y = swiglu_with_pytorch_forward(*inputs, checkpoint_8bit=True)
+    assert torch.equal(y, swiglu_with_pytorch_forward(*inputs))
+    d = randn(*y.shape, seed=3).to(dtype)
+    got = torch.autograd.grad(y, inputs, d)
+    kept = [_block8.decode(*_block8.encode(t.detach().reshape(-1)), t.numel()).view(t.shape).double().requires_grad_() for t in inputs]
+    want = torch.autograd.grad(torch.nn.functional.silu(kept[0]) * kept[1], kept, d.double())
+    for a, b, t in zip(got, want, inputs):
+        # a dozen roundings to 24 bits of factors of up to 4, 4 and 4, and a sum of at most 48 of them; and one to 16
+        assert a.shape == t.shape and a.dtype == dtype
+        own = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 * b.abs()
+        assert torch.all((a.double() - b).abs() <= (12 + 48) * 48 * 64 * 2.0**-24 + own)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_of_a_residual_that_broadcasts(dtype):
+    x, r = randn(3, 5, 16, seed=1).to(dtype).requires_grad_(), randn(16, seed=2).to(dtype).requires_grad_()
+    w, d, dh = torch.ones(16), randn(3, 5, 16, seed=3).to(dtype), randn(3, 5, 16, seed=4).to(dtype)
+    h, y = residual_rms_norm_with_pytorch(x, r, w, 1e-5, checkpoint_8bit=True)
+    dx, dr = torch.autograd.grad([h, y], [x, r], [dh, d])
+    h64 = h.detach().double()
+    rstd = (h64.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    hat = _block8.decode(*_block8.encode(h.detach()), 16).double() * rstd
+    want = rstd * (d.double() - hat * (d.double() * hat).mean(-1, keepdim=True)) + dh.double()
+    # roundings of terms of up to 4 * 4 * 4, a sum of 15 of them, and one to the type
+    for got, exact, terms in ((dx, want, 1), (dr, want.sum((0, 1)), 15)):
+        own = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 * exact.abs()
+        assert got.shape == exact.shape and torch.all((got.double() - exact).abs() <= (16 + terms) * terms * 64 * 2.0**-24 + own)
+
+
 @pytest.mark.parametrize("residual", [False, True])
 def test_norm_gradients_are_those_at_the_kept_values(residual):
     x, r, w, d, dh = (randn(4, 200, seed=k) for k in (1, 2, 3, 4, 5))
