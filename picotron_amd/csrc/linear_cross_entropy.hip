@@ -1318,7 +1318,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
   int64_t most = p.narrow ? all : p.grads ? kChunkBytes / each / kTile * kTile : kSumsBytes / (p.words / kTile * static_cast<int64_t>(sizeof(f32x2))) / kTile * kTile;
   if (most < kTile) most = kTile;
   if (!p.narrow && most > kMostChunk) most = kMostChunk;
-  if (!p.narrow && chunk_rows > 0 && up(chunk_rows, kTile) < most) most = up(chunk_rows, kTile);
+  if (!p.narrow && chunk_rows > 0 && chunk_rows < most) most = up(chunk_rows, kTile);  // most is whole tiles, so no less than this
   p.chunks = rows > 0 ? (rows + most - 1) / most : 1;
   p.chunk = up((rows + p.chunks - 1) / p.chunks, kTile);
   if (p.chunk < kTile) p.chunk = kTile;

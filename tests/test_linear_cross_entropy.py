@@ -135,6 +135,18 @@ def test_scale_entry_point_refuses():
     assert call(from_=None, to=None, n=0, scale=None) == _lib.PT_OK
 
 
+def test_any_number_of_rows_a_chunk():
+    """As many as an int64 holds: a limit that limits nothing."""
+
+    size = _lib.lib().pt_linear_cross_entropy_workspace_bytes
+    weight = ctypes.c_void_p(256)
+    for hidden in (64, 256):
+        whole = size(5000, 32000, hidden, weight, hidden, _lib.PT_BFLOAT16, 1, 1, 0)
+        for chunk in (5000, 5120, 5121, 1 << 31, (1 << 63) - 257, (1 << 63) - 256, (1 << 63) - 255, (1 << 63) - 1):
+            assert size(5000, 32000, hidden, weight, hidden, _lib.PT_BFLOAT16, 1, 1, chunk) == whole
+    assert call(ws_bytes=100, chunk=(1 << 63) - 1) == _lib.PT_EINVAL
+
+
 def test_workspace_holds_at_most_two_gib_of_exponentials():
     size = _lib.lib().pt_linear_cross_entropy_workspace_bytes
     weight = ctypes.c_void_p(256)
