@@ -921,6 +921,8 @@ def linear_cross_entropy(
     shape (of a mean or sum 1 where it is absent).  At most ``chunk_tokens`` tokens are worked on at a time (0: as many as keep the
     exponentials within 2 GiB)."""
 
+    if not -(2**63) <= ignore_index < 2**63:  # ctypes would take it modulo 2^64, which may be a label
+        raise ValueError("ignore_index must fit an int64, as the labels do")
     device = _check_cuda(hidden, weight, labels)
     outer, inner, dx_inner = head_rows(hidden, weight, labels, shift)
     if hidden.stride(-1) != 1:

@@ -82,6 +82,13 @@ def test_shapes():
             ops.head_rows(*args)
 
 
+@pytest.mark.parametrize("ignore_index", [2**63, 2**64 + 5, -(2**63) - 1])
+def test_an_ignore_index_that_is_no_label_of_any(ignore_index):
+    x, w, t = (y.detach() for y in make(torch.float32))
+    with pytest.raises(ValueError, match="ignore_index"):
+        ops.linear_cross_entropy(x, w, t, ignore_index=ignore_index)
+
+
 def call(**change):
     """The entry point with addresses that no kernel may reach: every call here is refused before a launch."""
 
