@@ -443,6 +443,8 @@ int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blo
  * Gradients, where dx or dw is non-NULL: dx [outer, dx_inner, hidden] contiguous (rows inner.. and ignored rows zero),
  * dw [vocab, hidden] contiguous, of grad_dtype (dtype or fp32), for the incoming gradient dloss: of the mean or sum one
  * fp32 value (NULL: 1), of the loss without a reduction one a row (fp32, the given strides).  16-byte aligned.
+ * A row of dx is exact relative to its own weight, whatever the others are; in dw, whose sums go over the rows, fp16 and fp32 inputs'
+ * terms have fewer bits where weight times softmax lies below 2^-28 of the call's largest weight, in fp16 none below 2^-39.
  * loss may be NULL where gradients are asked for.  workspace: 256-byte aligned, _workspace_bytes for the same arguments.
  *   pt_scale_gradients: to = from * scale (fp32 device scalar), rounded once, of up to two arrays: in place, or from fp32 to
  *     another type.  Nothing is touched in place for a scale of 1.

@@ -104,6 +104,7 @@ struct Meta {
   int count;        // kept rows
   float alpha;      // of the gradients' sums
   float inv_weight; // of the rows' own weights
+  int unit;         // the power of two that they are relative to
   unsigned top_x, top_w;  // bits of the largest finite magnitudes (32-bit inputs)
   int splits[2][3];       // of a whole chunk's products, and of the last one's
 };
@@ -140,18 +141,32 @@ template <typename T>
 struct Split {
   typedef T plane;
   static constexpr bool kSplit = false;
+  static constexpr bool kHalf = __is_same(T, _Float16);  // planes with few exponents: see slope_kernel
   static __device__ __forceinline__ void put(T* p, int64_t, T v) { *p = v; }
 };
 template <>
 struct Split<float> {
   typedef _Float16 plane;
   static constexpr bool kSplit = true;
+  static constexpr bool kHalf = true;
   static __device__ __forceinline__ void parts(float v, _Float16* hi, _Float16* lo) {
     *hi = static_cast<_Float16>(v);
     *lo = static_cast<_Float16>((v - static_cast<float>(*hi)) * kLow);
   }
   static __device__ __forceinline__ void put(_Float16* p, int64_t plane, float v) { parts(v, p, p + plane); }
 };
+
+// A row's weight as m * 2^e, 1 <= |m| < 2; one that is zero or not finite as itself.
+struct Weight {
+  float m;
+  int e;
+};
+__device__ __forceinline__ Weight weight_parts(float c) {
+  if (!(fabsf(c) > 0.f && fabsf(c) < INFINITY)) return {c, 0};
+  int e;
+  const float m = frexpf(c, &e);
+  return {2.f * m, e - 1};
+}
 
 // The largest finite magnitudes of 32-bit inputs: workgroups below `x_blocks` take the kept rows of x, the others the weight's.
 // One atomic a workgroup, whose order a maximum does not depend on.
@@ -411,6 +426,7 @@ __global__ __launch_bounds__(1024) void keep_kernel(Rows r, Lay lay, Splits spli
     meta->count = base;
     meta->alpha = alpha;
     meta->inv_weight = inv_weight;
+    meta->unit = static_cast<int>(e >> 23) - 127;
     meta->top_x = meta->top_w = 0u;
   }
   if (wave >= 1 && wave < 7) {
@@ -761,12 +777,18 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
 }
 
 // G from exp(l - m), in place: a workgroup takes half of a block, eight elements a thread of each 32 rows.
+//
+// Rows with weights of their own: G holds the row's weight relative to a power of two near the largest one.  Where it is held in
+// fp16 and dx is asked for (`apart`), it holds only the weight's significand, between 1 and 2: a row whose weight is 2^-28 of the
+// largest would fall among fp16's last subnormals, and its dx would be off by its own size.  dx's sums then take the row's power of
+// two in fp32, and weigh_kernel scales G by it, relative to the largest, for dw, whose sums go over the rows.
+// 8192 tokens, 2048 wide, 32000 words in fp16: 0.16 ms of 3.95, where the weights differ by more than a factor of two.
 constexpr int kSlopeRows = 128;
 
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, const f32x2* __restrict__ sums, int64_t padded,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
-                                                    const int* __restrict__ label_of, const float* __restrict__ weight_of,
+                                                    const int* __restrict__ label_of, const float* __restrict__ weight_of, bool apart,
                                                     const float* __restrict__ target, const float* __restrict__ z) {
   typedef typename Split<T>::plane P;
   constexpr int kPer = kSlopeRows / 32;
@@ -796,7 +818,7 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
     if (row < rows) {
       const float lse = z[first + row];
       const int label = label_of[first + row];
-      const float weight = weight_of == nullptr ? 1.f : weight_of[first + row] * meta->inv_weight;
+      const float weight = weight_of == nullptr ? 1.f : apart ? weight_parts(weight_of[first + row]).m : weight_of[first + row] * meta->inv_weight;
       const float m = sums[blockIdx.x / (kTile / kBlockWords) * padded + row][0];
       // a label outside the vocabulary leaves a NaN, as its loss
       const float factor = label < 0 ? NAN : (m == -INFINITY ? 0.f : __expf(m - lse)) * weight;
@@ -825,6 +847,45 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
   }
 }
 
+// G with the significands of the rows' weights, to G with the weights relative to the largest one, in place: exact but for what falls
+// among the subnormals.  Threads as in slope_kernel; rows within a factor of two of the largest are left alone.
+template <typename T>
+__global__ __launch_bounds__(256) void weigh_kernel(_Float16* __restrict__ e, int64_t plane, const Meta* __restrict__ meta, int64_t first,
+                                                    int64_t chunk, const float* __restrict__ weight_of) {
+  constexpr int kPer = kSlopeRows / 32;
+  const int rows = rows_here(meta, first, chunk);
+  const int row0 = static_cast<int>(blockIdx.y) * kSlopeRows + threadIdx.x / 8;
+  const int half = blockIdx.y % (kBlockRows / kSlopeRows);
+  _Float16* const at = e + (static_cast<int64_t>(blockIdx.y / (kBlockRows / kSlopeRows)) * gridDim.x + blockIdx.x) * kBlockElements +
+                       half * (kSlopeRows * kBlockWords) + threadIdx.x * 8;
+  int by[kPer];
+  Vec16<_Float16> v[kPer], low[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int row = row0 + k * 32;
+    by[k] = row < rows ? weight_parts(weight_of[first + row]).e - meta->unit : 0;
+    if (by[k] == 0) continue;
+    v[k].raw = *reinterpret_cast<const u32x4*>(at + k * 2048);
+    if constexpr (Split<T>::kSplit) low[k].raw = *reinterpret_cast<const u32x4*>(at + k * 2048 + plane);
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    if (by[k] == 0) continue;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float g = static_cast<float>(v[k].e[i]);
+      if constexpr (Split<T>::kSplit) {
+        g += static_cast<float>(low[k].e[i]) * (1.0f / kLow);
+        Split<T>::parts(ldexpf(g, by[k]), &v[k].e[i], &low[k].e[i]);
+      } else {
+        v[k].e[i] = static_cast<_Float16>(ldexpf(g, by[k]));
+      }
+    }
+    *reinterpret_cast<u32x4*>(at + k * 2048) = v[k].raw;
+    if constexpr (Split<T>::kSplit) *reinterpret_cast<u32x4*>(at + k * 2048 + plane) = low[k].raw;
+  }
+}
+
 enum { kFinal = 0, kAdd = 1, kAddFinal = 2 };
 
 // Where a product's sums go: times alpha to rows of `p`, (rows, cols), or as they are to a part of their own, to be
@@ -836,7 +897,12 @@ struct Out {
   int64_t rows, cols;
   const int* row_of;  // rows of p, or null for their own
   float* parts;       // (splits, tiles_m * 256, tiles_n * 256) or the chunks' sum
+  const float* weight_of;  // the rows' weights, whose powers of two G lacks (see slope_kernel), or null
 };
+
+// The factor of the sums, and the power of two of a row's beside it.
+__device__ __forceinline__ float factor_of(const Out& o, const Meta* meta) { return o.weight_of == nullptr ? meta->alpha : 1.0f / kScale; }
+__device__ __forceinline__ int power_of(const Out& o, int64_t row) { return o.weight_of == nullptr ? 0 : weight_parts(o.weight_of[row]).e; }
 
 template <typename T>
 __device__ __forceinline__ void put4_as(T* p, f32x4 v, int valid, bool vec) {
@@ -892,7 +958,8 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
   const Out& o = s.out;
   const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
-  const float alpha = s.meta->alpha;
+  constexpr bool kRows = Split<T>::kHalf && !A_COLUMNS;  // rows with powers of two of their own
+  const float alpha = factor_of(o, s.meta);
   if (!Split<T>::kSplit && splits == 1 && o.how == kFinal && o.dtype != PT_FLOAT32 && o.cols % 8 == 0) {
     // 16-bit results go through LDS, a row's 512 bytes contiguous (chunks of 16 permuted by bits of the row), and leave in whole
     // lines: 40 rows of 4096, 118914 words, whose dw is 1 GB: 438 us by 8 bytes a lane, 303 so
@@ -900,6 +967,8 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
 #pragma unroll
     for (int f = 0; f < P::FM; ++f) {
       const int row = p.wm * P::TM + f * 16 + i;
+      const int64_t at = static_cast<int64_t>(tm) * kTile + row;
+      const int power = kRows && at < limit ? power_of(o, s.first + at) : 0;
 #pragma unroll
       for (int h = 0; h < P::FN; ++h) {
         const int chunk = p.wn * (P::TN / 8) + h * 2 + g / 2;
@@ -907,7 +976,8 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
         s16x4 v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          typename Split<T>::plane e = static_cast<typename Split<T>::plane>(p.sums[f][h][k] * alpha);
+          const float sum = p.sums[f][h][k] * alpha;
+          typename Split<T>::plane e = static_cast<typename Split<T>::plane>(kRows ? ldexpf(sum, power) : sum);
           v[k] = __builtin_bit_cast(short, e);
         }
         *(lds4)(lds + row * 512 + ((chunk ^ (row & 15)) * 16) + (g & 1) * 8) = v;
@@ -932,6 +1002,7 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   for (int f = 0; f < P::FM; ++f) {
     const int64_t row = static_cast<int64_t>(tm) * kTile + p.wm * P::TM + f * 16 + i;
     if (row >= limit) continue;
+    const int power = kRows ? shift + power_of(o, s.first + row) : shift;
     const int64_t col0 = static_cast<int64_t>(tn) * kTile + p.wn * P::TN + 4 * g;
     float* part = o.parts + (static_cast<int64_t>(split) * tiles_m * kTile + row) * s.tiles_n * kTile + col0;
     const int64_t at = (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col0;
@@ -945,9 +1016,9 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
         continue;
       }
       v *= alpha;
-      if constexpr (Split<T>::kSplit) {
+      if constexpr (Split<T>::kSplit || kRows) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], shift);
+        for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], power);
       }
       if (o.how == kAdd || o.how == kAddFinal) {
         if (s.first > 0) v += *reinterpret_cast<f32x4*>(part + h * 16);
@@ -1231,7 +1302,7 @@ __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
   if (splits == 1) return;
   const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
   const int64_t quads = (o.cols + 3) / 4, ld = static_cast<int64_t>(s.tiles_n) * kTile, size = ld * tiles_m * kTile;
-  const float alpha = s.meta->alpha;
+  const float alpha = factor_of(o, s.meta);
   const bool vec = o.cols % 4 == 0;
   const int shift = s.top_b != nullptr ? -shift_of(*s.top_b) : 0;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < limit * quads; q += static_cast<int64_t>(gridDim.x) * 256) {
@@ -1240,11 +1311,10 @@ __global__ __launch_bounds__(256) void parts_kernel(Gradient s) {
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll 4
     for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(p + k * size);
+    const int power = shift + power_of(o, s.first + row);
     v *= alpha;
-    if (s.top_b != nullptr) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], shift);
-    }
+    for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], power);
     const int64_t left = o.cols - col;
     put4<T>(o.p, o.dtype, (o.row_of != nullptr ? o.row_of[s.first + row] : row) * o.cols + col, v, left < 4 ? static_cast<int>(left) : 4, vec);
   }
@@ -1417,14 +1487,14 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
   hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, p.chunk, meta, row_of, label_of,
                      target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent);
   if (dx != nullptr) {
-    s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
+    s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts, nullptr};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDx>), grid_x, dim3(256), 0, st, s);
     hipLaunchKernelGGL((narrow_parts_kernel<T, HP, kNarrowDx>), join_grid(p.rows, hidden), dim3(256), 0, st, s);
   }
   if (dw != nullptr) {
     s.outer = ow;
     s.inner = ox;
-    s.out = Out{dw, grad_dtype, kFinal, vocab, hidden, nullptr, parts};
+    s.out = Out{dw, grad_dtype, kFinal, vocab, hidden, nullptr, parts, nullptr};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDw>), grid_w, dim3(256), 0, st, s);
     hipLaunchKernelGGL((narrow_parts_kernel<T, HP, kNarrowDw>), join_grid(vocab, hidden), dim3(256), 0, st, s);
   }
@@ -1530,21 +1600,24 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows_most + 31) / 32)), dim3(1024), 0, st, sums, p.padded, tiles_v, meta, first,
                        p.chunk, row_of, label_of, target, z, row_loss, losses, r.inner, r.dx_inner);
     if (!p.grads) continue;
+    const bool apart = Split<T>::kHalf && weight_of != nullptr && dx != nullptr;
     const dim3 slope(static_cast<unsigned>(p.words / kBlockWords), static_cast<unsigned>((rows_most + kSlopeRows - 1) / kSlopeRows));
     hipLaunchKernelGGL(slope_kernel<T>, slope, dim3(256), 0, st, e,
-                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, target, z);
+                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, apart, target, z);
     const int64_t plane = p.chunk * p.words;
     if (dx != nullptr) {
       Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), kSplitX, top_w, {}};
-      d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts};
+      d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts, apart ? weight_of : nullptr};
       hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
       if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel<T>, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
     }
     if (dw != nullptr) {
+      if constexpr (Split<T>::kHalf)
+        if (apart) hipLaunchKernelGGL(weigh_kernel<T>, slope, dim3(256), 0, st, e, plane, meta, first, p.chunk, weight_of);
       const Operand oxc = columns_operand(x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2);
       const int how = p.chunks == 1 ? kFinal : (c + 1 == p.chunks ? kAddFinal : kAdd);
       Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, kSplitW, top_x, {}};
-      d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts)};
+      d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts), nullptr};
       hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
       if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel<T>, join_grid(vocab, hidden), dim3(256), 0, st, d);
     }

@@ -74,6 +74,17 @@ def check(loss, dx, dw, x, w, t, factors, scale=1.0, reduction="none", ignore=-1
             assert torch.all(off <= limit), float((off / limit).max())
 
 
+def check_rows(dx, x, w, t, factors, floor=1e-36):
+    """The states' gradients with what check allows, each state's relative to its own."""
+
+    _, want, _, total, _, slack = oracle(x, w, t, factors)
+    eps = torch.finfo(x.dtype).eps
+    part = {torch.float32: 2.0**-22}.get(x.dtype, eps / 2 + 2.0**-11) + 4 * slack + 2.0**-18 + w.shape[0] * 2.0**-24
+    limit = part * total + eps * want.abs() + floor + 2.0**-28 * total.amax(1, keepdim=True)
+    off = (dx.double() - want).abs()
+    assert torch.all(off <= limit), float((off / limit).max())
+
+
 SIZES = [(1, 1, 1), (1, 64, 260), (2, 20, 257), (33, 32, 64), (255, 64, 256), (256, 128, 255), (300, 100, 1000), (513, 200, 1027),
          (1100, 72, 3001), (700, 520, 130), (5, 192, 64), (1030, 160, 2100), (70, 129, 70000), (12, 2000, 168), (300, 1100, 90)]
 
@@ -554,3 +565,66 @@ def test_calls_of_two_threads(gpu):
     for thread in threads:
         thread.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dtype,h", [(torch.float32, 64), (torch.float32, 200), (torch.float16, 64), (torch.float16, 192), (torch.bfloat16, 64),
+                                     (torch.bfloat16, 192)])
+@pytest.mark.parametrize("n,v,chunk", [(300, 1000, 0), (40, 1000, 0), (300, 20000, 0), (600, 1000, 256)])
+def test_token_weights_far_apart(gpu, dtype, h, n, v, chunk):
+    """Weights from 1 down to 2^-60: every state's gradient is right relative to its own size, whatever the others weigh."""
+
+    x, w, t = make(n, h, v, dtype, gpu, seed=n + v)
+    power = torch.linspace(0, -60, n, device=gpu)[torch.randperm(n, generator=torch.Generator().manual_seed(2)).to(gpu)]
+    factors = power.exp2() * torch.where(torch.arange(n, device=gpu) % 3 == 0, -1.0, 1.0)
+    _, dx, dw = ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=False, want_dx=True, want_dw=True, grad_losses=factors,
+                                         grad_dtype=torch.float32, chunk_tokens=chunk)
+    check(None, None, dw, x, w, t, factors)
+    check_rows(dx, x, w, t, factors)
+    # one gradient alone: the same
+    alone = ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=False, want_dx=True, grad_losses=factors, grad_dtype=torch.float32,
+                                     chunk_tokens=chunk)[1]
+    assert torch.equal(alone, dx)
+    alone = ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=False, want_dw=True, grad_losses=factors, grad_dtype=torch.float32,
+                                     chunk_tokens=chunk)[2]
+    check(None, None, alone, x, w, t, factors)
+
+
+@pytest.mark.parametrize("h", [192, 72])
+def test_token_weights_far_apart_in_16_bits(gpu, h):
+    """Gradients in fp16, through whole lines (192) and in parts (72): from 2^14 down to 2^-10."""
+
+    x, w, t = make(300, h, 1000, torch.float16, gpu, spread=4.0)
+    factors = torch.linspace(14, -10, 300, device=gpu).exp2() * 0.75
+    x.requires_grad_()
+    loss = triton_linear_cross_entropy(x, w, t, reduction="none")
+    dx = torch.autograd.grad([loss], [x], [factors])[0]
+    check_rows(dx, x.detach(), w, t, factors, floor=2.0**-25)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h", [64, 192])
+def test_token_weights_of_any_kind(gpu, dtype, h):
+    """Zeros, the largest and smallest of fp32, all of them small, and infinities, which stay with their state."""
+
+    x, w, t = make(64, h, 300, dtype, gpu, ignored=0)
+
+    def dx_of(factors):
+        return ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=False, want_dx=True, want_dw=True, grad_losses=factors,
+                                        grad_dtype=torch.float32)[1:]
+
+    ones = torch.ones(64, device=gpu)
+    one, dw_one = dx_of(ones)
+    for power in (-80, -20, 20, 80):  # a power of two of all changes nothing else
+        dx, dw = dx_of(ones * 2.0**power)
+        assert torch.equal(dx * 2.0**-power, one) and torch.equal(dw * 2.0**-power, dw_one)
+    factors = ones.clone()
+    factors[3], factors[5], factors[7] = 0.0, 2.0**-126, 2.0**-140
+    dx, dw = dx_of(factors)
+    assert not dx[3].any()
+    keep = torch.arange(64, device=gpu) > 7
+    assert torch.equal(dx[keep], one[keep])
+    check(None, None, dw, x, w, t, factors)
+    assert not dx_of(ones * 0)[0].any() and not dx_of(ones * 0)[1].any()
+    factors[3], factors[5] = torch.inf, -torch.inf
+    dx = dx_of(factors)[0]
+    assert not dx[3].isfinite().all() and not dx[5].isfinite().all() and torch.equal(dx[keep], one[keep])
