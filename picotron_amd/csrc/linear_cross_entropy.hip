@@ -1116,7 +1116,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) adds[b] = next_adds[b];
       words = next_words;
-      hit = static_cast<unsigned>(words - static_cast<int>(o0)) < 64u;
+      hit = static_cast<unsigned>(words - static_cast<int>(o0)) < 64u || first + kNarrowInner > rows;
       if (t + 1 < to) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) next_adds[b] = *reinterpret_cast<const f32x4*>(s.exponent + first + kNarrowInner + b * 16 + 4 * g);
@@ -1208,7 +1208,8 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
           grad[f] = __builtin_bit_cast(s16x8, v.raw);
         }
         if constexpr (PASS == kNarrowDw) {
-          if (hit || s.weight_of != nullptr) {  // the labels' own entries, and the tokens' own weights
+          // the labels' own entries, the tokens' own weights, and tokens that are none: their zeros times an infinity of the weight are NaN
+          if (hit || s.weight_of != nullptr) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -1222,6 +1223,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
                 for (int f = 0; f < OF; ++f) {
                   float e = __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, adds[pair * 2 + b][k]));
                   if (w == f * 16 + i) e = d;
+                  if (!in) e = 0.f;
                   grad[f][b * 4 + k] = __builtin_bit_cast(short, static_cast<T>(e * c));
                 }
               }

@@ -628,3 +628,37 @@ def test_token_weights_of_any_kind(gpu, dtype, h):
     factors[3], factors[5] = torch.inf, -torch.inf
     dx = dx_of(factors)[0]
     assert not dx[3].isfinite().all() and not dx[5].isfinite().all() and torch.equal(dx[keep], one[keep])
+
+
+def minus_infinity(dtype, h, n, v, gpu):
+    """An infinite entry of the weight takes its word out of the softmax, and leaves everything else as it was."""
+
+    x, w, t = make(n, h, v, dtype, gpu, ignored=0)
+    t = t.masked_fill((t == 7) | (t == v - 1), 9)
+    x[:, 3] = x[:, 3].abs() + 0.5
+    out = w.clone()
+    out[7, 3] = out[v - 1, 3] = -math.inf
+    a, b = x.clone().requires_grad_(), out.clone().requires_grad_()
+    loss = triton_linear_cross_entropy(a, b, t, reduction="none")
+    assert loss.isfinite().all()
+    dx, dw = torch.autograd.grad([loss], [a, b], [torch.ones(n, device=gpu)])
+    # as if the words were not there; in the entry's column dx is 0 * -inf
+    words = (torch.arange(v, device=gpu) != 7) & (torch.arange(v, device=gpu) != v - 1)
+    place = torch.cumsum(words, 0) - 1
+    others = torch.arange(h, device=gpu) != 3
+    check(loss.detach(), None, dw[words], x, w[words], place[t], torch.ones(n, device=gpu))
+    assert not dw[~words].any()
+    losses, dx64, _, ax, _, slack = oracle(x, w[words], place[t], torch.ones(n, device=gpu))
+    part = {torch.float32: 2.0**-22}.get(dtype, torch.finfo(dtype).eps / 2 + 2.0**-11) + 4 * slack + 2.0**-18 + v * 2.0**-24
+    limit = (part + torch.finfo(dtype).eps) * ax + 2.0**-24
+    assert torch.all(((dx.double() - dx64).abs() <= limit)[:, others])
+    t[0] = 7
+    loss = triton_linear_cross_entropy(x, out, t, reduction="none")
+    assert loss[0] == math.inf and loss[1:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("h", [20, 64, 128, 192])
+@pytest.mark.parametrize("n,v", [(40, 500), (300, 500), (300, 9000), (512, 512)])
+def test_words_whose_logits_are_minus_infinity(gpu, dtype, h, n, v):
+    minus_infinity(dtype, h, n, v, gpu)
