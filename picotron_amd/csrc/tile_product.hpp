@@ -290,10 +290,17 @@ struct TileProduct {
       }
       multiply(1);
       if (SPLIT && phase == 0) {
+        // An infinity has no low plane (inf - inf), and its high one times the other side's low one may have either sign: such sums
+        // are dropped, and hi hi alone says what comes of it.  Sums of finite elements are below 2^28 a term.
 #pragma unroll
         for (int f = 0; f < FM; ++f)
 #pragma unroll
-          for (int h = 0; h < FN; ++h) sums[f][h] *= 1.0f / kLow;
+          for (int h = 0; h < FN; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float low = sums[f][h][k] * (1.0f / kLow);
+              sums[f][h][k] = fabsf(low) < INFINITY ? low : 0.f;
+            }
       }
       PT_ARRIVED();
     }

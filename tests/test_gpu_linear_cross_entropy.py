@@ -662,3 +662,27 @@ def minus_infinity(dtype, h, n, v, gpu):
 @pytest.mark.parametrize("n,v", [(40, 500), (300, 500), (300, 9000), (512, 512)])
 def test_words_whose_logits_are_minus_infinity(gpu, dtype, h, n, v):
     minus_infinity(dtype, h, n, v, gpu)
+
+
+@pytest.mark.parametrize("h", [20, 64, 192])
+@pytest.mark.parametrize("n,v", [(1, 12), (40, 500), (300, 500), (300, 9000)])
+def test_words_whose_logits_are_minus_infinity_in_32_bits(gpu, h, n, v):
+    minus_infinity(torch.float32, h, n, v, gpu)
+
+
+@pytest.mark.parametrize("n,v", [(40, 500), (300, 9000)])
+def test_infinities_in_32_bits_are_those_of_the_product(gpu, n, v):
+    """Of either sign, in states and words: each loss is what the formula gives, and tokens without one are as they were."""
+
+    x, w, t = make(n, 64, v, torch.float32, gpu, ignored=0)
+    clean = triton_linear_cross_entropy(x, w, t, reduction="none")
+    for bad in (math.inf, -math.inf, math.nan):
+        y = x.clone()
+        y[5, 3] = bad
+        loss = triton_linear_cross_entropy(y, w, t, reduction="none")
+        assert loss[5].isnan() and torch.equal(loss[torch.arange(n, device=gpu) != 5], clean[torch.arange(n, device=gpu) != 5])
+    u = w.clone()
+    u[7, 3] = math.inf  # a logit of +inf or -inf, by the state's sign
+    t = t.masked_fill(t == 7, 9)
+    loss = triton_linear_cross_entropy(x, u, t, reduction="none")
+    assert torch.equal(loss.isnan(), x[:, 3] > 0) and loss[x[:, 3] < 0].isfinite().all()
