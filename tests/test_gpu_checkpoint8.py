@@ -420,3 +420,76 @@ def test_many_rows(gpu):
     want, total = (x.double() * kept).sum(0), (x.double() * kept).abs().sum(0)
     # each slot adds up some thousands of rows one after the other, in fp32
     assert torch.all((dw.double() - want).abs() <= 2.0**-24 * (rows // 8192 + 40) * total)
+
+
+def operators(gpu):
+    x, r, d = (randn((40, 300), torch.bfloat16, gpu, seed) for seed in (1, 2, 3))
+    w = randn((300,), torch.float32, gpu, 4, 0.1, 1.0)
+    return d, [(lambda a, b: triton_swiglu(a, b, checkpoint_8bit=True), (x, r)),
+               (lambda a, b: triton_rms_norm(a, b, EPS, checkpoint_8bit=True), (x, w)),
+               (lambda a, b, c: torch.stack(triton_residual_rms_norm(a, b, c, EPS, checkpoint_8bit=True)), (x, r, w))]
+
+
+def test_saved_tensors_hooks(gpu):
+    """Codes, steps and small tensors go through them, no input does."""
+
+    d, cases = operators(gpu)
+    for f, inputs in cases:
+        packed = []
+
+        def pack(tensor):
+            packed.append(tensor)
+            return tensor.cpu()
+
+        grads = []
+        for hooks in (False, True):
+            leaves = [t.detach().requires_grad_() for t in inputs]
+            if hooks:
+                with torch.autograd.graph.saved_tensors_hooks(pack, lambda tensor: tensor.to(gpu)):
+                    y = f(*leaves)
+            else:
+                y = f(*leaves)
+            grads.append(torch.autograd.grad(y, leaves, d.expand_as(y)))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+        assert any(t.dtype == torch.uint8 for t in packed) and not any(t.dtype == torch.bfloat16 for t in packed)
+
+
+@pytest.mark.parametrize("use_reentrant", [False, True])
+def test_under_activation_checkpointing(gpu, use_reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    d, cases = operators(gpu)
+    for f, inputs in cases:
+        grads = []
+        for run in (f, lambda *a, f=f: checkpoint(f, *a, use_reentrant=use_reentrant)):
+            leaves = [t.detach().requires_grad_() for t in inputs]
+            y = run(*(t * 1 for t in leaves))
+            y.backward(d.expand_as(y))
+            grads.append([t.grad for t in leaves])
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_transforms_are_refused(gpu):
+    d, cases = operators(gpu)
+    for f, inputs in cases:
+        for transform in (lambda: torch.func.grad(lambda a: f(a, *inputs[1:]).sum())(inputs[0]),
+                          lambda: torch.func.jvp(lambda a: f(a, *inputs[1:]), (inputs[0],), (d,)),
+                          lambda: torch.func.vmap(lambda a: f(a, *(t[0] if t.dim() == 2 else t for t in inputs[1:])))(inputs[0])):
+            with pytest.raises(RuntimeError):
+                transform()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(5, 7), (40, 128), (30, 1090), (20, 4096), (7, 16385)])
+def test_norm_is_the_one_without_the_option_to_a_rounding(gpu, dtype, rows, cols):
+    """Other lanes add a row's squares in another order: the inverse RMS differs by its last bits, and y by a rounding more."""
+
+    x, r = randn((rows, cols), dtype, gpu, 1), randn((rows, cols), dtype, gpu, 2, 2.0)
+    w = randn((cols,), torch.float32, gpu, 3, 0.1, 1.0).requires_grad_()
+    h, y = triton_residual_rms_norm(x, r, w, EPS, checkpoint_8bit=True)
+    other_h, other = triton_residual_rms_norm(x, r, w, EPS)
+    assert torch.equal(h, other_h)
+    for a, b in ((y, other), (triton_rms_norm(x, w, EPS, checkpoint_8bit=True), triton_rms_norm(x, w, EPS))):
+        # two sums of cols positive terms, half their errors in the root; a division and a root; a rounding to the type each
+        limit = b.double().abs() * ((cols + 16) * 2.0**-24 + torch.finfo(dtype).eps)
+        assert torch.all((a.double() - b.double()).abs() <= limit + (2.0**-24 if dtype == torch.float16 else 0))

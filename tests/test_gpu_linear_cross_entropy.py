@@ -686,3 +686,68 @@ def test_infinities_in_32_bits_are_those_of_the_product(gpu, n, v):
     t = t.masked_fill(t == 7, 9)
     loss = triton_linear_cross_entropy(x, u, t, reduction="none")
     assert torch.equal(loss.isnan(), x[:, 3] > 0) and loss[x[:, 3] < 0].isfinite().all()
+
+
+def gradients_of(run, x, w):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = run(x, w)
+    return (loss.detach(), *torch.autograd.grad(loss.sum(), [x, w]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_saved_tensors_hooks(gpu, dtype, reduction):
+    """What a deferred loss saves goes through them; a mean's or sum's gradients, which are no saved tensors, do not."""
+
+    x, w, t = make(600, 64, 300, dtype, gpu)
+    packed = []
+
+    def pack(tensor):
+        packed.append(tensor.shape)
+        return tensor.cpu()
+
+    def hooked(a, b):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda tensor: tensor.to(gpu)):
+            return triton_linear_cross_entropy(a, b, t, reduction=reduction)
+
+    got = gradients_of(hooked, x, w)
+    want = gradients_of(lambda a, b: triton_linear_cross_entropy(a, b, t, reduction=reduction), x, w)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert sorted(map(tuple, packed)) == ([] if reduction == "mean" else [(300, 64), (600,), (600, 64)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("use_reentrant", [False, True])
+def test_under_activation_checkpointing(gpu, dtype, reduction, use_reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    x, w, t = make(90, 64, 300, dtype, gpu)
+
+    def head(a, b):
+        return triton_linear_cross_entropy(a.tanh(), b, t, reduction=reduction)
+
+    want = gradients_of(lambda a, b: head(a.sin(), b), x, w)
+    a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = checkpoint(head, a.sin(), b, use_reentrant=use_reentrant)
+    loss.sum().backward()
+    assert all(torch.equal(p, q) for p, q in zip((loss.detach(), a.grad, b.grad), want))
+
+
+def test_transforms_are_refused_and_fall_back(gpu):
+    """Forward-mode and functorch's transforms see no derivative of the kernels: an error, or the PyTorch form's."""
+
+    x, w, t = make(20, 64, 30, torch.float32, gpu)
+    head = LinearCrossEntropyWithFallback(use_triton=True)
+    plain = LinearCrossEntropyWithFallback()
+    along = torch.randn(20, 64, device=gpu)
+    for transform in (lambda f: torch.func.grad(lambda a: f(a, w, t))(x), lambda f: torch.func.jvp(lambda a: f(a, w, t), (x,), (along,))[1],
+                      lambda f: torch.func.vmap(lambda a: f(a[None], w, t[:1]))(x)):
+        with pytest.raises(RuntimeError):
+            transform(triton_linear_cross_entropy)
+        head._fallback_warned = False
+        with pytest.warns(RuntimeWarning, match="linear cross-entropy unavailable"):
+            got = transform(head)
+        assert torch.equal(got, transform(plain))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        triton_linear_cross_entropy(torch.autograd.forward_ad.make_dual(x, along), w, t)
