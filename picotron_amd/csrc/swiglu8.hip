@@ -16,71 +16,49 @@ using namespace block8;
 
 __device__ __forceinline__ float sigmoid8(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
-template <typename T, bool ALIGNED, bool NT, int UNROLL>
+template <typename T, bool ALIGNED, bool NT>
 __global__ __launch_bounds__(256) void swiglu8_fwd_kernel(const T* __restrict__ g, const T* __restrict__ u, T* __restrict__ o,
                                                           u32x4* __restrict__ codes, float2* __restrict__ steps, int64_t n) {
   const int64_t units = (n + kBlock - 1) / kBlock * (kBlock / kUnit);  // whole blocks
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 * UNROLL + threadIdx.x;
-  Unit<T> gv[UNROLL], uv[UNROLL];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  Unit<T> gv, uv, out;
+  gv.template load<ALIGNED, NT>(g + i * kUnit, n - i * kUnit);
+  uv.template load<ALIGNED, NT>(u + i * kUnit, n - i * kUnit);
+  const Step a = step_of(row16_max(gv.top())), b = step_of(row16_max(uv.top()));
+  const u32x2 ca = encode(gv, a.inv), cb = encode(uv, b.inv);
 #pragma unroll
-  for (int k = 0; k < UNROLL; ++k) {
-    const int64_t i = first + k * 256;
-    gv[k].template load<ALIGNED, NT>(g + i * kUnit, n - i * kUnit);
-    uv[k].template load<ALIGNED, NT>(u + i * kUnit, n - i * kUnit);
+  for (int e = 0; e < kUnit; ++e) {
+    const float x = gv.at(e);
+    out.set(e, (x * sigmoid8(x)) * uv.at(e));
   }
-#pragma unroll
-  for (int k = 0; k < UNROLL; ++k) {
-    const int64_t i = first + k * 256;
-    const Step a = step_of(row16_max(gv[k].top())), b = step_of(row16_max(uv[k].top()));
-    const u32x2 ca = encode(gv[k], a.inv), cb = encode(uv[k], b.inv);
-    Unit<T> out;
-#pragma unroll
-    for (int e = 0; e < kUnit; ++e) {
-      const float x = gv[k].at(e);
-      out.set(e, (x * sigmoid8(x)) * uv[k].at(e));
-    }
-    if (i < units) {
-      store16<NT>(codes + i, u32x4{ca[0], ca[1], cb[0], cb[1]});
-      if (threadIdx.x % 16 == 0) steps[i / 16] = float2{a.step, b.step};
-      out.template store<ALIGNED, NT>(o + i * kUnit, n - i * kUnit);
-    }
+  if (i < units) {
+    store16<NT>(codes + i, u32x4{ca[0], ca[1], cb[0], cb[1]});
+    if (threadIdx.x % 16 == 0) steps[i / 16] = float2{a.step, b.step};
+    out.template store<ALIGNED, NT>(o + i * kUnit, n - i * kUnit);
   }
 }
 
-template <typename T, bool ALIGNED, bool NT, int UNROLL>
+template <typename T, bool ALIGNED, bool NT>
 __global__ __launch_bounds__(256) void swiglu8_bwd_kernel(const T* __restrict__ dy, const u32x4* __restrict__ codes,
                                                           const float2* __restrict__ steps, T* __restrict__ dg, T* __restrict__ du,
                                                           int64_t n) {
   const int64_t units = (n + kUnit - 1) / kUnit;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 * UNROLL + threadIdx.x;
-  Unit<T> d[UNROLL];
-  u32x4 c[UNROLL];
-  float2 s[UNROLL];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= units) return;
+  const u32x4 c = load16<NT>(codes + i);
+  const float2 s = steps[i / 16];
+  Unit<T> d, a, b;
+  d.template load<ALIGNED, NT>(dy + i * kUnit, n - i * kUnit);
+  const u32x2 ca = {c[0], c[1]}, cb = {c[2], c[3]};
 #pragma unroll
-  for (int k = 0; k < UNROLL; ++k) {
-    const int64_t i = first + k * 256;
-    if (i < units) {
-      c[k] = load16<NT>(codes + i);
-      s[k] = steps[i / 16];
-      d[k].template load<ALIGNED, NT>(dy + i * kUnit, n - i * kUnit);
-    }
+  for (int e = 0; e < kUnit; ++e) {
+    const float x = decode(ca, e, s.x), up = decode(cb, e, s.y), grad = d.at(e);
+    const float sig = sigmoid8(x);
+    a.set(e, (grad * up) * (sig * (1.0f + x * (1.0f - sig))));
+    b.set(e, grad * (x * sig));
   }
-#pragma unroll
-  for (int k = 0; k < UNROLL; ++k) {
-    const int64_t i = first + k * 256;
-    if (i >= units) break;
-    const u32x2 ca = {c[k][0], c[k][1]}, cb = {c[k][2], c[k][3]};
-    Unit<T> a, b;
-#pragma unroll
-    for (int e = 0; e < kUnit; ++e) {
-      const float x = decode(ca, e, s[k].x), up = decode(cb, e, s[k].y), grad = d[k].at(e);
-      const float sig = sigmoid8(x);
-      a.set(e, (grad * up) * (sig * (1.0f + x * (1.0f - sig))));
-      b.set(e, grad * (x * sig));
-    }
-    if (dg != nullptr) a.template store<ALIGNED, NT>(dg + i * kUnit, n - i * kUnit);
-    if (du != nullptr) b.template store<ALIGNED, NT>(du + i * kUnit, n - i * kUnit);
-  }
+  if (dg != nullptr) a.template store<ALIGNED, NT>(dg + i * kUnit, n - i * kUnit);
+  if (du != nullptr) b.template store<ALIGNED, NT>(du + i * kUnit, n - i * kUnit);
 }
 
 // A launch has fewer than 2^32 work-items: 2^30 units, 2^33 elements, at a time.
@@ -93,7 +71,7 @@ int fwd8(const void* g, const void* u, void* o, void* codes, float* steps, int64
   const bool nt = n * static_cast<int64_t>(sizeof(T)) > (int64_t{1} << 25);
   const dim3 grid(static_cast<unsigned>((units + 255) / 256));
 #define PT_FWD8(A, N)                                                                                                       \
-  hipLaunchKernelGGL((swiglu8_fwd_kernel<T, A, N, 1>), grid, dim3(256), 0, st, static_cast<const T*>(g), static_cast<const T*>(u), \
+  hipLaunchKernelGGL((swiglu8_fwd_kernel<T, A, N>), grid, dim3(256), 0, st, static_cast<const T*>(g), static_cast<const T*>(u), \
                      static_cast<T*>(o), static_cast<u32x4*>(codes), reinterpret_cast<float2*>(steps), n)
   if (aligned) {
     if (nt) PT_FWD8(true, true);
@@ -113,7 +91,7 @@ int bwd8(const void* dy, const void* codes, const float* steps, void* dg, void* 
   const bool nt = n * static_cast<int64_t>(sizeof(T)) > (int64_t{1} << 25);
   const dim3 grid(static_cast<unsigned>((units + 255) / 256));
 #define PT_BWD8(A, N)                                                                                                        \
-  hipLaunchKernelGGL((swiglu8_bwd_kernel<T, A, N, 1>), grid, dim3(256), 0, st, static_cast<const T*>(dy),                          \
+  hipLaunchKernelGGL((swiglu8_bwd_kernel<T, A, N>), grid, dim3(256), 0, st, static_cast<const T*>(dy),                          \
                      static_cast<const u32x4*>(codes), reinterpret_cast<const float2*>(steps), static_cast<T*>(dg), static_cast<T*>(du), n)
   if (aligned) {
     if (nt) PT_BWD8(true, true);
