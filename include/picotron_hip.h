@@ -438,16 +438,16 @@ int pt_adamw8_moments(const int64_t* table, int64_t n_tensors, int64_t total_blo
  * is not ignore_index: their mean (NaN of none) or sum as one fp32 value, or with PT_REDUCTION_NONE each row's, fp32
  * [outer, inner], 0 at ignored rows.  A label outside the vocabulary gives NaN, in the loss and in every gradient it
  * enters.  The logits are never held whole: exponentials of at most 2 GiB (chunk_rows rows, where that is fewer;
- * 0: as many as fit) are.  x and weight share `dtype`; fp32 operands are multiplied as two fp16 planes
+ * 0 or less: as many as fit; a multiple of 256 is taken) are.  x and weight share `dtype`; fp32 operands are multiplied as two fp16 planes
  * each (22 bits and a sign, relative to the tensor's largest element down to 2^-28 of it).
  * Gradients, where dx or dw is non-NULL: dx [outer, dx_inner, hidden] contiguous (rows inner.. and ignored rows zero),
  * dw [vocab, hidden] contiguous, of grad_dtype (dtype or fp32), for the incoming gradient dloss: of the mean or sum one
  * fp32 value (NULL: 1), of the loss without a reduction one a row (fp32, the given strides).  16-byte aligned.
- * A row of dx is exact relative to its own weight, whatever the others are; in dw, whose sums go over the rows, fp16 and fp32 inputs'
- * terms have fewer bits where weight times softmax lies below 2^-28 of the call's largest weight, in fp16 none below 2^-39.
+ * A row of dx is as accurate relative to its own weight as to any other's; in dw, whose sums go over the rows, a row's terms have
+ * fewer bits where weight times softmax lies below 2^-28 of the call's largest weight (fp16 and fp32 inputs; fp16: none below 2^-39).
  * loss may be NULL where gradients are asked for.  workspace: 256-byte aligned, _workspace_bytes for the same arguments.
- *   pt_scale_gradients: to = from * scale (fp32 device scalar), rounded once, of up to two arrays: in place, or from fp32 to
- *     another type.  Nothing is touched in place for a scale of 1.
+ *   pt_scale_gradients: to = from * scale (fp32 device scalar), of up to two arrays: in place, or from fp32 to another type.
+ *     The products are rounded once; what came rounded to 16 bits is so rounded twice.  Nothing is touched in place for a scale of 1.
  * Replaces the head's product and F.cross_entropy behind it (src/picotron/training/train_loop.py:136-145). */
 #define PT_REDUCTION_MEAN 0
 #define PT_REDUCTION_SUM 1

@@ -10,8 +10,9 @@
 // - Tokens whose label is ignored take no part: the kept rows of x are gathered first, and their number stays on the device.
 // - The first product's workgroups, a tile of 256 tokens by 256 words each, leave exp(l - m) with m the largest logit
 //   of the token in the tile, and m and the sum of the tile: one pass, no logits.  From z a second pass makes G of it
-//   in place: an exp for each token and tile, a product for each element, and at the label expm1(l_t - z), which
-//   keeps its accuracy where the softmax is close to 1.
+//   in place: an exp for each token and tile, a product for each element, and at the label expm1(-loss).
+// - Where the softmax is close to 1 at the label, the loss is a small difference of z and l_t: it is taken as
+//   (top - l_t) + ln sum exp(l - top), top the row's largest logit, and the sum holds exactly 1 for the largest.
 // - With 16-bit inputs exp(l - m) is held as fp16 scaled by 2^14: 11 bits where the largest bf16 error below is 8,
 //   down to 2^-28 of the tile's largest.  G is rounded to the inputs' type, as the matrix cores take it, scaled by 2^14
 //   too (fp16 keeps softmax values down to 2^-28 normal), and the scale is taken out of the fp32 sums.
@@ -550,6 +551,8 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
       }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
+    // `start` is rounded, by up to |top| 2^-23: all of the row's exponentials are off by what the largest is off by
+    sum = Split<T>::kSplit ? sum * (1.0f / kScale) : sum / __builtin_amdgcn_exp2f(__builtin_fmaf(top, kLog2e, start));
     if (g == 0) red[p.wn * BM + p.wm * P::TM + f * 16 + i] = sum;
     if (to != nullptr) {
       Vec16<_Float16> v[2], low[2];
@@ -576,7 +579,7 @@ __global__ __launch_bounds__(BM * 2 < 256 ? 256 : BM * 2) void scores_kernel(Sco
   const int m = threadIdx.x;
   if (m < BM && tm * BM + m < rows) {
     const float sum = (red[m] + red[BM + m]) + (red[2 * BM + m] + red[3 * BM + m]);
-    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * BM + m)[1] = sum * (1.0f / kScale);
+    reinterpret_cast<float*>(s.sums + static_cast<int64_t>(tn) * s.padded + tm * BM + m)[1] = sum;
   }
   if (p.wn == 0 && g == 0) {
 #pragma unroll
@@ -730,8 +733,8 @@ __device__ __forceinline__ void join_rows(const f32x2* __restrict__ sums, int64_
   sum = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) sum += tops[k][c] == -INFINITY ? parts[k][c] : parts[k][c] * __expf(tops[k][c] - top);
-  const float lse = top + logf(sum);
-  const float loss = label_of[first + row] < 0 ? NAN : lse - target[first + row];
+  const float rest = logf(sum), lse = top + rest;
+  const float loss = label_of[first + row] < 0 ? NAN : (top - target[first + row]) + rest;
   z[first + row] = lse;
   row_loss[first + row] = loss;
   // the softmax times kScale is exp2(l * log2(e) + exponent); a label outside the vocabulary leaves a NaN, as its loss
@@ -789,7 +792,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, const f32x2* __restrict__ sums, int64_t padded,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
                                                     const int* __restrict__ label_of, const float* __restrict__ weight_of, bool apart,
-                                                    const float* __restrict__ target, const float* __restrict__ z) {
+                                                    const float* __restrict__ row_loss, const float* __restrict__ z) {
   typedef typename Split<T>::plane P;
   constexpr int kPer = kSlopeRows / 32;
   const int rows = rows_here(meta, first, chunk);
@@ -831,7 +834,7 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
         out[i] *= factor;
       }
       if (place >= 0 && place < 8) {
-        const float d = expm1f(target[first + row] - lse) * weight * kScale;
+        const float d = expm1f(-row_loss[first + row]) * weight * kScale;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (i == place) out[i] = d;
@@ -1043,7 +1046,7 @@ struct Narrow {
   f32x2* sums;  // (splits, outer tiles * 256)
   float* target;
   const float* exponent;
-  const float* z;
+  const float* row_loss;
   Out out;
 };
 
@@ -1089,7 +1092,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
     label[f] = PASS != kNarrowDw && o < rows ? s.label_of[o] : -1;
     if constexpr (PASS == kNarrowDx) {
       add[f] = s.exponent[o];
-      at_label[f] = o < rows ? expm1f(s.target[o] - s.z[o]) * kScale : 0.f;
+      at_label[f] = o < rows ? expm1f(-s.row_loss[o]) * kScale : 0.f;
     }
   }
 
@@ -1167,10 +1170,12 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
           sum[f] *= __builtin_amdgcn_exp2f((top[f] - level) * kLog2e);
           top[f] = most;
           const float start = -level * kLog2e;
+          float e[8];
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, start));
+            for (int k = 0; k < 4; ++k) e[b * 4 + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[b][f][k], kLog2e, start));
+          sum[f] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));  // an eighth of the roundings near the sum's size
           const int place = label[f] - base;
           if (hit && place >= 0 && place < 20 && (place & 15) < 4) {
             float v = 0.f;
@@ -1217,7 +1222,7 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
                 const int at = base + b * 16 + k;
                 const bool in = at < rows;
                 const int w = in ? s.label_of[at] - static_cast<int>(o0) : -1;
-                const float d = in && w >= 0 && w < 64 ? expm1f(s.target[at] - s.z[at]) * kScale : 0.f;
+                const float d = in && w >= 0 && w < 64 ? expm1f(-s.row_loss[at]) * kScale : 0.f;
                 const float c = in && s.weight_of != nullptr ? s.weight_of[at] * s.meta->inv_weight : 1.f;
 #pragma unroll
                 for (int f = 0; f < OF; ++f) {
@@ -1245,7 +1250,11 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
     if constexpr (PASS == kNarrowSums) {
       float most = fmaxf(top[f], __shfl_xor(top[f], 16));
       most = fmaxf(most, __shfl_xor(most, 32));
-      float all = top[f] == -INFINITY ? sum[f] : sum[f] * __builtin_amdgcn_exp2f((top[f] - most) * kLog2e);
+      float all = sum[f];
+      if (top[f] != -INFINITY) {  // over what the largest's exponential is, as in scores_kernel
+        all /= __builtin_amdgcn_exp2f(__builtin_fmaf(top[f], kLog2e, -top[f] * kLog2e));
+        all *= __builtin_amdgcn_exp2f((top[f] - most) * kLog2e);
+      }
       all += __shfl_xor(all, 16);
       all += __shfl_xor(all, 32);
       if (g == 0 && o < rows) s.sums[static_cast<int64_t>(split) * outer_tiles * kNarrowOuter + o] = f32x2{most, all};
@@ -1480,14 +1489,15 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
   const int* label_of = reinterpret_cast<const int*>(ws + p.label_of);
   float* target = reinterpret_cast<float*>(ws + p.target);
   float* z = reinterpret_cast<float*>(ws + p.z);
+  float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
   float* exponent = reinterpret_cast<float*>(ws + p.exponent);
   f32x2* sums = reinterpret_cast<f32x2*>(ws + p.sums);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
-  Narrow s{ox, ow, meta, label_of, weight_of, vocab, p.chunk, sums, target, exponent, z, {}};
+  Narrow s{ox, ow, meta, label_of, weight_of, vocab, p.chunk, sums, target, exponent, row_loss, {}};
   const dim3 grid_x(static_cast<unsigned>(p.grid_x)), grid_w(static_cast<unsigned>(p.grid_w));
   hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowSums>), grid_x, dim3(256), 0, st, s);
   hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, p.chunk, meta, row_of, label_of,
-                     target, z, reinterpret_cast<float*>(ws + p.row_loss), losses, r.inner, r.dx_inner, exponent);
+                     target, z, row_loss, losses, r.inner, r.dx_inner, exponent);
   if (dx != nullptr) {
     s.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts, nullptr};
     hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowDx>), grid_x, dim3(256), 0, st, s);
@@ -1605,7 +1615,7 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     const bool apart = Split<T>::kHalf && weight_of != nullptr && dx != nullptr;
     const dim3 slope(static_cast<unsigned>(p.words / kBlockWords), static_cast<unsigned>((rows_most + kSlopeRows - 1) / kSlopeRows));
     hipLaunchKernelGGL(slope_kernel<T>, slope, dim3(256), 0, st, e,
-                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, apart, target, z);
+                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, apart, row_loss, z);
     const int64_t plane = p.chunk * p.words;
     if (dx != nullptr) {
       Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), kSplitX, top_w, {}};

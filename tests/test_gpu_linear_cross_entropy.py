@@ -751,3 +751,49 @@ def test_transforms_are_refused_and_fall_back(gpu):
         assert torch.equal(got, transform(plain))
     with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
         triton_linear_cross_entropy(torch.autograd.forward_ad.make_dual(x, along), w, t)
+
+
+def confident(n, h, v, dtype, gpu, level):
+    """Labels ahead of all other words by 0 to 24, every logit near ``level``."""
+
+    x, w, t = make(n, h, v, dtype, gpu, ignored=0, spread=0.5)
+    x = x * 0.25
+    x[:, 0], w[:, 0] = 8.0, level / 8  # exact in each type
+    direction = w[t, 1:].double()
+    gap = torch.linspace(0, 24, n, device=gpu, dtype=torch.float64)[:, None]
+    x[:, 1:] = (x[:, 1:].double() + gap * direction / direction.square().sum(1, keepdim=True)).to(dtype)
+    return x, w, t
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h", [20, 64, 192])
+@pytest.mark.parametrize("n,v", [(50, 300), (300, 1000), (300, 9000)])
+@pytest.mark.parametrize("level", [0, 40, -90])
+def test_confident_labels(gpu, dtype, h, n, v, level):
+    """A softmax close to 1 at the label: the loss and its gradient are right to a few roundings of 1, not of the logits' level."""
+
+    x, w, t = confident(n, h, v, dtype, gpu, level)
+    one = torch.ones(n, device=gpu)
+    loss, dx, dw = ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=True, want_dx=True, want_dw=True, grad_losses=one,
+                                            grad_dtype=torch.float32)
+    losses, dx64, dw64, ax, aw, slack = oracle(x, w, t, one)
+    rest = -torch.expm1(-losses)  # of the softmax, beside the label's
+    # logits that are off by the slack move the loss by twice that times the rest; the sum of exponentials near 1, its logarithm
+    # and exp - 1 round a few times to 24 bits; a narrow model's sum grows by 8 words of every 32 at a time, each time rounded by half
+    # a step of 2^-23 while it lies below 2
+    few = 2.0**-21 + v / 32 * 2.0**-24
+    assert torch.all((loss.double() - losses).abs() <= 2 * slack * rest + few * (1 + losses))
+    part = {torch.float32: 2.0**-22}.get(dtype, torch.finfo(dtype).eps / 2 + 2.0**-11) + 4 * slack + 2.0**-18 + max(n, v) * 2.0**-24
+    at_label = torch.zeros_like(dw64).index_add_(0, t, x.double().abs())
+    floor = 2.0**-28 * float(ax.max())
+    assert torch.all((dx.double() - dx64).abs() <= part * ax + few * w[t].double().abs() + floor)
+    assert torch.all((dw.double() - dw64).abs() <= part * aw + few * at_label + 2.0**-28 * float(aw.max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h", [64, 192])
+def test_a_vocabulary_of_one_word(gpu, dtype, h):
+    x, w, t = make(300, h, 1, dtype, gpu, ignored=0, spread=30.0)
+    loss, dx, dw = ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=True, want_dx=True, want_dw=True,
+                                            grad_losses=torch.ones(300, device=gpu))
+    assert not loss.any() and not dx.any() and not dw.any()
