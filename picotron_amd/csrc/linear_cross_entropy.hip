@@ -450,6 +450,54 @@ using Product = TileProduct<typename Split<T>::plane, Split<T>::kSplit, BM, kTil
 // way from memory.  One token of 4096 at 128256 words: 247 us in tiles of 256.
 constexpr int kFewRows = 64;
 
+// 16-bit inputs: rounding G's entry at the label moves a whole row of dx, and of dw, by up to half a step of the type.  Over many
+// tokens that is as much as the results' own rounding, 1.4 times the error in all; over a few it may be 2.4 times.  Calls of up to
+// so many rows keep what is rounded off in fp32, and add it times the label's word (or the token's state) to the sums: 256 tokens,
+// 128256 words of 4096, bf16: 1.10 ms, without 1.06; 260 words of 2048, where each tile has half of the labels: 102 us, without 84.
+constexpr int kExactRows = 256;
+
+// What rounding v to T takes off; 0 where that is no number.
+template <typename T>
+__device__ __forceinline__ float rounded_off(float v) {
+  const float r = v - static_cast<float>(static_cast<T>(v));
+  return fabsf(r) < INFINITY ? r : 0.f;
+}
+
+// sum += r * (four elements), where there is a residual: 0 times an infinity would be a NaN.
+template <typename T4>
+__device__ __forceinline__ void add_times(f32x4* sum, float r, T4 v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) (*sum)[k] += r * (r != 0.f ? static_cast<float>(v[k]) : 0.f);
+}
+
+// Calls f(token, word) for the tokens of [begin, end), below kExactRows, whose label is one of the `count` words from `first` on,
+// those of a word in order, by a whole wave: lane i of each sixteen takes the words i, i + 16, ..., and -1 as the word while others
+// have more.
+template <typename F>
+__device__ __forceinline__ void for_labels(const int* label_of, int begin, int end, int first, int count, F&& f) {
+  const int lane = threadIdx.x % 64, i = lane % 16;
+  int words[kExactRows / 64];
+#pragma unroll
+  for (int b = 0; b < kExactRows / 64; ++b) {
+    const int at = b * 64 + lane, label = at >= begin && at < end ? label_of[at] : -1;
+    words[b] = label >= first && label - first < count ? label - first : -1;
+  }
+#pragma unroll
+  for (int b = 0; b < kExactRows / 64; ++b) {
+    if (!__any(words[b] >= 0)) continue;
+    uint64_t mine = 0;
+    for (int j = 0; j < 16; ++j) {
+      const uint64_t all = __ballot(words[b] >= 0 && words[b] % 16 == j);
+      mine = i == j ? all : mine;
+    }
+    while (__any(mine != 0)) {
+      const int from = mine != 0 ? __builtin_ctzll(mine) : 0, word = __shfl(words[b], from);
+      f(b * 64 + from, mine != 0 ? word : -1);
+      mine &= mine - 1;
+    }
+  }
+}
+
 __device__ __forceinline__ int rows_here(const Meta* meta, int64_t first, int64_t chunk) {
   const int64_t n = meta->count - first;
   return static_cast<int>(n < 0 ? 0 : (n > chunk ? chunk : n));
@@ -792,7 +840,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, int64_t plane, const f32x2* __restrict__ sums, int64_t padded,
                                                     const Meta* __restrict__ meta, int64_t first, int64_t chunk,
                                                     const int* __restrict__ label_of, const float* __restrict__ weight_of, bool apart,
-                                                    const float* __restrict__ row_loss, const float* __restrict__ z) {
+                                                    const float* __restrict__ row_loss, const float* __restrict__ z,
+                                                    float* __restrict__ residual) {
   typedef typename Split<T>::plane P;
   constexpr int kPer = kSlopeRows / 32;
   const int rows = rows_here(meta, first, chunk);
@@ -838,6 +887,7 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (i == place) out[i] = d;
+        if (!Split<T>::kSplit && residual != nullptr) residual[row] = rounded_off<P>(d);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -854,7 +904,7 @@ __global__ __launch_bounds__(256) void slope_kernel(_Float16* __restrict__ e, in
 // among the subnormals.  Threads as in slope_kernel; rows within a factor of two of the largest are left alone.
 template <typename T>
 __global__ __launch_bounds__(256) void weigh_kernel(_Float16* __restrict__ e, int64_t plane, const Meta* __restrict__ meta, int64_t first,
-                                                    int64_t chunk, const float* __restrict__ weight_of) {
+                                                    int64_t chunk, const float* __restrict__ weight_of, float* __restrict__ residual) {
   constexpr int kPer = kSlopeRows / 32;
   const int rows = rows_here(meta, first, chunk);
   const int row0 = static_cast<int>(blockIdx.y) * kSlopeRows + threadIdx.x / 8;
@@ -868,6 +918,7 @@ __global__ __launch_bounds__(256) void weigh_kernel(_Float16* __restrict__ e, in
     const int row = row0 + k * 32;
     by[k] = row < rows ? weight_parts(weight_of[first + row]).e - meta->unit : 0;
     if (by[k] == 0) continue;
+    if (residual != nullptr && blockIdx.x == 0 && threadIdx.x % 8 == 0) residual[row] = ldexpf(residual[row], by[k]);
     v[k].raw = *reinterpret_cast<const u32x4*>(at + k * 2048);
     if constexpr (Split<T>::kSplit) low[k].raw = *reinterpret_cast<const u32x4*>(at + k * 2048 + plane);
   }
@@ -938,11 +989,60 @@ struct Gradient {
   int which;             // of the splits
   const unsigned* top_b;  // of b's magnitudes (32-bit inputs)
   Out out;
+  const int* label_of;
+  const float* residual;  // what the rounding of G's entries at the labels took off, or null
 };
 
-template <typename T, bool A_COLUMNS>
-__global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
-  extern __shared__ char lds_raw[];
+// What the rounding of G's entries at the labels took off, to a tile's sums (see kExactRows).  dx: times the label's word.
+template <typename T, typename P>
+__device__ __forceinline__ void exact_dx(P* p, const Gradient& s, int tm, int tn, int rows) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+  const int64_t col = static_cast<int64_t>(tn) * kTile + p->wn * P::TN + 4 * g;
+  const T* const b = static_cast<const T*>(s.b.p) + col;
+  int words[P::FM];
+  float r[P::FM];
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f) {
+    const int row = tm * kTile + p->wm * P::TM + f * 16 + i;
+    words[f] = row < rows ? s.label_of[row] : -1;
+    r[f] = words[f] >= 0 ? s.residual[row] : 0.f;
+  }
+#pragma unroll
+  for (int f = 0; f < P::FM; ++f)
+#pragma unroll
+    for (int h = 0; h < P::FN; ++h)
+      if (col + h * 16 < s.out.cols) add_times(&p->sums[f][h], r[f], *reinterpret_cast<const T4*>(b + (words[f] < 0 ? 0 : words[f]) * s.b.ld + h * 16));
+}
+
+// dw, of the part's tokens: times their states.
+template <typename T, typename P>
+__device__ __forceinline__ void exact_dw(P* p, const Gradient& s, int tm, int tn, int rows, int from, int to) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const int g = threadIdx.x % 64 / 16;
+  const int64_t col = static_cast<int64_t>(tn) * kTile + p->wn * P::TN + 4 * g;
+  const T* const b = static_cast<const T*>(s.b.p) + col;
+  for_labels(s.label_of, from * kStep, to * kStep < rows ? to * kStep : rows, tm * kTile + p->wm * P::TM, P::TM, [&](int token, int word) {
+    const float r = word >= 0 ? s.residual[token] : 0.f;
+    f32x4 v[P::FN];
+#pragma unroll
+    for (int h = 0; h < P::FN; ++h) {
+      T4 e = {};
+      if (col + h * 16 < s.out.cols) e = *reinterpret_cast<const T4*>(b + token * s.b.ld + h * 16);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[h][k] = r != 0.f ? static_cast<float>(e[k]) : 0.f;
+    }
+#pragma unroll
+    for (int f = 0; f < P::FM; ++f) {
+      const float rf = word / 16 == f ? r : 0.f;
+#pragma unroll
+      for (int h = 0; h < P::FN; ++h) p->sums[f][h] += v[h] * rf;
+    }
+  });
+}
+
+template <typename T, bool A_COLUMNS, bool EXACT>
+__device__ __forceinline__ void gradient_tile(const Gradient& s, char* lds_raw) {
   typedef Product<T, A_COLUMNS, true> P;
   const int rows = rows_here(s.meta, s.first, s.chunk);
   const int tiles_m = s.tiles_m < 0 ? (rows + kTile - 1) / kTile : s.tiles_m;
@@ -960,6 +1060,10 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
 
   const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
   const Out& o = s.out;
+  if constexpr (EXACT) {
+    if constexpr (A_COLUMNS) exact_dw<T>(&p, s, tm, tn, rows, from, to);
+    else if (split == 0) exact_dx<T>(&p, s, tm, tn, rows);
+  }
   const int64_t limit = s.tiles_m < 0 ? rows : o.rows;
   constexpr bool kRows = Split<T>::kHalf && !A_COLUMNS;  // rows with powers of two of their own
   const float alpha = factor_of(o, s.meta);
@@ -1035,6 +1139,19 @@ __global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
   }
 }
 
+template <typename T, bool A_COLUMNS>
+__global__ __launch_bounds__(512) void gradient_kernel(Gradient s) {
+  extern __shared__ char lds_raw[];
+  gradient_tile<T, A_COLUMNS, false>(s, lds_raw);
+}
+
+// Of calls of up to kExactRows; apart from gradient_kernel, as what it adds takes registers.
+template <typename T, bool A_COLUMNS>
+__global__ __launch_bounds__(512) void exact_gradient_kernel(Gradient s) {
+  extern __shared__ char lds_raw[];
+  gradient_tile<T, A_COLUMNS, true>(s, lds_raw);
+}
+
 // ------------------------------------------------------------------ narrow models
 
 struct Narrow {
@@ -1047,6 +1164,7 @@ struct Narrow {
   float* target;
   const float* exponent;
   const float* row_loss;
+  bool exact;  // the entries at the labels (see kExactRows)
   Out out;
 };
 
@@ -1244,6 +1362,31 @@ __device__ __forceinline__ void narrow_pass(const Narrow& s, lds_char* lds) {
     }
   }
 
+  if (PASS != kNarrowSums && s.exact && (PASS == kNarrowDw || split == 0)) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T* const in = static_cast<const T*>(s.inner.p) + 4 * g;
+    if constexpr (PASS == kNarrowDw) {
+      const int end = to * kNarrowInner < rows ? to * kNarrowInner : rows;
+      for_labels(s.label_of, from * kNarrowInner, end, static_cast<int>(o0), 64, [&](int token, int word) {
+        const float c = s.weight_of != nullptr ? s.weight_of[token] * s.meta->inv_weight : 1.f;
+        const float r = word >= 0 ? rounded_off<T>(expm1f(-s.row_loss[token]) * kScale * c) : 0.f;
+#pragma unroll
+        for (int h = 0; h < HF; ++h) {
+          const T4 v = *reinterpret_cast<const T4*>(in + token * s.inner.ld + h * 16);
+#pragma unroll
+          for (int f = 0; f < OF; ++f) add_times(&acc[f][h], word / 16 == f ? r : 0.f, v);
+        }
+      });
+    } else if constexpr (PASS == kNarrowDx) {
+#pragma unroll
+      for (int f = 0; f < OF; ++f) {
+        const float r = label[f] >= 0 ? rounded_off<T>(at_label[f]) : 0.f;
+#pragma unroll
+        for (int h = 0; h < HF; ++h) add_times(&acc[f][h], r, *reinterpret_cast<const T4*>(in + (label[f] < 0 ? 0 : label[f]) * s.inner.ld + h * 16));
+      }
+    }
+  }
+
 #pragma unroll
   for (int f = 0; f < OF; ++f) {
     const int64_t o = o0 + f * 16 + i;
@@ -1380,7 +1523,7 @@ struct Plan {
   int planes;
   int64_t grid_x, grid_w;    // workgroups of the products, and the tiles of the parts they may be split into
   int64_t parts_s, parts_x, parts_w;
-  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, sum_w, exponent, total;
+  size_t row_of, label_of, weight_of, target, z, row_loss, meta, x, w, e, sums, parts, sum_w, exponent, residual, total;
 };
 
 Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_t ldw, int dtype, bool want_dx, bool want_dw,
@@ -1431,6 +1574,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int64_t hidden, const void* w, int64_
     p.total = at;
     return p;
   }
+  p.residual = take(p.grads && p.chunks == 1 && rows <= kExactRows ? kExactRows * 4 : 0);
   p.sums = take(p.words / kTile * p.padded * sizeof(f32x2));
   p.e = take(p.grads ? p.chunk * p.words * 2 * p.planes : 0);
   const int64_t rounds = p.fp32 ? 3 : 1, cols = up(hidden, kTile);
@@ -1493,7 +1637,7 @@ int run_narrow(const Rows& r, const Operand& ox, const Operand& ow, int64_t voca
   float* exponent = reinterpret_cast<float*>(ws + p.exponent);
   f32x2* sums = reinterpret_cast<f32x2*>(ws + p.sums);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
-  Narrow s{ox, ow, meta, label_of, weight_of, vocab, p.chunk, sums, target, exponent, row_loss, {}};
+  Narrow s{ox, ow, meta, label_of, weight_of, vocab, p.chunk, sums, target, exponent, row_loss, p.rows <= kExactRows, {}};
   const dim3 grid_x(static_cast<unsigned>(p.grid_x)), grid_w(static_cast<unsigned>(p.grid_w));
   hipLaunchKernelGGL((narrow_kernel<T, HP, kNarrowSums>), grid_x, dim3(256), 0, st, s);
   hipLaunchKernelGGL(narrow_join_kernel, dim3(static_cast<unsigned>(p.chunk / 32)), dim3(1024), 0, st, sums, p.chunk, meta, row_of, label_of,
@@ -1524,6 +1668,21 @@ int scores(const Scores& s, dim3 grid, dim3 parts, dim3 finish, bool may_split, 
     hipLaunchKernelGGL((parts_scores_kernel<T, BM>), parts, dim3(threads), lds, st, s);
     hipLaunchKernelGGL((finish_kernel<T, BM>), finish, dim3(256), 0, st, s);
   }
+  return PT_OK;
+}
+
+template <typename T, bool A_COLUMNS>
+int gradient(bool exact, dim3 grid, const Gradient& s, hipStream_t st) {
+  constexpr size_t lds = Product<T, A_COLUMNS, true>::kLds;
+  if constexpr (!Split<T>::kSplit) {
+    if (exact) {
+      if (int rc = allow(exact_gradient_kernel<T, A_COLUMNS>, lds)) return rc;
+      hipLaunchKernelGGL((exact_gradient_kernel<T, A_COLUMNS>), grid, dim3(512), lds, st, s);
+      return PT_OK;
+    }
+  }
+  if (int rc = allow(gradient_kernel<T, A_COLUMNS>, lds)) return rc;
+  hipLaunchKernelGGL((gradient_kernel<T, A_COLUMNS>), grid, dim3(512), lds, st, s);
   return PT_OK;
 }
 
@@ -1589,11 +1748,9 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
       return check_launch("pt_linear_cross_entropy");
     }
   }
-  constexpr size_t lds = Product<T, false, true>::kLds;
-  static_assert(lds == Product<T, true, true>::kLds, "one size for both gradients");
-  if (int rc = allow(gradient_kernel<T, false>, lds)) return rc;
-  if (int rc = allow(gradient_kernel<T, true>, lds)) return rc;
+  const bool exact = !Split<T>::kSplit && p.chunks == 1 && p.rows <= kExactRows;
   float* parts = reinterpret_cast<float*>(ws + p.parts + p.sum_w);
+  float* residual = exact ? reinterpret_cast<float*>(ws + p.residual) : nullptr;
   auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>(up(tiles, 8))); };
 
   for (int64_t c = 0; c < p.chunks; ++c) {
@@ -1615,22 +1772,22 @@ int run(const Rows& r, const void* w, int64_t ldw, int64_t vocab, int64_t hidden
     const bool apart = Split<T>::kHalf && weight_of != nullptr && dx != nullptr;
     const dim3 slope(static_cast<unsigned>(p.words / kBlockWords), static_cast<unsigned>((rows_most + kSlopeRows - 1) / kSlopeRows));
     hipLaunchKernelGGL(slope_kernel<T>, slope, dim3(256), 0, st, e,
-                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, apart, row_loss, z);
+                       p.chunk * p.words, sums, p.padded, meta, first, p.chunk, label_of, weight_of, apart, row_loss, z, residual);
     const int64_t plane = p.chunk * p.words;
     if (dx != nullptr) {
-      Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), kSplitX, top_w, {}};
+      Gradient d{blocked_rows(e, p.words, plane, plane * 2), ow_columns, meta, first, p.chunk, -1, tiles_h, static_cast<int>(word_steps), kSplitX, top_w, {}, label_of, residual};
       d.out = Out{dx, grad_dtype, kFinal, p.chunk, hidden, row_of, parts, apart ? weight_of : nullptr};
-      hipLaunchKernelGGL((gradient_kernel<T, false>), grid(p.grid_x), dim3(512), lds, st, d);
+      if (int rc = gradient<T, false>(exact, grid(p.grid_x), d, st)) return rc;
       if (p.parts_x > 0) hipLaunchKernelGGL(parts_kernel<T>, join_grid(p.chunk, hidden), dim3(256), 0, st, d);
     }
     if (dw != nullptr) {
       if constexpr (Split<T>::kHalf)
-        if (apart) hipLaunchKernelGGL(weigh_kernel<T>, slope, dim3(256), 0, st, e, plane, meta, first, p.chunk, weight_of);
+        if (apart) hipLaunchKernelGGL(weigh_kernel<T>, slope, dim3(256), 0, st, e, plane, meta, first, p.chunk, weight_of, residual);
       const Operand oxc = columns_operand(x + first * p.width, p.width, all * p.width, (all - first) * p.width * 2);
       const int how = p.chunks == 1 ? kFinal : (c + 1 == p.chunks ? kAddFinal : kAdd);
-      Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, kSplitW, top_x, {}};
+      Gradient d{blocked_columns(e, p.words, plane, plane * 2), oxc, meta, first, p.chunk, tiles_v, tiles_h, -1, kSplitW, top_x, {}, label_of, residual};
       d.out = Out{dw, grad_dtype, how, vocab, hidden, nullptr, p.chunks == 1 ? parts : reinterpret_cast<float*>(ws + p.parts), nullptr};
-      hipLaunchKernelGGL((gradient_kernel<T, true>), grid(p.grid_w), dim3(512), lds, st, d);
+      if (int rc = gradient<T, true>(exact, grid(p.grid_w), d, st)) return rc;
       if (p.parts_w > 0) hipLaunchKernelGGL(parts_kernel<T>, join_grid(vocab, hidden), dim3(256), 0, st, d);
     }
     if (int rc = check_launch("pt_linear_cross_entropy")) return rc;

@@ -797,3 +797,31 @@ def test_a_vocabulary_of_one_word(gpu, dtype, h):
     loss, dx, dw = ops.linear_cross_entropy(x, w, t, reduction="none", want_loss=True, want_dx=True, want_dw=True,
                                             grad_losses=torch.ones(300, device=gpu))
     assert not loss.any() and not dx.any() and not dw.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("h", [20, 64, 128, 192, 1030])
+@pytest.mark.parametrize("n,v", [(1, 300), (3, 40), (50, 1000), (256, 3000), (250, 200)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_tokens_are_exact_at_their_labels(gpu, dtype, h, n, v, reduction):
+    """The softmax's entries at the labels, most of each gradient, are not those of the matrix cores' 16 bits."""
+
+    x, w, t = make(n, h, v, dtype, gpu, spread=0.5, ignored=0.25 if n > 3 else 0, seed=n)
+    t[n // 2:] = t[: n - n // 2].clone()  # words that are several tokens' label
+    factors = torch.randn(n, device=gpu, generator=torch.Generator(device=gpu).manual_seed(5))
+    if reduction == "mean":
+        factors = torch.ones(n, device=gpu) / (t != -100).sum()
+    _, dx, dw = ops.linear_cross_entropy(x, w, t, reduction=reduction, want_loss=False, want_dx=True, want_dw=True, grad_dtype=torch.float32,
+                                         grad_losses=factors if reduction == "none" else None)
+    losses, dx64, dw64, ax, aw, slack = oracle(x, w, t, factors)
+    keep = t != -100
+    label = torch.where(keep, -torch.expm1(-losses) * factors.abs(), 0.0)[:, None]  # what G holds there
+    at = t.clamp_min(0)
+    own_x = label * w[at].double().abs()
+    own_w = torch.zeros_like(dw64).index_add_(0, at, label * torch.where(keep[:, None], x, 0).double().abs())
+    exact = 4 * slack + 2.0**-18 + max(n, v) * 2.0**-24
+    part = exact + torch.finfo(dtype).eps / 2 + 2.0**-11
+    for got, want, total, own in ((dx, dx64, ax, own_x), (dw, dw64, aw, own_w)):
+        limit = exact * own + part * (total - own) + 2.0**-28 * float(total.max())
+        off = (got.double() - want).abs()
+        assert torch.all(off <= limit), float((off / limit).max())
