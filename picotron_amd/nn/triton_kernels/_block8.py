@@ -1,4 +1,4 @@
-"""Activations held in 8 bits, in PyTorch: what the kernels of ``csrc/block8.hpp`` hold, to the bit.
+"""Activations held in 8 bits, in PyTorch: what the kernels of ``csrc/block8.hpp`` hold, to the bit in blocks of finite elements.
 
 A block of 128 elements shares ``step = top / 127``, top its largest magnitude; an element's code is ``128 + round(x * (127 / top))``
 and its value ``(code - 128) * step``, all in fp32.  A block whose top is below 2^-100 is held as zeros; one with an infinity or a
