@@ -291,7 +291,7 @@ struct TileProduct {
       multiply(1);
       if (SPLIT && phase == 0) {
         // An infinity has no low plane (inf - inf), and its high one times the other side's low one may have either sign: such sums
-        // are dropped, and hi hi alone says what comes of it.  Sums of finite elements are below 2^28 a term.
+        // are dropped, and hi hi alone says what comes of it.  A term of finite elements is below 2^30.
 #pragma unroll
         for (int f = 0; f < FM; ++f)
 #pragma unroll
