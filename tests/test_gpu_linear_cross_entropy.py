@@ -825,3 +825,41 @@ def test_few_tokens_are_exact_at_their_labels(gpu, dtype, h, n, v, reduction):
         limit = exact * own + part * (total - own) + 2.0**-28 * float(total.max())
         off = (got.double() - want).abs()
         assert torch.all(off <= limit), float((off / limit).max())
+
+
+@pytest.mark.parametrize("dtype,n,h", [(torch.float32, 300, 64), (torch.float16, 300, 192), (torch.float16, 100, 192), (torch.float16, 100, 64),
+                                       (torch.bfloat16, 100, 192), (torch.bfloat16, 100, 64)])
+def test_captured_with_weights(gpu, dtype, n, h):
+    """Tokens with weights of their own, far apart in some replays and alike in others; calls of few tokens."""
+
+    x, w, t = make(n, h, 700, dtype, gpu)
+    factors = torch.ones(n, device=gpu)
+    x.requires_grad_()
+    w.requires_grad_()
+
+    def step():
+        loss = triton_linear_cross_entropy(x, w, t, reduction="none")
+        return (loss, *torch.autograd.grad([loss], [x, w], [factors]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(4):
+        y, v, s = make(n, h, 700, dtype, gpu, seed=seed + 20, ignored=0.3 * seed)
+        with torch.no_grad():
+            x.copy_(y)
+            w.copy_(v)
+            t.copy_(s)
+            factors.copy_(torch.linspace(0, -10 * seed, n, device=gpu).exp2())
+        graph.replay()
+        got = [o.detach().clone() for o in out]
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        check(got[0], got[1], got[2], x.detach(), w.detach(), t, factors)
